@@ -228,6 +228,22 @@ extern "C"
 			                * A token may hold at most one slot per expert, as every router of this library and of the reference writes its table; of
 			                * duplicates in a hand-made table only the lowest slot counts, where the reference's atomic additions would add them all. */
 
+	/* ---- training and answering of the token-wise half of a transformer, no counterpart in the reference ABI (whose cuda_layernorm_* keep their
+	 *      stubs): tensors of the rows are fp16 or fp32 with the features in the last dimension, any number of rows before it, zero among them. Results of these
+	 *      calls are rounded to nearest. Gradients of weights and biases are sums over all rows in fp32, added up in a fixed order (the same bits on every run), and may be asked for
+	 *      in fp32 where the tensors are fp16. A gradient tensor whose data is NULL is not computed; where a beta is not 0, what the gradient tensor held is multiplied
+	 *      by it and added (gradients of several batches). Workspaces are the caller's: at least as many bytes as the call's own function says, aligned to
+	 *      16 bytes, free for anything else once the call's work on the stream is done; calls that may run at the same time (other contexts, graphs replayed on other streams) need one each.
+	 *      Tensors need the alignment of one element only. Results may not overlap inputs unless a call says so. ---- */
+	/*
+	 * y[i, j] = (x[i, j] - mean_i) / sqrt(var_i + epsilon) * w[j] + b[j] over the last dimension; w and b may be empty. y may be x.
+	 * Backward: dx = beta_dx * dx + the gradient of x, dw = beta_weights * dw + sum_i dy n, db = beta_weights * db + sum_i dy; the statistics are computed again from x. dx may be dy or x.
+	 */
+	void hip_layer_norm_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, mlTensor_t y, float epsilon);
+	size_t hip_layer_norm_get_workspace_size(mlShape_t shape, mlDataType_t dtype); /* bytes, for the backward pass */
+	void hip_layer_norm_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t dy, float beta_dx, mlTensor_t dx, float beta_weights,
+			mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size, float epsilon);
+
 	/* ---- additions with no counterpart in the reference ABI ----
 	 * hip_quantized_conv_forward: the whole int8 convolution of reference src/layers/Conv2D.cpp:240-308 (int8 implicit GEMM with
 	 * zero-point padding, int32 accumulation, per-channel scale + bias, optional int8 residual, activation, requantisation)

@@ -111,6 +111,9 @@ SIGNATURES = {
     "moe_forward": (None, [_vp, _T, _T, _T, _f, _T, _i]),
     "scatter_tokens_forward": (None, [_vp, _T, _T, _f, _T]),
     "quantized_conv_forward": (None, [_vp, _S, _S, _vp, _Q, _vp, _vp, _vp, _i, _vp, _Q, _vp, _Q, _i]),
+    "layer_norm_forward": (None, [_vp, _T, _T, _T, _T, _f]),
+    "layer_norm_get_workspace_size": (_sz, [_S, _i]),
+    "layer_norm_backward": (None, [_vp, _T, _T, _T, _f, _T, _f, _T, _T, _vp, _sz, _f]),
     "get_stream": (_vp, [_vp]),
     "graph_begin_capture": (None, [_vp]),
     "graph_end_capture": (_vp, [_vp]),

@@ -156,6 +156,12 @@ class Tensor:
             self.ptr = _ptr
             self._owning = False
 
+    @staticmethod
+    def over(ptr, shape, dtype, device_index=0, owner=None):
+        """Tensor over dense memory of the caller's, which `owner` keeps alive (an array of another library on the same device). Whoever wrote it on a stream of its
+        own has to have finished, or the two streams have to be ordered; a context's stream waits for the legacy default stream by itself."""
+        return Tensor(shape, dtype, device_index, _ptr=ptr, _owner=owner)
+
     # ---- shape helpers named as in the reference's Shape / Tensor
     def rank(self):
         return len(self.shape)
@@ -711,6 +717,47 @@ def scatterTokensForward(context, input, indicesAndValues, beta, output):
     _require(output.shape[0] == b and output.shape[3] == c and indicesAndValues.shape == (b, 2, e, k), "shapes do not agree")
     _require(_same_dtype(input, output, indicesAndValues) and input.dtype in (B.DTYPE_FLOAT16, B.DTYPE_FLOAT32), "fp16 or fp32 tensors of one type")
     _launch("scatter_tokens_forward", context.handle, input.desc(), indicesAndValues.desc(), beta, output.desc())
+
+
+_FLOATS = (B.DTYPE_FLOAT16, B.DTYPE_FLOAT32)
+
+
+def _all(t):
+    """The descriptor of an optional tensor, also where it has no elements."""
+    return _EMPTY if t is None else t.desc()
+
+
+def _space(workspace):
+    return (None, 0) if workspace is None else (workspace.ptr, workspace.sizeInBytes())
+
+
+def _require_gradient(t, like, dtype, what):
+    _require(t is None or (t.volume() == like and t.dtype in (dtype, B.DTYPE_FLOAT32)), "%s: shape or type" % what)
+
+
+def layerNormForward(context, input, weights, bias, output, epsilon=1e-5):
+    """y = (x - mean) / sqrt(var + epsilon) * weights + bias over the last dimension; weights and bias may be None, output may be the input."""
+    _require(input.dtype in _FLOATS and _same_dtype(input, output, weights, bias) and tuple(input.shape) == tuple(output.shape), "shape / dtype mismatch")
+    for t in (weights, bias):
+        _require(t is None or t.volume() == input.lastDim(), "weights / bias must have one element per column")
+    _launch("layer_norm_forward", context.handle, input.desc(), _all(weights), _all(bias), output.desc(), epsilon)
+
+
+def layerNormGetWorkspaceSize(context, input):
+    """Bytes of workspace that layerNormBackward needs."""
+    return B.fn("layer_norm_get_workspace_size")(input.shape_desc(), input.dtype)
+
+
+def layerNormBackward(context, input, weights, gradient, beta, gradient_input, beta_weights, gradient_weights, gradient_bias, workspace, epsilon=1e-5):
+    """From `gradient` (of the output): gradient_input = its share + beta * gradient_input; gradient_weights and gradient_bias likewise with beta_weights, of the tensors' type or fp32. Each of
+    the three may be None; gradient_input may be `gradient` or `input`. The statistics are computed again from `input`."""
+    _require(input.dtype in _FLOATS and _same_dtype(input, gradient, gradient_input, weights), "dtype mismatch")
+    _require(tuple(input.shape) == tuple(gradient.shape) and (gradient_input is None or tuple(gradient_input.shape) == tuple(input.shape)), "shape mismatch")
+    _require(weights is None or weights.volume() == input.lastDim(), "weights must have one element per column")
+    _require_gradient(gradient_weights, input.lastDim(), input.dtype, "gradient of the weights")
+    _require_gradient(gradient_bias, input.lastDim(), input.dtype, "gradient of the bias")
+    _launch("layer_norm_backward", context.handle, input.desc(), _all(weights), gradient.desc(), beta, _all(gradient_input), beta_weights, _all(gradient_weights),
+            _all(gradient_bias), *_space(workspace), epsilon)
 
 
 def foldBatchnorm(context, layer_weights, layer_bias, bn_weights, bn_bias, bn_avg_var):

@@ -1,0 +1,153 @@
+/*
+ * training_utils.hpp — what the operators with a backward pass share: element access for rows of any length and alignment, results rounded to nearest,
+ * and the sums that become gradients of weights.
+ *
+ * These operators have no counterpart whose bits they reproduce, so fp16 results are rounded to nearest (half a step, 2^-11 of the value) and not towards
+ * zero as the inference path does after the reference: a gradient that is rounded towards zero is too small in every element, and a training run adds that up.
+ */
+#ifndef MINML_AMD_TRAINING_UTILS_HPP_
+#define MINML_AMD_TRAINING_UTILS_HPP_
+
+#include "common.hpp"
+#include "device_utils.hpp"
+
+namespace mlhip
+{
+	/* VEC consecutive elements that need no more alignment than one of them: one memory instruction all the same (global memory takes any address) */
+	template<typename T, int VEC>
+	struct Elements
+	{
+			typedef T vec_t __attribute__((ext_vector_type(VEC)));
+			typedef vec_t unaligned_t __attribute__((aligned(sizeof(T))));
+			vec_t raw;
+
+			__device__ __forceinline__ void load(const T *p)
+			{
+				raw = *reinterpret_cast<const unaligned_t*>(p);
+			}
+			__device__ __forceinline__ float operator[](int e) const
+			{
+				return static_cast<float>(raw[e]);
+			}
+	};
+	template<typename T>
+	struct Elements<T, 1>
+	{
+			T raw;
+
+			__device__ __forceinline__ void load(const T *p)
+			{
+				raw = *p;
+			}
+			__device__ __forceinline__ float operator[](int) const
+			{
+				return static_cast<float>(raw);
+			}
+	};
+	/* VEC results rounded to nearest; those before `skip` are left out (the first ones of the vector that ends a row, see RowPlace) */
+	template<int VEC, typename T>
+	__device__ __forceinline__ void store_nearest(T *p, const float (&v)[VEC], int skip = 0)
+	{
+		if (skip == 0)
+		{
+			if constexpr (VEC == 1)
+				*p = static_cast<T>(v[0]);
+			else
+			{
+				typename Elements<T, VEC>::vec_t tmp;
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					tmp[e] = static_cast<T>(v[e]);
+				*reinterpret_cast<typename Elements<T, VEC>::unaligned_t*>(p) = tmp;
+			}
+		}
+		else
+		{
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				if (e >= skip)
+					p[e] = static_cast<T>(v[e]);
+		}
+	}
+	/*
+	 * Where the vector that begins at column j of a row of `columns` (>= VEC) elements lies. The vector that would pass the row's end is moved back to end with it; its first `skip`
+	 * elements belong to the vector before it and count for nothing here. So every load is a whole vector inside its row, for any length, and none stands under a test.
+	 */
+	struct RowPlace
+	{
+			int start, skip;
+	};
+	template<int VEC>
+	__device__ __forceinline__ RowPlace place_in_row(int j, int columns)
+	{
+		const int start = min(j, columns - VEC);
+		return RowPlace { start, min(j - start, VEC) };
+	}
+
+	/* sum over the LANES (a power of two) neighbouring lanes that share a row; every lane gets it */
+	template<int LANES>
+	__device__ __forceinline__ float lanes_sum(float v)
+	{
+#pragma unroll
+		for (int offset = LANES / 2; offset >= 1; offset >>= 1)
+			v += __shfl_xor(v, offset);
+		return v;
+	}
+
+	/*
+	 * out[j] = sum over `parts` rows of partial[.][stride] (column j) + beta * out[j]: the second half of every sum over rows. The first half leaves one row of sums per workgroup, here 8
+	 * threads to a column add up every eighth of them and meet in LDS: a fixed order, so the same bits every time, which additions by atomic operations would not give.
+	 */
+	template<typename Out>
+	__global__ __launch_bounds__(256) void kernel_sum_partials(const float *partial, int parts, size_t stride, Out *out, int columns, float beta)
+	{
+		__shared__ float sums[8][33];
+		const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
+		const int j = blockIdx.x * 32 + c;
+		float sum = 0.0f;
+		if (j < columns)
+		{
+			const float *src = partial + j;
+			int p = group;
+			for (; p + 56 < parts; p += 64)
+			{
+				float v[8];
+#pragma unroll
+				for (int u = 0; u < 8; u++)
+					v[u] = src[static_cast<size_t>(p + 8 * u) * stride];
+#pragma unroll
+				for (int u = 0; u < 8; u++)
+					sum += v[u];
+			}
+			for (; p < parts; p += 8)
+				sum += src[static_cast<size_t>(p) * stride];
+		}
+		sums[group][c] = sum;
+		__syncthreads();
+		if (group == 0 && j < columns)
+		{
+#pragma unroll
+			for (int g = 1; g < 8; g++)
+				sum += sums[g][c];
+			out[j] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(out[j]), sum) : sum);
+		}
+	}
+	/* the gradient of a weight: of the tensors' type, or fp32 */
+	inline void launch_sum_partials(hipStream_t stream, const float *partial, int parts, size_t stride, void *out, mlDataType_t dtype, int columns, float beta)
+	{
+		if (columns == 0)
+			return;
+		const dim3 grid(ceil_div(columns, 32));
+		if (dtype == DTYPE_FLOAT16)
+			hipLaunchKernelGGL((kernel_sum_partials<half_t>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<half_t*>(out), columns, beta);
+		else
+			hipLaunchKernelGGL((kernel_sum_partials<float>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<float*>(out), columns, beta);
+		MLHIP_CHECK(hipGetLastError());
+	}
+	inline size_t round_up(size_t n, size_t to)
+	{
+		return (n + to - 1) / to * to;
+	}
+} /* namespace mlhip */
+
+#endif /* MINML_AMD_TRAINING_UTILS_HPP_ */

@@ -1,0 +1,57 @@
+"""No-GPU checks of the operators with a backward pass: what the library and the mirror refuse, before anything reaches a device."""
+import numpy as np
+import pytest
+
+from minml_amd import backend as B
+from minml_amd import core as ml
+
+
+def fake(shape, dtype="float16"):
+    return ml.Tensor(shape, dtype, _ptr=0x7000)
+
+
+NULL = B.make_tensor(None, B.DTYPE_UNKNOWN, ())
+
+
+def refused(name, *args):
+    with pytest.raises(ValueError):
+        B.fn(name)(None, *args)
+
+
+def test_layer_norm_refusals_of_the_library():
+    x, w = fake((4, 16)).desc(), fake((16,)).desc()
+    forward = lambda x, w, b, y, eps=1e-5: refused("layer_norm_forward", x, w, b, y, eps)
+    forward(x, w, w, fake((4, 15)).desc())
+    forward(x, w, w, fake((4, 16), "float32").desc())
+    forward(x, fake((15,)).desc(), w, x)
+    forward(x, w, fake((16,), "float32").desc(), x)
+    forward(fake((4, 16), "int32").desc(), w, w, fake((4, 16), "int32").desc())
+    forward(x, w, w, x, -1.0)
+    forward(x, w, w, x, float("nan"))
+    forward(x, w, w, x)  # all is well but the context
+    backward = lambda x, w, dy, dx, dw, db, space=0x7000, size=1 << 30: refused("layer_norm_backward", x, w, dy, 0.0, dx, 0.0, dw, db, space, size, 1e-5)
+    need = B.fn("layer_norm_get_workspace_size")(fake((4, 16)).shape_desc(), B.DTYPE_FLOAT16)
+    assert need >= 2 * 16 * 4
+    backward(x, w, fake((4, 17)).desc(), x, w, w)
+    backward(x, w, x, fake((3, 16)).desc(), w, w)
+    backward(x, w, x, x, fake((17,)).desc(), w)
+    backward(x, w, x, x, w, fake((16,), "int32").desc())
+    backward(x, w, x, x, w, w, None, 0)
+    backward(x, w, x, x, w, w, 0x7000, need - 1)
+    backward(x, w, x, x, w, w, 0x7004, need)
+    backward(fake((4, 16), "float32").desc(), fake((16,), "float32").desc(), fake((4, 16), "float32").desc(), NULL, w, NULL)  # fp16 sums of fp32 tensors
+    B.fn("layer_norm_backward")(None, x, w, x, 0.0, NULL, 0.0, NULL, NULL, None, 0, 1e-5)  # nothing asked for
+    B.fn("layer_norm_forward")(None, fake((0, 16)).desc(), w, w, fake((0, 16)).desc(), 1e-5)
+
+
+def test_layer_norm_refusals_of_the_mirror():
+    class Ctx:
+        handle = None
+
+    x, w, f = fake((4, 16)), fake((16,)), fake((16,), "float32")
+    for call in (lambda: ml.layerNormForward(Ctx, x, w, w, fake((4, 8))), lambda: ml.layerNormForward(Ctx, x, f, w, x), lambda: ml.layerNormForward(Ctx, x, w, fake((8,)), x),
+                 lambda: ml.layerNormBackward(Ctx, x, w, fake((4, 8)), 0.0, x, 0.0, w, w, None), lambda: ml.layerNormBackward(Ctx, x, w, x, 0.0, fake((4, 16), "float32"), 0.0, w, w, None),
+                 lambda: ml.layerNormBackward(Ctx, x, w, x, 0.0, x, 0.0, fake((8,)), w, None), lambda: ml.layerNormBackward(Ctx, x, w, x, 0.0, x, 0.0, fake((16,), "int32"), w, None),
+                 lambda: ml.layerNormBackward(Ctx, x, w, x, 0.0, x, 0.0, f, f, None)):
+        with pytest.raises(ValueError):
+            call()
