@@ -244,6 +244,21 @@ extern "C"
 	void hip_layer_norm_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t dy, float beta_dx, mlTensor_t dx, float beta_weights,
 			mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size, float epsilon);
 
+	/*
+	 * The gated dense layer: y = a(x Wg^T + bg) * (x Wu^T + bu). x [.., features], w [2, hidden, features] (the gate's matrix, then the other), b [2, hidden] or empty, y [.., hidden]; `projections`
+	 * [.., 2, hidden] takes both projections, which the backward pass needs, or is empty. Backward: dy [.., hidden] -> dx, dw, db as above. x and w have to be aligned to 16 bytes, workspaces of
+	 * these calls to 256. Gradients of the projections are kept in the tensors' type in between.
+	 */
+	typedef enum
+	{
+		GATE_SIGMOID, GATE_RELU, GATE_SILU /* g sigmoid(g) */, GATE_GELU /* g P(g), P the integral of the normal distribution */
+	} mlGate_t;
+	size_t hip_gated_dense_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, mlDataType_t dtype, bool backward); /* bytes */
+	void hip_gated_dense_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, mlTensor_t y, mlTensor_t projections, mlGate_t gate, void *workspace,
+			size_t workspace_size);
+	void hip_gated_dense_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t projections, const mlTensor_t dy, float beta_dx, mlTensor_t dx,
+			float beta_weights, mlTensor_t dw, mlTensor_t db, mlGate_t gate, void *workspace, size_t workspace_size);
+
 	/* ---- additions with no counterpart in the reference ABI ----
 	 * hip_quantized_conv_forward: the whole int8 convolution of reference src/layers/Conv2D.cpp:240-308 (int8 implicit GEMM with
 	 * zero-point padding, int32 accumulation, per-channel scale + bias, optional int8 residual, activation, requantisation)

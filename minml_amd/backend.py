@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(HERE, "libminml_hip.so")
 # mlDataType_t / mlActivationType_t (reference: include/minml/backend/backend_types.h:40-63)
 DTYPE_UNKNOWN, DTYPE_FLOAT8, DTYPE_FLOAT16, DTYPE_FLOAT32, DTYPE_FLOAT64, DTYPE_UINT8, DTYPE_INT8, DTYPE_INT16, DTYPE_INT32 = range(9)
 ACTIVATION_LINEAR, ACTIVATION_SIGMOID, ACTIVATION_TANH, ACTIVATION_RELU, ACTIVATION_LEAKY_RELU, ACTIVATION_EXP = range(6)
+# mlGate_t
+GATE_SIGMOID, GATE_RELU, GATE_SILU, GATE_GELU = range(4)
 
 DTYPE_SIZE = {DTYPE_FLOAT16: 2, DTYPE_FLOAT32: 4, DTYPE_INT8: 1, DTYPE_UINT8: 1, DTYPE_INT16: 2, DTYPE_INT32: 4, DTYPE_FLOAT64: 8}
 
@@ -114,6 +116,9 @@ SIGNATURES = {
     "layer_norm_forward": (None, [_vp, _T, _T, _T, _T, _f]),
     "layer_norm_get_workspace_size": (_sz, [_S, _i]),
     "layer_norm_backward": (None, [_vp, _T, _T, _T, _f, _T, _f, _T, _T, _vp, _sz, _f]),
+    "gated_dense_get_workspace_size": (_sz, [_S, _S, _i, _b]),
+    "gated_dense_forward": (None, [_vp, _T, _T, _T, _T, _T, _i, _vp, _sz]),
+    "gated_dense_backward": (None, [_vp, _T, _T, _T, _T, _f, _T, _f, _T, _T, _i, _vp, _sz]),
     "get_stream": (_vp, [_vp]),
     "graph_begin_capture": (None, [_vp]),
     "graph_end_capture": (_vp, [_vp]),

@@ -28,6 +28,9 @@ def dtype_of(x):
     return int(x)
 
 
+GATES = {"sigmoid": B.GATE_SIGMOID, "relu": B.GATE_RELU, "silu": B.GATE_SILU, "gelu": B.GATE_GELU}
+
+
 def act_of(a):
     if isinstance(a, str):
         return ACTIVATIONS[a]
@@ -758,6 +761,43 @@ def layerNormBackward(context, input, weights, gradient, beta, gradient_input, b
     _require_gradient(gradient_bias, input.lastDim(), input.dtype, "gradient of the bias")
     _launch("layer_norm_backward", context.handle, input.desc(), _all(weights), gradient.desc(), beta, _all(gradient_input), beta_weights, _all(gradient_weights),
             _all(gradient_bias), *_space(workspace), epsilon)
+
+
+def _require_gated(input, weights, gate):
+    _require(input.dtype in _FLOATS and _same_dtype(input, weights), "dtype mismatch")
+    _require(len(weights.shape) == 3 and weights.shape[0] == 2 and len(input.shape) >= 1 and weights.shape[2] == input.shape[-1], "weights must be [2, hidden, features]")
+    _require(gate in GATES or gate in GATES.values(), "unknown gate")
+    return GATES.get(gate, gate)
+
+
+def gatedDenseGetWorkspaceSize(context, input, weights, backward):
+    """Bytes of workspace (aligned to 256) that gatedDenseForward or gatedDenseBackward needs."""
+    return B.fn("gated_dense_get_workspace_size")(input.shape_desc(), weights.shape_desc(), input.dtype, bool(backward))
+
+
+def gatedDenseForward(context, input, weights, bias, output, projections, gate, workspace):
+    """output = a(input Wg^T + bg) * (input Wu^T + bu): input [.., features], weights [2, hidden, features], bias [2, hidden] or None, output [.., hidden]; projections [.., 2, hidden] takes both
+    projections for the backward pass, or is None. gate: "sigmoid", "relu", "silu" or "gelu"."""
+    gate = _require_gated(input, weights, gate)
+    hidden, lead = weights.shape[1], tuple(input.shape[:-1])
+    _require(_same_dtype(input, bias, output, projections) and tuple(output.shape) == lead + (hidden,), "output: shape or type")
+    _require(bias is None or bias.volume() == 2 * hidden, "bias must be [2, hidden]")
+    _require(projections is None or tuple(projections.shape) == lead + (2, hidden), "projections must be [.., 2, hidden]")
+    _launch("gated_dense_forward", context.handle, input.desc(), weights.desc(), _all(bias), output.desc(), _all(projections), gate, *_space(workspace))
+
+
+def gatedDenseBackward(context, input, weights, projections, gradient, beta, gradient_input, beta_weights, gradient_weights, gradient_bias, gate, workspace):
+    """From `gradient` (of the output) and the projections that the forward pass kept: gradient_input = its share + beta * gradient_input; gradient_weights and gradient_bias likewise with
+    beta_weights, of the tensors' type or fp32. Each of the three may be None."""
+    gate = _require_gated(input, weights, gate)
+    hidden, lead = weights.shape[1], tuple(input.shape[:-1])
+    _require(_same_dtype(input, projections, gradient, gradient_input), "dtype mismatch")
+    _require(tuple(projections.shape) == lead + (2, hidden) and tuple(gradient.shape) == lead + (hidden,), "projections must be [.., 2, hidden], the gradient [.., hidden]")
+    _require(gradient_input is None or tuple(gradient_input.shape) == tuple(input.shape), "gradient of the input: shape")
+    _require_gradient(gradient_weights, weights.volume(), input.dtype, "gradient of the weights")
+    _require_gradient(gradient_bias, 2 * hidden, input.dtype, "gradient of the bias")
+    _launch("gated_dense_backward", context.handle, input.desc(), weights.desc(), projections.desc(), gradient.desc(), beta, _all(gradient_input), beta_weights,
+            _all(gradient_weights), _all(gradient_bias), gate, *_space(workspace))
 
 
 def foldBatchnorm(context, layer_weights, layer_bias, bn_weights, bn_bias, bn_avg_var):

@@ -1,0 +1,554 @@
+/*
+ * gated.hip — the gated dense layer of a transformer's feed-forward half, and its backward pass.
+ *
+ *   g = x Wg^T + bg,  u = x Wu^T + bu,  y = a(g) u           a: sigmoid, relu, silu (g sigmoid(g)), gelu (g P(g), P the normal distribution)
+ *   dg = dy u a'(g),  du = dy a(g),  d = [dg | du]
+ *   dx = d W,  dW = d^T x,  db = sum_rows d                   W = [Wg; Wu], stored as [2, hidden, features]
+ *
+ * Forward: one launch. A tile's columns are half gate, half up of the same hidden units, so the epilogue has both projections of an element and neither goes to memory, unless the backward pass is to have
+ * them (`projections`, in the tensors' type). Up to 64 rows the weights stream through registers (few_rows.hpp). Where there are too few tiles for the chip the product is split along the
+ * features, and the launch that adds the parts up applies the gate.
+ * Backward: one pass over dy and the projections makes d and the partial sums of db (bound by memory), then two products (bound by the matrix cores). d is stored in the tensors' type: its rounding, half a step per
+ * element, averages out in sums over as many hidden units or rows as the products have, and is what a stored gradient costs anywhere else in a network of that type; db is summed before the rounding.
+ */
+#include "few_rows.hpp"
+#include "product_tiles.hpp"
+
+namespace
+{
+	using namespace mlhip;
+
+	/* exp and 1 / x for gates whose results are rounded to fp16: the hardware's own, 2^-21 off at most for |x| < 8, where 2^-11 is rounded away; fp32 takes the library's */
+	template<typename T>
+	__device__ __forceinline__ float sigmoid_of(float g)
+	{
+		if constexpr (sizeof(T) == 2)
+			return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+		else
+			return 1.0f / (1.0f + expf(-g));
+	}
+	/*
+	 * The normal distribution's integral, 0.5 erfc(-g / sqrt 2). For fp16 erfc(z) exp(z^2) / t is a polynomial of degree 6 in t = 1 / (1 + 0.37 z), fitted to the smallest relative error over
+	 * z = 0 .. 7 (3.7e-7, 7e-7 in 32 bits): the tail, where gelu is small, is as exact as the rest, with a dozen instructions instead of the 60 of the library's erfc, which fp32 takes.
+	 */
+	template<typename T>
+	__device__ __forceinline__ float normal_integral(float g)
+	{
+		if constexpr (sizeof(T) == 2)
+		{
+			const float z = fabsf(g) * 0.70710678118654752f;
+			const float t = __builtin_amdgcn_rcpf(fmaf(0.37f, z, 1.0f));
+			float poly = fmaf(t, -0.14591303f, 0.44789582f);
+			poly = fmaf(t, poly, -0.20436039f);
+			poly = fmaf(t, poly, 0.33090103f);
+			poly = fmaf(t, poly, 0.14716733f);
+			poly = fmaf(t, poly, 0.21602353f);
+			poly = fmaf(t, poly, 0.20828535f);
+			const float tail = 0.5f * t * poly * __expf(-z * z);
+			return g < 0.0f ? tail : 1.0f - tail;
+		}
+		else
+			return 0.5f * erfcf(g * -0.70710678118654752f);
+	}
+	/* a(g) and, if asked, its derivative */
+	template<typename T, bool SLOPE>
+	__device__ __forceinline__ void gate_of(int gate, float g, float &a, float &slope)
+	{
+		switch (gate)
+		{
+			case GATE_SIGMOID:
+				a = sigmoid_of<T>(g);
+				if (SLOPE)
+					slope = a * (1.0f - a);
+				break;
+			case GATE_RELU:
+				a = (g > 0.0f || g != g) ? g : 0.0f; /* NaN stays */
+				if (SLOPE)
+					slope = g > 0.0f ? 1.0f : 0.0f;
+				break;
+			case GATE_SILU:
+			{
+				const float s = sigmoid_of<T>(g);
+				a = g * s;
+				if (SLOPE)
+					slope = s * fmaf(g, 1.0f - s, 1.0f);
+				break;
+			}
+			default: /* GATE_GELU */
+			{
+				const float p = normal_integral<T>(g);
+				a = g * p;
+				if (SLOPE)
+					slope = fmaf(g * 0.39894228040143268f, (sizeof(T) == 2) ? __expf(-0.5f * g * g) : expf(-0.5f * g * g), p);
+				break;
+			}
+		}
+	}
+
+	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
+	template<typename T>
+	struct GatedEpilogue
+	{
+			static constexpr int SHARE = 16; /* 8 of each projection */
+			static constexpr bool HAS_END = false;
+			struct State
+			{
+					float bias[2][8];
+			};
+			T *y, *projections;
+			const T *bias;
+			int hidden, gate;
+
+			template<int BN>
+			__device__ __forceinline__ void begin(State &state, int group, int tile_n) const
+			{
+				const int n = tile_n * (BN / 2) + group * 8;
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+#pragma unroll
+					for (int e = 0; e < 8; e++)
+						state.bias[i][e] = (bias != nullptr && n + e < hidden) ? static_cast<float>(bias[i * hidden + n + e]) : 0.0f;
+			}
+			template<int BN>
+			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
+			{
+				const int n = tile_n * (BN / 2) + group * 8;
+				if (n >= hidden)
+					return;
+				float g[8], u[8], out[8];
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+				{
+					g[e] = row[group * 8 + e] + state.bias[0][e];
+					u[e] = row[BN / 2 + group * 8 + e] + state.bias[1][e];
+					float a, unused;
+					gate_of<T, false>(gate, g[e], a, unused);
+					out[e] = a * u[e];
+				}
+				T *dst = y + static_cast<size_t>(m) * hidden + n;
+				T *kept = projections + static_cast<size_t>(m) * 2 * hidden + n;
+				if (n + 8 <= hidden)
+				{
+					store_nearest<8>(dst, out);
+					if (projections != nullptr)
+					{
+						store_nearest<8>(kept, g);
+						store_nearest<8>(kept + hidden, u);
+					}
+				}
+				else
+					for (int e = 0; e < hidden - n; e++)
+					{
+						dst[e] = static_cast<T>(out[e]);
+						if (projections != nullptr)
+						{
+							kept[e] = static_cast<T>(g[e]);
+							kept[hidden + e] = static_cast<T>(u[e]);
+						}
+					}
+			}
+	};
+	/* the sums of a split product: [part][row][2][hidden] */
+	struct GatedPartEpilogue
+	{
+			static constexpr int SHARE = 16;
+			static constexpr bool HAS_END = false;
+			struct State
+			{
+			};
+			float *partial;
+			size_t part_stride;
+			int hidden;
+
+			template<int BN>
+			__device__ __forceinline__ void begin(State&, int, int) const
+			{
+			}
+			template<int BN>
+			__device__ __forceinline__ void apply(State&, int m, int group, const float *row, int tile_n, int part) const
+			{
+				const int n = tile_n * (BN / 2) + group * 8;
+				float *dst = partial + part * part_stride + static_cast<size_t>(m) * 2 * hidden + n;
+				for (int e = 0; e < 8; e++)
+					if (n + e < hidden)
+					{
+						dst[e] = row[group * 8 + e];
+						dst[hidden + e] = row[BN / 2 + group * 8 + e];
+					}
+			}
+	};
+	template<typename T>
+	__device__ __forceinline__ void finish_element(float g, float u, size_t row, int n, const T *bias, T *y, T *projections, int hidden, int gate)
+	{
+		if (bias != nullptr)
+		{
+			g += static_cast<float>(bias[n]);
+			u += static_cast<float>(bias[hidden + n]);
+		}
+		float a, unused;
+		gate_of<T, false>(gate, g, a, unused);
+		y[row * hidden + n] = static_cast<T>(a * u);
+		if (projections != nullptr)
+		{
+			projections[row * 2 * hidden + n] = static_cast<T>(g);
+			projections[(row * 2 + 1) * hidden + n] = static_cast<T>(u);
+		}
+	}
+	template<typename T>
+	__global__ __launch_bounds__(256) void kernel_gate_parts(const float *partial, int parts, size_t part_stride, int rows, int hidden, const T *bias, T *y, T *projections, int gate)
+	{
+		const size_t count = static_cast<size_t>(rows) * hidden;
+		for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<size_t>(gridDim.x) * 256)
+		{
+			int n;
+			const size_t row = split_index(i, hidden, n);
+			float g = 0.0f, u = 0.0f;
+			for (int p = 0; p < parts; p++)
+			{
+				const float *src = partial + p * part_stride + row * 2 * hidden + n;
+				g += src[0];
+				u += src[hidden];
+			}
+			finish_element(g, u, row, n, bias, y, projections, hidden, gate);
+		}
+	}
+	template<typename T, int MB>
+	__global__ __launch_bounds__(256) void kernel_gated_few_rows(const T *x, const T *w, T *y, int rows, int hidden, int features, const T *bias, T *projections, int gate)
+	{
+		__shared__ __attribute__((aligned(16))) float sums[2][16 * MB][16];
+		const int n0 = blockIdx.x * 16, last = min(15, hidden - 1 - n0);
+		few_rows_sums<T, MB>(x, rows, w + static_cast<size_t>(n0) * features, w + (static_cast<size_t>(hidden) + n0) * features, last, last, features, sums);
+		for (int i = threadIdx.x; i < 16 * MB * 16; i += 256)
+		{
+			const int row = i >> 4, n = i & 15;
+			if (row < rows && n <= last)
+				finish_element(sums[0][row][n], sums[1][row][n], row, n0 + n, bias, y, projections, hidden, gate);
+		}
+	}
+
+	/* ---- backward: d and the sums of its columns ------------------------------------------------------------------------------
+	 * d [rows][row_elements] holds dg at column n and du at column hidden + n, zeros from 2 hidden on. A workgroup has 256 hidden units (32 threads of 8) and 8 rows at a time of its share of the rows;
+	 * partial [gridDim.y][2 hidden] takes the sums over its rows. */
+	template<typename T>
+	__global__ __launch_bounds__(256) void kernel_gated_gradient(const T *projections, const T *dy, T *d, int rows, int hidden, int row_elements, int gate, float *partial)
+	{
+		__shared__ float sums[2][8][32 * 8 + 8];
+		const int group = threadIdx.x & 31, first_row = threadIdx.x >> 5;
+		const int n = blockIdx.x * 256 + group * 8;
+		float sum[2][8];
+#pragma unroll
+		for (int i = 0; i < 2; i++)
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				sum[i][e] = 0.0f;
+		for (int row = blockIdx.y * 8 + first_row; row < rows; row += gridDim.y * 8)
+		{
+			const T *kept = projections + static_cast<size_t>(row) * 2 * hidden + n;
+			const T *grad = dy + static_cast<size_t>(row) * hidden + n;
+			T *dst = d + static_cast<size_t>(row) * row_elements + n;
+			const int there = min(hidden - n, 8);
+			if (there == 8)
+			{
+				Elements<T, 8> g, u, v;
+				g.load(kept);
+				u.load(kept + hidden);
+				v.load(grad);
+				float dg[8], du[8];
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+				{
+					float a, slope;
+					gate_of<T, true>(gate, g[e], a, slope);
+					dg[e] = v[e] * u[e] * slope;
+					du[e] = v[e] * a;
+					sum[0][e] += dg[e];
+					sum[1][e] += du[e];
+				}
+				store_nearest<8>(dst, dg);
+				store_nearest<8>(dst + hidden, du);
+			}
+			else
+			{
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					if (e < there)
+					{
+						float a, slope;
+						gate_of<T, true>(gate, static_cast<float>(kept[e]), a, slope);
+						const float v = static_cast<float>(grad[e]);
+						const float dg = v * static_cast<float>(kept[hidden + e]) * slope, du = v * a;
+						sum[0][e] += dg;
+						sum[1][e] += du;
+						dst[e] = static_cast<T>(dg);
+						dst[hidden + e] = static_cast<T>(du);
+					}
+			}
+			if (n == 0)
+				for (int j = 2 * hidden; j < row_elements; j++)
+					d[static_cast<size_t>(row) * row_elements + j] = static_cast<T>(0.0f);
+		}
+		if (partial == nullptr)
+			return;
+#pragma unroll
+		for (int i = 0; i < 2; i++)
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				sums[i][first_row][group * 8 + e] = sum[i][e];
+		__syncthreads();
+		const int column = blockIdx.x * 256 + threadIdx.x;
+		if (column < hidden)
+#pragma unroll
+			for (int i = 0; i < 2; i++)
+			{
+				float total = 0.0f;
+#pragma unroll
+				for (int r = 0; r < 8; r++)
+					total += sums[i][r][threadIdx.x];
+				partial[static_cast<size_t>(blockIdx.y) * 2 * hidden + i * hidden + column] = total;
+			}
+	}
+
+	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
+	struct GatedShape
+	{
+			int rows, features, hidden, element_size;
+			mlDataType_t dtype;
+	};
+	GatedShape gated_shape(const mlShape_t &x, const mlShape_t &w, mlDataType_t dtype, const char *name)
+	{
+		const std::string who(name);
+		MLHIP_REQUIRE(dtype == DTYPE_FLOAT16 || dtype == DTYPE_FLOAT32, who + ": unsupported data type");
+		MLHIP_REQUIRE(x.rank >= 1 && x.rank <= 6 && w.rank == 3 && w.dim[0] == 2, who + ": the input needs one to six dimensions, the weights must be [2, hidden, features]");
+		for (int i = 0; i < x.rank; i++)
+			MLHIP_REQUIRE(x.dim[i] >= 0, who + ": negative dimension");
+		MLHIP_REQUIRE(w.dim[1] >= 0 && w.dim[2] >= 0 && w.dim[2] == last_dim(x), who + ": the weights' last dimension must be the input's");
+		MLHIP_REQUIRE(w.dim[2] > 0, who + ": no features");
+		const size_t rows = volume(x) / w.dim[2];
+		MLHIP_REQUIRE(rows <= 0x3fffffff && w.dim[1] <= (1 << 18) && w.dim[2] <= (1 << 18) && static_cast<size_t>(w.dim[1]) * w.dim[2] * size_of(dtype) <= (size_t(1) << 30),
+				who + ": too many rows, hidden units or features");
+		return GatedShape { static_cast<int>(rows), w.dim[2], w.dim[1], size_of(dtype), dtype };
+	}
+	int gradient_parts(const GatedShape &s)
+	{
+		/* about 8 workgroups of 256 threads per compute unit */
+		return std::max(1, std::min(ceil_div(s.rows, 8), 2048 / std::max(1, ceil_div(s.hidden, 256))));
+	}
+	ProductPlan forward_plan(const GatedShape &s)
+	{
+		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true);
+	}
+	ProductPlan input_plan(const GatedShape &s)
+	{
+		return plan_product(s.rows, s.features, false, 2 * s.hidden, s.element_size, true);
+	}
+	ProductPlan weights_plan(const GatedShape &s)
+	{
+		return plan_product(2 * s.hidden, s.features, false, s.rows, s.element_size, true);
+	}
+	/* the pieces of a workspace, each aligned to 256 bytes */
+	struct GatedSpace
+	{
+			size_t x, w, parts, d, sums, total;
+	};
+	GatedSpace gated_space(const GatedShape &s, bool backward)
+	{
+		GatedSpace space;
+		size_t at = 0;
+		const auto take = [&](size_t bytes)
+		{
+			const size_t begin = at;
+			at += round_up(bytes, 256);
+			return begin;
+		};
+		const int pieces = 16 / s.element_size;
+		const size_t padded = (s.features % pieces == 0) ? 0 : round_up(s.features, pieces) * s.element_size;
+		const bool tiles = backward || s.rows > MOST_FEW_ROWS;
+		space.x = take(tiles ? padded * s.rows : 0);
+		space.w = take(tiles ? padded * 2 * s.hidden : 0);
+		if (backward)
+		{
+			space.parts = take(std::max(part_bytes(input_plan(s), s.rows, s.features), part_bytes(weights_plan(s), 2 * s.hidden, s.features)));
+			space.d = take(round_up(2 * s.hidden, pieces) * s.element_size * s.rows);
+			space.sums = take(sizeof(float) * 2 * s.hidden * gradient_parts(s));
+		}
+		else
+		{
+			space.parts = take(tiles ? part_bytes(forward_plan(s), s.rows, 2 * s.hidden) : 0);
+			space.d = space.sums = at;
+		}
+		space.total = at;
+		return space;
+	}
+
+	template<typename T>
+	void gated_forward(hipStream_t stream, const GatedShape &s, const T *x, const T *w, const T *bias, T *y, T *projections, int gate, uint8_t *workspace)
+	{
+		if (s.rows <= MOST_FEW_ROWS)
+		{
+			const dim3 grid(ceil_div(s.hidden, 16));
+			const auto launch = [&](auto kernel)
+			{
+				hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, w, y, s.rows, s.hidden, s.features, bias, projections, gate);
+			};
+			if (s.rows <= 16)
+				launch(kernel_gated_few_rows<T, 1>);
+			else if (s.rows <= 32)
+				launch(kernel_gated_few_rows<T, 2>);
+			else
+				launch(kernel_gated_few_rows<T, 4>);
+			MLHIP_CHECK(hipGetLastError());
+			return;
+		}
+		const GatedSpace space = gated_space(s, false);
+		const size_t row_bytes = static_cast<size_t>(padded_columns<T>(s.features)) * sizeof(T);
+		x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
+		w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), 2 * static_cast<size_t>(s.hidden), s.features);
+		const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded_columns<T>(s.features) };
+		const Operand b { reinterpret_cast<const uint8_t*>(w), row_bytes, s.hidden, padded_columns<T>(s.features), row_bytes * s.hidden };
+		const ProductPlan plan = forward_plan(s);
+		if (plan.parts == 1)
+			launch_product<T, Side::ROWS, Side::ROWS, true>(stream, plan, a, b, s.rows, GatedEpilogue<T> { y, projections, bias, s.hidden, gate });
+		else
+		{
+			float *partial = reinterpret_cast<float*>(workspace + space.parts);
+			const size_t stride = static_cast<size_t>(s.rows) * 2 * s.hidden, count = static_cast<size_t>(s.rows) * s.hidden;
+			launch_product<T, Side::ROWS, Side::ROWS, true>(stream, plan, a, b, s.rows, GatedPartEpilogue { partial, stride, s.hidden });
+			hipLaunchKernelGGL((kernel_gate_parts<T>), dim3(static_cast<unsigned int>(std::min<size_t>((count + 255) / 256, 8192))), dim3(256), 0, stream, partial, plan.parts, stride, s.rows,
+					s.hidden, bias, y, projections, gate);
+			MLHIP_CHECK(hipGetLastError());
+		}
+	}
+	template<typename T>
+	void gated_backward(hipStream_t stream, const GatedShape &s, const T *x, const T *w, const T *projections, const T *dy, float beta_dx, T *dx, float beta_weights,
+			const mlTensor_t &dw, const mlTensor_t &db, int gate, uint8_t *workspace)
+	{
+		const GatedSpace space = gated_space(s, true);
+		const int both = 2 * s.hidden, row_elements = padded_columns<T>(both), padded = padded_columns<T>(s.features);
+		T *d = reinterpret_cast<T*>(workspace + space.d);
+		float *sums = reinterpret_cast<float*>(workspace + space.sums), *partial = reinterpret_cast<float*>(workspace + space.parts);
+		const int parts = gradient_parts(s);
+		if (s.rows > 0 && s.hidden > 0)
+		{
+			hipLaunchKernelGGL((kernel_gated_gradient<T>), dim3(ceil_div(s.hidden, 256), parts), dim3(256), 0, stream, projections, dy, d, s.rows, s.hidden, row_elements, gate,
+					db.data != nullptr ? sums : nullptr);
+			MLHIP_CHECK(hipGetLastError());
+		}
+		if (db.data != nullptr)
+			launch_sum_partials(stream, sums, s.rows > 0 ? parts : 0, static_cast<size_t>(both), db.data, db.dtype, both, beta_weights);
+		const Operand d_rows { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), s.rows, row_elements };
+		if (dx != nullptr && s.rows > 0)
+		{
+			w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), static_cast<size_t>(both), s.features);
+			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), padded, both };
+			product_to<T, T, Side::ROWS, Side::COLUMNS>(stream, input_plan(s), d_rows, b, s.rows, s.features, dx, beta_dx, nullptr, partial);
+		}
+		if (dw.data != nullptr)
+		{
+			x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
+			const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), row_elements, s.rows };
+			const Operand b { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), padded, s.rows };
+			if (dw.dtype == DTYPE_FLOAT32)
+				product_to<T, float, Side::COLUMNS, Side::COLUMNS>(stream, weights_plan(s), a, b, both, s.features, ptr<float>(dw), beta_weights, nullptr, partial);
+			else if constexpr (sizeof(T) == 2)
+				product_to<T, T, Side::COLUMNS, Side::COLUMNS>(stream, weights_plan(s), a, b, both, s.features, ptr<T>(dw), beta_weights, nullptr, partial);
+		}
+	}
+	void require_like(const mlTensor_t &t, const mlTensor_t &x, int last, const char *what)
+	{
+		MLHIP_REQUIRE(t.dtype == x.dtype && t.rank == x.rank && last_dim(t) == last, std::string(what) + ": shape or type");
+		for (int i = 0; i + 1 < x.rank; i++)
+			MLHIP_REQUIRE(t.dim[i] == x.dim[i], std::string(what) + ": shape");
+	}
+	void require_workspace(const void *workspace, size_t given, size_t needed, const char *name)
+	{
+		MLHIP_REQUIRE(needed == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && given >= needed),
+				std::string(name) + ": the workspace is too small or not aligned to 256 bytes");
+	}
+	bool aligned_16(const mlTensor_t &t)
+	{
+		return reinterpret_cast<uintptr_t>(t.data) % 16 == 0;
+	}
+}
+
+extern "C"
+{
+	using namespace mlhip;
+
+	size_t hip_gated_dense_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, mlDataType_t dtype, bool backward)
+	try
+	{
+		return gated_space(gated_shape(input_shape, weights_shape, dtype, "gated_dense_get_workspace_size"), backward).total;
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<size_t>();
+	}
+
+	void hip_gated_dense_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, mlTensor_t y, mlTensor_t projections, mlGate_t gate, void *workspace,
+			size_t workspace_size)
+	try
+	{
+		const char *name = "gated_dense_forward";
+		const GatedShape s = gated_shape(shape_of(x), shape_of(w), x.dtype, name);
+		MLHIP_REQUIRE(gate >= GATE_SIGMOID && gate <= GATE_GELU, "gated_dense_forward: unknown gate");
+		MLHIP_REQUIRE(w.dtype == x.dtype, "gated_dense_forward: weights must have the input's type");
+		MLHIP_REQUIRE(b.data == nullptr || (b.dtype == x.dtype && volume(b) == 2 * static_cast<size_t>(s.hidden)), "gated_dense_forward: the bias must be [2, hidden] of the input's type");
+		require_like(y, x, s.hidden, "gated_dense_forward: output");
+		MLHIP_REQUIRE(projections.data == nullptr || (projections.dtype == x.dtype && volume(projections) == 2 * static_cast<size_t>(s.hidden) * s.rows && last_dim(projections) == s.hidden),
+				"gated_dense_forward: the projections must be [.., 2, hidden] of the input's type");
+		if (s.rows == 0 || s.hidden == 0)
+			return;
+		MLHIP_REQUIRE(x.data != nullptr && w.data != nullptr && y.data != nullptr, "gated_dense_forward: null pointer");
+		MLHIP_REQUIRE(aligned_16(x) && aligned_16(w), "gated_dense_forward: input and weights must be aligned to 16 bytes");
+		require_workspace(workspace, workspace_size, gated_space(s, false).total, name);
+		const hipStream_t stream = stream_of(context);
+		if (x.dtype == DTYPE_FLOAT16)
+			gated_forward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<half_t>(y), ptr<half_t>(projections), gate, reinterpret_cast<uint8_t*>(workspace));
+		else
+			gated_forward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<float>(y), ptr<float>(projections), gate, reinterpret_cast<uint8_t*>(workspace));
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+
+	void hip_gated_dense_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t projections, const mlTensor_t dy, float beta_dx, mlTensor_t dx,
+			float beta_weights, mlTensor_t dw, mlTensor_t db, mlGate_t gate, void *workspace, size_t workspace_size)
+	try
+	{
+		const char *name = "gated_dense_backward";
+		const GatedShape s = gated_shape(shape_of(x), shape_of(w), x.dtype, name);
+		MLHIP_REQUIRE(gate >= GATE_SIGMOID && gate <= GATE_GELU, "gated_dense_backward: unknown gate");
+		MLHIP_REQUIRE(w.dtype == x.dtype, "gated_dense_backward: weights must have the input's type");
+		require_like(dy, x, s.hidden, "gated_dense_backward: gradient");
+		MLHIP_REQUIRE(projections.dtype == x.dtype && volume(projections) == 2 * static_cast<size_t>(s.hidden) * s.rows && (s.rows == 0 || last_dim(projections) == s.hidden),
+				"gated_dense_backward: the projections must be [.., 2, hidden] of the input's type");
+		if (dx.data != nullptr)
+			require_like(dx, x, s.features, "gated_dense_backward: dx");
+		const auto weight_type = [&](const mlTensor_t &t)
+		{
+			return t.dtype == x.dtype || t.dtype == DTYPE_FLOAT32;
+		};
+		MLHIP_REQUIRE(dw.data == nullptr || (weight_type(dw) && volume(dw) == volume(w)), "gated_dense_backward: dw must be [2, hidden, features] of the input's type or fp32");
+		MLHIP_REQUIRE(db.data == nullptr || (weight_type(db) && volume(db) == 2 * static_cast<size_t>(s.hidden)), "gated_dense_backward: db must be [2, hidden] of the input's type or fp32");
+		if (dx.data == nullptr && dw.data == nullptr && db.data == nullptr)
+			return;
+		if (s.hidden == 0 && (dx.data == nullptr || s.rows == 0))
+			return;
+		MLHIP_REQUIRE(s.hidden > 0, "gated_dense_backward: no hidden units");
+		MLHIP_REQUIRE(s.rows == 0 || (x.data != nullptr && w.data != nullptr && projections.data != nullptr && dy.data != nullptr), "gated_dense_backward: null pointer");
+		MLHIP_REQUIRE(aligned_16(x) && aligned_16(w), "gated_dense_backward: input and weights must be aligned to 16 bytes");
+		require_workspace(workspace, workspace_size, gated_space(s, true).total, name);
+		const hipStream_t stream = stream_of(context);
+		if (x.dtype == DTYPE_FLOAT16)
+			gated_backward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(projections), ptr<half_t>(dy), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, gate,
+					reinterpret_cast<uint8_t*>(workspace));
+		else
+			gated_backward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(projections), ptr<float>(dy), beta_dx, ptr<float>(dx), beta_weights, dw, db, gate,
+					reinterpret_cast<uint8_t*>(workspace));
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+}

@@ -1,0 +1,789 @@
+/*
+ * product_tiles.hpp — the products of a layer's forward and backward pass on tiles of 256x256 or 128x128: ACC[m][n] = sum_k A(m, k) B(n, k), where each operand lies in memory
+ * either with its rows along k (ROWS) or with its rows across k (COLUMNS: element (m, k) at [k][m]). The three products of a layer y = x W^T need both:
+ *     y  = x W^T       m = token, n = output, k = input     A = x ROWS,        B = W ROWS
+ *     dx = d W         m = token, n = input,  k = output    A = d ROWS,        B = W COLUMNS
+ *     dW = d^T x       m = output, n = input, k = token     A = d COLUMNS,     B = x COLUMNS
+ * so no operand is transposed in memory.
+ *
+ * Operands move L2 -> LDS by direct-to-LDS loads in panels of 128 rows (of m or n) by 128 bytes of k, 16 KB each, which lie in LDS as they lie in memory:
+ *   ROWS     [128 rows][128 bytes of k], the 16-byte pieces of a row permuted by (row / 2) % 8: an MFMA fragment is 16 bytes of one row, and the rows of a wavefront's read meet all banks;
+ *   COLUMNS  [k][128 columns], the 32-column blocks of a row permuted by k: a fragment is gathered across k, in fp16 by the LDS's transposing read (a group of 16 lanes reads 4 rows of 16 columns, and each lane
+ *            gets the 4 values of one column), in fp32 element by element.
+ * Both kinds give a lane the same k, so they can be mixed. The loads go through a buffer descriptor whose base is a scalar that walks along k: a lane holds one 32-bit offset per load for the whole
+ * product, whatever the size of the operand, and a lane that lies outside (a row past the end, k past the end) is sent behind the buffer's end, which reads as zero. So no element outside an operand
+ * reaches an accumulator, and NaN or infinities beside it do not either.
+ *
+ * 256x256 (8 wavefronts, one workgroup per compute unit): two slots of four panels, refilled panel by panel: the wavefront's 128 x 64 share is multiplied in four phases of 64 x 32, and a panel's place
+ * takes the chunk after the next one as soon as its last phase is over, so a load has six phases (one and a half chunks of 64 k) to arrive.
+ * 128x128 (4 wavefronts, two workgroups per compute unit, which hide each other's waits): where 256x256 tiles would leave units without work.
+ * A product with a long k and few tiles is split along k (gridDim.y): each part leaves its sums in fp32, and a launch of its own adds them up in order.
+ *
+ * The tile's accumulators pass through LDS in fp32, 128 rows at a time, so that the epilogue sees 8 consecutive columns per thread and whole lines per wavefront.
+ */
+#ifndef MINML_AMD_PRODUCT_TILES_HPP_
+#define MINML_AMD_PRODUCT_TILES_HPP_
+
+#include "common.hpp"
+#include "gemm_dma.hpp"
+#include "training_utils.hpp"
+
+#include <algorithm>
+
+namespace mlhip
+{
+	enum class Side
+	{
+		ROWS, COLUMNS
+	};
+	/*
+	 * One operand. Bytes between rows (of memory) and the base are multiples of 16. `depth` counts what lies along k: elements for ROWS (whole 16-byte pieces: what lies behind the last element of its piece
+	 * has to be zero), rows for COLUMNS. extent: rows of m (n) that exist; for COLUMNS whole 16-byte pieces.
+	 * PAIRED rows: the operand is two matrices of `extent` rows, `pair_bytes` apart, and a tile takes half its rows from each (first half of the tile: first matrix).
+	 */
+	struct Operand
+	{
+			const uint8_t *base;
+			size_t row_bytes;
+			int extent;
+			int depth;
+			size_t pair_bytes = 0;
+	};
+	constexpr int PANEL = 128; /* rows of a panel */
+	constexpr int PANEL_BYTES = PANEL * 128;
+	constexpr int OUTSIDE = static_cast<int>(0x80000000u); /* as an unsigned offset behind any buffer's end */
+
+	/* in a scalar register, as the addresses made of it are then */
+	__device__ __forceinline__ int wave_number()
+	{
+		return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	}
+	/* 16 bytes per lane from the buffer to `place` + 16 * lane of LDS. The builtin is for the device pass alone: in the host pass every template that holds it loses its launch stub from the second
+	 * instance on */
+	__device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t buffer, uint8_t *place, int offset)
+	{
+#if defined(__HIP_DEVICE_COMPILE__)
+		__builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_ptr_t) place, 16, offset, 0, 0, 0);
+#endif
+	}
+
+	/* the loads of one panel by WAVES wavefronts, 1 KB each. SEGMENT: consecutive rows of the operand in a panel (64 where a panel holds both halves of a paired tile) */
+	template<typename T, Side SIDE, int WAVES, int SEGMENT = PANEL>
+	struct PanelLoads
+	{
+			static constexpr int COUNT = 16 / WAVES;
+			static constexpr int CHUNK = 128 / sizeof(T); /* k of a chunk */
+			static constexpr int K_PER_LOAD = 1024 / (PANEL * sizeof(T)); /* COLUMNS: rows of k that one load covers */
+			int offset[COUNT];
+			int k; /* ROWS: first byte of the lane's piece in its 128; COLUMNS: row of k of the lane's first load */
+
+			/* `there`: rows of the operand from the panel's first on */
+			__device__ __forceinline__ void begin(int there, size_t row_bytes, size_t pair_bytes)
+			{
+				const int lane = threadIdx.x & 63, wave = wave_number();
+				if constexpr (SIDE == Side::ROWS)
+				{
+					/* the permutation (row / 2) % 8 is the same for all loads of a lane: their rows differ by multiples of 16 */
+					k = ((lane & 7) ^ dma_swizzle(wave * 8 + (lane >> 3))) * 16;
+#pragma unroll
+					for (int u = 0; u < COUNT; u++)
+					{
+						const int place = (wave + WAVES * u) * 8 + (lane >> 3);
+						const int row = place % SEGMENT;
+						offset[u] = (row < there) ? static_cast<int>(row * row_bytes + (place / SEGMENT) * pair_bytes) + k : OUTSIDE;
+					}
+				}
+				else
+				{
+					constexpr int PIECES = 32 * sizeof(T) / 16, LANES = 64 / K_PER_LOAD; /* 16-byte pieces of a block of 32 columns; lanes of a row */
+					k = wave * K_PER_LOAD + lane / LANES;
+#pragma unroll
+					for (int u = 0; u < COUNT; u++)
+					{
+						const int row = k + u * WAVES * K_PER_LOAD, position = lane % LANES;
+						const int permuted = (sizeof(T) == 2) ? (row & 3) : ((row >> 2) & 1);
+						const int column = ((position / PIECES) ^ permuted) * 32 + (position % PIECES) * (16 / static_cast<int>(sizeof(T)));
+						offset[u] = (column < there) ? static_cast<int>(row * row_bytes + column * sizeof(T)) : OUTSIDE;
+					}
+				}
+			}
+			/* `left`: bytes (ROWS) or rows (COLUMNS) of k from the chunk's first on */
+			__device__ __forceinline__ void request(const uint8_t *base, int left, uint8_t *panel) const
+			{
+				const int wave = wave_number();
+				const __amdgpu_buffer_rsrc_t buffer = buffer_of(const_cast<uint8_t*>(base));
+#pragma unroll
+				for (int u = 0; u < COUNT; u++)
+				{
+					const int at = (SIDE == Side::ROWS) ? k : k + u * WAVES * K_PER_LOAD;
+					buffer_to_lds(buffer, panel + (wave + WAVES * u) * 1024, (at < left) ? offset[u] : OUTSIDE);
+				}
+			}
+	};
+	/* where the scalar base of an operand's panels walks */
+	template<typename T, Side SIDE>
+	struct PanelWalk
+	{
+			const uint8_t *base;
+			size_t step;
+			int left;
+
+			__device__ __forceinline__ void begin(const Operand &o, int first_row, int first_chunk, int chunks)
+			{
+				constexpr int CHUNK = 128 / sizeof(T);
+				step = (SIDE == Side::ROWS) ? 128 : CHUNK * o.row_bytes;
+				base = o.base + (SIDE == Side::ROWS ? first_row * o.row_bytes : first_row * sizeof(T)) + first_chunk * step;
+				const int per_chunk = (SIDE == Side::ROWS) ? 128 : CHUNK;
+				const int depth = (SIDE == Side::ROWS) ? o.depth * static_cast<int>(sizeof(T)) : o.depth;
+				left = min(depth - first_chunk * per_chunk, chunks * per_chunk);
+			}
+			__device__ __forceinline__ void advance()
+			{
+				base += step;
+				left -= (SIDE == Side::ROWS) ? 128 : 128 / static_cast<int>(sizeof(T));
+			}
+	};
+	/*
+	 * The transposing read of LDS. The compiler would wait for every outstanding direct-to-LDS load before a read that says nothing about what it may alias, which is to wait for the panels two chunks
+	 * ahead; a restricted pointer says that, as the type does for ordinary reads. What a read really depends on is counted by the kernels.
+	 */
+	typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+	typedef __attribute__((address_space(3))) fp16x4 *transposed_place_t;
+	__device__ __forceinline__ uint2_t read_transposed(const transposed_place_t __restrict__ place)
+	{
+		return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16(place));
+	}
+	/* fragments of a panel: block b (32 rows of the panel), k step kk of 4. Lane l: row l % 32, k = 16 / sizeof(T) * (2 kk + l / 32) onwards */
+	template<typename T, Side SIDE>
+	struct PanelFragments
+	{
+			int first;
+
+			__device__ __forceinline__ void begin(int block)
+			{
+				const int lane = threadIdx.x & 63;
+				if constexpr (SIDE == Side::ROWS)
+					first = (block * 32 + (lane & 31)) * 128 + (((lane >> 5) ^ dma_swizzle(lane & 31)) * 16);
+				else if constexpr (sizeof(T) == 2)
+				{
+					const int t = lane & 15;
+					first = ((lane >> 5) * 8 + (t >> 2)) * 256 + ((block ^ (t >> 2)) * 64) + ((lane >> 4) & 1) * 32 + (t & 3) * 8;
+				}
+				else
+					first = (lane >> 5) * 2048 + ((block ^ (lane >> 5)) * 128) + (lane & 31) * 4;
+			}
+			__device__ __forceinline__ uint4_t read(const uint8_t *panel, int kk) const
+			{
+				if constexpr (SIDE == Side::ROWS)
+					return *reinterpret_cast<const uint4_t*>(panel + (first ^ (kk * 32)));
+				else if constexpr (sizeof(T) == 2)
+				{
+					const uint2_t lo = read_transposed((transposed_place_t) (panel + first + kk * 4096));
+					const uint2_t hi = read_transposed((transposed_place_t) (panel + first + kk * 4096 + 1024));
+					return uint4_t { lo[0], lo[1], hi[0], hi[1] };
+				}
+				else
+				{
+					uint4_t v;
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						v[e] = *reinterpret_cast<const uint32_t*>(panel + first + kk * 4096 + e * 512);
+					return v;
+				}
+			}
+	};
+
+	struct ProductArgs
+	{
+			Operand a, b;
+			int rows; /* of the result */
+			int tiles_m, tiles_n;
+			int chunks; /* of the whole product */
+			int chunks_per_part; /* of one gridDim.y */
+	};
+	constexpr int TILE_GROUP = 8;
+	/*
+	 * Order of the tiles: every XCD has one contiguous eighth of them, walked in groups of 8 rows of tiles, down the rows first: the 32 tiles that an XCD has in hand at a time then need 8 panels' worth of
+	 * rows and 4 of columns, near the least that 32 tiles can share.
+	 */
+	__device__ __forceinline__ void tile_of_block(const ProductArgs &p, int &tile_m, int &tile_n)
+	{
+		const unsigned int id = xcd_contiguous_block_id(blockIdx.x, gridDim.x);
+		const unsigned int group_tiles = TILE_GROUP * p.tiles_n;
+		const unsigned int group = id / group_tiles, within = id - group * group_tiles;
+		const unsigned int rows = min(static_cast<unsigned int>(p.tiles_m) - group * TILE_GROUP, static_cast<unsigned int>(TILE_GROUP));
+		tile_n = within / rows;
+		tile_m = group * TILE_GROUP + within - tile_n * rows;
+	}
+
+	/*
+	 * The end of a tile: accumulator blocks to LDS, then rows to the epilogue. Lane l, register r of block (i, j) holds n = 32 j' + 8 (r / 4) + 4 (l / 32) + r % 4, m = 32 i' + l % 32.
+	 * Epilogue: a thread takes SHARE of the BN sums of a row. begin(state, group, tile_n) once per tile, apply(state, m, group, row, tile_n, part) for every row m < rows with `row` its sums in LDS (all threads
+	 * of a row together), and, where HAS_END, end(state, group, stage, tile_m, tile_n) once all rows are through, by all threads.
+	 */
+	template<int BN, int WAVES, typename Epilogue, typename State>
+	__device__ __forceinline__ void rows_to_epilogue(State &state, const float *stage, int m0, int M, int tile_n, const Epilogue &epilogue)
+	{
+		constexpr int STRIDE = BN + 4, GROUPS = BN / Epilogue::SHARE, ROWS_AT_A_TIME = WAVES * 64 / GROUPS;
+		const int group = threadIdx.x % GROUPS;
+		for (int row = threadIdx.x / GROUPS; row < PANEL; row += ROWS_AT_A_TIME)
+			if (m0 + row < M)
+				epilogue.template apply<BN>(state, m0 + row, group, stage + row * STRIDE, tile_n, blockIdx.y);
+	}
+	template<typename Acc>
+	__device__ __forceinline__ void block_to_stage(float *stage, int stride, int row, int column, const Acc &acc)
+	{
+		const int lane = threadIdx.x & 63;
+		float *dst = stage + (row + (lane & 31)) * stride + column + 4 * (lane >> 5);
+#pragma unroll
+		for (int q = 0; q < 4; q++)
+			*reinterpret_cast<float4_t*>(dst + 8 * q) = float4_t { acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3] };
+	}
+
+	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
+	__global__ __launch_bounds__(512, 1) void kernel_product_256(ProductArgs p, Epilogue epilogue)
+	{
+		typedef MfmaTraits<T> Traits;
+		typedef typename Traits::acc_vec acc_vec;
+		constexpr int WAVES = 8, LOADS = PanelLoads<T, SA, WAVES>::COUNT;
+		constexpr int A0 = 0, B0 = 1, B1 = 2, A1 = 3; /* panels of a slot */
+		constexpr int SLOT = 4 * PANEL_BYTES;
+		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+		int tile_m, tile_n;
+		tile_of_block(p, tile_m, tile_n);
+		const int first_chunk = blockIdx.y * p.chunks_per_part;
+		const int chunks = min(p.chunks_per_part, p.chunks - first_chunk);
+		const int wave = wave_number(), wave_m = wave >> 2, wave_n = wave & 3;
+
+		PanelLoads<T, SA, WAVES> a_loads[2];
+		PanelLoads<T, SB, WAVES> b_loads[2];
+		PanelWalk<T, SA> a_walk[2];
+		PanelWalk<T, SB> b_walk[2];
+#pragma unroll
+		for (int h = 0; h < 2; h++)
+		{
+			const int m = tile_m * 256 + h * PANEL;
+			a_loads[h].begin(p.a.extent - m, p.a.row_bytes, 0);
+			a_walk[h].begin(p.a, m, first_chunk, chunks);
+			const int n = PAIRED ? tile_n * PANEL : tile_n * 256 + h * PANEL;
+			b_loads[h].begin(p.b.extent - n, p.b.row_bytes, 0);
+			b_walk[h].begin(p.b, n, first_chunk, chunks);
+			if (PAIRED && h == 1)
+				b_walk[h].base += p.b.pair_bytes;
+		}
+		const auto request_a = [&](int chunk, auto half) __attribute__((always_inline))
+		{
+			constexpr int h = decltype(half)::value;
+			a_loads[h].request(a_walk[h].base, a_walk[h].left, lds + (chunk & 1) * SLOT + (h == 0 ? A0 : A1) * PANEL_BYTES);
+			a_walk[h].advance();
+		};
+		const auto request_b = [&](int chunk, auto half) __attribute__((always_inline))
+		{
+			constexpr int h = decltype(half)::value;
+			b_loads[h].request(b_walk[h].base, b_walk[h].left, lds + (chunk & 1) * SLOT + (h == 0 ? B0 : B1) * PANEL_BYTES);
+			b_walk[h].advance();
+		};
+		typedef std::integral_constant<int, 0> zero;
+		typedef std::integral_constant<int, 1> one;
+		typedef std::integral_constant<int, 2> two;
+
+		PanelFragments<T, SA> a_place[2];
+		PanelFragments<T, SB> b_place;
+		a_place[0].begin(2 * wave_m);
+		a_place[1].begin(2 * wave_m + 1);
+		b_place.begin(wave_n);
+		uint4_t fa[2][4], fb0[4], fb1[4];
+		const auto read_a = [&](int chunk, int panel, int kk) __attribute__((always_inline))
+		{
+			const uint8_t *src = lds + (chunk & 1) * SLOT + panel * PANEL_BYTES;
+#pragma unroll
+			for (int i = 0; i < 2; i++)
+				fa[i][kk] = a_place[i].read(src, kk);
+		};
+		const auto read_b = [&](int chunk, int panel, int kk, uint4_t (&regs)[4]) __attribute__((always_inline))
+		{
+			regs[kk] = b_place.read(lds + (chunk & 1) * SLOT + panel * PANEL_BYTES, kk);
+		};
+
+		acc_vec acc[4][2];
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+#pragma unroll
+			for (int j = 0; j < 2; j++)
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					acc[i][j][r] = 0;
+
+		for (int c = 0; c < 2; c++)
+			if (c < chunks)
+			{
+				request_a(c, zero());
+				request_b(c, zero());
+				request_b(c, one());
+				request_a(c, one());
+			}
+		if (chunks > 1)
+			wait_vmcnt<6 * LOADS>();
+		else
+			wait_vmcnt<2 * LOADS>();
+		barrier_no_fence();
+		if (chunks > 0)
+		{
+#pragma unroll
+			for (int kk = 0; kk < 4; kk++)
+			{
+				read_a(0, A0, kk);
+				read_b(0, B0, kk, fb0);
+			}
+		}
+		/* one chunk: whether there is a next one, and whether there is one after it */
+		const auto process_chunk = [&](int c, auto one_more, auto two_more) __attribute__((always_inline))
+		{
+			constexpr bool NEXT = decltype(one_more)::value, AFTER = decltype(two_more)::value;
+			const auto multiply = [&](int kk, const uint4_t (&regs)[4], auto row, auto column) __attribute__((always_inline))
+			{
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+					Traits::mma(regs[kk], fa[i][kk], acc[decltype(row)::value + i][decltype(column)::value]);
+			};
+			/* phase 0: A0 B0. Behind B1 of this chunk: its A1, all of the next one */
+			wait_vmcnt<NEXT ? 5 * LOADS : LOADS>();
+			barrier_no_fence();
+			multiply(0, fb0, zero(), zero());
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int kk = 0; kk < 4; kk++)
+				read_b(c, B1, kk, fb1);
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int kk = 1; kk < 4; kk++)
+				multiply(kk, fb0, zero(), zero());
+			__builtin_amdgcn_sched_barrier(0);
+			/* phase 1: A0 B1. Behind A1: all of the next chunk. A0 and B0 have been read by all */
+			wait_vmcnt<NEXT ? 4 * LOADS : 0>();
+			barrier_no_fence();
+			multiply(0, fb1, zero(), one());
+			__builtin_amdgcn_sched_barrier(0);
+			read_a(c, A1, 0);
+			if constexpr (AFTER)
+			{
+				request_a(c + 2, zero());
+				request_b(c + 2, zero());
+			}
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int kk = 1; kk < 4; kk++)
+			{
+				multiply(kk, fb1, zero(), one());
+				__builtin_amdgcn_sched_barrier(0);
+				read_a(c, A1, kk);
+				__builtin_amdgcn_sched_barrier(0);
+			}
+			/* phase 2: A1 B1, whose fragments are in registers */
+			barrier_no_fence();
+			multiply(0, fb1, two(), one());
+			__builtin_amdgcn_sched_barrier(0);
+			if constexpr (AFTER)
+				request_b(c + 2, one());
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int kk = 1; kk < 4; kk++)
+				multiply(kk, fb1, two(), one());
+			__builtin_amdgcn_sched_barrier(0);
+			/* phase 3: A1 B0. Behind A0 and B0 of the next chunk: its other two panels, three of the one after it */
+			if constexpr (NEXT)
+			{
+				wait_vmcnt<AFTER ? 5 * LOADS : 2 * LOADS>();
+				barrier_no_fence();
+			}
+			multiply(0, fb0, two(), zero());
+			__builtin_amdgcn_sched_barrier(0);
+			if constexpr (NEXT)
+			{
+				read_a(c + 1, A0, 0);
+				read_b(c + 1, B0, 0, fb0);
+			}
+			if constexpr (AFTER)
+				request_a(c + 2, one());
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int kk = 1; kk < 4; kk++)
+			{
+				multiply(kk, fb0, two(), zero());
+				__builtin_amdgcn_sched_barrier(0);
+				if constexpr (NEXT)
+				{
+					read_a(c + 1, A0, kk);
+					read_b(c + 1, B0, kk, fb0);
+				}
+				__builtin_amdgcn_sched_barrier(0);
+			}
+		};
+		int c = 0;
+		for (; c + 2 < chunks; c++)
+			process_chunk(c, std::true_type(), std::true_type());
+		if (c + 1 < chunks)
+			process_chunk(c++, std::true_type(), std::false_type());
+		if (c < chunks)
+			process_chunk(c, std::false_type(), std::false_type());
+
+		/* block (i, j): rows (i / 2) 128 + wave_m 64 + (i % 2) 32, columns j 128 + wave_n 32 */
+		float *stage = reinterpret_cast<float*>(lds);
+		const int group = threadIdx.x % (256 / Epilogue::SHARE);
+		typename Epilogue::State state;
+		epilogue.template begin<256>(state, group, tile_n);
+		static_for<2>([&](auto half)
+		{
+			constexpr int h = decltype(half)::value;
+			__syncthreads();
+#pragma unroll
+			for (int i = 0; i < 2; i++)
+#pragma unroll
+				for (int j = 0; j < 2; j++)
+					block_to_stage(stage, 260, wave_m * 64 + i * 32, j * PANEL + wave_n * 32, acc[2 * h + i][j]);
+			__syncthreads();
+			rows_to_epilogue<256, WAVES>(state, stage, tile_m * 256 + h * PANEL, p.rows, tile_n, epilogue);
+		});
+		if constexpr (Epilogue::HAS_END)
+		{
+			__syncthreads();
+			epilogue.template end<256, WAVES>(state, group, stage, tile_m, tile_n);
+		}
+	}
+
+	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
+	__global__ __launch_bounds__(256, 2) void kernel_product_128(ProductArgs p, Epilogue epilogue)
+	{
+		typedef MfmaTraits<T> Traits;
+		typedef typename Traits::acc_vec acc_vec;
+		constexpr int WAVES = 4, SLOT = 2 * PANEL_BYTES;
+		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+		int tile_m, tile_n;
+		tile_of_block(p, tile_m, tile_n);
+		const int first_chunk = blockIdx.y * p.chunks_per_part;
+		const int chunks = min(p.chunks_per_part, p.chunks - first_chunk);
+		const int wave = wave_number(), wave_m = wave >> 1, wave_n = wave & 1;
+
+		PanelLoads<T, SA, WAVES> a_loads;
+		PanelLoads<T, SB, WAVES, PAIRED ? 64 : PANEL> b_loads;
+		PanelWalk<T, SA> a_walk;
+		PanelWalk<T, SB> b_walk;
+		const int m0 = tile_m * PANEL, n0 = tile_n * (PAIRED ? 64 : PANEL);
+		a_loads.begin(p.a.extent - m0, p.a.row_bytes, 0);
+		a_walk.begin(p.a, m0, first_chunk, chunks);
+		b_loads.begin(p.b.extent - n0, p.b.row_bytes, p.b.pair_bytes);
+		b_walk.begin(p.b, n0, first_chunk, chunks);
+		const auto request = [&](int chunk) __attribute__((always_inline))
+		{
+			uint8_t *slot = lds + (chunk & 1) * SLOT;
+			a_loads.request(a_walk.base, a_walk.left, slot);
+			b_loads.request(b_walk.base, b_walk.left, slot + PANEL_BYTES);
+			a_walk.advance();
+			b_walk.advance();
+		};
+		/* block (i, j): rows i 64 + wave_m 32, columns j 64 + wave_n 32 */
+		PanelFragments<T, SA> a_place[2];
+		PanelFragments<T, SB> b_place[2];
+#pragma unroll
+		for (int i = 0; i < 2; i++)
+		{
+			a_place[i].begin(2 * i + wave_m);
+			b_place[i].begin(2 * i + wave_n);
+		}
+		acc_vec acc[2][2];
+#pragma unroll
+		for (int i = 0; i < 2; i++)
+#pragma unroll
+			for (int j = 0; j < 2; j++)
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					acc[i][j][r] = 0;
+		if (chunks > 0)
+			request(0);
+		for (int c = 0; c < chunks; c++)
+		{
+			wait_lgkmcnt<0>(); /* this wavefront's reads of the other slot are complete before anyone may overwrite it */
+			wait_vmcnt<0>();
+			barrier_no_fence();
+			if (c + 1 < chunks)
+				request(c + 1);
+			const uint8_t *slot = lds + (c & 1) * SLOT;
+#pragma unroll
+			for (int kk = 0; kk < 4; kk++)
+			{
+				uint4_t fa[2], fb[2];
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+				{
+					fa[i] = a_place[i].read(slot, kk);
+					fb[i] = b_place[i].read(slot + PANEL_BYTES, kk);
+				}
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+#pragma unroll
+					for (int j = 0; j < 2; j++)
+						Traits::mma(fb[j], fa[i], acc[i][j]);
+			}
+		}
+		float *stage = reinterpret_cast<float*>(lds);
+		__syncthreads();
+#pragma unroll
+		for (int i = 0; i < 2; i++)
+#pragma unroll
+			for (int j = 0; j < 2; j++)
+				block_to_stage(stage, 132, i * 64 + wave_m * 32, j * 64 + wave_n * 32, acc[i][j]);
+		__syncthreads();
+		const int group = threadIdx.x % (128 / Epilogue::SHARE);
+		typename Epilogue::State state;
+		epilogue.template begin<128>(state, group, tile_n);
+		rows_to_epilogue<128, WAVES>(state, stage, m0, p.rows, tile_n, epilogue);
+		if constexpr (Epilogue::HAS_END)
+		{
+			__syncthreads();
+			epilogue.template end<128, WAVES>(state, group, stage, tile_m, tile_n);
+		}
+	}
+	constexpr int PRODUCT_LDS_256 = PANEL * 260 * 4 > 8 * PANEL_BYTES ? PANEL * 260 * 4 : 8 * PANEL_BYTES;
+	constexpr int PRODUCT_LDS_128 = PANEL * 132 * 4 > 4 * PANEL_BYTES ? PANEL * 132 * 4 : 4 * PANEL_BYTES;
+
+	/* how a product is cut: tiles of `tile` rows and columns, `parts` along k. A workspace is sized by the same rule, so it asks no device */
+	struct ProductPlan
+	{
+			int tile, tiles_m, tiles_n, chunks, parts, chunks_per_part;
+	};
+	/* columns: of the result (of one of the two matrices where the operand is paired) */
+	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split)
+	{
+		constexpr int UNITS = 256;
+		ProductPlan plan;
+		const auto tiles = [&](int tile)
+		{
+			plan.tile = tile;
+			plan.tiles_m = ceil_div(rows, tile);
+			plan.tiles_n = ceil_div(columns, paired ? tile / 2 : tile);
+			return static_cast<long long>(plan.tiles_m) * plan.tiles_n;
+		};
+		plan.chunks = ceil_div(depth, 128 / element_size);
+		long long count = tiles(256);
+		if (count < 3 * UNITS / 4)
+			count = tiles(128);
+		plan.parts = 1;
+		if (may_split && count < UNITS && count > 0)
+			plan.parts = static_cast<int>(std::max<long long>(1, std::min<long long>(UNITS * 2 / count, plan.chunks / 8)));
+		plan.chunks_per_part = std::max(1, ceil_div(plan.chunks, plan.parts));
+		plan.parts = std::max(1, ceil_div(plan.chunks, plan.chunks_per_part));
+		return plan;
+	}
+	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
+	inline void launch_product(hipStream_t stream, const ProductPlan &plan, const Operand &a, const Operand &b, int rows, const Epilogue &epilogue)
+	{
+		if (plan.tiles_m == 0 || plan.tiles_n == 0)
+			return;
+		const ProductArgs args { a, b, rows, plan.tiles_m, plan.tiles_n, plan.chunks, plan.chunks_per_part };
+		const long long tiles = static_cast<long long>(plan.tiles_m) * plan.tiles_n;
+		MLHIP_REQUIRE(tiles <= 0x7fffffff && plan.parts <= 65535 && a.row_bytes < (1u << 22) && b.row_bytes < (1u << 22), "product too large");
+		const dim3 grid(static_cast<unsigned int>(tiles), plan.parts);
+		if (plan.tile == 256)
+		{
+			auto kernel = kernel_product_256<T, SA, SB, PAIRED, Epilogue>;
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), PRODUCT_LDS_256);
+			hipLaunchKernelGGL(kernel, grid, dim3(512), PRODUCT_LDS_256, stream, args, epilogue);
+		}
+		else
+		{
+			auto kernel = kernel_product_128<T, SA, SB, PAIRED, Epilogue>;
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), PRODUCT_LDS_128);
+			hipLaunchKernelGGL(kernel, grid, dim3(256), PRODUCT_LDS_128, stream, args, epilogue);
+		}
+		MLHIP_CHECK(hipGetLastError());
+	}
+
+	/* out[m][n] = scale * sum + beta * out[m][n] */
+	template<typename Out>
+	struct StoreEpilogue
+	{
+			static constexpr int SHARE = 8;
+			static constexpr bool HAS_END = false;
+			struct State
+			{
+					float scale;
+			};
+			Out *out;
+			int columns;
+			float beta;
+			const float *scale; /* on the device; null: 1 */
+
+			template<int BN>
+			__device__ __forceinline__ void begin(State &state, int, int) const
+			{
+				state.scale = scale != nullptr ? *scale : 1.0f;
+			}
+			template<int BN>
+			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
+			{
+				const int n = tile_n * BN + group * 8;
+				if (n >= columns)
+					return;
+				float v[8];
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					v[e] = row[group * 8 + e] * state.scale;
+				Out *dst = out + static_cast<size_t>(m) * columns + n;
+				if (n + 8 <= columns)
+				{
+					if (beta != 0.0f)
+					{
+						Elements<Out, 8> old;
+						old.load(dst);
+#pragma unroll
+						for (int e = 0; e < 8; e++)
+							v[e] = fmaf(beta, old[e], v[e]);
+					}
+					store_nearest<8>(dst, v);
+				}
+				else
+					for (int e = 0; e < columns - n; e++)
+						dst[e] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(dst[e]), v[e]) : v[e]);
+			}
+	};
+	/* partial[part][m][n] = sum, or += sum: [parts][rows][columns] in fp32 */
+	struct PartEpilogue
+	{
+			static constexpr int SHARE = 8;
+			static constexpr bool HAS_END = false;
+			struct State
+			{
+			};
+			float *partial;
+			size_t part_stride;
+			int columns;
+			bool add;
+
+			template<int BN>
+			__device__ __forceinline__ void begin(State&, int, int) const
+			{
+			}
+			template<int BN>
+			__device__ __forceinline__ void apply(State&, int m, int group, const float *row, int tile_n, int part) const
+			{
+				const int n = tile_n * BN + group * 8;
+				float *dst = partial + part * part_stride + static_cast<size_t>(m) * columns + n;
+				if (n + 8 <= columns)
+				{
+					float v[8];
+#pragma unroll
+					for (int e = 0; e < 8; e++)
+						v[e] = row[group * 8 + e];
+					if (add)
+					{
+						Elements<float, 8> old;
+						old.load(dst);
+#pragma unroll
+						for (int e = 0; e < 8; e++)
+							v[e] += old[e];
+					}
+					store_nearest<8>(dst, v);
+				}
+				else
+					for (int e = 0; e < columns - n; e++)
+						dst[e] = add ? dst[e] + row[group * 8 + e] : row[group * 8 + e];
+			}
+	};
+	/* out = scale * (sum of the parts) + beta * out, parts in order */
+	template<typename Out>
+	__global__ __launch_bounds__(256) void kernel_join_parts(const float *partial, int parts, size_t count, Out *out, float beta, const float *scale)
+	{
+		const float factor = scale != nullptr ? *scale : 1.0f;
+		for (size_t i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < count; i += static_cast<size_t>(gridDim.x) * 1024)
+		{
+			const size_t at = (count >= 4 && i + 4 > count) ? count - 4 : i;
+			const int skip = static_cast<int>(i - at);
+			if (count >= 4)
+			{
+				float v[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+				for (int p = 0; p < parts; p++)
+				{
+					Elements<float, 4> x;
+					x.load(partial + p * count + at);
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						v[e] += x[e];
+				}
+				Elements<Out, 4> old;
+				if (beta != 0.0f)
+					old.load(out + at);
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					v[e] = beta != 0.0f ? fmaf(beta, old[e], v[e] * factor) : v[e] * factor;
+				store_nearest<4>(out + at, v, skip);
+			}
+			else
+				for (size_t j = i; j < count; j++)
+				{
+					float v = 0.0f;
+					for (int p = 0; p < parts; p++)
+						v += partial[p * count + j];
+					v *= factor;
+					out[j] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(out[j]), v) : v);
+				}
+		}
+	}
+	template<typename Out>
+	inline void launch_join_parts(hipStream_t stream, const float *partial, int parts, size_t count, Out *out, float beta, const float *scale)
+	{
+		const size_t groups = std::min<size_t>((count + 1023) / 1024, 4096);
+		if (groups > 0)
+			hipLaunchKernelGGL((kernel_join_parts<Out>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, partial, parts, count, out, beta, scale);
+		MLHIP_CHECK(hipGetLastError());
+	}
+	/*
+	 * out [rows][columns] = scale * A B + beta * out, split along k where the tiles alone would not fill the chip; `partial` holds parts * rows * columns floats then
+	 */
+	template<typename T, typename Out, Side SA, Side SB>
+	inline void product_to(hipStream_t stream, const ProductPlan &plan, const Operand &a, const Operand &b, int rows, int columns, Out *out, float beta, const float *scale, float *partial)
+	{
+		if (plan.parts == 1)
+			launch_product<T, SA, SB, false>(stream, plan, a, b, rows, StoreEpilogue<Out> { out, columns, beta, scale });
+		else
+		{
+			const size_t count = static_cast<size_t>(rows) * columns;
+			launch_product<T, SA, SB, false>(stream, plan, a, b, rows, PartEpilogue { partial, count, columns, false });
+			launch_join_parts(stream, partial, plan.parts, count, out, beta, scale);
+		}
+	}
+	inline size_t part_bytes(const ProductPlan &plan, int rows, int columns)
+	{
+		return plan.parts > 1 ? sizeof(float) * plan.parts * static_cast<size_t>(rows) * columns : 0;
+	}
+
+	/* rows of `columns` elements copied to rows that are whole 16-byte pieces, zeros behind the last element: what the panels' loads ask of an operand whose rows end anywhere */
+	template<typename T>
+	__global__ __launch_bounds__(256) void kernel_pad_rows(const T *src, T *dst, size_t rows, int columns, int padded)
+	{
+		const size_t count = rows * padded;
+		for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<size_t>(gridDim.x) * 256)
+		{
+			int column;
+			const size_t row = split_index(i, padded, column);
+			dst[i] = column < columns ? src[row * columns + column] : static_cast<T>(0.0f);
+		}
+	}
+	template<typename T>
+	inline int padded_columns(int columns)
+	{
+		return static_cast<int>(round_up(columns, 16 / sizeof(T)));
+	}
+	template<typename T>
+	inline const T* pad_rows(hipStream_t stream, const T *src, T *space, size_t rows, int columns)
+	{
+		const int padded = padded_columns<T>(columns);
+		if (padded == columns)
+			return src;
+		const size_t groups = std::min<size_t>((rows * padded + 255) / 256, 16384);
+		hipLaunchKernelGGL((kernel_pad_rows<T>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, src, space, rows, columns, padded);
+		MLHIP_CHECK(hipGetLastError());
+		return space;
+	}
+} /* namespace mlhip */
+
+#endif /* MINML_AMD_PRODUCT_TILES_HPP_ */

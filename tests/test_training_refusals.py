@@ -55,3 +55,55 @@ def test_layer_norm_refusals_of_the_mirror():
                  lambda: ml.layerNormBackward(Ctx, x, w, x, 0.0, x, 0.0, f, f, None)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_gated_dense_refusals_of_the_library():
+    x, w, b, y, p = (fake(s).desc() for s in ((4, 16), (2, 24, 16), (2, 24), (4, 24), (4, 2, 24)))
+    size = lambda backward: B.fn("gated_dense_get_workspace_size")(fake((4, 16)).shape_desc(), fake((2, 24, 16)).shape_desc(), B.DTYPE_FLOAT16, backward)
+    assert size(True) > 4 * 48 * 2
+    forward = lambda x=x, w=w, b=b, y=y, p=p, gate=B.GATE_SILU, space=0x7000, n=1 << 30: refused("gated_dense_forward", x, w, b, y, p, gate, space, n)
+    forward(x=fake((4, 15)).desc())
+    forward(x=fake((4, 16), "int8").desc())
+    forward(w=fake((3, 24, 16)).desc())
+    forward(w=fake((48, 16)).desc())
+    forward(w=fake((2, 24, 16), "float32").desc())
+    forward(b=fake((24,)).desc())
+    forward(y=fake((4, 25)).desc())
+    forward(y=fake((3, 24)).desc())
+    forward(p=fake((4, 24, 2)).desc())
+    forward(gate=4)
+    forward(gate=-1)
+    forward(x=ml.Tensor((4, 16), "float16", _ptr=0x7008).desc())
+    forward(w=ml.Tensor((2, 24, 16), "float16", _ptr=0x7002).desc())
+    forward()  # all is well but the context
+    odd = dict(x=fake((100, 15)).desc(), w=fake((2, 24, 15)).desc(), y=fake((100, 24)).desc(), p=NULL)  # rows that end between pieces need room
+    forward(**odd, space=None, n=0)
+    forward(**odd, n=100)
+    dx, dw, db = (fake(s).desc() for s in ((4, 16), (2, 24, 16), (2, 24)))
+    backward = lambda x=x, w=w, p=p, dy=y, dx=dx, dw=dw, db=db, space=0x7000, n=1 << 30: refused("gated_dense_backward", x, w, p, dy, 0.0, dx, 0.0, dw, db, B.GATE_SILU, space, n)
+    backward(dy=fake((4, 16)).desc())
+    backward(p=NULL)
+    backward(p=fake((4, 2, 12)).desc())
+    backward(dx=fake((4, 17)).desc())
+    backward(dx=fake((4, 16), "float32").desc())
+    backward(dw=fake((2, 24, 15)).desc())
+    backward(dw=fake((2, 24, 16), "int32").desc())
+    backward(db=fake((24,)).desc())
+    backward(space=None)
+    backward(space=0x7010)
+    backward(n=size(True) - 1)
+    backward()  # all is well but the context
+
+
+def test_gated_dense_refusals_of_the_mirror():
+    class Ctx:
+        handle = None
+
+    x, w, b, y, p = (fake(s) for s in ((4, 16), (2, 24, 16), (2, 24), (4, 24), (4, 2, 24)))
+    for call in (lambda: ml.gatedDenseForward(Ctx, x, w, b, y, p, "swish", None), lambda: ml.gatedDenseForward(Ctx, x, fake((2, 24, 8)), b, y, p, "silu", None),
+                 lambda: ml.gatedDenseForward(Ctx, x, w, b, fake((4, 8)), p, "silu", None), lambda: ml.gatedDenseForward(Ctx, x, w, fake((24,)), y, p, "silu", None),
+                 lambda: ml.gatedDenseForward(Ctx, x, w, b, y, y, "silu", None), lambda: ml.gatedDenseBackward(Ctx, x, w, p, x, 0.0, x, 0.0, w, b, "silu", None),
+                 lambda: ml.gatedDenseBackward(Ctx, x, w, p, y, 0.0, y, 0.0, w, b, "silu", None), lambda: ml.gatedDenseBackward(Ctx, x, w, p, y, 0.0, x, 0.0, b, b, "silu", None),
+                 lambda: ml.gatedDenseBackward(Ctx, x, w, p, y, 0.0, x, 0.0, w, w, "silu", None)):
+        with pytest.raises(ValueError):
+            call()

@@ -70,8 +70,68 @@ def layer_norm_gradient_bounds(x, w, dy, epsilon, dtype):
     return rounded(dx, dtype) + dx_off, rounded(dw, dtype) + adds * np.abs(dy * n).sum(0) + (np.abs(dy) * off).sum(0), rounded(db, dtype) + adds * np.abs(dy).sum(0)
 
 
+GATES = ("sigmoid", "relu", "silu", "gelu")
+# what the gates' functions may be off by, relative to 1 + |g| of their argument: a few steps of 2^-24, and in fp16 the hardware's exponential, whose argument is rounded too
+GATE_ERROR = {"float16": 2.0 ** -19, "float32": 2.0 ** -21}
+
+
+def gate(g, name):
+    """a(g) and its derivative."""
+    if name == "relu":
+        return np.maximum(g, 0), (g > 0).astype(float)
+    if name == "gelu":
+        p = 0.5 * (1 + erf(g / math.sqrt(2)))
+        return g * p, p + g * np.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    s = expit(g)
+    return (s, s * (1 - s)) if name == "sigmoid" else (g * s, s * (1 + g * (1 - s)))
+
+
+def product_error(a, b, dtype):
+    """How far a @ b may be off when it is summed in 32 bits: an instruction adds 16 (fp16) or 2 (fp32) products to a sum, its own additions and the sum's may be cut off instead of rounded
+    (2^-23 each); at most 16 of them inside, 8 where partial sums meet."""
+    steps = a.shape[-1] / (16 if dtype == "float16" else 2) + 24
+    return steps * 2 * FP32 * (np.abs(a) @ np.abs(b))
+
+
+def gated(x, w, b, name):
+    """y and the projections [rows, 2, hidden]."""
+    p = np.stack((x @ w[0].T + b[0], x @ w[1].T + b[1]), 1)
+    return gate(p[:, 0], name)[0] * p[:, 1], p
+
+
+def gated_bounds(x, w, b, name, dtype):
+    y, p = gated(x, w, b, name)
+    off = np.stack((product_error(x, w[0].T, dtype), product_error(x, w[1].T, dtype)), 1) + FP32 * np.abs(p)
+    a = gate(p[:, 0], name)[0]
+    off_a = 1.2 * off[:, 0] + GATE_ERROR[dtype] * (1 + np.abs(p[:, 0]))  # no gate is steeper than 1.13
+    return rounded(y, dtype) + off_a * (np.abs(p[:, 1]) + off[:, 1]) + np.abs(a) * off[:, 1] + FP32 * np.abs(y), rounded(p, dtype) + off
+
+
+def gated_gradients(x, w, p, dy, name):
+    a, slope = gate(p[:, 0], name)
+    d = np.concatenate((dy * p[:, 1] * slope, dy * a), 1)
+    return d @ w.reshape(-1, w.shape[2]), (d.T @ x).reshape(w.shape), d.sum(0).reshape(2, -1)
+
+
+def gated_gradient_bounds(x, w, p, dy, name, dtype):
+    a, slope = gate(p[:, 0], name)
+    d = np.concatenate((dy * p[:, 1] * slope, dy * a), 1)
+    off = np.concatenate((np.abs(dy * p[:, 1]) * (1 + np.abs(p[:, 0])), np.abs(dy) * (1 + np.abs(p[:, 0]))), 1) * 2 * GATE_ERROR[dtype] + 2 * FP32 * np.abs(d)
+    stored = off + rounded(d, dtype)  # d goes to memory in the tensors' type
+    dx, dw, db = gated_gradients(x, w, p, dy, name)
+    flat = w.reshape(-1, w.shape[2])
+    return (rounded(dx, dtype) + product_error(d, flat, dtype) + stored @ np.abs(flat),
+            rounded(dw, dtype) + (product_error(d.T, x, dtype) + stored.T @ np.abs(x)).reshape(w.shape),
+            rounded(db, dtype) + (off.sum(0) + (x.shape[0] + 80) * FP32 * np.abs(d).sum(0)).reshape(2, -1))
+
+
 def worst(got, want, bound):
-    """The largest error in units of its bound, and where; places that are not finite have to be the same."""
+    """The largest error in units of its bound; places that are not finite have to be the same. What rounds to more than fp16's largest value, 65504, is an infinity there: from half a step beyond, 65520,
+    on; within the bound of that place either is right."""
+    if np.asarray(got).dtype == np.uint16:
+        over, near = np.abs(want) >= 65520, np.abs(np.abs(want) - 65520) <= bound
+        want = np.where(over, np.copysign(np.inf, want), want)
+        want = np.where(near & np.isinf(numbers(got)), numbers(got), want)
     got, want, bound = np.broadcast_arrays(numbers(got), want, bound)
     if not want.size:
         return 0.0
