@@ -259,6 +259,19 @@ extern "C"
 	void hip_gated_dense_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t projections, const mlTensor_t dy, float beta_dx, mlTensor_t dx,
 			float beta_weights, mlTensor_t dw, mlTensor_t db, mlGate_t gate, void *workspace, size_t workspace_size);
 
+	/*
+	 * The softmax cross entropy of a last dense layer over many classes, from the layer's input: with z = x w^T + b, lse = log sum exp z and loss = lse - z[target], both fp32 [..]. x [.., features],
+	 * w [classes, features], b [classes] or empty, targets int32 [..]; a row whose target is none of 0 .. classes - 1 has loss 0 and no gradient (its lse is given all the same; its x has to be finite, since dw is a product
+	 * with zeros there). The logits are never in
+	 * memory: the backward pass makes them again, in pieces of the classes. Backward: dloss fp32 [..] (the gradient of every row's loss) -> dx, dw, db as above. x and w have to be aligned to 16
+	 * bytes, workspaces of these calls to 256.
+	 */
+	size_t hip_linear_cross_entropy_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, mlDataType_t dtype, bool backward); /* bytes; the backward pass's is enough for both */
+	void hip_linear_cross_entropy_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t targets, mlTensor_t loss, mlTensor_t lse,
+			void *workspace, size_t workspace_size);
+	void hip_linear_cross_entropy_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t targets, const mlTensor_t lse,
+			const mlTensor_t dloss, float beta_dx, mlTensor_t dx, float beta_weights, mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size);
+
 	/* ---- additions with no counterpart in the reference ABI ----
 	 * hip_quantized_conv_forward: the whole int8 convolution of reference src/layers/Conv2D.cpp:240-308 (int8 implicit GEMM with
 	 * zero-point padding, int32 accumulation, per-channel scale + bias, optional int8 residual, activation, requantisation)

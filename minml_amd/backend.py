@@ -119,6 +119,9 @@ SIGNATURES = {
     "gated_dense_get_workspace_size": (_sz, [_S, _S, _i, _b]),
     "gated_dense_forward": (None, [_vp, _T, _T, _T, _T, _T, _i, _vp, _sz]),
     "gated_dense_backward": (None, [_vp, _T, _T, _T, _T, _f, _T, _f, _T, _T, _i, _vp, _sz]),
+    "linear_cross_entropy_get_workspace_size": (_sz, [_S, _S, _i, _b]),
+    "linear_cross_entropy_forward": (None, [_vp, _T, _T, _T, _T, _T, _T, _vp, _sz]),
+    "linear_cross_entropy_backward": (None, [_vp, _T, _T, _T, _T, _T, _T, _f, _T, _f, _T, _T, _vp, _sz]),
     "get_stream": (_vp, [_vp]),
     "graph_begin_capture": (None, [_vp]),
     "graph_end_capture": (_vp, [_vp]),

@@ -800,6 +800,39 @@ def gatedDenseBackward(context, input, weights, projections, gradient, beta, gra
             _all(gradient_weights), _all(gradient_bias), gate, *_space(workspace))
 
 
+def _require_loss(input, weights, bias, targets, *fp32):
+    _require(input.dtype in _FLOATS and _same_dtype(input, weights, bias), "dtype mismatch")
+    _require(len(weights.shape) == 2 and len(input.shape) >= 1 and weights.shape[1] == input.shape[-1], "weights must be [classes, features]")
+    _require(bias is None or bias.volume() == weights.shape[0], "bias must be [classes]")
+    lead = tuple(input.shape[:-1])
+    _require(targets.dtype == B.DTYPE_INT32 and tuple(targets.shape) == lead, "one int32 target per row")
+    for t in fp32:
+        _require(t.dtype == B.DTYPE_FLOAT32 and tuple(t.shape) == lead, "loss, lse and their gradient must be fp32 with one element per row")
+
+
+def linearCrossEntropyGetWorkspaceSize(context, input, weights, backward):
+    """Bytes of workspace (aligned to 256) that linearCrossEntropyForward or, with backward, either of the two needs."""
+    return B.fn("linear_cross_entropy_get_workspace_size")(input.shape_desc(), weights.shape_desc(), input.dtype, bool(backward))
+
+
+def linearCrossEntropyForward(context, input, weights, bias, targets, loss, lse, workspace):
+    """loss = lse - z[target] and lse = log sum exp z for z = input weights^T + bias, without keeping z: input [.., features], weights [classes, features], bias [classes] or None, targets int32
+    [..], loss and lse fp32 [..]. A row whose target is no class has loss 0."""
+    _require_loss(input, weights, bias, targets, loss, lse)
+    _launch("linear_cross_entropy_forward", context.handle, input.desc(), weights.desc(), _all(bias), targets.desc(), loss.desc(), lse.desc(), *_space(workspace))
+
+
+def linearCrossEntropyBackward(context, input, weights, bias, targets, lse, gradient_loss, beta, gradient_input, beta_weights, gradient_weights, gradient_bias, workspace):
+    """From the gradient of every row's loss (fp32 [..]) and the forward pass's lse: gradient_input = its share + beta * gradient_input; gradient_weights and gradient_bias likewise with
+    beta_weights, of the tensors' type or fp32. Each of the three may be None."""
+    _require_loss(input, weights, bias, targets, lse, gradient_loss)
+    _require(_same_dtype(input, gradient_input) and (gradient_input is None or tuple(gradient_input.shape) == tuple(input.shape)), "gradient of the input: shape or type")
+    _require_gradient(gradient_weights, weights.volume(), input.dtype, "gradient of the weights")
+    _require_gradient(gradient_bias, weights.shape[0], input.dtype, "gradient of the bias")
+    _launch("linear_cross_entropy_backward", context.handle, input.desc(), weights.desc(), _all(bias), targets.desc(), lse.desc(), gradient_loss.desc(), beta, _all(gradient_input),
+            beta_weights, _all(gradient_weights), _all(gradient_bias), *_space(workspace))
+
+
 def foldBatchnorm(context, layer_weights, layer_bias, bn_weights, bn_bias, bn_avg_var):
     """Folds a batch normalisation into the preceding layer's weights and bias, in place (reference: src/core/math.cpp:786-802, which
     also synchronises with the context afterwards)."""

@@ -1,0 +1,555 @@
+/*
+ * cross_entropy.hip — the softmax cross entropy of the rows of a last dense layer over many classes (a vocabulary), from the layer's input, and its gradients. The logits are never kept.
+ *
+ *   z = x W^T + b,   lse[i] = log sum_j exp z[i, j],   loss[i] = lse[i] - z[i, target[i]]        rows whose target is no class: loss 0, no gradient
+ *   d[i, j] = (exp(z[i, j] - lse[i]) - [j = target[i]]) dloss[i]
+ *   dx = d W,   dW = d^T x,   db[j] = sum_i d[i, j]
+ *
+ * Forward: a tile's logits stay in the accumulators; every row of the tile leaves its largest logit and the sum of exponentials about it, and a second launch joins these pairs. Up to 64 rows the
+ * weights stream through registers instead (few_rows.hpp) and memory bounds it; above, the matrix cores do.
+ * Backward: the classes are taken in pieces of as many as make d 256 MB (so it stays in the last-level cache between its makers and users, and the workspace small whatever the vocabulary). For each
+ * piece the logits are made again, which costs a quarter of the operations and spares rows x classes of memory; the epilogue turns them into d; then d is multiplied with the piece's weights, added to
+ * dx in fp32, and with x, which gives the piece's rows of dW.
+ * d is stored in the tensors' type. In fp16 a probability of one class in 100 000 would be subnormal, and the rows' dloss may be anything, so d is scaled by 2^15 / s with s the power of two above the
+ * largest |dloss|: the largest d is 2^15 then, and probabilities down to 2e-9 keep their 11 bits. The products' results are scaled back, exactly, in fp32. Its rounding, half a step per element, averages
+ * out in the sums; db is summed before it.
+ */
+#include "few_rows.hpp"
+#include "product_tiles.hpp"
+
+#include <limits>
+
+namespace
+{
+	using namespace mlhip;
+
+	/* of one row and some classes: the largest logit and the sum of exp(z - largest). Nothing there: (-inf, 0) */
+	struct Partial
+	{
+			float top, sum;
+	};
+	__device__ __forceinline__ float exp_about(float z, float top)
+	{
+		/* infinities: exp(inf - inf) is 1 here, so that a row with a logit of +inf has lse = +inf, and one of -inf alone -inf */
+		return z == top ? 1.0f : __expf(z - top);
+	}
+	/* NaN passes: the sum becomes NaN */
+	__device__ __forceinline__ Partial join(const Partial &a, const Partial &b)
+	{
+		const float top = fmaxf(a.top, b.top);
+		const float from_a = (a.sum == 0.0f) ? 0.0f : a.sum * exp_about(a.top, top);
+		const float from_b = (b.sum == 0.0f) ? 0.0f : b.sum * exp_about(b.top, top);
+		return Partial { top, from_a + from_b };
+	}
+	template<int N>
+	__device__ __forceinline__ Partial partial_of(const float (&z)[N], const bool (&there)[N])
+	{
+		float top = -std::numeric_limits<float>::infinity();
+#pragma unroll
+		for (int e = 0; e < N; e++)
+			top = there[e] ? fmaxf(top, z[e]) : top;
+		float sum = 0.0f;
+#pragma unroll
+		for (int e = 0; e < N; e++)
+			sum += (there[e] && !(z[e] == -std::numeric_limits<float>::infinity())) ? exp_about(z[e], top) : 0.0f;
+		return Partial { top, sum };
+	}
+	template<int LANES>
+	__device__ __forceinline__ Partial lanes_join(Partial p)
+	{
+#pragma unroll
+		for (int offset = LANES / 2; offset >= 1; offset >>= 1)
+			p = join(p, Partial { __shfl_xor(p.top, offset), __shfl_xor(p.sum, offset) });
+		return p;
+	}
+
+	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
+	template<typename T>
+	struct LossEpilogue
+	{
+			static constexpr int SHARE = 8;
+			static constexpr bool HAS_END = false;
+			struct State
+			{
+					float bias[8];
+			};
+			const T *bias;
+			const int *targets;
+			Partial *partials; /* [rows][column tiles] */
+			float *target_logits;
+			int classes, tiles_n;
+
+			template<int BN>
+			__device__ __forceinline__ void begin(State &state, int group, int tile_n) const
+			{
+				const int n = tile_n * BN + group * 8;
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					state.bias[e] = (bias != nullptr && n + e < classes) ? static_cast<float>(bias[n + e]) : 0.0f;
+			}
+			template<int BN>
+			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
+			{
+				const int n = tile_n * BN + group * 8, target = targets[m];
+				float z[8];
+				bool there[8];
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+				{
+					z[e] = row[group * 8 + e] + state.bias[e];
+					there[e] = n + e < classes;
+					if (there[e] && n + e == target)
+						target_logits[m] = z[e];
+				}
+				const Partial p = lanes_join<BN / 8>(partial_of(z, there));
+				if (group == 0)
+					partials[static_cast<size_t>(m) * tiles_n + tile_n] = p;
+			}
+	};
+	constexpr int FEW_CLASSES = 32; /* of a workgroup of the few-rows kernel */
+	template<typename T, int MB>
+	__global__ __launch_bounds__(256) void kernel_loss_few_rows(const T *x, const T *w, const T *bias, const int *targets, int rows, int features, int classes, Partial *partials,
+			float *target_logits)
+	{
+		__shared__ __attribute__((aligned(16))) float sums[2][16 * MB][16];
+		const int n0 = blockIdx.x * FEW_CLASSES;
+		const T *first = w + static_cast<size_t>(n0) * features;
+		const bool second = n0 + 16 < classes; /* else the first block stands in for it */
+		few_rows_sums<T, MB>(x, rows, first, second ? first + static_cast<size_t>(16) * features : first, min(15, classes - 1 - n0), min(15, classes - 1 - n0 - (second ? 16 : 0)), features, sums);
+		const int c = threadIdx.x & 15;
+		for (int row = threadIdx.x >> 4; row < 16 * MB; row += 16)
+			if (row < rows)
+			{
+				const int target = targets[row];
+				float z[2];
+				bool there[2];
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+				{
+					const int n = n0 + 16 * i + c;
+					there[i] = n < classes;
+					z[i] = sums[i][row][c] + ((bias != nullptr && there[i]) ? static_cast<float>(bias[n]) : 0.0f);
+					if (there[i] && n == target)
+						target_logits[row] = z[i];
+				}
+				const Partial p = lanes_join<16>(partial_of(z, there));
+				if (c == 0)
+					partials[static_cast<size_t>(row) * gridDim.x + blockIdx.x] = p;
+			}
+	}
+	/* one wavefront per row */
+	__global__ __launch_bounds__(256) void kernel_join_partials(const Partial *partials, int count, const int *targets, const float *target_logits, int rows, int classes, float *loss, float *lse)
+	{
+		const int lane = threadIdx.x & 63;
+		const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+		if (row >= rows)
+			return;
+		Partial p { -std::numeric_limits<float>::infinity(), 0.0f };
+		const Partial *src = partials + static_cast<size_t>(row) * count;
+		for (int i = lane; i < count; i += 64)
+			p = join(p, src[i]);
+		p = lanes_join<64>(p);
+		if (lane == 0)
+		{
+			const float value = p.top + logf(p.sum);
+			const int target = targets[row];
+			lse[row] = value;
+			loss[row] = (target >= 0 && target < classes) ? value - target_logits[row] : 0.0f;
+		}
+	}
+
+	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
+	constexpr int SCALE_GROUPS = 256;
+	constexpr int SCALE_BITS = 15;
+	__global__ __launch_bounds__(256) void kernel_largest_gradient(const float *dloss, const int *targets, int rows, int classes, float *largest)
+	{
+		__shared__ float waves[4];
+		float top = 0.0f;
+		for (int i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256)
+		{
+			const float v = fabsf(dloss[i]);
+			if (targets[i] >= 0 && targets[i] < classes && v <= std::numeric_limits<float>::max())
+				top = fmaxf(top, v);
+		}
+#pragma unroll
+		for (int offset = 32; offset >= 1; offset >>= 1)
+			top = fmaxf(top, __shfl_xor(top, offset));
+		if ((threadIdx.x & 63) == 0)
+			waves[threadIdx.x >> 6] = top;
+		__syncthreads();
+		if (threadIdx.x == 0)
+			largest[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+	}
+	/* factors[i] = dloss[i] 2^15 / s, 0 for rows without a class; back = s / 2^15 */
+	__global__ __launch_bounds__(256) void kernel_row_factors(const float *dloss, const int *targets, int rows, int classes, const float *largest, int groups, float *factors, float *back)
+	{
+		float top = 0.0f;
+		for (int i = threadIdx.x & 63; i < groups; i += 64)
+			top = fmaxf(top, largest[i]);
+#pragma unroll
+		for (int offset = 32; offset >= 1; offset >>= 1)
+			top = fmaxf(top, __shfl_xor(top, offset));
+		int exponent = 0;
+		if (top > 0.0f)
+			(void) frexpf(top, &exponent); /* top < 2^exponent */
+		exponent = max(exponent, -100); /* so that the way back is a normal number */
+		for (int i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256)
+			factors[i] = (targets[i] >= 0 && targets[i] < classes) ? ldexpf(dloss[i], SCALE_BITS - exponent) : 0.0f;
+		if (blockIdx.x == 0 && threadIdx.x == 0)
+			*back = ldexpf(1.0f, exponent - SCALE_BITS);
+	}
+	template<typename T>
+	struct GradientEpilogue
+	{
+			static constexpr int SHARE = 8;
+			static constexpr bool HAS_END = true;
+			struct State
+			{
+					float bias[8], sum[8];
+			};
+			const T *bias; /* of the piece */
+			const int *targets;
+			const float *lse, *factors;
+			T *d; /* [rows][row_elements], zeros behind the piece's classes */
+			float *sums; /* [row tiles][classes of the piece], or null */
+			int first_class, classes, row_elements; /* classes: of the piece */
+
+			template<int BN>
+			__device__ __forceinline__ void begin(State &state, int group, int tile_n) const
+			{
+				const int n = tile_n * BN + group * 8;
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+				{
+					state.bias[e] = (bias != nullptr && n + e < classes) ? static_cast<float>(bias[n + e]) : 0.0f;
+					state.sum[e] = 0.0f;
+				}
+			}
+			template<int BN>
+			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
+			{
+				const int n = tile_n * BN + group * 8, target = targets[m] - first_class;
+				const float norm = lse[m], factor = factors[m];
+				float v[8];
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+				{
+					const float about = row[group * 8 + e] + state.bias[e] - norm;
+					const float p = (sizeof(T) == 2) ? __expf(about) : expf(about); /* the hardware's is 2^-20 off, which fp16 rounds away */
+					/* a row without gradient has none, whatever its logits are */
+					v[e] = (factor == 0.0f || n + e >= classes) ? 0.0f : (p - (n + e == target ? 1.0f : 0.0f)) * factor;
+					state.sum[e] += v[e];
+				}
+				T *dst = d + static_cast<size_t>(m) * row_elements + n;
+				if (n + 8 <= row_elements)
+					store_nearest<8>(dst, v);
+				else
+					for (int e = 0; e < row_elements - n; e++)
+						dst[e] = static_cast<T>(v[e]);
+			}
+			template<int BN, int WAVES>
+			__device__ __forceinline__ void end(State &state, int group, float *stage, int tile_m, int tile_n) const
+			{
+				if (sums == nullptr)
+					return;
+				constexpr int GROUPS = BN / SHARE, LINES = WAVES * 64 / GROUPS;
+				const int line = threadIdx.x / GROUPS;
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					stage[line * BN + group * 8 + e] = state.sum[e];
+				__syncthreads();
+				const int n = tile_n * BN + static_cast<int>(threadIdx.x);
+				if (static_cast<int>(threadIdx.x) < BN && n < classes)
+				{
+					float total = 0.0f;
+					for (int l = 0; l < LINES; l++)
+						total += stage[l * BN + threadIdx.x];
+					sums[static_cast<size_t>(tile_m) * classes + n] = total;
+				}
+			}
+	};
+
+	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
+	struct LossShape
+	{
+			int rows, features, classes, element_size;
+	};
+	LossShape loss_shape(const mlShape_t &x, const mlShape_t &w, mlDataType_t dtype, const char *name)
+	{
+		const std::string who(name);
+		MLHIP_REQUIRE(dtype == DTYPE_FLOAT16 || dtype == DTYPE_FLOAT32, who + ": unsupported data type");
+		MLHIP_REQUIRE(x.rank >= 1 && x.rank <= 6 && w.rank == 2, who + ": the input needs one to six dimensions, the weights must be [classes, features]");
+		for (int i = 0; i < x.rank; i++)
+			MLHIP_REQUIRE(x.dim[i] >= 0, who + ": negative dimension");
+		MLHIP_REQUIRE(w.dim[0] > 0 && w.dim[1] > 0 && w.dim[1] == last_dim(x), who + ": the weights' last dimension must be the input's, and there must be classes and features");
+		const size_t rows = volume(x) / w.dim[1];
+		MLHIP_REQUIRE(rows <= (1 << 28) && w.dim[0] <= (1 << 28) && w.dim[1] <= (1 << 18), who + ": too many rows, classes or features");
+		return LossShape { static_cast<int>(rows), w.dim[1], w.dim[0], size_of(dtype) };
+	}
+	constexpr size_t PIECE_BYTES = size_t(1) << 28;
+	/* classes of a piece: whole tiles, all pieces about the same */
+	int classes_of_piece(const LossShape &s)
+	{
+		const size_t most = std::max<size_t>(256, PIECE_BYTES / (static_cast<size_t>(std::max(s.rows, 1)) * s.element_size) / 256 * 256);
+		const size_t pieces = (s.classes + most - 1) / most;
+		return static_cast<int>(std::min<size_t>(round_up((s.classes + pieces - 1) / pieces, 256), s.classes));
+	}
+	ProductPlan logits_plan(const LossShape &s, int classes)
+	{
+		return plan_product(s.rows, classes, false, s.features, s.element_size, false);
+	}
+	ProductPlan input_plan(const LossShape &s, int classes)
+	{
+		return plan_product(s.rows, s.features, false, classes, s.element_size, true);
+	}
+	ProductPlan weights_plan(const LossShape &s, int classes)
+	{
+		return plan_product(classes, s.features, false, s.rows, s.element_size, true);
+	}
+	struct LossSpace
+	{
+			size_t x, w, partials, target_logits; /* forward */
+			size_t d, dx, parts, sums, factors, scale; /* backward */
+			size_t total;
+	};
+	LossSpace loss_space(const LossShape &s, bool backward)
+	{
+		LossSpace space { };
+		size_t at = 0;
+		const auto take = [&](size_t bytes)
+		{
+			const size_t begin = at;
+			at += round_up(bytes, 256);
+			return begin;
+		};
+		if (s.rows > 0)
+		{
+			const int pieces = 16 / s.element_size;
+			const size_t padded = (s.features % pieces == 0) ? 0 : round_up(s.features, pieces) * s.element_size;
+			const bool few = s.rows <= MOST_FEW_ROWS;
+			/* the forward pass's pieces lie in the same places as far as both have them: one workspace serves both */
+			space.x = take(backward || !few ? padded * s.rows : 0);
+			space.w = take(backward || !few ? padded * s.classes : 0);
+			const size_t begin = at;
+			const size_t columns = few ? ceil_div(s.classes, FEW_CLASSES) : logits_plan(s, s.classes).tiles_n;
+			space.partials = take(sizeof(Partial) * columns * s.rows);
+			space.target_logits = take(sizeof(float) * s.rows);
+			if (backward)
+			{
+				const size_t forward_end = at;
+				at = begin;
+				const int classes = classes_of_piece(s);
+				const ProductPlan input = input_plan(s, classes), weights = weights_plan(s, classes);
+				space.d = take(round_up(classes, pieces) * s.element_size * s.rows);
+				space.dx = take((classes < s.classes || input.parts > 1) ? sizeof(float) * input.parts * s.rows * s.features : 0);
+				space.parts = take(part_bytes(weights, classes, s.features));
+				space.sums = take(sizeof(float) * classes * logits_plan(s, classes).tiles_m);
+				space.factors = take(sizeof(float) * s.rows);
+				space.scale = take(sizeof(float) * (SCALE_GROUPS + 1));
+				at = std::max(at, forward_end);
+			}
+		}
+		space.total = at;
+		return space;
+	}
+
+	template<typename T>
+	void loss_forward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const int *targets, float *loss, float *lse, uint8_t *workspace)
+	{
+		const LossSpace space = loss_space(s, false);
+		Partial *partials = reinterpret_cast<Partial*>(workspace + space.partials);
+		float *target_logits = reinterpret_cast<float*>(workspace + space.target_logits);
+		int columns;
+		if (s.rows <= MOST_FEW_ROWS)
+		{
+			columns = ceil_div(s.classes, FEW_CLASSES);
+			const auto launch = [&](auto kernel)
+			{
+				hipLaunchKernelGGL(kernel, dim3(columns), dim3(256), 0, stream, x, w, bias, targets, s.rows, s.features, s.classes, partials, target_logits);
+			};
+			if (s.rows <= 16)
+				launch(kernel_loss_few_rows<T, 1>);
+			else if (s.rows <= 32)
+				launch(kernel_loss_few_rows<T, 2>);
+			else
+				launch(kernel_loss_few_rows<T, 4>);
+		}
+		else
+		{
+			const int padded = padded_columns<T>(s.features);
+			x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
+			w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
+			const ProductPlan plan = logits_plan(s, s.classes);
+			columns = plan.tiles_n;
+			const Operand a { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), s.rows, padded };
+			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), s.classes, padded };
+			launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, LossEpilogue<T> { bias, targets, partials, target_logits, s.classes, columns });
+		}
+		MLHIP_CHECK(hipGetLastError());
+		hipLaunchKernelGGL(kernel_join_partials, dim3(ceil_div(s.rows, 4)), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
+		MLHIP_CHECK(hipGetLastError());
+	}
+	template<typename T>
+	void loss_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const int *targets, const float *lse, const float *dloss, float beta_dx, T *dx,
+			float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, uint8_t *workspace)
+	{
+		const LossSpace space = loss_space(s, true);
+		const int padded = padded_columns<T>(s.features), most = classes_of_piece(s);
+		T *d = reinterpret_cast<T*>(workspace + space.d);
+		float *partial_dx = reinterpret_cast<float*>(workspace + space.dx), *parts = reinterpret_cast<float*>(workspace + space.parts);
+		float *sums = reinterpret_cast<float*>(workspace + space.sums), *factors = reinterpret_cast<float*>(workspace + space.factors);
+		float *largest = reinterpret_cast<float*>(workspace + space.scale), *back = largest + SCALE_GROUPS;
+		const int groups = std::min(ceil_div(s.rows, 256), SCALE_GROUPS);
+		hipLaunchKernelGGL(kernel_largest_gradient, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest);
+		hipLaunchKernelGGL(kernel_row_factors, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest, groups, factors, back);
+		MLHIP_CHECK(hipGetLastError());
+		x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
+		w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
+		const size_t row_bytes = padded * sizeof(T), outputs = static_cast<size_t>(s.rows) * s.features;
+		const ProductPlan whole_input = input_plan(s, most);
+		const bool dx_in_parts = most < s.classes || whole_input.parts > 1;
+		/* the last piece, which may be smaller, is cut by the plans of the others: the workspace is sized by them */
+		for (int first = 0; first < s.classes; first += most)
+		{
+			const int classes = std::min(most, s.classes - first), row_elements = padded_columns<T>(classes);
+			const uint8_t *weights = reinterpret_cast<const uint8_t*>(w) + first * row_bytes;
+			{
+				ProductPlan plan = logits_plan(s, most);
+				plan.tiles_n = ceil_div(classes, plan.tile);
+				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
+				const Operand b { weights, row_bytes, classes, padded };
+				launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T> { bias != nullptr ? bias + first : nullptr, targets, lse, factors, d,
+						db.data != nullptr ? sums : nullptr, first, classes, row_elements });
+				if (db.data != nullptr)
+					launch_sum_partials(stream, sums, plan.tiles_m, static_cast<size_t>(classes), static_cast<uint8_t*>(db.data) + static_cast<size_t>(first) * size_of(db.dtype), db.dtype, classes,
+							beta_weights, back);
+			}
+			if (dx != nullptr)
+			{
+				ProductPlan plan = whole_input; /* a part that has no chunk left adds nothing */
+				plan.chunks = ceil_div(classes, 128 / static_cast<int>(sizeof(T)));
+				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), s.rows, row_elements };
+				const Operand b { weights, row_bytes, padded, classes };
+				if (dx_in_parts)
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
+				else
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, StoreEpilogue<T> { dx, s.features, beta_dx, back });
+			}
+			if (dw.data != nullptr)
+			{
+				ProductPlan plan = weights_plan(s, most);
+				plan.tiles_m = ceil_div(classes, plan.tile);
+				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), row_elements, s.rows };
+				const Operand b { reinterpret_cast<const uint8_t*>(x), row_bytes, padded, s.rows };
+				const size_t offset = static_cast<size_t>(first) * s.features;
+				if (dw.dtype == DTYPE_FLOAT32)
+					product_to<T, float, Side::COLUMNS, Side::COLUMNS>(stream, plan, a, b, classes, s.features, ptr<float>(dw) + offset, beta_weights, back, parts);
+				else if constexpr (sizeof(T) == 2)
+					product_to<T, T, Side::COLUMNS, Side::COLUMNS>(stream, plan, a, b, classes, s.features, ptr<T>(dw) + offset, beta_weights, back, parts);
+			}
+		}
+		if (dx != nullptr && dx_in_parts)
+			launch_join_parts(stream, partial_dx, whole_input.parts, outputs, dx, beta_dx, back);
+	}
+
+	bool weight_type(const mlTensor_t &t, const mlTensor_t &x)
+	{
+		return t.dtype == x.dtype || t.dtype == DTYPE_FLOAT32;
+	}
+	bool per_row(const mlTensor_t &t, const LossShape &s, mlDataType_t dtype)
+	{
+		return t.dtype == dtype && volume(t) == static_cast<size_t>(s.rows) && (s.rows == 0 || (t.data != nullptr && reinterpret_cast<uintptr_t>(t.data) % 4 == 0));
+	}
+	LossShape check_loss(const mlTensor_t &x, const mlTensor_t &w, const mlTensor_t &b, const mlTensor_t &targets, const char *name)
+	{
+		const std::string who(name);
+		const LossShape s = loss_shape(shape_of(x), shape_of(w), x.dtype, name);
+		MLHIP_REQUIRE(w.dtype == x.dtype, who + ": weights must have the input's type");
+		MLHIP_REQUIRE(b.data == nullptr || (b.dtype == x.dtype && volume(b) == static_cast<size_t>(s.classes)), who + ": the bias must be [classes] of the input's type");
+		MLHIP_REQUIRE(per_row(targets, s, DTYPE_INT32), who + ": there must be one int32 target per row");
+		MLHIP_REQUIRE(s.rows == 0 || (x.data != nullptr && w.data != nullptr), who + ": null pointer");
+		MLHIP_REQUIRE(reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && reinterpret_cast<uintptr_t>(w.data) % 16 == 0, who + ": input and weights must be aligned to 16 bytes");
+		return s;
+	}
+	void check_space(const void *workspace, size_t given, size_t needed, const char *name)
+	{
+		MLHIP_REQUIRE(needed == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && given >= needed),
+				std::string(name) + ": the workspace is too small or not aligned to 256 bytes");
+	}
+}
+
+extern "C"
+{
+	using namespace mlhip;
+
+	size_t hip_linear_cross_entropy_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, mlDataType_t dtype, bool backward)
+	try
+	{
+		return loss_space(loss_shape(input_shape, weights_shape, dtype, "linear_cross_entropy_get_workspace_size"), backward).total;
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<size_t>();
+	}
+
+	void hip_linear_cross_entropy_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t targets, mlTensor_t loss, mlTensor_t lse,
+			void *workspace, size_t workspace_size)
+	try
+	{
+		const char *name = "linear_cross_entropy_forward";
+		const LossShape s = check_loss(x, w, b, targets, name);
+		MLHIP_REQUIRE(per_row(loss, s, DTYPE_FLOAT32) && per_row(lse, s, DTYPE_FLOAT32), "linear_cross_entropy_forward: loss and lse must be fp32 with one element per row");
+		if (s.rows == 0)
+			return;
+		check_space(workspace, workspace_size, loss_space(s, false).total, name);
+		const hipStream_t stream = stream_of(context);
+		if (x.dtype == DTYPE_FLOAT16)
+			loss_forward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), ptr<float>(loss), ptr<float>(lse), reinterpret_cast<uint8_t*>(workspace));
+		else
+			loss_forward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), ptr<float>(loss), ptr<float>(lse), reinterpret_cast<uint8_t*>(workspace));
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+
+	void hip_linear_cross_entropy_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t targets, const mlTensor_t lse, const mlTensor_t dloss,
+			float beta_dx, mlTensor_t dx, float beta_weights, mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size)
+	try
+	{
+		const char *name = "linear_cross_entropy_backward";
+		const LossShape s = check_loss(x, w, b, targets, name);
+		MLHIP_REQUIRE(per_row(lse, s, DTYPE_FLOAT32) && per_row(dloss, s, DTYPE_FLOAT32), "linear_cross_entropy_backward: lse and dloss must be fp32 with one element per row");
+		MLHIP_REQUIRE(dx.data == nullptr || (dx.dtype == x.dtype && volume(dx) == volume(x)), "linear_cross_entropy_backward: dx must have the input's shape and type");
+		MLHIP_REQUIRE(dw.data == nullptr || (weight_type(dw, x) && volume(dw) == volume(w)), "linear_cross_entropy_backward: dw must be [classes, features] of the input's type or fp32");
+		MLHIP_REQUIRE(db.data == nullptr || (weight_type(db, x) && volume(db) == static_cast<size_t>(s.classes)), "linear_cross_entropy_backward: db must be [classes] of the input's type or fp32");
+		if (dx.data == nullptr && dw.data == nullptr && db.data == nullptr)
+			return;
+		if (s.rows == 0)
+		{
+			/* sums over nothing */
+			const hipStream_t stream = stream_of(context);
+			for (const mlTensor_t &t : { dw, db })
+				if (t.data != nullptr)
+				{
+					if (t.dtype == DTYPE_FLOAT16)
+						launch_join_parts<half_t>(stream, nullptr, 0, volume(t), ptr<half_t>(t), beta_weights, nullptr);
+					else
+						launch_join_parts<float>(stream, nullptr, 0, volume(t), ptr<float>(t), beta_weights, nullptr);
+				}
+			return;
+		}
+		check_space(workspace, workspace_size, loss_space(s, true).total, name);
+		const hipStream_t stream = stream_of(context);
+		if (x.dtype == DTYPE_FLOAT16)
+			loss_backward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db,
+					reinterpret_cast<uint8_t*>(workspace));
+		else
+			loss_backward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db,
+					reinterpret_cast<uint8_t*>(workspace));
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+}

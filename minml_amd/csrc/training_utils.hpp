@@ -95,11 +95,11 @@ namespace mlhip
 	}
 
 	/*
-	 * out[j] = sum over `parts` rows of partial[.][stride] (column j) + beta * out[j]: the second half of every sum over rows. The first half leaves one row of sums per workgroup, here 8
+	 * out[j] = scale * (sum over `parts` rows of partial[.][stride], column j) + beta * out[j]: the second half of every sum over rows. The first half leaves one row of sums per workgroup, here 8
 	 * threads to a column add up every eighth of them and meet in LDS: a fixed order, so the same bits every time, which additions by atomic operations would not give.
 	 */
 	template<typename Out>
-	__global__ __launch_bounds__(256) void kernel_sum_partials(const float *partial, int parts, size_t stride, Out *out, int columns, float beta)
+	__global__ __launch_bounds__(256) void kernel_sum_partials(const float *partial, int parts, size_t stride, Out *out, int columns, float beta, const float *scale)
 	{
 		__shared__ float sums[8][33];
 		const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
@@ -129,19 +129,22 @@ namespace mlhip
 #pragma unroll
 			for (int g = 1; g < 8; g++)
 				sum += sums[g][c];
+			if (scale != nullptr)
+				sum *= *scale;
 			out[j] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(out[j]), sum) : sum);
 		}
 	}
-	/* the gradient of a weight: of the tensors' type, or fp32 */
-	inline void launch_sum_partials(hipStream_t stream, const float *partial, int parts, size_t stride, void *out, mlDataType_t dtype, int columns, float beta)
+	/* out: the gradient of a weight, of the tensors' type or fp32. scale: on the device, or null for 1 */
+	inline void launch_sum_partials(hipStream_t stream, const float *partial, int parts, size_t stride, void *out, mlDataType_t dtype, int columns, float beta,
+			const float *scale = nullptr)
 	{
 		if (columns == 0)
 			return;
 		const dim3 grid(ceil_div(columns, 32));
 		if (dtype == DTYPE_FLOAT16)
-			hipLaunchKernelGGL((kernel_sum_partials<half_t>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<half_t*>(out), columns, beta);
+			hipLaunchKernelGGL((kernel_sum_partials<half_t>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<half_t*>(out), columns, beta, scale);
 		else
-			hipLaunchKernelGGL((kernel_sum_partials<float>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<float*>(out), columns, beta);
+			hipLaunchKernelGGL((kernel_sum_partials<float>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<float*>(out), columns, beta, scale);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	inline size_t round_up(size_t n, size_t to)

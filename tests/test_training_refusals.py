@@ -107,3 +107,50 @@ def test_gated_dense_refusals_of_the_mirror():
                  lambda: ml.gatedDenseBackward(Ctx, x, w, p, y, 0.0, x, 0.0, w, w, "silu", None)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_cross_entropy_refusals_of_the_library():
+    x, w, b, t, f = fake((4, 16)).desc(), fake((90, 16)).desc(), fake((90,)).desc(), fake((4,), "int32").desc(), fake((4,), "float32").desc()
+    size = lambda backward: B.fn("linear_cross_entropy_get_workspace_size")(fake((4, 16)).shape_desc(), fake((90, 16)).shape_desc(), B.DTYPE_FLOAT16, backward)
+    assert size(True) >= size(False) > 0
+    forward = lambda x=x, w=w, b=b, t=t, loss=f, lse=f, space=0x7000, n=1 << 30: refused("linear_cross_entropy_forward", x, w, b, t, loss, lse, space, n)
+    forward(x=fake((4, 15)).desc())
+    forward(x=fake((4, 16), "int8").desc())
+    forward(w=fake((2, 90, 16)).desc())
+    forward(w=fake((0, 16)).desc())
+    forward(w=fake((90, 16), "float32").desc())
+    forward(b=fake((89,)).desc())
+    forward(t=fake((4,), "float32").desc())
+    forward(t=fake((3,), "int32").desc())
+    forward(t=NULL)
+    forward(loss=fake((4,)).desc())
+    forward(lse=fake((5,), "float32").desc())
+    forward(x=ml.Tensor((4, 16), "float16", _ptr=0x7008).desc())
+    forward(w=ml.Tensor((90, 16), "float16", _ptr=0x7002).desc())
+    forward(space=None)
+    forward(space=0x7080)
+    forward(n=size(False) - 1)
+    forward()  # all is well but the context
+    dx, dw, db = x, w, b
+    backward = lambda x=x, w=w, b=b, t=t, lse=f, dloss=f, dx=dx, dw=dw, db=db, space=0x7000, n=1 << 30: refused("linear_cross_entropy_backward", x, w, b, t, lse, dloss, 0.0, dx, 0.0, dw, db, space, n)
+    backward(lse=fake((4,)).desc())
+    backward(dloss=fake((4, 2), "float32").desc())
+    backward(dx=fake((4, 17)).desc())
+    backward(dx=fake((4, 16), "float32").desc())
+    backward(dw=fake((91, 16)).desc())
+    backward(dw=fake((90, 16), "int32").desc())
+    backward(db=fake((91,)).desc())
+    backward(n=size(True) - 1)
+    backward(space=None)
+    backward()
+    B.fn("linear_cross_entropy_backward")(None, x, w, b, t, f, f, 0.0, NULL, 0.0, NULL, NULL, None, 0)  # nothing asked for
+
+
+def test_cross_entropy_workspace_does_not_grow_with_the_vocabulary():
+    """256 MB of d at most, and what goes with it, whatever the number of classes; never the logits."""
+    for dtype, element in ((B.DTYPE_FLOAT16, 2), (B.DTYPE_FLOAT32, 4)):
+        for rows, features in ((1000, 64), (4096, 2048), (65536, 1024)):
+            sizes = [B.fn("linear_cross_entropy_get_workspace_size")(B.make_shape((rows, features)), B.make_shape((classes, features)), dtype, True) for classes in (200000, 2000000)]
+            # besides d: sums over rows, two floats a tile of logits and row, the fp32 sums of dx and of one piece of dw, each in parts of at most 512 tiles together
+            assert all(s <= (1 << 28) + rows * 20 + 8 * rows * classes / 128 + 2 * 4 * rows * features * 8 + (1 << 26) + 4 * 2000000 * (rows / 128 + 1) for s, classes in zip(sizes, (200000, 2000000)))
+            assert sizes[1] < rows * 2000000 * element / 2

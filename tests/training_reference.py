@@ -125,6 +125,60 @@ def gated_gradient_bounds(x, w, p, dy, name, dtype):
             rounded(db, dtype) + (off.sum(0) + (x.shape[0] + 80) * FP32 * np.abs(d).sum(0)).reshape(2, -1))
 
 
+def cross_entropy(x, w, b, targets):
+    """loss, lse and the logits; targets that are no class have loss 0."""
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        z = x @ w.T + b
+        top = z.max(1, keepdims=True)
+        lse = np.where(np.isfinite(top[:, 0]), top[:, 0] + np.log(np.exp(z - top).sum(1)), top[:, 0])
+        kept = (targets >= 0) & (targets < w.shape[0])
+        loss = np.where(kept, lse - z[np.arange(len(z)), np.where(kept, targets, 0)], 0.0)
+    return loss, lse, z
+
+
+def logit_error(x, w, z, dtype):
+    return product_error(x, w.T, dtype) + FP32 * np.abs(z)
+
+
+def cross_entropy_bounds(x, w, b, targets, dtype):
+    """A logarithm of sums is off by the largest error of a logit; by its exponentials, (|z - top| + 2) 2^-22 relative each, where those with |z - top| > 40 are nothing beside the largest; and by less than 200
+    additions."""
+    loss, lse, z = cross_entropy(x, w, b, targets)
+    off = logit_error(x, w, z, dtype)
+    off_lse = off.max(1) + 42 * 2.0 ** -22 + 200 * FP32 + 2 * FP32 * np.abs(lse)
+    return off_lse + off.max(1) + FP32 * np.abs(loss), off_lse
+
+
+def cross_entropy_gradients(x, w, b, targets, dloss, lse=None):
+    z = cross_entropy(x, w, b, targets)
+    p = np.exp(z[2] - (z[1] if lse is None else lse)[:, None])
+    kept = (targets >= 0) & (targets < w.shape[0])
+    d = p * np.where(kept, dloss, 0)[:, None]
+    at = np.nonzero(kept)[0]
+    d[at, targets[at]] -= dloss[at]
+    return d @ w, d.T @ x, d.sum(0)
+
+
+def cross_entropy_gradient_bounds(x, w, b, targets, dloss, dtype):
+    loss, lse, z = cross_entropy(x, w, b, targets)
+    kept = (targets >= 0) & (targets < w.shape[0])
+    weight = np.where(kept, np.abs(dloss), 0)[:, None]
+    about = z - lse[:, None]
+    p = np.exp(about)
+    # the exponent is off by the logit's error, the lse's and its own rounding
+    exponent = logit_error(x, w, z, dtype) + cross_entropy_bounds(x, w, b, targets, dtype)[1][:, None] + (np.abs(about) + 4) * 2.0 ** -22
+    off = weight * (p * np.expm1(np.minimum(exponent, 1)) + 2 * FP32 * (p + 1e-30))
+    d = p * weight
+    at = np.nonzero(kept)[0]
+    d[at, targets[at]] = np.abs(d[at, targets[at]] - np.abs(dloss[at]))
+    off[at, targets[at]] += 2 * FP32 * np.abs(dloss[at])
+    # d is kept in the tensors' type, times 2^15 over a power of two that is at most twice the largest |dloss|
+    stored = off + STEP[dtype] * d + TINY[dtype] * 2.0 ** -14 * weight.max(initial=0)
+    dx, dw, db = cross_entropy_gradients(x, w, b, targets, dloss)
+    return (rounded(dx, dtype) + product_error(d, w, dtype) + stored @ np.abs(w), rounded(dw, dtype) + product_error(d.T, x, dtype) + stored.T @ np.abs(x),
+            rounded(db, dtype) + off.sum(0) + (x.shape[0] + 80) * FP32 * d.sum(0))
+
+
 def worst(got, want, bound):
     """The largest error in units of its bound; places that are not finite have to be the same. What rounds to more than fp16's largest value, 65504, is an infinity there: from half a step beyond, 65520,
     on; within the bound of that place either is right."""
