@@ -64,46 +64,128 @@ namespace
 	}
 
 	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
+	/* a wavefront's share of the bias, and of what lies behind the last class */
+	template<typename T, int BM>
+	struct TileColumns
+	{
+			float bias[2][16];
+			int first[2]; /* column of the tile of the wavefront's blocks, counted from the first class */
+
+			__device__ __forceinline__ void begin(const TilePlace<BM> &at, const T *values, int classes)
+			{
+#pragma unroll
+				for (int j = 0; j < 2; j++)
+				{
+					first[j] = at.tile_n * BM + at.column(j);
+#pragma unroll
+					for (int r = 0; r < 16; r++)
+					{
+						const int n = column(j, r);
+						bias[j][r] = (values != nullptr && n < classes) ? static_cast<float>(values[n]) : 0.0f;
+					}
+				}
+			}
+			__device__ __forceinline__ int column(int j, int r) const
+			{
+				return first[j] + TilePlace<BM>::lane_column(r / 4) + r % 4;
+			}
+			/* f(j, r) for the register that holds class n, in the lane that holds it; most rows have their class in another tile */
+			template<typename F>
+			__device__ __forceinline__ void at_class(int n, F &&f) const
+			{
+#pragma unroll
+				for (int j = 0; j < 2; j++)
+				{
+					const int c = n - first[j];
+					if (c >= 0 && c < 32 && ((c >> 2) & 1) == ((threadIdx.x >> 5) & 1))
+#pragma unroll
+						for (int r = 0; r < 16; r++)
+							if (column(j, r) == n)
+								f(j, r);
+				}
+			}
+	};
 	template<typename T>
 	struct LossEpilogue
 	{
-			static constexpr int SHARE = 8;
-			static constexpr bool HAS_END = false;
-			struct State
-			{
-					float bias[8];
-			};
 			const T *bias;
 			const int *targets;
 			Partial *partials; /* [rows][column tiles] */
 			float *target_logits;
 			int classes, tiles_n;
 
-			template<int BN>
-			__device__ __forceinline__ void begin(State &state, int group, int tile_n) const
+			/* in registers: a lane has 32 columns of every of its rows, the lane 32 further the other 32 of the wavefront; the wavefronts of a row meet in LDS */
+			template<int BM, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-				const int n = tile_n * BN + group * 8;
+				constexpr int BLOCKS = TilePlace<BM>::BLOCKS, WAVES_N = BM / 64;
+				constexpr float NOTHING = -std::numeric_limits<float>::infinity();
+				TileColumns<T, BM> columns;
+				columns.begin(at, bias, classes);
+				int target[BLOCKS];
 #pragma unroll
-				for (int e = 0; e < 8; e++)
-					state.bias[e] = (bias != nullptr && n + e < classes) ? static_cast<float>(bias[n + e]) : 0.0f;
-			}
-			template<int BN>
-			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
-			{
-				const int n = tile_n * BN + group * 8, target = targets[m];
-				float z[8];
-				bool there[8];
-#pragma unroll
-				for (int e = 0; e < 8; e++)
+				for (int i = 0; i < BLOCKS; i++)
 				{
-					z[e] = row[group * 8 + e] + state.bias[e];
-					there[e] = n + e < classes;
-					if (there[e] && n + e == target)
-						target_logits[m] = z[e];
+					const int m = at.tile_m * BM + at.row(i);
+					target[i] = m < rows ? targets[m] : -1;
 				}
-				const Partial p = lanes_join<BN / 8>(partial_of(z, there));
-				if (group == 0)
-					partials[static_cast<size_t>(m) * tiles_n + tile_n] = p;
+				const bool edge = (at.tile_n + 1) * BM > classes;
+				Partial *meeting = reinterpret_cast<Partial*>(lds); /* [WAVES_N][BM] */
+				__syncthreads();
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++)
+				{
+					float z[2][16];
+#pragma unroll
+					for (int j = 0; j < 2; j++)
+#pragma unroll
+						for (int r = 0; r < 16; r++)
+						{
+							z[j][r] = acc[i][j][r] + columns.bias[j][r];
+							if (edge)
+								z[j][r] = columns.column(j, r) < classes ? z[j][r] : NOTHING;
+						}
+					if (target[i] >= 0 && target[i] < classes)
+						columns.at_class(target[i], [&](int j, int r) __attribute__((always_inline))
+						{
+							target_logits[at.tile_m * BM + at.row(i)] = z[j][r];
+						});
+					float top = NOTHING;
+#pragma unroll
+					for (int j = 0; j < 2; j++)
+#pragma unroll
+						for (int r = 0; r < 16; r++)
+							top = fmaxf(top, z[j][r]);
+					const float about = top == NOTHING ? 0.0f : top; /* a row of -inf alone: a sum of zeros */
+					float sum = 0.0f;
+#pragma unroll
+					for (int j = 0; j < 2; j++)
+#pragma unroll
+						for (int r = 0; r < 16; r++)
+							sum += __expf(z[j][r] - about);
+					if (top == -NOTHING) /* infinite logits are all that counts */
+					{
+						sum = 0.0f;
+#pragma unroll
+						for (int j = 0; j < 2; j++)
+#pragma unroll
+							for (int r = 0; r < 16; r++)
+								sum += z[j][r] == top ? 1.0f : (z[j][r] < top ? 0.0f : z[j][r]);
+					}
+					const Partial p = join(Partial { top, sum }, Partial { __shfl_xor(top, 32), __shfl_xor(sum, 32) });
+					if ((threadIdx.x & 32) == 0)
+						meeting[at.wave_n * BM + at.row(i)] = p;
+				}
+				__syncthreads();
+				const int row = threadIdx.x, m = at.tile_m * BM + row;
+				if (row < BM && m < rows)
+				{
+					Partial p = meeting[row];
+#pragma unroll
+					for (int w = 1; w < WAVES_N; w++)
+						p = join(p, meeting[w * BM + row]);
+					partials[static_cast<size_t>(m) * tiles_n + at.tile_n] = p;
+				}
 			}
 	};
 	constexpr int FEW_CLASSES = 32; /* of a workgroup of the few-rows kernel */
@@ -137,19 +219,36 @@ namespace
 					partials[static_cast<size_t>(row) * gridDim.x + blockIdx.x] = p;
 			}
 	}
-	/* one wavefront per row */
+	/* THREADS threads to a row: a wavefront where there are rows enough, else a workgroup, each thread with 8 pairs on their way at a time */
+	template<int THREADS>
 	__global__ __launch_bounds__(256) void kernel_join_partials(const Partial *partials, int count, const int *targets, const float *target_logits, int rows, int classes, float *loss, float *lse)
 	{
-		const int lane = threadIdx.x & 63;
-		const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+		__shared__ Partial waves[4];
+		const int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
 		if (row >= rows)
-			return;
+			return; /* whole wavefronts; a workgroup that shares a row has one */
 		Partial p { -std::numeric_limits<float>::infinity(), 0.0f };
 		const Partial *src = partials + static_cast<size_t>(row) * count;
-		for (int i = lane; i < count; i += 64)
-			p = join(p, src[i]);
+		for (int first = threadIdx.x % THREADS; first < count; first += 8 * THREADS)
+		{
+			Partial next[8];
+#pragma unroll
+			for (int u = 0; u < 8; u++)
+				next[u] = src[min(first + u * THREADS, count - 1)];
+#pragma unroll
+			for (int u = 0; u < 8; u++)
+				if (first + u * THREADS < count)
+					p = join(p, next[u]);
+		}
 		p = lanes_join<64>(p);
-		if (lane == 0)
+		if constexpr (THREADS > 64)
+		{
+			if ((threadIdx.x & 63) == 0)
+				waves[threadIdx.x >> 6] = p;
+			__syncthreads();
+			p = join(join(waves[0], waves[1]), join(waves[2], waves[3]));
+		}
+		if (threadIdx.x % THREADS == 0)
 		{
 			const float value = p.top + logf(p.sum);
 			const int target = targets[row];
@@ -201,12 +300,6 @@ namespace
 	template<typename T>
 	struct GradientEpilogue
 	{
-			static constexpr int SHARE = 8;
-			static constexpr bool HAS_END = true;
-			struct State
-			{
-					float bias[8], sum[8];
-			};
 			const T *bias; /* of the piece */
 			const int *targets;
 			const float *lse, *factors;
@@ -214,58 +307,97 @@ namespace
 			float *sums; /* [row tiles][classes of the piece], or null */
 			int first_class, classes, row_elements; /* classes: of the piece */
 
-			template<int BN>
-			__device__ __forceinline__ void begin(State &state, int group, int tile_n) const
+			/* in registers, rounded there; through LDS to whole rows. The column sums of a wavefront's 64 rows are folded so that each of 32 lanes ends up with one column of each block */
+			template<int BM, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-				const int n = tile_n * BN + group * 8;
+				constexpr int BLOCKS = TilePlace<BM>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : PANEL, PASSES = BM / ROWS;
+				TileColumns<T, BM> columns;
+				columns.begin(at, bias, classes);
+				const bool edge = (at.tile_n + 1) * BM > classes;
+				const Stage<T, BM> stage { reinterpret_cast<T*>(lds) };
+				float total[2][16];
 #pragma unroll
-				for (int e = 0; e < 8; e++)
-				{
-					state.bias[e] = (bias != nullptr && n + e < classes) ? static_cast<float>(bias[n + e]) : 0.0f;
-					state.sum[e] = 0.0f;
-				}
-			}
-			template<int BN>
-			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
-			{
-				const int n = tile_n * BN + group * 8, target = targets[m] - first_class;
-				const float norm = lse[m], factor = factors[m];
-				float v[8];
+				for (int j = 0; j < 2; j++)
 #pragma unroll
-				for (int e = 0; e < 8; e++)
+					for (int r = 0; r < 16; r++)
+						total[j][r] = 0.0f;
+				int target[BLOCKS];
+				float norm[BLOCKS], factor[BLOCKS];
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++)
 				{
-					const float about = row[group * 8 + e] + state.bias[e] - norm;
-					const float p = (sizeof(T) == 2) ? __expf(about) : expf(about); /* the hardware's is 2^-20 off, which fp16 rounds away */
-					/* a row without gradient has none, whatever its logits are */
-					v[e] = (factor == 0.0f || n + e >= classes) ? 0.0f : (p - (n + e == target ? 1.0f : 0.0f)) * factor;
-					state.sum[e] += v[e];
+					const int m = min(at.tile_m * BM + at.row(i), rows - 1);
+					target[i] = targets[m] - first_class;
+					norm[i] = lse[m];
+					factor[i] = at.tile_m * BM + at.row(i) < rows ? factors[m] : 0.0f;
 				}
-				T *dst = d + static_cast<size_t>(m) * row_elements + n;
-				if (n + 8 <= row_elements)
-					store_nearest<8>(dst, v);
-				else
-					for (int e = 0; e < row_elements - n; e++)
-						dst[e] = static_cast<T>(v[e]);
-			}
-			template<int BN, int WAVES>
-			__device__ __forceinline__ void end(State &state, int group, float *stage, int tile_m, int tile_n) const
-			{
+				static_for<PASSES>([&](auto pass)
+				{
+					constexpr int PASS = decltype(pass)::value, FIRST = PASS * BLOCKS / PASSES;
+					__syncthreads();
+#pragma unroll
+					for (int i = FIRST; i < FIRST + BLOCKS / PASSES; i++)
+					{
+						float v[2][16];
+#pragma unroll
+						for (int j = 0; j < 2; j++)
+#pragma unroll
+							for (int r = 0; r < 16; r++)
+							{
+								const float about = acc[i][j][r] + columns.bias[j][r] - norm[i];
+								const float p = (sizeof(T) == 2) ? __expf(about) : expf(about); /* the hardware's is 2^-20 off, which fp16 rounds away */
+								/* a row without gradient has none, whatever its logits are */
+								v[j][r] = factor[i] == 0.0f ? 0.0f : p * factor[i];
+								if (edge)
+									v[j][r] = columns.column(j, r) < classes ? v[j][r] : 0.0f;
+							}
+						if (factor[i] != 0.0f)
+							columns.at_class(target[i], [&](int j, int r) __attribute__((always_inline))
+							{
+								v[j][r] -= factor[i];
+							});
+#pragma unroll
+						for (int j = 0; j < 2; j++)
+#pragma unroll
+							for (int q = 0; q < 4; q++)
+							{
+								stage.put(at.row(i) - PASS * ROWS, at.column(j) + at.lane_column(q), v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
+#pragma unroll
+								for (int e = 0; e < 4; e++)
+									total[j][4 * q + e] += v[j][4 * q + e];
+							}
+					}
+					__syncthreads();
+					stage.template copy<ROWS, TilePlace<BM>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BM, row_elements);
+				});
 				if (sums == nullptr)
 					return;
-				constexpr int GROUPS = BN / SHARE, LINES = WAVES * 64 / GROUPS;
-				const int line = threadIdx.x / GROUPS;
-#pragma unroll
-				for (int e = 0; e < 8; e++)
-					stage[line * BN + group * 8 + e] = state.sum[e];
+				/* lane bits 4 .. 1 choose among the 16 registers, a half of them at a time; bit 0 adds up what is left */
+				float *meeting = reinterpret_cast<float*>(lds); /* [2 wavefront rows][BM] */
 				__syncthreads();
-				const int n = tile_n * BN + static_cast<int>(threadIdx.x);
-				if (static_cast<int>(threadIdx.x) < BN && n < classes)
+#pragma unroll
+				for (int j = 0; j < 2; j++)
 				{
-					float total = 0.0f;
-					for (int l = 0; l < LINES; l++)
-						total += stage[l * BN + threadIdx.x];
-					sums[static_cast<size_t>(tile_m) * classes + n] = total;
+#pragma unroll
+					for (int bit = 16; bit >= 2; bit >>= 1)
+#pragma unroll
+						for (int r = 0; r < bit / 2; r++)
+						{
+							const bool upper = (threadIdx.x & bit) != 0;
+							const float sent = upper ? total[j][r] : total[j][r + bit / 2];
+							const float kept = upper ? total[j][r + bit / 2] : total[j][r];
+							total[j][r] = kept + __shfl_xor(sent, bit);
+						}
+					const float sum = total[j][0] + __shfl_xor(total[j][0], 1);
+					const int r = (threadIdx.x & 31) >> 1;
+					if ((threadIdx.x & 1) == 0)
+						meeting[at.wave_m * BM + at.column(j) + TilePlace<BM>::lane_column(r / 4) + r % 4] = sum;
 				}
+				__syncthreads();
+				const int n = at.tile_n * BM + static_cast<int>(threadIdx.x);
+				if (static_cast<int>(threadIdx.x) < BM && n < classes)
+					sums[static_cast<size_t>(at.tile_m) * classes + n] = meeting[threadIdx.x] + meeting[BM + threadIdx.x];
 			}
 	};
 
@@ -386,7 +518,10 @@ namespace
 			launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, LossEpilogue<T> { bias, targets, partials, target_logits, s.classes, columns });
 		}
 		MLHIP_CHECK(hipGetLastError());
-		hipLaunchKernelGGL(kernel_join_partials, dim3(ceil_div(s.rows, 4)), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
+		if (s.rows <= 1024)
+			hipLaunchKernelGGL((kernel_join_partials<256>), dim3(s.rows), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
+		else
+			hipLaunchKernelGGL((kernel_join_partials<64>), dim3(ceil_div(s.rows, 4)), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	template<typename T>

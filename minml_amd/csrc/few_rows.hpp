@@ -100,6 +100,7 @@ namespace mlhip
 #pragma unroll
 					for (int h = 0; h < 2; h++)
 						weights[s][i][h] = load_piece(w[i] + (piece + 4 * s) * PIECE + (2 * q + h) * N);
+			__builtin_amdgcn_sched_barrier(0); /* all of them on their way before the first is used */
 #pragma unroll
 			for (int s = 0; s < STEPS; s++)
 				multiply(weights[s], (piece + 4 * s) * PIECE + 2 * q * N, std::false_type());

@@ -89,92 +89,113 @@ namespace
 	template<typename T>
 	struct GatedEpilogue
 	{
-			static constexpr int SHARE = 16; /* 8 of each projection */
-			static constexpr bool HAS_END = false;
-			struct State
-			{
-					float bias[2][8];
-			};
 			T *y, *projections;
 			const T *bias;
 			int hidden, gate;
 
-			template<int BN>
-			__device__ __forceinline__ void begin(State &state, int group, int tile_n) const
+			/*
+			 * The gate is applied in registers (blocks (i, 0) and (i, 1) hold both projections of an element). The results leave one after the other through the same place in LDS: y, then both projections
+			 * where they are kept.
+			 */
+			template<int BM, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-				const int n = tile_n * (BN / 2) + group * 8;
+				constexpr int ROWS = (sizeof(T) == 2) ? BM : PANEL, PASSES = BM / ROWS, BLOCKS = TilePlace<BM>::BLOCKS / PASSES;
+				const Stage<T, BM / 2> stage { reinterpret_cast<T*>(lds) };
+				const int n0 = at.tile_n * (BM / 2);
+				float shift[2][16];
 #pragma unroll
-				for (int i = 0; i < 2; i++)
+				for (int j = 0; j < 2; j++)
 #pragma unroll
-					for (int e = 0; e < 8; e++)
-						state.bias[i][e] = (bias != nullptr && n + e < hidden) ? static_cast<float>(bias[i * hidden + n + e]) : 0.0f;
-			}
-			template<int BN>
-			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
-			{
-				const int n = tile_n * (BN / 2) + group * 8;
-				if (n >= hidden)
-					return;
-				float g[8], u[8], out[8];
+					for (int q = 0; q < 4; q++)
 #pragma unroll
-				for (int e = 0; e < 8; e++)
-				{
-					g[e] = row[group * 8 + e] + state.bias[0][e];
-					u[e] = row[BN / 2 + group * 8 + e] + state.bias[1][e];
-					float a, unused;
-					gate_of<T, false>(gate, g[e], a, unused);
-					out[e] = a * u[e];
-				}
-				T *dst = y + static_cast<size_t>(m) * hidden + n;
-				T *kept = projections + static_cast<size_t>(m) * 2 * hidden + n;
-				if (n + 8 <= hidden)
-				{
-					store_nearest<8>(dst, out);
-					if (projections != nullptr)
-					{
-						store_nearest<8>(kept, g);
-						store_nearest<8>(kept + hidden, u);
-					}
-				}
-				else
-					for (int e = 0; e < hidden - n; e++)
-					{
-						dst[e] = static_cast<T>(out[e]);
-						if (projections != nullptr)
+						for (int e = 0; e < 4; e++)
 						{
-							kept[e] = static_cast<T>(g[e]);
-							kept[hidden + e] = static_cast<T>(u[e]);
+							const int n = n0 + at.wave_n * 32 + at.lane_column(q) + e;
+							shift[j][4 * q + e] = (bias != nullptr && n < hidden) ? static_cast<float>(bias[j * hidden + n]) : 0.0f;
 						}
+				static_for<PASSES>([&](auto pass)
+				{
+					constexpr int first = decltype(pass)::value * BLOCKS;
+					const int m0 = at.tile_m * BM + decltype(pass)::value * ROWS;
+					const auto put = [&](auto value) __attribute__((always_inline))
+					{
+						__syncthreads();
+#pragma unroll
+						for (int i = first; i < first + BLOCKS; i++)
+#pragma unroll
+							for (int q = 0; q < 4; q++)
+								stage.put(at.row(i) - decltype(pass)::value * ROWS, at.wave_n * 32 + at.lane_column(q), value(i, 4 * q), value(i, 4 * q + 1), value(i, 4 * q + 2), value(i, 4 * q + 3));
+						__syncthreads();
+					};
+					const auto projection = [&](int i, int j, int r) __attribute__((always_inline))
+					{
+						return acc[i][j][r] + shift[j][r];
+					};
+					const auto gated = [&](auto kind) __attribute__((always_inline))
+					{
+						put([&](int i, int r) __attribute__((always_inline))
+						{
+							float a, unused;
+							gate_of<T, false>(decltype(kind)::value, projection(i, 0, r), a, unused);
+							return a * projection(i, 1, r);
+						});
+					};
+					switch (gate) /* once per tile, not once per element */
+					{
+						case GATE_SIGMOID:
+							gated(std::integral_constant<int, GATE_SIGMOID>());
+							break;
+						case GATE_RELU:
+							gated(std::integral_constant<int, GATE_RELU>());
+							break;
+						case GATE_SILU:
+							gated(std::integral_constant<int, GATE_SILU>());
+							break;
+						default:
+							gated(std::integral_constant<int, GATE_GELU>());
+							break;
 					}
+					stage.template copy<ROWS, TilePlace<BM>::THREADS>(y, hidden, m0, rows, n0, hidden);
+					if (projections != nullptr)
+						static_for<2>([&](auto matrix)
+						{
+							put([&](int i, int r) __attribute__((always_inline))
+							{
+								return projection(i, decltype(matrix)::value, r);
+							});
+							stage.template copy<ROWS, TilePlace<BM>::THREADS>(projections + decltype(matrix)::value * hidden, 2 * static_cast<size_t>(hidden), m0, rows, n0, hidden);
+						});
+				});
 			}
 	};
 	/* the sums of a split product: [part][row][2][hidden] */
 	struct GatedPartEpilogue
 	{
-			static constexpr int SHARE = 16;
-			static constexpr bool HAS_END = false;
-			struct State
-			{
-			};
 			float *partial;
 			size_t part_stride;
 			int hidden;
 
-			template<int BN>
-			__device__ __forceinline__ void begin(State&, int, int) const
+			template<int BM, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-			}
-			template<int BN>
-			__device__ __forceinline__ void apply(State&, int m, int group, const float *row, int tile_n, int part) const
-			{
-				const int n = tile_n * (BN / 2) + group * 8;
-				float *dst = partial + part * part_stride + static_cast<size_t>(m) * 2 * hidden + n;
-				for (int e = 0; e < 8; e++)
-					if (n + e < hidden)
+				const Stage<float, BM / 2> stage { reinterpret_cast<float*>(lds) };
+				static_for<BM / PANEL>([&](auto half)
+				{
+					static_for<2>([&](auto matrix)
 					{
-						dst[e] = row[group * 8 + e];
-						dst[hidden + e] = row[BN / 2 + group * 8 + e];
-					}
+						constexpr int h = decltype(half)::value, j = decltype(matrix)::value;
+						__syncthreads();
+#pragma unroll
+						for (int i = 2 * h; i < 2 * h + 2; i++)
+#pragma unroll
+							for (int q = 0; q < 4; q++)
+								stage.put(at.row(i) - h * PANEL, at.wave_n * 32 + at.lane_column(q), acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+						__syncthreads();
+						stage.template copy<PANEL, TilePlace<BM>::THREADS>(partial + at.part * part_stride + j * hidden, 2 * static_cast<size_t>(hidden), at.tile_m * BM + h * PANEL, rows,
+								at.tile_n * (BM / 2), hidden);
+					});
+				});
 			}
 	};
 	template<typename T>

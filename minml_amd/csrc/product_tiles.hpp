@@ -217,27 +217,104 @@ namespace mlhip
 	}
 
 	/*
-	 * The end of a tile: accumulator blocks to LDS, then rows to the epilogue. Lane l, register r of block (i, j) holds n = 32 j' + 8 (r / 4) + 4 (l / 32) + r % 4, m = 32 i' + l % 32.
-	 * Epilogue: a thread takes SHARE of the BN sums of a row. begin(state, group, tile_n) once per tile, apply(state, m, group, row, tile_n, part) for every row m < rows with `row` its sums in LDS (all threads
-	 * of a row together), and, where HAS_END, end(state, group, stage, tile_m, tile_n) once all rows are through, by all threads.
+	 * Where a wavefront's accumulators lie in the tile, and how they leave it. Block (i, j) covers rows row(i) .. + 31 and columns column(j) .. + 31; lane l holds row l % 32 and, in registers 4 q .. 4 q + 3, columns
+	 * 8 q + 4 (l / 32) .. + 3. In a paired product blocks (i, 0) and (i, 1) are the two matrices' sums of the same place.
 	 */
-	template<int BN, int WAVES, typename Epilogue, typename State>
-	__device__ __forceinline__ void rows_to_epilogue(State &state, const float *stage, int m0, int M, int tile_n, const Epilogue &epilogue)
+	template<int BM>
+	struct TilePlace
 	{
-		constexpr int STRIDE = BN + 4, GROUPS = BN / Epilogue::SHARE, ROWS_AT_A_TIME = WAVES * 64 / GROUPS;
-		const int group = threadIdx.x % GROUPS;
-		for (int row = threadIdx.x / GROUPS; row < PANEL; row += ROWS_AT_A_TIME)
-			if (m0 + row < M)
-				epilogue.template apply<BN>(state, m0 + row, group, stage + row * STRIDE, tile_n, blockIdx.y);
-	}
-	template<typename Acc>
-	__device__ __forceinline__ void block_to_stage(float *stage, int stride, int row, int column, const Acc &acc)
+			static constexpr int BLOCKS = BM / 64, THREADS = 2 * BM;
+			int tile_m, tile_n, part, wave_m, wave_n;
+
+			__device__ __forceinline__ int row(int i) const
+			{
+				return (BM == 256 ? (i >> 1) * 128 + wave_m * 64 + (i & 1) * 32 : i * 64 + wave_m * 32) + lane_row();
+			}
+			__device__ __forceinline__ int column(int j) const
+			{
+				return j * (BM / 2) + wave_n * 32;
+			}
+			__device__ __forceinline__ static int lane_row()
+			{
+				return threadIdx.x & 31;
+			}
+			__device__ __forceinline__ static int lane_column(int q)
+			{
+				return 8 * q + 4 * ((threadIdx.x >> 5) & 1);
+			}
+	};
+	/*
+	 * A tile (or the rows of it that lie in LDS) to memory, 16 bytes per thread and whole rows by neighbouring threads. f(m, n, LDS place, elements): elements of the vector that exist, all of them or fewer at the
+	 * matrix's edge.
+	 */
+	template<typename Out, int COLUMNS>
+	struct Stage
 	{
-		const int lane = threadIdx.x & 63;
-		float *dst = stage + (row + (lane & 31)) * stride + column + 4 * (lane >> 5);
+			static constexpr int VECTOR = 16 / sizeof(Out), STRIDE = COLUMNS + VECTOR; /* a row more than a whole number of banks' turns: the lanes of a block write 32 rows at a time */
+			static constexpr int bytes(int rows)
+			{
+				return rows * STRIDE * static_cast<int>(sizeof(Out));
+			}
+			Out *place;
+
+			__device__ __forceinline__ void put(int row, int column, float a, float b, float c, float d) const
+			{
+				typedef Out vec4_t __attribute__((ext_vector_type(4)));
+				*reinterpret_cast<vec4_t*>(place + row * STRIDE + column) = vec4_t { static_cast<Out>(a), static_cast<Out>(b), static_cast<Out>(c), static_cast<Out>(d) };
+			}
+			template<int ROWS, int THREADS, typename F>
+			__device__ __forceinline__ void for_vectors(int m0, int rows, int n0, int columns, F &&f) const
+			{
+				constexpr int LANES = COLUMNS / VECTOR, AT_A_TIME = THREADS / LANES;
+				const int n = n0 + (threadIdx.x % LANES) * VECTOR;
+				const int there = min(columns - n, VECTOR);
+				if (there <= 0)
+					return;
+#pragma unroll 4
+				for (int row = threadIdx.x / LANES; row < ROWS; row += AT_A_TIME)
+					if (m0 + row < rows)
+						f(m0 + row, n, place + row * STRIDE + (n - n0), there);
+			}
+			/* to rows `stride` elements apart */
+			template<int ROWS, int THREADS>
+			__device__ __forceinline__ void copy(Out *out, size_t stride, int m0, int rows, int n0, int columns) const
+			{
+				for_vectors<ROWS, THREADS>(m0, rows, n0, columns, [&](int m, int n, const Out *src, int there) __attribute__((always_inline))
+				{
+					Out *dst = out + m * stride + n;
+					if (there == VECTOR)
+					{
+						typedef typename Elements<Out, VECTOR>::vec_t vec_t;
+						*reinterpret_cast<typename Elements<Out, VECTOR>::unaligned_t*>(dst) = *reinterpret_cast<const vec_t*>(src);
+					}
+					else
+						for (int e = 0; e < there; e++)
+							dst[e] = src[e];
+				});
+			}
+	};
+	/* the sums of a tile through LDS in fp32, 128 rows at a time: f(m, n, 4 sums in LDS, elements) */
+	template<int BM, typename Acc, typename F>
+	__device__ __forceinline__ void sums_in_rows(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows, int columns, F &&f)
+	{
+		const Stage<float, BM> stage { reinterpret_cast<float*>(lds) };
+		static_for<BM / PANEL>([&](auto half)
+		{
+			constexpr int h = decltype(half)::value;
+			__syncthreads();
 #pragma unroll
-		for (int q = 0; q < 4; q++)
-			*reinterpret_cast<float4_t*>(dst + 8 * q) = float4_t { acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3] };
+			for (int i = 0; i < 2; i++)
+#pragma unroll
+				for (int j = 0; j < 2; j++)
+#pragma unroll
+					for (int q = 0; q < 4; q++)
+					{
+						const Acc &v = acc[2 * h + i][j];
+						stage.put(at.row(2 * h + i) - h * PANEL, at.column(j) + at.lane_column(q), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+					}
+			__syncthreads();
+			stage.template for_vectors<PANEL, TilePlace<BM>::THREADS>(at.tile_m * BM + h * PANEL, rows, at.tile_n * BM, columns, f);
+		});
 	}
 
 	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
@@ -427,28 +504,7 @@ namespace mlhip
 		if (c < chunks)
 			process_chunk(c, std::false_type(), std::false_type());
 
-		/* block (i, j): rows (i / 2) 128 + wave_m 64 + (i % 2) 32, columns j 128 + wave_n 32 */
-		float *stage = reinterpret_cast<float*>(lds);
-		const int group = threadIdx.x % (256 / Epilogue::SHARE);
-		typename Epilogue::State state;
-		epilogue.template begin<256>(state, group, tile_n);
-		static_for<2>([&](auto half)
-		{
-			constexpr int h = decltype(half)::value;
-			__syncthreads();
-#pragma unroll
-			for (int i = 0; i < 2; i++)
-#pragma unroll
-				for (int j = 0; j < 2; j++)
-					block_to_stage(stage, 260, wave_m * 64 + i * 32, j * PANEL + wave_n * 32, acc[2 * h + i][j]);
-			__syncthreads();
-			rows_to_epilogue<256, WAVES>(state, stage, tile_m * 256 + h * PANEL, p.rows, tile_n, epilogue);
-		});
-		if constexpr (Epilogue::HAS_END)
-		{
-			__syncthreads();
-			epilogue.template end<256, WAVES>(state, group, stage, tile_m, tile_n);
-		}
+		epilogue.template tile<256>(acc, TilePlace<256> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
 	}
 
 	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
@@ -525,26 +581,12 @@ namespace mlhip
 						Traits::mma(fb[j], fa[i], acc[i][j]);
 			}
 		}
-		float *stage = reinterpret_cast<float*>(lds);
-		__syncthreads();
-#pragma unroll
-		for (int i = 0; i < 2; i++)
-#pragma unroll
-			for (int j = 0; j < 2; j++)
-				block_to_stage(stage, 132, i * 64 + wave_m * 32, j * 64 + wave_n * 32, acc[i][j]);
-		__syncthreads();
-		const int group = threadIdx.x % (128 / Epilogue::SHARE);
-		typename Epilogue::State state;
-		epilogue.template begin<128>(state, group, tile_n);
-		rows_to_epilogue<128, WAVES>(state, stage, m0, p.rows, tile_n, epilogue);
-		if constexpr (Epilogue::HAS_END)
-		{
-			__syncthreads();
-			epilogue.template end<128, WAVES>(state, group, stage, tile_m, tile_n);
-		}
+		epilogue.template tile<128>(acc, TilePlace<128> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
 	}
-	constexpr int PRODUCT_LDS_256 = PANEL * 260 * 4 > 8 * PANEL_BYTES ? PANEL * 260 * 4 : 8 * PANEL_BYTES;
-	constexpr int PRODUCT_LDS_128 = PANEL * 132 * 4 > 4 * PANEL_BYTES ? PANEL * 132 * 4 : 4 * PANEL_BYTES;
+	/* slots, or what an epilogue lays out there: 128 rows of fp32 or a whole tile of fp16 */
+	constexpr int PRODUCT_LDS_256 = std::max(8 * PANEL_BYTES, std::max(Stage<float, 256>::bytes(PANEL), Stage<half_t, 256>::bytes(256)));
+	constexpr int PRODUCT_LDS_128 = std::max(4 * PANEL_BYTES, std::max(Stage<float, 128>::bytes(PANEL), Stage<half_t, 128>::bytes(PANEL)));
+	static_assert(PRODUCT_LDS_256 <= 160 * 1024 && 2 * PRODUCT_LDS_128 <= 160 * 1024, "tiles must fit the LDS of a compute unit");
 
 	/* how a product is cut: tiles of `tile` rows and columns, `parts` along k. A workspace is sized by the same rule, so it asks no device */
 	struct ProductPlan
@@ -602,91 +644,93 @@ namespace mlhip
 	template<typename Out>
 	struct StoreEpilogue
 	{
-			static constexpr int SHARE = 8;
-			static constexpr bool HAS_END = false;
-			struct State
-			{
-					float scale;
-			};
 			Out *out;
 			int columns;
 			float beta;
 			const float *scale; /* on the device; null: 1 */
 
-			template<int BN>
-			__device__ __forceinline__ void begin(State &state, int, int) const
+			template<int BM, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-				state.scale = scale != nullptr ? *scale : 1.0f;
-			}
-			template<int BN>
-			__device__ __forceinline__ void apply(State &state, int m, int group, const float *row, int tile_n, int) const
-			{
-				const int n = tile_n * BN + group * 8;
-				if (n >= columns)
-					return;
-				float v[8];
-#pragma unroll
-				for (int e = 0; e < 8; e++)
-					v[e] = row[group * 8 + e] * state.scale;
-				Out *dst = out + static_cast<size_t>(m) * columns + n;
-				if (n + 8 <= columns)
+				const float factor = scale != nullptr ? *scale : 1.0f;
+				if (sizeof(Out) == 2 && beta == 0.0f)
 				{
-					if (beta != 0.0f)
-					{
-						Elements<Out, 8> old;
-						old.load(dst);
+					/* rounded in registers: the whole tile in one go */
+					const Stage<Out, BM> stage { reinterpret_cast<Out*>(lds) };
+					__syncthreads();
 #pragma unroll
-						for (int e = 0; e < 8; e++)
-							v[e] = fmaf(beta, old[e], v[e]);
-					}
-					store_nearest<8>(dst, v);
+					for (int i = 0; i < TilePlace<BM>::BLOCKS; i++)
+#pragma unroll
+						for (int j = 0; j < 2; j++)
+#pragma unroll
+							for (int q = 0; q < 4; q++)
+							{
+								const Acc &v = acc[i][j];
+								stage.put(at.row(i), at.column(j) + at.lane_column(q), v[4 * q] * factor, v[4 * q + 1] * factor, v[4 * q + 2] * factor, v[4 * q + 3] * factor);
+							}
+					__syncthreads();
+					stage.template copy<BM, TilePlace<BM>::THREADS>(out, columns, at.tile_m * BM, rows, at.tile_n * BM, columns);
 				}
 				else
-					for (int e = 0; e < columns - n; e++)
-						dst[e] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(dst[e]), v[e]) : v[e]);
+					sums_in_rows<BM>(acc, at, lds, rows, columns, [&](int m, int n, const float *sums, int there) __attribute__((always_inline))
+					{
+						Out *dst = out + static_cast<size_t>(m) * columns + n;
+						float v[4];
+#pragma unroll
+						for (int e = 0; e < 4; e++)
+							v[e] = sums[e] * factor;
+						if (there == 4)
+						{
+							if (beta != 0.0f)
+							{
+								Elements<Out, 4> old;
+								old.load(dst);
+#pragma unroll
+								for (int e = 0; e < 4; e++)
+									v[e] = fmaf(beta, old[e], v[e]);
+							}
+							store_nearest<4>(dst, v);
+						}
+						else
+#pragma unroll
+							for (int e = 0; e < 4; e++)
+								if (e < there)
+									dst[e] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(dst[e]), v[e]) : v[e]);
+					});
 			}
 	};
 	/* partial[part][m][n] = sum, or += sum: [parts][rows][columns] in fp32 */
 	struct PartEpilogue
 	{
-			static constexpr int SHARE = 8;
-			static constexpr bool HAS_END = false;
-			struct State
-			{
-			};
 			float *partial;
 			size_t part_stride;
 			int columns;
 			bool add;
 
-			template<int BN>
-			__device__ __forceinline__ void begin(State&, int, int) const
+			template<int BM, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-			}
-			template<int BN>
-			__device__ __forceinline__ void apply(State&, int m, int group, const float *row, int tile_n, int part) const
-			{
-				const int n = tile_n * BN + group * 8;
-				float *dst = partial + part * part_stride + static_cast<size_t>(m) * columns + n;
-				if (n + 8 <= columns)
+				float *out = partial + at.part * part_stride;
+				sums_in_rows<BM>(acc, at, lds, rows, columns, [&](int m, int n, const float *sums, int there) __attribute__((always_inline))
 				{
-					float v[8];
-#pragma unroll
-					for (int e = 0; e < 8; e++)
-						v[e] = row[group * 8 + e];
-					if (add)
+					float *dst = out + static_cast<size_t>(m) * columns + n;
+					if (there == 4)
 					{
-						Elements<float, 8> old;
-						old.load(dst);
+						float v[4] = { sums[0], sums[1], sums[2], sums[3] };
+						if (add)
+						{
+							Elements<float, 4> old;
+							old.load(dst);
 #pragma unroll
-						for (int e = 0; e < 8; e++)
-							v[e] += old[e];
+							for (int e = 0; e < 4; e++)
+								v[e] += old[e];
+						}
+						store_nearest<4>(dst, v);
 					}
-					store_nearest<8>(dst, v);
-				}
-				else
-					for (int e = 0; e < columns - n; e++)
-						dst[e] = add ? dst[e] + row[group * 8 + e] : row[group * 8 + e];
+					else
+						for (int e = 0; e < there; e++)
+							dst[e] = add ? dst[e] + sums[e] : sums[e];
+				});
 			}
 	};
 	/* out = scale * (sum of the parts) + beta * out, parts in order */
