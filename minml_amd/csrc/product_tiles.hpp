@@ -29,6 +29,7 @@
 #include "training_utils.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace mlhip
 {
@@ -593,28 +594,44 @@ namespace mlhip
 	{
 			int tile, tiles_m, tiles_n, chunks, parts, chunks_per_part;
 	};
-	/* columns: of the result (of one of the two matrices where the operand is paired) */
+	/*
+	 * The cheapest of both tile sizes and up to 16 parts, by what they take: a compute unit works off its tiles one after the other (two of 128x128 side by side take as long as one after the other), a tile takes
+	 * so long per chunk and something for its beginning and end, and parts have to be added up. Microseconds on a full chip, fp16 / fp32: a chunk of 256x256 1.7 / 8.4 (1.2 where at most half of the units have
+	 * a tile: what they read then comes faster), of 128x128 0.6 / 2.05 (its operands' way out of the L2 bounds it in fp16: 32 KB, 30 bytes per clock and unit). Measured, two sides each: dx of 4096 x 2048, k = 16384, fp16
+	 * (128 tiles of 256x256) whole 313, in 2 parts 228, 128x128 tiles 310; dW of 11008 x 2048, k = 8192, fp16 (344 tiles) 388, 385, 379; 2048 x 1024, k = 8192, fp16 143, 87, 79, 128x128 in 2 parts
+	 * 53; dW of 5462 x 1000, k = 1111, fp32 270, 160, 147, 128x128 in 2 parts 127.
+	 * columns: of the result (of one of the two matrices where the operand is paired)
+	 */
 	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split)
 	{
 		constexpr int UNITS = 256;
-		ProductPlan plan;
-		const auto tiles = [&](int tile)
+		const bool half = element_size == 2;
+		const int chunks = ceil_div(depth, 128 / element_size);
+		ProductPlan best { 256, 0, 0, chunks, 1, std::max(1, chunks) };
+		double least = 0.0;
+		for (int tile : { 256, 128 })
 		{
-			plan.tile = tile;
-			plan.tiles_m = ceil_div(rows, tile);
-			plan.tiles_n = ceil_div(columns, paired ? tile / 2 : tile);
-			return static_cast<long long>(plan.tiles_m) * plan.tiles_n;
-		};
-		plan.chunks = ceil_div(depth, 128 / element_size);
-		long long count = tiles(256);
-		if (count < 3 * UNITS / 4)
-			count = tiles(128);
-		plan.parts = 1;
-		if (may_split && count < UNITS && count > 0)
-			plan.parts = static_cast<int>(std::max<long long>(1, std::min<long long>(UNITS * 2 / count, plan.chunks / 8)));
-		plan.chunks_per_part = std::max(1, ceil_div(plan.chunks, plan.parts));
-		plan.parts = std::max(1, ceil_div(plan.chunks, plan.chunks_per_part));
-		return plan;
+			const int tiles_m = ceil_div(rows, tile), tiles_n = ceil_div(columns, paired ? tile / 2 : tile);
+			const double tiles = static_cast<double>(tiles_m) * tiles_n;
+			const int most = (may_split && tiles < 2 * UNITS) ? std::max(1, std::min(16, chunks / 4)) : 1;
+			for (int parts = 1; parts <= most; parts++)
+			{
+				const int per_part = std::max(1, ceil_div(chunks, parts));
+				if (parts > 1 && ceil_div(chunks, per_part) != parts)
+					continue;
+				const double turns = std::ceil(tiles * parts / UNITS);
+				const double chunk = tile == 128 ? (half ? 0.6 : 2.05) : (half ? (tiles * parts <= UNITS / 2 ? 1.2 : 1.7) : 8.4);
+				double cost = turns * ((tile == 128 ? 4.0 : 8.0) + per_part * chunk);
+				if (parts > 1)
+					cost += 6.0 + 8e-6 / 5.0 * parts * rows * (paired ? 2.0 : 1.0) * columns; /* written and read at 5 TB/s */
+				if (least == 0.0 || cost < least)
+				{
+					least = cost;
+					best = ProductPlan { tile, tiles_m, tiles_n, chunks, parts, per_part };
+				}
+			}
+		}
+		return best;
 	}
 	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
 	inline void launch_product(hipStream_t stream, const ProductPlan &plan, const Operand &a, const Operand &b, int rows, const Epilogue &epilogue)
