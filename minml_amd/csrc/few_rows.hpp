@@ -37,6 +37,12 @@ namespace mlhip
 		v.load(p);
 		return __builtin_bit_cast(uint4_t, v.raw);
 	}
+	/* the same for what is read once: not meant to be kept in the caches */
+	template<typename T>
+	__device__ __forceinline__ uint4_t load_streaming(const T *p)
+	{
+		return __builtin_bit_cast(uint4_t, __builtin_nontemporal_load(reinterpret_cast<const typename Elements<T, 16 / sizeof(T)>::unaligned_t*>(p)));
+	}
 	/* the same where only `left` elements (perhaps none, or less) are the row's; the others are zero */
 	template<typename T>
 	__device__ __forceinline__ uint4_t load_piece(const T *p, int left)
@@ -58,7 +64,8 @@ namespace mlhip
 	template<typename T, int MB>
 	__device__ __forceinline__ void few_rows_sums(const T *x, int rows, const T *w_first, const T *w_second, int last_first, int last_second, int k, float (*sums)[16 * MB][16])
 	{
-		constexpr int PIECE = 128 / sizeof(T), N = 16 / sizeof(T), STEPS = 4; /* elements of a 128-byte piece, of a load; pieces in flight */
+		/* elements of a 128-byte piece and of a load; pieces of a batch: two batches of 16 KB of weights are on their way (8 KB where many rows of x take the registers) */
+		constexpr int PIECE = 128 / sizeof(T), N = 16 / sizeof(T), STEPS = MB == 1 ? 4 : 2;
 		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
 		const T *w[2] = { w_first + static_cast<size_t>(min(r, last_first)) * k, w_second + static_cast<size_t>(min(r, last_second)) * k };
 		const T *xs[MB];
@@ -71,51 +78,75 @@ namespace mlhip
 #pragma unroll
 			for (int b = 0; b < MB; b++)
 				acc[i][b] = float4_t { 0.0f, 0.0f, 0.0f, 0.0f };
-		const int whole = k / PIECE;
-		int piece = wave;
-		const auto multiply = [&](const uint4_t (&weights)[2][2], int at, auto tail) __attribute__((always_inline))
+		struct Batch
+		{
+				uint4_t weights[STEPS][2][2], rows[STEPS][MB][2];
+		};
+		const auto request = [&](Batch &batch, int piece) __attribute__((always_inline))
 		{
 #pragma unroll
-			for (int b = 0; b < MB; b++)
+			for (int s = 0; s < STEPS; s++)
 #pragma unroll
 				for (int h = 0; h < 2; h++)
 				{
-					uint4_t v;
-					if constexpr (decltype(tail)::value)
-						v = load_piece(xs[b] + at + h * N, k - at - h * N);
-					else
-						v = load_piece(xs[b] + at + h * N);
+					const int at = (piece + 4 * s) * PIECE + (2 * q + h) * N;
 #pragma unroll
 					for (int i = 0; i < 2; i++)
-						mma_16x16<T>(weights[i][h], v, acc[i][b]);
+						batch.weights[s][i][h] = load_streaming(w[i] + at);
+#pragma unroll
+					for (int b = 0; b < MB; b++)
+						batch.rows[s][b][h] = load_piece(xs[b] + at);
 				}
 		};
-		for (; piece + 4 * (STEPS - 1) < whole; piece += 4 * STEPS)
+		const auto multiply = [&](const Batch &batch) __attribute__((always_inline))
 		{
-			uint4_t weights[STEPS][2][2];
 #pragma unroll
 			for (int s = 0; s < STEPS; s++)
-#pragma unroll
-				for (int i = 0; i < 2; i++)
-#pragma unroll
-					for (int h = 0; h < 2; h++)
-						weights[s][i][h] = load_piece(w[i] + (piece + 4 * s) * PIECE + (2 * q + h) * N);
-			__builtin_amdgcn_sched_barrier(0); /* all of them on their way before the first is used */
-#pragma unroll
-			for (int s = 0; s < STEPS; s++)
-				multiply(weights[s], (piece + 4 * s) * PIECE + 2 * q * N, std::false_type());
-		}
-		for (; piece * PIECE < k; piece += 4)
-		{
-			const int at = piece * PIECE + 2 * q * N;
-			uint4_t weights[2][2];
-#pragma unroll
-			for (int i = 0; i < 2; i++)
 #pragma unroll
 				for (int h = 0; h < 2; h++)
-					weights[i][h] = load_piece(w[i] + at + h * N, k - at - h * N);
-			multiply(weights, at, std::true_type());
+#pragma unroll
+					for (int b = 0; b < MB; b++)
+#pragma unroll
+						for (int i = 0; i < 2; i++)
+							mma_16x16<T>(batch.weights[s][i][h], batch.rows[s][b][h], acc[i][b]);
+		};
+		const int whole = k / PIECE;
+		const int batches = max(0, (whole - wave + 3) / 4) / STEPS; /* of this wavefront's pieces wave, wave + 4, ... */
+		Batch even, odd;
+		if (batches > 0)
+			request(even, wave);
+		for (int n = 0; n < batches; n += 2)
+		{
+			if (n + 1 < batches)
+				request(odd, wave + (n + 1) * 4 * STEPS);
+			__builtin_amdgcn_sched_barrier(0); /* the next batch is on its way before this one is waited for */
+			multiply(even);
+			if (n + 1 < batches)
+			{
+				if (n + 2 < batches)
+					request(even, wave + (n + 2) * 4 * STEPS);
+				__builtin_amdgcn_sched_barrier(0);
+				multiply(odd);
+			}
 		}
+		for (int piece = wave + batches * 4 * STEPS; piece * PIECE < k; piece += 4)
+#pragma unroll
+			for (int h = 0; h < 2; h++)
+			{
+				const int at = piece * PIECE + (2 * q + h) * N;
+				uint4_t weights[2];
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+					weights[i] = load_piece(w[i] + at, k - at);
+#pragma unroll
+				for (int b = 0; b < MB; b++)
+				{
+					const uint4_t v = load_piece(xs[b] + at, k - at);
+#pragma unroll
+					for (int i = 0; i < 2; i++)
+						mma_16x16<T>(weights[i], v, acc[i][b]);
+				}
+			}
 		/* lane: row of x r, rows 4 q .. 4 q + 3 of W. The wavefronts add theirs up in order */
 		for (int turn = 0; turn < 4; turn++)
 		{

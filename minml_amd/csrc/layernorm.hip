@@ -504,10 +504,16 @@ namespace
 						beta_dx, sums ? partial : nullptr, parts);
 			});
 		MLHIP_CHECK(hipGetLastError());
-		if (dw.data != nullptr)
-			launch_sum_partials(stream, partial, parts, 2 * static_cast<size_t>(columns), dw.data, dw.dtype, columns, beta_weights);
-		if (db.data != nullptr)
-			launch_sum_partials(stream, partial + columns, parts, 2 * static_cast<size_t>(columns), db.data, db.dtype, columns, beta_weights);
+		const size_t stride = 2 * static_cast<size_t>(columns);
+		if (dw.data != nullptr && db.data != nullptr && dw.dtype == db.dtype)
+			launch_sum_partials(stream, partial, parts, stride, dw.data, dw.dtype, columns, beta_weights, nullptr, db.data);
+		else
+		{
+			if (dw.data != nullptr)
+				launch_sum_partials(stream, partial, parts, stride, dw.data, dw.dtype, columns, beta_weights);
+			if (db.data != nullptr)
+				launch_sum_partials(stream, partial + columns, parts, stride, db.data, db.dtype, columns, beta_weights);
+		}
 	}
 
 	bool same_shape(const mlTensor_t &a, const mlTensor_t &b)

@@ -401,9 +401,9 @@ namespace mlhip
 				request_a(c, one());
 			}
 		if (chunks > 1)
-			wait_vmcnt<6 * LOADS>();
+			wait_vmcnt<5 * LOADS>();
 		else
-			wait_vmcnt<2 * LOADS>();
+			wait_vmcnt<LOADS>();
 		barrier_no_fence();
 		if (chunks > 0)
 		{
@@ -412,6 +412,7 @@ namespace mlhip
 			{
 				read_a(0, A0, kk);
 				read_b(0, B0, kk, fb0);
+				read_b(0, B1, kk, fb1);
 			}
 		}
 		/* one chunk: whether there is a next one, and whether there is one after it */
@@ -424,75 +425,51 @@ namespace mlhip
 				for (int i = 0; i < 2; i++)
 					Traits::mma(regs[kk], fa[i][kk], acc[decltype(row)::value + i][decltype(column)::value]);
 			};
-			/* phase 0: A0 B0. Behind B1 of this chunk: its A1, all of the next one */
-			wait_vmcnt<NEXT ? 5 * LOADS : LOADS>();
-			barrier_no_fence();
-			multiply(0, fb0, zero(), zero());
-			__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-			for (int kk = 0; kk < 4; kk++)
-				read_b(c, B1, kk, fb1);
-			__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-			for (int kk = 1; kk < 4; kk++)
-				multiply(kk, fb0, zero(), zero());
-			__builtin_amdgcn_sched_barrier(0);
-			/* phase 1: A0 B1. Behind A1: all of the next chunk. A0 and B0 have been read by all */
+			/* A0 with both halves of B. Behind A1 of this chunk: all of the next one. This wavefront's reads of A0, B0 and B1 are complete before anyone may overwrite them */
+			wait_lgkmcnt<0>();
 			wait_vmcnt<NEXT ? 4 * LOADS : 0>();
 			barrier_no_fence();
-			multiply(0, fb1, zero(), one());
-			__builtin_amdgcn_sched_barrier(0);
-			read_a(c, A1, 0);
-			if constexpr (AFTER)
-			{
-				request_a(c + 2, zero());
-				request_b(c + 2, zero());
-			}
-			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-			for (int kk = 1; kk < 4; kk++)
+			for (int kk = 0; kk < 4; kk++)
 			{
+				multiply(kk, fb0, zero(), zero());
 				multiply(kk, fb1, zero(), one());
 				__builtin_amdgcn_sched_barrier(0);
 				read_a(c, A1, kk);
+				if constexpr (AFTER)
+				{
+					if (kk == 0)
+						request_a(c + 2, zero());
+					if (kk == 1)
+						request_b(c + 2, zero());
+					if (kk == 2)
+						request_b(c + 2, one());
+				}
 				__builtin_amdgcn_sched_barrier(0);
 			}
-			/* phase 2: A1 B1, whose fragments are in registers */
-			barrier_no_fence();
-			multiply(0, fb1, two(), one());
-			__builtin_amdgcn_sched_barrier(0);
-			if constexpr (AFTER)
-				request_b(c + 2, one());
-			__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-			for (int kk = 1; kk < 4; kk++)
-				multiply(kk, fb1, two(), one());
-			__builtin_amdgcn_sched_barrier(0);
-			/* phase 3: A1 B0. Behind A0 and B0 of the next chunk: its other two panels, three of the one after it */
+			/* A1 with both halves of B. Behind A0, B0 and B1 of the next chunk: its A1, and three panels of the one after it */
 			if constexpr (NEXT)
 			{
-				wait_vmcnt<AFTER ? 5 * LOADS : 2 * LOADS>();
+				wait_lgkmcnt<0>();
+				wait_vmcnt<AFTER ? 4 * LOADS : LOADS>();
 				barrier_no_fence();
 			}
-			multiply(0, fb0, two(), zero());
-			__builtin_amdgcn_sched_barrier(0);
-			if constexpr (NEXT)
-			{
-				read_a(c + 1, A0, 0);
-				read_b(c + 1, B0, 0, fb0);
-			}
-			if constexpr (AFTER)
-				request_a(c + 2, one());
-			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-			for (int kk = 1; kk < 4; kk++)
+			for (int kk = 0; kk < 4; kk++)
 			{
 				multiply(kk, fb0, two(), zero());
+				multiply(kk, fb1, two(), one());
 				__builtin_amdgcn_sched_barrier(0);
 				if constexpr (NEXT)
 				{
 					read_a(c + 1, A0, kk);
 					read_b(c + 1, B0, kk, fb0);
+					read_b(c + 1, B1, kk, fb1);
+				}
+				if constexpr (AFTER)
+				{
+					if (kk == 0)
+						request_a(c + 2, one());
 				}
 				__builtin_amdgcn_sched_barrier(0);
 			}

@@ -99,9 +99,14 @@ namespace mlhip
 	 * threads to a column add up every eighth of them and meet in LDS: a fixed order, so the same bits every time, which additions by atomic operations would not give.
 	 */
 	template<typename Out>
-	__global__ __launch_bounds__(256) void kernel_sum_partials(const float *partial, int parts, size_t stride, Out *out, int columns, float beta, const float *scale)
+	__global__ __launch_bounds__(256) void kernel_sum_partials(const float *partial, int parts, size_t stride, Out *out, int columns, float beta, const float *scale, Out *second)
 	{
 		__shared__ float sums[8][33];
+		if (blockIdx.y == 1) /* the columns behind the first ones, for another result */
+		{
+			partial += columns;
+			out = second;
+		}
 		const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
 		const int j = blockIdx.x * 32 + c;
 		float sum = 0.0f;
@@ -134,17 +139,19 @@ namespace mlhip
 			out[j] = static_cast<Out>(beta != 0.0f ? fmaf(beta, static_cast<float>(out[j]), sum) : sum);
 		}
 	}
-	/* out: the gradient of a weight, of the tensors' type or fp32. scale: on the device, or null for 1 */
+	/* out: the gradient of a weight, of the tensors' type or fp32. scale: on the device, or null for 1. second: null, or a result of the same type for the next `columns` columns */
 	inline void launch_sum_partials(hipStream_t stream, const float *partial, int parts, size_t stride, void *out, mlDataType_t dtype, int columns, float beta,
-			const float *scale = nullptr)
+			const float *scale = nullptr, void *second = nullptr)
 	{
 		if (columns == 0)
 			return;
-		const dim3 grid(ceil_div(columns, 32));
+		const dim3 grid(ceil_div(columns, 32), second != nullptr ? 2 : 1);
 		if (dtype == DTYPE_FLOAT16)
-			hipLaunchKernelGGL((kernel_sum_partials<half_t>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<half_t*>(out), columns, beta, scale);
+			hipLaunchKernelGGL((kernel_sum_partials<half_t>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<half_t*>(out), columns, beta, scale,
+					reinterpret_cast<half_t*>(second));
 		else
-			hipLaunchKernelGGL((kernel_sum_partials<float>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<float*>(out), columns, beta, scale);
+			hipLaunchKernelGGL((kernel_sum_partials<float>), grid, dim3(256), 0, stream, partial, parts, stride, reinterpret_cast<float*>(out), columns, beta, scale,
+					reinterpret_cast<float*>(second));
 		MLHIP_CHECK(hipGetLastError());
 	}
 	inline size_t round_up(size_t n, size_t to)
