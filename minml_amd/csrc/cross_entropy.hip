@@ -189,17 +189,17 @@ namespace
 			}
 	};
 	constexpr int FEW_CLASSES = 32; /* of a workgroup of the few-rows kernel */
-	template<typename T, int MB>
-	__global__ __launch_bounds__(256) void kernel_loss_few_rows(const T *x, const T *w, const T *bias, const int *targets, int rows, int features, int classes, Partial *partials,
+	template<typename T, int MB, int WAVES>
+	__global__ __launch_bounds__(64 * WAVES) void kernel_loss_few_rows(const T *x, const T *w, const T *bias, const int *targets, int rows, int features, int classes, Partial *partials,
 			float *target_logits)
 	{
-		__shared__ __attribute__((aligned(16))) float sums[2][16 * MB][16];
+		__shared__ __attribute__((aligned(16))) float sums[WAVES][2][16 * MB][16];
 		const int n0 = blockIdx.x * FEW_CLASSES;
 		const T *first = w + static_cast<size_t>(n0) * features;
 		const bool second = n0 + 16 < classes; /* else the first block stands in for it */
-		few_rows_sums<T, MB>(x, rows, first, second ? first + static_cast<size_t>(16) * features : first, min(15, classes - 1 - n0), min(15, classes - 1 - n0 - (second ? 16 : 0)), features, sums);
+		few_rows_sums<T, MB, WAVES>(x, rows, first, second ? first + static_cast<size_t>(16) * features : first, min(15, classes - 1 - n0), min(15, classes - 1 - n0 - (second ? 16 : 0)), features, sums);
 		const int c = threadIdx.x & 15;
-		for (int row = threadIdx.x >> 4; row < 16 * MB; row += 16)
+		for (int row = threadIdx.x >> 4; row < 16 * MB; row += 4 * WAVES)
 			if (row < rows)
 			{
 				const int target = targets[row];
@@ -210,7 +210,7 @@ namespace
 				{
 					const int n = n0 + 16 * i + c;
 					there[i] = n < classes;
-					z[i] = sums[i][row][c] + ((bias != nullptr && there[i]) ? static_cast<float>(bias[n]) : 0.0f);
+					z[i] = sums[0][i][row][c] + ((bias != nullptr && there[i]) ? static_cast<float>(bias[n]) : 0.0f);
 					if (there[i] && n == target)
 						target_logits[row] = z[i];
 				}
@@ -418,6 +418,10 @@ namespace
 		MLHIP_REQUIRE(rows <= (1 << 28) && w.dim[0] <= (1 << 28) && w.dim[1] <= (1 << 18), who + ": too many rows, classes or features");
 		return LossShape { static_cast<int>(rows), w.dim[1], w.dim[0], size_of(dtype) };
 	}
+	bool few_rows(const LossShape &s)
+	{
+		return takes_few_rows(s.rows, static_cast<size_t>(s.classes) * s.features * s.element_size, s.element_size);
+	}
 	constexpr size_t PIECE_BYTES = size_t(1) << 28;
 	/* classes of a piece: whole tiles, all pieces about the same */
 	int classes_of_piece(const LossShape &s)
@@ -458,7 +462,7 @@ namespace
 		{
 			const int pieces = 16 / s.element_size;
 			const size_t padded = (s.features % pieces == 0) ? 0 : round_up(s.features, pieces) * s.element_size;
-			const bool few = s.rows <= MOST_FEW_ROWS;
+			const bool few = few_rows(s);
 			/* the forward pass's pieces lie in the same places as far as both have them: one workspace serves both */
 			space.x = take(backward || !few ? padded * s.rows : 0);
 			space.w = take(backward || !few ? padded * s.classes : 0);
@@ -492,19 +496,14 @@ namespace
 		Partial *partials = reinterpret_cast<Partial*>(workspace + space.partials);
 		float *target_logits = reinterpret_cast<float*>(workspace + space.target_logits);
 		int columns;
-		if (s.rows <= MOST_FEW_ROWS)
+		if (few_rows(s))
 		{
 			columns = ceil_div(s.classes, FEW_CLASSES);
-			const auto launch = [&](auto kernel)
+			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto waves)
 			{
-				hipLaunchKernelGGL(kernel, dim3(columns), dim3(256), 0, stream, x, w, bias, targets, s.rows, s.features, s.classes, partials, target_logits);
-			};
-			if (s.rows <= 16)
-				launch(kernel_loss_few_rows<T, 1>);
-			else if (s.rows <= 32)
-				launch(kernel_loss_few_rows<T, 2>);
-			else
-				launch(kernel_loss_few_rows<T, 4>);
+				constexpr int MB = decltype(blocks)::value, WAVES = decltype(waves)::value;
+				hipLaunchKernelGGL((kernel_loss_few_rows<T, MB, WAVES>), dim3(columns), dim3(64 * WAVES), 0, stream, x, w, bias, targets, s.rows, s.features, s.classes, partials, target_logits);
+			});
 		}
 		else
 		{

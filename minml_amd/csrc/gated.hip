@@ -233,17 +233,17 @@ namespace
 			finish_element(g, u, row, n, bias, y, projections, hidden, gate);
 		}
 	}
-	template<typename T, int MB>
-	__global__ __launch_bounds__(256) void kernel_gated_few_rows(const T *x, const T *w, T *y, int rows, int hidden, int features, const T *bias, T *projections, int gate)
+	template<typename T, int MB, int WAVES>
+	__global__ __launch_bounds__(64 * WAVES) void kernel_gated_few_rows(const T *x, const T *w, T *y, int rows, int hidden, int features, const T *bias, T *projections, int gate)
 	{
-		__shared__ __attribute__((aligned(16))) float sums[2][16 * MB][16];
+		__shared__ __attribute__((aligned(16))) float sums[WAVES][2][16 * MB][16];
 		const int n0 = blockIdx.x * 16, last = min(15, hidden - 1 - n0);
-		few_rows_sums<T, MB>(x, rows, w + static_cast<size_t>(n0) * features, w + (static_cast<size_t>(hidden) + n0) * features, last, last, features, sums);
-		for (int i = threadIdx.x; i < 16 * MB * 16; i += 256)
+		few_rows_sums<T, MB, WAVES>(x, rows, w + static_cast<size_t>(n0) * features, w + (static_cast<size_t>(hidden) + n0) * features, last, last, features, sums);
+		for (int i = threadIdx.x; i < 16 * MB * 16; i += 64 * WAVES)
 		{
 			const int row = i >> 4, n = i & 15;
 			if (row < rows && n <= last)
-				finish_element(sums[0][row][n], sums[1][row][n], row, n0 + n, bias, y, projections, hidden, gate);
+				finish_element(sums[0][0][row][n], sums[0][1][row][n], row, n0 + n, bias, y, projections, hidden, gate);
 		}
 	}
 
@@ -349,6 +349,10 @@ namespace
 				who + ": too many rows, hidden units or features");
 		return GatedShape { static_cast<int>(rows), w.dim[2], w.dim[1], size_of(dtype), dtype };
 	}
+	bool few_rows(const GatedShape &s)
+	{
+		return takes_few_rows(s.rows, 2 * static_cast<size_t>(s.hidden) * s.features * s.element_size, s.element_size);
+	}
 	int gradient_parts(const GatedShape &s)
 	{
 		/* about 8 workgroups of 256 threads per compute unit */
@@ -383,7 +387,7 @@ namespace
 		};
 		const int pieces = 16 / s.element_size;
 		const size_t padded = (s.features % pieces == 0) ? 0 : round_up(s.features, pieces) * s.element_size;
-		const bool tiles = backward || s.rows > MOST_FEW_ROWS;
+		const bool tiles = backward || !few_rows(s);
 		space.x = take(tiles ? padded * s.rows : 0);
 		space.w = take(tiles ? padded * 2 * s.hidden : 0);
 		if (backward)
@@ -404,19 +408,14 @@ namespace
 	template<typename T>
 	void gated_forward(hipStream_t stream, const GatedShape &s, const T *x, const T *w, const T *bias, T *y, T *projections, int gate, uint8_t *workspace)
 	{
-		if (s.rows <= MOST_FEW_ROWS)
+		if (few_rows(s))
 		{
-			const dim3 grid(ceil_div(s.hidden, 16));
-			const auto launch = [&](auto kernel)
+			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto waves)
 			{
-				hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, w, y, s.rows, s.hidden, s.features, bias, projections, gate);
-			};
-			if (s.rows <= 16)
-				launch(kernel_gated_few_rows<T, 1>);
-			else if (s.rows <= 32)
-				launch(kernel_gated_few_rows<T, 2>);
-			else
-				launch(kernel_gated_few_rows<T, 4>);
+				constexpr int MB = decltype(blocks)::value, WAVES = decltype(waves)::value;
+				hipLaunchKernelGGL((kernel_gated_few_rows<T, MB, WAVES>), dim3(ceil_div(s.hidden, 16)), dim3(64 * WAVES), 0, stream, x, w, y, s.rows, s.hidden, s.features, bias, projections,
+						gate);
+			});
 			MLHIP_CHECK(hipGetLastError());
 			return;
 		}
