@@ -114,6 +114,11 @@ namespace
 			float *target_logits;
 			int classes, tiles_n;
 
+			template<int BM>
+			static constexpr int lds()
+			{
+				return (BM / 64) * BM * static_cast<int>(sizeof(Partial));
+			}
 			/* in registers: a lane has 32 columns of every of its rows, the lane 32 further the other 32 of the wavefront; the wavefronts of a row meet in LDS */
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
@@ -307,6 +312,11 @@ namespace
 			float *sums; /* [row tiles][classes of the piece], or null */
 			int first_class, classes, row_elements; /* classes: of the piece */
 
+			template<int BM>
+			static constexpr int lds()
+			{
+				return Stage<T, BM>::bytes(sizeof(T) == 2 ? BM : PANEL);
+			}
 			/* in registers, rounded there; through LDS to whole rows. The column sums of a wavefront's 64 rows are folded so that each of 32 lanes ends up with one column of each block */
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
@@ -430,17 +440,18 @@ namespace
 		const size_t pieces = (s.classes + most - 1) / most;
 		return static_cast<int>(std::min<size_t>(round_up((s.classes + pieces - 1) / pieces, 256), s.classes));
 	}
-	ProductPlan logits_plan(const LossShape &s, int classes)
+	/* of the forward pass and of the backward pass, whose epilogue lays out a tile of d */
+	ProductPlan logits_plan(const LossShape &s, int classes, bool backward)
 	{
-		return plan_product(s.rows, classes, false, s.features, s.element_size, false);
+		return plan_product(s.rows, classes, false, s.features, s.element_size, false, !backward || s.element_size == 2);
 	}
 	ProductPlan input_plan(const LossShape &s, int classes)
 	{
-		return plan_product(s.rows, s.features, false, classes, s.element_size, true);
+		return plan_product(s.rows, s.features, false, classes, s.element_size, true, false);
 	}
 	ProductPlan weights_plan(const LossShape &s, int classes)
 	{
-		return plan_product(classes, s.features, false, s.rows, s.element_size, true);
+		return plan_product(classes, s.features, false, s.rows, s.element_size, true, false);
 	}
 	struct LossSpace
 	{
@@ -467,7 +478,7 @@ namespace
 			space.x = take(backward || !few ? padded * s.rows : 0);
 			space.w = take(backward || !few ? padded * s.classes : 0);
 			const size_t begin = at;
-			const size_t columns = few ? ceil_div(s.classes, FEW_CLASSES) : logits_plan(s, s.classes).tiles_n;
+			const size_t columns = few ? ceil_div(s.classes, FEW_CLASSES) : logits_plan(s, s.classes, false).tiles_n;
 			space.partials = take(sizeof(Partial) * columns * s.rows);
 			space.target_logits = take(sizeof(float) * s.rows);
 			if (backward)
@@ -479,7 +490,7 @@ namespace
 				space.d = take(round_up(classes, pieces) * s.element_size * s.rows);
 				space.dx = take((classes < s.classes || input.parts > 1) ? sizeof(float) * input.parts * s.rows * s.features : 0);
 				space.parts = take(part_bytes(weights, classes, s.features));
-				space.sums = take(sizeof(float) * classes * logits_plan(s, classes).tiles_m);
+				space.sums = take(sizeof(float) * classes * logits_plan(s, classes, true).tiles_m);
 				space.factors = take(sizeof(float) * s.rows);
 				space.scale = take(sizeof(float) * (SCALE_GROUPS + 1));
 				at = std::max(at, forward_end);
@@ -510,7 +521,7 @@ namespace
 			const int padded = padded_columns<T>(s.features);
 			x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
 			w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
-			const ProductPlan plan = logits_plan(s, s.classes);
+			const ProductPlan plan = logits_plan(s, s.classes, false);
 			columns = plan.tiles_n;
 			const Operand a { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), s.rows, padded };
 			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), s.classes, padded };
@@ -548,7 +559,7 @@ namespace
 			const int classes = std::min(most, s.classes - first), row_elements = padded_columns<T>(classes);
 			const uint8_t *weights = reinterpret_cast<const uint8_t*>(w) + first * row_bytes;
 			{
-				ProductPlan plan = logits_plan(s, most);
+				ProductPlan plan = logits_plan(s, most, true);
 				plan.tiles_n = ceil_div(classes, plan.tile);
 				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
 				const Operand b { weights, row_bytes, classes, padded };

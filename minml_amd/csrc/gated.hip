@@ -93,6 +93,11 @@ namespace
 			const T *bias;
 			int hidden, gate;
 
+			template<int BM>
+			static constexpr int lds()
+			{
+				return Stage<T, BM / 2>::bytes(sizeof(T) == 2 ? BM : PANEL);
+			}
 			/*
 			 * The gate is applied in registers (blocks (i, 0) and (i, 1) hold both projections of an element). The results leave one after the other through the same place in LDS: y, then both projections
 			 * where they are kept.
@@ -176,6 +181,11 @@ namespace
 			size_t part_stride;
 			int hidden;
 
+			template<int BM>
+			static constexpr int lds()
+			{
+				return Stage<float, BM / 2>::bytes(PANEL);
+			}
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
@@ -360,15 +370,15 @@ namespace
 	}
 	ProductPlan forward_plan(const GatedShape &s)
 	{
-		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true);
+		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true, true);
 	}
 	ProductPlan input_plan(const GatedShape &s)
 	{
-		return plan_product(s.rows, s.features, false, 2 * s.hidden, s.element_size, true);
+		return plan_product(s.rows, s.features, false, 2 * s.hidden, s.element_size, true, false);
 	}
 	ProductPlan weights_plan(const GatedShape &s)
 	{
-		return plan_product(2 * s.hidden, s.features, false, s.rows, s.element_size, true);
+		return plan_product(2 * s.hidden, s.features, false, s.rows, s.element_size, true, false);
 	}
 	/* the pieces of a workspace, each aligned to 256 bytes */
 	struct GatedSpace

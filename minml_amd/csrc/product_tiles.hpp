@@ -16,7 +16,8 @@
  *
  * 256x256 (8 wavefronts, one workgroup per compute unit): two slots of four panels, refilled panel by panel: the wavefront's 128 x 64 share is multiplied in four phases of 64 x 32, and a panel's place
  * takes the chunk after the next one as soon as its last phase is over, so a load has six phases (one and a half chunks of 64 k) to arrive.
- * 128x128 (4 wavefronts, two workgroups per compute unit, which hide each other's waits): where 256x256 tiles would leave units without work.
+ * 128x128 (4 wavefronts): where 256x256 tiles would leave units without work, with two slots and two workgroups per compute unit; and where k is so short that a tile is mostly beginning and end, with one
+ * slot and four workgroups per unit, which hide each other's waits.
  * A product with a long k and few tiles is split along k (gridDim.y): each part leaves its sums in fp32, and a launch of its own adds them up in order.
  *
  * The tile's accumulators pass through LDS in fp32, 128 rows at a time, so that the epilogue sees 8 consecutive columns per thread and whole lines per wavefront.
@@ -485,8 +486,8 @@ namespace mlhip
 		epilogue.template tile<256>(acc, TilePlace<256> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
 	}
 
-	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
-	__global__ __launch_bounds__(256, 2) void kernel_product_128(ProductArgs p, Epilogue epilogue)
+	template<typename T, Side SA, Side SB, bool PAIRED, int SLOTS, typename Epilogue>
+	__global__ __launch_bounds__(256, SLOTS == 1 ? 4 : 2) void kernel_product_128(ProductArgs p, Epilogue epilogue)
 	{
 		typedef MfmaTraits<T> Traits;
 		typedef typename Traits::acc_vec acc_vec;
@@ -509,7 +510,7 @@ namespace mlhip
 		b_walk.begin(p.b, n0, first_chunk, chunks);
 		const auto request = [&](int chunk) __attribute__((always_inline))
 		{
-			uint8_t *slot = lds + (chunk & 1) * SLOT;
+			uint8_t *slot = lds + chunk % SLOTS * SLOT;
 			a_loads.request(a_walk.base, a_walk.left, slot);
 			b_loads.request(b_walk.base, b_walk.left, slot + PANEL_BYTES);
 			a_walk.advance();
@@ -536,12 +537,19 @@ namespace mlhip
 			request(0);
 		for (int c = 0; c < chunks; c++)
 		{
-			wait_lgkmcnt<0>(); /* this wavefront's reads of the other slot are complete before anyone may overwrite it */
+			wait_lgkmcnt<0>(); /* this wavefront's reads of the chunk before are complete before anyone may overwrite its place */
+			if constexpr (SLOTS == 1)
+				if (c > 0)
+				{
+					barrier_no_fence();
+					request(c);
+				}
 			wait_vmcnt<0>();
 			barrier_no_fence();
-			if (c + 1 < chunks)
-				request(c + 1);
-			const uint8_t *slot = lds + (c & 1) * SLOT;
+			if constexpr (SLOTS == 2)
+				if (c + 1 < chunks)
+					request(c + 1);
+			const uint8_t *slot = lds + c % SLOTS * SLOT;
 #pragma unroll
 			for (int kk = 0; kk < 4; kk++)
 			{
@@ -561,30 +569,35 @@ namespace mlhip
 		}
 		epilogue.template tile<128>(acc, TilePlace<128> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
 	}
-	/* slots, or what an epilogue lays out there: 128 rows of fp32 or a whole tile of fp16 */
-	constexpr int PRODUCT_LDS_256 = std::max(8 * PANEL_BYTES, std::max(Stage<float, 256>::bytes(PANEL), Stage<half_t, 256>::bytes(256)));
-	constexpr int PRODUCT_LDS_128 = std::max(4 * PANEL_BYTES, std::max(Stage<float, 128>::bytes(PANEL), Stage<half_t, 128>::bytes(PANEL)));
-	static_assert(PRODUCT_LDS_256 <= 160 * 1024 && 2 * PRODUCT_LDS_128 <= 160 * 1024, "tiles must fit the LDS of a compute unit");
+	/* slots, or what an epilogue lays out there: Epilogue::lds<BM>() bytes */
+	template<typename Epilogue>
+	constexpr int product_lds(int tile, int slots)
+	{
+		return tile == 256 ? std::max(8 * PANEL_BYTES, Epilogue::template lds<256>()) : std::max(2 * slots * PANEL_BYTES, Epilogue::template lds<128>());
+	}
+	constexpr int LDS_OF_A_UNIT = 160 * 1024;
 
 	/* how a product is cut: tiles of `tile` rows and columns, `parts` along k. A workspace is sized by the same rule, so it asks no device */
 	struct ProductPlan
 	{
-			int tile, tiles_m, tiles_n, chunks, parts, chunks_per_part;
+			int tile, slots, tiles_m, tiles_n, chunks, parts, chunks_per_part;
 	};
 	/*
 	 * The cheapest of both tile sizes and up to 16 parts, by what they take: a compute unit works off its tiles one after the other (two of 128x128 side by side take as long as one after the other), a tile takes
 	 * so long per chunk and something for its beginning and end, and parts have to be added up. Microseconds on a full chip, fp16 / fp32: a chunk of 256x256 1.7 / 8.4 (1.2 where at most half of the units have
-	 * a tile: what they read then comes faster), of 128x128 0.6 / 2.05 (its operands' way out of the L2 bounds it in fp16: 32 KB, 30 bytes per clock and unit). Measured, two sides each: dx of 4096 x 2048, k = 16384, fp16
-	 * (128 tiles of 256x256) whole 313, in 2 parts 228, 128x128 tiles 310; dW of 11008 x 2048, k = 8192, fp16 (344 tiles) 388, 385, 379; 2048 x 1024, k = 8192, fp16 143, 87, 79, 128x128 in 2 parts
-	 * 53; dW of 5462 x 1000, k = 1111, fp32 270, 160, 147, 128x128 in 2 parts 127.
-	 * columns: of the result (of one of the two matrices where the operand is paired)
+	 * a tile: what they read then comes faster), of 128x128 0.6 / 2.05 (its operands' way out of the L2 bounds it in fp16: 32 KB, 30 bytes per clock and unit), and where there are four workgroups to
+	 * every unit, which one slot each lets in, 0.5 and hardly any beginning and end. Measured, two sides each: dx of 4096 x 2048, k = 16384, fp16 (128 tiles of 256x256) whole 313, in 2 parts 228, 128x128 tiles 310; dW of
+	 * 11008 x 2048, k = 8192, fp16 (344 tiles) 388, 385, 379; 2048 x 1024, k = 8192, fp16 143, 87, 79, 128x128 in 2 parts 53; dW of 5462 x 1000, k = 1111, fp32 270, 160, 147, 128x128 in 2 parts 127. 57600 rows
+	 * -> 2 x 1024 columns fp16, 256x256 / 128x128 with two slots / with one: k = 256 118 / 118 / 105, both projections kept 146 / 146 / 121, k = 512 160 / 179 / 157, k = 1024 264 / 298 / 277; 512 rows, k = 1024 -> 2 x 4096
+	 * 26 / 17 / 20.
+	 * columns: of the result (of one of the two matrices where the operand is paired). one_slot: whether the epilogue gets by with a fourth of a unit's LDS
 	 */
-	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split)
+	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split, bool one_slot)
 	{
 		constexpr int UNITS = 256;
 		const bool half = element_size == 2;
 		const int chunks = ceil_div(depth, 128 / element_size);
-		ProductPlan best { 256, 0, 0, chunks, 1, std::max(1, chunks) };
+		ProductPlan best { 256, 2, 0, 0, chunks, 1, std::max(1, chunks) };
 		double least = 0.0;
 		for (int tile : { 256, 128 })
 		{
@@ -596,15 +609,21 @@ namespace mlhip
 				const int per_part = std::max(1, ceil_div(chunks, parts));
 				if (parts > 1 && ceil_div(chunks, per_part) != parts)
 					continue;
-				const double turns = std::ceil(tiles * parts / UNITS);
-				const double chunk = tile == 128 ? (half ? 0.6 : 2.05) : (half ? (tiles * parts <= UNITS / 2 ? 1.2 : 1.7) : 8.4);
-				double cost = turns * ((tile == 128 ? 4.0 : 8.0) + per_part * chunk);
+				const double work = tiles * parts / UNITS;
+				const int slots = (tile == 128 && one_slot && work >= 4.0) ? 1 : 2;
+				double cost;
+				if (tile == 256)
+					cost = std::ceil(work) * (7.0 + per_part * (half ? (work <= 0.5 ? 1.2 : 1.7) : 8.4));
+				else if (slots == 2)
+					cost = std::ceil(work) * (4.0 + per_part * (half ? 0.6 : 2.05));
+				else
+					cost = work * (1.8 + per_part * (half ? 0.5 : 2.05));
 				if (parts > 1)
 					cost += 6.0 + 8e-6 / 5.0 * parts * rows * (paired ? 2.0 : 1.0) * columns; /* written and read at 5 TB/s */
 				if (least == 0.0 || cost < least)
 				{
 					least = cost;
-					best = ProductPlan { tile, tiles_m, tiles_n, chunks, parts, per_part };
+					best = ProductPlan { tile, slots, tiles_m, tiles_n, chunks, parts, per_part };
 				}
 			}
 		}
@@ -619,18 +638,31 @@ namespace mlhip
 		const long long tiles = static_cast<long long>(plan.tiles_m) * plan.tiles_n;
 		MLHIP_REQUIRE(tiles <= 0x7fffffff && plan.parts <= 65535 && a.row_bytes < (1u << 22) && b.row_bytes < (1u << 22), "product too large");
 		const dim3 grid(static_cast<unsigned int>(tiles), plan.parts);
+		static_assert(product_lds<Epilogue>(256, 2) <= LDS_OF_A_UNIT && product_lds<Epilogue>(128, 2) <= LDS_OF_A_UNIT / 2, "tiles must fit the LDS of a compute unit");
+		constexpr bool ONE_SLOT = product_lds<Epilogue>(128, 1) <= LDS_OF_A_UNIT / 4;
 		if (plan.tile == 256)
 		{
+			constexpr int bytes = product_lds<Epilogue>(256, 2);
 			auto kernel = kernel_product_256<T, SA, SB, PAIRED, Epilogue>;
-			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), PRODUCT_LDS_256);
-			hipLaunchKernelGGL(kernel, grid, dim3(512), PRODUCT_LDS_256, stream, args, epilogue);
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+			hipLaunchKernelGGL(kernel, grid, dim3(512), bytes, stream, args, epilogue);
+		}
+		else if (plan.slots == 2)
+		{
+			constexpr int bytes = product_lds<Epilogue>(128, 2);
+			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 2, Epilogue>;
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
+		}
+		else if constexpr (ONE_SLOT)
+		{
+			constexpr int bytes = product_lds<Epilogue>(128, 1);
+			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 1, Epilogue>;
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
 		}
 		else
-		{
-			auto kernel = kernel_product_128<T, SA, SB, PAIRED, Epilogue>;
-			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), PRODUCT_LDS_128);
-			hipLaunchKernelGGL(kernel, grid, dim3(256), PRODUCT_LDS_128, stream, args, epilogue);
-		}
+			fail_logic("HIP backend: a product was planned for less LDS than its epilogue takes");
 		MLHIP_CHECK(hipGetLastError());
 	}
 
@@ -643,6 +675,11 @@ namespace mlhip
 			float beta;
 			const float *scale; /* on the device; null: 1 */
 
+			template<int BM>
+			static constexpr int lds()
+			{
+				return std::max(Stage<float, BM>::bytes(PANEL), sizeof(Out) == 2 ? Stage<Out, BM>::bytes(BM) : 0);
+			}
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
@@ -701,6 +738,11 @@ namespace mlhip
 			int columns;
 			bool add;
 
+			template<int BM>
+			static constexpr int lds()
+			{
+				return Stage<float, BM>::bytes(PANEL);
+			}
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
