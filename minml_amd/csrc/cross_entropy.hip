@@ -77,12 +77,7 @@ namespace
 				for (int j = 0; j < 2; j++)
 				{
 					first[j] = at.tile_n * BM + at.column(j);
-#pragma unroll
-					for (int r = 0; r < 16; r++)
-					{
-						const int n = column(j, r);
-						bias[j][r] = (values != nullptr && n < classes) ? static_cast<float>(values[n]) : 0.0f;
-					}
+					load_lane_bias(bias[j], values, first[j], classes);
 				}
 			}
 			__device__ __forceinline__ int column(int j, int r) const
@@ -315,13 +310,13 @@ namespace
 			template<int BM>
 			static constexpr int lds()
 			{
-				return Stage<T, BM>::bytes(sizeof(T) == 2 ? BM : PANEL);
+				return Stage<T, BM>::bytes(sizeof(T) == 2 ? BM : BM / 2);
 			}
 			/* in registers, rounded there; through LDS to whole rows. The column sums of a wavefront's 64 rows are folded so that each of 32 lanes ends up with one column of each block */
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
 			{
-				constexpr int BLOCKS = TilePlace<BM>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : PANEL, PASSES = BM / ROWS;
+				constexpr int BLOCKS = TilePlace<BM>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : BM / 2, PASSES = BM / ROWS;
 				TileColumns<T, BM> columns;
 				columns.begin(at, bias, classes);
 				const bool edge = (at.tile_n + 1) * BM > classes;
@@ -428,9 +423,14 @@ namespace
 		MLHIP_REQUIRE(rows <= (1 << 28) && w.dim[0] <= (1 << 28) && w.dim[1] <= (1 << 18), who + ": too many rows, classes or features");
 		return LossShape { static_cast<int>(rows), w.dim[1], w.dim[0], size_of(dtype) };
 	}
+	/*
+	 * Here a tile per compute unit reads the weights faster than the few-rows kernel, and nothing is split: in fp16 tiles are taken from 256 column tiles on (us, few rows / tiles: 1 row of 2048 x 65536 classes 55 / 43,
+	 * 16 rows 70 / 45; of 1024 x 30000 18 / 20 and 21 / 21), in fp32 from 33 rows on (64 rows of 2048 x 65536 332 / 256, 16 rows 131 / 261).
+	 */
 	bool few_rows(const LossShape &s)
 	{
-		return takes_few_rows(s.rows, static_cast<size_t>(s.classes) * s.features * s.element_size, s.element_size);
+		const bool enough_tiles = (s.element_size == 2) ? ceil_div(s.classes, 128) >= 256 : s.rows > 32;
+		return !enough_tiles && takes_few_rows(s.rows, static_cast<size_t>(s.classes) * s.features * s.element_size, s.element_size);
 	}
 	constexpr size_t PIECE_BYTES = size_t(1) << 28;
 	/* classes of a piece: whole tiles, all pieces about the same */
@@ -440,18 +440,17 @@ namespace
 		const size_t pieces = (s.classes + most - 1) / most;
 		return static_cast<int>(std::min<size_t>(round_up((s.classes + pieces - 1) / pieces, 256), s.classes));
 	}
-	/* of the forward pass and of the backward pass, whose epilogue lays out a tile of d */
-	ProductPlan logits_plan(const LossShape &s, int classes, bool backward)
+	ProductPlan logits_plan(const LossShape &s, int classes)
 	{
-		return plan_product(s.rows, classes, false, s.features, s.element_size, false, !backward || s.element_size == 2);
+		return plan_product(s.rows, classes, false, s.features, s.element_size, false);
 	}
 	ProductPlan input_plan(const LossShape &s, int classes)
 	{
-		return plan_product(s.rows, s.features, false, classes, s.element_size, true, false);
+		return plan_product(s.rows, s.features, false, classes, s.element_size, true);
 	}
 	ProductPlan weights_plan(const LossShape &s, int classes)
 	{
-		return plan_product(classes, s.features, false, s.rows, s.element_size, true, false);
+		return plan_product(classes, s.features, false, s.rows, s.element_size, true);
 	}
 	struct LossSpace
 	{
@@ -478,7 +477,7 @@ namespace
 			space.x = take(backward || !few ? padded * s.rows : 0);
 			space.w = take(backward || !few ? padded * s.classes : 0);
 			const size_t begin = at;
-			const size_t columns = few ? ceil_div(s.classes, FEW_CLASSES) : logits_plan(s, s.classes, false).tiles_n;
+			const size_t columns = few ? ceil_div(s.classes, FEW_CLASSES) : logits_plan(s, s.classes).tiles_n;
 			space.partials = take(sizeof(Partial) * columns * s.rows);
 			space.target_logits = take(sizeof(float) * s.rows);
 			if (backward)
@@ -490,7 +489,7 @@ namespace
 				space.d = take(round_up(classes, pieces) * s.element_size * s.rows);
 				space.dx = take((classes < s.classes || input.parts > 1) ? sizeof(float) * input.parts * s.rows * s.features : 0);
 				space.parts = take(part_bytes(weights, classes, s.features));
-				space.sums = take(sizeof(float) * classes * logits_plan(s, classes, true).tiles_m);
+				space.sums = take(sizeof(float) * classes * logits_plan(s, classes).tiles_m);
 				space.factors = take(sizeof(float) * s.rows);
 				space.scale = take(sizeof(float) * (SCALE_GROUPS + 1));
 				at = std::max(at, forward_end);
@@ -521,7 +520,7 @@ namespace
 			const int padded = padded_columns<T>(s.features);
 			x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
 			w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
-			const ProductPlan plan = logits_plan(s, s.classes, false);
+			const ProductPlan plan = logits_plan(s, s.classes);
 			columns = plan.tiles_n;
 			const Operand a { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), s.rows, padded };
 			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), s.classes, padded };
@@ -559,7 +558,7 @@ namespace
 			const int classes = std::min(most, s.classes - first), row_elements = padded_columns<T>(classes);
 			const uint8_t *weights = reinterpret_cast<const uint8_t*>(w) + first * row_bytes;
 			{
-				ProductPlan plan = logits_plan(s, most, true);
+				ProductPlan plan = logits_plan(s, most);
 				plan.tiles_n = ceil_div(classes, plan.tile);
 				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
 				const Operand b { weights, row_bytes, classes, padded };

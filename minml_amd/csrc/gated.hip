@@ -28,27 +28,24 @@ namespace
 			return 1.0f / (1.0f + expf(-g));
 	}
 	/*
-	 * The normal distribution's integral, 0.5 erfc(-g / sqrt 2). For fp16 erfc(z) exp(z^2) / t is a polynomial of degree 6 in t = 1 / (1 + 0.37 z), fitted to the smallest relative error over
-	 * z = 0 .. 7 (3.7e-7, 7e-7 in 32 bits): the tail, where gelu is small, is as exact as the rest, with a dozen instructions instead of the 60 of the library's erfc, which fp32 takes.
+	 * The normal distribution's integral up to -|g|, 0.5 erfc(|g| / sqrt 2). For fp16 erfc(z) exp(z^2) / t is a polynomial of degree 5 in t = 1 / (1 + 0.43 z), fitted to the smallest relative error over
+	 * z = 0 .. 7 (2.5e-6): the tail, where gelu is small, is as exact as the rest, with a dozen instructions instead of the 60 of the library's erfc, which fp32 takes.
 	 */
 	template<typename T>
-	__device__ __forceinline__ float normal_integral(float g)
+	__device__ __forceinline__ float normal_tail(float g)
 	{
 		if constexpr (sizeof(T) == 2)
 		{
-			const float z = fabsf(g) * 0.70710678118654752f;
-			const float t = __builtin_amdgcn_rcpf(fmaf(0.37f, z, 1.0f));
-			float poly = fmaf(t, -0.14591303f, 0.44789582f);
-			poly = fmaf(t, poly, -0.20436039f);
-			poly = fmaf(t, poly, 0.33090103f);
-			poly = fmaf(t, poly, 0.14716733f);
-			poly = fmaf(t, poly, 0.21602353f);
-			poly = fmaf(t, poly, 0.20828535f);
-			const float tail = 0.5f * t * poly * __expf(-z * z);
-			return g < 0.0f ? tail : 1.0f - tail;
+			const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.43f * 0.70710678118654752f, 1.0f));
+			float poly = fmaf(t, -0.078892514f, 0.21006414f);
+			poly = fmaf(t, poly, -0.012823527f);
+			poly = fmaf(t, poly, 0.14469013f);
+			poly = fmaf(t, poly, 0.11523368f);
+			poly = fmaf(t, poly, 0.12172684f);
+			return t * poly * __builtin_amdgcn_exp2f(g * g * -0.72134752044448170f); /* exp(-g^2 / 2) */
 		}
 		else
-			return 0.5f * erfcf(g * -0.70710678118654752f);
+			return 0.5f * erfcf(fabsf(g) * 0.70710678118654752f);
 	}
 	/* a(g) and, if asked, its derivative */
 	template<typename T, bool SLOPE>
@@ -76,10 +73,10 @@ namespace
 			}
 			default: /* GATE_GELU */
 			{
-				const float p = normal_integral<T>(g);
-				a = g * p;
+				const float tail = normal_tail<T>(g);
+				a = fmaf(-fminf(fabsf(g), 3.0e38f), tail, fmaxf(g, 0.0f)); /* g P(g) for either sign, +inf for +inf */
 				if (SLOPE)
-					slope = fmaf(g * 0.39894228040143268f, (sizeof(T) == 2) ? __expf(-0.5f * g * g) : expf(-0.5f * g * g), p);
+					slope = fmaf(g * 0.39894228040143268f, (sizeof(T) == 2) ? __expf(-0.5f * g * g) : expf(-0.5f * g * g), g < 0.0f ? tail : 1.0f - tail);
 				break;
 			}
 		}
@@ -111,14 +108,7 @@ namespace
 				float shift[2][16];
 #pragma unroll
 				for (int j = 0; j < 2; j++)
-#pragma unroll
-					for (int q = 0; q < 4; q++)
-#pragma unroll
-						for (int e = 0; e < 4; e++)
-						{
-							const int n = n0 + at.wave_n * 32 + at.lane_column(q) + e;
-							shift[j][4 * q + e] = (bias != nullptr && n < hidden) ? static_cast<float>(bias[j * hidden + n]) : 0.0f;
-						}
+					load_lane_bias(shift[j], bias != nullptr ? bias + j * hidden : nullptr, n0 + at.wave_n * 32, hidden);
 				static_for<PASSES>([&](auto pass)
 				{
 					constexpr int first = decltype(pass)::value * BLOCKS;
@@ -370,15 +360,15 @@ namespace
 	}
 	ProductPlan forward_plan(const GatedShape &s)
 	{
-		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true, true);
+		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true);
 	}
 	ProductPlan input_plan(const GatedShape &s)
 	{
-		return plan_product(s.rows, s.features, false, 2 * s.hidden, s.element_size, true, false);
+		return plan_product(s.rows, s.features, false, 2 * s.hidden, s.element_size, true);
 	}
 	ProductPlan weights_plan(const GatedShape &s)
 	{
-		return plan_product(2 * s.hidden, s.features, false, s.rows, s.element_size, true, false);
+		return plan_product(2 * s.hidden, s.features, false, s.rows, s.element_size, true);
 	}
 	/* the pieces of a workspace, each aligned to 256 bytes */
 	struct GatedSpace

@@ -245,6 +245,36 @@ namespace mlhip
 				return 8 * q + 4 * ((threadIdx.x >> 5) & 1);
 			}
 	};
+	/* the bias of a lane's 16 columns of a block that begins at column n0 of the result; zeros where there is none, and behind the last column */
+	template<typename T>
+	__device__ __forceinline__ void load_lane_bias(float (&out)[16], const T *bias, int n0, int columns)
+	{
+#pragma unroll
+		for (int r = 0; r < 16; r++)
+			out[r] = 0.0f;
+		if (bias == nullptr)
+			return;
+		const int lane_column = n0 + 4 * ((threadIdx.x >> 5) & 1);
+		if (n0 + 32 <= columns)
+		{
+			Elements<T, 4> v[4];
+#pragma unroll
+			for (int q = 0; q < 4; q++)
+				v[q].load(bias + lane_column + 8 * q);
+#pragma unroll
+			for (int q = 0; q < 4; q++)
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					out[4 * q + e] = v[q][e];
+		}
+		else
+#pragma unroll
+			for (int q = 0; q < 4; q++)
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					if (lane_column + 8 * q + e < columns)
+						out[4 * q + e] = static_cast<float>(bias[lane_column + 8 * q + e]);
+	}
 	/*
 	 * A tile (or the rows of it that lie in LDS) to memory, 16 bytes per thread and whole rows by neighbouring threads. f(m, n, LDS place, elements): elements of the vector that exist, all of them or fewer at the
 	 * matrix's edge.
@@ -295,27 +325,28 @@ namespace mlhip
 				});
 			}
 	};
-	/* the sums of a tile through LDS in fp32, 128 rows at a time: f(m, n, 4 sums in LDS, elements) */
+	/* the sums of a tile through LDS in fp32, half its rows at a time: f(m, n, 4 sums in LDS, elements) */
 	template<int BM, typename Acc, typename F>
 	__device__ __forceinline__ void sums_in_rows(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows, int columns, F &&f)
 	{
+		constexpr int ROWS = BM / 2, BLOCKS = TilePlace<BM>::BLOCKS / 2;
 		const Stage<float, BM> stage { reinterpret_cast<float*>(lds) };
-		static_for<BM / PANEL>([&](auto half)
+		static_for<2>([&](auto half)
 		{
 			constexpr int h = decltype(half)::value;
 			__syncthreads();
 #pragma unroll
-			for (int i = 0; i < 2; i++)
+			for (int i = h * BLOCKS; i < (h + 1) * BLOCKS; i++)
 #pragma unroll
 				for (int j = 0; j < 2; j++)
 #pragma unroll
 					for (int q = 0; q < 4; q++)
 					{
-						const Acc &v = acc[2 * h + i][j];
-						stage.put(at.row(2 * h + i) - h * PANEL, at.column(j) + at.lane_column(q), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+						const Acc &v = acc[i][j];
+						stage.put(at.row(i) - h * ROWS, at.column(j) + at.lane_column(q), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 					}
 			__syncthreads();
-			stage.template for_vectors<PANEL, TilePlace<BM>::THREADS>(at.tile_m * BM + h * PANEL, rows, at.tile_n * BM, columns, f);
+			stage.template for_vectors<ROWS, TilePlace<BM>::THREADS>(at.tile_m * BM + h * ROWS, rows, at.tile_n * BM, columns, f);
 		});
 	}
 
@@ -584,15 +615,15 @@ namespace mlhip
 	};
 	/*
 	 * The cheapest of both tile sizes and up to 16 parts, by what they take: a compute unit works off its tiles one after the other (two of 128x128 side by side take as long as one after the other), a tile takes
-	 * so long per chunk and something for its beginning and end, and parts have to be added up. Microseconds on a full chip, fp16 / fp32: a chunk of 256x256 1.7 / 8.4 (1.2 where at most half of the units have
+	 * so long per chunk and something for its beginning and end, and parts have to be added up. Microseconds on a full chip, fp16 / fp32: a chunk of 256x256 1.7 / 7.8 (1.2 where at most half of the units have
 	 * a tile: what they read then comes faster), of 128x128 0.6 / 2.05 (its operands' way out of the L2 bounds it in fp16: 32 KB, 30 bytes per clock and unit), and where there are four workgroups to
-	 * every unit, which one slot each lets in, 0.5 and hardly any beginning and end. Measured, two sides each: dx of 4096 x 2048, k = 16384, fp16 (128 tiles of 256x256) whole 313, in 2 parts 228, 128x128 tiles 310; dW of
+	 * every unit, which one slot each lets in, 0.5 / 2.15 and hardly any beginning and end. Measured, two sides each: dx of 4096 x 2048, k = 16384, fp16 (128 tiles of 256x256) whole 313, in 2 parts 228, 128x128 tiles 310; dW of
 	 * 11008 x 2048, k = 8192, fp16 (344 tiles) 388, 385, 379; 2048 x 1024, k = 8192, fp16 143, 87, 79, 128x128 in 2 parts 53; dW of 5462 x 1000, k = 1111, fp32 270, 160, 147, 128x128 in 2 parts 127. 57600 rows
 	 * -> 2 x 1024 columns fp16, 256x256 / 128x128 with two slots / with one: k = 256 118 / 118 / 105, both projections kept 146 / 146 / 121, k = 512 160 / 179 / 157, k = 1024 264 / 298 / 277; 512 rows, k = 1024 -> 2 x 4096
-	 * 26 / 17 / 20.
-	 * columns: of the result (of one of the two matrices where the operand is paired). one_slot: whether the epilogue gets by with a fourth of a unit's LDS
+	 * 26 / 17 / 20; fp32 57600 rows, k = 256 -> 2 x 1024 589 / 551 / 520, 8192 rows, k = 2048 -> 2 x 2048 1011 / 1071 / 1100.
+	 * columns: of the result (of one of the two matrices where the operand is paired)
 	 */
-	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split, bool one_slot)
+	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split)
 	{
 		constexpr int UNITS = 256;
 		const bool half = element_size == 2;
@@ -610,14 +641,20 @@ namespace mlhip
 				if (parts > 1 && ceil_div(chunks, per_part) != parts)
 					continue;
 				const double work = tiles * parts / UNITS;
-				const int slots = (tile == 128 && one_slot && work >= 4.0) ? 1 : 2;
 				double cost;
+				int slots = 2;
 				if (tile == 256)
-					cost = std::ceil(work) * (7.0 + per_part * (half ? (work <= 0.5 ? 1.2 : 1.7) : 8.4));
-				else if (slots == 2)
-					cost = std::ceil(work) * (4.0 + per_part * (half ? 0.6 : 2.05));
+					cost = std::ceil(work) * (7.0 + per_part * (half ? (work <= 0.5 ? 1.2 : 1.7) : 7.8));
 				else
-					cost = work * (1.8 + per_part * (half ? 0.5 : 2.05));
+				{
+					cost = std::ceil(work) * (4.0 + per_part * (half ? 0.6 : 2.05));
+					const double one_slot = work * (1.8 + per_part * (half ? 0.5 : 2.15));
+					if (work >= 4.0 && one_slot < cost)
+					{
+						slots = 1;
+						cost = one_slot;
+					}
+				}
 				if (parts > 1)
 					cost += 6.0 + 8e-6 / 5.0 * parts * rows * (paired ? 2.0 : 1.0) * columns; /* written and read at 5 TB/s */
 				if (least == 0.0 || cost < least)
@@ -638,8 +675,8 @@ namespace mlhip
 		const long long tiles = static_cast<long long>(plan.tiles_m) * plan.tiles_n;
 		MLHIP_REQUIRE(tiles <= 0x7fffffff && plan.parts <= 65535 && a.row_bytes < (1u << 22) && b.row_bytes < (1u << 22), "product too large");
 		const dim3 grid(static_cast<unsigned int>(tiles), plan.parts);
-		static_assert(product_lds<Epilogue>(256, 2) <= LDS_OF_A_UNIT && product_lds<Epilogue>(128, 2) <= LDS_OF_A_UNIT / 2, "tiles must fit the LDS of a compute unit");
-		constexpr bool ONE_SLOT = product_lds<Epilogue>(128, 1) <= LDS_OF_A_UNIT / 4;
+		static_assert(product_lds<Epilogue>(256, 2) <= LDS_OF_A_UNIT && product_lds<Epilogue>(128, 2) <= LDS_OF_A_UNIT / 2 && product_lds<Epilogue>(128, 1) <= LDS_OF_A_UNIT / 4,
+				"tiles must fit the LDS of a compute unit");
 		if (plan.tile == 256)
 		{
 			constexpr int bytes = product_lds<Epilogue>(256, 2);
@@ -654,15 +691,13 @@ namespace mlhip
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
 		}
-		else if constexpr (ONE_SLOT)
+		else
 		{
 			constexpr int bytes = product_lds<Epilogue>(128, 1);
 			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 1, Epilogue>;
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
 		}
-		else
-			fail_logic("HIP backend: a product was planned for less LDS than its epilogue takes");
 		MLHIP_CHECK(hipGetLastError());
 	}
 
@@ -678,7 +713,7 @@ namespace mlhip
 			template<int BM>
 			static constexpr int lds()
 			{
-				return std::max(Stage<float, BM>::bytes(PANEL), sizeof(Out) == 2 ? Stage<Out, BM>::bytes(BM) : 0);
+				return std::max(Stage<float, BM>::bytes(BM / 2), sizeof(Out) == 2 ? Stage<Out, BM>::bytes(BM) : 0);
 			}
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
@@ -741,7 +776,7 @@ namespace mlhip
 			template<int BM>
 			static constexpr int lds()
 			{
-				return Stage<float, BM>::bytes(PANEL);
+				return Stage<float, BM>::bytes(BM / 2);
 			}
 			template<int BM, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
