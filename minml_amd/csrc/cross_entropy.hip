@@ -189,17 +189,23 @@ namespace
 			}
 	};
 	constexpr int FEW_CLASSES = 32; /* of a workgroup of the few-rows kernel */
-	template<typename T, int MB, int WAVES>
-	__global__ __launch_bounds__(64 * WAVES) void kernel_loss_few_rows(const T *x, const T *w, const T *bias, const int *targets, int rows, int features, int classes, Partial *partials,
+	template<typename T, int MB, bool STREAM>
+	__global__ __launch_bounds__(256) void kernel_loss_few_rows(const T *x, const T *w, const T *bias, const int *targets, int rows, int features, int classes, Partial *partials,
 			float *target_logits)
 	{
-		__shared__ __attribute__((aligned(16))) float sums[WAVES][2][16 * MB][16];
+		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+		float (*sums)[2][16 * MB][16] = reinterpret_cast<float (*)[2][16 * MB][16]>(lds);
 		const int n0 = blockIdx.x * FEW_CLASSES;
 		const T *first = w + static_cast<size_t>(n0) * features;
 		const bool second = n0 + 16 < classes; /* else the first block stands in for it */
-		few_rows_sums<T, MB, WAVES>(x, rows, first, second ? first + static_cast<size_t>(16) * features : first, min(15, classes - 1 - n0), min(15, classes - 1 - n0 - (second ? 16 : 0)), features, sums);
+		const int last_first = min(15, classes - 1 - n0), last_second = second ? min(15, classes - 1 - n0 - 16) : last_first;
+		const T *next = second ? first + static_cast<size_t>(16) * features : first;
+		if constexpr (STREAM)
+			few_rows_stream<T, MB>(x, rows, first, next, last_first, last_second, features, lds);
+		else
+			few_rows_sums<T, MB>(x, rows, first, next, last_first, last_second, features, sums);
 		const int c = threadIdx.x & 15;
-		for (int row = threadIdx.x >> 4; row < 16 * MB; row += 4 * WAVES)
+		for (int row = threadIdx.x >> 4; row < 16 * MB; row += 16)
 			if (row < rows)
 			{
 				const int target = targets[row];
@@ -423,14 +429,9 @@ namespace
 		MLHIP_REQUIRE(rows <= (1 << 28) && w.dim[0] <= (1 << 28) && w.dim[1] <= (1 << 18), who + ": too many rows, classes or features");
 		return LossShape { static_cast<int>(rows), w.dim[1], w.dim[0], size_of(dtype) };
 	}
-	/*
-	 * Here a tile per compute unit reads the weights faster than the few-rows kernel, and nothing is split: in fp16 tiles are taken from 256 column tiles on (us, few rows / tiles: 1 row of 2048 x 65536 classes 55 / 43,
-	 * 16 rows 70 / 45; of 1024 x 30000 18 / 20 and 21 / 21), in fp32 from 33 rows on (64 rows of 2048 x 65536 332 / 256, 16 rows 131 / 261).
-	 */
 	bool few_rows(const LossShape &s)
 	{
-		const bool enough_tiles = (s.element_size == 2) ? ceil_div(s.classes, 128) >= 256 : s.rows > 32;
-		return !enough_tiles && takes_few_rows(s.rows, static_cast<size_t>(s.classes) * s.features * s.element_size, s.element_size);
+		return takes_few_rows(s.rows, static_cast<size_t>(s.classes) * s.features * s.element_size);
 	}
 	constexpr size_t PIECE_BYTES = size_t(1) << 28;
 	/* classes of a piece: whole tiles, all pieces about the same */
@@ -509,10 +510,12 @@ namespace
 		if (few_rows(s))
 		{
 			columns = ceil_div(s.classes, FEW_CLASSES);
-			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto waves)
+			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto streamed)
 			{
-				constexpr int MB = decltype(blocks)::value, WAVES = decltype(waves)::value;
-				hipLaunchKernelGGL((kernel_loss_few_rows<T, MB, WAVES>), dim3(columns), dim3(64 * WAVES), 0, stream, x, w, bias, targets, s.rows, s.features, s.classes, partials, target_logits);
+				constexpr int MB = decltype(blocks)::value, bytes = few_rows_lds<MB>(decltype(streamed)::value);
+				auto kernel = kernel_loss_few_rows<T, MB, decltype(streamed)::value>;
+				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+				hipLaunchKernelGGL(kernel, dim3(columns), dim3(256), bytes, stream, x, w, bias, targets, s.rows, s.features, s.classes, partials, target_logits);
 			});
 		}
 		else

@@ -233,13 +233,18 @@ namespace
 			finish_element(g, u, row, n, bias, y, projections, hidden, gate);
 		}
 	}
-	template<typename T, int MB, int WAVES>
-	__global__ __launch_bounds__(64 * WAVES) void kernel_gated_few_rows(const T *x, const T *w, T *y, int rows, int hidden, int features, const T *bias, T *projections, int gate)
+	template<typename T, int MB, bool STREAM>
+	__global__ __launch_bounds__(256) void kernel_gated_few_rows(const T *x, const T *w, T *y, int rows, int hidden, int features, const T *bias, T *projections, int gate)
 	{
-		__shared__ __attribute__((aligned(16))) float sums[WAVES][2][16 * MB][16];
+		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 		const int n0 = blockIdx.x * 16, last = min(15, hidden - 1 - n0);
-		few_rows_sums<T, MB, WAVES>(x, rows, w + static_cast<size_t>(n0) * features, w + (static_cast<size_t>(hidden) + n0) * features, last, last, features, sums);
-		for (int i = threadIdx.x; i < 16 * MB * 16; i += 64 * WAVES)
+		const T *first = w + static_cast<size_t>(n0) * features, *second = w + (static_cast<size_t>(hidden) + n0) * features;
+		float (*sums)[2][16 * MB][16] = reinterpret_cast<float (*)[2][16 * MB][16]>(lds);
+		if constexpr (STREAM)
+			few_rows_stream<T, MB>(x, rows, first, second, last, last, features, lds);
+		else
+			few_rows_sums<T, MB>(x, rows, first, second, last, last, features, sums);
+		for (int i = threadIdx.x; i < 16 * MB * 16; i += 256)
 		{
 			const int row = i >> 4, n = i & 15;
 			if (row < rows && n <= last)
@@ -351,7 +356,7 @@ namespace
 	}
 	bool few_rows(const GatedShape &s)
 	{
-		return takes_few_rows(s.rows, 2 * static_cast<size_t>(s.hidden) * s.features * s.element_size, s.element_size);
+		return takes_few_rows(s.rows, 2 * static_cast<size_t>(s.hidden) * s.features * s.element_size);
 	}
 	int gradient_parts(const GatedShape &s)
 	{
@@ -362,13 +367,13 @@ namespace
 	{
 		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true);
 	}
-	ProductPlan input_plan(const GatedShape &s)
+	TwoPlans input_plan(const GatedShape &s)
 	{
-		return plan_product(s.rows, s.features, false, 2 * s.hidden, s.element_size, true);
+		return plan_in_turns(s.rows, s.features, 2 * s.hidden, s.element_size);
 	}
-	ProductPlan weights_plan(const GatedShape &s)
+	TwoPlans weights_plan(const GatedShape &s)
 	{
-		return plan_product(2 * s.hidden, s.features, false, s.rows, s.element_size, true);
+		return plan_in_turns(2 * s.hidden, s.features, s.rows, s.element_size);
 	}
 	/* the pieces of a workspace, each aligned to 256 bytes */
 	struct GatedSpace
@@ -410,11 +415,12 @@ namespace
 	{
 		if (few_rows(s))
 		{
-			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto waves)
+			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto streamed)
 			{
-				constexpr int MB = decltype(blocks)::value, WAVES = decltype(waves)::value;
-				hipLaunchKernelGGL((kernel_gated_few_rows<T, MB, WAVES>), dim3(ceil_div(s.hidden, 16)), dim3(64 * WAVES), 0, stream, x, w, y, s.rows, s.hidden, s.features, bias, projections,
-						gate);
+				constexpr int MB = decltype(blocks)::value, bytes = few_rows_lds<MB>(decltype(streamed)::value);
+				auto kernel = kernel_gated_few_rows<T, MB, decltype(streamed)::value>;
+				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+				hipLaunchKernelGGL(kernel, dim3(ceil_div(s.hidden, 16)), dim3(256), bytes, stream, x, w, y, s.rows, s.hidden, s.features, bias, projections, gate);
 			});
 			MLHIP_CHECK(hipGetLastError());
 			return;

@@ -623,7 +623,7 @@ namespace mlhip
 	 * 26 / 17 / 20; fp32 57600 rows, k = 256 -> 2 x 1024 589 / 551 / 520, 8192 rows, k = 2048 -> 2 x 2048 1011 / 1071 / 1100.
 	 * columns: of the result (of one of the two matrices where the operand is paired)
 	 */
-	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split)
+	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split, double *cost_out = nullptr)
 	{
 		constexpr int UNITS = 256;
 		const bool half = element_size == 2;
@@ -649,7 +649,7 @@ namespace mlhip
 				{
 					cost = std::ceil(work) * (4.0 + per_part * (half ? 0.6 : 2.05));
 					const double one_slot = work * (1.8 + per_part * (half ? 0.5 : 2.15));
-					if (work >= 4.0 && one_slot < cost)
+					if (work >= 4.0 && parts == 1 && per_part <= 32 && one_slot < cost)
 					{
 						slots = 1;
 						cost = one_slot;
@@ -662,6 +662,39 @@ namespace mlhip
 					least = cost;
 					best = ProductPlan { tile, slots, tiles_m, tiles_n, chunks, parts, per_part };
 				}
+			}
+		}
+		if (cost_out != nullptr)
+			*cost_out = least;
+		return best;
+	}
+	/*
+	 * A product whose last turn would leave most compute units idle, in two: the rows of whole turns, and the rest, which is split along k. dW of 11008 x 2048, k = 8192, fp16 (344 tiles: 32 rows of 8 tiles and 11 that
+	 * are cut in two) whole 388 us, so 330.
+	 */
+	struct TwoPlans
+	{
+			ProductPlan first, rest;
+			int first_rows; /* the rest may be none */
+	};
+	inline TwoPlans plan_in_turns(int rows, int columns, int depth, int element_size)
+	{
+		constexpr int UNITS = 256;
+		double whole, first, rest;
+		TwoPlans best { plan_product(rows, columns, false, depth, element_size, true, &whole), ProductPlan { }, rows };
+		for (int tile : { 256, 128 })
+		{
+			const int tiles_n = ceil_div(columns, tile), turns = static_cast<int>(static_cast<long long>(ceil_div(rows, tile)) * tiles_n / UNITS);
+			if (turns < 1 || turns > 8 || tiles_n > UNITS)
+				continue;
+			const int first_rows = turns * UNITS / tiles_n * tile;
+			if (first_rows >= rows)
+				continue;
+			TwoPlans two { plan_product(first_rows, columns, false, depth, element_size, false, &first), plan_product(rows - first_rows, columns, false, depth, element_size, true, &rest), first_rows };
+			if (first + rest + 3.0 < 0.95 * whole)
+			{
+				whole = first + rest + 3.0;
+				best = two;
 			}
 		}
 		return best;
@@ -852,7 +885,7 @@ namespace mlhip
 		MLHIP_CHECK(hipGetLastError());
 	}
 	/*
-	 * out [rows][columns] = scale * A B + beta * out, split along k where the tiles alone would not fill the chip; `partial` holds parts * rows * columns floats then
+	 * out [rows][columns] = scale * A B + beta * out; `partial` holds parts * rows * columns floats where the plan has parts
 	 */
 	template<typename T, typename Out, Side SA, Side SB>
 	inline void product_to(hipStream_t stream, const ProductPlan &plan, const Operand &a, const Operand &b, int rows, int columns, Out *out, float beta, const float *scale, float *partial)
@@ -869,6 +902,25 @@ namespace mlhip
 	inline size_t part_bytes(const ProductPlan &plan, int rows, int columns)
 	{
 		return plan.parts > 1 ? sizeof(float) * plan.parts * static_cast<size_t>(rows) * columns : 0;
+	}
+	template<typename T, typename Out, Side SA, Side SB>
+	inline void product_to(hipStream_t stream, const TwoPlans &plans, const Operand &a, const Operand &b, int rows, int columns, Out *out, float beta, const float *scale, float *partial)
+	{
+		const int first = plans.first_rows;
+		Operand head = a, rest = a;
+		if (first < rows)
+			head.extent = first; /* a multiple of the tile's rows, so of 16 bytes too */
+		product_to<T, Out, SA, SB>(stream, plans.first, head, b, first, columns, out, beta, scale, partial);
+		if (first >= rows)
+			return;
+		rest.base += (SA == Side::ROWS) ? first * a.row_bytes : first * sizeof(T);
+		rest.extent -= first;
+		product_to<T, Out, SA, SB>(stream, plans.rest, rest, b, rows - first, columns, out + static_cast<size_t>(first) * columns, beta, scale, partial);
+	}
+	inline size_t part_bytes(const TwoPlans &plans, int rows, int columns)
+	{
+		return plans.first_rows >= rows ? part_bytes(plans.first, rows, columns)
+				: std::max(part_bytes(plans.first, plans.first_rows, columns), part_bytes(plans.rest, rows - plans.first_rows, columns));
 	}
 
 	/* rows of `columns` elements copied to rows that are whole 16-byte pieces, zeros behind the last element: what the panels' loads ask of an operand whose rows end anywhere */

@@ -55,7 +55,7 @@ def test_forward(ctx, rows, features, hidden, dtype):
     check_guards(ctx, kept, 9.0)
 
 
-BACKWARD = [(1, 8, 1), (1, 200, 64), (3, 63, 20), (17, 130, 16), (65, 40, 64), (300, 200, 130), (129, 333, 257), (1030, 72, 24), (3500, 3600, 24), (33, 3600, 1800), (700, 16, 5)]
+BACKWARD = [(1, 8, 1), (1, 200, 64), (3, 63, 20), (17, 130, 16), (65, 40, 64), (300, 200, 130), (129, 333, 257), (1030, 72, 24), (3500, 3600, 24), (33, 3600, 1800), (700, 16, 5), (4600, 4096, 1056)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "float32"])
