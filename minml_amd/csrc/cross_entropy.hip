@@ -266,6 +266,14 @@ namespace
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
 	constexpr int SCALE_GROUPS = 256;
 	constexpr int SCALE_BITS = 15;
+	/* the power of two above the largest |dloss| */
+	__device__ __forceinline__ int scale_exponent(float top)
+	{
+		int exponent = 0;
+		if (top > 0.0f)
+			(void) frexpf(top, &exponent);
+		return max(exponent, -100); /* so that the way back is a normal number */
+	}
 	__global__ __launch_bounds__(256) void kernel_largest_gradient(const float *dloss, const int *targets, int rows, int classes, float *largest)
 	{
 		__shared__ float waves[4];
@@ -294,13 +302,36 @@ namespace
 #pragma unroll
 		for (int offset = 32; offset >= 1; offset >>= 1)
 			top = fmaxf(top, __shfl_xor(top, offset));
-		int exponent = 0;
-		if (top > 0.0f)
-			(void) frexpf(top, &exponent); /* top < 2^exponent */
-		exponent = max(exponent, -100); /* so that the way back is a normal number */
+		const int exponent = scale_exponent(top);
 		for (int i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256)
 			factors[i] = (targets[i] >= 0 && targets[i] < classes) ? ldexpf(dloss[i], SCALE_BITS - exponent) : 0.0f;
 		if (blockIdx.x == 0 && threadIdx.x == 0)
+			*back = ldexpf(1.0f, exponent - SCALE_BITS);
+	}
+	/* both in one launch of one workgroup */
+	constexpr int ROWS_OF_ONE_GROUP = 8192;
+	__global__ __launch_bounds__(1024) void kernel_row_factors_of_few(const float *dloss, const int *targets, int rows, int classes, float *factors, float *back)
+	{
+		__shared__ float waves[16];
+		float top = 0.0f;
+		for (int i = threadIdx.x; i < rows; i += 1024)
+		{
+			const float v = fabsf(dloss[i]);
+			if (targets[i] >= 0 && targets[i] < classes && v <= std::numeric_limits<float>::max())
+				top = fmaxf(top, v);
+		}
+#pragma unroll
+		for (int offset = 32; offset >= 1; offset >>= 1)
+			top = fmaxf(top, __shfl_xor(top, offset));
+		if ((threadIdx.x & 63) == 0)
+			waves[threadIdx.x >> 6] = top;
+		__syncthreads();
+		for (int w = 0; w < 16; w++)
+			top = fmaxf(top, waves[w]);
+		const int exponent = scale_exponent(top);
+		for (int i = threadIdx.x; i < rows; i += 1024)
+			factors[i] = (targets[i] >= 0 && targets[i] < classes) ? ldexpf(dloss[i], SCALE_BITS - exponent) : 0.0f;
+		if (threadIdx.x == 0)
 			*back = ldexpf(1.0f, exponent - SCALE_BITS);
 	}
 	template<typename T>
@@ -339,9 +370,9 @@ namespace
 				for (int i = 0; i < BLOCKS; i++)
 				{
 					const int m = min(at.tile_m * BM + at.row(i), rows - 1);
-					target[i] = targets[m] - first_class;
 					norm[i] = lse[m];
 					factor[i] = at.tile_m * BM + at.row(i) < rows ? factors[m] : 0.0f;
+					target[i] = factor[i] != 0.0f ? targets[m] - first_class : -1; /* a class then */
 				}
 				static_for<PASSES>([&](auto pass)
 				{
@@ -437,7 +468,8 @@ namespace
 	/* classes of a piece: whole tiles, all pieces about the same */
 	int classes_of_piece(const LossShape &s)
 	{
-		const size_t most = std::max<size_t>(256, PIECE_BYTES / (static_cast<size_t>(std::max(s.rows, 1)) * s.element_size) / 256 * 256);
+		/* and a row of d below 4 MB, which the panels' offsets ask for */
+		const size_t most = std::min<size_t>(1 << 19, std::max<size_t>(256, PIECE_BYTES / (static_cast<size_t>(std::max(s.rows, 1)) * s.element_size) / 256 * 256));
 		const size_t pieces = (s.classes + most - 1) / most;
 		return static_cast<int>(std::min<size_t>(round_up((s.classes + pieces - 1) / pieces, 256), s.classes));
 	}
@@ -547,8 +579,13 @@ namespace
 		float *sums = reinterpret_cast<float*>(workspace + space.sums), *factors = reinterpret_cast<float*>(workspace + space.factors);
 		float *largest = reinterpret_cast<float*>(workspace + space.scale), *back = largest + SCALE_GROUPS;
 		const int groups = std::min(ceil_div(s.rows, 256), SCALE_GROUPS);
-		hipLaunchKernelGGL(kernel_largest_gradient, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest);
-		hipLaunchKernelGGL(kernel_row_factors, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest, groups, factors, back);
+		if (s.rows <= ROWS_OF_ONE_GROUP)
+			hipLaunchKernelGGL(kernel_row_factors_of_few, dim3(1), dim3(1024), 0, stream, dloss, targets, s.rows, s.classes, factors, back);
+		else
+		{
+			hipLaunchKernelGGL(kernel_largest_gradient, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest);
+			hipLaunchKernelGGL(kernel_row_factors, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest, groups, factors, back);
+		}
 		MLHIP_CHECK(hipGetLastError());
 		x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
 		w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
@@ -649,11 +686,12 @@ extern "C"
 		if (s.rows == 0)
 			return;
 		check_space(workspace, workspace_size, loss_space(s, false).total, name);
-		const hipStream_t stream = stream_of(context);
+		require_apart( { loss, lse, Extent(workspace, workspace_size) }, { x, w, b, targets }, name);
+		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			loss_forward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), ptr<float>(loss), ptr<float>(lse), reinterpret_cast<uint8_t*>(workspace));
+			loss_forward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), ptr<float>(loss), ptr<float>(lse), reinterpret_cast<uint8_t*>(workspace));
 		else
-			loss_forward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), ptr<float>(loss), ptr<float>(lse), reinterpret_cast<uint8_t*>(workspace));
+			loss_forward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), ptr<float>(loss), ptr<float>(lse), reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)
 	{
@@ -675,24 +713,25 @@ extern "C"
 		if (s.rows == 0)
 		{
 			/* sums over nothing */
-			const hipStream_t stream = stream_of(context);
+			const OnDeviceOf on(context);
 			for (const mlTensor_t &t : { dw, db })
 				if (t.data != nullptr)
 				{
 					if (t.dtype == DTYPE_FLOAT16)
-						launch_join_parts<half_t>(stream, nullptr, 0, volume(t), ptr<half_t>(t), beta_weights, nullptr);
+						launch_join_parts<half_t>(on.stream, nullptr, 0, volume(t), ptr<half_t>(t), beta_weights, nullptr);
 					else
-						launch_join_parts<float>(stream, nullptr, 0, volume(t), ptr<float>(t), beta_weights, nullptr);
+						launch_join_parts<float>(on.stream, nullptr, 0, volume(t), ptr<float>(t), beta_weights, nullptr);
 				}
 			return;
 		}
 		check_space(workspace, workspace_size, loss_space(s, true).total, name);
-		const hipStream_t stream = stream_of(context);
+		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, b, targets, lse, dloss }, name);
+		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			loss_backward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db,
+			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db,
 					reinterpret_cast<uint8_t*>(workspace));
 		else
-			loss_backward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db,
+			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db,
 					reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)

@@ -527,11 +527,12 @@ extern "C"
 		MLHIP_REQUIRE(x.data != nullptr && w.data != nullptr && y.data != nullptr, "gated_dense_forward: null pointer");
 		MLHIP_REQUIRE(aligned_16(x) && aligned_16(w), "gated_dense_forward: input and weights must be aligned to 16 bytes");
 		require_workspace(workspace, workspace_size, gated_space(s, false).total, name);
-		const hipStream_t stream = stream_of(context);
+		require_apart( { y, projections, Extent(workspace, workspace_size) }, { x, w, b }, name);
+		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			gated_forward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<half_t>(y), ptr<half_t>(projections), gate, reinterpret_cast<uint8_t*>(workspace));
+			gated_forward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<half_t>(y), ptr<half_t>(projections), gate, reinterpret_cast<uint8_t*>(workspace));
 		else
-			gated_forward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<float>(y), ptr<float>(projections), gate, reinterpret_cast<uint8_t*>(workspace));
+			gated_forward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<float>(y), ptr<float>(projections), gate, reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)
 	{
@@ -565,12 +566,13 @@ extern "C"
 		MLHIP_REQUIRE(s.rows == 0 || (x.data != nullptr && w.data != nullptr && projections.data != nullptr && dy.data != nullptr), "gated_dense_backward: null pointer");
 		MLHIP_REQUIRE(aligned_16(x) && aligned_16(w), "gated_dense_backward: input and weights must be aligned to 16 bytes");
 		require_workspace(workspace, workspace_size, gated_space(s, true).total, name);
-		const hipStream_t stream = stream_of(context);
+		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, projections, dy }, name);
+		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			gated_backward(stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(projections), ptr<half_t>(dy), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, gate,
+			gated_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(projections), ptr<half_t>(dy), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, gate,
 					reinterpret_cast<uint8_t*>(workspace));
 		else
-			gated_backward(stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(projections), ptr<float>(dy), beta_dx, ptr<float>(dx), beta_weights, dw, db, gate,
+			gated_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(projections), ptr<float>(dy), beta_dx, ptr<float>(dx), beta_weights, dw, db, gate,
 					reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)

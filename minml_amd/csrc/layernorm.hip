@@ -556,10 +556,12 @@ extern "C"
 		if (volume(x) == 0)
 			return;
 		MLHIP_REQUIRE(x.data != nullptr && y.data != nullptr, "layer_norm_forward: null pointer");
+		require_apart( { y }, { x, w, b }, "layer_norm_forward", x.data);
+		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			layer_norm_forward<half_t>(stream_of(context), x, w, b, y, epsilon);
+			layer_norm_forward<half_t>(on.stream, x, w, b, y, epsilon);
 		else
-			layer_norm_forward<float>(stream_of(context), x, w, b, y, epsilon);
+			layer_norm_forward<float>(on.stream, x, w, b, y, epsilon);
 	}
 	catch (...)
 	{
@@ -603,10 +605,12 @@ extern "C"
 			MLHIP_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_size >= hip_layer_norm_get_workspace_size(shape_of(x), x.dtype),
 					"layer_norm_backward: the workspace is too small or not aligned to 16 bytes");
 		}
+		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, dy }, "layer_norm_backward", dx.data);
+		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			layer_norm_backward<half_t>(stream_of(context), x, w, dy, beta_dx, dx, beta_weights, dw, db, reinterpret_cast<float*>(workspace), epsilon);
+			layer_norm_backward<half_t>(on.stream, x, w, dy, beta_dx, dx, beta_weights, dw, db, reinterpret_cast<float*>(workspace), epsilon);
 		else
-			layer_norm_backward<float>(stream_of(context), x, w, dy, beta_dx, dx, beta_weights, dw, db, reinterpret_cast<float*>(workspace), epsilon);
+			layer_norm_backward<float>(on.stream, x, w, dy, beta_dx, dx, beta_weights, dw, db, reinterpret_cast<float*>(workspace), epsilon);
 	}
 	catch (...)
 	{

@@ -11,8 +11,64 @@
 #include "common.hpp"
 #include "device_utils.hpp"
 
+#include <initializer_list>
+
 namespace mlhip
 {
+	/* a call's device is its context's, whichever is current when it is made; the caller's comes back at its end */
+	class OnDeviceOf
+	{
+			int before = 0, device;
+		public:
+			const hipStream_t stream;
+			explicit OnDeviceOf(mlContext_t context) :
+					device(get(context)->device_index),
+					stream(stream_of(context))
+			{
+				MLHIP_CHECK(hipGetDevice(&before));
+				if (before != device)
+					MLHIP_CHECK(hipSetDevice(device));
+			}
+			~OnDeviceOf()
+			{
+				if (before != device)
+					(void) hipSetDevice(before);
+			}
+			OnDeviceOf(const OnDeviceOf&) = delete;
+			OnDeviceOf& operator=(const OnDeviceOf&) = delete;
+	};
+	/* memory that a call reads or writes */
+	struct Extent
+	{
+			const uint8_t *begin;
+			size_t bytes;
+
+			Extent(const void *data, size_t size) :
+					begin(static_cast<const uint8_t*>(data)),
+					bytes(data == nullptr ? 0 : size)
+			{
+			}
+			Extent(const mlTensor_t &t) :
+					Extent(t.data, volume(t) * size_of(t.dtype))
+			{
+			}
+			bool meets(const Extent &other) const
+			{
+				return bytes > 0 && other.bytes > 0 && begin < other.begin + other.bytes && other.begin < begin + bytes;
+			}
+	};
+	/* results may lie over nothing else of the call, but for the one named `in_place` where it is exactly one of the inputs that may be overwritten */
+	inline void require_apart(std::initializer_list<Extent> results, std::initializer_list<Extent> inputs, const char *name, const void *in_place = nullptr)
+	{
+		for (const Extent *r = results.begin(); r != results.end(); r++)
+		{
+			for (const Extent *other = results.begin(); other != r; other++)
+				MLHIP_REQUIRE(!r->meets(*other), std::string(name) + ": results overlap");
+			for (const Extent &input : inputs)
+				MLHIP_REQUIRE(!r->meets(input) || (r->begin == in_place && r->begin == input.begin && r->bytes == input.bytes), std::string(name) + ": a result overlaps an input");
+		}
+	}
+
 	/* VEC consecutive elements that need no more alignment than one of them: one memory instruction all the same (global memory takes any address) */
 	template<typename T, int VEC>
 	struct Elements

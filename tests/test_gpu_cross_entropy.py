@@ -24,7 +24,7 @@ def space(ctx, x, w, backward):
 
 
 SIZES = [(1, 8, 1), (1, 64, 300), (3, 63, 20), (16, 200, 37), (17, 130, 16), (33, 72, 1000), (64, 333, 100), (65, 40, 513), (130, 65, 257), (300, 200, 130), (129, 1096, 24), (2, 2056, 70),
-         (3500, 24, 3700), (513, 64, 8), (1, 16, 40001)]
+         (3500, 24, 3700), (513, 64, 8), (1, 16, 40001), (2, 8, 1100000), (9000, 8, 20)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "float32"])

@@ -6,15 +6,20 @@ from minml_amd import backend as B
 from minml_amd import core as ml
 
 
+_next = [1 << 40]
+
+
 def fake(shape, dtype="float16"):
-    return ml.Tensor(shape, dtype, _ptr=0x7000)
+    """A tensor at an address of its own, which no call of these tests reaches."""
+    _next[0] += 1 << 24
+    return ml.Tensor(shape, dtype, _ptr=_next[0])
 
 
 NULL = B.make_tensor(None, B.DTYPE_UNKNOWN, ())
 
 
-def refused(name, *args):
-    with pytest.raises(ValueError):
+def refused(name, *args, why=None):
+    with pytest.raises(ValueError, match=why):
         B.fn(name)(None, *args)
 
 
@@ -28,7 +33,7 @@ def test_layer_norm_refusals_of_the_library():
     forward(fake((4, 16), "int32").desc(), w, w, fake((4, 16), "int32").desc())
     forward(x, w, w, x, -1.0)
     forward(x, w, w, x, float("nan"))
-    forward(x, w, w, x)  # all is well but the context
+    refused("layer_norm_forward", x, w, w, x, 1e-5, why="null context")  # all is well but the context
     backward = lambda x, w, dy, dx, dw, db, space=0x7000, size=1 << 30: refused("layer_norm_backward", x, w, dy, 0.0, dx, 0.0, dw, db, space, size, 1e-5)
     need = B.fn("layer_norm_get_workspace_size")(fake((4, 16)).shape_desc(), B.DTYPE_FLOAT16)
     assert need >= 2 * 16 * 4
@@ -131,7 +136,7 @@ def test_cross_entropy_refusals_of_the_library():
     forward(space=0x7080)
     forward(n=size(False) - 1)
     forward()  # all is well but the context
-    dx, dw, db = x, w, b
+    dx, dw, db = fake((4, 16)).desc(), fake((90, 16)).desc(), fake((90,)).desc()
     backward = lambda x=x, w=w, b=b, t=t, lse=f, dloss=f, dx=dx, dw=dw, db=db, space=0x7000, n=1 << 30: refused("linear_cross_entropy_backward", x, w, b, t, lse, dloss, 0.0, dx, 0.0, dw, db, space, n)
     backward(lse=fake((4,)).desc())
     backward(dloss=fake((4, 2), "float32").desc())
@@ -154,3 +159,31 @@ def test_cross_entropy_workspace_does_not_grow_with_the_vocabulary():
             # besides d: sums over rows, two floats a tile of logits and row, the fp32 sums of dx and of one piece of dw, each in parts of at most 512 tiles together
             assert all(s <= (1 << 28) + rows * 20 + 8 * rows * classes / 128 + 2 * 4 * rows * features * 8 + (1 << 26) + 4 * 2000000 * (rows / 128 + 1) for s, classes in zip(sizes, (200000, 2000000)))
             assert sizes[1] < rows * 2000000 * element / 2
+
+
+def test_results_over_inputs_are_refused():
+    """Where a call does not say that a result may lie over an input, it may not; and never in part."""
+    whole = fake((64, 16))
+    part = lambda shape, offset: whole.view(shape, offset).desc()
+    x, w, b = fake((4, 16)).desc(), fake((16,)).desc(), fake((16,)).desc()
+    overlaps = "overlap"
+    refused("layer_norm_forward", part((4, 16), 0), w, b, part((4, 16), 16), 1e-5, why=overlaps)
+    refused("layer_norm_forward", x, part((16,), 0), b, part((4, 16), 0), 1e-5, why=overlaps)
+    refused("layer_norm_forward", x, w, b, x, 1e-5, why="null context")  # in place is allowed
+    space, n = 0x7000, 1 << 20
+    refused("layer_norm_backward", x, w, part((4, 16), 0), 0.0, part((4, 16), 8), 0.0, w, b, space, n, 1e-5, why=overlaps)
+    refused("layer_norm_backward", x, w, fake((4, 16)).desc(), 0.0, x, 0.0, b, b, space, n, 1e-5, why=overlaps)
+    refused("layer_norm_backward", x, w, fake((4, 16)).desc(), 0.0, x, 0.0, w, b, space, n, 1e-5, why=overlaps)
+    refused("layer_norm_backward", x, w, x, 0.0, x, 0.0, fake((16,)).desc(), b, space, n, 1e-5, why="null context")
+    w2, y, p = fake((2, 24, 16)).desc(), fake((4, 24)).desc(), fake((4, 2, 24)).desc()
+    refused("gated_dense_forward", part((4, 16), 0), w2, NULL, part((4, 24), 32), p, B.GATE_SILU, None, 0, why=overlaps)
+    refused("gated_dense_forward", x, w2, NULL, part((4, 24), 0), part((4, 2, 24), 0), B.GATE_SILU, None, 0, why=overlaps)
+    refused("gated_dense_forward", x, w2, NULL, y, p, B.GATE_SILU, None, 0, why="null context")
+    refused("gated_dense_backward", x, w2, p, y, 0.0, x, 0.0, NULL, NULL, B.GATE_SILU, space, n, why=overlaps)
+    refused("gated_dense_backward", x, w2, p, y, 0.0, fake((4, 16)).desc(), 0.0, w2, NULL, B.GATE_SILU, space, n, why=overlaps)
+    refused("gated_dense_backward", ml.Tensor((4, 16), "float16", _ptr=space + 256).desc(), w2, p, y, 0.0, fake((4, 16)).desc(), 0.0, NULL, NULL, B.GATE_SILU, space, n, why=overlaps)
+    wc, t, f, g = fake((90, 16)).desc(), fake((4,), "int32").desc(), fake((4,), "float32").desc(), fake((4,), "float32").desc()
+    refused("linear_cross_entropy_forward", x, wc, NULL, t, f, f, space, n, why=overlaps)
+    refused("linear_cross_entropy_forward", x, wc, NULL, t, f, g, space, n, why="null context")
+    refused("linear_cross_entropy_backward", x, wc, NULL, t, f, g, 0.0, x, 0.0, NULL, NULL, space, n, why=overlaps)
+    refused("linear_cross_entropy_backward", x, wc, NULL, t, f, g, 0.0, NULL, 0.0, wc, NULL, space, n, why=overlaps)
