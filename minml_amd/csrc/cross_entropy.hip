@@ -65,24 +65,24 @@ namespace
 
 	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
 	/* a wavefront's share of the bias, and of what lies behind the last class */
-	template<typename T, int BM>
+	template<typename T, int BM, int BN>
 	struct TileColumns
 	{
 			float bias[2][16];
 			int first[2]; /* column of the tile of the wavefront's blocks, counted from the first class */
 
-			__device__ __forceinline__ void begin(const TilePlace<BM> &at, const T *values, int classes)
+			__device__ __forceinline__ void begin(const TilePlace<BM, BN> &at, const T *values, int classes)
 			{
 #pragma unroll
 				for (int j = 0; j < 2; j++)
 				{
-					first[j] = at.tile_n * BM + at.column(j);
+					first[j] = at.tile_n * BN + at.column(j);
 					load_lane_bias(bias[j], values, first[j], classes);
 				}
 			}
 			__device__ __forceinline__ int column(int j, int r) const
 			{
-				return first[j] + TilePlace<BM>::lane_column(r / 4) + r % 4;
+				return first[j] + TilePlace<BM, BN>::lane_column(r / 4) + r % 4;
 			}
 			/* f(j, r) for the register that holds class n, in the lane that holds it; most rows have their class in another tile */
 			template<typename F>
@@ -109,18 +109,18 @@ namespace
 			float *target_logits;
 			int classes, tiles_n;
 
-			template<int BM>
+			template<int BM, int BN>
 			static constexpr int lds()
 			{
-				return (BM / 64) * BM * static_cast<int>(sizeof(Partial));
+				return (BN / 64) * BM * static_cast<int>(sizeof(Partial));
 			}
 			/* in registers: a lane has 32 columns of every of its rows, the lane 32 further the other 32 of the wavefront; the wavefronts of a row meet in LDS */
-			template<int BM, typename Acc>
-			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
-				constexpr int BLOCKS = TilePlace<BM>::BLOCKS, WAVES_N = BM / 64;
+				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, WAVES_N = BN / 64;
 				constexpr float NOTHING = -std::numeric_limits<float>::infinity();
-				TileColumns<T, BM> columns;
+				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
 				int target[BLOCKS];
 #pragma unroll
@@ -129,7 +129,7 @@ namespace
 					const int m = at.tile_m * BM + at.row(i);
 					target[i] = m < rows ? targets[m] : -1;
 				}
-				const bool edge = (at.tile_n + 1) * BM > classes;
+				const bool edge = (at.tile_n + 1) * BN > classes;
 				Partial *meeting = reinterpret_cast<Partial*>(lds); /* [WAVES_N][BM] */
 				__syncthreads();
 #pragma unroll
@@ -344,20 +344,20 @@ namespace
 			float *sums; /* [row tiles][classes of the piece], or null */
 			int first_class, classes, row_elements; /* classes: of the piece */
 
-			template<int BM>
+			template<int BM, int BN>
 			static constexpr int lds()
 			{
-				return Stage<T, BM>::bytes(sizeof(T) == 2 ? BM : BM / 2);
+				return Stage<T, BN>::bytes(sizeof(T) == 2 ? BM : rows_at_a_time(BM));
 			}
 			/* in registers, rounded there; through LDS to whole rows. The column sums of a wavefront's 64 rows are folded so that each of 32 lanes ends up with one column of each block */
-			template<int BM, typename Acc>
-			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
-				constexpr int BLOCKS = TilePlace<BM>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : BM / 2, PASSES = BM / ROWS;
-				TileColumns<T, BM> columns;
+				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : rows_at_a_time(BM), PASSES = BM / ROWS;
+				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
-				const bool edge = (at.tile_n + 1) * BM > classes;
-				const Stage<T, BM> stage { reinterpret_cast<T*>(lds) };
+				const bool edge = (at.tile_n + 1) * BN > classes;
+				const Stage<T, BN> stage { reinterpret_cast<T*>(lds) };
 				float total[2][16];
 #pragma unroll
 				for (int j = 0; j < 2; j++)
@@ -411,12 +411,12 @@ namespace
 							}
 					}
 					__syncthreads();
-					stage.template copy<ROWS, TilePlace<BM>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BM, row_elements);
+					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
 				});
 				if (sums == nullptr)
 					return;
 				/* lane bits 4 .. 1 choose among the 16 registers, a half of them at a time; bit 0 adds up what is left */
-				float *meeting = reinterpret_cast<float*>(lds); /* [2 wavefront rows][BM] */
+				float *meeting = reinterpret_cast<float*>(lds); /* [2 wavefront rows][BN] */
 				__syncthreads();
 #pragma unroll
 				for (int j = 0; j < 2; j++)
@@ -434,12 +434,12 @@ namespace
 					const float sum = total[j][0] + __shfl_xor(total[j][0], 1);
 					const int r = (threadIdx.x & 31) >> 1;
 					if ((threadIdx.x & 1) == 0)
-						meeting[at.wave_m * BM + at.column(j) + TilePlace<BM>::lane_column(r / 4) + r % 4] = sum;
+						meeting[at.wave_m * BN + at.column(j) + TilePlace<BM, BN>::lane_column(r / 4) + r % 4] = sum;
 				}
 				__syncthreads();
-				const int n = at.tile_n * BM + static_cast<int>(threadIdx.x);
-				if (static_cast<int>(threadIdx.x) < BM && n < classes)
-					sums[static_cast<size_t>(at.tile_m) * classes + n] = meeting[threadIdx.x] + meeting[BM + threadIdx.x];
+				const int n = at.tile_n * BN + static_cast<int>(threadIdx.x);
+				if (static_cast<int>(threadIdx.x) < BN && n < classes)
+					sums[static_cast<size_t>(at.tile_m) * classes + n] = meeting[threadIdx.x] + meeting[BN + threadIdx.x];
 			}
 	};
 
@@ -483,7 +483,7 @@ namespace
 	}
 	ProductPlan weights_plan(const LossShape &s, int classes)
 	{
-		return plan_product(classes, s.features, false, s.rows, s.element_size, true);
+		return plan_product(classes, s.features, false, s.rows, s.element_size, true, false);
 	}
 	struct LossSpace
 	{
@@ -599,7 +599,7 @@ namespace
 			const uint8_t *weights = reinterpret_cast<const uint8_t*>(w) + first * row_bytes;
 			{
 				ProductPlan plan = logits_plan(s, most);
-				plan.tiles_n = ceil_div(classes, plan.tile);
+				plan.tiles_n = ceil_div(classes, std::max(plan.tile, 128));
 				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
 				const Operand b { weights, row_bytes, classes, padded };
 				launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T> { bias != nullptr ? bias + first : nullptr, targets, lse, factors, d,

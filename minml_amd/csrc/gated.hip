@@ -90,21 +90,21 @@ namespace
 			const T *bias;
 			int hidden, gate;
 
-			template<int BM>
+			template<int BM, int BN>
 			static constexpr int lds()
 			{
-				return Stage<T, BM / 2>::bytes(sizeof(T) == 2 ? BM : PANEL);
+				return Stage<T, BN / 2>::bytes(sizeof(T) == 2 ? BM : std::min(BM, PANEL));
 			}
 			/*
 			 * The gate is applied in registers (blocks (i, 0) and (i, 1) hold both projections of an element). The results leave one after the other through the same place in LDS: y, then both projections
 			 * where they are kept.
 			 */
-			template<int BM, typename Acc>
-			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
-				constexpr int ROWS = (sizeof(T) == 2) ? BM : PANEL, PASSES = BM / ROWS, BLOCKS = TilePlace<BM>::BLOCKS / PASSES;
-				const Stage<T, BM / 2> stage { reinterpret_cast<T*>(lds) };
-				const int n0 = at.tile_n * (BM / 2);
+				constexpr int ROWS = (sizeof(T) == 2) ? BM : std::min(BM, PANEL), PASSES = BM / ROWS, BLOCKS = TilePlace<BM, BN>::BLOCKS / PASSES;
+				const Stage<T, BN / 2> stage { reinterpret_cast<T*>(lds) };
+				const int n0 = at.tile_n * (BN / 2);
 				float shift[2][16];
 #pragma unroll
 				for (int j = 0; j < 2; j++)
@@ -151,7 +151,7 @@ namespace
 							gated(std::integral_constant<int, GATE_GELU>());
 							break;
 					}
-					stage.template copy<ROWS, TilePlace<BM>::THREADS>(y, hidden, m0, rows, n0, hidden);
+					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(y, hidden, m0, rows, n0, hidden);
 					if (projections != nullptr)
 						static_for<2>([&](auto matrix)
 						{
@@ -159,7 +159,7 @@ namespace
 							{
 								return projection(i, decltype(matrix)::value, r);
 							});
-							stage.template copy<ROWS, TilePlace<BM>::THREADS>(projections + decltype(matrix)::value * hidden, 2 * static_cast<size_t>(hidden), m0, rows, n0, hidden);
+							stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(projections + decltype(matrix)::value * hidden, 2 * static_cast<size_t>(hidden), m0, rows, n0, hidden);
 						});
 				});
 			}
@@ -171,29 +171,30 @@ namespace
 			size_t part_stride;
 			int hidden;
 
-			template<int BM>
+			template<int BM, int BN>
 			static constexpr int lds()
 			{
-				return Stage<float, BM / 2>::bytes(PANEL);
+				return Stage<float, BN / 2>::bytes(std::min(BM, PANEL));
 			}
-			template<int BM, typename Acc>
-			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
-				const Stage<float, BM / 2> stage { reinterpret_cast<float*>(lds) };
-				static_for<BM / PANEL>([&](auto half)
+				constexpr int ROWS = std::min(BM, PANEL), BLOCKS = ROWS / 64;
+				const Stage<float, BN / 2> stage { reinterpret_cast<float*>(lds) };
+				static_for<BM / ROWS>([&](auto half)
 				{
 					static_for<2>([&](auto matrix)
 					{
 						constexpr int h = decltype(half)::value, j = decltype(matrix)::value;
 						__syncthreads();
 #pragma unroll
-						for (int i = 2 * h; i < 2 * h + 2; i++)
+						for (int i = h * BLOCKS; i < (h + 1) * BLOCKS; i++)
 #pragma unroll
 							for (int q = 0; q < 4; q++)
-								stage.put(at.row(i) - h * PANEL, at.wave_n * 32 + at.lane_column(q), acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+								stage.put(at.row(i) - h * ROWS, at.wave_n * 32 + at.lane_column(q), acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
 						__syncthreads();
-						stage.template copy<PANEL, TilePlace<BM>::THREADS>(partial + at.part * part_stride + j * hidden, 2 * static_cast<size_t>(hidden), at.tile_m * BM + h * PANEL, rows,
-								at.tile_n * (BM / 2), hidden);
+						stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(partial + at.part * part_stride + j * hidden, 2 * static_cast<size_t>(hidden), at.tile_m * BM + h * ROWS, rows,
+								at.tile_n * (BN / 2), hidden);
 					});
 				});
 			}
@@ -369,11 +370,11 @@ namespace
 	}
 	TwoPlans input_plan(const GatedShape &s)
 	{
-		return plan_in_turns(s.rows, s.features, 2 * s.hidden, s.element_size);
+		return plan_in_turns(s.rows, s.features, 2 * s.hidden, s.element_size, true);
 	}
 	TwoPlans weights_plan(const GatedShape &s)
 	{
-		return plan_in_turns(2 * s.hidden, s.features, s.rows, s.element_size);
+		return plan_in_turns(2 * s.hidden, s.features, s.rows, s.element_size, false);
 	}
 	/* the pieces of a workspace, each aligned to 256 bytes */
 	struct GatedSpace

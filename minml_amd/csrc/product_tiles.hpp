@@ -17,7 +17,7 @@
  * 256x256 (8 wavefronts, one workgroup per compute unit): two slots of four panels, refilled panel by panel: the wavefront's 128 x 64 share is multiplied in four phases of 64 x 32, and a panel's place
  * takes the chunk after the next one as soon as its last phase is over, so a load has six phases (one and a half chunks of 64 k) to arrive.
  * 128x128 (4 wavefronts): where 256x256 tiles would leave units without work, with two slots and two workgroups per compute unit; and where k is so short that a tile is mostly beginning and end, with one
- * slot and four workgroups per unit, which hide each other's waits.
+ * slot and four workgroups per unit, which hide each other's waits. fp32, which the matrix cores bound by far, also has 64x128.
  * A product with a long k and few tiles is split along k (gridDim.y): each part leaves its sums in fp32, and a launch of its own adds them up in order.
  *
  * The tile's accumulators pass through LDS in fp32, 128 rows at a time, so that the epilogue sees 8 consecutive columns per thread and whole lines per wavefront.
@@ -69,11 +69,12 @@ namespace mlhip
 #endif
 	}
 
-	/* the loads of one panel by WAVES wavefronts, 1 KB each. SEGMENT: consecutive rows of the operand in a panel (64 where a panel holds both halves of a paired tile) */
-	template<typename T, Side SIDE, int WAVES, int SEGMENT = PANEL>
+	/* the loads of one panel (or of its first LOADED rows) by WAVES wavefronts, 1 KB each. SEGMENT: consecutive rows of the operand in a panel (64 where a panel holds both halves of a paired tile) */
+	template<typename T, Side SIDE, int WAVES, int SEGMENT = PANEL, int LOADED = PANEL>
 	struct PanelLoads
 	{
-			static constexpr int COUNT = 16 / WAVES;
+			static_assert(LOADED == PANEL || SIDE == Side::ROWS, "columns come in whole panels");
+			static constexpr int COUNT = LOADED / 8 / WAVES;
 			static constexpr int CHUNK = 128 / sizeof(T); /* k of a chunk */
 			static constexpr int K_PER_LOAD = 1024 / (PANEL * sizeof(T)); /* COLUMNS: rows of k that one load covers */
 			int offset[COUNT];
@@ -222,10 +223,10 @@ namespace mlhip
 	 * Where a wavefront's accumulators lie in the tile, and how they leave it. Block (i, j) covers rows row(i) .. + 31 and columns column(j) .. + 31; lane l holds row l % 32 and, in registers 4 q .. 4 q + 3, columns
 	 * 8 q + 4 (l / 32) .. + 3. In a paired product blocks (i, 0) and (i, 1) are the two matrices' sums of the same place.
 	 */
-	template<int BM>
+	template<int BM, int BN>
 	struct TilePlace
 	{
-			static constexpr int BLOCKS = BM / 64, THREADS = 2 * BM;
+			static constexpr int BLOCKS = BM / 64, THREADS = BM == 256 ? 512 : 256;
 			int tile_m, tile_n, part, wave_m, wave_n;
 
 			__device__ __forceinline__ int row(int i) const
@@ -234,7 +235,7 @@ namespace mlhip
 			}
 			__device__ __forceinline__ int column(int j) const
 			{
-				return j * (BM / 2) + wave_n * 32;
+				return j * (BN / 2) + wave_n * 32;
 			}
 			__device__ __forceinline__ static int lane_row()
 			{
@@ -325,13 +326,18 @@ namespace mlhip
 				});
 			}
 	};
-	/* the sums of a tile through LDS in fp32, half its rows at a time: f(m, n, 4 sums in LDS, elements) */
-	template<int BM, typename Acc, typename F>
-	__device__ __forceinline__ void sums_in_rows(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows, int columns, F &&f)
+	/* rows of a tile that lie in LDS at a time in fp32: half of them, of the smallest tile all */
+	constexpr int rows_at_a_time(int rows)
 	{
-		constexpr int ROWS = BM / 2, BLOCKS = TilePlace<BM>::BLOCKS / 2;
-		const Stage<float, BM> stage { reinterpret_cast<float*>(lds) };
-		static_for<2>([&](auto half)
+		return std::max(rows / 2, 64);
+	}
+	/* the sums of a tile through LDS in fp32: f(m, n, 4 sums in LDS, elements) */
+	template<int BM, int BN, typename Acc, typename F>
+	__device__ __forceinline__ void sums_in_rows(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows, int columns, F &&f)
+	{
+		constexpr int ROWS = rows_at_a_time(BM), BLOCKS = ROWS / 64;
+		const Stage<float, BN> stage { reinterpret_cast<float*>(lds) };
+		static_for<BM / ROWS>([&](auto half)
 		{
 			constexpr int h = decltype(half)::value;
 			__syncthreads();
@@ -346,7 +352,7 @@ namespace mlhip
 						stage.put(at.row(i) - h * ROWS, at.column(j) + at.lane_column(q), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 					}
 			__syncthreads();
-			stage.template for_vectors<ROWS, TilePlace<BM>::THREADS>(at.tile_m * BM + h * ROWS, rows, at.tile_n * BM, columns, f);
+			stage.template for_vectors<ROWS, TilePlace<BM, BN>::THREADS>(at.tile_m * BM + h * ROWS, rows, at.tile_n * BN, columns, f);
 		});
 	}
 
@@ -514,15 +520,15 @@ namespace mlhip
 		if (c < chunks)
 			process_chunk(c, std::false_type(), std::false_type());
 
-		epilogue.template tile<256>(acc, TilePlace<256> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
+		epilogue.template tile<256, 256>(acc, TilePlace<256, 256> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
 	}
 
-	template<typename T, Side SA, Side SB, bool PAIRED, int SLOTS, typename Epilogue>
+	template<typename T, Side SA, Side SB, bool PAIRED, int BM, int SLOTS, typename Epilogue>
 	__global__ __launch_bounds__(256, SLOTS == 1 ? 4 : 2) void kernel_product_128(ProductArgs p, Epilogue epilogue)
 	{
 		typedef MfmaTraits<T> Traits;
 		typedef typename Traits::acc_vec acc_vec;
-		constexpr int WAVES = 4, SLOT = 2 * PANEL_BYTES;
+		constexpr int WAVES = 4, A_BYTES = BM * 128, SLOT = A_BYTES + PANEL_BYTES, BLOCKS = BM / 64;
 		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 		int tile_m, tile_n;
 		tile_of_block(p, tile_m, tile_n);
@@ -530,11 +536,11 @@ namespace mlhip
 		const int chunks = min(p.chunks_per_part, p.chunks - first_chunk);
 		const int wave = wave_number(), wave_m = wave >> 1, wave_n = wave & 1;
 
-		PanelLoads<T, SA, WAVES> a_loads;
+		PanelLoads<T, SA, WAVES, PANEL, BM> a_loads;
 		PanelLoads<T, SB, WAVES, PAIRED ? 64 : PANEL> b_loads;
 		PanelWalk<T, SA> a_walk;
 		PanelWalk<T, SB> b_walk;
-		const int m0 = tile_m * PANEL, n0 = tile_n * (PAIRED ? 64 : PANEL);
+		const int m0 = tile_m * BM, n0 = tile_n * (PAIRED ? 64 : PANEL);
 		a_loads.begin(p.a.extent - m0, p.a.row_bytes, 0);
 		a_walk.begin(p.a, m0, first_chunk, chunks);
 		b_loads.begin(p.b.extent - n0, p.b.row_bytes, p.b.pair_bytes);
@@ -543,22 +549,22 @@ namespace mlhip
 		{
 			uint8_t *slot = lds + chunk % SLOTS * SLOT;
 			a_loads.request(a_walk.base, a_walk.left, slot);
-			b_loads.request(b_walk.base, b_walk.left, slot + PANEL_BYTES);
+			b_loads.request(b_walk.base, b_walk.left, slot + A_BYTES);
 			a_walk.advance();
 			b_walk.advance();
 		};
 		/* block (i, j): rows i 64 + wave_m 32, columns j 64 + wave_n 32 */
-		PanelFragments<T, SA> a_place[2];
+		PanelFragments<T, SA> a_place[BLOCKS];
 		PanelFragments<T, SB> b_place[2];
 #pragma unroll
-		for (int i = 0; i < 2; i++)
-		{
+		for (int i = 0; i < BLOCKS; i++)
 			a_place[i].begin(2 * i + wave_m);
-			b_place[i].begin(2 * i + wave_n);
-		}
-		acc_vec acc[2][2];
 #pragma unroll
-		for (int i = 0; i < 2; i++)
+		for (int j = 0; j < 2; j++)
+			b_place[j].begin(2 * j + wave_n);
+		acc_vec acc[BLOCKS][2];
+#pragma unroll
+		for (int i = 0; i < BLOCKS; i++)
 #pragma unroll
 			for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -584,55 +590,61 @@ namespace mlhip
 #pragma unroll
 			for (int kk = 0; kk < 4; kk++)
 			{
-				uint4_t fa[2], fb[2];
+				uint4_t fa[BLOCKS], fb[2];
 #pragma unroll
-				for (int i = 0; i < 2; i++)
-				{
+				for (int i = 0; i < BLOCKS; i++)
 					fa[i] = a_place[i].read(slot, kk);
-					fb[i] = b_place[i].read(slot + PANEL_BYTES, kk);
-				}
 #pragma unroll
-				for (int i = 0; i < 2; i++)
+				for (int j = 0; j < 2; j++)
+					fb[j] = b_place[j].read(slot + A_BYTES, kk);
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++)
 #pragma unroll
 					for (int j = 0; j < 2; j++)
 						Traits::mma(fb[j], fa[i], acc[i][j]);
 			}
 		}
-		epilogue.template tile<128>(acc, TilePlace<128> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
+		epilogue.template tile<BM, 128>(acc, TilePlace<BM, 128> { tile_m, tile_n, static_cast<int>(blockIdx.y), wave_m, wave_n }, lds, p.rows);
 	}
-	/* slots, or what an epilogue lays out there: Epilogue::lds<BM>() bytes */
+	/* slots, or what an epilogue lays out there: Epilogue::lds<BM, BN>() bytes */
 	template<typename Epilogue>
 	constexpr int product_lds(int tile, int slots)
 	{
-		return tile == 256 ? std::max(8 * PANEL_BYTES, Epilogue::template lds<256>()) : std::max(2 * slots * PANEL_BYTES, Epilogue::template lds<128>());
+		return tile == 256 ? std::max(8 * PANEL_BYTES, Epilogue::template lds<256, 256>())
+				: tile == 128 ? std::max(2 * slots * PANEL_BYTES, Epilogue::template lds<128, 128>()) : std::max(slots * (PANEL_BYTES + 64 * 128), Epilogue::template lds<64, 128>());
 	}
 	constexpr int LDS_OF_A_UNIT = 160 * 1024;
 
-	/* how a product is cut: tiles of `tile` rows and columns, `parts` along k. A workspace is sized by the same rule, so it asks no device */
+	/* how a product is cut: tiles of `tile` rows and as many columns (at least 128), `parts` along k. A workspace is sized by the same rule, so it asks no device */
 	struct ProductPlan
 	{
 			int tile, slots, tiles_m, tiles_n, chunks, parts, chunks_per_part;
 	};
 	/*
-	 * The cheapest of both tile sizes and up to 16 parts, by what they take: a compute unit works off its tiles one after the other (two of 128x128 side by side take as long as one after the other), a tile takes
+	 * The cheapest of the tile sizes and up to 16 parts, by what they take: a compute unit works off its tiles one after the other (two of 128x128 side by side take as long as one after the other), a tile takes
 	 * so long per chunk and something for its beginning and end, and parts have to be added up. Microseconds on a full chip, fp16 / fp32: a chunk of 256x256 1.7 / 7.8 (1.2 where at most half of the units have
 	 * a tile: what they read then comes faster), of 128x128 0.6 / 2.05 (its operands' way out of the L2 bounds it in fp16: 32 KB, 30 bytes per clock and unit), and where there are four workgroups to
 	 * every unit, which one slot each lets in, 0.5 / 2.15 and hardly any beginning and end. Measured, two sides each: dx of 4096 x 2048, k = 16384, fp16 (128 tiles of 256x256) whole 313, in 2 parts 228, 128x128 tiles 310; dW of
 	 * 11008 x 2048, k = 8192, fp16 (344 tiles) 388, 385, 379; 2048 x 1024, k = 8192, fp16 143, 87, 79, 128x128 in 2 parts 53; dW of 5462 x 1000, k = 1111, fp32 270, 160, 147, 128x128 in 2 parts 127. 57600 rows
 	 * -> 2 x 1024 columns fp16, 256x256 / 128x128 with two slots / with one: k = 256 118 / 118 / 105, both projections kept 146 / 146 / 121, k = 512 160 / 179 / 157, k = 1024 264 / 298 / 277; 512 rows, k = 1024 -> 2 x 4096
 	 * 26 / 17 / 20; fp32 57600 rows, k = 256 -> 2 x 1024 589 / 551 / 520, 8192 rows, k = 2048 -> 2 x 2048 1011 / 1071 / 1100.
+	 * 64x128 tiles, fp32 with A in rows: half a tile is half the work there, so the last turn costs less and few rows are padded less (901 rows, k = 520 -> 10007 117 -> 109, 64 rows, k = 1024 -> 30000 75 -> 46); in fp16 they would read
+	 * more operands per product, which bounds even 128x128.
 	 * columns: of the result (of one of the two matrices where the operand is paired)
 	 */
-	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split, double *cost_out = nullptr)
+	inline ProductPlan plan_product(int rows, int columns, bool paired, int depth, int element_size, bool may_split, bool a_in_rows = true, double *cost_out = nullptr)
 	{
 		constexpr int UNITS = 256;
 		const bool half = element_size == 2;
 		const int chunks = ceil_div(depth, 128 / element_size);
 		ProductPlan best { 256, 2, 0, 0, chunks, 1, std::max(1, chunks) };
 		double least = 0.0;
-		for (int tile : { 256, 128 })
+		for (int tile : { 256, 128, 64 })
 		{
-			const int tiles_m = ceil_div(rows, tile), tiles_n = ceil_div(columns, paired ? tile / 2 : tile);
+			if (tile == 64 && (half || !a_in_rows))
+				continue;
+			const int width = std::max(tile, 128);
+			const int tiles_m = ceil_div(rows, tile), tiles_n = ceil_div(columns, paired ? width / 2 : width);
 			const double tiles = static_cast<double>(tiles_m) * tiles_n;
 			const int most = (may_split && tiles < 2 * UNITS) ? std::max(1, std::min(16, chunks / 4)) : 1;
 			for (int parts = 1; parts <= most; parts++)
@@ -645,6 +657,8 @@ namespace mlhip
 				int slots = 2;
 				if (tile == 256)
 					cost = std::ceil(work) * (7.0 + per_part * (half ? (work <= 0.5 ? 1.2 : 1.7) : 7.8));
+				else if (tile == 64)
+					cost = std::ceil(work) * (3.0 + per_part * 1.1);
 				else
 				{
 					cost = std::ceil(work) * (4.0 + per_part * (half ? 0.6 : 2.05));
@@ -677,11 +691,11 @@ namespace mlhip
 			ProductPlan first, rest;
 			int first_rows; /* the rest may be none */
 	};
-	inline TwoPlans plan_in_turns(int rows, int columns, int depth, int element_size)
+	inline TwoPlans plan_in_turns(int rows, int columns, int depth, int element_size, bool a_in_rows)
 	{
 		constexpr int UNITS = 256;
 		double whole, first, rest;
-		TwoPlans best { plan_product(rows, columns, false, depth, element_size, true, &whole), ProductPlan { }, rows };
+		TwoPlans best { plan_product(rows, columns, false, depth, element_size, true, a_in_rows, &whole), ProductPlan { }, rows };
 		for (int tile : { 256, 128 })
 		{
 			const int tiles_n = ceil_div(columns, tile), turns = static_cast<int>(static_cast<long long>(ceil_div(rows, tile)) * tiles_n / UNITS);
@@ -690,7 +704,7 @@ namespace mlhip
 			const int first_rows = turns * UNITS / tiles_n * tile;
 			if (first_rows >= rows)
 				continue;
-			TwoPlans two { plan_product(first_rows, columns, false, depth, element_size, false, &first), plan_product(rows - first_rows, columns, false, depth, element_size, true, &rest), first_rows };
+			TwoPlans two { plan_product(first_rows, columns, false, depth, element_size, false, a_in_rows, &first), plan_product(rows - first_rows, columns, false, depth, element_size, true, a_in_rows, &rest), first_rows };
 			if (first + rest + 3.0 < 0.95 * whole)
 			{
 				whole = first + rest + 3.0;
@@ -717,17 +731,29 @@ namespace mlhip
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 			hipLaunchKernelGGL(kernel, grid, dim3(512), bytes, stream, args, epilogue);
 		}
+		else if (plan.tile == 64)
+		{
+			if constexpr (sizeof(T) == 4 && SA == Side::ROWS)
+			{
+				constexpr int bytes = product_lds<Epilogue>(64, 2);
+				auto kernel = kernel_product_128<T, SA, SB, PAIRED, 64, 2, Epilogue>;
+				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+				hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
+			}
+			else
+				fail_logic("HIP backend: tiles of 64 rows are for fp32 rows");
+		}
 		else if (plan.slots == 2)
 		{
 			constexpr int bytes = product_lds<Epilogue>(128, 2);
-			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 2, Epilogue>;
+			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 128, 2, Epilogue>;
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
 		}
 		else
 		{
 			constexpr int bytes = product_lds<Epilogue>(128, 1);
-			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 1, Epilogue>;
+			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 128, 1, Epilogue>;
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
 		}
@@ -743,22 +769,22 @@ namespace mlhip
 			float beta;
 			const float *scale; /* on the device; null: 1 */
 
-			template<int BM>
+			template<int BM, int BN>
 			static constexpr int lds()
 			{
-				return std::max(Stage<float, BM>::bytes(BM / 2), sizeof(Out) == 2 ? Stage<Out, BM>::bytes(BM) : 0);
+				return std::max(Stage<float, BN>::bytes(rows_at_a_time(BM)), sizeof(Out) == 2 ? Stage<Out, BN>::bytes(BM) : 0);
 			}
-			template<int BM, typename Acc>
-			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
 				const float factor = scale != nullptr ? *scale : 1.0f;
 				if (sizeof(Out) == 2 && beta == 0.0f)
 				{
 					/* rounded in registers: the whole tile in one go */
-					const Stage<Out, BM> stage { reinterpret_cast<Out*>(lds) };
+					const Stage<Out, BN> stage { reinterpret_cast<Out*>(lds) };
 					__syncthreads();
 #pragma unroll
-					for (int i = 0; i < TilePlace<BM>::BLOCKS; i++)
+					for (int i = 0; i < TilePlace<BM, BN>::BLOCKS; i++)
 #pragma unroll
 						for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -768,10 +794,10 @@ namespace mlhip
 								stage.put(at.row(i), at.column(j) + at.lane_column(q), v[4 * q] * factor, v[4 * q + 1] * factor, v[4 * q + 2] * factor, v[4 * q + 3] * factor);
 							}
 					__syncthreads();
-					stage.template copy<BM, TilePlace<BM>::THREADS>(out, columns, at.tile_m * BM, rows, at.tile_n * BM, columns);
+					stage.template copy<BM, TilePlace<BM, BN>::THREADS>(out, columns, at.tile_m * BM, rows, at.tile_n * BN, columns);
 				}
 				else
-					sums_in_rows<BM>(acc, at, lds, rows, columns, [&](int m, int n, const float *sums, int there) __attribute__((always_inline))
+					sums_in_rows<BM, BN>(acc, at, lds, rows, columns, [&](int m, int n, const float *sums, int there) __attribute__((always_inline))
 					{
 						Out *dst = out + static_cast<size_t>(m) * columns + n;
 						float v[4];
@@ -806,16 +832,16 @@ namespace mlhip
 			int columns;
 			bool add;
 
-			template<int BM>
+			template<int BM, int BN>
 			static constexpr int lds()
 			{
-				return Stage<float, BM>::bytes(BM / 2);
+				return Stage<float, BN>::bytes(rows_at_a_time(BM));
 			}
-			template<int BM, typename Acc>
-			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM>::BLOCKS][2], const TilePlace<BM> &at, uint8_t *lds, int rows) const
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
 				float *out = partial + at.part * part_stride;
-				sums_in_rows<BM>(acc, at, lds, rows, columns, [&](int m, int n, const float *sums, int there) __attribute__((always_inline))
+				sums_in_rows<BM, BN>(acc, at, lds, rows, columns, [&](int m, int n, const float *sums, int there) __attribute__((always_inline))
 				{
 					float *dst = out + static_cast<size_t>(m) * columns + n;
 					if (there == 4)
