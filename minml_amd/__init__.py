@@ -4,6 +4,7 @@
   minml_amd/csrc/               HIP kernels and the C-ABI implementation -> minml_amd/libminml_hip.so
   minml_amd/backend.py          ctypes binding of that library
   minml_amd/core.py             Context / Tensor / math functions named as in the reference's core
+                                and the operators with a backward pass (layer norm, gated dense, cross entropy)
   minml_amd/conv2d.py           Conv2D layer mirror (algorithm choice, workspace contract, int8 path)
   minml_amd/resnet.py           the synthetic residual network of the benchmark configurations
 """

@@ -5,14 +5,16 @@
  *   d[i, j] = (exp(z[i, j] - lse[i]) - [j = target[i]]) dloss[i]
  *   dx = d W,   dW = d^T x,   db[j] = sum_i d[i, j]
  *
- * Forward: a tile's logits stay in the accumulators; every row of the tile leaves its largest logit and the sum of exponentials about it, and a second launch joins these pairs. Up to 64 rows the
- * weights stream through registers instead (few_rows.hpp) and memory bounds it; above, the matrix cores do.
+ * Forward: a tile's logits stay in the accumulators; every row of the tile leaves its largest logit and the sum of exponentials about it, and a second launch joins these pairs. A few rows stream
+ * the weights past themselves instead (few_rows.hpp) and memory bounds it; else the matrix cores do.
  * Backward: the classes are taken in pieces of as many as make d 256 MB (so it stays in the last-level cache between its makers and users, and the workspace small whatever the vocabulary). For each
  * piece the logits are made again, which costs a quarter of the operations and spares rows x classes of memory; the epilogue turns them into d; then d is multiplied with the piece's weights, added to
  * dx in fp32, and with x, which gives the piece's rows of dW.
  * d is stored in the tensors' type. In fp16 a probability of one class in 100 000 would be subnormal, and the rows' dloss may be anything, so d is scaled by 2^15 / s with s the power of two above the
  * largest |dloss|: the largest d is 2^15 then, and probabilities down to 2e-9 keep their 11 bits. The products' results are scaled back, exactly, in fp32. Its rounding, half a step per element, averages
  * out in the sums; db is summed before it.
+ * fp16: 7 rows of 2048 x 65536 classes 50 us (5.3 TB/s); 4096 rows of 1024 x 50001 433 us (0.97 PFLOP/s), of 2048 x 65536 940 us (1.17); the gradients of the latter 2.93 ms, in two pieces of d 553 us each (0.99 PFLOP/s, a
+ * fourth of it the epilogue), dx 461 (1.19), dW 457 (1.20).
  */
 #include "few_rows.hpp"
 #include "product_tiles.hpp"
@@ -119,7 +121,7 @@ namespace
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
 				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, WAVES_N = BN / 64;
-				constexpr float NOTHING = -std::numeric_limits<float>::infinity();
+				constexpr float NOTHING = -std::numeric_limits<float>::infinity(), LOG2_E = 1.44269504088896341f;
 				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
 				int target[BLOCKS];
@@ -156,13 +158,13 @@ namespace
 #pragma unroll
 						for (int r = 0; r < 16; r++)
 							top = fmaxf(top, z[j][r]);
-					const float about = top == NOTHING ? 0.0f : top; /* a row of -inf alone: a sum of zeros */
+					const float scaled = top == NOTHING ? 0.0f : top * -LOG2_E; /* a row of -inf alone: a sum of zeros */
 					float sum = 0.0f;
 #pragma unroll
 					for (int j = 0; j < 2; j++)
 #pragma unroll
 						for (int r = 0; r < 16; r++)
-							sum += __expf(z[j][r] - about);
+							sum += __builtin_amdgcn_exp2f(fmaf(z[j][r], LOG2_E, scaled)); /* exp(z - top): `scaled` is half a step off, no more than the rounding of lse itself */
 					if (top == -NOTHING) /* infinite logits are all that counts */
 					{
 						sum = 0.0f;
