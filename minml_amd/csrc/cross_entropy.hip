@@ -121,7 +121,7 @@ namespace
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
 				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, WAVES_N = BN / 64;
-				constexpr float NOTHING = -std::numeric_limits<float>::infinity(), LOG2_E = 1.44269504088896341f;
+				constexpr float NOTHING = -std::numeric_limits<float>::infinity();
 				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
 				int target[BLOCKS];
@@ -158,13 +158,13 @@ namespace
 #pragma unroll
 						for (int r = 0; r < 16; r++)
 							top = fmaxf(top, z[j][r]);
-					const float scaled = top == NOTHING ? 0.0f : top * -LOG2_E; /* a row of -inf alone: a sum of zeros */
+					const float about = top == NOTHING ? 0.0f : top; /* a row of -inf alone: a sum of zeros */
 					float sum = 0.0f;
 #pragma unroll
 					for (int j = 0; j < 2; j++)
 #pragma unroll
 						for (int r = 0; r < 16; r++)
-							sum += __builtin_amdgcn_exp2f(fmaf(z[j][r], LOG2_E, scaled)); /* exp(z - top): `scaled` is half a step off, no more than the rounding of lse itself */
+							sum += __expf(z[j][r] - about); /* not exp2 of a product and a sum: the type's lowest value, which masks, has no product */
 					if (top == -NOTHING) /* infinite logits are all that counts */
 					{
 						sum = 0.0f;

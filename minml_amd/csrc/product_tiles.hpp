@@ -949,16 +949,30 @@ namespace mlhip
 				: std::max(part_bytes(plans.first, plans.first_rows, columns), part_bytes(plans.rest, rows - plans.first_rows, columns));
 	}
 
-	/* rows of `columns` elements copied to rows that are whole 16-byte pieces, zeros behind the last element: what the panels' loads ask of an operand whose rows end anywhere */
+	/*
+	 * Rows of `columns` elements copied to rows that are whole 16-byte pieces, zeros behind the last element: what the panels' loads ask of an operand whose rows end anywhere. A thread writes a piece, which it
+	 * reads in one go, at whatever address; pieces of a launch are counted with 32 bits while they fit (split_index).
+	 */
 	template<typename T>
-	__global__ __launch_bounds__(256) void kernel_pad_rows(const T *src, T *dst, size_t rows, int columns, int padded)
+	__global__ __launch_bounds__(256) void kernel_pad_rows(const T *src, T *dst, size_t rows, int columns, int pieces)
 	{
-		const size_t count = rows * padded;
+		constexpr int N = 16 / sizeof(T);
+		typedef typename Elements<T, N>::vec_t vec_t;
+		const size_t count = rows * pieces;
 		for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<size_t>(gridDim.x) * 256)
 		{
-			int column;
-			const size_t row = split_index(i, padded, column);
-			dst[i] = column < columns ? src[row * columns + column] : static_cast<T>(0.0f);
+			int piece;
+			const size_t row = split_index(i, pieces, piece);
+			const T *from = src + row * columns + piece * N;
+			const int there = columns - piece * N;
+			Elements<T, N> v;
+			if (there >= N)
+				v.load(from);
+			else
+#pragma unroll
+				for (int e = 0; e < N; e++)
+					v.raw[e] = e < there ? from[e] : static_cast<T>(0.0f);
+			*reinterpret_cast<vec_t*>(dst + i * N) = v.raw;
 		}
 	}
 	template<typename T>
@@ -972,8 +986,10 @@ namespace mlhip
 		const int padded = padded_columns<T>(columns);
 		if (padded == columns)
 			return src;
-		const size_t groups = std::min<size_t>((rows * padded + 255) / 256, 16384);
-		hipLaunchKernelGGL((kernel_pad_rows<T>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, src, space, rows, columns, padded);
+		const int pieces = padded * static_cast<int>(sizeof(T)) / 16;
+		const size_t groups = std::min<size_t>((rows * pieces + 255) / 256, 16384);
+		if (groups > 0)
+			hipLaunchKernelGGL((kernel_pad_rows<T>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, src, space, rows, columns, pieces);
 		MLHIP_CHECK(hipGetLastError());
 		return space;
 	}
