@@ -336,13 +336,14 @@ namespace
 		if (threadIdx.x == 0)
 			*back = ldexpf(1.0f, exponent - SCALE_BITS);
 	}
-	template<typename T>
+	/* WITH_LOW: what rounding leaves of d is written too */
+	template<typename T, bool WITH_LOW>
 	struct GradientEpilogue
 	{
 			const T *bias; /* of the piece */
 			const int *targets;
 			const float *lse, *factors;
-			T *d; /* [rows][row_elements], zeros behind the piece's classes */
+			T *d, *low; /* [rows][row_elements], zeros behind the piece's classes */
 			float *sums; /* [row tiles][classes of the piece], or null */
 			int first_class, classes, row_elements; /* classes: of the piece */
 
@@ -379,6 +380,9 @@ namespace
 				static_for<PASSES>([&](auto pass)
 				{
 					constexpr int PASS = decltype(pass)::value, FIRST = PASS * BLOCKS / PASSES;
+					static_for<WITH_LOW ? 2 : 1>([&](auto half) __attribute__((always_inline))
+					{
+					constexpr int part = decltype(half)::value;
 					__syncthreads();
 #pragma unroll
 					for (int i = FIRST; i < FIRST + BLOCKS / PASSES; i++)
@@ -401,6 +405,12 @@ namespace
 							{
 								v[j][r] -= factor[i];
 							});
+						if constexpr (part == 1)
+#pragma unroll
+							for (int j = 0; j < 2; j++)
+#pragma unroll
+								for (int r = 0; r < 16; r++)
+									v[j][r] = low_part<T>(v[j][r]);
 #pragma unroll
 						for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -409,11 +419,12 @@ namespace
 								stage.put(at.row(i) - PASS * ROWS, at.column(j) + at.lane_column(q), v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
 #pragma unroll
 								for (int e = 0; e < 4; e++)
-									total[j][4 * q + e] += v[j][4 * q + e];
+									total[j][4 * q + e] += part == 0 ? v[j][4 * q + e] : 0.0f;
 							}
 					}
 					__syncthreads();
-					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
+					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(part == 0 ? d : low, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
+					});
 				});
 				if (sums == nullptr)
 					return;
@@ -479,9 +490,14 @@ namespace
 	{
 		return plan_product(s.rows, classes, false, s.features, s.element_size, false);
 	}
+	/* rows of d: with its low part, which dx is made of too, twice as many */
+	int rows_of_d(const LossShape &s)
+	{
+		return keeps_low_part(s.rows, s.element_size) ? 2 * s.rows : s.rows;
+	}
 	ProductPlan input_plan(const LossShape &s, int classes)
 	{
-		return plan_product(s.rows, s.features, false, classes, s.element_size, true);
+		return plan_product(rows_of_d(s), s.features, false, classes, s.element_size, true);
 	}
 	ProductPlan weights_plan(const LossShape &s, int classes)
 	{
@@ -521,8 +537,8 @@ namespace
 				at = begin;
 				const int classes = classes_of_piece(s);
 				const ProductPlan input = input_plan(s, classes), weights = weights_plan(s, classes);
-				space.d = take(round_up(classes, pieces) * s.element_size * s.rows);
-				space.dx = take((classes < s.classes || input.parts > 1) ? sizeof(float) * input.parts * s.rows * s.features : 0);
+				space.d = take(round_up(classes, pieces) * s.element_size * rows_of_d(s));
+				space.dx = take((classes < s.classes || input.parts > 1 || rows_of_d(s) > s.rows) ? sizeof(float) * input.parts * rows_of_d(s) * s.features : 0);
 				space.parts = take(part_bytes(weights, classes, s.features));
 				space.sums = take(sizeof(float) * classes * logits_plan(s, classes).tiles_m);
 				space.factors = take(sizeof(float) * s.rows);
@@ -593,7 +609,8 @@ namespace
 		w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
 		const size_t row_bytes = padded * sizeof(T), outputs = static_cast<size_t>(s.rows) * s.features;
 		const ProductPlan whole_input = input_plan(s, most);
-		const bool dx_in_parts = most < s.classes || whole_input.parts > 1;
+		const int d_rows = rows_of_d(s), halves = d_rows / std::max(s.rows, 1); /* [part][d, its low part][rows][features] */
+		const bool dx_in_parts = most < s.classes || whole_input.parts > 1 || halves > 1;
 		/* the last piece, which may be smaller, is cut by the plans of the others: the workspace is sized by them */
 		for (int first = 0; first < s.classes; first += most)
 		{
@@ -604,8 +621,20 @@ namespace
 				plan.tiles_n = ceil_div(classes, std::max(plan.tile, 128));
 				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
 				const Operand b { weights, row_bytes, classes, padded };
-				launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T> { bias != nullptr ? bias + first : nullptr, targets, lse, factors, d,
-						db.data != nullptr ? sums : nullptr, first, classes, row_elements });
+				const auto make_d = [&](auto with_low)
+				{
+					launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T, decltype(with_low)::value> { bias != nullptr ? bias + first : nullptr, targets, lse,
+							factors, d, d + static_cast<size_t>(s.rows) * row_elements, db.data != nullptr ? sums : nullptr, first, classes, row_elements });
+				};
+				if constexpr (sizeof(T) == 2)
+				{
+					if (halves > 1 && dx != nullptr)
+						make_d(std::true_type());
+					else
+						make_d(std::false_type());
+				}
+				else
+					make_d(std::false_type());
 				if (db.data != nullptr)
 					launch_sum_partials(stream, sums, plan.tiles_m, static_cast<size_t>(classes), static_cast<uint8_t*>(db.data) + static_cast<size_t>(first) * size_of(db.dtype), db.dtype, classes,
 							beta_weights, back);
@@ -614,10 +643,10 @@ namespace
 			{
 				ProductPlan plan = whole_input; /* a part that has no chunk left adds nothing */
 				plan.chunks = ceil_div(classes, 128 / static_cast<int>(sizeof(T)));
-				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), s.rows, row_elements };
+				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), d_rows, row_elements };
 				const Operand b { weights, row_bytes, padded, classes };
 				if (dx_in_parts)
-					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, d_rows, PartEpilogue { partial_dx, halves * outputs, s.features, first > 0 });
 				else
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, StoreEpilogue<T> { dx, s.features, beta_dx, back });
 			}
@@ -635,7 +664,7 @@ namespace
 			}
 		}
 		if (dx != nullptr && dx_in_parts)
-			launch_join_parts(stream, partial_dx, whole_input.parts, outputs, dx, beta_dx, back);
+			launch_join_parts(stream, partial_dx, halves * whole_input.parts, outputs, dx, beta_dx, back);
 	}
 
 	bool weight_type(const mlTensor_t &t, const mlTensor_t &x)

@@ -9,7 +9,8 @@
  * them (`projections`, in the tensors' type). Up to 64 rows the weights stream through registers (few_rows.hpp). Where there are too few tiles for the chip the product is split along the
  * features, and the launch that adds the parts up applies the gate.
  * Backward: one pass over dy and the projections makes d and the partial sums of db (bound by memory), then two products (bound by the matrix cores). d is stored in the tensors' type: its rounding, half a step per
- * element, averages out in sums over as many hidden units or rows as the products have, and is what a stored gradient costs anywhere else in a network of that type; db is summed before the rounding.
+ * element, averages out in sums over as many hidden units or rows as the products have, and is what a stored gradient costs anywhere else in a network of that type (few
+ * rows: keeps_low_part); db is summed before the rounding.
  * fp16: 1 row of 4096 -> 8192 23.5 us (5.7 TB/s); 57600 x 256 -> 1024 with gelu, bias and the projections kept 133 us (2.9 TB/s: neither memory, 74 us, nor the matrix cores, 47 us, but what is left of their
  * overlap with the gate's arithmetic); backward of 8192 x 2048 -> 5504 715 us (1.03 PFLOP/s): d 77 us (5.9 TB/s), dx 303 us (1.22 PFLOP/s), dW 340 us.
  */
@@ -257,9 +258,9 @@ namespace
 
 	/* ---- backward: d and the sums of its columns ------------------------------------------------------------------------------
 	 * d [rows][row_elements] holds dg at column n and du at column hidden + n, zeros from 2 hidden on. A workgroup has 256 hidden units (32 threads of 8) and 8 rows at a time of its share of the rows;
-	 * partial [gridDim.y][2 hidden] takes the sums over its rows. */
+	 * partial [gridDim.y][2 hidden] takes the sums over its rows. What rounding leaves goes `low` elements further, if that is not 0. */
 	template<typename T>
-	__global__ __launch_bounds__(256) void kernel_gated_gradient(const T *projections, const T *dy, T *d, int rows, int hidden, int row_elements, int gate, float *partial)
+	__global__ __launch_bounds__(256) void kernel_gated_gradient(const T *projections, const T *dy, T *d, int rows, int hidden, int row_elements, int gate, float *partial, size_t low)
 	{
 		__shared__ float sums[2][8][32 * 8 + 8];
 		const int group = threadIdx.x & 31, first_row = threadIdx.x >> 5;
@@ -295,6 +296,17 @@ namespace
 				}
 				store_nearest<8>(dst, dg);
 				store_nearest<8>(dst + hidden, du);
+				if (low != 0)
+				{
+#pragma unroll
+					for (int e = 0; e < 8; e++)
+					{
+						dg[e] = low_part<T>(dg[e]);
+						du[e] = low_part<T>(du[e]);
+					}
+					store_nearest<8>(dst + low, dg);
+					store_nearest<8>(dst + low + hidden, du);
+				}
 			}
 			else
 			{
@@ -310,11 +322,19 @@ namespace
 						sum[1][e] += du;
 						dst[e] = static_cast<T>(dg);
 						dst[hidden + e] = static_cast<T>(du);
+						if (low != 0)
+						{
+							dst[low + e] = static_cast<T>(low_part<T>(dg));
+							dst[low + hidden + e] = static_cast<T>(low_part<T>(du));
+						}
 					}
 			}
 			if (n == 0)
 				for (int j = 2 * hidden; j < row_elements; j++)
+				{
 					d[static_cast<size_t>(row) * row_elements + j] = static_cast<T>(0.0f);
+					d[static_cast<size_t>(row) * row_elements + low + j] = static_cast<T>(0.0f);
+				}
 		}
 		if (partial == nullptr)
 			return;
@@ -374,6 +394,11 @@ namespace
 	{
 		return plan_in_turns(s.rows, s.features, 2 * s.hidden, s.element_size, true);
 	}
+	/* of d with its low part */
+	ProductPlan split_input_plan(const GatedShape &s)
+	{
+		return plan_product(2 * s.rows, s.features, false, 2 * s.hidden, s.element_size, true);
+	}
 	TwoPlans weights_plan(const GatedShape &s)
 	{
 		return plan_in_turns(2 * s.hidden, s.features, s.rows, s.element_size, false);
@@ -400,8 +425,10 @@ namespace
 		space.w = take(tiles ? padded * 2 * s.hidden : 0);
 		if (backward)
 		{
-			space.parts = take(std::max(part_bytes(input_plan(s), s.rows, s.features), part_bytes(weights_plan(s), 2 * s.hidden, s.features)));
-			space.d = take(round_up(2 * s.hidden, pieces) * s.element_size * s.rows);
+			const bool low = keeps_low_part(s.rows, s.element_size);
+			const size_t for_input = low ? sizeof(float) * split_input_plan(s).parts * 2 * s.rows * s.features : part_bytes(input_plan(s), s.rows, s.features);
+			space.parts = take(std::max(for_input, part_bytes(weights_plan(s), 2 * s.hidden, s.features)));
+			space.d = take(round_up(2 * s.hidden, pieces) * s.element_size * s.rows * (low ? 2 : 1));
 			space.sums = take(sizeof(float) * 2 * s.hidden * gradient_parts(s));
 		}
 		else
@@ -456,20 +483,31 @@ namespace
 		T *d = reinterpret_cast<T*>(workspace + space.d);
 		float *sums = reinterpret_cast<float*>(workspace + space.sums), *partial = reinterpret_cast<float*>(workspace + space.parts);
 		const int parts = gradient_parts(s);
+		const bool with_low = keeps_low_part(s.rows, s.element_size) && dx != nullptr;
+		const size_t low = with_low ? static_cast<size_t>(s.rows) * row_elements : 0;
 		if (s.rows > 0 && s.hidden > 0)
 		{
 			hipLaunchKernelGGL((kernel_gated_gradient<T>), dim3(ceil_div(s.hidden, 256), parts), dim3(256), 0, stream, projections, dy, d, s.rows, s.hidden, row_elements, gate,
-					db.data != nullptr ? sums : nullptr);
+					db.data != nullptr ? sums : nullptr, low);
 			MLHIP_CHECK(hipGetLastError());
 		}
 		if (db.data != nullptr)
 			launch_sum_partials(stream, sums, s.rows > 0 ? parts : 0, static_cast<size_t>(both), db.data, db.dtype, both, beta_weights);
-		const Operand d_rows { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), s.rows, row_elements };
+		const Operand d_rows { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), with_low ? 2 * s.rows : s.rows, row_elements };
 		if (dx != nullptr && s.rows > 0)
 		{
 			w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), static_cast<size_t>(both), s.features);
 			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), padded, both };
-			product_to<T, T, Side::ROWS, Side::COLUMNS>(stream, input_plan(s), d_rows, b, s.rows, s.features, dx, beta_dx, nullptr, partial);
+			if (with_low)
+			{
+				/* [part][d, its low part][rows][features]: twice as many parts to add up */
+				const ProductPlan plan = split_input_plan(s);
+				const size_t outputs = static_cast<size_t>(s.rows) * s.features;
+				launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, d_rows, b, 2 * s.rows, PartEpilogue { partial, 2 * outputs, s.features, false });
+				launch_join_parts(stream, partial, 2 * plan.parts, outputs, dx, beta_dx, nullptr);
+			}
+			else
+				product_to<T, T, Side::ROWS, Side::COLUMNS>(stream, input_plan(s), d_rows, b, s.rows, s.features, dx, beta_dx, nullptr, partial);
 		}
 		if (dw.data != nullptr)
 		{
