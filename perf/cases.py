@@ -12,7 +12,7 @@ A case names a kind of pass and its sizes:
 
 `issue` says how the program issues a network's pass: "recorded" replays a recorded pass (core.Graph) as programs with few positions in
 flight do, "calls" makes the library calls one by one, and "layers" (resnet) does so with three calls per 3x3 layer, as the reference's
-own Conv2D issues them. Everything here is inference: the library has no backward path.
+own Conv2D issues them. Everything here is inference; the operators with a backward pass have their cases in operators.py.
 """
 import math
 
