@@ -236,7 +236,7 @@ extern "C"
 	 *      16 bytes, free for anything else once the call's work on the stream is done; calls that may run at the same time (other contexts, graphs replayed on other streams) need one each.
 	 *      Tensors need the alignment of one element only. Results may not overlap inputs unless a call says so. ---- */
 	/*
-	 * y[i, j] = (x[i, j] - mean_i) / sqrt(var_i + epsilon) * w[j] + b[j] over the last dimension; w and b may be empty. y may be x.
+	 * y[i, j] = (x[i, j] - mean_i) / sqrt(var_i + epsilon) * w[j] + b[j] over the last dimension, of at most 2^28 elements; w and b may be empty. y may be x.
 	 * Backward: dx = beta_dx * dx + the gradient of x, dw = beta_weights * dw + sum_i dy n, db = beta_weights * db + sum_i dy; the statistics are computed again from x. dx may be dy or x.
 	 */
 	void hip_layer_norm_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, mlTensor_t y, float epsilon);

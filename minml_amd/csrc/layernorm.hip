@@ -23,6 +23,7 @@ namespace
 
 	constexpr int MAX_PARTS = 512; /* workgroups of a backward pass, two per compute unit: what each leaves is written and read once more */
 	constexpr int LONGEST_IN_REGISTERS = 16384;
+	constexpr int LONGEST_ROW = 1 << 28; /* columns are counted with 32 bits, also one step beyond a row's end, and 8 threads of a launch sum a column */
 
 	/* the threads that share a row, and their sums. LANES <= 64: part of a wavefront; else the whole workgroup, through LDS */
 	template<int LANES>
@@ -531,6 +532,7 @@ namespace
 		MLHIP_REQUIRE(x.rank >= 1 && x.rank <= 6, std::string(name) + ": the input needs one to six dimensions");
 		for (int i = 0; i < x.rank; i++)
 			MLHIP_REQUIRE(x.dim[i] >= 0, std::string(name) + ": negative dimension");
+		MLHIP_REQUIRE(last_dim(x) <= LONGEST_ROW, std::string(name) + ": rows are too long");
 		MLHIP_REQUIRE(x.dtype == DTYPE_FLOAT16 || x.dtype == DTYPE_FLOAT32, std::string(name) + ": unsupported data type");
 	}
 	void require_weight(const mlTensor_t &t, const mlTensor_t &x, bool may_be_fp32, const char *what)

@@ -49,6 +49,16 @@ def test_layer_norm_refusals_of_the_library():
     B.fn("layer_norm_forward")(None, fake((0, 16)).desc(), w, w, fake((0, 16)).desc(), 1e-5)
 
 
+@pytest.mark.parametrize("columns", [2 ** 28 + 1, 2 ** 31 - 1])
+def test_layer_norm_refuses_rows_that_its_counters_do_not_reach(columns):
+    x, y, dy, w = (ml.Tensor(s, "float16", _ptr=(k + 1) << 44).desc() for k, s in enumerate([(2, columns)] * 3 + [(columns,)]))
+    refused("layer_norm_forward", x, w, NULL, y, 1e-5, why="too long")
+    refused("layer_norm_backward", x, w, dy, 0.0, y, 0.0, NULL, NULL, 0x7000, 1 << 50, 1e-5, why="too long")
+    with pytest.raises(ValueError, match="too long"):
+        B.fn("layer_norm_get_workspace_size")(B.make_shape((2, columns)), B.DTYPE_FLOAT16)
+    refused("layer_norm_forward", *(ml.Tensor(s, "float16", _ptr=(k + 1) << 44).desc() for k, s in enumerate([(2, 2 ** 28)] + [(2 ** 28,)] * 2 + [(2, 2 ** 28)])), 1e-5, why="null context")
+
+
 def test_layer_norm_refusals_of_the_mirror():
     class Ctx:
         handle = None
