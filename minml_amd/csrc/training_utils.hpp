@@ -12,6 +12,7 @@
 #include "device_utils.hpp"
 
 #include <initializer_list>
+#include <limits>
 
 namespace mlhip
 {
@@ -218,11 +219,12 @@ namespace mlhip
 	{
 		return element_size == 2 && rows <= 64;
 	}
-	/* what rounding x to the type leaves */
+	/* what rounding x to the type leaves; nothing of what is infinite there, so that infinities stay what they are (inf - inf is no number) */
 	template<typename T>
 	__device__ __forceinline__ float low_part(float x)
 	{
-		return x - static_cast<float>(static_cast<T>(x));
+		const float high = static_cast<float>(static_cast<T>(x));
+		return fabsf(high) <= std::numeric_limits<float>::max() ? x - high : 0.0f;
 	}
 	inline size_t round_up(size_t n, size_t to)
 	{
