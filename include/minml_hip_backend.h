@@ -247,7 +247,8 @@ extern "C"
 	/*
 	 * The gated dense layer: y = a(x Wg^T + bg) * (x Wu^T + bu). x [.., features], w [2, hidden, features] (the gate's matrix, then the other), b [2, hidden] or empty, y [.., hidden]; `projections`
 	 * [.., 2, hidden] takes both projections, which the backward pass needs, or is empty. Backward: dy [.., hidden] -> dx, dw, db as above. x and w have to be aligned to 16 bytes, workspaces of
-	 * these calls to 256. Gradients of the projections are kept in the tensors' type in between.
+	 * these calls to 256. Gradients of the projections are kept in the tensors' type in between, in fp16 with a common power of two where their largest is below 2^-3 or not below 2^15, so that they neither overflow
+	 * nor lose bits; rounded to nearest, which costs dx and dw as much as their own rounding does.
 	 */
 	typedef enum
 	{

@@ -267,24 +267,14 @@ namespace
 
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
 	constexpr int SCALE_GROUPS = 256;
-	constexpr int SCALE_BITS = 15;
-	/* the power of two above the largest |dloss| */
-	__device__ __forceinline__ int scale_exponent(float top)
-	{
-		int exponent = 0;
-		if (top > 0.0f)
-			(void) frexpf(top, &exponent);
-		return max(exponent, -100); /* so that the way back is a normal number */
-	}
 	__global__ __launch_bounds__(256) void kernel_largest_gradient(const float *dloss, const int *targets, int rows, int classes, float *largest)
 	{
 		__shared__ float waves[4];
 		float top = 0.0f;
 		for (int i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256)
 		{
-			const float v = fabsf(dloss[i]);
-			if (targets[i] >= 0 && targets[i] < classes && v <= std::numeric_limits<float>::max())
-				top = fmaxf(top, v);
+			if (targets[i] >= 0 && targets[i] < classes)
+				top = larger_finite(top, dloss[i]);
 		}
 #pragma unroll
 		for (int offset = 32; offset >= 1; offset >>= 1)
@@ -318,9 +308,8 @@ namespace
 		float top = 0.0f;
 		for (int i = threadIdx.x; i < rows; i += 1024)
 		{
-			const float v = fabsf(dloss[i]);
-			if (targets[i] >= 0 && targets[i] < classes && v <= std::numeric_limits<float>::max())
-				top = fmaxf(top, v);
+			if (targets[i] >= 0 && targets[i] < classes)
+				top = larger_finite(top, dloss[i]);
 		}
 #pragma unroll
 		for (int offset = 32; offset >= 1; offset >>= 1)

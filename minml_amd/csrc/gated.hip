@@ -10,7 +10,7 @@
  * features, and the launch that adds the parts up applies the gate.
  * Backward: one pass over dy and the projections makes d and the partial sums of db (bound by memory), then two products (bound by the matrix cores). d is stored in the tensors' type: its rounding, half a step per
  * element, averages out in sums over as many hidden units or rows as the products have, and is what a stored gradient costs anywhere else in a network of that type (few
- * rows: keeps_low_part); db is summed before the rounding.
+ * rows: keeps_low_part); db is summed before the rounding. In fp16 d is scaled where it would leave the type's range (shift_of).
  * fp16: 1 row of 4096 -> 8192 23.5 us (5.7 TB/s); 57600 x 256 -> 1024 with gelu, bias and the projections kept 133 us (2.9 TB/s: neither memory, 74 us, nor the matrix cores, 47 us, but what is left of their
  * overlap with the gate's arithmetic); backward of 8192 x 2048 -> 5504 715 us (1.03 PFLOP/s): d 77 us (5.9 TB/s), dx 303 us (1.22 PFLOP/s), dW 340 us.
  */
@@ -256,13 +256,52 @@ namespace
 		}
 	}
 
-	/* ---- backward: d and the sums of its columns ------------------------------------------------------------------------------
-	 * d [rows][row_elements] holds dg at column n and du at column hidden + n, zeros from 2 hidden on. A workgroup has 256 hidden units (32 threads of 8) and 8 rows at a time of its share of the rows;
-	 * partial [gridDim.y][2 hidden] takes the sums over its rows. What rounding leaves goes `low` elements further, if that is not 0. */
-	template<typename T>
-	__global__ __launch_bounds__(256) void kernel_gated_gradient(const T *projections, const T *dy, T *d, int rows, int hidden, int row_elements, int gate, float *partial, size_t low)
+	/* ---- backward: d and the sums of its columns ------------------------------------------------------------------------------ */
+	/*
+	 * d is in memory as d 2^shift. In fp16 dy u a'(g) may pass the type's largest value, 65504, where dx, a sum of such terms with weights, does not; and gradients of losses that nobody scaled, 1e-5 or so, are subnormal
+	 * there (dw 2.8e-3 off instead of 3e-4, also where it is asked for in fp32). With its largest element between 2^-3 and 2^15 d stays as it is: elements down to 2^-11 of the largest are normal numbers then, and
+	 * those below are off by at most 2^-22 of it. Else the largest is brought just below 2^15, and what the products give is scaled back in fp32, exactly.
+	 */
+	__device__ __forceinline__ int shift_of(float top)
 	{
-		__shared__ float sums[2][8][32 * 8 + 8];
+		const int exponent = scale_exponent(top);
+		return (top == 0.0f || (exponent >= -2 && exponent <= SCALE_BITS)) ? 0 : SCALE_BITS - exponent;
+	}
+	/*
+	 * d [rows][row_elements] holds dg at column n and du at column hidden + n, zeros from 2 hidden on. A workgroup has 256 hidden units (32 threads of 8) and 8 rows at a time of its share of the rows;
+	 * partial [gridDim.y][2 hidden] takes the sums over its rows. What rounding leaves goes `low` elements further, if that is not 0.
+	 * Scaling takes two launches, because only the first one finds out what the largest element is: it leaves that of every workgroup in `largest` (fp16; null: no one asks). The second one (AGAIN) reads the `groups` of them,
+	 * writes `back` = 2^-shift, and is done if there is nothing to scale, as is usual (3 us); else it makes d once more, as many bytes as the first time.
+	 */
+	template<typename T, bool AGAIN>
+	__global__ __launch_bounds__(256) void kernel_gated_gradient(const T *projections, const T *dy, T *d, int rows, int hidden, int row_elements, int gate, float *partial, size_t low, float *largest,
+			int groups, float *back)
+	{
+		__shared__ float sums[AGAIN ? 1 : 2][8][32 * 8 + 8];
+		__shared__ float waves[4];
+		/* of the workgroup's threads */
+		const auto largest_of = [&](float v) __attribute__((always_inline))
+		{
+#pragma unroll
+			for (int offset = 32; offset >= 1; offset >>= 1)
+				v = fmaxf(v, __shfl_xor(v, offset));
+			if ((threadIdx.x & 63) == 0)
+				waves[threadIdx.x >> 6] = v;
+			__syncthreads();
+			return fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+		};
+		float top = 0.0f, factor = 1.0f;
+		if constexpr (AGAIN)
+		{
+			for (int i = threadIdx.x; i < groups; i += 256)
+				top = fmaxf(top, largest[i]);
+			const int shift = shift_of(largest_of(top));
+			if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+				*back = ldexpf(1.0f, -shift);
+			if (shift == 0)
+				return;
+			factor = ldexpf(1.0f, shift);
+		}
 		const int group = threadIdx.x & 31, first_row = threadIdx.x >> 5;
 		const int n = blockIdx.x * 256 + group * 8;
 		float sum[2][8];
@@ -271,6 +310,25 @@ namespace
 #pragma unroll
 			for (int e = 0; e < 8; e++)
 				sum[i][e] = 0.0f;
+		const auto gradient = [&](int e, float g, float u, float v, float &dg, float &du) __attribute__((always_inline))
+		{
+			float a, slope;
+			gate_of<T, true>(gate, g, a, slope);
+			dg = v * u * slope;
+			du = v * a;
+			if constexpr (AGAIN)
+			{
+				dg *= factor;
+				du *= factor;
+			}
+			else
+			{
+				sum[0][e] += dg;
+				sum[1][e] += du;
+				if constexpr (sizeof(T) == 2)
+					top = larger_finite(larger_finite(top, dg), du);
+			}
+		};
 		for (int row = blockIdx.y * 8 + first_row; row < rows; row += gridDim.y * 8)
 		{
 			const T *kept = projections + static_cast<size_t>(row) * 2 * hidden + n;
@@ -286,14 +344,7 @@ namespace
 				float dg[8], du[8];
 #pragma unroll
 				for (int e = 0; e < 8; e++)
-				{
-					float a, slope;
-					gate_of<T, true>(gate, g[e], a, slope);
-					dg[e] = v[e] * u[e] * slope;
-					du[e] = v[e] * a;
-					sum[0][e] += dg[e];
-					sum[1][e] += du[e];
-				}
+					gradient(e, g[e], u[e], v[e], dg[e], du[e]);
 				store_nearest<8>(dst, dg);
 				store_nearest<8>(dst + hidden, du);
 				if (low != 0)
@@ -314,12 +365,8 @@ namespace
 				for (int e = 0; e < 8; e++)
 					if (e < there)
 					{
-						float a, slope;
-						gate_of<T, true>(gate, static_cast<float>(kept[e]), a, slope);
-						const float v = static_cast<float>(grad[e]);
-						const float dg = v * static_cast<float>(kept[hidden + e]) * slope, du = v * a;
-						sum[0][e] += dg;
-						sum[1][e] += du;
+						float dg, du;
+						gradient(e, static_cast<float>(kept[e]), static_cast<float>(kept[hidden + e]), static_cast<float>(grad[e]), dg, du);
 						dst[e] = static_cast<T>(dg);
 						dst[hidden + e] = static_cast<T>(du);
 						if (low != 0)
@@ -336,25 +383,34 @@ namespace
 					d[static_cast<size_t>(row) * row_elements + low + j] = static_cast<T>(0.0f);
 				}
 		}
-		if (partial == nullptr)
-			return;
-#pragma unroll
-		for (int i = 0; i < 2; i++)
-#pragma unroll
-			for (int e = 0; e < 8; e++)
-				sums[i][first_row][group * 8 + e] = sum[i][e];
-		__syncthreads();
-		const int column = blockIdx.x * 256 + threadIdx.x;
-		if (column < hidden)
+		if constexpr (!AGAIN)
+		{
+			if (sizeof(T) == 2 && largest != nullptr)
+			{
+				const float of_all = largest_of(top);
+				if (threadIdx.x == 0)
+					largest[blockIdx.y * gridDim.x + blockIdx.x] = of_all;
+			}
+			if (partial == nullptr)
+				return;
 #pragma unroll
 			for (int i = 0; i < 2; i++)
-			{
-				float total = 0.0f;
 #pragma unroll
-				for (int r = 0; r < 8; r++)
-					total += sums[i][r][threadIdx.x];
-				partial[static_cast<size_t>(blockIdx.y) * 2 * hidden + i * hidden + column] = total;
-			}
+				for (int e = 0; e < 8; e++)
+					sums[i][first_row][group * 8 + e] = sum[i][e];
+			__syncthreads();
+			const int column = blockIdx.x * 256 + threadIdx.x;
+			if (column < hidden)
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+				{
+					float total = 0.0f;
+#pragma unroll
+					for (int r = 0; r < 8; r++)
+						total += sums[i][r][threadIdx.x];
+					partial[static_cast<size_t>(blockIdx.y) * 2 * hidden + i * hidden + column] = total;
+				}
+		}
 	}
 
 	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
@@ -386,6 +442,10 @@ namespace
 		/* about 8 workgroups of 256 threads per compute unit */
 		return std::max(1, std::min(ceil_div(s.rows, 8), 2048 / std::max(1, ceil_div(s.hidden, 256))));
 	}
+	int gradient_groups(const GatedShape &s)
+	{
+		return ceil_div(s.hidden, 256) * gradient_parts(s);
+	}
 	ProductPlan forward_plan(const GatedShape &s)
 	{
 		return plan_product(s.rows, s.hidden, true, s.features, s.element_size, true);
@@ -406,7 +466,7 @@ namespace
 	/* the pieces of a workspace, each aligned to 256 bytes */
 	struct GatedSpace
 	{
-			size_t x, w, parts, d, sums, total;
+			size_t x, w, parts, d, sums, largest, total;
 	};
 	GatedSpace gated_space(const GatedShape &s, bool backward)
 	{
@@ -430,11 +490,12 @@ namespace
 			space.parts = take(std::max(for_input, part_bytes(weights_plan(s), 2 * s.hidden, s.features)));
 			space.d = take(round_up(2 * s.hidden, pieces) * s.element_size * s.rows * (low ? 2 : 1));
 			space.sums = take(sizeof(float) * 2 * s.hidden * gradient_parts(s));
+			space.largest = take(s.element_size == 2 ? sizeof(float) * (gradient_groups(s) + 1) : 0);
 		}
 		else
 		{
 			space.parts = take(tiles ? part_bytes(forward_plan(s), s.rows, 2 * s.hidden) : 0);
-			space.d = space.sums = at;
+			space.d = space.sums = space.largest = at;
 		}
 		space.total = at;
 		return space;
@@ -485,11 +546,24 @@ namespace
 		const int parts = gradient_parts(s);
 		const bool with_low = keeps_low_part(s.rows, s.element_size) && dx != nullptr;
 		const size_t low = with_low ? static_cast<size_t>(s.rows) * row_elements : 0;
+		float *back = nullptr; /* what takes d's scale back */
 		if (s.rows > 0 && s.hidden > 0)
 		{
-			hipLaunchKernelGGL((kernel_gated_gradient<T>), dim3(ceil_div(s.hidden, 256), parts), dim3(256), 0, stream, projections, dy, d, s.rows, s.hidden, row_elements, gate,
-					db.data != nullptr ? sums : nullptr, low);
+			const dim3 grid(ceil_div(s.hidden, 256), parts);
+			const int groups = gradient_groups(s);
+			float *largest = reinterpret_cast<float*>(workspace + space.largest);
+			const bool scaled = sizeof(T) == 2 && (dx != nullptr || dw.data != nullptr); /* else nothing reads d */
+			hipLaunchKernelGGL((kernel_gated_gradient<T, false>), grid, dim3(256), 0, stream, projections, dy, d, s.rows, s.hidden, row_elements, gate, db.data != nullptr ? sums : nullptr, low,
+					scaled ? largest : nullptr, groups, static_cast<float*>(nullptr));
 			MLHIP_CHECK(hipGetLastError());
+			if constexpr (sizeof(T) == 2)
+				if (scaled)
+				{
+					back = largest + groups;
+					hipLaunchKernelGGL((kernel_gated_gradient<T, true>), dim3(grid.x, ceil_div(parts, 2)), dim3(256), 0, stream, projections, dy, d, s.rows, s.hidden, row_elements, gate,
+							static_cast<float*>(nullptr), low, largest, groups, back);
+					MLHIP_CHECK(hipGetLastError());
+				}
 		}
 		if (db.data != nullptr)
 			launch_sum_partials(stream, sums, s.rows > 0 ? parts : 0, static_cast<size_t>(both), db.data, db.dtype, both, beta_weights);
@@ -504,10 +578,10 @@ namespace
 				const ProductPlan plan = split_input_plan(s);
 				const size_t outputs = static_cast<size_t>(s.rows) * s.features;
 				launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, d_rows, b, 2 * s.rows, PartEpilogue { partial, 2 * outputs, s.features, false });
-				launch_join_parts(stream, partial, 2 * plan.parts, outputs, dx, beta_dx, nullptr);
+				launch_join_parts(stream, partial, 2 * plan.parts, outputs, dx, beta_dx, back);
 			}
 			else
-				product_to<T, T, Side::ROWS, Side::COLUMNS>(stream, input_plan(s), d_rows, b, s.rows, s.features, dx, beta_dx, nullptr, partial);
+				product_to<T, T, Side::ROWS, Side::COLUMNS>(stream, input_plan(s), d_rows, b, s.rows, s.features, dx, beta_dx, back, partial);
 		}
 		if (dw.data != nullptr)
 		{
@@ -515,9 +589,9 @@ namespace
 			const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), row_elements, s.rows };
 			const Operand b { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), padded, s.rows };
 			if (dw.dtype == DTYPE_FLOAT32)
-				product_to<T, float, Side::COLUMNS, Side::COLUMNS>(stream, weights_plan(s), a, b, both, s.features, ptr<float>(dw), beta_weights, nullptr, partial);
+				product_to<T, float, Side::COLUMNS, Side::COLUMNS>(stream, weights_plan(s), a, b, both, s.features, ptr<float>(dw), beta_weights, back, partial);
 			else if constexpr (sizeof(T) == 2)
-				product_to<T, T, Side::COLUMNS, Side::COLUMNS>(stream, weights_plan(s), a, b, both, s.features, ptr<T>(dw), beta_weights, nullptr, partial);
+				product_to<T, T, Side::COLUMNS, Side::COLUMNS>(stream, weights_plan(s), a, b, both, s.features, ptr<T>(dw), beta_weights, back, partial);
 		}
 	}
 	void require_like(const mlTensor_t &t, const mlTensor_t &x, int last, const char *what)

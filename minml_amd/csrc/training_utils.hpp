@@ -226,6 +226,20 @@ namespace mlhip
 		const float high = static_cast<float>(static_cast<T>(x));
 		return fabsf(high) <= std::numeric_limits<float>::max() ? x - high : 0.0f;
 	}
+	constexpr int SCALE_BITS = 15; /* a gradient that is scaled has its largest element just below 2^15: fp16 ends at 2^16 */
+	/* the exponent of the power of two above the largest element */
+	__device__ __forceinline__ int scale_exponent(float top)
+	{
+		int exponent = 0;
+		if (top > 0.0f)
+			(void) frexpf(top, &exponent);
+		return max(exponent, -100); /* so that the way back is a normal number */
+	}
+	/* the larger of top and |v| where v is finite, else top (inf * 0 is no number, and a maximum passes over those): rows that are not finite have no say in the scale of the others */
+	__device__ __forceinline__ float larger_finite(float top, float v)
+	{
+		return fmaxf(top, fmaf(v, 0.0f, fabsf(v)));
+	}
 	inline size_t round_up(size_t n, size_t to)
 	{
 		return (n + to - 1) / to * to;

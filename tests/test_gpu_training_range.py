@@ -30,3 +30,72 @@ def test_an_infinite_gradient_of_the_gated_layer_stays_infinite(ctx, rows):
     others = np.arange(rows) != 1
     args = finite[0][others], finite[1], finite[2][others], finite[3][others], "relu"
     assert R.worst(got[others], R.gated_gradients(*args)[0], R.gated_gradient_bounds(*args, "float16")[0]) <= 1
+
+
+def gradient_bounds(x, w, p, dy, name):
+    """As R.gated_gradient_bounds, for fp16 with the power of two that d is kept with: half a step of its smallest numbers is 2^-25 where the largest element is between 2^-3 and 2^15, and else 2^-25 of what the largest is
+    2^14 of, at least."""
+    a, slope = R.gate(p[:, 0], name)
+    d = np.concatenate((dy * p[:, 1] * slope, dy * a), 1)
+    off = np.concatenate((np.abs(dy * p[:, 1]) * (1 + np.abs(p[:, 0])), np.abs(dy) * (1 + np.abs(p[:, 0]))), 1) * 2 * R.GATE_ERROR["float16"] + 2 * R.FP32 * np.abs(d)
+    top = np.abs(d).max()
+    stored = off + R.STEP["float16"] * np.abs(d) + (2.0 ** -25 if 2.0 ** -3 <= top < 2.0 ** 15 else 2.0 ** -39 * top)
+    dx, dw, db = R.gated_gradients(x, w, p, dy, name)
+    flat = w.reshape(-1, w.shape[2])
+    return (R.rounded(dx, "float16") + R.product_error(d, flat, "float16") + stored @ np.abs(flat),
+            R.rounded(dw, "float32") + (R.product_error(d.T, x, "float16") + stored.T @ np.abs(x)).reshape(w.shape),
+            R.rounded(db, "float32") + (off.sum(0) + (x.shape[0] + 80) * R.FP32 * np.abs(d).sum(0)).reshape(2, -1))
+
+
+def worst_of_fp16(got, want, bound):
+    """R.worst where results may pass the type's end: from 65520 on a value rounds to an infinity, and within the bound of that place both are right, the infinity and the last finite number."""
+    got = R.numbers(got)
+    near = np.abs(np.abs(want) - 65520) <= bound
+    rounded_up = np.where(near, np.isinf(got), np.abs(want) >= 65520)
+    return R.worst(got, np.where(rounded_up, np.copysign(np.inf, want), want), bound)
+
+
+# of dy, of the other projection and of the weights: d beyond 65504 with a dx that is not; d at both sides of the limits of scaling; d among the subnormal numbers
+SCALES = {"beyond": (2e4, 100.0, 1e-4), "at the upper limit": (2.0 ** 13, 2.0, 1.0), "usual": (1.0, 1.0, 0.1), "at the lower limit": (2.0 ** -5, 1.0, 0.1), "small": (2e-6, 1.0, 1.0), "smallest": (2.0 ** -23, 2.0 ** -12, 1.0)}
+
+
+@pytest.mark.parametrize("rows", [1, 8, 64, 90, 700])
+@pytest.mark.parametrize("scale", SCALES)
+def test_gradients_of_the_gated_layer_of_any_size(ctx, scale, rows):
+    """dx in fp16 and the sums in fp32, which have to keep their bits whatever size d has; what was in them is added."""
+    rng = np.random.default_rng(rows)
+    features, hidden = 72, 300
+    of_dy, of_u, of_w = SCALES[scale]
+    x, w = rng.standard_normal((rows, features)), of_w * rng.standard_normal((2, hidden, features))
+    p, dy = rng.standard_normal((rows, 2, hidden)), of_dy * np.clip(rng.standard_normal((rows, hidden)), -3, 3)
+    p[:, 1] *= of_u
+    x, w, p, dy = (R.bits(a, "float16") for a in (x, w, p, dy))
+    X, W, P, DY = (ml.toDevice(ctx, a) for a in (x, w, p, dy))
+    args = [R.numbers(a) for a in (x, w, p, dy)] + ["silu"]
+    wants, bounds = R.gated_gradients(*args), gradient_bounds(*args)
+    old = np.ascontiguousarray(wants[1] / 4, np.float32)
+    dx, dw, db = ml.Tensor((rows, features), "float16"), ml.toDevice(ctx, old), ml.Tensor((2, hidden), "float32")
+    ml.gatedDenseBackward(ctx, X, W, P, DY, 0.0, dx, 0.0, None, None, "silu", space(ctx, X, W, True))
+    assert worst_of_fp16(dx.copyToHost(ctx), wants[0], bounds[0]) <= 1
+    ml.gatedDenseBackward(ctx, X, W, P, DY, 0.0, None, -1.0, dw, None, "silu", space(ctx, X, W, True))
+    assert R.worst(dw.copyToHost(ctx), wants[1] - old.astype(np.float64), bounds[1] + 2 * R.rounded(old, "float32")) <= 1
+    ml.gatedDenseBackward(ctx, X, W, P, DY, 0.0, None, 0.0, None, db, "silu", space(ctx, X, W, True))
+    assert R.worst(db.copyToHost(ctx), wants[2], bounds[2]) <= 1
+
+
+def test_one_infinite_row_has_no_say_in_the_scale_of_the_others(ctx):
+    """Small gradients beside a row of infinities: dx of the other rows keeps the bits that it has without that row."""
+    rng = np.random.default_rng(5)
+    rows, features, hidden = 90, 64, 128
+    x, w, p, dy = (R.bits(a, "float16") for a in (rng.standard_normal((rows, features)), rng.standard_normal((2, hidden, features)), rng.standard_normal((rows, 2, hidden)), 2e-4 * rng.standard_normal((rows, hidden))))
+    dy[4] = 0
+    results = []
+    for bad in (False, True):
+        if bad:
+            dy[4, :9], dy[4, 9] = 0x7c00, 0x7e00
+        X, W, P, DY = (ml.toDevice(ctx, a) for a in (x, w, p, dy))
+        dx = ml.Tensor((rows, features), "float16")
+        ml.gatedDenseBackward(ctx, X, W, P, DY, 0.0, dx, 0.0, None, None, "gelu", space(ctx, X, W, True))
+        results.append(R.numbers(dx.copyToHost(ctx)))
+    others = np.arange(rows) != 4
+    assert np.array_equal(results[0][others], results[1][others]) and np.isnan(results[1][4]).all()
