@@ -21,14 +21,30 @@ namespace
 {
 	using namespace mlhip;
 
-	/* exp and 1 / x for gates whose results are rounded to fp16: the hardware's own, 2^-21 off at most for |x| < 8, where 2^-11 is rounded away; fp32 takes the library's */
-	template<typename T>
-	__device__ __forceinline__ float sigmoid_of(float g)
+	/*
+	 * sigmoid(g), and sigmoid(-g) = 1 - sigmoid(g), of one exponential that does not overflow and without the difference, in which the slope of the sigmoid's right half would lose its digits (all of them from g = 17 on).
+	 * exp and 1 / x for gates whose results are rounded to fp16 are the hardware's own, 2^-21 off at most for |x| < 8, where 2^-11 is rounded away; fp32 takes the library's.
+	 */
+	struct Sigmoid
 	{
+			float value, complement;
+	};
+	template<typename T>
+	__device__ __forceinline__ Sigmoid sigmoid_of(float g)
+	{
+		float e, larger;
 		if constexpr (sizeof(T) == 2)
-			return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+		{
+			e = __expf(-fabsf(g));
+			larger = __builtin_amdgcn_rcpf(1.0f + e);
+		}
 		else
-			return 1.0f / (1.0f + expf(-g));
+		{
+			e = expf(-fabsf(g));
+			larger = 1.0f / (1.0f + e);
+		}
+		const float smaller = e * larger;
+		return g >= 0.0f ? Sigmoid { larger, smaller } : Sigmoid { smaller, larger };
 	}
 	/*
 	 * The normal distribution's integral up to -|g|, 0.5 erfc(|g| / sqrt 2). For fp16 erfc(z) exp(z^2) / t is a polynomial of degree 5 in t = 1 / (1 + 0.43 z), fitted to the smallest relative error over
@@ -57,10 +73,13 @@ namespace
 		switch (gate)
 		{
 			case GATE_SIGMOID:
-				a = sigmoid_of<T>(g);
+			{
+				const Sigmoid s = sigmoid_of<T>(g);
+				a = s.value;
 				if (SLOPE)
-					slope = a * (1.0f - a);
+					slope = s.value * s.complement;
 				break;
+			}
 			case GATE_RELU:
 				a = (g > 0.0f || g != g) ? g : 0.0f; /* NaN stays */
 				if (SLOPE)
@@ -68,10 +87,10 @@ namespace
 				break;
 			case GATE_SILU:
 			{
-				const float s = sigmoid_of<T>(g);
-				a = g * s;
+				const Sigmoid s = sigmoid_of<T>(g);
+				a = g * s.value;
 				if (SLOPE)
-					slope = s * fmaf(g, 1.0f - s, 1.0f);
+					slope = s.value * fmaf(g, s.complement, 1.0f);
 				break;
 			}
 			default: /* GATE_GELU */

@@ -99,3 +99,19 @@ def test_one_infinite_row_has_no_say_in_the_scale_of_the_others(ctx):
         results.append(R.numbers(dx.copyToHost(ctx)))
     others = np.arange(rows) != 4
     assert np.array_equal(results[0][others], results[1][others]) and np.isnan(results[1][4]).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_slope_of_the_sigmoid_keeps_its_digits_on_both_sides(ctx, dtype):
+    """db of one row with dy = u = 1 is the slope itself, e^-|g| / (1 + e^-|g|)^2, in fp32. Steps of 2^-24: the exponential 2 and, in fp16, the rounding of its argument, |g| and its scaling's |g|; 1 + e and its inverse 5, twice,
+    and two products."""
+    g = R.numbers(R.bits(np.concatenate([np.linspace(-20, 20, 401), [-60.0, 60.0]]), dtype))
+    p = np.stack((g, np.ones_like(g)))[None]
+    x, w = R.bits(np.ones((1, 8)), dtype), R.bits(np.ones((2, g.size, 8)), dtype)
+    X, W, P, DY = (ml.toDevice(ctx, a) for a in (x, w, R.bits(p, dtype), R.bits(np.ones((1, g.size)), dtype)))
+    db = ml.Tensor((2, g.size), "float32")
+    ml.gatedDenseBackward(ctx, X, W, P, DY, 0.0, None, 0.0, None, db, "sigmoid", space(ctx, X, W, True))
+    e = np.exp(-np.abs(g))
+    want = e / (1 + e) ** 2
+    steps = 14 + (2 * np.abs(g) if dtype == "float16" else 0)
+    assert R.worst(db.copyToHost(ctx)[0], want, steps * R.FP32 * want) <= 1
