@@ -11,7 +11,8 @@
  * 1024 threads a longer one; beyond 16384 elements the row is read again for every step.
  * The sums over the rows stay in the registers of the thread that owns the columns, while its workgroup walks over the rows; every workgroup leaves one row of them in
  * the caller's workspace, and a second launch adds these rows up in a fixed order.
- * Forward 57600 x 256 fp16 11.9 us (5.0 TB/s, launch included); backward 16384 x 4096 fp16 79 us (5.1 TB/s, a large copy moves 5.2), 7001 x 1001 fp32, whose rows begin anywhere, 21.5 us (3.9 TB/s).
+ * Forward 57600 x 256 fp16 11.9 us (5.0 TB/s, launch included); backward 16384 x 4096 fp16 79 us (5.1 TB/s, a large copy moves 5.2), 7001 x 1001 fp32, whose rows begin anywhere, 21 us (4.0 TB/s);
+ * beyond 8192 elements a workgroup fills a compute unit and has one row in hand at a time: 4096 x 16384 fp16 115 us (3.5 TB/s), fp32 175 us (4.6 TB/s).
  */
 #include "training_utils.hpp"
 
@@ -60,6 +61,17 @@ namespace
 				}
 			}
 	};
+	/* nothing that the compiler made of the value before stays in registers: it is made again where it is used. Scalar: the same for all lanes */
+	template<typename V>
+	__device__ __forceinline__ void take_as_new(V &value)
+	{
+		asm volatile("" : "+v"(value));
+	}
+	template<typename V>
+	__device__ __forceinline__ void take_as_new_scalar(V &value)
+	{
+		asm volatile("" : "+s"(value));
+	}
 	template<int LANES>
 	constexpr int threads_of()
 	{
@@ -84,9 +96,9 @@ namespace
 		{
 			place[i] = place_in_row<VEC>((lane + LANES * i) * VEC, columns);
 			if (w != nullptr)
-				gamma[i].load(w + place[i].start);
+				gamma[i].load(place[i].in(w));
 			if (b != nullptr)
-				shift[i].load(b + place[i].start);
+				shift[i].load(place[i].in(b));
 		}
 		for (size_t first = static_cast<size_t>(blockIdx.x) * ROWS; first < rows; first += static_cast<size_t>(gridDim.x) * ROWS)
 		{
@@ -96,7 +108,7 @@ namespace
 			Elements<T, VEC> raw[ITEMS];
 #pragma unroll
 			for (int i = 0; i < ITEMS; i++)
-				raw[i].load(src + place[i].start);
+				raw[i].load(place[i].in(src));
 			float sum[1] = { 0.0f };
 #pragma unroll
 			for (int i = 0; i < ITEMS; i++)
@@ -130,7 +142,7 @@ namespace
 							const float n = (raw[i][e] - mean) * r;
 							out[e] = fmaf(n, w != nullptr ? gamma[i][e] : 1.0f, b != nullptr ? shift[i][e] : 0.0f);
 						}
-						store_nearest<VEC>(dst + place[i].start, out, place[i].skip);
+						store_nearest<VEC>(place[i].in(dst), out, place[i].skip);
 					}
 			}
 		}
@@ -144,6 +156,12 @@ namespace
 			const T *w, float *partial)
 	{
 		constexpr int THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
+		/*
+		 * The next row is on its way while this one is summed, where the registers hold both. 1024 threads have 128 registers each: one row at 16 elements a thread, the weights and both sums fit if nothing else is kept
+		 * across the row's steps, which the compiler has to be told (it would keep differences and products of the row, addresses of every lane and the tests of `skip`, and spill). us, two rows that spill / so: 4096 x 16384
+		 * fp16 164 / 115, fp32 423 / 175 (4.6 TB/s), 4096 x 8200 122 / 86, 352 / 105.
+		 */
+		constexpr bool AHEAD = LANES < 1024 || VEC * ITEMS < 16;
 		/* the workgroup's row groups meet here at the end: all but the first leave their sums, [ROWS - 1][2][LANES * VEC * ITEMS] in pieces of one item */
 		__shared__ float scratch[LANES > 64 ? 6 * (LANES / 64) : 2 * THREADS * VEC];
 		RowSum<LANES> row_sum { scratch, 0 };
@@ -157,7 +175,7 @@ namespace
 		{
 			place[i] = place_in_row<VEC>((lane + LANES * i) * VEC, columns);
 			if (w != nullptr)
-				gamma[i].load(w + place[i].start);
+				gamma[i].load(place[i].in(w));
 #pragma unroll
 			for (int e = 0; e < VEC; e++)
 				sum_w[i][e] = sum_b[i][e] = 0.0f;
@@ -167,18 +185,22 @@ namespace
 		Elements<T, VEC> next_x[ITEMS], next_dy[ITEMS];
 		const auto request = [&](size_t group) __attribute__((always_inline))
 		{
-			const size_t offset = min(group + threadIdx.x / LANES, rows - 1) * columns;
+			size_t offset = min(group + threadIdx.x / LANES, rows - 1) * columns;
+			if constexpr (!AHEAD)
+				take_as_new_scalar(offset);
 #pragma unroll
 			for (int i = 0; i < ITEMS; i++)
 			{
-				next_x[i].load(x + offset + place[i].start);
-				next_dy[i].load(dy + offset + place[i].start);
+				next_x[i].load(place[i].in(x + offset));
+				next_dy[i].load(place[i].in(dy + offset));
 			}
 		};
-		if (first < rows)
+		if (AHEAD && first < rows)
 			request(first);
 		for (; first < rows; first += step)
 		{
+			if (!AHEAD)
+				request(first);
 			const size_t wanted = first + threadIdx.x / LANES;
 			const bool there = wanted < rows;
 			Elements<T, VEC> raw_x[ITEMS], raw_dy[ITEMS];
@@ -187,9 +209,11 @@ namespace
 			{
 				raw_x[i] = next_x[i];
 				raw_dy[i] = next_dy[i];
+				if constexpr (!AHEAD)
+					take_as_new(place[i].skip);
 			}
-			if (first + step < rows)
-				request(first + step); /* the next row arrives while this one is summed */
+			if (AHEAD && first + step < rows)
+				request(first + step);
 			float sum[1] = { 0.0f };
 #pragma unroll
 			for (int i = 0; i < ITEMS; i++)
@@ -201,26 +225,36 @@ namespace
 			float sums[3] = { 0.0f, 0.0f, 0.0f }; /* of (x - m)^2, g, g (x - m) */
 #pragma unroll
 			for (int i = 0; i < ITEMS; i++)
+			{
 #pragma unroll
 				for (int e = 0; e < VEC; e++)
-					if (e >= place[i].skip)
-					{
-						const float d = raw_x[i][e] - mean;
-						const float g = w != nullptr ? raw_dy[i][e] * gamma[i][e] : raw_dy[i][e];
-						sums[0] = fmaf(d, d, sums[0]);
-						sums[1] += g;
-						sums[2] = fmaf(g, d, sums[2]);
-					}
+				{
+					const bool counts = e >= place[i].skip;
+					const float d = counts ? raw_x[i][e] - mean : 0.0f;
+					const float g = counts ? (w != nullptr ? raw_dy[i][e] * gamma[i][e] : raw_dy[i][e]) : 0.0f;
+					sums[0] = fmaf(d, d, sums[0]);
+					sums[1] += g;
+					sums[2] = fmaf(g, d, sums[2]);
+				}
+			}
 			row_sum(sums);
 			const float r = 1.0f / sqrtf(sums[0] * inv_columns + epsilon);
 			const float mean_g = sums[1] * inv_columns, mean_gn = sums[2] * r * inv_columns;
 			if (there)
 			{
-				T *dst = dx + wanted * columns;
+				size_t offset = wanted * columns;
+				if constexpr (!AHEAD)
+					take_as_new_scalar(offset);
+				T *dst = dx + offset;
 #pragma unroll
 				for (int i = 0; i < ITEMS; i++)
 				{
 					float out[VEC];
+					if constexpr (!AHEAD)
+					{
+						take_as_new(raw_x[i].raw);
+						take_as_new(raw_dy[i].raw);
+					}
 #pragma unroll
 					for (int e = 0; e < VEC; e++)
 					{
@@ -235,12 +269,12 @@ namespace
 						if (beta != 0.0f)
 						{
 							Elements<T, VEC> old;
-							old.load(dst + place[i].start);
+							old.load(place[i].in(dst));
 #pragma unroll
 							for (int e = 0; e < VEC; e++)
 								out[e] = fmaf(beta, old[e], out[e]);
 						}
-						store_nearest<VEC>(dst + place[i].start, out, place[i].skip);
+						store_nearest<VEC>(place[i].in(dst), out, place[i].skip);
 					}
 				}
 			}
@@ -273,8 +307,8 @@ namespace
 			}
 			if (threadIdx.x < LANES && place[i].skip < VEC)
 			{
-				store_nearest<VEC>(mine + place[i].start, sum_w[i], place[i].skip);
-				store_nearest<VEC>(mine + columns + place[i].start, sum_b[i], place[i].skip);
+				store_nearest<VEC>(place[i].in(mine), sum_w[i], place[i].skip);
+				store_nearest<VEC>(place[i].in(mine + columns), sum_b[i], place[i].skip);
 			}
 		}
 	}

@@ -133,6 +133,14 @@ namespace mlhip
 	struct RowPlace
 	{
 			int start, skip;
+
+			/* a scalar base and 32 bits of offset where the row is the same for the whole wavefront (rows that go by RowPlace are below 2^31 bytes) */
+			template<typename T>
+			__device__ __forceinline__ T* in(T *row) const
+			{
+				typedef typename std::conditional<std::is_const<T>::value, const char, char>::type byte;
+				return reinterpret_cast<T*>(reinterpret_cast<byte*>(row) + static_cast<uint32_t>(start) * static_cast<uint32_t>(sizeof(T)));
+			}
 	};
 	template<int VEC>
 	__device__ __forceinline__ RowPlace place_in_row(int j, int columns)

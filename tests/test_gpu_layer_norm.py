@@ -176,3 +176,18 @@ def test_recorded_pass_and_two_contexts(ctx):
             for _, out in sets:
                 assert all(np.array_equal(t.copyToHost(ctx), e) for t, e in zip(out, eager))
     other.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("columns", [8200, 9001, 16384])
+def test_several_long_rows_of_a_workgroup(ctx, columns, dtype):
+    """More rows than workgroups, of lengths that 1024 threads hold in their registers; dx over dy."""
+    rng = np.random.default_rng(columns)
+    x, w, b, dy = tensors(ctx, rng, 1030, columns, dtype)
+    X, W, DY = (ml.toDevice(ctx, a) for a in (x, w, dy))
+    dw, db = ml.Tensor((columns,), "float32"), ml.Tensor((columns,), "float32")
+    ml.layerNormBackward(ctx, X, W, DY, 0.0, DY, 0.0, dw, db, workspace(ctx, X), EPSILON)
+    xf, wf, dyf = map(R.numbers, (x, w, dy))
+    want, bounds, sums = R.layer_norm_gradients(xf, wf, dyf, EPSILON), R.layer_norm_gradient_bounds(xf, wf, dyf, EPSILON, dtype), R.layer_norm_gradient_bounds(xf, wf, dyf, EPSILON, "float32")
+    assert R.worst(DY.copyToHost(ctx), want[0], bounds[0]) <= 1
+    assert R.worst(dw.copyToHost(ctx), want[1], sums[1]) <= 1 and R.worst(db.copyToHost(ctx), want[2], sums[2]) <= 1
