@@ -227,41 +227,43 @@ namespace
 					partials[static_cast<size_t>(row) * gridDim.x + blockIdx.x] = p;
 			}
 	}
-	/* THREADS threads to a row: a wavefront where there are rows enough, else a workgroup, each thread with 8 pairs on their way at a time */
+	/* THREADS threads to a row: a wavefront where there are rows enough, else a workgroup, each thread with 8 pairs on their way at a time. Workgroups of wavefronts take further rows: 2^26 and more would be too many threads for a launch */
 	template<int THREADS>
 	__global__ __launch_bounds__(256) void kernel_join_partials(const Partial *partials, int count, const int *targets, const float *target_logits, int rows, int classes, float *loss, float *lse)
 	{
 		__shared__ Partial waves[4];
-		const int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
-		if (row >= rows)
-			return; /* whole wavefronts; a workgroup that shares a row has one */
-		Partial p { -std::numeric_limits<float>::infinity(), 0.0f };
-		const Partial *src = partials + static_cast<size_t>(row) * count;
-		for (int first = threadIdx.x % THREADS; first < count; first += 8 * THREADS)
+		for (int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS; row < rows; row += gridDim.x * (256 / THREADS))
 		{
-			Partial next[8];
+			Partial p { -std::numeric_limits<float>::infinity(), 0.0f };
+			const Partial *src = partials + static_cast<size_t>(row) * count;
+			for (int first = threadIdx.x % THREADS; first < count; first += 8 * THREADS)
+			{
+				Partial next[8];
 #pragma unroll
-			for (int u = 0; u < 8; u++)
-				next[u] = src[min(first + u * THREADS, count - 1)];
+				for (int u = 0; u < 8; u++)
+					next[u] = src[min(first + u * THREADS, count - 1)];
 #pragma unroll
-			for (int u = 0; u < 8; u++)
-				if (first + u * THREADS < count)
-					p = join(p, next[u]);
-		}
-		p = lanes_join<64>(p);
-		if constexpr (THREADS > 64)
-		{
-			if ((threadIdx.x & 63) == 0)
-				waves[threadIdx.x >> 6] = p;
-			__syncthreads();
-			p = join(join(waves[0], waves[1]), join(waves[2], waves[3]));
-		}
-		if (threadIdx.x % THREADS == 0)
-		{
-			const float value = p.top + logf(p.sum);
-			const int target = targets[row];
-			lse[row] = value;
-			loss[row] = (target >= 0 && target < classes) ? value - target_logits[row] : 0.0f;
+				for (int u = 0; u < 8; u++)
+					if (first + u * THREADS < count)
+						p = join(p, next[u]);
+			}
+			p = lanes_join<64>(p);
+			if constexpr (THREADS > 64)
+			{
+				if ((threadIdx.x & 63) == 0)
+					waves[threadIdx.x >> 6] = p;
+				__syncthreads();
+				p = join(join(waves[0], waves[1]), join(waves[2], waves[3]));
+			}
+			if (threadIdx.x % THREADS == 0)
+			{
+				const float value = p.top + logf(p.sum);
+				const int target = targets[row];
+				lse[row] = value;
+				loss[row] = (target >= 0 && target < classes) ? value - target_logits[row] : 0.0f;
+			}
+			if (THREADS > 64)
+				return; /* one row, `waves` is in use */
 		}
 	}
 
@@ -572,7 +574,7 @@ namespace
 		if (s.rows <= 1024)
 			hipLaunchKernelGGL((kernel_join_partials<256>), dim3(s.rows), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
 		else
-			hipLaunchKernelGGL((kernel_join_partials<64>), dim3(ceil_div(s.rows, 4)), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
+			hipLaunchKernelGGL((kernel_join_partials<64>), dim3(std::min(ceil_div(s.rows, 4), 1 << 20)), dim3(256), 0, stream, partials, columns, targets, target_logits, s.rows, s.classes, loss, lse);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	template<typename T>

@@ -200,7 +200,7 @@ namespace mlhip
 	{
 			Operand a, b;
 			int rows; /* of the result */
-			int tiles_m, tiles_n;
+			int first_tile_m, tiles_m, tiles_n; /* rows of tiles of this launch, columns */
 			int chunks; /* of the whole product */
 			int chunks_per_part; /* of one gridDim.y */
 	};
@@ -216,7 +216,7 @@ namespace mlhip
 		const unsigned int group = id / group_tiles, within = id - group * group_tiles;
 		const unsigned int rows = min(static_cast<unsigned int>(p.tiles_m) - group * TILE_GROUP, static_cast<unsigned int>(TILE_GROUP));
 		tile_n = within / rows;
-		tile_m = group * TILE_GROUP + within - tile_n * rows;
+		tile_m = p.first_tile_m + group * TILE_GROUP + within - tile_n * rows;
 	}
 
 	/*
@@ -713,51 +713,65 @@ namespace mlhip
 		}
 		return best;
 	}
+	/* a launch has less than 2^32 threads along x: 2^23 tiles of 256x256 (2^21 tokens against 2^18 classes) are one more than that, and go out in two. Whole groups of rows of tiles where there is room for one */
+	inline int tile_rows_of_a_launch(const ProductPlan &plan)
+	{
+		const int threads = plan.tile == 256 ? 512 : 256;
+		const long long rows = 0xffffffffll / threads / plan.tiles_n;
+		MLHIP_REQUIRE(rows > 0, "product too large");
+		if (rows >= plan.tiles_m)
+			return plan.tiles_m;
+		return static_cast<int>(rows > TILE_GROUP ? rows / TILE_GROUP * TILE_GROUP : rows);
+	}
 	template<typename T, Side SA, Side SB, bool PAIRED, typename Epilogue>
 	inline void launch_product(hipStream_t stream, const ProductPlan &plan, const Operand &a, const Operand &b, int rows, const Epilogue &epilogue)
 	{
 		if (plan.tiles_m == 0 || plan.tiles_n == 0)
 			return;
-		const ProductArgs args { a, b, rows, plan.tiles_m, plan.tiles_n, plan.chunks, plan.chunks_per_part };
-		const long long tiles = static_cast<long long>(plan.tiles_m) * plan.tiles_n;
-		MLHIP_REQUIRE(tiles <= 0x7fffffff && plan.parts <= 65535 && a.row_bytes < (1u << 22) && b.row_bytes < (1u << 22), "product too large");
-		const dim3 grid(static_cast<unsigned int>(tiles), plan.parts);
+		MLHIP_REQUIRE(plan.parts <= 65535 && a.row_bytes < (1u << 22) && b.row_bytes < (1u << 22), "product too large");
 		static_assert(product_lds<Epilogue>(256, 2) <= LDS_OF_A_UNIT && product_lds<Epilogue>(128, 2) <= LDS_OF_A_UNIT / 2 && product_lds<Epilogue>(128, 1) <= LDS_OF_A_UNIT / 4,
 				"tiles must fit the LDS of a compute unit");
-		if (plan.tile == 256)
+		const int most = tile_rows_of_a_launch(plan);
+		for (int first = 0; first < plan.tiles_m; first += most)
 		{
-			constexpr int bytes = product_lds<Epilogue>(256, 2);
-			auto kernel = kernel_product_256<T, SA, SB, PAIRED, Epilogue>;
-			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
-			hipLaunchKernelGGL(kernel, grid, dim3(512), bytes, stream, args, epilogue);
-		}
-		else if (plan.tile == 64)
-		{
-			if constexpr (sizeof(T) == 4 && SA == Side::ROWS)
+			const int tiles_m = std::min(most, plan.tiles_m - first);
+			const ProductArgs args { a, b, rows, first, tiles_m, plan.tiles_n, plan.chunks, plan.chunks_per_part };
+			const dim3 grid(static_cast<unsigned int>(tiles_m) * plan.tiles_n, plan.parts);
+			if (plan.tile == 256)
 			{
-				constexpr int bytes = product_lds<Epilogue>(64, 2);
-				auto kernel = kernel_product_128<T, SA, SB, PAIRED, 64, 2, Epilogue>;
+				constexpr int bytes = product_lds<Epilogue>(256, 2);
+				auto kernel = kernel_product_256<T, SA, SB, PAIRED, Epilogue>;
+				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+				hipLaunchKernelGGL(kernel, grid, dim3(512), bytes, stream, args, epilogue);
+			}
+			else if (plan.tile == 64)
+			{
+				if constexpr (sizeof(T) == 4 && SA == Side::ROWS)
+				{
+					constexpr int bytes = product_lds<Epilogue>(64, 2);
+					auto kernel = kernel_product_128<T, SA, SB, PAIRED, 64, 2, Epilogue>;
+					ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+					hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
+				}
+				else
+					fail_logic("HIP backend: tiles of 64 rows are for fp32 rows");
+			}
+			else if (plan.slots == 2)
+			{
+				constexpr int bytes = product_lds<Epilogue>(128, 2);
+				auto kernel = kernel_product_128<T, SA, SB, PAIRED, 128, 2, Epilogue>;
 				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
 				hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
 			}
 			else
-				fail_logic("HIP backend: tiles of 64 rows are for fp32 rows");
+			{
+				constexpr int bytes = product_lds<Epilogue>(128, 1);
+				auto kernel = kernel_product_128<T, SA, SB, PAIRED, 128, 1, Epilogue>;
+				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+				hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
+			}
+			MLHIP_CHECK(hipGetLastError());
 		}
-		else if (plan.slots == 2)
-		{
-			constexpr int bytes = product_lds<Epilogue>(128, 2);
-			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 128, 2, Epilogue>;
-			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
-			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
-		}
-		else
-		{
-			constexpr int bytes = product_lds<Epilogue>(128, 1);
-			auto kernel = kernel_product_128<T, SA, SB, PAIRED, 128, 1, Epilogue>;
-			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
-			hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, stream, args, epilogue);
-		}
-		MLHIP_CHECK(hipGetLastError());
 	}
 
 	/* out[m][n] = scale * sum + beta * out[m][n] */

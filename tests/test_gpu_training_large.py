@@ -73,3 +73,37 @@ def test_cross_entropy(ctx):
     assert R.worst(loss.copyToHost(ctx)[picked], R.cross_entropy(*args)[0], R.cross_entropy_bounds(*args, "float16")[0]) <= 1
     args += (dloss[picked].astype(np.float64),)
     assert R.worst(at_rows(ctx, dx, picked), R.cross_entropy_gradients(*args)[0], R.cross_entropy_gradient_bounds(*args, "float16")[0]) <= 1
+
+
+def test_loss_of_more_tiles_than_a_launch_has_threads_for(ctx):
+    """2^21 + 3 rows and 2^18 classes are more than 2^23 tiles of 256 x 256; the two numbers that each leaves for a row are 17 GB."""
+    rng = np.random.default_rng(4)
+    rows, features, classes = 2 ** 21 + 3, 8, 2 ** 18
+    picked = [0, 255, 256, 1234567, 2 ** 21 - 2048, 2 ** 21 - 2049, 2 ** 21 - 1, 2 ** 21, rows - 1]
+    x, w = (R.bits(a, "float16") for a in (rng.standard_normal((rows, features)), rng.standard_normal((classes, features)) / 2))
+    targets = rng.integers(0, classes, rows).astype(np.int32)
+    X, W, T = (ml.toDevice(ctx, a) for a in (x, w, targets))
+    loss, lse = ml.Tensor((rows,), "float32"), ml.Tensor((rows,), "float32")
+    space = ml.Tensor((ml.linearCrossEntropyGetWorkspaceSize(ctx, X, W, False),), "uint8")
+    ml.linearCrossEntropyForward(ctx, X, W, None, T, loss, lse, space)
+    args = R.numbers(x)[picked], R.numbers(w), np.zeros(classes), targets[picked]
+    want, bounds = R.cross_entropy(*args), R.cross_entropy_bounds(*args, "float16")
+    losses = loss.copyToHost(ctx)
+    assert R.worst(losses[picked], want[0], bounds[0]) <= 1 and R.worst(lse.copyToHost(ctx)[picked], want[1], bounds[1]) <= 1
+    assert np.isfinite(losses).all() and (losses > 0).all()
+
+
+def test_loss_of_more_rows_than_a_launch_has_wavefronts_for(ctx):
+    """2^26 + 5 rows of zeros, three classes: the loss is that of the bias alone."""
+    rows = 2 ** 26 + 5
+    x, w = ml.Tensor((rows, 8), "float16"), ml.toDevice(ctx, R.bits(np.ones((3, 8)), "float16"))
+    bias = np.array([0.0, 1.0, -2.0])
+    targets, loss, lse = ml.Tensor((rows,), "int32"), ml.Tensor((rows,), "float32"), ml.Tensor((rows,), "float32")
+    x.zeroall(ctx)
+    targets.zeroall(ctx)
+    loss.setall(ctx, -1.0)
+    space = ml.Tensor((ml.linearCrossEntropyGetWorkspaceSize(ctx, x, w, False),), "uint8")
+    ml.linearCrossEntropyForward(ctx, x, w, ml.toDevice(ctx, R.bits(bias, "float16")), targets, loss, lse, space)
+    want = np.log(np.exp(bias).sum())
+    # three exponentials, two additions, a logarithm and a difference: below 20 roundings of numbers up to 2
+    assert np.abs(loss.copyToHost(ctx).astype(np.float64) - want).max() <= 40 * R.FP32
