@@ -10,9 +10,9 @@
  * Backward: the classes are taken in pieces of as many as make d 256 MB (so it stays in the last-level cache between its makers and users, and the workspace small whatever the vocabulary). For each
  * piece the logits are made again, which costs a quarter of the operations and spares rows x classes of memory; the epilogue turns them into d; then d is multiplied with the piece's weights, added to
  * dx in fp32, and with x, which gives the piece's rows of dW.
- * d is stored in the tensors' type. In fp16 a probability of one class in 100 000 would be subnormal, and the rows' dloss may be anything, so d is scaled by 2^15 / s with s the power of two above the
- * largest |dloss|: the largest d is 2^15 then, and probabilities down to 2e-9 keep their 11 bits. The products' results are scaled back, exactly, in fp32. Its rounding, half a step per element, averages
- * out in the sums; db is summed before it.
+ * d is stored in the tensors' type. In fp16 a probability of one class in 100 000 would be subnormal, so d is scaled by 2^15 / s with s the power of two above the largest |dloss|: of that loss's row probabilities down to
+ * 2^-28 keep their 11 bits, of a row whose dloss is 2^-k of it down to 2^(k - 28); what is smaller is off by 2^-39 of the largest |dloss| at most. The products' results are scaled back, exactly, in fp32. What the rounding of
+ * d, half a step per element, does to dx is given back (GradientEpilogue); in dW it counts as much as the rounding of dW itself; db is summed before it.
  * fp16: 7 rows of 2048 x 65536 classes 50 us (5.3 TB/s); 4096 rows of 1024 x 50001 433 us (0.97 PFLOP/s), of 2048 x 65536 940 us (1.17); the gradients of the latter 2.93 ms, in two pieces of d 553 us each (0.99 PFLOP/s, a
  * fourth of it the epilogue), dx 461 (1.19), dW 457 (1.20).
  */
@@ -327,15 +327,31 @@ namespace
 		if (threadIdx.x == 0)
 			*back = ldexpf(1.0f, exponent - SCALE_BITS);
 	}
-	/* WITH_LOW: what rounding leaves of d is written too */
-	template<typename T, bool WITH_LOW>
+	/* the sum of four elements less that of what is stored of them, in fp32 (its own roundings are 2^-24 of d). Dot products with ones take the halves as they lie in pairs, subnormal ones too: differences element by element
+	 * take twice the instructions and registers that a 256 x 256 tile does not have (d of 4096 x 32768, k = 2048: 2 % longer than without any of this, 581 against 570 us; element by element 5 %) */
+	template<typename V>
+	__device__ __forceinline__ float what_rounding_takes(const float *v, const V &stored)
+	{
+		const half2_t ones { static_cast<half_t>(1.0f), static_cast<half_t>(1.0f) };
+		const float kept = __builtin_amdgcn_fdot2(half2_t { stored[0], stored[1] }, ones, __builtin_amdgcn_fdot2(half2_t { stored[2], stored[3] }, ones, 0.0f, false), false);
+		return ((v[0] + v[1]) + (v[2] + v[3])) - kept;
+	}
+	/*
+	 * d, the sums of its columns for db, and what rounding to fp16 took from its rows. The elements of a row add up to zero by definition, so that what the rows of W have in common has no part in dx; their roundings
+	 * do not, and with W's common part ten times the rest dx would be 1.9e-3 off (2.8e-4 without one). What was taken from a row is therefore added up here, in fp32, and given back to the target's class when dx is made,
+	 * dx += lost W[target]: the row adds up to zero again, and the target's element, the largest of d by far until a model is sure of something else, counts unrounded. dx is 2.1e-4 off then, as much as its own rounding
+	 * costs, and 2.6e-4 where other classes have large probabilities; dW, where nothing cancels, 2.8e-4.
+	 */
+	template<typename T>
 	struct GradientEpilogue
 	{
 			const T *bias; /* of the piece */
 			const int *targets;
 			const float *lse, *factors;
-			T *d, *low; /* [rows][row_elements], zeros behind the piece's classes */
+			T *d; /* [rows][row_elements], zeros behind the piece's classes */
 			float *sums; /* [row tiles][classes of the piece], or null */
+			float *lost; /* [rows][lost_tiles], at this piece's first column tile; fp16, or null */
+			int lost_tiles;
 			int first_class, classes, row_elements; /* classes: of the piece */
 
 			template<int BM, int BN>
@@ -347,12 +363,13 @@ namespace
 			template<int BM, int BN, typename Acc>
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
-				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : rows_at_a_time(BM), PASSES = BM / ROWS;
+				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : rows_at_a_time(BM), PASSES = BM / ROWS, WAVES_N = BN / 64;
+				static_assert((2 * BN + WAVES_N * BM) * static_cast<int>(sizeof(float)) <= GradientEpilogue::template lds<BM, BN>(), "the sums meet where the rows were");
 				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
 				const bool edge = (at.tile_n + 1) * BN > classes;
 				const Stage<T, BN> stage { reinterpret_cast<T*>(lds) };
-				float total[2][16];
+				float total[2][16], taken[BLOCKS];
 #pragma unroll
 				for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -367,13 +384,11 @@ namespace
 					norm[i] = lse[m];
 					factor[i] = at.tile_m * BM + at.row(i) < rows ? factors[m] : 0.0f;
 					target[i] = factor[i] != 0.0f ? targets[m] - first_class : -1; /* a class then */
+					taken[i] = 0.0f;
 				}
 				static_for<PASSES>([&](auto pass)
 				{
 					constexpr int PASS = decltype(pass)::value, FIRST = PASS * BLOCKS / PASSES;
-					static_for<WITH_LOW ? 2 : 1>([&](auto half) __attribute__((always_inline))
-					{
-					constexpr int part = decltype(half)::value;
 					__syncthreads();
 #pragma unroll
 					for (int i = FIRST; i < FIRST + BLOCKS / PASSES; i++)
@@ -396,56 +411,136 @@ namespace
 							{
 								v[j][r] -= factor[i];
 							});
-						if constexpr (part == 1)
-#pragma unroll
-							for (int j = 0; j < 2; j++)
-#pragma unroll
-								for (int r = 0; r < 16; r++)
-									v[j][r] = low_part<T>(v[j][r]);
 #pragma unroll
 						for (int j = 0; j < 2; j++)
 #pragma unroll
 							for (int q = 0; q < 4; q++)
 							{
-								stage.put(at.row(i) - PASS * ROWS, at.column(j) + at.lane_column(q), v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
+								typename Stage<T, BN>::vec4_t stored;
 #pragma unroll
 								for (int e = 0; e < 4; e++)
-									total[j][4 * q + e] += part == 0 ? v[j][4 * q + e] : 0.0f;
+									stored[e] = static_cast<T>(v[j][4 * q + e]);
+								stage.put(at.row(i) - PASS * ROWS, at.column(j) + at.lane_column(q), stored);
+#pragma unroll
+								for (int e = 0; e < 4; e++)
+									total[j][4 * q + e] += v[j][4 * q + e];
+								if constexpr (sizeof(T) == 2)
+									taken[i] += what_rounding_takes(&v[j][4 * q], stored);
 							}
 					}
 					__syncthreads();
-					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(part == 0 ? d : low, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
-					});
+					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
 				});
-				if (sums == nullptr)
+				const bool of_columns = sums != nullptr, of_rows = sizeof(T) == 2 && lost != nullptr;
+				if (!of_columns && !of_rows)
 					return;
-				/* lane bits 4 .. 1 choose among the 16 registers, a half of them at a time; bit 0 adds up what is left */
-				float *meeting = reinterpret_cast<float*>(lds); /* [2 wavefront rows][BN] */
+				float *meeting = reinterpret_cast<float*>(lds); /* of columns: [2 wavefront rows][BN], of rows: [WAVES_N][BM] */
 				__syncthreads();
+				if (of_columns)
 #pragma unroll
-				for (int j = 0; j < 2; j++)
-				{
+					for (int j = 0; j < 2; j++)
+					{
+						/* lane bits 4 .. 1 choose among the 16 registers, a half of them at a time; bit 0 adds up what is left */
 #pragma unroll
-					for (int bit = 16; bit >= 2; bit >>= 1)
+						for (int bit = 16; bit >= 2; bit >>= 1)
 #pragma unroll
-						for (int r = 0; r < bit / 2; r++)
-						{
-							const bool upper = (threadIdx.x & bit) != 0;
-							const float sent = upper ? total[j][r] : total[j][r + bit / 2];
-							const float kept = upper ? total[j][r + bit / 2] : total[j][r];
-							total[j][r] = kept + __shfl_xor(sent, bit);
-						}
-					const float sum = total[j][0] + __shfl_xor(total[j][0], 1);
-					const int r = (threadIdx.x & 31) >> 1;
-					if ((threadIdx.x & 1) == 0)
-						meeting[at.wave_m * BN + at.column(j) + TilePlace<BM, BN>::lane_column(r / 4) + r % 4] = sum;
-				}
+							for (int r = 0; r < bit / 2; r++)
+							{
+								const bool upper = (threadIdx.x & bit) != 0;
+								const float sent = upper ? total[j][r] : total[j][r + bit / 2];
+								const float kept = upper ? total[j][r + bit / 2] : total[j][r];
+								total[j][r] = kept + __shfl_xor(sent, bit);
+							}
+						const float sum = total[j][0] + __shfl_xor(total[j][0], 1);
+						const int r = (threadIdx.x & 31) >> 1;
+						if ((threadIdx.x & 1) == 0)
+							meeting[at.wave_m * BN + at.column(j) + TilePlace<BM, BN>::lane_column(r / 4) + r % 4] = sum;
+					}
+				if (of_rows)
+#pragma unroll
+					for (int i = 0; i < BLOCKS; i++)
+					{
+						const float sum = taken[i] + __shfl_xor(taken[i], 32);
+						if ((threadIdx.x & 32) == 0)
+							meeting[2 * BN + at.wave_n * BM + at.row(i)] = sum;
+					}
 				__syncthreads();
-				const int n = at.tile_n * BN + static_cast<int>(threadIdx.x);
-				if (static_cast<int>(threadIdx.x) < BN && n < classes)
+				const int n = at.tile_n * BN + static_cast<int>(threadIdx.x), m = at.tile_m * BM + static_cast<int>(threadIdx.x);
+				if (of_columns && static_cast<int>(threadIdx.x) < BN && n < classes)
 					sums[static_cast<size_t>(at.tile_m) * classes + n] = meeting[threadIdx.x] + meeting[BN + threadIdx.x];
+				if (of_rows && static_cast<int>(threadIdx.x) < BM && m < rows)
+				{
+					float sum = 0.0f;
+#pragma unroll
+					for (int w = 0; w < WAVES_N; w++)
+						sum += meeting[2 * BN + w * BM + threadIdx.x];
+					lost[static_cast<size_t>(m) * lost_tiles + at.tile_n] = sum;
+				}
 			}
 	};
+	/*
+	 * dx = back (sum of the parts + lost W[target]) + beta dx in fp16. A wavefront has 256 columns of a row at a time and adds up what the tiles of the row lost by itself; the last 4 columns of a row are moved back to end
+	 * with it, as in RowPlace.
+	 */
+	template<typename T>
+	__global__ __launch_bounds__(256) void kernel_join_input(const float *partial, int parts, int rows, int features, int spans, T *dx, float beta, const float *back, const float *lost, int lost_tiles,
+			const int *targets, int classes, const T *w, int w_elements)
+	{
+		const int lane = threadIdx.x & 63;
+		const size_t units = static_cast<size_t>(rows) * spans, count = static_cast<size_t>(rows) * features;
+		const float scale = *back;
+		for (size_t unit = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); unit < units; unit += static_cast<size_t>(gridDim.x) * 4)
+		{
+			int span;
+			const size_t row = split_index(unit, spans, span);
+			float taken = 0.0f;
+			for (int t = lane; t < lost_tiles; t += 64)
+				taken += lost[row * lost_tiles + t];
+			taken = lanes_sum<64>(taken);
+			const int target = targets[row];
+			const bool given = target >= 0 && target < classes; /* else nothing was lost, and there is no row of weights to look at */
+			const T *weights = w + static_cast<size_t>(given ? target : 0) * w_elements;
+			const int column = span * 256 + lane * 4;
+			if (column >= features)
+				continue;
+			const float *src = partial + row * features;
+			T *dst = dx + row * features;
+			if (features >= 4)
+			{
+				const RowPlace place = place_in_row<4>(column, features);
+				float v[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+				for (int p = 0; p < parts; p++)
+				{
+					Elements<float, 4> x;
+					x.load(place.in(src + p * count));
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						v[e] += x[e];
+				}
+				Elements<T, 4> of_target, old;
+				of_target.load(place.in(weights));
+				if (beta != 0.0f)
+					old.load(place.in(dst));
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+				{
+					v[e] = scale * (given ? fmaf(taken, of_target[e], v[e]) : v[e]);
+					if (beta != 0.0f)
+						v[e] = fmaf(beta, old[e], v[e]);
+				}
+				store_nearest<4>(place.in(dst), v, place.skip);
+			}
+			else
+				for (int c = column; c < features; c++)
+				{
+					float v = 0.0f;
+					for (int p = 0; p < parts; p++)
+						v += src[p * count + c];
+					v = scale * (given ? fmaf(taken, static_cast<float>(weights[c]), v) : v);
+					dst[c] = static_cast<T>(beta != 0.0f ? fmaf(beta, static_cast<float>(dst[c]), v) : v);
+				}
+		}
+	}
 
 	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
 	struct LossShape
@@ -481,25 +576,30 @@ namespace
 	{
 		return plan_product(s.rows, classes, false, s.features, s.element_size, false);
 	}
-	/* rows of d: with its low part, which dx is made of too, twice as many */
-	int rows_of_d(const LossShape &s)
-	{
-		return keeps_low_part(s.rows, s.element_size) ? 2 * s.rows : s.rows;
-	}
 	ProductPlan input_plan(const LossShape &s, int classes)
 	{
-		return plan_product(rows_of_d(s), s.features, false, classes, s.element_size, true);
+		return plan_product(s.rows, s.features, false, classes, s.element_size, true);
 	}
 	ProductPlan weights_plan(const LossShape &s, int classes)
 	{
 		return plan_product(classes, s.features, false, s.rows, s.element_size, true, false);
 	}
+	/* columns of tiles of all pieces; a piece's classes are whole tiles, but for the last one's */
+	int tile_width(const LossShape &s, int piece)
+	{
+		return std::max(logits_plan(s, piece).tile, 128);
+	}
 	struct LossSpace
 	{
 			size_t x, w, partials, target_logits; /* forward */
-			size_t d, dx, parts, sums, factors, scale; /* backward */
+			size_t d, dx, parts, sums, lost, factors, scale; /* backward */
 			size_t total;
 	};
+	/* whether dx comes about in fp32 first: several pieces or parts, or something to give back to it */
+	bool dx_in_parts(const LossShape &s, int piece)
+	{
+		return s.element_size == 2 || piece < s.classes || input_plan(s, piece).parts > 1;
+	}
 	LossSpace loss_space(const LossShape &s, bool backward)
 	{
 		LossSpace space { };
@@ -528,10 +628,11 @@ namespace
 				at = begin;
 				const int classes = classes_of_piece(s);
 				const ProductPlan input = input_plan(s, classes), weights = weights_plan(s, classes);
-				space.d = take(round_up(classes, pieces) * s.element_size * rows_of_d(s));
-				space.dx = take((classes < s.classes || input.parts > 1 || rows_of_d(s) > s.rows) ? sizeof(float) * input.parts * rows_of_d(s) * s.features : 0);
+				space.d = take(round_up(classes, pieces) * s.element_size * s.rows);
+				space.dx = take(dx_in_parts(s, classes) ? sizeof(float) * input.parts * s.rows * s.features : 0);
 				space.parts = take(part_bytes(weights, classes, s.features));
 				space.sums = take(sizeof(float) * classes * logits_plan(s, classes).tiles_m);
+				space.lost = take(s.element_size == 2 ? sizeof(float) * s.rows * ceil_div(s.classes, tile_width(s, classes)) : 0);
 				space.factors = take(sizeof(float) * s.rows);
 				space.scale = take(sizeof(float) * (SCALE_GROUPS + 1));
 				at = std::max(at, forward_end);
@@ -600,8 +701,9 @@ namespace
 		w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
 		const size_t row_bytes = padded * sizeof(T), outputs = static_cast<size_t>(s.rows) * s.features;
 		const ProductPlan whole_input = input_plan(s, most);
-		const int d_rows = rows_of_d(s), halves = d_rows / std::max(s.rows, 1); /* [part][d, its low part][rows][features] */
-		const bool dx_in_parts = most < s.classes || whole_input.parts > 1 || halves > 1;
+		const bool in_parts = dx_in_parts(s, most);
+		const int width = tile_width(s, most), lost_tiles = ceil_div(s.classes, width);
+		float *lost = reinterpret_cast<float*>(workspace + space.lost);
 		/* the last piece, which may be smaller, is cut by the plans of the others: the workspace is sized by them */
 		for (int first = 0; first < s.classes; first += most)
 		{
@@ -609,23 +711,11 @@ namespace
 			const uint8_t *weights = reinterpret_cast<const uint8_t*>(w) + first * row_bytes;
 			{
 				ProductPlan plan = logits_plan(s, most);
-				plan.tiles_n = ceil_div(classes, std::max(plan.tile, 128));
+				plan.tiles_n = ceil_div(classes, width);
 				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
 				const Operand b { weights, row_bytes, classes, padded };
-				const auto make_d = [&](auto with_low)
-				{
-					launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T, decltype(with_low)::value> { bias != nullptr ? bias + first : nullptr, targets, lse,
-							factors, d, d + static_cast<size_t>(s.rows) * row_elements, db.data != nullptr ? sums : nullptr, first, classes, row_elements });
-				};
-				if constexpr (sizeof(T) == 2)
-				{
-					if (halves > 1 && dx != nullptr)
-						make_d(std::true_type());
-					else
-						make_d(std::false_type());
-				}
-				else
-					make_d(std::false_type());
+				launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T> { bias != nullptr ? bias + first : nullptr, targets, lse, factors, d,
+						db.data != nullptr ? sums : nullptr, dx != nullptr ? lost + first / width : nullptr, lost_tiles, first, classes, row_elements });
 				if (db.data != nullptr)
 					launch_sum_partials(stream, sums, plan.tiles_m, static_cast<size_t>(classes), static_cast<uint8_t*>(db.data) + static_cast<size_t>(first) * size_of(db.dtype), db.dtype, classes,
 							beta_weights, back);
@@ -634,11 +724,11 @@ namespace
 			{
 				ProductPlan plan = whole_input; /* a part that has no chunk left adds nothing */
 				plan.chunks = ceil_div(classes, 128 / static_cast<int>(sizeof(T)));
-				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), d_rows, row_elements };
+				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), s.rows, row_elements };
 				const Operand b { weights, row_bytes, padded, classes };
-				if (dx_in_parts)
-					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, d_rows, PartEpilogue { partial_dx, halves * outputs, s.features, first > 0 });
-				else
+				if (in_parts)
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
+				else if constexpr (sizeof(T) == 4)
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, StoreEpilogue<T> { dx, s.features, beta_dx, back });
 			}
 			if (dw.data != nullptr)
@@ -654,8 +744,19 @@ namespace
 					product_to<T, T, Side::COLUMNS, Side::COLUMNS>(stream, plan, a, b, classes, s.features, ptr<T>(dw) + offset, beta_weights, back, parts);
 			}
 		}
-		if (dx != nullptr && dx_in_parts)
-			launch_join_parts(stream, partial_dx, halves * whole_input.parts, outputs, dx, beta_dx, back);
+		if (dx != nullptr && in_parts)
+		{
+			if constexpr (sizeof(T) == 2)
+			{
+				const int spans = ceil_div(s.features, 256);
+				const size_t groups = std::min<size_t>((static_cast<size_t>(s.rows) * spans + 3) / 4, 1 << 16);
+				hipLaunchKernelGGL((kernel_join_input<T>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, partial_dx, whole_input.parts, s.rows, s.features, spans, dx, beta_dx, back, lost,
+						lost_tiles, targets, s.classes, w, padded);
+				MLHIP_CHECK(hipGetLastError());
+			}
+			else
+				launch_join_parts(stream, partial_dx, whole_input.parts, outputs, dx, beta_dx, back);
+		}
 	}
 
 	bool weight_type(const mlTensor_t &t, const mlTensor_t &x)

@@ -290,10 +290,15 @@ namespace mlhip
 			}
 			Out *place;
 
+			typedef Out vec4_t __attribute__((ext_vector_type(4)));
+
+			__device__ __forceinline__ void put(int row, int column, vec4_t v) const
+			{
+				*reinterpret_cast<vec4_t*>(place + row * STRIDE + column) = v;
+			}
 			__device__ __forceinline__ void put(int row, int column, float a, float b, float c, float d) const
 			{
-				typedef Out vec4_t __attribute__((ext_vector_type(4)));
-				*reinterpret_cast<vec4_t*>(place + row * STRIDE + column) = vec4_t { static_cast<Out>(a), static_cast<Out>(b), static_cast<Out>(c), static_cast<Out>(d) };
+				put(row, column, vec4_t { static_cast<Out>(a), static_cast<Out>(b), static_cast<Out>(c), static_cast<Out>(d) });
 			}
 			template<int ROWS, int THREADS, typename F>
 			__device__ __forceinline__ void for_vectors(int m0, int rows, int n0, int columns, F &&f) const

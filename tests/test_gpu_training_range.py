@@ -115,3 +115,50 @@ def test_slope_of_the_sigmoid_keeps_its_digits_on_both_sides(ctx, dtype):
     want = e / (1 + e) ** 2
     steps = 14 + (2 * np.abs(g) if dtype == "float16" else 0)
     assert R.worst(db.copyToHost(ctx)[0], want, steps * R.FP32 * want) <= 1
+
+
+# One rounding to fp16 is off by 2^-11 / sqrt 3 of a step's lower end, and 0.735 of that over numbers of any size: 2.07e-4 in norm. dx alone is rounded where what rounding leaves of d is kept; where d were rounded too, both would
+# add up to 2.07e-4 sqrt 2 = 2.93e-4. Between the two:
+ONE_ROUNDING = 2.45e-4
+
+
+def off_in_norm(got, want):
+    return np.linalg.norm(R.numbers(got) - want) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("rows,features,hidden", [(1, 2048, 700), (5, 1001, 129), (33, 1003, 513), (64, 520, 301)])
+def test_dx_of_few_rows_of_the_gated_layer_has_no_rounding_of_d(ctx, rows, features, hidden):
+    rng = np.random.default_rng(rows)
+    x, w = rng.standard_normal((rows, features)), rng.standard_normal((2, hidden, features)) / np.sqrt(features)
+    p, dy = rng.standard_normal((rows, 2, hidden)), rng.standard_normal((rows, hidden))
+    x, w, p, dy = (R.bits(a, "float16") for a in (x, w, p, dy))
+    X, W, P, DY = (ml.toDevice(ctx, a) for a in (x, w, p, dy))
+    dx = ml.Tensor((rows, features), "float16")
+    ml.gatedDenseBackward(ctx, X, W, P, DY, 0.0, dx, 0.0, None, None, "silu", space(ctx, X, W, True))
+    assert off_in_norm(dx.copyToHost(ctx), R.gated_gradients(*[R.numbers(a) for a in (x, w, p, dy)], "silu")[0]) <= ONE_ROUNDING
+
+
+DX_OF_LOSSES = [(*size, sharp, common) for size in [(1, 2048, 3000), (5, 1001, 400), (33, 1003, 777), (64, 333, 2001), (65, 256, 4000), (300, 3, 900), (700, 333, 2001)] for sharp in (False, True) for common in (0, 3, 10)]
+
+
+@pytest.mark.parametrize("rows,features,classes,sharp,common", DX_OF_LOSSES + [(2100, 64, 70003, False, 10)])  # the last one in two pieces
+def test_dx_of_the_cross_entropy_has_no_rounding_of_d(ctx, rows, features, classes, sharp, common):
+    """For any number of rows and with weights whose rows have a large part in common, which the rounding of d would carry into dx: up to 2e-3 where it is ten times the rest. sharp: probabilities near 1 among the other
+    classes, each of which is rounded, so that dx has two roundings after all."""
+    rng = np.random.default_rng(100 + rows)
+    x, w = (3.0 if sharp else 0.3) * rng.standard_normal((rows, features)), (rng.standard_normal((classes, features)) + common * rng.standard_normal(features)) / np.sqrt(features)
+    targets, dloss = rng.integers(0, classes, rows).astype(np.int32), (rng.uniform(0.7, 1.3, rows) * np.sqrt(2)).astype(np.float32)
+    targets[3::11] = -1
+    x, w = R.bits(x, "float16"), R.bits(w, "float16")
+    X, W, T, DL = (ml.toDevice(ctx, a) for a in (x, w, targets, dloss))
+    old = R.bits(rng.standard_normal((rows, features)), "float16")
+    loss, lse, dx, added = ml.Tensor((rows,), "float32"), ml.Tensor((rows,), "float32"), ml.Tensor((rows, features), "float16"), ml.toDevice(ctx, old)
+    work = ml.Tensor((ml.linearCrossEntropyGetWorkspaceSize(ctx, X, W, True),), "uint8")
+    work.setall(ctx, 0xff)
+    ml.linearCrossEntropyForward(ctx, X, W, None, T, loss, lse, work)
+    ml.linearCrossEntropyBackward(ctx, X, W, None, T, lse, DL, 0.0, dx, 0.0, None, None, work)
+    want = R.cross_entropy_gradients(R.numbers(x), R.numbers(w), np.zeros(classes), targets, dloss.astype(np.float64))[0]
+    assert off_in_norm(dx.copyToHost(ctx), want) <= (1.2 * np.sqrt(2) * 2.07e-4 if sharp else ONE_ROUNDING)
+    assert (R.numbers(dx.copyToHost(ctx))[3::11] == 0).all()
+    ml.linearCrossEntropyBackward(ctx, X, W, None, T, lse, DL, 0.5, added, 0.0, None, None, work)
+    assert off_in_norm(added.copyToHost(ctx), want + 0.5 * R.numbers(old)) <= (1.2 * np.sqrt(2) * 2.07e-4 if sharp else ONE_ROUNDING)
