@@ -6,16 +6,18 @@
  *   dx = d W,  dW = d^T x,  db = sum_rows d                   W = [Wg; Wu], stored as [2, hidden, features]
  *
  * Forward: one launch. A tile's columns are half gate, half up of the same hidden units, so the epilogue has both projections of an element and neither goes to memory, unless the backward pass is to have
- * them (`projections`, in the tensors' type). Up to 64 rows the weights stream through registers (few_rows.hpp). Where there are too few tiles for the chip the product is split along the
+ * them (`projections`, in the tensors' type). The weights of few rows are streamed past them (few_rows.hpp). Where there are too few tiles for the chip the product is split along the
  * features, and the launch that adds the parts up applies the gate.
- * Backward: one pass over dy and the projections makes d and the partial sums of db (bound by memory), then two products (bound by the matrix cores). d is stored in the tensors' type: its rounding, half a step per
- * element, averages out in sums over as many hidden units or rows as the products have, and is what a stored gradient costs anywhere else in a network of that type (few
- * rows: keeps_low_part); db is summed before the rounding. In fp16 d is scaled where it would leave the type's range (shift_of).
+ * Backward: one pass over dy and the projections makes d and the partial sums of db (bound by memory), then two products (bound by the matrix cores). The matrix cores take operands of the tensors' type, so d is stored
+ * in it, in fp16 scaled where it would leave the type's range (shift_of). Its rounding, half a step per element, adds as much to dx and dW as their own rounding does (2.9e-4 off instead of 2.1e-4; dx of few
+ * rows 2.1e-4: keeps_low_part); keeping all of d would double both products. db is summed before the rounding.
  * fp16: 1 row of 4096 -> 8192 23.5 us (5.7 TB/s); 57600 x 256 -> 1024 with gelu, bias and the projections kept 133 us (2.9 TB/s: neither memory, 74 us, nor the matrix cores, 47 us, but what is left of their
  * overlap with the gate's arithmetic); backward of 8192 x 2048 -> 5504 715 us (1.03 PFLOP/s): d 77 us (5.9 TB/s), dx 303 us (1.22 PFLOP/s), dW 340 us.
  */
 #include "few_rows.hpp"
 #include "product_tiles.hpp"
+
+#include <limits>
 
 namespace
 {
@@ -276,6 +278,23 @@ namespace
 	}
 
 	/* ---- backward: d and the sums of its columns ------------------------------------------------------------------------------ */
+	/*
+	 * Whether what fp16 leaves of d is kept beside it, as more rows of d, and multiplied with the weights like them. dx is 2.1e-4 off then (in norm, against 64 bits), which its own rounding costs; else 2.9e-4, two roundings:
+	 * a relative error of every term is the same error of their sum, however many terms it has. This is a matter of cost alone. Up to 64 rows both parts lie in the 128 rows of one tile and the weights are read once; further
+	 * on dx takes another product. us without / with, 2048 -> 5504: 1 row 40 / 43, 64 rows 45 / 52; 65 rows 47 / 57, 256 rows 65 / 85, 2048 rows 287 / 309, 8192 rows 303 more of 720. dw, a sum over the rows, would need x
+	 * twice, and has two roundings for any number of rows.
+	 */
+	bool keeps_low_part(int rows, int element_size)
+	{
+		return element_size == 2 && rows <= 64;
+	}
+	/* what rounding x to the type leaves; nothing of what is infinite there, so that infinities stay what they are (inf - inf is no number) */
+	template<typename T>
+	__device__ __forceinline__ float low_part(float x)
+	{
+		const float high = static_cast<float>(static_cast<T>(x));
+		return fabsf(high) <= std::numeric_limits<float>::max() ? x - high : 0.0f;
+	}
 	/*
 	 * d is in memory as d 2^shift. In fp16 dy u a'(g) may pass the type's largest value, 65504, where dx, a sum of such terms with weights, does not; and gradients of losses that nobody scaled, 1e-5 or so, are subnormal
 	 * there (dw 2.8e-3 off instead of 3e-4, also where it is asked for in fp32). With its largest element between 2^-3 and 2^15 d stays as it is: elements down to 2^-11 of the largest are normal numbers then, and

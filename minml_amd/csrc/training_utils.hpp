@@ -219,21 +219,6 @@ namespace mlhip
 					reinterpret_cast<float*>(second));
 		MLHIP_CHECK(hipGetLastError());
 	}
-	/*
-	 * Whether what fp16 leaves of a product's gradient d is kept beside it, as more rows of d, and multiplied with the weights like them. With few rows that costs nothing (a tile has room for them, and dx is added up from
-	 * parts as it is), and the rounding of d, which many rows or columns average out, would show: dx is 2.1e-4 off against 64 bits instead of 3.0e-4 to 3.3e-4.
-	 */
-	inline bool keeps_low_part(int rows, int element_size)
-	{
-		return element_size == 2 && rows <= 64;
-	}
-	/* what rounding x to the type leaves; nothing of what is infinite there, so that infinities stay what they are (inf - inf is no number) */
-	template<typename T>
-	__device__ __forceinline__ float low_part(float x)
-	{
-		const float high = static_cast<float>(static_cast<T>(x));
-		return fabsf(high) <= std::numeric_limits<float>::max() ? x - high : 0.0f;
-	}
 	constexpr int SCALE_BITS = 15; /* a gradient that is scaled has its largest element just below 2^15: fp16 ends at 2^16 */
 	/* the exponent of the power of two above the largest element */
 	__device__ __forceinline__ int scale_exponent(float top)
