@@ -261,7 +261,7 @@ extern "C"
 			float beta_weights, mlTensor_t dw, mlTensor_t db, mlGate_t gate, void *workspace, size_t workspace_size);
 
 	/*
-	 * The softmax cross entropy of a last dense layer over many classes, from the layer's input: with z = x w^T + b, lse = log sum exp z and loss = lse - z[target], both fp32 [..]. x [.., features],
+	 * The softmax cross entropy of a last dense layer over many classes, from the layer's input: with z = x w^T + b, lse = log sum exp z and loss = lse - z[target], both fp32 [..] ([1] for x [features]). x [.., features],
 	 * w [classes, features], b [classes] or empty, targets int32 [..]; a row whose target is none of 0 .. classes - 1 has loss 0 and no gradient (its lse is given all the same; its x has to be finite, since dw is a product
 	 * with zeros there). The logits are never in
 	 * memory: the backward pass makes them again, in pieces of the classes. Backward: dloss fp32 [..] (the gradient of every row's loss) -> dx, dw, db as above. x and w have to be aligned to 16

@@ -804,7 +804,7 @@ def _require_loss(input, weights, bias, targets, *fp32):
     _require(input.dtype in _FLOATS and _same_dtype(input, weights, bias), "dtype mismatch")
     _require(len(weights.shape) == 2 and len(input.shape) >= 1 and weights.shape[1] == input.shape[-1], "weights must be [classes, features]")
     _require(bias is None or bias.volume() == weights.shape[0], "bias must be [classes]")
-    lead = tuple(input.shape[:-1])
+    lead = tuple(input.shape[:-1]) or (1,)  # a tensor without dimensions has no elements
     _require(targets.dtype == B.DTYPE_INT32 and tuple(targets.shape) == lead, "one int32 target per row")
     for t in fp32:
         _require(t.dtype == B.DTYPE_FLOAT32 and tuple(t.shape) == lead, "loss, lse and their gradient must be fp32 with one element per row")
@@ -817,7 +817,7 @@ def linearCrossEntropyGetWorkspaceSize(context, input, weights, backward):
 
 def linearCrossEntropyForward(context, input, weights, bias, targets, loss, lse, workspace):
     """loss = lse - z[target] and lse = log sum exp z for z = input weights^T + bias, without keeping z: input [.., features], weights [classes, features], bias [classes] or None, targets int32
-    [..], loss and lse fp32 [..]. A row whose target is no class has loss 0."""
+    [..], loss and lse fp32 [..] (of a single row [features]: [1]). A row whose target is no class has loss 0."""
     _require_loss(input, weights, bias, targets, loss, lse)
     _launch("linear_cross_entropy_forward", context.handle, input.desc(), weights.desc(), _all(bias), targets.desc(), loss.desc(), lse.desc(), *_space(workspace))
 

@@ -220,3 +220,18 @@ def test_recorded_pass_gives_the_eager_bits(ctx, rows, features, classes):
             for _, out in passes:
                 assert all(np.array_equal(t.copyToHost(ctx), e) for t, e in zip(out, eager))
     other.destroy()
+
+
+def test_a_single_row_without_leading_dimensions(ctx):
+    rng = np.random.default_rng(10)
+    x, w, b, _, _ = inputs(rng, 1, 72, 300, "float16")
+    results = []
+    for lead in ((1,), ()):
+        X, W, Bias = (ml.toDevice(ctx, a) for a in (x.reshape(lead + (72,)), w, b))
+        T, DL = ml.toDevice(ctx, np.array([17], np.int32)), ml.toDevice(ctx, np.array([0.75], np.float32))
+        loss, lse, dx = ml.Tensor((1,), "float32"), ml.Tensor((1,), "float32"), ml.Tensor(X.shape, "float16")
+        work = space(ctx, X, W, True)
+        ml.linearCrossEntropyForward(ctx, X, W, Bias, T, loss, lse, work)
+        ml.linearCrossEntropyBackward(ctx, X, W, Bias, T, lse, DL, 0.0, dx, 0.0, None, None, work)
+        results.append([t.copyToHost(ctx).reshape(-1) for t in (loss, lse, dx)])
+    assert all(np.array_equal(a, c) for a, c in zip(*results)) and results[0][0][0] > 0

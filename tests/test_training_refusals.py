@@ -197,3 +197,20 @@ def test_results_over_inputs_are_refused():
     refused("linear_cross_entropy_forward", x, wc, NULL, t, f, g, space, n, why="null context")
     refused("linear_cross_entropy_backward", x, wc, NULL, t, f, g, 0.0, x, 0.0, NULL, NULL, space, n, why=overlaps)
     refused("linear_cross_entropy_backward", x, wc, NULL, t, f, g, 0.0, NULL, 0.0, wc, NULL, space, n, why=overlaps)
+
+
+def test_a_single_row_without_leading_dimensions_is_taken():
+    class Ctx:
+        handle = None
+
+    x, w, wc = fake((16,)), fake((2, 24, 16)), fake((90, 16))
+    t, loss, lse, g = fake((1,), "int32"), *(fake((1,), "float32") for _ in range(3))
+    space = ml.Tensor((1 << 22,), "uint8", _ptr=1 << 50)
+    for call in (lambda: ml.layerNormForward(Ctx, x, None, None, fake((16,))), lambda: ml.gatedDenseForward(Ctx, x, w, None, fake((24,)), fake((2, 24)), "silu", space),
+                 lambda: ml.gatedDenseBackward(Ctx, x, w, fake((2, 24)), fake((24,)), 0.0, fake((16,)), 0.0, None, None, "silu", space),
+                 lambda: ml.linearCrossEntropyForward(Ctx, x, wc, None, t, loss, lse, space),
+                 lambda: ml.linearCrossEntropyBackward(Ctx, x, wc, None, t, lse, g, 0.0, fake((16,)), 0.0, None, None, space)):
+        with pytest.raises(ValueError, match="null context"):
+            call()
+    with pytest.raises(ValueError, match="one int32 target per row"):
+        ml.linearCrossEntropyForward(Ctx, x, wc, None, fake((2,), "int32"), loss, lse, space)
