@@ -281,7 +281,7 @@ namespace
 	/*
 	 * Whether what fp16 leaves of d is kept beside it, as more rows of d, and multiplied with the weights like them. dx is 2.1e-4 off then (in norm, against 64 bits), which its own rounding costs; else 2.9e-4, two roundings:
 	 * a relative error of every term is the same error of their sum, however many terms it has. This is a matter of cost alone. Up to 64 rows both parts lie in the 128 rows of one tile and the weights are read once; further
-	 * on dx takes another product. us without / with, 2048 -> 5504: 1 row 40 / 43, 64 rows 45 / 52; 65 rows 47 / 57, 256 rows 65 / 85, 2048 rows 287 / 309, 8192 rows 303 more of 720. dw, a sum over the rows, would need x
+	 * on dx takes another product. us without / with, 2048 -> 5504: 1 row 40 / 43, 64 rows 45 / 52; 65 rows 47 / 57, 256 rows 65 / 85, 2048 rows 287 / 309, 8192 rows 732 / 1101. dw, a sum over the rows, would need x
 	 * twice, and has two roundings for any number of rows.
 	 */
 	bool keeps_low_part(int rows, int element_size)

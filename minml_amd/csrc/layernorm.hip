@@ -593,7 +593,7 @@ extern "C"
 		if (volume(x) == 0)
 			return;
 		MLHIP_REQUIRE(x.data != nullptr && y.data != nullptr, "layer_norm_forward: null pointer");
-		require_apart( { y }, { x, w, b }, "layer_norm_forward", x.data);
+		require_apart( { y }, { w, b }, "layer_norm_forward", { x });
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
 			layer_norm_forward<half_t>(on.stream, x, w, b, y, epsilon);
@@ -642,7 +642,7 @@ extern "C"
 			MLHIP_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_size >= hip_layer_norm_get_workspace_size(shape_of(x), x.dtype),
 					"layer_norm_backward: the workspace is too small or not aligned to 16 bytes");
 		}
-		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, dy }, "layer_norm_backward", dx.data);
+		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { w }, "layer_norm_backward", { x, dy });
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
 			layer_norm_backward<half_t>(on.stream, x, w, dy, beta_dx, dx, beta_weights, dw, db, reinterpret_cast<float*>(workspace), epsilon);

@@ -58,15 +58,17 @@ namespace mlhip
 				return bytes > 0 && other.bytes > 0 && begin < other.begin + other.bytes && other.begin < begin + bytes;
 			}
 	};
-	/* results may lie over nothing else of the call, but for the one named `in_place` where it is exactly one of the inputs that may be overwritten */
-	inline void require_apart(std::initializer_list<Extent> results, std::initializer_list<Extent> inputs, const char *name, const void *in_place = nullptr)
+	/* results may lie over nothing else of the call; but the first one may be exactly one of the inputs that may be overwritten */
+	inline void require_apart(std::initializer_list<Extent> results, std::initializer_list<Extent> inputs, const char *name, std::initializer_list<Extent> replaceable = { })
 	{
 		for (const Extent *r = results.begin(); r != results.end(); r++)
 		{
 			for (const Extent *other = results.begin(); other != r; other++)
 				MLHIP_REQUIRE(!r->meets(*other), std::string(name) + ": results overlap");
 			for (const Extent &input : inputs)
-				MLHIP_REQUIRE(!r->meets(input) || (r->begin == in_place && r->begin == input.begin && r->bytes == input.bytes), std::string(name) + ": a result overlaps an input");
+				MLHIP_REQUIRE(!r->meets(input), std::string(name) + ": a result overlaps an input");
+			for (const Extent &input : replaceable)
+				MLHIP_REQUIRE(!r->meets(input) || (r == results.begin() && r->begin == input.begin && r->bytes == input.bytes), std::string(name) + ": a result overlaps an input");
 		}
 	}
 

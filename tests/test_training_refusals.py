@@ -214,3 +214,18 @@ def test_a_single_row_without_leading_dimensions_is_taken():
             call()
     with pytest.raises(ValueError, match="one int32 target per row"):
         ml.linearCrossEntropyForward(Ctx, x, wc, None, fake((2,), "int32"), loss, lse, space)
+
+
+def test_layer_norm_may_overwrite_its_rows_but_not_its_weights():
+    """Of a single row the weights have the row's size; only the input and the gradient may be where dx is."""
+    x, dy, w, b = (fake((1, 16)).desc() for _ in range(4))
+    backward = lambda dx, dw, why: refused("layer_norm_backward", x, w, dy, 0.0, dx, 0.0, dw, NULL, 0x7000, 1 << 20, 1e-5, why=why)
+    backward(w, NULL, "overlap")
+    backward(NULL, x, "overlap")
+    backward(fake((1, 16)).desc(), dy, "overlap")
+    backward(x, NULL, "null context")
+    backward(dy, b, "null context")
+    refused("layer_norm_forward", x, w, b, w, 1e-5, why="overlap")
+    refused("layer_norm_forward", x, w, b, b, 1e-5, why="overlap")
+    refused("layer_norm_forward", x, x, b, x, 1e-5, why="overlap")
+    refused("layer_norm_forward", x, w, b, x, 1e-5, why="null context")
