@@ -233,8 +233,8 @@ extern "C"
 	 *      calls are rounded to nearest. Gradients of weights and biases are sums over all rows in fp32, added up in a fixed order (the same bits on every run), and may be asked for
 	 *      in fp32 where the tensors are fp16. A gradient tensor whose data is NULL is not computed; where a beta is not 0, what the gradient tensor held is multiplied
 	 *      by it and added (gradients of several batches). Workspaces are the caller's: at least as many bytes as the call's own function says, aligned to
-	 *      16 bytes, free for anything else once the call's work on the stream is done; calls that may run at the same time (other contexts, graphs replayed on other streams) need one each.
-	 *      Tensors need the alignment of one element only. Results may not overlap inputs unless a call says so. ---- */
+	 *      256 bytes (layer normalisation: 16), free for anything else once the call's work on the stream is done; calls that may run at the same time (other contexts, graphs replayed on other streams) need one each.
+	 *      x and w of the gated layer and the cross entropy have to be aligned to 16 bytes, all other tensors to one element. Results may not overlap inputs unless a call says so. ---- */
 	/*
 	 * y[i, j] = (x[i, j] - mean_i) / sqrt(var_i + epsilon) * w[j] + b[j] over the last dimension, of at most 2^28 elements; w and b may be empty. y may be x.
 	 * Backward: dx = beta_dx * dx + the gradient of x, dw = beta_weights * dw + sum_i dy n, db = beta_weights * db + sum_i dy; the statistics are computed again from x. dx may be dy or x.
@@ -246,9 +246,9 @@ extern "C"
 
 	/*
 	 * The gated dense layer: y = a(x Wg^T + bg) * (x Wu^T + bu). x [.., features], w [2, hidden, features] (the gate's matrix, then the other), b [2, hidden] or empty, y [.., hidden]; `projections`
-	 * [.., 2, hidden] takes both projections, which the backward pass needs, or is empty. Backward: dy [.., hidden] -> dx, dw, db as above. x and w have to be aligned to 16 bytes, workspaces of
-	 * these calls to 256. Gradients of the projections are kept in the tensors' type in between, in fp16 with a common power of two where their largest is below 2^-3 or not below 2^15, so that they neither overflow
-	 * nor lose bits; rounded to nearest, which costs dx and dw as much as their own rounding does.
+	 * [.., 2, hidden] takes both projections, which the backward pass needs, or is empty. Backward: dy [.., hidden] -> dx, dw, db as above. Gradients
+	 * of the projections are kept in the tensors' type in between, rounded to nearest, which costs dx and dw as much as their own rounding does (also where dw is asked for in fp32); in fp16 with a common power of two
+	 * where their largest is below 2^-3 or not below 2^15, so that they neither overflow nor lose bits among the subnormal numbers. The gates of fp16 tensors are 2^-19 off at most, also in an fp32 db.
 	 */
 	typedef enum
 	{
@@ -263,9 +263,10 @@ extern "C"
 	/*
 	 * The softmax cross entropy of a last dense layer over many classes, from the layer's input: with z = x w^T + b, lse = log sum exp z and loss = lse - z[target], both fp32 [..] ([1] for x [features]). x [.., features],
 	 * w [classes, features], b [classes] or empty, targets int32 [..]; a row whose target is none of 0 .. classes - 1 has loss 0 and no gradient (its lse is given all the same; its x has to be finite, since dw is a product
-	 * with zeros there). The logits are never in
-	 * memory: the backward pass makes them again, in pieces of the classes. Backward: dloss fp32 [..] (the gradient of every row's loss) -> dx, dw, db as above. x and w have to be aligned to 16
-	 * bytes, workspaces of these calls to 256.
+	 * with zeros there). The logits are never in memory: the backward pass makes them again, in pieces of the classes. Backward: dloss fp32 [..] (the gradient of every row's loss) -> dx, dw, db as above. The
+	 * gradients of the logits are kept in the tensors' type in between, in fp16 with one power of two for all rows, that of the largest |dloss|: probabilities below 2^-28 times (largest |dloss| / the row's) lose bits,
+	 * and the rounding costs dw as much as its own does.
+	 * The workspace holds up to 256 MB of these gradients, dx in fp32, 8 bytes for every row of every tile of logits, and a copy of x and w where their rows are no multiple of 16 bytes.
 	 */
 	size_t hip_linear_cross_entropy_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, mlDataType_t dtype, bool backward); /* bytes; the backward pass's is enough for both */
 	void hip_linear_cross_entropy_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t targets, mlTensor_t loss, mlTensor_t lse,

@@ -7,14 +7,15 @@
  *
  * Forward: a tile's logits stay in the accumulators; every row of the tile leaves its largest logit and the sum of exponentials about it, and a second launch joins these pairs. A few rows stream
  * the weights past themselves instead (few_rows.hpp) and memory bounds it; else the matrix cores do.
- * Backward: the classes are taken in pieces of as many as make d 256 MB (so it stays in the last-level cache between its makers and users, and the workspace small whatever the vocabulary). For each
+ * Backward: the classes are taken in pieces of as many as make d 256 MB, so that it stays in the last-level cache between its makers and users and does not grow with the vocabulary, as the 8 bytes of a row and a tile of
+ * the forward pass do, and the padded copy of the weights where their rows are no multiple of 16 bytes. For each
  * piece the logits are made again, which costs a quarter of the operations and spares rows x classes of memory; the epilogue turns them into d; then d is multiplied with the piece's weights, added to
  * dx in fp32, and with x, which gives the piece's rows of dW.
  * d is stored in the tensors' type. In fp16 a probability of one class in 100 000 would be subnormal, so d is scaled by 2^15 / s with s the power of two above the largest |dloss|: of that loss's row probabilities down to
  * 2^-28 keep their 11 bits, of a row whose dloss is 2^-k of it down to 2^(k - 28); what is smaller is off by 2^-39 of the largest |dloss| at most. The products' results are scaled back, exactly, in fp32. What the rounding of
  * d, half a step per element, does to dx is given back (GradientEpilogue); in dW it counts as much as the rounding of dW itself; db is summed before it.
- * fp16: 7 rows of 2048 x 65536 classes 50 us (5.3 TB/s); 4096 rows of 1024 x 50001 433 us (0.97 PFLOP/s), of 2048 x 65536 940 us (1.17); the gradients of the latter 2.93 ms, in two pieces of d 553 us each (0.99 PFLOP/s, a
- * fourth of it the epilogue), dx 461 (1.19), dW 457 (1.20).
+ * fp16: 7 rows of 2048 x 65536 classes 50 us (5.3 TB/s); 4096 rows of 1024 x 50001 427 us (0.98 PFLOP/s), of 2048 x 65536 950 us (1.16); the gradients of the latter 2.98 ms, in two pieces of d 576 us each (0.95 PFLOP/s, a
+ * fourth of it the epilogue), dx 470 (1.17), dW 462 (1.19), and 30 us to join the parts of dx.
  */
 #include "few_rows.hpp"
 #include "product_tiles.hpp"
@@ -30,6 +31,10 @@ namespace
 	{
 			float top, sum;
 	};
+	/*
+	 * exp(z - top) by the hardware's exponential in fp32, too: the rounding of its argument costs |z - top| 2^-24 of a term, and of their sum the mean of that over the probabilities, which is at most the logarithm of the
+	 * number of classes: lse is off by 7e-7 for 65536 of them, about as much as its own rounding to fp32.
+	 */
 	__device__ __forceinline__ float exp_about(float z, float top)
 	{
 		/* infinities: exp(inf - inf) is 1 here, so that a row with a logit of +inf has lse = +inf, and one of -inf alone -inf */

@@ -14,13 +14,14 @@
  * product, whatever the size of the operand, and a lane that lies outside (a row past the end, k past the end) is sent behind the buffer's end, which reads as zero. So no element outside an operand
  * reaches an accumulator, and NaN or infinities beside it do not either.
  *
- * 256x256 (8 wavefronts, one workgroup per compute unit): two slots of four panels, refilled panel by panel: the wavefront's 128 x 64 share is multiplied in four phases of 64 x 32, and a panel's place
- * takes the chunk after the next one as soon as its last phase is over, so a load has six phases (one and a half chunks of 64 k) to arrive.
+ * 256x256 (8 wavefronts, one workgroup per compute unit): two slots of four panels. A chunk of 64 k (fp32: 32) is multiplied in two phases, 64 x 64 of every wavefront each, with a barrier before each; a panel's
+ * place takes the chunk after the next one as soon as it has been read, so a load has about one and a half chunks to arrive.
  * 128x128 (4 wavefronts): where 256x256 tiles would leave units without work, with two slots and two workgroups per compute unit; and where k is so short that a tile is mostly beginning and end, with one
  * slot and four workgroups per unit, which hide each other's waits. fp32, which the matrix cores bound by far, also has 64x128.
  * A product with a long k and few tiles is split along k (gridDim.y): each part leaves its sums in fp32, and a launch of its own adds them up in order.
  *
- * The tile's accumulators pass through LDS in fp32, 128 rows at a time, so that the epilogue sees 8 consecutive columns per thread and whole lines per wavefront.
+ * Epilogues work on the accumulators in registers, where a lane has 16 columns of every block (TilePlace), and what goes to memory passes through LDS, in the result's own type where nothing has to be added to it
+ * there, so that neighbouring threads write whole rows, 16 bytes each.
  */
 #ifndef MINML_AMD_PRODUCT_TILES_HPP_
 #define MINML_AMD_PRODUCT_TILES_HPP_

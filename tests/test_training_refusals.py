@@ -171,6 +171,19 @@ def test_cross_entropy_workspace_does_not_grow_with_the_vocabulary():
             assert sizes[1] < rows * 2000000 * element / 2
 
 
+def test_cross_entropy_workspace_of_odd_widths_holds_the_padded_rows():
+    """Where rows are no multiple of 16 bytes a copy of x and of all of w is on top of what the next multiple needs, and nothing else."""
+    for dtype, element in ((B.DTYPE_FLOAT16, 2), (B.DTYPE_FLOAT32, 4)):
+        for rows, features, classes in ((4096, 2047, 65536), (100, 1021, 2000000), (7, 2045, 65536)):
+            piece = 16 // element
+            whole = -(-features // piece) * piece
+            for backward in (False, True):
+                odd, even = (B.fn("linear_cross_entropy_get_workspace_size")(B.make_shape((rows, f)), B.make_shape((classes, f)), dtype, backward) for f in (features, whole))
+                copies = (rows + classes) * whole * element if backward or rows > 64 else 0
+                # dx in fp32 and its parts are a little narrower
+                assert copies - 16 * 4 * rows * piece <= odd - even <= copies + 1024
+
+
 def test_results_over_inputs_are_refused():
     """Where a call does not say that a result may lie over an input, it may not; and never in part."""
     whole = fake((64, 16))
