@@ -332,14 +332,14 @@ namespace
 		if (threadIdx.x == 0)
 			*back = ldexpf(1.0f, exponent - SCALE_BITS);
 	}
-	/* the sum of four elements less that of what is stored of them, in fp32 (its own roundings are 2^-24 of d). Dot products with ones take the halves as they lie in pairs, subnormal ones too: differences element by element
-	 * take twice the instructions and registers that a 256 x 256 tile does not have (d of 4096 x 32768, k = 2048: 2 % longer than without any of this, 581 against 570 us; element by element 5 %) */
+	/* sum + what rounding takes from four elements: they, less what is stored of them, in fp32 (its own roundings are 2^-24 of d). Dot products with minus ones take the halves as they lie in pairs, subnormal ones too: differences element
+	 * by element take twice the instructions, and registers that a 256 x 256 tile does not have (d of 4096 x 32768, k = 2048: 2 % longer than without any of this, 581 against 570 us; element by element 5 %) */
 	template<typename V>
-	__device__ __forceinline__ float what_rounding_takes(const float *v, const V &stored)
+	__device__ __forceinline__ float add_what_rounding_takes(float sum, const float *v, const V &stored)
 	{
-		const half2_t ones { static_cast<half_t>(1.0f), static_cast<half_t>(1.0f) };
-		const float kept = __builtin_amdgcn_fdot2(half2_t { stored[0], stored[1] }, ones, __builtin_amdgcn_fdot2(half2_t { stored[2], stored[3] }, ones, 0.0f, false), false);
-		return ((v[0] + v[1]) + (v[2] + v[3])) - kept;
+		const half2_t minus_ones { static_cast<half_t>(-1.0f), static_cast<half_t>(-1.0f) };
+		sum = __builtin_amdgcn_fdot2(half2_t { stored[0], stored[1] }, minus_ones, sum + (v[0] + v[1]), false);
+		return __builtin_amdgcn_fdot2(half2_t { stored[2], stored[3] }, minus_ones, sum + (v[2] + v[3]), false);
 	}
 	/*
 	 * d, the sums of its columns for db, and what rounding to fp16 took from its rows. The elements of a row add up to zero by definition, so that what the rows of W have in common has no part in dx; their roundings
@@ -430,7 +430,7 @@ namespace
 								for (int e = 0; e < 4; e++)
 									total[j][4 * q + e] += v[j][4 * q + e];
 								if constexpr (sizeof(T) == 2)
-									taken[i] += what_rounding_takes(&v[j][4 * q], stored);
+									taken[i] = add_what_rounding_takes(taken[i], &v[j][4 * q], stored);
 							}
 					}
 					__syncthreads();
@@ -484,7 +484,94 @@ namespace
 			}
 	};
 	/*
-	 * dx = back (sum of the parts + lost W[target]) + beta dx in fp16. A wavefront has 256 columns of a row at a time and adds up what the tiles of the row lost by itself; the last 4 columns of a row are moved back to end
+	 * dx = back (sum + lost W[target]) + beta dx in fp16, where one product gives all of dx: in the accumulators, so that nothing in fp32 goes to memory. us, so / over fp32 and the launch that joins parts / without
+	 * giving back: gradients of 65536 x 1024, 300 classes 383 / 521 / 363, 8192 x 4096, 1000 classes 387 / 442 / 376, 16384 x 2048, 4000 classes 1031 / 1075 / 986 (its rows of W, 67 MB, come from beyond the L2).
+	 */
+	template<typename T>
+	struct InputEpilogue
+	{
+			T *out;
+			int columns;
+			float beta;
+			const float *back, *lost;
+			int lost_tiles;
+			const int *targets;
+			int classes;
+			const T *w;
+			int w_elements;
+
+			template<int BM, int BN>
+			static constexpr int lds()
+			{
+				return StoreEpilogue<T>::template lds<BM, BN>();
+			}
+			/* the rows of weights to LDS, whole rows to neighbouring threads (rows without a class: zeros), from where every lane takes what belongs to its accumulators */
+			template<int BM, int BN, typename Acc>
+			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
+			{
+				typedef Stage<T, BN> TileStage;
+				typedef typename Elements<T, TileStage::VECTOR>::vec_t vec_t;
+				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, LANES = BN / TileStage::VECTOR, AT_A_TIME = TilePlace<BM, BN>::THREADS / LANES, TURNS = BM / AT_A_TIME;
+				const TileStage stage { reinterpret_cast<T*>(lds) };
+				const int first = at.tile_m * BM, column = static_cast<int>(threadIdx.x) % LANES * TileStage::VECTOR, row0 = static_cast<int>(threadIdx.x) / LANES;
+				int target[TURNS];
+				vec_t weights_of[TURNS]; /* all on their way at once: one workgroup has the unit to itself and would wait for each */
+#pragma unroll
+				for (int u = 0; u < TURNS; u++)
+					target[u] = targets[min(first + row0 + u * AT_A_TIME, rows - 1)];
+#pragma unroll
+				for (int u = 0; u < TURNS; u++)
+				{
+					weights_of[u] = vec_t(static_cast<T>(0.0f));
+					if (target[u] >= 0 && target[u] < classes && at.tile_n * BN + column < columns) /* whole vectors: the rows of the weights are */
+						weights_of[u] = *reinterpret_cast<const vec_t*>(w + static_cast<size_t>(target[u]) * w_elements + at.tile_n * BN + column);
+				}
+				float taken[BLOCKS];
+				const float *mine[BLOCKS];
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++)
+				{
+					mine[i] = lost + static_cast<size_t>(min(first + at.row(i), rows - 1)) * lost_tiles;
+					taken[i] = 0.0f;
+				}
+				constexpr int AHEAD = 16 / BLOCKS; /* 16 loads on their way at a time */
+				for (int t = 0; t < lost_tiles; t += AHEAD)
+				{
+					float v[AHEAD][BLOCKS];
+#pragma unroll
+					for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+						for (int i = 0; i < BLOCKS; i++)
+							v[u][i] = mine[i][min(t + u, lost_tiles - 1)];
+#pragma unroll
+					for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+						for (int i = 0; i < BLOCKS; i++)
+							taken[i] += t + u < lost_tiles ? v[u][i] : 0.0f;
+				}
+				__syncthreads();
+#pragma unroll
+				for (int u = 0; u < TURNS; u++)
+					*reinterpret_cast<vec_t*>(stage.place + (row0 + u * AT_A_TIME) * TileStage::STRIDE + column) = weights_of[u];
+				__syncthreads();
+				Acc whole[BLOCKS][2];
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++)
+#pragma unroll
+					for (int j = 0; j < 2; j++)
+#pragma unroll
+						for (int q = 0; q < 4; q++)
+						{
+							const typename TileStage::vec4_t weights = *reinterpret_cast<const typename TileStage::vec4_t*>(stage.place + at.row(i) * TileStage::STRIDE + at.column(j) + at.lane_column(q));
+#pragma unroll
+							for (int e = 0; e < 4; e++)
+								whole[i][j][4 * q + e] = fmaf(taken[i], static_cast<float>(weights[e]), acc[i][j][4 * q + e]);
+						}
+				StoreEpilogue<T> { out, columns, beta, back }.template tile<BM, BN>(whole, at, lds, rows);
+			}
+	};
+	/*
+	 * The same where dx comes about in parts or over several pieces of the classes. A wavefront has 256 columns of a row at a time and adds up what the tiles of the row lost by itself; the last 4 columns of a row are moved back to end
 	 * with it, as in RowPlace.
 	 */
 	template<typename T>
@@ -600,10 +687,10 @@ namespace
 			size_t d, dx, parts, sums, lost, factors, scale; /* backward */
 			size_t total;
 	};
-	/* whether dx comes about in fp32 first: several pieces or parts, or something to give back to it */
+	/* whether dx comes about in fp32 first */
 	bool dx_in_parts(const LossShape &s, int piece)
 	{
-		return s.element_size == 2 || piece < s.classes || input_plan(s, piece).parts > 1;
+		return piece < s.classes || input_plan(s, piece).parts > 1;
 	}
 	LossSpace loss_space(const LossShape &s, bool backward)
 	{
@@ -733,7 +820,9 @@ namespace
 				const Operand b { weights, row_bytes, padded, classes };
 				if (in_parts)
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
-				else if constexpr (sizeof(T) == 4)
+				else if constexpr (sizeof(T) == 2)
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, InputEpilogue<T> { dx, s.features, beta_dx, back, lost, lost_tiles, targets, s.classes, w, padded });
+				else
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, StoreEpilogue<T> { dx, s.features, beta_dx, back });
 			}
 			if (dw.data != nullptr)

@@ -141,7 +141,8 @@ def test_dx_of_few_rows_of_the_gated_layer_has_no_rounding_of_d(ctx, rows, featu
 DX_OF_LOSSES = [(*size, sharp, common) for size in [(1, 2048, 3000), (5, 1001, 400), (33, 1003, 777), (64, 333, 2001), (65, 256, 4000), (300, 3, 900), (700, 333, 2001)] for sharp in (False, True) for common in (0, 3, 10)]
 
 
-@pytest.mark.parametrize("rows,features,classes,sharp,common", DX_OF_LOSSES + [(2100, 64, 70003, False, 10)])  # the last one in two pieces
+@pytest.mark.parametrize("rows,features,classes,sharp,common", DX_OF_LOSSES + [(5000, 1100, 300, False, 10), (5000, 1100, 1500, False, 10), (9001, 20, 33, False, 3),
+                                                                             (2100, 64, 70003, False, 10)])  # dx in one go on 256 x 256 and 128 x 128 tiles; in two pieces
 def test_dx_of_the_cross_entropy_has_no_rounding_of_d(ctx, rows, features, classes, sharp, common):
     """For any number of rows and with weights whose rows have a large part in common, which the rounding of d would carry into dx: up to 2e-3 where it is ten times the rest. sharp: probabilities near 1 among the other
     classes, each of which is rounded, so that dx has two roundings after all."""
