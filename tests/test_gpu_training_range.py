@@ -163,3 +163,31 @@ def test_dx_of_the_cross_entropy_has_no_rounding_of_d(ctx, rows, features, class
     assert (R.numbers(dx.copyToHost(ctx))[3::11] == 0).all()
     ml.linearCrossEntropyBackward(ctx, X, W, None, T, lse, DL, 0.5, added, 0.0, None, None, work)
     assert off_in_norm(added.copyToHost(ctx), want + 0.5 * R.numbers(old)) <= (1.2 * np.sqrt(2) * 2.07e-4 if sharp else ONE_ROUNDING)
+
+
+@pytest.mark.parametrize("rows", [9, 90, 9000])
+def test_one_infinite_loss_has_no_say_in_the_others_gradients(ctx, rows):
+    """A row whose dloss is an infinity or no number, beside small ones: dx of the others keeps the bits that it has where that row has no gradient, also beside rows without a class and with NaN in their x."""
+    rng = np.random.default_rng(rows)
+    features, classes = 40, 300
+    x, w = rng.standard_normal((rows, features)), rng.standard_normal((classes, features)) / 4
+    targets, dloss = rng.integers(0, classes, rows).astype(np.int32), (1e-5 * rng.uniform(0.5, 1, rows)).astype(np.float32)
+    targets[5] = -1
+    x, w = R.bits(x, "float16"), R.bits(w, "float16")
+    x[5] = 0x7e00
+    W, T = ml.toDevice(ctx, w), ml.toDevice(ctx, targets)
+    X = ml.toDevice(ctx, x)
+    loss, lse = ml.Tensor((rows,), "float32"), ml.Tensor((rows,), "float32")
+    work = ml.Tensor((ml.linearCrossEntropyGetWorkspaceSize(ctx, X, W, True),), "uint8")
+    work.setall(ctx, 0xff)
+    ml.linearCrossEntropyForward(ctx, X, W, None, T, loss, lse, work)
+    results = []
+    for value in (0.0, np.inf, np.nan):
+        dloss[2] = value
+        dx = ml.Tensor((rows, features), "float16")
+        ml.linearCrossEntropyBackward(ctx, X, W, None, T, lse, ml.toDevice(ctx, dloss), 0.0, dx, 0.0, None, None, work)
+        results.append(R.numbers(dx.copyToHost(ctx)))
+    others = np.arange(rows) != 2
+    assert np.isfinite(results[0]).all() and (results[0][[2, 5]] == 0).all() and (results[0][3] != 0).any()
+    for got in results[1:]:
+        assert np.array_equal(got[others], results[0][others]) and not np.isfinite(got[2]).any()
