@@ -14,7 +14,7 @@
  * d is stored in the tensors' type. In fp16 a probability of one class in 100 000 would be subnormal, so d is scaled by 2^15 / s with s the power of two above the largest |dloss|: of that loss's row probabilities down to
  * 2^-28 keep their 11 bits, of a row whose dloss is 2^-k of it down to 2^(k - 28); what is smaller is off by 2^-39 of the largest |dloss| at most. The products' results are scaled back, exactly, in fp32. What the rounding of
  * d, half a step per element, does to dx is given back (GradientEpilogue); in dW it counts as much as the rounding of dW itself; db is summed before it.
- * fp16: 7 rows of 2048 x 65536 classes 50 us (5.3 TB/s); 4096 rows of 1024 x 50001 427 us (0.98 PFLOP/s), of 2048 x 65536 950 us (1.16); the gradients of the latter 2.98 ms, in two pieces of d 576 us each (0.95 PFLOP/s, a
+ * fp16: 7 rows of 2048 x 65536 classes 50 us (5.3 TB/s); 4096 rows of 1024 x 50001 430 us (0.98 PFLOP/s), of 2048 x 65536 950 us (1.16); the gradients of the latter 2.98 ms, in two pieces of d 576 us each (0.95 PFLOP/s, a
  * fourth of it the epilogue), dx 470 (1.17), dW 462 (1.19), and 30 us to join the parts of dx.
  */
 #include "few_rows.hpp"

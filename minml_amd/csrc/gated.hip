@@ -12,7 +12,7 @@
  * in it, in fp16 scaled where it would leave the type's range (shift_of). Its rounding, half a step per element, adds as much to dx and dW as their own rounding does (2.9e-4 off instead of 2.1e-4; dx of few
  * rows 2.1e-4: keeps_low_part); keeping all of d would double both products. db is summed before the rounding.
  * fp16: 1 row of 4096 -> 8192 23.5 us (5.7 TB/s); 57600 x 256 -> 1024 with gelu, bias and the projections kept 133 us (2.9 TB/s, matrix cores 20 % busy: four chunks of k make a tile mostly beginning and end);
- * backward of 8192 x 2048 -> 5504 727 us (1.02 PFLOP/s): d 79 us (5.8 TB/s), 4 to see that it needs no scale, dx 310 us (1.19 PFLOP/s), dW 340 us.
+ * backward of 8192 x 2048 -> 5504 713 us (1.04 PFLOP/s): d 79 us (5.8 TB/s), 4 to see that it needs no scale, dx 300 us (1.23 PFLOP/s), dW 335 us.
  */
 #include "few_rows.hpp"
 #include "product_tiles.hpp"
