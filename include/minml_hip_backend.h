@@ -274,6 +274,34 @@ extern "C"
 	void hip_linear_cross_entropy_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t targets, const mlTensor_t lse,
 			const mlTensor_t dloss, float beta_dx, mlTensor_t dx, float beta_weights, mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size);
 
+	/*
+	 * What a model over a vocabulary begins with: y[i] = scale * table[tokens[i]], tokens int32 [..], table [classes, features], y [.., features] of the table's type; a token that is none of 0 .. classes - 1 gives zeros.
+	 * Backward: dtable = beta_weights * dtable + scale * (the sum of the rows of dy [.., features] whose token is the class), of dy's type or fp32; rows of dy without a class count for nothing, whatever they hold.
+	 * Everything is aligned to one element. The workspace holds the tokens in order, 16 bytes for each at most, and sums of every 64 of them in fp32.
+	 */
+	void hip_embedding_forward(mlContext_t context, const mlTensor_t tokens, const mlTensor_t table, float scale, mlTensor_t y);
+	size_t hip_embedding_get_workspace_size(mlShape_t tokens_shape, mlShape_t table_shape, mlDataType_t dtype); /* bytes, for the backward pass */
+	void hip_embedding_backward(mlContext_t context, const mlTensor_t tokens, const mlTensor_t dy, float scale, float beta_weights, mlTensor_t dtable, void *workspace, size_t workspace_size);
+
+	/*
+	 * The clipped policy loss over sampled tokens, fp32 [sequences, tokens] (or [tokens] of one sequence): nll, the negative log likelihoods that hip_linear_cross_entropy_forward gives as its loss; old_nll, what they were when
+	 * the tokens were sampled; reference_nll, those of a model to stay close to, or empty; advantages of every sequence or of every token; targets int32 as for the cross entropy: a token whose target is none of
+	 * 0 .. classes - 1 (prompts, padding) has no part in anything, whatever the other tensors hold for it. With r = exp(old_nll - nll) and q = nll - reference_nll a token's loss is
+	 *     -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(q) - q - 1).
+	 * loss fp32 [4]: the mean loss, its two parts -min(..) and exp(q) - q - 1, and the share of tokens that the clip holds. AVERAGE_TOKENS: over all tokens; AVERAGE_SEQUENCES: over the means of the sequences that have tokens.
+	 * Without any token all four are 0. weights fp32 [sequences]: what a token of each sequence counts in the means, for the backward pass.
+	 * Backward: dnll = beta * dnll + the gradient of nll for the loss's gradient dloss (one fp32 number on the device, or empty for 1); it is hip_linear_cross_entropy_backward's dloss.
+	 */
+	typedef enum
+	{
+		AVERAGE_TOKENS, AVERAGE_SEQUENCES
+	} mlAverage_t;
+	size_t hip_policy_loss_get_workspace_size(mlShape_t shape); /* bytes, for the forward pass */
+	void hip_policy_loss_forward(mlContext_t context, const mlTensor_t nll, const mlTensor_t old_nll, const mlTensor_t reference_nll, const mlTensor_t advantages, const mlTensor_t targets, int classes,
+			double clip_low, double clip_high, float kl_weight, mlAverage_t average, mlTensor_t loss, mlTensor_t weights, void *workspace, size_t workspace_size);
+	void hip_policy_loss_backward(mlContext_t context, const mlTensor_t nll, const mlTensor_t old_nll, const mlTensor_t reference_nll, const mlTensor_t advantages, const mlTensor_t targets, int classes,
+			double clip_low, double clip_high, float kl_weight, const mlTensor_t weights, const mlTensor_t dloss, float beta, mlTensor_t dnll);
+
 	/* ---- additions with no counterpart in the reference ABI ----
 	 * hip_quantized_conv_forward: the whole int8 convolution of reference src/layers/Conv2D.cpp:240-308 (int8 implicit GEMM with
 	 * zero-point padding, int32 accumulation, per-channel scale + bias, optional int8 residual, activation, requantisation)

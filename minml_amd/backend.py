@@ -14,6 +14,8 @@ DTYPE_UNKNOWN, DTYPE_FLOAT8, DTYPE_FLOAT16, DTYPE_FLOAT32, DTYPE_FLOAT64, DTYPE_
 ACTIVATION_LINEAR, ACTIVATION_SIGMOID, ACTIVATION_TANH, ACTIVATION_RELU, ACTIVATION_LEAKY_RELU, ACTIVATION_EXP = range(6)
 # mlGate_t
 GATE_SIGMOID, GATE_RELU, GATE_SILU, GATE_GELU = range(4)
+# mlAverage_t
+AVERAGE_TOKENS, AVERAGE_SEQUENCES = range(2)
 
 DTYPE_SIZE = {DTYPE_FLOAT16: 2, DTYPE_FLOAT32: 4, DTYPE_INT8: 1, DTYPE_UINT8: 1, DTYPE_INT16: 2, DTYPE_INT32: 4, DTYPE_FLOAT64: 8}
 
@@ -47,7 +49,7 @@ def make_tensor(ptr, dtype, dims):
     return mlTensor_t(ptr, dtype, len(dims), _dims(dims)) if ptr else mlTensor_t(ptr, dtype, 0)
 
 
-_vp, _sz, _i, _f, _b, _c = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float, ctypes.c_bool, ctypes.c_char
+_vp, _sz, _i, _f, _d, _b, _c = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_bool, ctypes.c_char
 _T, _S, _Q = mlTensor_t, mlShape_t, mlQuantizationData_t
 
 # name -> (restype, argtypes); must list every function declared in include/minml_hip_backend.h
@@ -122,6 +124,12 @@ SIGNATURES = {
     "linear_cross_entropy_get_workspace_size": (_sz, [_S, _S, _i, _b]),
     "linear_cross_entropy_forward": (None, [_vp, _T, _T, _T, _T, _T, _T, _vp, _sz]),
     "linear_cross_entropy_backward": (None, [_vp, _T, _T, _T, _T, _T, _T, _f, _T, _f, _T, _T, _vp, _sz]),
+    "embedding_forward": (None, [_vp, _T, _T, _f, _T]),
+    "embedding_get_workspace_size": (_sz, [_S, _S, _i]),
+    "embedding_backward": (None, [_vp, _T, _T, _f, _f, _T, _vp, _sz]),
+    "policy_loss_get_workspace_size": (_sz, [_S]),
+    "policy_loss_forward": (None, [_vp, _T, _T, _T, _T, _T, _i, _d, _d, _f, _i, _T, _T, _vp, _sz]),
+    "policy_loss_backward": (None, [_vp, _T, _T, _T, _T, _T, _i, _d, _d, _f, _T, _T, _f, _T]),
     "get_stream": (_vp, [_vp]),
     "graph_begin_capture": (None, [_vp]),
     "graph_end_capture": (_vp, [_vp]),

@@ -833,6 +833,74 @@ def linearCrossEntropyBackward(context, input, weights, bias, targets, lse, grad
             beta_weights, _all(gradient_weights), _all(gradient_bias), *_space(workspace))
 
 
+def _require_embedding(tokens, table):
+    _require(tokens.dtype == B.DTYPE_INT32 and len(tokens.shape) >= 1, "tokens must be int32 [..]")
+    _require(table.dtype in _FLOATS and len(table.shape) == 2, "the table must be [classes, features], fp16 or fp32")
+
+
+def embeddingForward(context, tokens, table, scale, output):
+    """output = scale * table[tokens]: tokens int32 [..], table [classes, features], output [.., features]. A token that is no class of the table gives zeros."""
+    _require_embedding(tokens, table)
+    _require(_same_dtype(table, output) and output.volume() == tokens.volume() * table.shape[1] and output.shape[-1] == table.shape[1], "output must be [.., features] of the table's type")
+    _launch("embedding_forward", context.handle, tokens.desc(), table.desc(), scale, output.desc())
+
+
+def embeddingGetWorkspaceSize(context, tokens, table):
+    """Bytes of workspace (aligned to 256) that embeddingBackward needs; `table` may be the table or its gradient."""
+    return B.fn("embedding_get_workspace_size")(tokens.shape_desc(), table.shape_desc(), table.dtype)
+
+
+def embeddingBackward(context, tokens, gradient, scale, beta_weights, gradient_table, workspace):
+    """gradient_table = beta_weights * gradient_table + scale * (the rows of `gradient` [.., features] of every class added up), of the gradient's type or fp32."""
+    _require_embedding(tokens, gradient_table)
+    _require(gradient.dtype in _FLOATS and gradient_table.dtype in (gradient.dtype, B.DTYPE_FLOAT32), "the table's gradient must be of the gradient's type or fp32")
+    _require(gradient.volume() == tokens.volume() * gradient_table.shape[1] and gradient.shape[-1] == gradient_table.shape[1], "the gradient must be [.., features]")
+    _launch("embedding_backward", context.handle, tokens.desc(), gradient.desc(), scale, beta_weights, gradient_table.desc(), *_space(workspace))
+
+
+AVERAGES = {"tokens": B.AVERAGE_TOKENS, "sequences": B.AVERAGE_SEQUENCES}
+
+
+def _require_policy(nll, old_nll, reference_nll, advantages, targets, clip):
+    shape = tuple(nll.shape)
+    _require(len(shape) in (1, 2), "likelihoods must be [sequences, tokens] or [tokens]")
+    sequences = shape[0] if len(shape) == 2 else 1
+    for t in (nll, old_nll, reference_nll):
+        _require(t is None or (t.dtype == B.DTYPE_FLOAT32 and tuple(t.shape) == shape), "likelihoods must be fp32 tensors of one shape")
+    _require(targets.dtype == B.DTYPE_INT32 and tuple(targets.shape) == shape, "one int32 target per token")
+    _require(advantages.dtype == B.DTYPE_FLOAT32 and tuple(advantages.shape) in (shape, (sequences,)), "one fp32 advantage per token or per sequence")
+    _require(len(clip) == 2, "clip must be a pair: how far below 1 and how far above")
+    return sequences
+
+
+def policyLossGetWorkspaceSize(context, nll):
+    """Bytes of workspace (aligned to 256) that policyLossForward needs."""
+    return B.fn("policy_loss_get_workspace_size")(nll.shape_desc())
+
+
+def policyLossForward(context, nll, old_nll, reference_nll, advantages, targets, classes, clip, kl_weight, average, loss, weights, workspace):
+    """loss fp32 [4] = the mean of -min(r A, clip(r, 1 - clip[0], 1 + clip[1]) A) + kl_weight (exp(q) - q - 1) with r = exp(old_nll - nll) and q = nll - reference_nll, its two parts, and the share
+    of clipped tokens. nll (linearCrossEntropyForward's loss) and the others fp32 [sequences, tokens], advantages [sequences, tokens] or [sequences], reference_nll may be None. A token whose target is
+    none of 0 .. classes - 1 has no part in it. average: "tokens" or "sequences" (of the means of the sequences that have tokens). weights fp32 [sequences] are for policyLossBackward."""
+    sequences = _require_policy(nll, old_nll, reference_nll, advantages, targets, clip)
+    _require(average in AVERAGES or average in AVERAGES.values(), "unknown average")
+    _require(loss.dtype == B.DTYPE_FLOAT32 and loss.volume() == 4, "the loss must be fp32 [4]")
+    _require(weights.dtype == B.DTYPE_FLOAT32 and tuple(weights.shape) == (sequences,), "the weights must be fp32 [sequences]")
+    _launch("policy_loss_forward", context.handle, nll.desc(), old_nll.desc(), _all(reference_nll), advantages.desc(), targets.desc(), classes, clip[0], clip[1], kl_weight,
+            AVERAGES.get(average, average), loss.desc(), weights.desc(), *_space(workspace))
+
+
+def policyLossBackward(context, nll, old_nll, reference_nll, advantages, targets, classes, clip, kl_weight, weights, gradient_loss, beta, gradient_nll):
+    """gradient_nll = beta * gradient_nll + the gradient of every token's nll, for the gradient of loss[0] (one fp32 number on the device, None for 1) and the forward pass's weights. It is what
+    linearCrossEntropyBackward takes as gradient_loss."""
+    sequences = _require_policy(nll, old_nll, reference_nll, advantages, targets, clip)
+    _require(weights.dtype == B.DTYPE_FLOAT32 and tuple(weights.shape) == (sequences,), "the weights must be fp32 [sequences]")
+    _require(gradient_loss is None or (gradient_loss.dtype == B.DTYPE_FLOAT32 and gradient_loss.volume() == 1), "the loss's gradient must be one fp32 number")
+    _require(gradient_nll.dtype == B.DTYPE_FLOAT32 and tuple(gradient_nll.shape) == tuple(nll.shape), "the gradient must be fp32 of the likelihoods' shape")
+    _launch("policy_loss_backward", context.handle, nll.desc(), old_nll.desc(), _all(reference_nll), advantages.desc(), targets.desc(), classes, clip[0], clip[1], kl_weight, weights.desc(),
+            _all(gradient_loss), beta, gradient_nll.desc())
+
+
 def foldBatchnorm(context, layer_weights, layer_bias, bn_weights, bn_bias, bn_avg_var):
     """Folds a batch normalisation into the preceding layer's weights and bias, in place (reference: src/core/math.cpp:786-802, which
     also synchronises with the context afterwards)."""

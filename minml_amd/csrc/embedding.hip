@@ -1,0 +1,554 @@
+/*
+ * embedding.hip — rows of a table by token, and the table's gradient.
+ *
+ *   y[i] = scale table[token[i]]                                           a token that is none of the table's: zeros
+ *   dtable[v] = scale sum over i with token[i] = v of dy[i] + beta dtable[v]     in fp32, in the order of i
+ *
+ * Forward: memory bounds it (a row of the table read for every row written, from the caches where tokens repeat).
+ * Backward: tokens are sorted first, stably, so that a class's rows stand in a list in the order they have in dy, and one reader adds them up: no two threads meet at a row of the table, every element of dy is read once and
+ * every row of the table written once, with zeros where there is no token. The same bits on every run.
+ */
+#include "training_utils.hpp"
+
+#include <algorithm>
+#include <tuple>
+#include <utility>
+
+namespace
+{
+	using namespace mlhip;
+
+	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
+	template<typename T, int VEC>
+	__global__ __launch_bounds__(256) void kernel_embedding_forward(const int *tokens, const T *table, T *y, int rows, int columns, int classes, int vectors, float scale)
+	{
+		const size_t count = static_cast<size_t>(rows) * vectors;
+		for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<size_t>(gridDim.x) * 256)
+		{
+			int vector;
+			const size_t row = split_index(i, vectors, vector);
+			const RowPlace place = place_in_row<VEC>(vector * VEC, columns);
+			const int token = tokens[row];
+			float v[VEC];
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				v[e] = 0.0f;
+			if (token >= 0 && token < classes)
+			{
+				Elements<T, VEC> of_table;
+				of_table.load(place.in(table + static_cast<size_t>(token) * columns));
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] = scale * of_table[e];
+			}
+			store_nearest<VEC>(place.in(y + row * columns), v, place.skip);
+		}
+	}
+
+	/* ---- tokens in order ---------------------------------------------------------------------------------------------------- */
+	/*
+	 * A stable sort by digits, lowest first: an element's place is the number of elements with smaller digits and of equal ones before it. A wavefront looks at 64 elements at a time; the lanes with equal digits find one another by
+	 * one ballot per bit. Tokens that are none of the table's are taken for class `classes`, so they end up last.
+	 */
+	__device__ __forceinline__ uint64_t lanes_alike(int digit, int bits, bool there)
+	{
+		uint64_t same = __ballot(there);
+		for (int b = 0; b < bits; b++)
+		{
+			const bool one = (digit >> b) & 1;
+			const uint64_t ones = __ballot(one);
+			same &= one ? ones : ~ones;
+		}
+		return same;
+	}
+	__device__ __forceinline__ int lanes_below(uint64_t mask)
+	{
+		return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+	}
+	/* what the lanes of a wavefront wrote to LDS before is there for all of them behind it: LDS serves a wavefront in order, the compiler has to */
+	__device__ __forceinline__ void wave_in_order()
+	{
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		__builtin_amdgcn_wave_barrier();
+	}
+	__device__ __forceinline__ int key_of(int token, int classes)
+	{
+		return (token >= 0 && token < classes) ? token : classes;
+	}
+	/* sum of the values of the threads before; of a workgroup of 64 WAVES threads. Every thread calls it */
+	template<int WAVES>
+	__device__ __forceinline__ int scan_exclusive(int value, int *waves)
+	{
+		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+		int sum = value;
+#pragma unroll
+		for (int offset = 1; offset < 64; offset <<= 1)
+		{
+			const int below = __shfl_up(sum, offset);
+			sum += lane >= offset ? below : 0;
+		}
+		if (lane == 63)
+			waves[wave] = sum;
+		__syncthreads();
+		int before = sum - value;
+#pragma unroll
+		for (int w = 0; w < WAVES; w++)
+			before += w < wave ? waves[w] : 0;
+		__syncthreads();
+		return before;
+	}
+	/* up to 4096 tokens by one workgroup, in LDS */
+	constexpr int SMALL_SORT = 4096;
+	__global__ __launch_bounds__(1024) void kernel_sort_small(const int *tokens, int count, int classes, int bits, int *keys_out, int *positions_out)
+	{
+		constexpr int WAVES = 16, ROUNDS = SMALL_SORT / 1024, DIGIT = 8, DIGITS = 1 << DIGIT;
+		__shared__ int keys[SMALL_SORT], positions[SMALL_SORT];
+		__shared__ int counters[WAVES][DIGITS];
+		__shared__ int waves[WAVES];
+		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+		int key[ROUNDS], position[ROUNDS], rank[ROUNDS];
+		/* a wavefront has 256 neighbours */
+#pragma unroll
+		for (int u = 0; u < ROUNDS; u++)
+		{
+			position[u] = wave * 64 * ROUNDS + u * 64 + lane;
+			key[u] = position[u] < count ? key_of(tokens[position[u]], classes) : 0x7fffffff;
+		}
+		for (int shift = 0; shift < bits; shift += DIGIT)
+		{
+#pragma unroll
+			for (int u = 0; u < WAVES * DIGITS / 1024; u++)
+				(&counters[0][0])[u * 1024 + threadIdx.x] = 0;
+			__syncthreads();
+#pragma unroll
+			for (int u = 0; u < ROUNDS; u++)
+			{
+				const int digit = (key[u] >> shift) & (DIGITS - 1);
+				const uint64_t same = lanes_alike(digit, DIGIT, true);
+				const int below = lanes_below(same);
+				int *counter = &counters[wave][digit];
+				rank[u] = *counter + below;
+				wave_in_order();
+				if (below == 0)
+					*counter += __popcll(same);
+				wave_in_order();
+			}
+			__syncthreads();
+			int total = 0;
+			if (threadIdx.x < DIGITS)
+				for (int w = 0; w < WAVES; w++)
+					total += counters[w][threadIdx.x];
+			int begin = scan_exclusive<WAVES>(total, waves);
+			if (threadIdx.x < DIGITS)
+				for (int w = 0; w < WAVES; w++)
+				{
+					const int here = counters[w][threadIdx.x];
+					counters[w][threadIdx.x] = begin;
+					begin += here;
+				}
+			__syncthreads();
+#pragma unroll
+			for (int u = 0; u < ROUNDS; u++)
+			{
+				const int place = counters[wave][(key[u] >> shift) & (DIGITS - 1)] + rank[u];
+				keys[place] = key[u];
+				positions[place] = position[u];
+			}
+			__syncthreads();
+#pragma unroll
+			for (int u = 0; u < ROUNDS; u++)
+			{
+				const int from = wave * 64 * ROUNDS + u * 64 + lane;
+				key[u] = keys[from];
+				position[u] = positions[from];
+			}
+			__syncthreads();
+		}
+#pragma unroll
+		for (int u = 0; u < ROUNDS; u++)
+		{
+			const int to = wave * 64 * ROUNDS + u * 64 + lane;
+			if (to < count)
+			{
+				keys_out[to] = key[u];
+				positions_out[to] = position[u];
+			}
+		}
+	}
+	/*
+	 * More of them: a launch that counts the digits of every group's tokens and one that puts them in place, for every digit of up to 11 bits. At most SORT_GROUPS groups, so that each can add up the others' counts by itself.
+	 * `keys` null: the tokens themselves, which stand where they are
+	 */
+	constexpr int SORT_GROUPS = 64;
+	struct SortPass
+	{
+			const int *tokens, *keys, *positions;
+			int *keys_out, *positions_out;
+			int *counts; /* [groups][2^bits] */
+			int count, classes, shift, bits, per_group; /* per_group: a multiple of 256 */
+
+			__device__ __forceinline__ int key(int i) const
+			{
+				return keys != nullptr ? keys[i] : key_of(tokens[i], classes);
+			}
+			__device__ __forceinline__ int digit(int key) const
+			{
+				return (key >> shift) & ((1 << bits) - 1);
+			}
+	};
+	__global__ __launch_bounds__(256) void kernel_sort_count(SortPass p)
+	{
+		extern __shared__ int counters[];
+		const int digits = 1 << p.bits;
+		for (int d = threadIdx.x; d < digits; d += 256)
+			counters[d] = 0;
+		__syncthreads();
+		const int first = blockIdx.x * p.per_group, last = first + min(p.per_group, p.count - first);
+		for (int i = first + threadIdx.x; i < last; i += 256)
+			atomicAdd(&counters[p.digit(p.key(i))], 1);
+		__syncthreads();
+		for (int d = threadIdx.x; d < digits; d += 256)
+			p.counts[static_cast<size_t>(blockIdx.x) * digits + d] = counters[d];
+	}
+	__global__ __launch_bounds__(256) void kernel_sort_place(SortPass p)
+	{
+		extern __shared__ int counters[]; /* [4 wavefronts][digits], then [digits] */
+		__shared__ int waves[4];
+		const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+		int *begin = counters + 4 * digits, *mine = counters + wave * digits;
+		for (int d = threadIdx.x; d < 4 * digits; d += 256)
+			counters[d] = 0;
+		__syncthreads();
+		/* a wavefront has a quarter of the group's tokens, in their order */
+		const int group_first = blockIdx.x * p.per_group, quarter = p.per_group / 4;
+		const int left = p.count - group_first - wave * quarter, here = max(0, min(quarter, left)), first = group_first + wave * quarter;
+		for (int i = lane; i < here; i += 64)
+			atomicAdd(&mine[p.digit(p.key(first + i))], 1);
+		/* of every digit: the tokens of all groups, and those of the groups before */
+		const int each = max(1, digits / 256); /* neighbouring digits of a thread */
+		int sum = 0;
+		for (int u = 0; u < each; u++)
+		{
+			const int d = threadIdx.x * each + u;
+			int before = 0, total = 0;
+			if (d < digits)
+			{
+				for (int g = 0; g < static_cast<int>(gridDim.x); g++)
+				{
+					const int c = p.counts[static_cast<size_t>(g) * digits + d];
+					before += g < static_cast<int>(blockIdx.x) ? c : 0;
+					total += c;
+				}
+				begin[d] = sum + before;
+			}
+			sum += total;
+		}
+		const int smaller = scan_exclusive<4>(sum, waves); /* its barriers stand behind the counts of the wavefronts, too */
+		for (int u = 0; u < each; u++)
+		{
+			const int d = threadIdx.x * each + u;
+			if (d < digits)
+			{
+				int at = begin[d] + smaller;
+#pragma unroll
+				for (int w = 0; w < 4; w++)
+				{
+					const int n = counters[w * digits + d];
+					counters[w * digits + d] = at;
+					at += n;
+				}
+			}
+		}
+		__syncthreads();
+		for (int i = 0; i < here; i += 64)
+		{
+			const bool there = i + lane < here;
+			const int from = first + min(i + lane, here - 1);
+			const int key = p.key(from), position = p.keys != nullptr ? p.positions[from] : from;
+			const int digit = p.digit(key);
+			const uint64_t same = lanes_alike(digit, p.bits, there);
+			const int below = lanes_below(same);
+			const int place = mine[digit] + below;
+			wave_in_order();
+			if (there && below == 0)
+				mine[digit] += __popcll(same);
+			wave_in_order();
+			if (there)
+			{
+				p.keys_out[place] = key;
+				p.positions_out[place] = position;
+			}
+		}
+	}
+
+	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
+	template<typename T, typename Out>
+	struct TableGradient
+	{
+			const int *keys, *positions; /* in order */
+			const T *dy;
+			Out *out;
+			int count, classes, columns, classes_of_group, lanes; /* lanes: threads of a row, a power of two */
+			float scale, beta;
+	};
+	/* the first place whose key is not below `key` */
+	__device__ __forceinline__ int lower_bound(const int *keys, int count, int key)
+	{
+		int first = 0, length = count;
+		while (length > 0)
+		{
+			const int half = length / 2;
+			const bool below = keys[first + half] < key;
+			first = below ? first + half + 1 : first;
+			length = below ? length - half - 1 : half;
+		}
+		return first;
+	}
+	constexpr int MOST_CLASSES_OF_GROUP = 32;
+	template<typename T, typename Out, int VEC>
+	__global__ __launch_bounds__(256) void kernel_table_gradient(TableGradient<T, Out> p)
+	{
+		__shared__ int bounds[MOST_CLASSES_OF_GROUP + 1];
+		const int first_class = blockIdx.x * p.classes_of_group, classes = min(p.classes_of_group, p.classes - first_class);
+		for (int i = threadIdx.x; i <= classes; i += 256)
+			bounds[i] = lower_bound(p.keys, p.count, first_class + i);
+		__syncthreads();
+		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC;
+		if (column >= p.columns)
+			return;
+		const RowPlace place = place_in_row<VEC>(column, p.columns);
+		for (int c = threadIdx.x / p.lanes; c < classes; c += 256 / p.lanes)
+		{
+			const int begin = bounds[c], end = bounds[c + 1];
+			Out *dst = place.in(p.out + static_cast<size_t>(first_class + c) * p.columns);
+			float v[VEC];
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				v[e] = 0.0f;
+			for (int i = begin; i < end; i++)
+			{
+				Elements<T, VEC> x;
+				x.load(place.in(p.dy + static_cast<size_t>(p.positions[i]) * p.columns));
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] += x[e];
+			}
+			Elements<Out, VEC> old;
+			if (p.beta != 0.0f)
+				old.load(dst);
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				v[e] = p.beta != 0.0f ? fmaf(p.beta, old[e], p.scale * v[e]) : p.scale * v[e];
+			store_nearest<VEC>(dst, v, place.skip);
+		}
+	}
+
+	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
+	struct EmbeddingShape
+	{
+			int rows, classes, columns;
+	};
+	EmbeddingShape embedding_shape(const mlShape_t &tokens, const mlShape_t &table, mlDataType_t dtype, const char *name)
+	{
+		const std::string who(name);
+		MLHIP_REQUIRE(dtype == DTYPE_FLOAT16 || dtype == DTYPE_FLOAT32, who + ": unsupported data type");
+		MLHIP_REQUIRE(tokens.rank >= 1 && tokens.rank <= 6 && table.rank == 2, who + ": tokens need one to six dimensions, the table must be [classes, features]");
+		for (int i = 0; i < tokens.rank; i++)
+			MLHIP_REQUIRE(tokens.dim[i] >= 0, who + ": negative dimension");
+		MLHIP_REQUIRE(table.dim[0] > 0 && table.dim[1] > 0, who + ": there must be classes and features");
+		const size_t rows = volume(tokens);
+		MLHIP_REQUIRE(rows <= (1 << 28) && table.dim[0] <= (1 << 28) && table.dim[1] <= (1 << 18), who + ": too many tokens, classes or features");
+		return EmbeddingShape { static_cast<int>(rows), table.dim[0], table.dim[1] };
+	}
+	struct SortPlan
+	{
+			int bits, passes, digit_bits, groups, per_group;
+	};
+	SortPlan sort_plan(const EmbeddingShape &s)
+	{
+		SortPlan plan { };
+		while ((s.classes >> plan.bits) > 0)
+			plan.bits++;
+		plan.passes = ceil_div(plan.bits, 11);
+		plan.digit_bits = ceil_div(plan.bits, plan.passes);
+		plan.per_group = std::max(1024, static_cast<int>(round_up(ceil_div(s.rows, SORT_GROUPS), 256)));
+		plan.groups = ceil_div(s.rows, plan.per_group);
+		return plan;
+	}
+	struct EmbeddingSpace
+	{
+			size_t keys[2], positions[2], counts, total;
+	};
+	EmbeddingSpace embedding_space(const EmbeddingShape &s)
+	{
+		EmbeddingSpace space { };
+		size_t at = 0;
+		const auto take = [&](size_t bytes)
+		{
+			const size_t begin = at;
+			at += round_up(bytes, 256);
+			return begin;
+		};
+		if (s.rows > 0)
+		{
+			const SortPlan plan = sort_plan(s);
+			const bool small = s.rows <= SMALL_SORT;
+			for (int i = 0; i < (small || plan.passes == 1 ? 1 : 2); i++)
+			{
+				space.keys[i] = take(sizeof(int) * s.rows);
+				space.positions[i] = take(sizeof(int) * s.rows);
+			}
+			space.counts = take(small ? 0 : (sizeof(int) * plan.groups << plan.digit_bits));
+		}
+		space.total = at;
+		return space;
+	}
+
+	template<typename T, int VEC>
+	void embedding_forward(hipStream_t stream, const EmbeddingShape &s, const int *tokens, const T *table, T *y, float scale)
+	{
+		const int vectors = ceil_div(s.columns, VEC);
+		const size_t groups = std::min<size_t>((static_cast<size_t>(s.rows) * vectors + 255) / 256, 1 << 20);
+		hipLaunchKernelGGL((kernel_embedding_forward<T, VEC>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, tokens, table, y, s.rows, s.columns, s.classes, vectors, scale);
+		MLHIP_CHECK(hipGetLastError());
+	}
+	/* the tokens in order: keys and positions */
+	std::pair<const int*, const int*> sort_tokens(hipStream_t stream, const EmbeddingShape &s, const int *tokens, uint8_t *workspace)
+	{
+		const EmbeddingSpace space = embedding_space(s);
+		const SortPlan plan = sort_plan(s);
+		const auto keys = [&](int i)
+		{
+			return reinterpret_cast<int*>(workspace + space.keys[i]);
+		};
+		const auto positions = [&](int i)
+		{
+			return reinterpret_cast<int*>(workspace + space.positions[i]);
+		};
+		if (s.rows <= SMALL_SORT)
+		{
+			hipLaunchKernelGGL(kernel_sort_small, dim3(1), dim3(1024), 0, stream, tokens, s.rows, s.classes, plan.bits, keys(0), positions(0));
+			MLHIP_CHECK(hipGetLastError());
+			return { keys(0), positions(0) };
+		}
+		for (int pass = 0; pass < plan.passes; pass++)
+		{
+			const int from = (pass + 1) & 1, to = pass & 1;
+			const SortPass p { tokens, pass == 0 ? nullptr : keys(from), pass == 0 ? nullptr : positions(from), keys(to), positions(to), reinterpret_cast<int*>(workspace + space.counts), s.rows, s.classes,
+					pass * plan.digit_bits, plan.digit_bits, plan.per_group };
+			const int bytes = static_cast<int>(sizeof(int)) << plan.digit_bits;
+			hipLaunchKernelGGL(kernel_sort_count, dim3(plan.groups), dim3(256), bytes, stream, p);
+			hipLaunchKernelGGL(kernel_sort_place, dim3(plan.groups), dim3(256), 5 * bytes, stream, p);
+			MLHIP_CHECK(hipGetLastError());
+		}
+		const int last = (plan.passes - 1) & 1;
+		return { keys(last), positions(last) };
+	}
+	template<typename T, typename Out, int VEC>
+	void table_gradient(hipStream_t stream, const EmbeddingShape &s, const int *keys, const int *positions, const T *dy, float scale, float beta, Out *out)
+	{
+		int lanes = 1;
+		while (lanes < 256 && lanes * VEC < s.columns)
+			lanes *= 2;
+		const int spans = ceil_div(s.columns, lanes * VEC);
+		const size_t units = static_cast<size_t>(s.classes) * spans;
+		const int most = static_cast<int>(std::min<size_t>(MOST_CLASSES_OF_GROUP, std::max<size_t>(1, units / 2048)));
+		const TableGradient<T, Out> p { keys, positions, dy, out, s.rows, s.classes, s.columns, most, lanes, scale, beta };
+		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3(ceil_div(s.classes, most), spans), dim3(256), 0, stream, p);
+		MLHIP_CHECK(hipGetLastError());
+	}
+	template<typename T, typename Out>
+	void embedding_backward(hipStream_t stream, const EmbeddingShape &s, const int *tokens, const T *dy, float scale, float beta, Out *out, uint8_t *workspace)
+	{
+		constexpr int VEC = 16 / sizeof(T);
+		const int *keys = nullptr, *positions = nullptr;
+		if (s.rows > 0)
+			std::tie(keys, positions) = sort_tokens(stream, s, tokens, workspace);
+		if (s.columns >= VEC)
+			table_gradient<T, Out, VEC>(stream, s, keys, positions, dy, scale, beta, out);
+		else
+			table_gradient<T, Out, 1>(stream, s, keys, positions, dy, scale, beta, out);
+	}
+	void check_tokens(const mlTensor_t &tokens, const EmbeddingShape &s, const char *name)
+	{
+		MLHIP_REQUIRE(tokens.dtype == DTYPE_INT32, std::string(name) + ": tokens must be int32");
+		MLHIP_REQUIRE(s.rows == 0 || (tokens.data != nullptr && reinterpret_cast<uintptr_t>(tokens.data) % 4 == 0), std::string(name) + ": null or misaligned tokens");
+	}
+	/* one row of features for every token */
+	bool rows_of(const mlTensor_t &t, const EmbeddingShape &s)
+	{
+		return t.rank >= 1 && last_dim(t) == s.columns && volume(t) == static_cast<size_t>(s.rows) * s.columns && (s.rows == 0 || t.data != nullptr);
+	}
+}
+
+extern "C"
+{
+	using namespace mlhip;
+
+	void hip_embedding_forward(mlContext_t context, const mlTensor_t tokens, const mlTensor_t table, float scale, mlTensor_t y)
+	try
+	{
+		const char *name = "embedding_forward";
+		const EmbeddingShape s = embedding_shape(shape_of(tokens), shape_of(table), table.dtype, name);
+		check_tokens(tokens, s, name);
+		MLHIP_REQUIRE(y.dtype == table.dtype && rows_of(y, s), "embedding_forward: the result must hold a row of the table's type and width for every token");
+		if (s.rows == 0)
+			return;
+		MLHIP_REQUIRE(table.data != nullptr, "embedding_forward: null table");
+		require_apart( { y }, { tokens, table }, name);
+		const OnDeviceOf on(context);
+		if (table.dtype == DTYPE_FLOAT16)
+		{
+			if (s.columns >= 8)
+				embedding_forward<half_t, 8>(on.stream, s, ptr<int>(tokens), ptr<half_t>(table), ptr<half_t>(y), scale);
+			else
+				embedding_forward<half_t, 1>(on.stream, s, ptr<int>(tokens), ptr<half_t>(table), ptr<half_t>(y), scale);
+		}
+		else if (s.columns >= 4)
+			embedding_forward<float, 4>(on.stream, s, ptr<int>(tokens), ptr<float>(table), ptr<float>(y), scale);
+		else
+			embedding_forward<float, 1>(on.stream, s, ptr<int>(tokens), ptr<float>(table), ptr<float>(y), scale);
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+
+	size_t hip_embedding_get_workspace_size(mlShape_t tokens_shape, mlShape_t table_shape, mlDataType_t dtype)
+	try
+	{
+		return embedding_space(embedding_shape(tokens_shape, table_shape, dtype, "embedding_get_workspace_size")).total;
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<size_t>();
+	}
+
+	void hip_embedding_backward(mlContext_t context, const mlTensor_t tokens, const mlTensor_t dy, float scale, float beta_weights, mlTensor_t dtable, void *workspace, size_t workspace_size)
+	try
+	{
+		const char *name = "embedding_backward";
+		if (dtable.data == nullptr)
+			return;
+		const EmbeddingShape s = embedding_shape(shape_of(tokens), shape_of(dtable), dy.dtype, name);
+		check_tokens(tokens, s, name);
+		MLHIP_REQUIRE(rows_of(dy, s), "embedding_backward: there must be a gradient of the table's width for every token");
+		MLHIP_REQUIRE(dtable.dtype == dy.dtype || dtable.dtype == DTYPE_FLOAT32, "embedding_backward: the table's gradient must be of the gradients' type or fp32");
+		const EmbeddingSpace space = embedding_space(s);
+		MLHIP_REQUIRE(space.total == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_size >= space.total),
+				"embedding_backward: the workspace is too small or not aligned to 256 bytes");
+		require_apart( { dtable, Extent(workspace, workspace_size) }, { tokens, dy }, name);
+		const OnDeviceOf on(context);
+		uint8_t *memory = reinterpret_cast<uint8_t*>(workspace);
+		if (dy.dtype == DTYPE_FLOAT32)
+			embedding_backward<float, float>(on.stream, s, ptr<int>(tokens), ptr<float>(dy), scale, beta_weights, ptr<float>(dtable), memory);
+		else if (dtable.dtype == DTYPE_FLOAT32)
+			embedding_backward<half_t, float>(on.stream, s, ptr<int>(tokens), ptr<half_t>(dy), scale, beta_weights, ptr<float>(dtable), memory);
+		else
+			embedding_backward<half_t, half_t>(on.stream, s, ptr<int>(tokens), ptr<half_t>(dy), scale, beta_weights, ptr<half_t>(dtable), memory);
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+}

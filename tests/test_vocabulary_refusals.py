@@ -1,0 +1,156 @@
+"""No-GPU checks of the embedding and the policy loss: what the library and the mirror refuse, before anything reaches a device."""
+import pytest
+
+from minml_amd import backend as B
+from minml_amd import core as ml
+from test_training_refusals import NULL, fake, refused
+
+
+class Ctx:
+    handle = None
+
+
+def test_embedding_refusals_of_the_library():
+    t, w, y = fake((4,), "int32").desc(), fake((90, 16)).desc(), fake((4, 16)).desc()
+    forward = lambda t=t, w=w, y=y, why=None: refused("embedding_forward", t, w, 2.0, y, why=why)
+    forward(t=fake((4,), "float32").desc(), why="int32")
+    forward(t=NULL)
+    forward(t=ml.Tensor((4,), "int32", _ptr=0x7002).desc(), why="misaligned")
+    forward(w=fake((90, 16), "int8").desc(), why="data type")
+    forward(w=fake((2, 90, 16)).desc())
+    forward(w=fake((0, 16)).desc())
+    forward(y=fake((4, 15)).desc())
+    forward(y=fake((3, 16)).desc())
+    forward(y=fake((16, 4)).desc())
+    forward(y=fake((4, 16), "float32").desc())
+    forward(y=fake((90, 16)).view((4, 16), 16).desc(), w=w, why="null context")
+    whole = fake((90, 16))
+    forward(w=whole.desc(), y=whole.view((4, 16), 160).desc(), why="overlap")
+    forward(why="null context")
+    size = B.fn("embedding_get_workspace_size")(fake((5000,), "int32").shape_desc(), fake((90, 16)).shape_desc(), B.DTYPE_FLOAT16)
+    assert size >= 5000 * 8
+    t, dy = fake((5000,), "int32").desc(), fake((5000, 16)).desc()
+    backward = lambda t=t, dy=dy, dw=w, space=0x7000, n=size, why=None: refused("embedding_backward", t, dy, 1.0, 0.0, dw, space, n, why=why)
+    backward(t=fake((4999,), "int32").desc())
+    backward(dy=fake((5000, 8)).desc())
+    backward(dy=fake((5000, 16), "int8").desc())
+    backward(dw=fake((90, 17)).desc())
+    backward(dw=fake((90,)).desc())
+    backward(dw=fake((90, 16), "int32").desc())
+    backward(dy=fake((5000, 16), "float32").desc())  # fp16 sums of fp32 rows
+    backward(n=size - 1, why="workspace")
+    backward(space=None, why="workspace")
+    backward(space=0x7010, why="workspace")
+    backward(dw=ml.Tensor((90, 16), "float16", _ptr=0x7000).desc(), why="overlap")
+    rows = fake((5000, 16))
+    backward(dy=rows.desc(), dw=rows.view((90, 16), 64).desc(), why="overlap")
+    backward(why="null context")
+    B.fn("embedding_backward")(None, t, dy, 1.0, 0.0, NULL, None, 0)  # nothing asked for
+
+
+def test_embedding_refuses_what_its_counters_do_not_reach():
+    shape = lambda *dims: B.make_shape(dims)
+    for tokens, table in (((2 ** 28 + 1,), (8, 8)), ((8,), (2 ** 28 + 1, 8)), ((8,), (8, 2 ** 18 + 1))):
+        with pytest.raises(ValueError, match="too many"):
+            B.fn("embedding_get_workspace_size")(shape(*tokens), shape(*table), B.DTYPE_FLOAT32)
+    for dtype in (B.DTYPE_INT8, B.DTYPE_INT32):
+        with pytest.raises(ValueError):
+            B.fn("embedding_get_workspace_size")(shape(8), shape(8, 8), dtype)
+
+
+def test_embedding_refusals_of_the_mirror():
+    t, w, y = fake((2, 3), "int32"), fake((90, 16)), fake((2, 3, 16))
+    space = ml.Tensor((1 << 22,), "uint8", _ptr=1 << 50)
+    for call in (lambda: ml.embeddingForward(Ctx, fake((2, 3)), w, 1.0, y), lambda: ml.embeddingForward(Ctx, t, w, 1.0, fake((2, 16))), lambda: ml.embeddingForward(Ctx, t, w, 1.0, fake((2, 3, 16), "float32")),
+                 lambda: ml.embeddingForward(Ctx, t, fake((16,)), 1.0, y), lambda: ml.embeddingBackward(Ctx, t, fake((2, 3, 8)), 1.0, 0.0, w, space),
+                 lambda: ml.embeddingBackward(Ctx, t, fake((2, 3, 16), "float32"), 1.0, 0.0, w, space), lambda: ml.embeddingBackward(Ctx, t, y, 1.0, 0.0, w, None)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ml.embeddingForward(Ctx, t, w, 1.0, y), lambda: ml.embeddingBackward(Ctx, t, y, 1.0, 0.0, w, space),
+                 lambda: ml.embeddingForward(Ctx, fake((1,), "int32"), w, 1.0, fake((16,))), lambda: ml.embeddingBackward(Ctx, t, y, 1.0, 0.0, fake((90, 16), "float32"), space)):
+        with pytest.raises(ValueError, match="null context"):
+            call()
+
+
+def policy_tensors(sequences=3, length=7):
+    return [fake((sequences, length), "float32") for _ in range(3)] + [fake((sequences,), "float32"), fake((sequences, length), "int32")]
+
+
+def test_policy_loss_refusals_of_the_library():
+    names = ("nll", "old", "reference", "advantages", "targets")
+    given = dict(zip(names, (t.desc() for t in policy_tensors())))
+    loss, weights = fake((4,), "float32").desc(), fake((3,), "float32").desc()
+    need = B.fn("policy_loss_get_workspace_size")(B.make_shape((3, 7)))
+
+    def forward(clip=(0.2, 0.2), kl=0.1, average=0, loss=loss, weights=weights, space=0x7000, n=need, why=None, **other):
+        refused("policy_loss_forward", *dict(given, **other).values(), 100, *clip, kl, average, loss, weights, space, n, why=why)
+
+    def backward(clip=(0.2, 0.2), kl=0.1, weights=weights, dloss=NULL, dnll=fake((3, 7), "float32").desc(), why=None, **other):
+        refused("policy_loss_backward", *dict(given, **other).values(), 100, *clip, kl, weights, dloss, 0.0, dnll, why=why)
+
+    for call in (forward, backward):
+        call(why="null context")
+        call(reference=NULL, why="null context")
+        call(advantages=fake((3, 7), "float32").desc(), why="null context")
+        call(clip=(1.5, float("inf")), why="null context")
+        for name in names:
+            call(**{name: fake((3, 6), "float32").desc()})
+            call(**{name: fake((3, 7), "float16").desc()})
+        for name in ("nll", "old", "advantages", "targets"):
+            call(**{name: NULL})
+        call(nll=ml.Tensor((3, 7), "float32", _ptr=0x7002).desc())
+        call(nll=fake((1, 3, 7), "float32").desc(), why=r"\[sequences, tokens\]")
+        call(advantages=fake((7,), "float32").desc(), why="advantage")
+        call(clip=(-0.1, 0.2), why="clip")
+        call(clip=(0.2, float("nan")), why="clip")
+        call(kl=float("inf"), why="weight must be finite")
+        call(weights=fake((4,), "float32").desc())
+        call(weights=fake((3,), "float16").desc())
+    forward(average=2, why="average")
+    forward(average=-1, why="average")
+    forward(loss=fake((1,), "float32").desc())
+    forward(loss=NULL)
+    forward(loss=fake((4,)).desc())
+    forward(weights=NULL)
+    forward(space=None, why="workspace")
+    forward(space=0x7010, why="workspace")
+    forward(n=need - 1, why="workspace")
+    forward(loss=weights, weights=weights, why="4")
+    forward(weights=given["advantages"], why="overlap")
+    forward(loss=ml.Tensor((4,), "float32", _ptr=0x7000).desc(), why="overlap")
+    backward(dnll=fake((3, 8), "float32").desc())
+    backward(dnll=NULL)
+    backward(dnll=given["nll"], why="overlap")
+    backward(dloss=fake((2,), "float32").desc(), why="single")
+    backward(dloss=fake((1,)).desc(), why="single")
+    with pytest.raises(ValueError, match="too many"):
+        B.fn("policy_loss_get_workspace_size")(B.make_shape((1, 2 ** 28 + 1)))
+
+
+def test_policy_loss_workspace_does_not_grow_with_the_tokens():
+    for sequences, length in ((1, 2 ** 27), (500, 2 ** 20), (2 ** 20, 10), (4096, 4096)):
+        assert B.fn("policy_loss_get_workspace_size")(B.make_shape((sequences, length))) <= 32 * 1024 + 256 + 4 * sequences
+
+
+def test_policy_loss_refusals_of_the_mirror():
+    tensors = policy_tensors()
+    loss, weights, dnll = fake((4,), "float32"), fake((3,), "float32"), fake((3, 7), "float32")
+    space = ml.Tensor((1 << 20,), "uint8", _ptr=1 << 50)
+
+    def forward(clip=(0.2, 0.2), average="tokens", loss=loss, weights=weights, **other):
+        ml.policyLossForward(Ctx, *(other.get(str(i), t) for i, t in enumerate(tensors)), 100, clip, 0.1, average, loss, weights, space)
+
+    def backward(clip=(0.2, 0.2), weights=weights, dloss=None, dnll=dnll, **other):
+        ml.policyLossBackward(Ctx, *(other.get(str(i), t) for i, t in enumerate(tensors)), 100, clip, 0.1, weights, dloss, 0.0, dnll)
+
+    bad = [lambda: forward(average="words"), lambda: forward(loss=weights), lambda: forward(weights=loss), lambda: backward(weights=loss), lambda: backward(dloss=fake((2,), "float32")),
+           lambda: backward(dnll=fake((7, 3), "float32"))]
+    for call in (forward, backward):
+        bad += [lambda call=call, i=i: call(**{str(i): fake((3, 5), "float32")}) for i in range(5)] + [lambda call=call: call(clip=(0.2,))]
+    for call in bad:
+        with pytest.raises(ValueError) as failure:
+            call()
+        assert "null context" not in str(failure.value)
+    for call in (forward, backward, lambda: forward(**{"2": None}), lambda: backward(**{"2": None}, dloss=fake((1,), "float32"))):
+        with pytest.raises(ValueError, match="null context"):
+            call()
