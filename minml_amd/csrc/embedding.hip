@@ -282,11 +282,18 @@ namespace
 	}
 
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
+	/*
+	 * A class's rows are added up by those who write its row of the table; but where one class has many (a few tokens are in every line), they would wait for it alone. The list is therefore cut into chunks of 64 places, and of
+	 * a class of 64 and more rows every chunk that it has from its first place on is added up beforehand, by a launch of its own, so that what is left is at most 63 rows before its first whole chunk and a sum in fp32 for every
+	 * 64 further ones. Neither asks more than the list to know who does what.
+	 */
+	constexpr int CHUNK = 64;
 	template<typename T, typename Out>
 	struct TableGradient
 	{
 			const int *keys, *positions; /* in order */
 			const T *dy;
+			float *partial; /* [chunks][columns] */
 			Out *out;
 			int count, classes, columns, classes_of_group, lanes; /* lanes: threads of a row, a power of two */
 			float scale, beta;
@@ -304,35 +311,97 @@ namespace
 		}
 		return first;
 	}
+	/* v += the rows of every `step`th place from `first` on, AHEAD of them on their way at a time. row(i): where the i-th lies */
+	template<typename T, int VEC, typename Row>
+	__device__ __forceinline__ void add_rows(float (&v)[VEC], int first, int last, int step, Row &&row)
+	{
+		constexpr int AHEAD = 8;
+		for (int i = first; i < last; i += AHEAD * step)
+		{
+			Elements<T, VEC> x[AHEAD];
+#pragma unroll
+			for (int u = 0; u < AHEAD; u++)
+				x[u].load(row(min(i + u * step, last - 1)));
+#pragma unroll
+			for (int u = 0; u < AHEAD; u++)
+				if (i + u * step < last)
+#pragma unroll
+					for (int e = 0; e < VEC; e++)
+						v[e] += x[u][e];
+		}
+	}
+	/* the sums of a workgroup's 256 / lanes groups of threads in the first of them, in order. Every thread calls it */
+	template<int VEC>
+	__device__ __forceinline__ void join_groups(float (&v)[VEC], int lanes, float (*meeting)[VEC])
+	{
+		if (lanes == 256)
+			return;
+		__syncthreads();
+#pragma unroll
+		for (int e = 0; e < VEC; e++)
+			meeting[threadIdx.x][e] = v[e];
+		__syncthreads();
+		if (static_cast<int>(threadIdx.x) < lanes)
+			for (int t = threadIdx.x + lanes; t < 256; t += lanes)
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] += meeting[t][e];
+	}
+	template<typename T, typename Out, int VEC>
+	__global__ __launch_bounds__(256) void kernel_chunk_sums(TableGradient<T, Out> p)
+	{
+		__shared__ float meeting[256][VEC];
+		__shared__ int rows[CHUNK];
+		const int first = blockIdx.x * CHUNK, lane = threadIdx.x & 63;
+		const int key = p.keys[first];
+		if (key >= p.classes)
+			return;
+		/* 64 places of one class with the chunk's first one among them; and where the class ends in the chunk */
+		const int from = first - lane, to = from + CHUNK - 1;
+		const bool all = from >= 0 && to < p.count && p.keys[max(from, 0)] == key && p.keys[min(to, p.count - 1)] == key;
+		if (__ballot(all) == 0)
+			return;
+		const bool mine = first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
+		const int here = __popcll(__ballot(mine));
+		if (threadIdx.x < CHUNK)
+			rows[threadIdx.x] = p.positions[min(first + lane, p.count - 1)];
+		__syncthreads();
+		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC;
+		const RowPlace place = place_in_row<VEC>(min(column, p.columns - 1), p.columns);
+		float v[VEC];
+#pragma unroll
+		for (int e = 0; e < VEC; e++)
+			v[e] = 0.0f;
+		add_rows<T, VEC>(v, threadIdx.x / p.lanes, here, 256 / p.lanes, [&](int i) __attribute__((always_inline))
+		{
+			return place.in(p.dy + static_cast<size_t>(rows[i]) * p.columns);
+		});
+		join_groups<VEC>(v, p.lanes, meeting);
+		if (static_cast<int>(threadIdx.x) < p.lanes && column < p.columns)
+			store_nearest<VEC>(place.in(p.partial + static_cast<size_t>(blockIdx.x) * p.columns), v, place.skip);
+	}
 	constexpr int MOST_CLASSES_OF_GROUP = 32;
+	/* a class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's */
+	constexpr int ROWS_OF_ALL = 16;
 	template<typename T, typename Out, int VEC>
 	__global__ __launch_bounds__(256) void kernel_table_gradient(TableGradient<T, Out> p)
 	{
 		__shared__ int bounds[MOST_CLASSES_OF_GROUP + 1];
+		__shared__ float meeting[256][VEC];
 		const int first_class = blockIdx.x * p.classes_of_group, classes = min(p.classes_of_group, p.classes - first_class);
 		for (int i = threadIdx.x; i <= classes; i += 256)
 			bounds[i] = lower_bound(p.keys, p.count, first_class + i);
 		__syncthreads();
-		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC;
-		if (column >= p.columns)
-			return;
-		const RowPlace place = place_in_row<VEC>(column, p.columns);
-		for (int c = threadIdx.x / p.lanes; c < classes; c += 256 / p.lanes)
+		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC, groups = 256 / p.lanes, group = threadIdx.x / p.lanes;
+		const bool inside = column < p.columns;
+		const RowPlace place = place_in_row<VEC>(min(column, p.columns - 1), p.columns);
+		const auto row_of_list = [&](int i) __attribute__((always_inline))
 		{
-			const int begin = bounds[c], end = bounds[c + 1];
+			return place.in(p.dy + static_cast<size_t>(p.positions[i]) * p.columns);
+		};
+		const auto write = [&](int c, float (&v)[VEC]) __attribute__((always_inline))
+		{
 			Out *dst = place.in(p.out + static_cast<size_t>(first_class + c) * p.columns);
-			float v[VEC];
-#pragma unroll
-			for (int e = 0; e < VEC; e++)
-				v[e] = 0.0f;
-			for (int i = begin; i < end; i++)
-			{
-				Elements<T, VEC> x;
-				x.load(place.in(p.dy + static_cast<size_t>(p.positions[i]) * p.columns));
-#pragma unroll
-				for (int e = 0; e < VEC; e++)
-					v[e] += x[e];
-			}
 			Elements<Out, VEC> old;
 			if (p.beta != 0.0f)
 				old.load(dst);
@@ -340,6 +409,39 @@ namespace
 			for (int e = 0; e < VEC; e++)
 				v[e] = p.beta != 0.0f ? fmaf(p.beta, old[e], p.scale * v[e]) : p.scale * v[e];
 			store_nearest<VEC>(dst, v, place.skip);
+		};
+		if (inside)
+			for (int c = group; c < classes; c += groups)
+			{
+				const int begin = bounds[c], end = bounds[c + 1];
+				if ((groups > 1 && end - begin >= ROWS_OF_ALL) || end - begin >= CHUNK)
+					continue;
+				float v[VEC];
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] = 0.0f;
+				add_rows<T, VEC>(v, begin, end, 1, row_of_list);
+				write(c, v);
+			}
+		for (int c = 0; c < classes; c++)
+		{
+			const int begin = bounds[c], end = bounds[c + 1];
+			if (!((groups > 1 && end - begin >= ROWS_OF_ALL) || end - begin >= CHUNK))
+				continue;
+			const int chunk = (begin + CHUNK - 1) / CHUNK, direct = end - begin < CHUNK ? end : min(end, chunk * CHUNK);
+			float v[VEC];
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				v[e] = 0.0f;
+			add_rows<T, VEC>(v, begin + group, direct, groups, row_of_list);
+			if (direct < end)
+				add_rows<float, VEC>(v, chunk + group, (end + CHUNK - 1) / CHUNK, groups, [&](int i) __attribute__((always_inline))
+				{
+					return place.in(static_cast<const float*>(p.partial) + static_cast<size_t>(i) * p.columns);
+				});
+			join_groups<VEC>(v, p.lanes, meeting);
+			if (group == 0 && inside)
+				write(c, v);
 		}
 	}
 
@@ -377,7 +479,7 @@ namespace
 	}
 	struct EmbeddingSpace
 	{
-			size_t keys[2], positions[2], counts, total;
+			size_t keys[2], positions[2], counts, partial, total;
 	};
 	EmbeddingSpace embedding_space(const EmbeddingShape &s)
 	{
@@ -399,6 +501,7 @@ namespace
 				space.positions[i] = take(sizeof(int) * s.rows);
 			}
 			space.counts = take(small ? 0 : (sizeof(int) * plan.groups << plan.digit_bits));
+			space.partial = take(s.rows >= CHUNK ? sizeof(float) * ceil_div(s.rows, CHUNK) * s.columns : 0);
 		}
 		space.total = at;
 		return space;
@@ -445,7 +548,7 @@ namespace
 		return { keys(last), positions(last) };
 	}
 	template<typename T, typename Out, int VEC>
-	void table_gradient(hipStream_t stream, const EmbeddingShape &s, const int *keys, const int *positions, const T *dy, float scale, float beta, Out *out)
+	void table_gradient(hipStream_t stream, const EmbeddingShape &s, const int *keys, const int *positions, const T *dy, float *partial, float scale, float beta, Out *out)
 	{
 		int lanes = 1;
 		while (lanes < 256 && lanes * VEC < s.columns)
@@ -453,7 +556,12 @@ namespace
 		const int spans = ceil_div(s.columns, lanes * VEC);
 		const size_t units = static_cast<size_t>(s.classes) * spans;
 		const int most = static_cast<int>(std::min<size_t>(MOST_CLASSES_OF_GROUP, std::max<size_t>(1, units / 2048)));
-		const TableGradient<T, Out> p { keys, positions, dy, out, s.rows, s.classes, s.columns, most, lanes, scale, beta };
+		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, scale, beta };
+		if (s.rows >= CHUNK)
+		{
+			hipLaunchKernelGGL((kernel_chunk_sums<T, Out, VEC>), dim3(ceil_div(s.rows, CHUNK), spans), dim3(256), 0, stream, p);
+			MLHIP_CHECK(hipGetLastError());
+		}
 		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3(ceil_div(s.classes, most), spans), dim3(256), 0, stream, p);
 		MLHIP_CHECK(hipGetLastError());
 	}
@@ -462,12 +570,13 @@ namespace
 	{
 		constexpr int VEC = 16 / sizeof(T);
 		const int *keys = nullptr, *positions = nullptr;
+		float *partial = reinterpret_cast<float*>(workspace + embedding_space(s).partial);
 		if (s.rows > 0)
 			std::tie(keys, positions) = sort_tokens(stream, s, tokens, workspace);
 		if (s.columns >= VEC)
-			table_gradient<T, Out, VEC>(stream, s, keys, positions, dy, scale, beta, out);
+			table_gradient<T, Out, VEC>(stream, s, keys, positions, dy, partial, scale, beta, out);
 		else
-			table_gradient<T, Out, 1>(stream, s, keys, positions, dy, scale, beta, out);
+			table_gradient<T, Out, 1>(stream, s, keys, positions, dy, partial, scale, beta, out);
 	}
 	void check_tokens(const mlTensor_t &tokens, const EmbeddingShape &s, const char *name)
 	{
