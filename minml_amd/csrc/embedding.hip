@@ -73,7 +73,7 @@ namespace
 	}
 	__device__ __forceinline__ int key_of(int token, int classes)
 	{
-		return (token >= 0 && token < classes) ? token : classes;
+		return static_cast<int>(min(static_cast<uint32_t>(token), static_cast<uint32_t>(classes)));
 	}
 	/* sum of the values of the threads before; of a workgroup of 64 WAVES threads. Every thread calls it */
 	template<int WAVES>
@@ -97,82 +97,39 @@ namespace
 		__syncthreads();
 		return before;
 	}
-	/* up to 4096 tokens by one workgroup, in LDS */
-	constexpr int SMALL_SORT = 4096;
-	__global__ __launch_bounds__(1024) void kernel_sort_small(const int *tokens, int count, int classes, int bits, int *keys_out, int *positions_out)
+	/*
+	 * Few tokens: every one counts those that come before it, 64 tokens of a workgroup against all others, a sixteenth of them by each wavefront, which reads them through scalar registers.
+	 */
+	__global__ __launch_bounds__(1024) void kernel_sort_by_counting(const int *tokens, int count, int classes, int *keys_out, int *positions_out)
 	{
-		constexpr int WAVES = 16, ROUNDS = SMALL_SORT / 1024, DIGIT = 8, DIGITS = 1 << DIGIT;
-		__shared__ int keys[SMALL_SORT], positions[SMALL_SORT];
-		__shared__ int counters[WAVES][DIGITS];
-		__shared__ int waves[WAVES];
-		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-		int key[ROUNDS], position[ROUNDS], rank[ROUNDS];
-		/* a wavefront has 256 neighbours */
-#pragma unroll
-		for (int u = 0; u < ROUNDS; u++)
+		constexpr int WAVES = 16;
+		__shared__ int counts[WAVES][64];
+		const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+		const int first = blockIdx.x * 64, position = first + lane;
+		const int key = position < count ? key_of(tokens[position], classes) : 0;
+		const int each = (count + WAVES - 1) / WAVES, from = min(wave * each, count), to = min(from + each, count);
+		int before = 0;
+		/* neither of the workgroup's own tokens nor of those behind counts an equal one, of those before it does */
+		const auto count_below = [&](int begin, int end, int limit) __attribute__((always_inline))
 		{
-			position[u] = wave * 64 * ROUNDS + u * 64 + lane;
-			key[u] = position[u] < count ? key_of(tokens[position[u]], classes) : 0x7fffffff;
-		}
-		for (int shift = 0; shift < bits; shift += DIGIT)
+#pragma unroll 16
+			for (int i = begin; i < end; i++)
+				before += key_of(tokens[i], classes) < limit ? 1 : 0;
+		};
+		count_below(from, min(to, first), key + 1);
+		count_below(max(from, first + 64), to, key);
+		for (int i = max(from, first); i < min(to, first + 64); i++)
+			before += key_of(tokens[i], classes) < key + (i < position ? 1 : 0) ? 1 : 0;
+		counts[wave][lane] = before;
+		__syncthreads();
+		if (wave == 0 && position < count)
 		{
+			int place = 0;
 #pragma unroll
-			for (int u = 0; u < WAVES * DIGITS / 1024; u++)
-				(&counters[0][0])[u * 1024 + threadIdx.x] = 0;
-			__syncthreads();
-#pragma unroll
-			for (int u = 0; u < ROUNDS; u++)
-			{
-				const int digit = (key[u] >> shift) & (DIGITS - 1);
-				const uint64_t same = lanes_alike(digit, DIGIT, true);
-				const int below = lanes_below(same);
-				int *counter = &counters[wave][digit];
-				rank[u] = *counter + below;
-				wave_in_order();
-				if (below == 0)
-					*counter += __popcll(same);
-				wave_in_order();
-			}
-			__syncthreads();
-			int total = 0;
-			if (threadIdx.x < DIGITS)
-				for (int w = 0; w < WAVES; w++)
-					total += counters[w][threadIdx.x];
-			int begin = scan_exclusive<WAVES>(total, waves);
-			if (threadIdx.x < DIGITS)
-				for (int w = 0; w < WAVES; w++)
-				{
-					const int here = counters[w][threadIdx.x];
-					counters[w][threadIdx.x] = begin;
-					begin += here;
-				}
-			__syncthreads();
-#pragma unroll
-			for (int u = 0; u < ROUNDS; u++)
-			{
-				const int place = counters[wave][(key[u] >> shift) & (DIGITS - 1)] + rank[u];
-				keys[place] = key[u];
-				positions[place] = position[u];
-			}
-			__syncthreads();
-#pragma unroll
-			for (int u = 0; u < ROUNDS; u++)
-			{
-				const int from = wave * 64 * ROUNDS + u * 64 + lane;
-				key[u] = keys[from];
-				position[u] = positions[from];
-			}
-			__syncthreads();
-		}
-#pragma unroll
-		for (int u = 0; u < ROUNDS; u++)
-		{
-			const int to = wave * 64 * ROUNDS + u * 64 + lane;
-			if (to < count)
-			{
-				keys_out[to] = key[u];
-				positions_out[to] = position[u];
-			}
+			for (int w = 0; w < WAVES; w++)
+				place += counts[w][lane];
+			keys_out[place] = key;
+			positions_out[place] = position;
 		}
 	}
 	/*
@@ -214,7 +171,7 @@ namespace
 	{
 		extern __shared__ int counters[]; /* [4 wavefronts][digits], then [digits] */
 		__shared__ int waves[4];
-		const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+		const int digits = 1 << p.bits, groups = gridDim.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 		int *begin = counters + 4 * digits, *mine = counters + wave * digits;
 		for (int d = threadIdx.x; d < 4 * digits; d += 256)
 			counters[d] = 0;
@@ -229,15 +186,23 @@ namespace
 		int sum = 0;
 		for (int u = 0; u < each; u++)
 		{
+			constexpr int AHEAD = 16;
 			const int d = threadIdx.x * each + u;
 			int before = 0, total = 0;
 			if (d < digits)
 			{
-				for (int g = 0; g < static_cast<int>(gridDim.x); g++)
+				for (int g = 0; g < groups; g += AHEAD)
 				{
-					const int c = p.counts[static_cast<size_t>(g) * digits + d];
-					before += g < static_cast<int>(blockIdx.x) ? c : 0;
-					total += c;
+					int c[AHEAD];
+#pragma unroll
+					for (int a = 0; a < AHEAD; a++)
+						c[a] = p.counts[min(g + a, groups - 1) * digits + d];
+#pragma unroll
+					for (int a = 0; a < AHEAD; a++)
+					{
+						before += g + a < static_cast<int>(blockIdx.x) ? c[a] : 0;
+						total += g + a < groups ? c[a] : 0;
+					}
 				}
 				begin[d] = sum + before;
 			}
@@ -295,7 +260,7 @@ namespace
 			const T *dy;
 			float *partial; /* [chunks][columns] */
 			Out *out;
-			int count, classes, columns, classes_of_group, lanes; /* lanes: threads of a row, a power of two */
+			int count, classes, columns, classes_of_group, lanes, spans; /* lanes: threads of a row, a power of two; spans: that a row takes of them */
 			float scale, beta;
 	};
 	/* the first place whose key is not below `key` */
@@ -312,10 +277,9 @@ namespace
 		return first;
 	}
 	/* v += the rows of every `step`th place from `first` on, AHEAD of them on their way at a time. row(i): where the i-th lies */
-	template<typename T, int VEC, typename Row>
+	template<typename T, int AHEAD, int VEC, typename Row>
 	__device__ __forceinline__ void add_rows(float (&v)[VEC], int first, int last, int step, Row &&row)
 	{
-		constexpr int AHEAD = 8;
 		for (int i = first; i < last; i += AHEAD * step)
 		{
 			Elements<T, VEC> x[AHEAD];
@@ -358,10 +322,10 @@ namespace
 			return;
 		/* 64 places of one class with the chunk's first one among them; and where the class ends in the chunk */
 		const int from = first - lane, to = from + CHUNK - 1;
-		const bool all = from >= 0 && to < p.count && p.keys[max(from, 0)] == key && p.keys[min(to, p.count - 1)] == key;
+		const bool all = lane < CHUNK && from >= 0 && to < p.count && p.keys[max(from, 0)] == key && p.keys[min(to, p.count - 1)] == key;
 		if (__ballot(all) == 0)
 			return;
-		const bool mine = first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
+		const bool mine = lane < CHUNK && first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
 		const int here = __popcll(__ballot(mine));
 		if (threadIdx.x < CHUNK)
 			rows[threadIdx.x] = p.positions[min(first + lane, p.count - 1)];
@@ -372,7 +336,7 @@ namespace
 #pragma unroll
 		for (int e = 0; e < VEC; e++)
 			v[e] = 0.0f;
-		add_rows<T, VEC>(v, threadIdx.x / p.lanes, here, 256 / p.lanes, [&](int i) __attribute__((always_inline))
+		add_rows<T, 16>(v, threadIdx.x / p.lanes, here, 256 / p.lanes, [&](int i) __attribute__((always_inline))
 		{
 			return place.in(p.dy + static_cast<size_t>(rows[i]) * p.columns);
 		});
@@ -386,62 +350,120 @@ namespace
 	template<typename T, typename Out, int VEC>
 	__global__ __launch_bounds__(256) void kernel_table_gradient(TableGradient<T, Out> p)
 	{
+		constexpr int AHEAD = 8;
 		__shared__ int bounds[MOST_CLASSES_OF_GROUP + 1];
 		__shared__ float meeting[256][VEC];
-		const int first_class = blockIdx.x * p.classes_of_group, classes = min(p.classes_of_group, p.classes - first_class);
+		const int unit = blockIdx.x / p.spans, span = blockIdx.x % p.spans;
+		const int first_class = unit * p.classes_of_group, classes = min(p.classes_of_group, p.classes - first_class);
 		for (int i = threadIdx.x; i <= classes; i += 256)
 			bounds[i] = lower_bound(p.keys, p.count, first_class + i);
 		__syncthreads();
-		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC, groups = 256 / p.lanes, group = threadIdx.x / p.lanes;
+		const int column = (span * p.lanes + threadIdx.x % p.lanes) * VEC, groups = 256 / p.lanes, group = threadIdx.x / p.lanes;
 		const bool inside = column < p.columns;
 		const RowPlace place = place_in_row<VEC>(min(column, p.columns - 1), p.columns);
+		const auto of_all = [&](int c)
+		{
+			const int rows = bounds[c + 1] - bounds[c];
+			return (groups > 1 && rows >= ROWS_OF_ALL) || rows >= CHUNK;
+		};
 		const auto row_of_list = [&](int i) __attribute__((always_inline))
 		{
 			return place.in(p.dy + static_cast<size_t>(p.positions[i]) * p.columns);
 		};
-		const auto write = [&](int c, float (&v)[VEC]) __attribute__((always_inline))
+		const auto row_of_table = [&](int c) __attribute__((always_inline))
 		{
-			Out *dst = place.in(p.out + static_cast<size_t>(first_class + c) * p.columns);
-			Elements<Out, VEC> old;
-			if (p.beta != 0.0f)
-				old.load(dst);
+			return place.in(p.out + static_cast<size_t>(c) * p.columns);
+		};
+		const auto write = [&](int c, float (&v)[VEC], const Elements<Out, VEC> &old) __attribute__((always_inline))
+		{
 #pragma unroll
 			for (int e = 0; e < VEC; e++)
 				v[e] = p.beta != 0.0f ? fmaf(p.beta, old[e], p.scale * v[e]) : p.scale * v[e];
-			store_nearest<VEC>(dst, v, place.skip);
+			store_nearest<VEC>(row_of_table(c), v, place.skip);
 		};
+		float v[VEC];
+		Elements<Out, VEC> old;
 		if (inside)
-			for (int c = group; c < classes; c += groups)
-			{
-				const int begin = bounds[c], end = bounds[c + 1];
-				if ((groups > 1 && end - begin >= ROWS_OF_ALL) || end - begin >= CHUNK)
-					continue;
-				float v[VEC];
+		{
+			/* neighbouring classes of a group of threads: first those without rows, which wait for nothing; then the others' rows in one go, whichever class they are of */
+			const int each = (classes + groups - 1) / groups, begin = min(group * each, classes), end = min(begin + each, classes);
+			if (p.beta != 1.0f)
+				for (int c = begin; c < end; c++)
+					if (bounds[c] == bounds[c + 1])
+					{
 #pragma unroll
-				for (int e = 0; e < VEC; e++)
-					v[e] = 0.0f;
-				add_rows<T, VEC>(v, begin, end, 1, row_of_list);
-				write(c, v);
+						for (int e = 0; e < VEC; e++)
+							v[e] = 0.0f;
+						if (p.beta != 0.0f)
+							old.load(row_of_table(first_class + c));
+						write(first_class + c, v, old);
+					}
+			for (int c = begin; c < end;)
+			{
+				if (of_all(c))
+				{
+					c++;
+					continue;
+				}
+				const int first = bounds[c];
+				while (c < end && !of_all(c))
+					c++;
+				const int last = bounds[c];
+				int current = -1;
+				for (int i = first; i < last; i += AHEAD)
+				{
+					Elements<T, VEC> x[AHEAD];
+					int key[AHEAD];
+#pragma unroll
+					for (int u = 0; u < AHEAD; u++)
+					{
+						key[u] = p.keys[min(i + u, last - 1)];
+						x[u].load(row_of_list(min(i + u, last - 1)));
+					}
+#pragma unroll
+					for (int u = 0; u < AHEAD; u++)
+						if (i + u < last)
+						{
+							if (key[u] != current)
+							{
+								if (current >= 0)
+									write(current, v, old);
+								current = key[u];
+								if (p.beta != 0.0f)
+									old.load(row_of_table(current));
+#pragma unroll
+								for (int e = 0; e < VEC; e++)
+									v[e] = 0.0f;
+							}
+#pragma unroll
+							for (int e = 0; e < VEC; e++)
+								v[e] += x[u][e];
+						}
+				}
+				if (current >= 0)
+					write(current, v, old);
 			}
+		}
 		for (int c = 0; c < classes; c++)
 		{
-			const int begin = bounds[c], end = bounds[c + 1];
-			if (!((groups > 1 && end - begin >= ROWS_OF_ALL) || end - begin >= CHUNK))
+			if (!of_all(c))
 				continue;
+			const int begin = bounds[c], end = bounds[c + 1];
 			const int chunk = (begin + CHUNK - 1) / CHUNK, direct = end - begin < CHUNK ? end : min(end, chunk * CHUNK);
-			float v[VEC];
 #pragma unroll
 			for (int e = 0; e < VEC; e++)
 				v[e] = 0.0f;
-			add_rows<T, VEC>(v, begin + group, direct, groups, row_of_list);
+			if (p.beta != 0.0f && group == 0)
+				old.load(row_of_table(first_class + c));
+			add_rows<T, AHEAD>(v, begin + group, direct, groups, row_of_list);
 			if (direct < end)
-				add_rows<float, VEC>(v, chunk + group, (end + CHUNK - 1) / CHUNK, groups, [&](int i) __attribute__((always_inline))
+				add_rows<float, AHEAD>(v, chunk + group, (end + CHUNK - 1) / CHUNK, groups, [&](int i) __attribute__((always_inline))
 				{
 					return place.in(static_cast<const float*>(p.partial) + static_cast<size_t>(i) * p.columns);
 				});
 			join_groups<VEC>(v, p.lanes, meeting);
 			if (group == 0 && inside)
-				write(c, v);
+				write(first_class + c, v, old);
 		}
 	}
 
@@ -477,6 +499,10 @@ namespace
 		plan.groups = ceil_div(s.rows, plan.per_group);
 		return plan;
 	}
+	bool sorted_by_counting(const EmbeddingShape &s)
+	{
+		return s.rows <= 16384;
+	}
 	struct EmbeddingSpace
 	{
 			size_t keys[2], positions[2], counts, partial, total;
@@ -494,7 +520,7 @@ namespace
 		if (s.rows > 0)
 		{
 			const SortPlan plan = sort_plan(s);
-			const bool small = s.rows <= SMALL_SORT;
+			const bool small = sorted_by_counting(s);
 			for (int i = 0; i < (small || plan.passes == 1 ? 1 : 2); i++)
 			{
 				space.keys[i] = take(sizeof(int) * s.rows);
@@ -528,9 +554,9 @@ namespace
 		{
 			return reinterpret_cast<int*>(workspace + space.positions[i]);
 		};
-		if (s.rows <= SMALL_SORT)
+		if (sorted_by_counting(s))
 		{
-			hipLaunchKernelGGL(kernel_sort_small, dim3(1), dim3(1024), 0, stream, tokens, s.rows, s.classes, plan.bits, keys(0), positions(0));
+			hipLaunchKernelGGL(kernel_sort_by_counting, dim3(ceil_div(s.rows, 64)), dim3(1024), 0, stream, tokens, s.rows, s.classes, keys(0), positions(0));
 			MLHIP_CHECK(hipGetLastError());
 			return { keys(0), positions(0) };
 		}
@@ -556,13 +582,13 @@ namespace
 		const int spans = ceil_div(s.columns, lanes * VEC);
 		const size_t units = static_cast<size_t>(s.classes) * spans;
 		const int most = static_cast<int>(std::min<size_t>(MOST_CLASSES_OF_GROUP, std::max<size_t>(1, units / 2048)));
-		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, scale, beta };
+		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, scale, beta };
 		if (s.rows >= CHUNK)
 		{
 			hipLaunchKernelGGL((kernel_chunk_sums<T, Out, VEC>), dim3(ceil_div(s.rows, CHUNK), spans), dim3(256), 0, stream, p);
 			MLHIP_CHECK(hipGetLastError());
 		}
-		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3(ceil_div(s.classes, most), spans), dim3(256), 0, stream, p);
+		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3(static_cast<unsigned int>(ceil_div(s.classes, most)) * spans), dim3(256), 0, stream, p);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	template<typename T, typename Out>
