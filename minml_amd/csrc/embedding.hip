@@ -133,16 +133,16 @@ namespace
 		}
 	}
 	/*
-	 * More of them: a launch that counts the digits of every group's tokens and one that puts them in place, for every digit of up to 11 bits. At most SORT_GROUPS groups, so that each can add up the others' counts by itself.
-	 * `keys` null: the tokens themselves, which stand where they are
+	 * More of them: a launch that counts the digits of every group's tokens and one that puts them in place, for every digit of up to 11 bits. At most 64 groups, so that each can add up the others' counts by itself (that it also
+	 * counts the others' tokens, without the first launch, takes 16 us where the two take 12, at 16384 tokens). `keys` null: the tokens themselves, which stand where they are
 	 */
-	constexpr int SORT_GROUPS = 64;
+	constexpr int SORT_GROUPS = 64, SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES;
 	struct SortPass
 	{
 			const int *tokens, *keys, *positions;
 			int *keys_out, *positions_out;
 			int *counts; /* [groups][2^bits] */
-			int count, classes, shift, bits, per_group; /* per_group: a multiple of 256 */
+			int count, classes, shift, bits, per_group; /* per_group: a multiple of 512 */
 
 			__device__ __forceinline__ int key(int i) const
 			{
@@ -152,77 +152,92 @@ namespace
 			{
 				return (key >> shift) & ((1 << bits) - 1);
 			}
+			/* counters[digit] of the tokens of [first, last); several tokens of a thread on their way at a time */
+			template<int THREADS>
+			__device__ __forceinline__ void count_digits(int *counters, int first, int last, int thread) const
+			{
+				constexpr int AHEAD = 8;
+				for (int i = first + thread; i < last; i += AHEAD * THREADS)
+				{
+					int k[AHEAD];
+#pragma unroll
+					for (int u = 0; u < AHEAD; u++)
+						k[u] = key(min(i + u * THREADS, last - 1));
+#pragma unroll
+					for (int u = 0; u < AHEAD; u++)
+						if (i + u * THREADS < last)
+							atomicAdd(&counters[digit(k[u])], 1);
+				}
+			}
 	};
-	__global__ __launch_bounds__(256) void kernel_sort_count(SortPass p)
+	__global__ __launch_bounds__(SORT_THREADS) void kernel_sort_count(SortPass p)
 	{
 		extern __shared__ int counters[];
 		const int digits = 1 << p.bits;
-		for (int d = threadIdx.x; d < digits; d += 256)
+		for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
 			counters[d] = 0;
 		__syncthreads();
 		const int first = blockIdx.x * p.per_group, last = first + min(p.per_group, p.count - first);
-		for (int i = first + threadIdx.x; i < last; i += 256)
-			atomicAdd(&counters[p.digit(p.key(i))], 1);
+		p.count_digits<SORT_THREADS>(counters, first, last, threadIdx.x);
 		__syncthreads();
-		for (int d = threadIdx.x; d < digits; d += 256)
-			p.counts[static_cast<size_t>(blockIdx.x) * digits + d] = counters[d];
+		for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
+			p.counts[blockIdx.x * digits + d] = counters[d];
 	}
-	__global__ __launch_bounds__(256) void kernel_sort_place(SortPass p)
+	__global__ __launch_bounds__(SORT_THREADS) void kernel_sort_place(SortPass p)
 	{
-		extern __shared__ int counters[]; /* [4 wavefronts][digits], then [digits] */
-		__shared__ int waves[4];
+		extern __shared__ int counters[]; /* [wavefronts][digits]; of the groups before [digits], of those behind */
+		__shared__ int waves[SORT_WAVES];
 		const int digits = 1 << p.bits, groups = gridDim.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-		int *begin = counters + 4 * digits, *mine = counters + wave * digits;
-		for (int d = threadIdx.x; d < 4 * digits; d += 256)
+		int *before = counters + SORT_WAVES * digits, *behind = before + digits, *mine = counters + wave * digits;
+		for (int d = threadIdx.x; d < (SORT_WAVES + 2) * digits; d += SORT_THREADS)
 			counters[d] = 0;
 		__syncthreads();
-		/* a wavefront has a quarter of the group's tokens, in their order */
-		const int group_first = blockIdx.x * p.per_group, quarter = p.per_group / 4;
-		const int left = p.count - group_first - wave * quarter, here = max(0, min(quarter, left)), first = group_first + wave * quarter;
-		for (int i = lane; i < here; i += 64)
-			atomicAdd(&mine[p.digit(p.key(first + i))], 1);
-		/* of every digit: the tokens of all groups, and those of the groups before */
-		const int each = max(1, digits / 256); /* neighbouring digits of a thread */
-		int sum = 0;
-		for (int u = 0; u < each; u++)
+		/* a wavefront has an eighth of the group's tokens, in their order */
+		const int group_first = blockIdx.x * p.per_group, group_last = group_first + min(p.per_group, p.count - group_first), share = p.per_group / SORT_WAVES;
+		const int first = group_first + wave * share, here = max(0, min(share, group_last - first));
+		p.count_digits<64>(mine, first, first + here, lane);
+		for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
 		{
 			constexpr int AHEAD = 16;
-			const int d = threadIdx.x * each + u;
-			int before = 0, total = 0;
-			if (d < digits)
+			int sum_before = 0, sum_behind = 0;
+			for (int g = 0; g < groups; g += AHEAD)
 			{
-				for (int g = 0; g < groups; g += AHEAD)
+				int c[AHEAD];
+#pragma unroll
+				for (int a = 0; a < AHEAD; a++)
+					c[a] = p.counts[min(g + a, groups - 1) * digits + d];
+#pragma unroll
+				for (int a = 0; a < AHEAD; a++)
 				{
-					int c[AHEAD];
-#pragma unroll
-					for (int a = 0; a < AHEAD; a++)
-						c[a] = p.counts[min(g + a, groups - 1) * digits + d];
-#pragma unroll
-					for (int a = 0; a < AHEAD; a++)
-					{
-						before += g + a < static_cast<int>(blockIdx.x) ? c[a] : 0;
-						total += g + a < groups ? c[a] : 0;
-					}
+					sum_before += g + a < static_cast<int>(blockIdx.x) ? c[a] : 0;
+					sum_behind += g + a > static_cast<int>(blockIdx.x) && g + a < groups ? c[a] : 0;
 				}
-				begin[d] = sum + before;
 			}
-			sum += total;
+			before[d] = sum_before;
+			behind[d] = sum_behind;
 		}
-		const int smaller = scan_exclusive<4>(sum, waves); /* its barriers stand behind the counts of the wavefronts, too */
-		for (int u = 0; u < each; u++)
+		__syncthreads();
+		const int each = max(1, digits / SORT_THREADS); /* neighbouring digits of a thread */
+		int sum = 0;
+		for (int d = threadIdx.x * each; d < min(static_cast<int>(threadIdx.x + 1) * each, digits); d++)
 		{
-			const int d = threadIdx.x * each + u;
-			if (d < digits)
-			{
-				int at = begin[d] + smaller;
+			sum += before[d] + behind[d];
 #pragma unroll
-				for (int w = 0; w < 4; w++)
-				{
-					const int n = counters[w * digits + d];
-					counters[w * digits + d] = at;
-					at += n;
-				}
+			for (int w = 0; w < SORT_WAVES; w++)
+				sum += counters[w * digits + d];
+		}
+		int smaller = scan_exclusive<SORT_WAVES>(sum, waves);
+		for (int d = threadIdx.x * each; d < min(static_cast<int>(threadIdx.x + 1) * each, digits); d++)
+		{
+			int at = smaller + before[d];
+#pragma unroll
+			for (int w = 0; w < SORT_WAVES; w++)
+			{
+				const int n = counters[w * digits + d];
+				counters[w * digits + d] = at;
+				at += n;
 			}
+			smaller = at + behind[d];
 		}
 		__syncthreads();
 		for (int i = 0; i < here; i += 64)
@@ -248,11 +263,11 @@ namespace
 
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
 	/*
-	 * A class's rows are added up by those who write its row of the table; but where one class has many (a few tokens are in every line), they would wait for it alone. The list is therefore cut into chunks of 64 places, and of
-	 * a class of 64 and more rows every chunk that it has from its first place on is added up beforehand, by a launch of its own, so that what is left is at most 63 rows before its first whole chunk and a sum in fp32 for every
-	 * 64 further ones. Neither asks more than the list to know who does what.
+	 * A class's rows are added up by those who write its row of the table; but where one class has many (a few tokens are in every line), they would wait for it alone. The list is therefore cut into chunks of 64 places (32 where a row takes
+	 * all threads of a workgroup, so that nothing adds up rows side by side), and of a class of as many rows and more every chunk that it has from its first place on is added up beforehand, by a launch of its own, so that what is
+	 * left is less than a chunk's rows before its first whole chunk and one sum in fp32 for every further one. Neither asks more than the list to know who does what.
 	 */
-	constexpr int CHUNK = 64;
+	constexpr int MOST_OF_CHUNK = 64;
 	template<typename T, typename Out>
 	struct TableGradient
 	{
@@ -260,19 +275,33 @@ namespace
 			const T *dy;
 			float *partial; /* [chunks][columns] */
 			Out *out;
-			int count, classes, columns, classes_of_group, lanes, spans; /* lanes: threads of a row, a power of two; spans: that a row takes of them */
+			int count, classes, columns, classes_of_group, lanes, spans, chunk; /* lanes: threads of a row, a power of two; spans: that a row takes of them */
 			float scale, beta;
 	};
-	/* the first place whose key is not below `key` */
-	__device__ __forceinline__ int lower_bound(const int *keys, int count, int key)
+	/* the first place of [first, first + length) whose key is not below `key` */
+	__device__ __forceinline__ int lower_bound(const int *keys, int first, int length, int key)
 	{
-		int first = 0, length = count;
 		while (length > 0)
 		{
 			const int half = length / 2;
 			const bool below = keys[first + half] < key;
 			first = below ? first + half + 1 : first;
 			length = below ? length - half - 1 : half;
+		}
+		return first;
+	}
+	/* the same by a whole wavefront, which looks at 64 places at a time: three reads one after another where halving takes 17 */
+	__device__ __forceinline__ int lower_bound_by_wave(const int *keys, int length, int key)
+	{
+		const int lane = threadIdx.x & 63;
+		int first = 0;
+		while (length > 0)
+		{
+			const int step = (length + 63) / 64, at = (lane + 1) * step - 1;
+			const bool below = at < length && keys[first + min(at, length - 1)] < key;
+			const int whole = __popcll(__ballot(below));
+			first += whole * step;
+			length = min(step - 1, length - whole * step);
 		}
 		return first;
 	}
@@ -315,19 +344,19 @@ namespace
 	__global__ __launch_bounds__(256) void kernel_chunk_sums(TableGradient<T, Out> p)
 	{
 		__shared__ float meeting[256][VEC];
-		__shared__ int rows[CHUNK];
-		const int first = blockIdx.x * CHUNK, lane = threadIdx.x & 63;
+		__shared__ int rows[MOST_OF_CHUNK];
+		const int first = blockIdx.x * p.chunk, lane = threadIdx.x & 63;
 		const int key = p.keys[first];
 		if (key >= p.classes)
 			return;
-		/* 64 places of one class with the chunk's first one among them; and where the class ends in the chunk */
-		const int from = first - lane, to = from + CHUNK - 1;
-		const bool all = lane < CHUNK && from >= 0 && to < p.count && p.keys[max(from, 0)] == key && p.keys[min(to, p.count - 1)] == key;
+		/* as many places as a chunk's of one class with the chunk's first one among them; and where the class ends in the chunk */
+		const int from = first - lane, to = from + p.chunk - 1;
+		const bool all = lane < p.chunk && from >= 0 && to < p.count && p.keys[max(from, 0)] == key && p.keys[min(to, p.count - 1)] == key;
 		if (__ballot(all) == 0)
 			return;
-		const bool mine = lane < CHUNK && first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
+		const bool mine = lane < p.chunk && first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
 		const int here = __popcll(__ballot(mine));
-		if (threadIdx.x < CHUNK)
+		if (static_cast<int>(threadIdx.x) < p.chunk)
 			rows[threadIdx.x] = p.positions[min(first + lane, p.count - 1)];
 		__syncthreads();
 		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC;
@@ -351,12 +380,19 @@ namespace
 	__global__ __launch_bounds__(256) void kernel_table_gradient(TableGradient<T, Out> p)
 	{
 		constexpr int AHEAD = 8;
-		__shared__ int bounds[MOST_CLASSES_OF_GROUP + 1];
+		__shared__ int bounds[MOST_CLASSES_OF_GROUP + 1], ends[2];
 		__shared__ float meeting[256][VEC];
 		const int unit = blockIdx.x / p.spans, span = blockIdx.x % p.spans;
 		const int first_class = unit * p.classes_of_group, classes = min(p.classes_of_group, p.classes - first_class);
-		for (int i = threadIdx.x; i <= classes; i += 256)
-			bounds[i] = lower_bound(p.keys, p.count, first_class + i);
+		if (threadIdx.x < 128)
+		{
+			const int wave = threadIdx.x >> 6, bound = lower_bound_by_wave(p.keys, p.count, first_class + wave * classes);
+			if ((threadIdx.x & 63) == 0)
+				ends[wave] = bound;
+		}
+		__syncthreads();
+		if (static_cast<int>(threadIdx.x) <= classes)
+			bounds[threadIdx.x] = lower_bound(p.keys, ends[0], ends[1] - ends[0], first_class + threadIdx.x);
 		__syncthreads();
 		const int column = (span * p.lanes + threadIdx.x % p.lanes) * VEC, groups = 256 / p.lanes, group = threadIdx.x / p.lanes;
 		const bool inside = column < p.columns;
@@ -364,7 +400,7 @@ namespace
 		const auto of_all = [&](int c)
 		{
 			const int rows = bounds[c + 1] - bounds[c];
-			return (groups > 1 && rows >= ROWS_OF_ALL) || rows >= CHUNK;
+			return (groups > 1 && rows >= ROWS_OF_ALL) || rows >= p.chunk;
 		};
 		const auto row_of_list = [&](int i) __attribute__((always_inline))
 		{
@@ -449,7 +485,7 @@ namespace
 			if (!of_all(c))
 				continue;
 			const int begin = bounds[c], end = bounds[c + 1];
-			const int chunk = (begin + CHUNK - 1) / CHUNK, direct = end - begin < CHUNK ? end : min(end, chunk * CHUNK);
+			const int chunk = (begin + p.chunk - 1) / p.chunk, direct = end - begin < p.chunk ? end : min(end, chunk * p.chunk);
 #pragma unroll
 			for (int e = 0; e < VEC; e++)
 				v[e] = 0.0f;
@@ -457,7 +493,7 @@ namespace
 				old.load(row_of_table(first_class + c));
 			add_rows<T, AHEAD>(v, begin + group, direct, groups, row_of_list);
 			if (direct < end)
-				add_rows<float, AHEAD>(v, chunk + group, (end + CHUNK - 1) / CHUNK, groups, [&](int i) __attribute__((always_inline))
+				add_rows<float, AHEAD>(v, chunk + group, (end + p.chunk - 1) / p.chunk, groups, [&](int i) __attribute__((always_inline))
 				{
 					return place.in(static_cast<const float*>(p.partial) + static_cast<size_t>(i) * p.columns);
 				});
@@ -495,19 +531,37 @@ namespace
 			plan.bits++;
 		plan.passes = ceil_div(plan.bits, 11);
 		plan.digit_bits = ceil_div(plan.bits, plan.passes);
-		plan.per_group = std::max(1024, static_cast<int>(round_up(ceil_div(s.rows, SORT_GROUPS), 256)));
+		plan.per_group = std::max(1024, static_cast<int>(round_up(ceil_div(s.rows, SORT_GROUPS), 512)));
 		plan.groups = ceil_div(s.rows, plan.per_group);
 		return plan;
 	}
 	bool sorted_by_counting(const EmbeddingShape &s)
 	{
-		return s.rows <= 16384;
+		return s.rows <= 8192;
+	}
+	/* threads that a row takes, a power of two */
+	int lanes_of_row(const EmbeddingShape &s, int vector)
+	{
+		int lanes = 1;
+		while (lanes < 256 && lanes * vector < s.columns)
+			lanes *= 2;
+		return lanes;
+	}
+	int chunk_of(const EmbeddingShape &s, int vector)
+	{
+		return lanes_of_row(s, vector) == 256 ? 32 : MOST_OF_CHUNK;
+	}
+	/* elements of dy that a thread takes at a time */
+	int vector_of(const EmbeddingShape &s, mlDataType_t dtype)
+	{
+		const int vector = 16 / size_of(dtype);
+		return s.columns >= vector ? vector : 1;
 	}
 	struct EmbeddingSpace
 	{
 			size_t keys[2], positions[2], counts, partial, total;
 	};
-	EmbeddingSpace embedding_space(const EmbeddingShape &s)
+	EmbeddingSpace embedding_space(const EmbeddingShape &s, mlDataType_t dtype)
 	{
 		EmbeddingSpace space { };
 		size_t at = 0;
@@ -527,7 +581,8 @@ namespace
 				space.positions[i] = take(sizeof(int) * s.rows);
 			}
 			space.counts = take(small ? 0 : (sizeof(int) * plan.groups << plan.digit_bits));
-			space.partial = take(s.rows >= CHUNK ? sizeof(float) * ceil_div(s.rows, CHUNK) * s.columns : 0);
+			const int chunk = chunk_of(s, vector_of(s, dtype));
+			space.partial = take(s.rows >= chunk ? sizeof(float) * ceil_div(s.rows, chunk) * s.columns : 0);
 		}
 		space.total = at;
 		return space;
@@ -542,9 +597,8 @@ namespace
 		MLHIP_CHECK(hipGetLastError());
 	}
 	/* the tokens in order: keys and positions */
-	std::pair<const int*, const int*> sort_tokens(hipStream_t stream, const EmbeddingShape &s, const int *tokens, uint8_t *workspace)
+	std::pair<const int*, const int*> sort_tokens(hipStream_t stream, const EmbeddingShape &s, const EmbeddingSpace &space, const int *tokens, uint8_t *workspace)
 	{
-		const EmbeddingSpace space = embedding_space(s);
 		const SortPlan plan = sort_plan(s);
 		const auto keys = [&](int i)
 		{
@@ -566,8 +620,9 @@ namespace
 			const SortPass p { tokens, pass == 0 ? nullptr : keys(from), pass == 0 ? nullptr : positions(from), keys(to), positions(to), reinterpret_cast<int*>(workspace + space.counts), s.rows, s.classes,
 					pass * plan.digit_bits, plan.digit_bits, plan.per_group };
 			const int bytes = static_cast<int>(sizeof(int)) << plan.digit_bits;
-			hipLaunchKernelGGL(kernel_sort_count, dim3(plan.groups), dim3(256), bytes, stream, p);
-			hipLaunchKernelGGL(kernel_sort_place, dim3(plan.groups), dim3(256), 5 * bytes, stream, p);
+			hipLaunchKernelGGL(kernel_sort_count, dim3(plan.groups), dim3(SORT_THREADS), bytes, stream, p);
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel_sort_place), (SORT_WAVES + 2) * bytes);
+			hipLaunchKernelGGL(kernel_sort_place, dim3(plan.groups), dim3(SORT_THREADS), (SORT_WAVES + 2) * bytes, stream, p);
 			MLHIP_CHECK(hipGetLastError());
 		}
 		const int last = (plan.passes - 1) & 1;
@@ -576,29 +631,27 @@ namespace
 	template<typename T, typename Out, int VEC>
 	void table_gradient(hipStream_t stream, const EmbeddingShape &s, const int *keys, const int *positions, const T *dy, float *partial, float scale, float beta, Out *out)
 	{
-		int lanes = 1;
-		while (lanes < 256 && lanes * VEC < s.columns)
-			lanes *= 2;
+		const int lanes = lanes_of_row(s, VEC);
 		const int spans = ceil_div(s.columns, lanes * VEC);
 		const size_t units = static_cast<size_t>(s.classes) * spans;
 		const int most = static_cast<int>(std::min<size_t>(MOST_CLASSES_OF_GROUP, std::max<size_t>(1, units / 2048)));
-		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, scale, beta };
-		if (s.rows >= CHUNK)
+		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk_of(s, VEC), scale, beta };
+		if (s.rows >= p.chunk)
 		{
-			hipLaunchKernelGGL((kernel_chunk_sums<T, Out, VEC>), dim3(ceil_div(s.rows, CHUNK), spans), dim3(256), 0, stream, p);
+			hipLaunchKernelGGL((kernel_chunk_sums<T, Out, VEC>), dim3(ceil_div(s.rows, p.chunk), spans), dim3(256), 0, stream, p);
 			MLHIP_CHECK(hipGetLastError());
 		}
 		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3(static_cast<unsigned int>(ceil_div(s.classes, most)) * spans), dim3(256), 0, stream, p);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	template<typename T, typename Out>
-	void embedding_backward(hipStream_t stream, const EmbeddingShape &s, const int *tokens, const T *dy, float scale, float beta, Out *out, uint8_t *workspace)
+	void embedding_backward(hipStream_t stream, const EmbeddingShape &s, const int *tokens, const T *dy, float scale, float beta, Out *out, const EmbeddingSpace &space, uint8_t *workspace)
 	{
 		constexpr int VEC = 16 / sizeof(T);
 		const int *keys = nullptr, *positions = nullptr;
-		float *partial = reinterpret_cast<float*>(workspace + embedding_space(s).partial);
+		float *partial = reinterpret_cast<float*>(workspace + space.partial);
 		if (s.rows > 0)
-			std::tie(keys, positions) = sort_tokens(stream, s, tokens, workspace);
+			std::tie(keys, positions) = sort_tokens(stream, s, space, tokens, workspace);
 		if (s.columns >= VEC)
 			table_gradient<T, Out, VEC>(stream, s, keys, positions, dy, partial, scale, beta, out);
 		else
@@ -652,7 +705,7 @@ extern "C"
 	size_t hip_embedding_get_workspace_size(mlShape_t tokens_shape, mlShape_t table_shape, mlDataType_t dtype)
 	try
 	{
-		return embedding_space(embedding_shape(tokens_shape, table_shape, dtype, "embedding_get_workspace_size")).total;
+		return embedding_space(embedding_shape(tokens_shape, table_shape, dtype, "embedding_get_workspace_size"), dtype).total;
 	}
 	catch (...)
 	{
@@ -669,18 +722,18 @@ extern "C"
 		check_tokens(tokens, s, name);
 		MLHIP_REQUIRE(rows_of(dy, s), "embedding_backward: there must be a gradient of the table's width for every token");
 		MLHIP_REQUIRE(dtable.dtype == dy.dtype || dtable.dtype == DTYPE_FLOAT32, "embedding_backward: the table's gradient must be of the gradients' type or fp32");
-		const EmbeddingSpace space = embedding_space(s);
+		const EmbeddingSpace space = embedding_space(s, dy.dtype);
 		MLHIP_REQUIRE(space.total == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_size >= space.total),
 				"embedding_backward: the workspace is too small or not aligned to 256 bytes");
 		require_apart( { dtable, Extent(workspace, workspace_size) }, { tokens, dy }, name);
 		const OnDeviceOf on(context);
 		uint8_t *memory = reinterpret_cast<uint8_t*>(workspace);
 		if (dy.dtype == DTYPE_FLOAT32)
-			embedding_backward<float, float>(on.stream, s, ptr<int>(tokens), ptr<float>(dy), scale, beta_weights, ptr<float>(dtable), memory);
+			embedding_backward<float, float>(on.stream, s, ptr<int>(tokens), ptr<float>(dy), scale, beta_weights, ptr<float>(dtable), space, memory);
 		else if (dtable.dtype == DTYPE_FLOAT32)
-			embedding_backward<half_t, float>(on.stream, s, ptr<int>(tokens), ptr<half_t>(dy), scale, beta_weights, ptr<float>(dtable), memory);
+			embedding_backward<half_t, float>(on.stream, s, ptr<int>(tokens), ptr<half_t>(dy), scale, beta_weights, ptr<float>(dtable), space, memory);
 		else
-			embedding_backward<half_t, half_t>(on.stream, s, ptr<int>(tokens), ptr<half_t>(dy), scale, beta_weights, ptr<half_t>(dtable), memory);
+			embedding_backward<half_t, half_t>(on.stream, s, ptr<int>(tokens), ptr<half_t>(dy), scale, beta_weights, ptr<half_t>(dtable), space, memory);
 	}
 	catch (...)
 	{
