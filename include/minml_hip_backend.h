@@ -284,6 +284,20 @@ extern "C"
 	void hip_embedding_backward(mlContext_t context, const mlTensor_t tokens, const mlTensor_t dy, float scale, float beta_weights, mlTensor_t dtable, void *workspace, size_t workspace_size);
 
 	/*
+	 * The distillation of a teacher into a last dense layer over many classes, from the layer's input: x [.., features], w [classes, features], b [classes] or empty as for the cross entropy; the teacher's best `count` classes of
+	 * every row (1 to 1024), int32 [.., count], in any order, and their logits [.., count] of x's type or fp32. With z = (x w^T + b) / temperature, lse = log sum exp z, log p = z[class] - lse and q = softmax(logits / temperature)
+	 * over the row's classes: loss = sum of q (log q - log p), fp32 [..], with lse fp32 [..] and log_probabilities (log p) fp32 [.., count] as the backward pass needs them. A place whose class is none of 0 .. classes - 1 or
+	 * whose logit is -inf does not count, whatever else it holds (log p is 0 there); a class that stands there twice has the sum of both probabilities; a row where nothing counts has loss 0 and no gradient (its lse is given
+	 * all the same; its x has to be finite). Loss and gradients are of the softened distributions: callers that want them multiplied by temperature^2 do so in dloss.
+	 * Backward: dloss fp32 [..] -> dx, dw, db as above, with the gradients of the logits kept as the cross entropy's are. The workspace holds what the cross entropy's does, 16 bytes for every place, and 2 for every row of every tile.
+	 */
+	size_t hip_linear_distillation_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, int count, mlDataType_t dtype, bool backward); /* bytes; the backward pass's is enough for both */
+	void hip_linear_distillation_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t classes, const mlTensor_t logits, float temperature, mlTensor_t loss,
+			mlTensor_t lse, mlTensor_t log_probabilities, void *workspace, size_t workspace_size);
+	void hip_linear_distillation_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t classes, const mlTensor_t logits, float temperature,
+			const mlTensor_t lse, const mlTensor_t log_probabilities, const mlTensor_t dloss, float beta_dx, mlTensor_t dx, float beta_weights, mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size);
+
+	/*
 	 * The clipped policy loss over sampled tokens, fp32 [sequences, tokens] (or [tokens] of one sequence): nll, the negative log likelihoods that hip_linear_cross_entropy_forward gives as its loss; old_nll, what they were when
 	 * the tokens were sampled; reference_nll, those of a model to stay close to, or empty; advantages of every sequence or of every token; targets int32 as for the cross entropy: a token whose target is none of
 	 * 0 .. classes - 1 (prompts, padding) has no part in anything, whatever the other tensors hold for it. With r = exp(old_nll - nll) and q = nll - reference_nll a token's loss is

@@ -127,6 +127,9 @@ SIGNATURES = {
     "embedding_forward": (None, [_vp, _T, _T, _f, _T]),
     "embedding_get_workspace_size": (_sz, [_S, _S, _i]),
     "embedding_backward": (None, [_vp, _T, _T, _f, _f, _T, _vp, _sz]),
+    "linear_distillation_get_workspace_size": (_sz, [_S, _S, _i, _i, _b]),
+    "linear_distillation_forward": (None, [_vp, _T, _T, _T, _T, _T, _f, _T, _T, _T, _vp, _sz]),
+    "linear_distillation_backward": (None, [_vp, _T, _T, _T, _T, _T, _f, _T, _T, _T, _f, _T, _f, _T, _T, _vp, _sz]),
     "policy_loss_get_workspace_size": (_sz, [_S]),
     "policy_loss_forward": (None, [_vp, _T, _T, _T, _T, _T, _i, _d, _d, _f, _i, _T, _T, _vp, _sz]),
     "policy_loss_backward": (None, [_vp, _T, _T, _T, _T, _T, _i, _d, _d, _f, _T, _T, _f, _T]),

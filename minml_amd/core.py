@@ -858,6 +858,44 @@ def embeddingBackward(context, tokens, gradient, scale, beta_weights, gradient_t
     _launch("embedding_backward", context.handle, tokens.desc(), gradient.desc(), scale, beta_weights, gradient_table.desc(), *_space(workspace))
 
 
+def _require_distillation(input, weights, bias, classes, logits, log_probabilities, *fp32):
+    _require(input.dtype in _FLOATS and _same_dtype(input, weights, bias), "dtype mismatch")
+    _require(len(weights.shape) == 2 and len(input.shape) >= 1 and weights.shape[1] == input.shape[-1], "weights must be [classes, features]")
+    _require(bias is None or bias.volume() == weights.shape[0], "bias must be [classes]")
+    lead = tuple(input.shape[:-1])
+    _require(classes.dtype == B.DTYPE_INT32 and len(classes.shape) >= 1 and tuple(classes.shape[:-1]) == lead, "the teacher's classes must be int32 [.., count]")
+    _require(logits.dtype in (input.dtype, B.DTYPE_FLOAT32) and tuple(logits.shape) == tuple(classes.shape), "one logit for every class of the teacher, of the input's type or fp32")
+    _require(log_probabilities.dtype == B.DTYPE_FLOAT32 and tuple(log_probabilities.shape) == tuple(classes.shape), "log probabilities must be fp32 of the teacher's shape")
+    for t in fp32:
+        _require(t.dtype == B.DTYPE_FLOAT32 and tuple(t.shape) == (lead or (1,)), "loss, lse and their gradient must be fp32 with one element per row")
+
+
+def linearDistillationGetWorkspaceSize(context, input, weights, count, backward):
+    """Bytes of workspace (aligned to 256) that linearDistillationForward or, with backward, either of the two needs; count: the teacher's classes of a row."""
+    return B.fn("linear_distillation_get_workspace_size")(input.shape_desc(), weights.shape_desc(), count, input.dtype, bool(backward))
+
+
+def linearDistillationForward(context, input, weights, bias, classes, logits, temperature, loss, lse, log_probabilities, workspace):
+    """loss = sum of q (log q - log p) over the teacher's classes of every row, int32 [.., count], with q = softmax(logits / temperature) over them and p the softmax over all classes of
+    (input weights^T + bias) / temperature: input [.., features], weights [classes, features], bias [classes] or None, logits [.., count], loss and lse fp32 [..] (of a single row [features]: [1]),
+    log_probabilities (log p at the teacher's classes) fp32 [.., count]. A place whose class is none or whose logit is -inf does not count; a row without any that does has loss 0."""
+    _require_distillation(input, weights, bias, classes, logits, log_probabilities, loss, lse)
+    _launch("linear_distillation_forward", context.handle, input.desc(), weights.desc(), _all(bias), classes.desc(), logits.desc(), temperature, loss.desc(), lse.desc(), log_probabilities.desc(),
+            *_space(workspace))
+
+
+def linearDistillationBackward(context, input, weights, bias, classes, logits, temperature, lse, log_probabilities, gradient_loss, beta, gradient_input, beta_weights, gradient_weights, gradient_bias,
+                               workspace):
+    """From the gradient of every row's loss (fp32 [..]) and the forward pass's lse and log_probabilities: gradient_input = its share + beta * gradient_input; gradient_weights and gradient_bias
+    likewise with beta_weights, of the tensors' type or fp32. Each of the three may be None."""
+    _require_distillation(input, weights, bias, classes, logits, log_probabilities, lse, gradient_loss)
+    _require(_same_dtype(input, gradient_input) and (gradient_input is None or tuple(gradient_input.shape) == tuple(input.shape)), "gradient of the input: shape or type")
+    _require_gradient(gradient_weights, weights.volume(), input.dtype, "gradient of the weights")
+    _require_gradient(gradient_bias, weights.shape[0], input.dtype, "gradient of the bias")
+    _launch("linear_distillation_backward", context.handle, input.desc(), weights.desc(), _all(bias), classes.desc(), logits.desc(), temperature, lse.desc(), log_probabilities.desc(),
+            gradient_loss.desc(), beta, _all(gradient_input), beta_weights, _all(gradient_weights), _all(gradient_bias), *_space(workspace))
+
+
 AVERAGES = {"tokens": B.AVERAGE_TOKENS, "sequences": B.AVERAGE_SEQUENCES}
 
 

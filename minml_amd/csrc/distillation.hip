@@ -1,0 +1,598 @@
+/*
+ * distillation.hip — the distillation of a teacher into a last dense layer over many classes, from the layer's input and the teacher's top logits of every row, and its gradients. Neither the logits of the student nor a
+ * distribution over all classes is ever kept.
+ *
+ *   z = (x W^T + b) / t,   lse[i] = log sum_j exp z[i, j],   log p[i, k] = z[i, c[i, k]] - lse[i]
+ *   q[i, k] = softmax over k of v[i, k] / t,   loss[i] = sum_k q[i, k] (log q[i, k] - log p[i, k])
+ *   d[i, j] = (exp(z[i, j] - lse[i]) - sum over k with c[i, k] = j of q[i, k]) dloss[i] / t,   dx = d W,   dW = d^T x,   db[j] = sum_i d[i, j]
+ *
+ * A place k whose class c is none of the layer's, or whose logit v is -inf, does not count; a row without any that does has loss 0 and no gradient. A class that a row names twice has the sum of both probabilities.
+ * The passes are the cross entropy's (vocabulary_loss.hpp). What is new is that a row has many classes of its own, spread over the tiles of logits. A launch before sorts every row's classes and notes where each column of tiles
+ * begins among them; then one thread of a tile has a row's few in that tile, and they meet the logits in LDS, through which the tile goes anyway in the backward pass, and in the forward pass where it has any.
+ * In the backward pass the student's probability at these places is known from the forward pass's log p, so that d there is p - q in fp32, rounded once, however close p and q are.
+ */
+#include "vocabulary_loss.hpp"
+
+#include <cmath>
+
+namespace
+{
+	using namespace mlhip;
+
+	constexpr int MOST_CLASSES_OF_ROW = 1024;
+
+	/* ---- the teacher's classes ---------------------------------------------------------------------------------------------- */
+	/* what a row's classes look like in order */
+	struct Teaching
+	{
+			int *classes; /* [rows][count], ascending; those that do not count behind all others */
+			uint16_t *places; /* [rows][count]: where they stand in the caller's order */
+			float *shares; /* [rows][count]: the class's probability, at its first place if the row names it twice, else 0 */
+			float *known; /* backward, [rows][count]: the student's probability */
+			uint16_t *begins; /* [column tiles + 1][rows]: how many of them lie before a column of tiles */
+			int *anchors; /* [rows]: the class with the largest share, -1 where none counts */
+			float *entropies; /* forward, [rows]: sum of q log q */
+	};
+	template<typename V>
+	__device__ __forceinline__ V lanes_max(V v)
+	{
+#pragma unroll
+		for (int offset = 32; offset >= 1; offset >>= 1)
+			v = max(v, __shfl_xor(v, offset));
+		return v;
+	}
+	/* a wavefront per row. What a class's place is, is counted: as many classes are smaller, or equal and named before. L: type of the logits */
+	template<typename L>
+	__global__ __launch_bounds__(256) void kernel_sort_teacher(const int *classes_in, const L *logits, const float *log_probabilities, int rows, int count, int classes, float temperature, int width, int tiles, Teaching out)
+	{
+		extern __shared__ int memory[];
+		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave;
+		if (row >= rows)
+			return;
+		int *named = memory + wave * 4 * count, *sorted = named + count;
+		float *values = reinterpret_cast<float*>(sorted + count), *shares = values + count;
+		const size_t base = static_cast<size_t>(row) * count;
+		float top = -std::numeric_limits<float>::infinity();
+		int there = 0;
+		for (int k = lane; k < count; k += 64)
+		{
+			const int c = classes_in[base + k];
+			const float v = static_cast<float>(logits[base + k]) / temperature;
+			const bool counts = c >= 0 && c < classes && !(v == -std::numeric_limits<float>::infinity());
+			named[k] = counts ? c : 0x7fffffff;
+			values[k] = v;
+			top = counts ? fmaxf(top, v) : top;
+			there += counts ? 1 : 0;
+		}
+		top = lanes_max(top);
+#pragma unroll
+		for (int offset = 32; offset >= 1; offset >>= 1)
+			there += __shfl_xor(there, offset);
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		float sum = 0.0f;
+		for (int k = lane; k < count; k += 64)
+			if (named[k] != 0x7fffffff)
+			{
+				values[k] = expf(values[k] - top);
+				sum += values[k];
+			}
+		sum = lanes_sum<64>(sum);
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		for (int k = lane; k < count; k += 64)
+		{
+			const int c = named[k];
+			int place = 0;
+			for (int other = 0; other < count; other++)
+				place += named[other] < c + (other < k && c != 0x7fffffff ? 1 : 0) ? 1 : 0;
+			if (c == 0x7fffffff)
+			{
+				place = there;
+				for (int other = 0; other < k; other++)
+					place += named[other] == c ? 1 : 0;
+			}
+			sorted[place] = c;
+			shares[place] = c == 0x7fffffff ? 0.0f : values[k] / sum;
+			out.places[base + place] = static_cast<uint16_t>(k);
+			if (log_probabilities != nullptr)
+				out.known[base + place] = expf(log_probabilities[base + k]);
+		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		float entropy = 0.0f, best = -1.0f;
+		int best_at = there > 0 ? 0 : -1;
+		for (int p = lane; p < count; p += 64)
+		{
+			const int c = sorted[p];
+			float share = 0.0f;
+			if (p < there)
+			{
+				if (p == 0 || sorted[p - 1] != c)
+				{
+					for (int e = p; e < there && sorted[e] == c; e++)
+						share += shares[e];
+					entropy += share > 0.0f ? share * logf(share) : share;
+					if (share > best)
+					{
+						best = share;
+						best_at = p;
+					}
+				}
+			}
+			out.classes[base + p] = c;
+			out.shares[base + p] = share;
+		}
+		entropy = lanes_sum<64>(entropy);
+		const float largest = lanes_max(best);
+		const uint64_t has = __ballot(best == largest && best >= 0.0f);
+		best_at = has != 0 ? __shfl(best_at, __ffsll(static_cast<unsigned long long>(has)) - 1) : best_at;
+		if (lane == 0)
+		{
+			out.anchors[row] = best_at >= 0 ? sorted[best_at] : -1;
+			if (log_probabilities == nullptr)
+				out.entropies[row] = entropy;
+		}
+		for (int t = lane; t <= tiles; t += 64)
+		{
+			const int class_of_tile = t < tiles ? t * width : 0x7fffffff;
+			int first = 0, length = there;
+			while (length > 0)
+			{
+				const int half = length / 2;
+				const bool below = sorted[first + half] < class_of_tile;
+				first = below ? first + half + 1 : first;
+				length = below ? length - half - 1 : half;
+			}
+			out.begins[static_cast<size_t>(t) * rows + row] = static_cast<uint16_t>(first);
+		}
+	}
+
+	/* ---- the goal: several classes of every row ------------------------------------------------------------------------------ */
+	struct TopClasses
+	{
+			static constexpr bool ONE = false;
+			static constexpr int FIXED_BITS = 38;
+			const int *targets; /* none here */
+			const int *classes;
+			const float *shares, *known;
+			const uint16_t *begins; /* from the piece's first column of tiles on */
+			float *logits; /* forward: [rows][count] */
+			int count, all_rows;
+			float slope; /* 1 / t */
+
+			__device__ __forceinline__ void range_of(int tile_n, int m, int &first, int &last) const
+			{
+				first = begins[static_cast<size_t>(tile_n) * all_rows + m];
+				last = begins[static_cast<size_t>(tile_n + 1) * all_rows + m];
+			}
+			template<int BLOCKS>
+			struct Rows
+			{
+					__device__ __forceinline__ void begin(const TopClasses&, int, int, int, int)
+					{
+					}
+					template<typename Columns>
+					__device__ __forceinline__ void take_row(const TopClasses&, int, int, const Columns&, const float (&)[2][16]) const
+					{
+					}
+			};
+			__device__ __forceinline__ float scaled(float z) const
+			{
+				return z * slope;
+			}
+			__device__ __forceinline__ float less(float z, float norm) const
+			{
+				return fmaf(z, slope, -norm);
+			}
+			template<int BM, int BN>
+			static constexpr int loss_lds()
+			{
+				return Stage<float, BN>::bytes(rows_at_a_time(BM));
+			}
+			/* the logits of the rows' classes, through LDS in fp32, a part of the rows at a time */
+			template<int BM, int BN, typename Acc, typename Columns>
+			__device__ __forceinline__ void take_tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const Columns &columns, const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
+			{
+				constexpr int ROWS = rows_at_a_time(BM), BLOCKS = ROWS / 64;
+				typedef Stage<float, BN> TileStage;
+				const TileStage stage { reinterpret_cast<float*>(lds) };
+				const int row = threadIdx.x, m = at.tile_m * BM + row;
+				int first = 0, last = 0;
+				if (row < BM && m < rows)
+					range_of(at.tile_n, m, first, last);
+				if (__syncthreads_or(first < last) == 0)
+					return;
+				static_for<BM / ROWS>([&](auto part)
+				{
+					constexpr int h = decltype(part)::value;
+					if (h > 0)
+						__syncthreads();
+#pragma unroll
+					for (int i = h * BLOCKS; i < (h + 1) * BLOCKS; i++)
+#pragma unroll
+						for (int j = 0; j < 2; j++)
+#pragma unroll
+							for (int q = 0; q < 4; q++)
+							{
+								float z[4];
+#pragma unroll
+								for (int e = 0; e < 4; e++)
+									z[e] = scaled(acc[i][j][4 * q + e] + columns.bias[j][4 * q + e]);
+								stage.put(at.row(i) - h * ROWS, at.column(j) + at.lane_column(q), z[0], z[1], z[2], z[3]);
+							}
+					__syncthreads();
+					if (row >= h * ROWS && row < (h + 1) * ROWS)
+						for (int k = first; k < last; k++)
+						{
+							const size_t place = static_cast<size_t>(m) * count + k;
+							logits[place] = stage.place[(row - h * ROWS) * TileStage::STRIDE + classes[place] - at.tile_n * BN];
+						}
+				});
+			}
+
+			/* behind the tile: what is taken from the sums of the columns, in whole numbers of 2^-38, whose sum no order changes; whether it is no number; what rounding took from the rows beside what the tile's threads counted */
+			template<int BM, int BN>
+			static constexpr int gradient_lds()
+			{
+				return BN * 12 + BM * 4;
+			}
+			template<int BM, int BN>
+			struct Extra
+			{
+					unsigned long long *columns;
+					int *no_number;
+					float *lost;
+					__device__ __forceinline__ explicit Extra(uint8_t *lds) :
+							columns(reinterpret_cast<unsigned long long*>(lds)),
+							no_number(reinterpret_cast<int*>(lds + BN * 8)),
+							lost(reinterpret_cast<float*>(lds + BN * 12))
+					{
+					}
+			};
+			template<int BM, int BN>
+			__device__ __forceinline__ void begin_gradient(uint8_t *lds) const
+			{
+				for (int i = threadIdx.x; i < gradient_lds<BM, BN>() / 4; i += TilePlace<BM, BN>::THREADS)
+					reinterpret_cast<int*>(lds)[i] = 0;
+			}
+			/* the places of the rows' classes in a tile that lies in LDS, written again with p - q instead of p; a thread has a row's, so what rounding takes of them is added up in order */
+			template<int BM, int BN, int ROWS, typename TileStage>
+			__device__ __forceinline__ void correct(const TileStage &stage, uint8_t *lds, const TilePlace<BM, BN> &at, int first_row, int rows, int first_class, int, const float *factors) const
+			{
+				typedef typename std::remove_pointer<decltype(stage.place)>::type T;
+				const Extra<BM, BN> extra(lds);
+				const int row = threadIdx.x, m = at.tile_m * BM + first_row + row;
+				if (row < ROWS && m < rows)
+				{
+					const float factor = factors[m];
+					int first = 0, last = 0;
+					if (factor != 0.0f)
+						range_of(at.tile_n, m, first, last);
+					float taken = 0.0f;
+					int before = -1;
+					for (int k = first; k < last; k++)
+					{
+						const size_t place = static_cast<size_t>(m) * count + k;
+						const int column = classes[place] - first_class - at.tile_n * BN;
+						if (column == before) /* its share is at the class's first place */
+							continue;
+						before = column;
+						const float pf = known[place] * factor, qf = shares[place] * factor, d = pf - qf;
+						T *stored = stage.place + row * TileStage::STRIDE + column;
+						const T rounded = static_cast<T>(d);
+						taken += (d - static_cast<float>(rounded)) - (pf - static_cast<float>(*stored));
+						*stored = rounded;
+						if (fabsf(qf) < std::numeric_limits<float>::infinity())
+							atomicAdd(&extra.columns[column], static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(qf) * static_cast<double>(1ll << FIXED_BITS))));
+						else
+							extra.no_number[column] = 1;
+					}
+					extra.lost[first_row + row] = taken;
+				}
+				__syncthreads();
+			}
+			template<int BM, int BN>
+			__device__ __forceinline__ float column_sum(float sum, uint8_t *lds) const
+			{
+				const Extra<BM, BN> extra(lds);
+				const double taken = static_cast<double>(static_cast<long long>(extra.columns[threadIdx.x])) / static_cast<double>(1ll << FIXED_BITS);
+				return extra.no_number[threadIdx.x] != 0 ? std::numeric_limits<float>::quiet_NaN() : static_cast<float>(static_cast<double>(sum) - taken);
+			}
+			template<int BM, int BN>
+			__device__ __forceinline__ float row_lost(float sum, uint8_t *lds) const
+			{
+				return sum + Extra<BM, BN>(lds).lost[threadIdx.x];
+			}
+	};
+
+	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
+	template<typename T, int MB, bool STREAM>
+	__global__ __launch_bounds__(256) void kernel_distillation_few_rows(const T *x, const T *w, const T *bias, TopClasses goal, int rows, int features, int classes, Partial *partials)
+	{
+		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+		float (*sums)[2][16 * MB][16] = reinterpret_cast<float (*)[2][16 * MB][16]>(lds);
+		const int n0 = blockIdx.x * FEW_CLASSES;
+		const T *first = w + static_cast<size_t>(n0) * features;
+		const bool second = n0 + 16 < classes; /* else the first block stands in for it */
+		const int last_first = min(15, classes - 1 - n0), last_second = second ? min(15, classes - 1 - n0 - 16) : last_first;
+		const T *next = second ? first + static_cast<size_t>(16) * features : first;
+		if constexpr (STREAM)
+			few_rows_stream<T, MB>(x, rows, first, next, last_first, last_second, features, lds);
+		else
+			few_rows_sums<T, MB>(x, rows, first, next, last_first, last_second, features, sums);
+		const int c = threadIdx.x & 15;
+		for (int row = threadIdx.x >> 4; row < 16 * MB; row += 16)
+			if (row < rows)
+			{
+				float z[2];
+				bool there[2];
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+				{
+					const int n = n0 + 16 * i + c;
+					there[i] = n < classes;
+					z[i] = goal.scaled(sums[0][i][row][c] + ((bias != nullptr && there[i]) ? static_cast<float>(bias[n]) : 0.0f));
+				}
+				const Partial p = lanes_join<16>(partial_of(z, there));
+				if (c == 0)
+					partials[static_cast<size_t>(row) * gridDim.x + blockIdx.x] = p;
+				/* 16 threads share a row's classes */
+				int from, to;
+				goal.range_of(blockIdx.x, row, from, to);
+				for (int k = from + c; k < to; k += 16)
+				{
+					const size_t place = static_cast<size_t>(row) * goal.count + k;
+					const int n = goal.classes[place] - n0;
+					goal.logits[place] = goal.scaled(sums[0][n >> 4][row][n & 15] + (bias != nullptr ? static_cast<float>(bias[n0 + n]) : 0.0f));
+				}
+			}
+	}
+	/* as the cross entropy's, then the row's own classes: log p in the caller's order, and the loss */
+	template<int THREADS>
+	__global__ __launch_bounds__(256) void kernel_join_distillation(const Partial *partials, int tiles, const Teaching teaching, const float *logits, int rows, int count, float *loss, float *lse, float *log_probabilities)
+	{
+		__shared__ Partial waves[4];
+		__shared__ float crosses[4];
+		for (int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS; row < rows; row += gridDim.x * (256 / THREADS))
+		{
+			const Partial p = join_row<THREADS>(partials + static_cast<size_t>(row) * tiles, tiles, waves);
+			const float value = p.top + logf(p.sum);
+			const size_t base = static_cast<size_t>(row) * count;
+			const int there = teaching.begins[static_cast<size_t>(tiles) * rows + row];
+			float cross = 0.0f;
+			for (int k = threadIdx.x % THREADS; k < count; k += THREADS)
+			{
+				float log_p = 0.0f;
+				if (k < there)
+				{
+					const float share = teaching.shares[base + k];
+					log_p = logits[base + k] - value;
+					cross += share == 0.0f ? 0.0f : share * log_p;
+				}
+				log_probabilities[base + teaching.places[base + k]] = log_p;
+			}
+			cross = lanes_sum<64>(cross);
+			if constexpr (THREADS > 64)
+			{
+				if ((threadIdx.x & 63) == 0)
+					crosses[threadIdx.x >> 6] = cross;
+				__syncthreads();
+				cross = (crosses[0] + crosses[1]) + (crosses[2] + crosses[3]);
+			}
+			if (threadIdx.x % THREADS == 0)
+			{
+				lse[row] = value;
+				loss[row] = there > 0 ? teaching.entropies[row] - cross : 0.0f;
+			}
+			if (THREADS > 64)
+				return; /* one row, the meeting places are in use */
+		}
+	}
+
+	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
+	struct DistillationSpace
+	{
+			LossSpace loss;
+			size_t classes, places, shares, known, begins, anchors, entropies, logits, total;
+	};
+	int forward_width(const LossShape &s)
+	{
+		return few_rows(s) ? FEW_CLASSES : tile_width(s, s.classes);
+	}
+	DistillationSpace distillation_space(const LossShape &s, int count, bool backward)
+	{
+		DistillationSpace space { };
+		space.loss = loss_space(s, backward);
+		size_t at = space.loss.total;
+		const auto take = [&](size_t bytes)
+		{
+			const size_t begin = at;
+			at += round_up(bytes, 256);
+			return begin;
+		};
+		if (s.rows > 0)
+		{
+			const size_t rows = s.rows, places = rows * count;
+			const size_t forward_tiles = ceil_div(s.classes, forward_width(s)), backward_tiles = ceil_div(s.classes, tile_width(s, classes_of_piece(s)));
+			space.classes = take(sizeof(int) * places);
+			space.places = take(sizeof(uint16_t) * places);
+			space.shares = take(sizeof(float) * places);
+			space.logits = space.known = take(sizeof(float) * places);
+			space.begins = take(sizeof(uint16_t) * rows * ((backward ? std::max(forward_tiles, backward_tiles) : forward_tiles) + 1));
+			space.anchors = take(sizeof(int) * rows);
+			space.entropies = take(sizeof(float) * rows);
+		}
+		space.total = at;
+		return space;
+	}
+	template<typename V>
+	V* at(uint8_t *workspace, size_t offset)
+	{
+		return reinterpret_cast<V*>(workspace + offset);
+	}
+	Teaching teaching_of(uint8_t *workspace, const DistillationSpace &space)
+	{
+		return Teaching { at<int>(workspace, space.classes), at<uint16_t>(workspace, space.places), at<float>(workspace, space.shares), at<float>(workspace, space.known), at<uint16_t>(workspace, space.begins),
+				at<int>(workspace, space.anchors), at<float>(workspace, space.entropies) };
+	}
+	void sort_teacher(hipStream_t stream, const LossShape &s, const mlTensor_t &classes, const mlTensor_t &logits, const float *log_probabilities, int count, float temperature, int width, const Teaching &out)
+	{
+		const int tiles = ceil_div(s.classes, width), bytes = 4 * 4 * static_cast<int>(sizeof(int)) * count;
+		const auto launch = [&](auto kernel, auto values)
+		{
+			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+			hipLaunchKernelGGL(kernel, dim3(ceil_div(s.rows, 4)), dim3(256), bytes, stream, ptr<int>(classes), values, log_probabilities, s.rows, count, s.classes, temperature, width, tiles, out);
+		};
+		if (logits.dtype == DTYPE_FLOAT16)
+			launch(kernel_sort_teacher<half_t>, static_cast<const half_t*>(ptr<half_t>(logits)));
+		else
+			launch(kernel_sort_teacher<float>, static_cast<const float*>(ptr<float>(logits)));
+		MLHIP_CHECK(hipGetLastError());
+	}
+	template<typename T>
+	void distillation_forward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const mlTensor_t &classes, const mlTensor_t &logits, int count, float temperature, float *loss,
+			float *lse, float *log_probabilities, uint8_t *workspace)
+	{
+		const DistillationSpace space = distillation_space(s, count, false);
+		const Teaching teaching = teaching_of(workspace, space);
+		const int width = forward_width(s), columns = ceil_div(s.classes, width);
+		Partial *partials = at<Partial>(workspace, space.loss.partials);
+		sort_teacher(stream, s, classes, logits, nullptr, count, temperature, width, teaching);
+		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, at<float>(workspace, space.logits), count, s.rows, 1.0f / temperature };
+		if (few_rows(s))
+			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto streamed)
+			{
+				constexpr int MB = decltype(blocks)::value, bytes = few_rows_lds<MB>(decltype(streamed)::value);
+				auto kernel = kernel_distillation_few_rows<T, MB, decltype(streamed)::value>;
+				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+				hipLaunchKernelGGL(kernel, dim3(columns), dim3(256), bytes, stream, x, w, bias, goal, s.rows, s.features, s.classes, partials);
+			});
+		else
+		{
+			const int padded = padded_columns<T>(s.features);
+			x = pad_rows(stream, x, at<T>(workspace, space.loss.x), s.rows, s.features);
+			w = pad_rows(stream, w, at<T>(workspace, space.loss.w), s.classes, s.features);
+			const ProductPlan plan = logits_plan(s, s.classes);
+			const Operand a { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), s.rows, padded };
+			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), s.classes, padded };
+			launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, LossEpilogue<T, TopClasses> { bias, goal, partials, s.classes, columns });
+		}
+		MLHIP_CHECK(hipGetLastError());
+		if (s.rows <= 1024)
+			hipLaunchKernelGGL((kernel_join_distillation<256>), dim3(s.rows), dim3(256), 0, stream, partials, columns, teaching, goal.logits, s.rows, count, loss, lse, log_probabilities);
+		else
+			hipLaunchKernelGGL((kernel_join_distillation<64>), dim3(std::min(ceil_div(s.rows, 4), 1 << 20)), dim3(256), 0, stream, partials, columns, teaching, goal.logits, s.rows, count, loss, lse,
+					log_probabilities);
+		MLHIP_CHECK(hipGetLastError());
+	}
+	template<typename T>
+	void distillation_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const mlTensor_t &classes, const mlTensor_t &logits, int count, float temperature, const float *lse,
+			const float *log_probabilities, const float *dloss, float beta_dx, T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, uint8_t *workspace)
+	{
+		const DistillationSpace space = distillation_space(s, count, true);
+		const Teaching teaching = teaching_of(workspace, space);
+		sort_teacher(stream, s, classes, logits, log_probabilities, count, temperature, tile_width(s, classes_of_piece(s)), teaching);
+		const auto goal = [&](int first_tile)
+		{
+			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + static_cast<size_t>(first_tile) * s.rows, nullptr, count, s.rows, 1.0f / temperature };
+		};
+		loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, workspace);
+	}
+
+	/* the rows' shape with another last dimension */
+	bool places_of_rows(const mlTensor_t &t, const LossShape &s, int count)
+	{
+		return t.rank >= 1 && last_dim(t) == count && volume(t) == static_cast<size_t>(s.rows) * count && (s.rows == 0 || t.data != nullptr);
+	}
+	LossShape check_distillation(const mlTensor_t &x, const mlTensor_t &w, const mlTensor_t &b, const mlTensor_t &classes, const mlTensor_t &logits, float temperature, int &count, const char *name)
+	{
+		const std::string who(name);
+		const LossShape s = loss_shape(shape_of(x), shape_of(w), x.dtype, name);
+		MLHIP_REQUIRE(w.dtype == x.dtype, who + ": weights must have the input's type");
+		MLHIP_REQUIRE(b.data == nullptr || (b.dtype == x.dtype && volume(b) == static_cast<size_t>(s.classes)), who + ": the bias must be [classes] of the input's type");
+		count = last_dim(classes);
+		MLHIP_REQUIRE(count >= 1 && count <= MOST_CLASSES_OF_ROW, who + ": the teacher must name 1 to 1024 classes for every row");
+		MLHIP_REQUIRE(classes.dtype == DTYPE_INT32 && places_of_rows(classes, s, count) && reinterpret_cast<uintptr_t>(classes.data) % 4 == 0, who + ": the teacher's classes must be int32, as many for every row");
+		MLHIP_REQUIRE((logits.dtype == x.dtype || logits.dtype == DTYPE_FLOAT32) && places_of_rows(logits, s, count), who + ": there must be one logit of the input's type or fp32 for every class of the teacher");
+		MLHIP_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(1.0f / temperature), who + ": the temperature must be positive and finite");
+		MLHIP_REQUIRE(s.rows == 0 || (x.data != nullptr && w.data != nullptr), who + ": null pointer");
+		MLHIP_REQUIRE(reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && reinterpret_cast<uintptr_t>(w.data) % 16 == 0, who + ": input and weights must be aligned to 16 bytes");
+		return s;
+	}
+}
+
+extern "C"
+{
+	using namespace mlhip;
+
+	size_t hip_linear_distillation_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, int count, mlDataType_t dtype, bool backward)
+	try
+	{
+		const char *name = "linear_distillation_get_workspace_size";
+		MLHIP_REQUIRE(count >= 1 && count <= MOST_CLASSES_OF_ROW, std::string(name) + ": the teacher must name 1 to 1024 classes for every row");
+		const LossShape s = loss_shape(input_shape, weights_shape, dtype, name);
+		/* the forward pass may have the backward pass's workspace */
+		return backward ? std::max(distillation_space(s, count, true).total, distillation_space(s, count, false).total) : distillation_space(s, count, false).total;
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<size_t>();
+	}
+
+	void hip_linear_distillation_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t classes, const mlTensor_t logits, float temperature, mlTensor_t loss,
+			mlTensor_t lse, mlTensor_t log_probabilities, void *workspace, size_t workspace_size)
+	try
+	{
+		const char *name = "linear_distillation_forward";
+		int count;
+		const LossShape s = check_distillation(x, w, b, classes, logits, temperature, count, name);
+		MLHIP_REQUIRE(per_row(loss, s, DTYPE_FLOAT32) && per_row(lse, s, DTYPE_FLOAT32), "linear_distillation_forward: loss and lse must be fp32 with one element per row");
+		MLHIP_REQUIRE(log_probabilities.dtype == DTYPE_FLOAT32 && places_of_rows(log_probabilities, s, count), "linear_distillation_forward: the log probabilities must be fp32, one for every class of the teacher");
+		if (s.rows == 0)
+			return;
+		check_space(workspace, workspace_size, distillation_space(s, count, false).total, name);
+		require_apart( { loss, lse, log_probabilities, Extent(workspace, workspace_size) }, { x, w, b, classes, logits }, name);
+		const OnDeviceOf on(context);
+		if (x.dtype == DTYPE_FLOAT16)
+			distillation_forward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), classes, logits, count, temperature, ptr<float>(loss), ptr<float>(lse), ptr<float>(log_probabilities),
+					reinterpret_cast<uint8_t*>(workspace));
+		else
+			distillation_forward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), classes, logits, count, temperature, ptr<float>(loss), ptr<float>(lse), ptr<float>(log_probabilities),
+					reinterpret_cast<uint8_t*>(workspace));
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+
+	void hip_linear_distillation_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t b, const mlTensor_t classes, const mlTensor_t logits, float temperature,
+			const mlTensor_t lse, const mlTensor_t log_probabilities, const mlTensor_t dloss, float beta_dx, mlTensor_t dx, float beta_weights, mlTensor_t dw, mlTensor_t db, void *workspace, size_t workspace_size)
+	try
+	{
+		const char *name = "linear_distillation_backward";
+		int count;
+		const LossShape s = check_distillation(x, w, b, classes, logits, temperature, count, name);
+		MLHIP_REQUIRE(per_row(lse, s, DTYPE_FLOAT32) && per_row(dloss, s, DTYPE_FLOAT32), "linear_distillation_backward: lse and dloss must be fp32 with one element per row");
+		MLHIP_REQUIRE(log_probabilities.dtype == DTYPE_FLOAT32 && places_of_rows(log_probabilities, s, count), "linear_distillation_backward: the log probabilities must be fp32, one for every class of the teacher");
+		check_gradients(x, w, s, dx, dw, db, name);
+		if (dx.data == nullptr && dw.data == nullptr && db.data == nullptr)
+			return;
+		if (s.rows == 0)
+		{
+			const OnDeviceOf on(context);
+			sums_over_nothing(on.stream, dw, db, beta_weights);
+			return;
+		}
+		check_space(workspace, workspace_size, distillation_space(s, count, true).total, name);
+		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, b, classes, logits, lse, log_probabilities, dloss }, name);
+		const OnDeviceOf on(context);
+		if (x.dtype == DTYPE_FLOAT16)
+			distillation_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), classes, logits, count, temperature, ptr<float>(lse), ptr<float>(log_probabilities), ptr<float>(dloss), beta_dx,
+					ptr<half_t>(dx), beta_weights, dw, db, reinterpret_cast<uint8_t*>(workspace));
+		else
+			distillation_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), classes, logits, count, temperature, ptr<float>(lse), ptr<float>(log_probabilities), ptr<float>(dloss), beta_dx,
+					ptr<float>(dx), beta_weights, dw, db, reinterpret_cast<uint8_t*>(workspace));
+	}
+	catch (...)
+	{
+		return mlhip::entry_failed<void>();
+	}
+}

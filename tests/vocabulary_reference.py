@@ -1,7 +1,7 @@
 """What a model over a vocabulary learns from, in 64 bits and straight from the definitions, and bounds of what rounding may do to it."""
 import numpy as np
 
-from training_reference import FP32, rounded
+from training_reference import FP32, STEP, TINY, product_error, rounded
 
 
 def embedding(tokens, table, scale):
@@ -61,3 +61,76 @@ def policy(nll, old, reference, advantages, targets, classes, clip, kl_weight, a
     size = np.array([abs(parts[1]) + kl_weight * parts[2]] + [abs(v) for v in parts[1:]])
     gradient_off = each * (gain_off + kl_weight * slope_off) + 6 * FP32 * each * (np.abs(free) + kl_weight * np.abs(slope))
     return (parts, weights, gradient), (off + 4 * FP32 * size + 1e-14, 2 * FP32 * weights, gradient_off + 2.0 ** -140)
+
+
+def teacher(classes, logits, total, temperature):
+    """The teacher's distribution over all classes [rows, total], that of every place [rows, count], and which places count."""
+    kept = (classes >= 0) & (classes < total) & ~np.isneginf(logits)
+    with np.errstate(invalid="ignore", over="ignore"):
+        v = np.where(kept, logits / temperature, -np.inf)
+        top = v.max(1, keepdims=True)
+        q = np.where(kept, np.exp(v - np.where(np.isfinite(top), top, 0)), 0)
+    q = q / np.where(kept.any(1), q.sum(1), 1)[:, None]
+    dense = np.zeros((len(classes), total))
+    np.add.at(dense, (np.nonzero(kept)[0], classes[kept]), q[kept])
+    return dense, q, kept
+
+
+def distillation(x, w, b, classes, logits, temperature):
+    """loss, lse, log p at the teacher's classes, and the scaled logits."""
+    z = (x @ w.T + b) / temperature
+    top = z.max(1, keepdims=True)
+    lse = top[:, 0] + np.log(np.exp(z - top).sum(1))
+    dense, _, kept = teacher(classes, logits, len(w), temperature)
+    log_p = z - lse[:, None]
+    loss = np.where(dense > 0, dense * (np.log(np.where(dense > 0, dense, 1)) - log_p), 0).sum(1)
+    return loss, lse, np.where(kept, np.take_along_axis(log_p, np.where(kept, classes, 0), 1), 0), z
+
+
+def share_error(classes, logits, total, temperature):
+    """How far a probability of the teacher may be off, relative to it: the exponent's two numbers are rounded, the exponential is a step off, then a sum of `count` and a division."""
+    _, _, kept = teacher(classes, logits, total, temperature)
+    return FP32 * (4 * np.abs(np.where(kept, logits, 0) / temperature).max(1) + 24 + classes.shape[1] / 32)
+
+
+def scaled_logit_error(x, w, b, z, temperature, dtype):
+    return (product_error(x, w.T, dtype) + FP32 * np.abs(temperature * z)) / temperature + 3 * FP32 * np.abs(z)
+
+
+def distillation_bounds(x, w, b, classes, logits, temperature, dtype):
+    """As the cross entropy's; the loss is a mean over the teacher's probabilities, whose own errors it takes times what they weigh."""
+    loss, lse, log_p, z = distillation(x, w, b, classes, logits, temperature)
+    dense, q, kept = teacher(classes, logits, len(w), temperature)
+    off = scaled_logit_error(x, w, b, z, temperature, dtype)
+    off_lse = off.max(1) + 42 * 2.0 ** -22 + 200 * FP32 + 2 * FP32 * np.abs(lse)
+    off_p = np.where(kept, np.take_along_axis(off, np.where(kept, classes, 0), 1) + off_lse[:, None] + FP32 * np.abs(log_p), 0)
+    log_q = np.log(np.where(dense > 0, dense, 1))
+    weighed = dense * (np.abs(log_q) + np.abs(z - lse[:, None]))
+    relative = share_error(classes, logits, len(w), temperature)
+    return (q * off_p).sum(1) + (relative + (classes.shape[1] / 32 + 20) * FP32) * (weighed.sum(1) + 1) + FP32 * np.abs(loss), off_lse, off_p
+
+
+def distillation_gradients(x, w, b, classes, logits, temperature, dloss):
+    z, lse = distillation(x, w, b, classes, logits, temperature)[3], distillation(x, w, b, classes, logits, temperature)[1]
+    dense, _, kept = teacher(classes, logits, len(w), temperature)
+    d = (np.exp(z - lse[:, None]) - dense) * np.where(kept.any(1), dloss, 0)[:, None] / temperature
+    return d @ w, d.T @ x, d.sum(0)
+
+
+def distillation_gradient_bounds(x, w, b, classes, logits, temperature, dloss, dtype):
+    """dx in fp16: with e_j what rounding takes from d_j, and -sum e_j given back to the class a with the teacher's largest share, it is off by sum e_j W_j - (sum e_j) W_a = sum over j other than a of
+    e_j (W_j - W_a), so by |e_j| (|W_j| + |W_a|) for each of them at most: the sums of d's errors with |W|, and their sum for the row times |W_a|."""
+    _, lse, _, z = distillation(x, w, b, classes, logits, temperature)
+    dense, _, kept = teacher(classes, logits, len(w), temperature)
+    weight = np.where(kept.any(1), np.abs(dloss), 0)[:, None] / temperature
+    about = z - lse[:, None]
+    p = np.exp(about)
+    exponent = scaled_logit_error(x, w, b, z, temperature, dtype) + distillation_bounds(x, w, b, classes, logits, temperature, dtype)[1][:, None] + (np.abs(about) + 4) * 2.0 ** -22
+    off = weight * (p * np.expm1(np.minimum(exponent, 1)) + 4 * FP32 * (p + 1e-30) + dense * (share_error(classes, logits, len(w), temperature)[:, None] + 4 * FP32))
+    d = np.abs(p - dense) * weight
+    # d is kept in the tensors' type, times 2^15 over a power of two that is at most twice the largest |dloss|
+    stored = off + STEP[dtype] * d + TINY[dtype] * 2.0 ** -14 * weight.max(initial=0)
+    given_back = stored.sum(1, keepdims=True) * np.abs(w[dense.argmax(1)]) if dtype == "float16" else 0
+    dx, dw, db = distillation_gradients(x, w, b, classes, logits, temperature, dloss)
+    return (rounded(dx, dtype) + product_error(d, w, dtype) + stored @ np.abs(w) + given_back, rounded(dw, dtype) + product_error(d.T, x, dtype) + stored.T @ np.abs(x),
+            rounded(db, dtype) + off.sum(0) + (x.shape[0] + 80) * FP32 * (weight * (p + dense)).sum(0))
