@@ -29,7 +29,7 @@ namespace
 			uint16_t *places; /* [rows][count]: where they stand in the caller's order */
 			float *shares; /* [rows][count]: the class's probability, at its first place if the row names it twice, else 0 */
 			float *known; /* backward, [rows][count]: the student's probability */
-			uint16_t *begins; /* [column tiles + 1][rows]: how many of them lie before a column of tiles */
+			uint16_t *begins; /* [rows][column tiles + 1]: how many of them lie before a column of tiles */
 			int *anchors; /* [rows]: the class with the largest share, -1 where none counts */
 			float *entropies; /* forward, [rows]: sum of q log q */
 	};
@@ -82,6 +82,7 @@ namespace
 		{
 			const int c = named[k];
 			int place = 0;
+#pragma unroll 8
 			for (int other = 0; other < count; other++)
 				place += named[other] < c + (other < k && c != 0x7fffffff ? 1 : 0) ? 1 : 0;
 			if (c == 0x7fffffff)
@@ -130,18 +131,27 @@ namespace
 			if (log_probabilities == nullptr)
 				out.entropies[row] = entropy;
 		}
-		for (int t = lane; t <= tiles; t += 64)
+		/* several columns of tiles at a time, by halves of the row's classes: no read of LDS waits for another column's */
+		constexpr int AT_A_TIME = 8;
+		for (int t0 = lane; t0 <= tiles; t0 += 64 * AT_A_TIME)
 		{
-			const int class_of_tile = t < tiles ? t * width : 0x7fffffff;
-			int first = 0, length = there;
-			while (length > 0)
-			{
-				const int half = length / 2;
-				const bool below = sorted[first + half] < class_of_tile;
-				first = below ? first + half + 1 : first;
-				length = below ? length - half - 1 : half;
-			}
-			out.begins[static_cast<size_t>(t) * rows + row] = static_cast<uint16_t>(first);
+			int first[AT_A_TIME];
+#pragma unroll
+			for (int u = 0; u < AT_A_TIME; u++)
+				first[u] = 0;
+			for (int step = MOST_CLASSES_OF_ROW; step > 0; step >>= 1)
+				if (step <= there)
+#pragma unroll
+					for (int u = 0; u < AT_A_TIME; u++)
+					{
+						const int t = t0 + 64 * u, next = first[u] + step;
+						const bool below = sorted[min(next, there) - 1] < (t < tiles ? t * width : 0x7fffffff);
+						first[u] = next <= there && below ? next : first[u];
+					}
+#pragma unroll
+			for (int u = 0; u < AT_A_TIME; u++)
+				if (t0 + 64 * u <= tiles)
+					out.begins[static_cast<size_t>(row) * (tiles + 1) + t0 + 64 * u] = static_cast<uint16_t>(first[u]);
 		}
 	}
 
@@ -155,13 +165,14 @@ namespace
 			const float *shares, *known;
 			const uint16_t *begins; /* from the piece's first column of tiles on */
 			float *logits; /* forward: [rows][count] */
-			int count, all_rows;
+			int count, stride; /* stride: of begins */
 			float slope; /* 1 / t */
 
 			__device__ __forceinline__ void range_of(int tile_n, int m, int &first, int &last) const
 			{
-				first = begins[static_cast<size_t>(tile_n) * all_rows + m];
-				last = begins[static_cast<size_t>(tile_n + 1) * all_rows + m];
+				const uint16_t *of_row = begins + static_cast<size_t>(m) * stride + tile_n;
+				first = of_row[0];
+				last = of_row[1];
 			}
 			template<int BLOCKS>
 			struct Rows
@@ -304,8 +315,9 @@ namespace
 	};
 
 	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
+	/* few rows: all their logits are kept, which is little beside the weights (at most 64 of them), and whoever joins the tiles' sums finds the teacher's classes there */
 	template<typename T, int MB, bool STREAM>
-	__global__ __launch_bounds__(256) void kernel_distillation_few_rows(const T *x, const T *w, const T *bias, TopClasses goal, int rows, int features, int classes, Partial *partials)
+	__global__ __launch_bounds__(256) void kernel_distillation_few_rows(const T *x, const T *w, const T *bias, int rows, int features, int classes, float slope, Partial *partials, float *logits)
 	{
 		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 		float (*sums)[2][16 * MB][16] = reinterpret_cast<float (*)[2][16 * MB][16]>(lds);
@@ -329,21 +341,90 @@ namespace
 				{
 					const int n = n0 + 16 * i + c;
 					there[i] = n < classes;
-					z[i] = goal.scaled(sums[0][i][row][c] + ((bias != nullptr && there[i]) ? static_cast<float>(bias[n]) : 0.0f));
+					z[i] = slope * (sums[0][i][row][c] + ((bias != nullptr && there[i]) ? static_cast<float>(bias[n]) : 0.0f));
+					if (there[i])
+						logits[static_cast<size_t>(row) * classes + n] = z[i];
 				}
 				const Partial p = lanes_join<16>(partial_of(z, there));
 				if (c == 0)
 					partials[static_cast<size_t>(row) * gridDim.x + blockIdx.x] = p;
-				/* 16 threads share a row's classes */
-				int from, to;
-				goal.range_of(blockIdx.x, row, from, to);
-				for (int k = from + c; k < to; k += 16)
-				{
-					const size_t place = static_cast<size_t>(row) * goal.count + k;
-					const int n = goal.classes[place] - n0;
-					goal.logits[place] = goal.scaled(sums[0][n >> 4][row][n & 15] + (bias != nullptr ? static_cast<float>(bias[n0 + n]) : 0.0f));
-				}
 			}
+	}
+	/*
+	 * A workgroup to a row: lse, log p, and the loss with the teacher's probabilities made here. Of a class that stands there twice every place counts its own probability times the logarithm of their sum, which adds up to the
+	 * same as the sum times its logarithm.
+	 */
+	template<typename L>
+	__global__ __launch_bounds__(256) void kernel_join_few_rows(const Partial *partials, int tiles, const int *classes_in, const L *taught, const float *logits, int count, int classes, float temperature, float *loss,
+			float *lse, float *log_probabilities)
+	{
+		__shared__ Partial waves[4];
+		__shared__ float numbers[4];
+		__shared__ int named[MOST_CLASSES_OF_ROW];
+		__shared__ float shares[MOST_CLASSES_OF_ROW];
+		const size_t row = blockIdx.x, base = row * count;
+		float top = -std::numeric_limits<float>::infinity();
+		for (int k = threadIdx.x; k < count; k += 256)
+		{
+			const int c = classes_in[base + k];
+			const float v = static_cast<float>(taught[base + k]) / temperature;
+			const bool counts = c >= 0 && c < classes && !(v == -std::numeric_limits<float>::infinity());
+			named[k] = counts ? c : -1;
+			shares[k] = v;
+			top = counts ? fmaxf(top, v) : top;
+		}
+		const Partial p = join_row<256>(partials + row * tiles, tiles, waves);
+		const float value = p.top + logf(p.sum);
+		const auto of_all = [&](float v, auto &&join)
+		{
+#pragma unroll
+			for (int offset = 32; offset >= 1; offset >>= 1)
+				v = join(v, __shfl_xor(v, offset));
+			__syncthreads();
+			if ((threadIdx.x & 63) == 0)
+				numbers[threadIdx.x >> 6] = v;
+			__syncthreads();
+			return join(join(numbers[0], numbers[1]), join(numbers[2], numbers[3]));
+		};
+		const auto add = [](float a, float b)
+		{
+			return a + b;
+		};
+		top = of_all(top, [](float a, float b)
+		{
+			return fmaxf(a, b);
+		});
+		float sum = 0.0f;
+		for (int k = threadIdx.x; k < count; k += 256)
+			if (named[k] >= 0)
+			{
+				shares[k] = expf(shares[k] - top);
+				sum += shares[k];
+			}
+		sum = of_all(sum, add); /* behind its barriers every share is there for all */
+		float divergence = 0.0f;
+		for (int k = threadIdx.x; k < count; k += 256)
+		{
+			const int c = named[k];
+			float log_p = 0.0f;
+			if (c >= 0)
+			{
+				float together = 0.0f;
+#pragma unroll 8
+				for (int other = 0; other < count; other++)
+					together += named[other] == c ? shares[other] : 0.0f;
+				log_p = logits[row * classes + c] - value;
+				const float share = shares[k] / sum;
+				divergence += share == 0.0f ? 0.0f : share * (logf(together / sum) - log_p);
+			}
+			log_probabilities[base + k] = log_p;
+		}
+		divergence = of_all(divergence, add);
+		if (threadIdx.x == 0)
+		{
+			lse[row] = value;
+			loss[row] = divergence;
+		}
 	}
 	/* as the cross entropy's, then the row's own classes: log p in the caller's order, and the loss */
 	template<int THREADS>
@@ -356,7 +437,7 @@ namespace
 			const Partial p = join_row<THREADS>(partials + static_cast<size_t>(row) * tiles, tiles, waves);
 			const float value = p.top + logf(p.sum);
 			const size_t base = static_cast<size_t>(row) * count;
-			const int there = teaching.begins[static_cast<size_t>(tiles) * rows + row];
+			const int there = teaching.begins[static_cast<size_t>(row) * (tiles + 1) + tiles];
 			float cross = 0.0f;
 			for (int k = threadIdx.x % THREADS; k < count; k += THREADS)
 			{
@@ -393,10 +474,6 @@ namespace
 			LossSpace loss;
 			size_t classes, places, shares, known, begins, anchors, entropies, logits, total;
 	};
-	int forward_width(const LossShape &s)
-	{
-		return few_rows(s) ? FEW_CLASSES : tile_width(s, s.classes);
-	}
 	DistillationSpace distillation_space(const LossShape &s, int count, bool backward)
 	{
 		DistillationSpace space { };
@@ -408,15 +485,16 @@ namespace
 			at += round_up(bytes, 256);
 			return begin;
 		};
-		if (s.rows > 0)
+		const size_t rows = s.rows, places = rows * count;
+		if (s.rows > 0 && !backward && few_rows(s))
+			space.logits = take(sizeof(float) * rows * s.classes);
+		else if (s.rows > 0)
 		{
-			const size_t rows = s.rows, places = rows * count;
-			const size_t forward_tiles = ceil_div(s.classes, forward_width(s)), backward_tiles = ceil_div(s.classes, tile_width(s, classes_of_piece(s)));
 			space.classes = take(sizeof(int) * places);
 			space.places = take(sizeof(uint16_t) * places);
 			space.shares = take(sizeof(float) * places);
 			space.logits = space.known = take(sizeof(float) * places);
-			space.begins = take(sizeof(uint16_t) * rows * ((backward ? std::max(forward_tiles, backward_tiles) : forward_tiles) + 1));
+			space.begins = take(sizeof(uint16_t) * rows * (ceil_div(s.classes, tile_width(s, backward ? classes_of_piece(s) : s.classes)) + 1));
 			space.anchors = take(sizeof(int) * rows);
 			space.entropies = take(sizeof(float) * rows);
 		}
@@ -452,34 +530,45 @@ namespace
 			float *lse, float *log_probabilities, uint8_t *workspace)
 	{
 		const DistillationSpace space = distillation_space(s, count, false);
-		const Teaching teaching = teaching_of(workspace, space);
-		const int width = forward_width(s), columns = ceil_div(s.classes, width);
 		Partial *partials = at<Partial>(workspace, space.loss.partials);
-		sort_teacher(stream, s, classes, logits, nullptr, count, temperature, width, teaching);
-		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, at<float>(workspace, space.logits), count, s.rows, 1.0f / temperature };
+		float *kept = at<float>(workspace, space.logits);
 		if (few_rows(s))
+		{
+			const int columns = ceil_div(s.classes, FEW_CLASSES);
 			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto streamed)
 			{
 				constexpr int MB = decltype(blocks)::value, bytes = few_rows_lds<MB>(decltype(streamed)::value);
 				auto kernel = kernel_distillation_few_rows<T, MB, decltype(streamed)::value>;
 				ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
-				hipLaunchKernelGGL(kernel, dim3(columns), dim3(256), bytes, stream, x, w, bias, goal, s.rows, s.features, s.classes, partials);
+				hipLaunchKernelGGL(kernel, dim3(columns), dim3(256), bytes, stream, x, w, bias, s.rows, s.features, s.classes, 1.0f / temperature, partials, kept);
 			});
-		else
-		{
-			const int padded = padded_columns<T>(s.features);
-			x = pad_rows(stream, x, at<T>(workspace, space.loss.x), s.rows, s.features);
-			w = pad_rows(stream, w, at<T>(workspace, space.loss.w), s.classes, s.features);
-			const ProductPlan plan = logits_plan(s, s.classes);
-			const Operand a { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), s.rows, padded };
-			const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), s.classes, padded };
-			launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, LossEpilogue<T, TopClasses> { bias, goal, partials, s.classes, columns });
+			MLHIP_CHECK(hipGetLastError());
+			const auto join = [&](auto kernel, auto taught)
+			{
+				hipLaunchKernelGGL(kernel, dim3(s.rows), dim3(256), 0, stream, partials, columns, ptr<int>(classes), taught, kept, count, s.classes, temperature, loss, lse, log_probabilities);
+			};
+			if (logits.dtype == DTYPE_FLOAT16)
+				join(kernel_join_few_rows<half_t>, static_cast<const half_t*>(ptr<half_t>(logits)));
+			else
+				join(kernel_join_few_rows<float>, static_cast<const float*>(ptr<float>(logits)));
+			MLHIP_CHECK(hipGetLastError());
+			return;
 		}
+		const Teaching teaching = teaching_of(workspace, space);
+		const int width = tile_width(s, s.classes), columns = ceil_div(s.classes, width), padded = padded_columns<T>(s.features);
+		sort_teacher(stream, s, classes, logits, nullptr, count, temperature, width, teaching);
+		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, kept, count, columns + 1, 1.0f / temperature };
+		x = pad_rows(stream, x, at<T>(workspace, space.loss.x), s.rows, s.features);
+		w = pad_rows(stream, w, at<T>(workspace, space.loss.w), s.classes, s.features);
+		const ProductPlan plan = logits_plan(s, s.classes);
+		const Operand a { reinterpret_cast<const uint8_t*>(x), padded * sizeof(T), s.rows, padded };
+		const Operand b { reinterpret_cast<const uint8_t*>(w), padded * sizeof(T), s.classes, padded };
+		launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, LossEpilogue<T, TopClasses> { bias, goal, partials, s.classes, columns });
 		MLHIP_CHECK(hipGetLastError());
 		if (s.rows <= 1024)
-			hipLaunchKernelGGL((kernel_join_distillation<256>), dim3(s.rows), dim3(256), 0, stream, partials, columns, teaching, goal.logits, s.rows, count, loss, lse, log_probabilities);
+			hipLaunchKernelGGL((kernel_join_distillation<256>), dim3(s.rows), dim3(256), 0, stream, partials, columns, teaching, kept, s.rows, count, loss, lse, log_probabilities);
 		else
-			hipLaunchKernelGGL((kernel_join_distillation<64>), dim3(std::min(ceil_div(s.rows, 4), 1 << 20)), dim3(256), 0, stream, partials, columns, teaching, goal.logits, s.rows, count, loss, lse,
+			hipLaunchKernelGGL((kernel_join_distillation<64>), dim3(std::min(ceil_div(s.rows, 4), 1 << 20)), dim3(256), 0, stream, partials, columns, teaching, kept, s.rows, count, loss, lse,
 					log_probabilities);
 		MLHIP_CHECK(hipGetLastError());
 	}
@@ -489,10 +578,11 @@ namespace
 	{
 		const DistillationSpace space = distillation_space(s, count, true);
 		const Teaching teaching = teaching_of(workspace, space);
-		sort_teacher(stream, s, classes, logits, log_probabilities, count, temperature, tile_width(s, classes_of_piece(s)), teaching);
+		const int width = tile_width(s, classes_of_piece(s)), tiles = ceil_div(s.classes, width);
+		sort_teacher(stream, s, classes, logits, log_probabilities, count, temperature, width, teaching);
 		const auto goal = [&](int first_tile)
 		{
-			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + static_cast<size_t>(first_tile) * s.rows, nullptr, count, s.rows, 1.0f / temperature };
+			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + first_tile, nullptr, count, tiles + 1, 1.0f / temperature };
 		};
 		loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, workspace);
 	}

@@ -19,29 +19,38 @@ namespace
 	using namespace mlhip;
 
 	/* ---- forward ------------------------------------------------------------------------------------------------------------ */
-	template<typename T, int VEC>
+	/* EACH vectors of a thread, on their way at once */
+	template<typename T, int VEC, int EACH>
 	__global__ __launch_bounds__(256) void kernel_embedding_forward(const int *tokens, const T *table, T *y, int rows, int columns, int classes, int vectors, float scale)
 	{
 		const size_t count = static_cast<size_t>(rows) * vectors;
-		for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<size_t>(gridDim.x) * 256)
+		for (size_t first = static_cast<size_t>(blockIdx.x) * 256 * EACH + threadIdx.x; first < count; first += static_cast<size_t>(gridDim.x) * 256 * EACH)
 		{
-			int vector;
-			const size_t row = split_index(i, vectors, vector);
-			const RowPlace place = place_in_row<VEC>(vector * VEC, columns);
-			const int token = tokens[row];
-			float v[VEC];
+			size_t row[EACH];
+			int token[EACH];
+			RowPlace place[EACH];
+			Elements<T, VEC> of_table[EACH];
 #pragma unroll
-			for (int e = 0; e < VEC; e++)
-				v[e] = 0.0f;
-			if (token >= 0 && token < classes)
+			for (int u = 0; u < EACH; u++)
 			{
-				Elements<T, VEC> of_table;
-				of_table.load(place.in(table + static_cast<size_t>(token) * columns));
-#pragma unroll
-				for (int e = 0; e < VEC; e++)
-					v[e] = scale * of_table[e];
+				int vector;
+				row[u] = split_index(min(first + u * 256, count - 1), vectors, vector);
+				place[u] = place_in_row<VEC>(vector * VEC, columns);
+				token[u] = tokens[row[u]];
 			}
-			store_nearest<VEC>(place.in(y + row * columns), v, place.skip);
+#pragma unroll
+			for (int u = 0; u < EACH; u++)
+				of_table[u].load(place[u].in(table + static_cast<size_t>(token[u] >= 0 && token[u] < classes ? token[u] : 0) * columns));
+#pragma unroll
+			for (int u = 0; u < EACH; u++)
+				if (first + u * 256 < count)
+				{
+					float v[VEC];
+#pragma unroll
+					for (int e = 0; e < VEC; e++)
+						v[e] = token[u] >= 0 && token[u] < classes ? scale * of_table[u][e] : 0.0f;
+					store_nearest<VEC>(place[u].in(y + row[u] * columns), v, place[u].skip);
+				}
 		}
 	}
 
@@ -592,8 +601,16 @@ namespace
 	void embedding_forward(hipStream_t stream, const EmbeddingShape &s, const int *tokens, const T *table, T *y, float scale)
 	{
 		const int vectors = ceil_div(s.columns, VEC);
-		const size_t groups = std::min<size_t>((static_cast<size_t>(s.rows) * vectors + 255) / 256, 1 << 20);
-		hipLaunchKernelGGL((kernel_embedding_forward<T, VEC>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, tokens, table, y, s.rows, s.columns, s.classes, vectors, scale);
+		const size_t count = static_cast<size_t>(s.rows) * vectors;
+		const auto launch = [&](auto kernel, int each)
+		{
+			const size_t groups = std::min<size_t>((count + 256 * each - 1) / (256 * each), 1 << 20);
+			hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, tokens, table, y, s.rows, s.columns, s.classes, vectors, scale);
+		};
+		if (count < (1 << 19))
+			launch(kernel_embedding_forward<T, VEC, 1>, 1);
+		else
+			launch(kernel_embedding_forward<T, VEC, 4>, 4);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	/* the tokens in order: keys and positions */

@@ -134,6 +134,45 @@ namespace
 	{
 		return s.count > 0.0 ? Sums { s.gain / s.count, s.kl / s.count, s.clipped / s.count, 1.0 } : Sums { 0.0, 0.0, 0.0, 0.0 };
 	}
+	/* the loss of all means, by one thread */
+	__device__ __forceinline__ void write_loss(const Sums &total, double each, float kl_weight, float *loss)
+	{
+		const double gain = total.gain * each, kl = total.kl * each;
+		loss[0] = static_cast<float>(kl_weight * kl - gain);
+		loss[1] = static_cast<float>(-gain);
+		loss[2] = static_cast<float>(kl);
+		loss[3] = static_cast<float>(total.clipped * each);
+	}
+	/* what a token of a sequence counts */
+	__device__ __forceinline__ float weight_of_sequence(double count, double each, bool average_sequences)
+	{
+		return static_cast<float>(count > 0.0 ? (average_sequences ? each / count : each) : 0.0);
+	}
+	/* of the tokens [begin, end) of a sequence those of one of LANES threads */
+	template<int LANES, int VEC>
+	__device__ __forceinline__ Sums sums_of_thread(const PolicyArgs &p, int sequence, int begin, int end)
+	{
+		Sums sums { 0.0, 0.0, 0.0, 0.0 };
+		int clipped = 0, count = 0;
+		for (int i = begin + (static_cast<int>(threadIdx.x) % LANES) * VEC; i < end; i += LANES * VEC)
+		{
+			Tokens<VEC> tokens;
+			tokens.load(p, sequence, i);
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				if (tokens.there(p, e))
+				{
+					const TokenLoss t = tokens.loss(p, e);
+					sums.gain += static_cast<double>(t.gain);
+					sums.kl += static_cast<double>(t.kl);
+					clipped += t.clipped ? 1 : 0;
+					count++;
+				}
+		}
+		sums.clipped = clipped;
+		sums.count = count;
+		return sums;
+	}
 	/*
 	 * Sums of the workgroups. Whole sequences by LANES threads each, `sequences_of_group` by a workgroup (chunk_length 0), or a workgroup for every chunk_length tokens of a sequence (gridDim.y of them).
 	 * counts: tokens of every sequence, where they are whole
@@ -150,26 +189,7 @@ namespace
 			const int sequence = s0 + static_cast<int>(threadIdx.x) / LANES;
 			Sums sums { 0.0, 0.0, 0.0, 0.0 };
 			if (sequence < last)
-			{
-				int clipped = 0, count = 0;
-				for (int i = begin + (static_cast<int>(threadIdx.x) % LANES) * VEC; i < end; i += LANES * VEC)
-				{
-					Tokens<VEC> tokens;
-					tokens.load(p, sequence, i);
-#pragma unroll
-					for (int e = 0; e < VEC; e++)
-						if (tokens.there(p, e))
-						{
-							const TokenLoss t = tokens.loss(p, e);
-							sums.gain += static_cast<double>(t.gain);
-							sums.kl += static_cast<double>(t.kl);
-							clipped += t.clipped ? 1 : 0;
-							count++;
-						}
-				}
-				sums.clipped = clipped;
-				sums.count = count;
-			}
+				sums = sums_of_thread<LANES, VEC>(p, sequence, begin, end);
 			if constexpr (LANES == 256)
 				sums = group_sum(sums, waves);
 			else
@@ -213,18 +233,43 @@ namespace
 		total = group_sum(total, waves);
 		const double each = total.count > 0.0 ? 1.0 / total.count : 0.0;
 		if (blockIdx.x == 0 && threadIdx.x == 0)
-		{
-			const double gain = total.gain * each, kl = total.kl * each;
-			loss[0] = static_cast<float>(kl_weight * kl - gain);
-			loss[1] = static_cast<float>(-gain);
-			loss[2] = static_cast<float>(kl);
-			loss[3] = static_cast<float>(total.clipped * each);
-		}
+			write_loss(total, each, kl_weight, loss);
 		for (int s = blockIdx.x * 256 + threadIdx.x; s < sequences; s += gridDim.x * 256)
 		{
 			const double count = chunks > 0 ? of_sequence(s).count : static_cast<double>(counts[s]);
-			weights[s] = static_cast<float>(count > 0.0 ? (average_sequences ? each / count : each) : 0.0);
+			weights[s] = weight_of_sequence(count, each, average_sequences);
 		}
+	}
+
+	/* few tokens: everything by one workgroup, a wavefront to a sequence */
+	constexpr int FEW_TOKENS = 8192, FEW_SEQUENCES = 256;
+	template<int VEC>
+	__global__ __launch_bounds__(1024) void kernel_policy_few(PolicyArgs p, bool average_sequences, float *loss, float *weights)
+	{
+		constexpr int WAVES = 16;
+		__shared__ Sums waves[WAVES];
+		__shared__ int counts[FEW_SEQUENCES];
+		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+		Sums total { 0.0, 0.0, 0.0, 0.0 };
+		for (int s = wave; s < p.sequences; s += WAVES)
+		{
+			Sums sums = lanes_sum<64>(sums_of_thread<64, VEC>(p, s, 0, p.length));
+			if (lane == 0)
+				counts[s] = static_cast<int>(sums.count);
+			total = total + (average_sequences ? mean_of_sequence(sums) : sums);
+		}
+		if (lane == 0)
+			waves[wave] = total;
+		__syncthreads();
+		total = waves[0];
+#pragma unroll
+		for (int w = 1; w < WAVES; w++)
+			total = total + waves[w];
+		const double each = total.count > 0.0 ? 1.0 / total.count : 0.0;
+		if (threadIdx.x == 0)
+			write_loss(total, each, p.kl_weight, loss);
+		for (int s = threadIdx.x; s < p.sequences; s += 64 * WAVES)
+			weights[s] = weight_of_sequence(counts[s], each, average_sequences);
 	}
 
 	/* dnll = dloss * weight of the sequence * slope + beta dnll */
@@ -271,7 +316,7 @@ namespace
 	PolicyPlan policy_plan(int sequences, int length)
 	{
 		PolicyPlan plan { };
-		plan.lanes = length <= 64 ? 8 : length <= 1024 ? 64 : 256;
+		plan.lanes = length <= 64 ? 8 : length <= 256 || (length <= 1024 && sequences >= 2048) ? 64 : 256;
 		const int at_a_time = 256 / plan.lanes;
 		plan.sequences_of_group = static_cast<int>(round_up(std::max(1, ceil_div(sequences, MOST_GROUPS)), at_a_time));
 		plan.groups = ceil_div(sequences, plan.sequences_of_group);
@@ -295,8 +340,14 @@ namespace
 		MLHIP_REQUIRE(sequences <= (1 << 28) && length <= (1 << 28), who + ": too many sequences or tokens");
 		return PolicyShape { sequences, length };
 	}
+	bool few_tokens(const PolicyShape &s)
+	{
+		return s.sequences <= FEW_SEQUENCES && static_cast<size_t>(s.sequences) * s.length <= FEW_TOKENS;
+	}
 	size_t policy_space(const PolicyShape &s)
 	{
+		if (few_tokens(s))
+			return 0;
 		const PolicyPlan plan = policy_plan(s.sequences, s.length);
 		return round_up(sizeof(Sums) * (plan.chunks > 0 ? static_cast<size_t>(s.sequences) * plan.chunks : plan.groups), 256) + sizeof(int) * s.sequences;
 	}
@@ -356,6 +407,15 @@ extern "C"
 		const OnDeviceOf on(context);
 		const PolicyPlan plan = policy_plan(p.sequences, p.length);
 		const bool average_sequences = average == AVERAGE_SEQUENCES;
+		if (few_tokens(s))
+		{
+			if (p.length < 4)
+				hipLaunchKernelGGL((kernel_policy_few<1>), dim3(1), dim3(1024), 0, on.stream, p, average_sequences, ptr<float>(loss), ptr<float>(weights));
+			else
+				hipLaunchKernelGGL((kernel_policy_few<4>), dim3(1), dim3(1024), 0, on.stream, p, average_sequences, ptr<float>(loss), ptr<float>(weights));
+			MLHIP_CHECK(hipGetLastError());
+			return;
+		}
 		Sums *partial = reinterpret_cast<Sums*>(workspace);
 		const size_t units = plan.chunks > 0 ? static_cast<size_t>(p.sequences) * plan.chunks : plan.groups;
 		int *counts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(workspace) + round_up(sizeof(Sums) * units, 256));
