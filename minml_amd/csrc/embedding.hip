@@ -192,22 +192,42 @@ namespace
 		for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
 			p.counts[blockIdx.x * digits + d] = counters[d];
 	}
+	/* KEPT: a wavefront's share is at most 128 tokens, which it reads once */
+	template<bool KEPT>
 	__global__ __launch_bounds__(SORT_THREADS) void kernel_sort_place(SortPass p)
 	{
 		extern __shared__ int counters[]; /* [wavefronts][digits]; of the groups before [digits], of those behind */
 		__shared__ int waves[SORT_WAVES];
 		const int digits = 1 << p.bits, groups = gridDim.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 		int *before = counters + SORT_WAVES * digits, *behind = before + digits, *mine = counters + wave * digits;
-		for (int d = threadIdx.x; d < (SORT_WAVES + 2) * digits; d += SORT_THREADS)
-			counters[d] = 0;
-		__syncthreads();
 		/* a wavefront has an eighth of the group's tokens, in their order */
 		const int group_first = blockIdx.x * p.per_group, group_last = group_first + min(p.per_group, p.count - group_first), share = p.per_group / SORT_WAVES;
 		const int first = group_first + wave * share, here = max(0, min(share, group_last - first));
-		p.count_digits<64>(mine, first, first + here, lane);
+		constexpr int ROUNDS = 2;
+		int keys[ROUNDS], positions[ROUNDS];
+		if constexpr (KEPT)
+#pragma unroll
+			for (int u = 0; u < ROUNDS; u++)
+			{
+				const int from = min(first + 64 * u + lane, p.count - 1);
+				keys[u] = p.key(from);
+				positions[u] = p.keys != nullptr ? p.positions[from] : from;
+			}
+		for (int d = threadIdx.x; d < SORT_WAVES * digits; d += SORT_THREADS)
+			counters[d] = 0;
+		__syncthreads();
+		if constexpr (KEPT)
+		{
+#pragma unroll
+			for (int u = 0; u < ROUNDS; u++)
+				if (64 * u + lane < here)
+					atomicAdd(&mine[p.digit(keys[u])], 1);
+		}
+		else
+			p.count_digits<64>(mine, first, first + here, lane);
 		for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
 		{
-			constexpr int AHEAD = 16;
+			constexpr int AHEAD = 32;
 			int sum_before = 0, sum_behind = 0;
 			for (int g = 0; g < groups; g += AHEAD)
 			{
@@ -249,11 +269,8 @@ namespace
 			smaller = at + behind[d];
 		}
 		__syncthreads();
-		for (int i = 0; i < here; i += 64)
+		const auto place_tokens = [&](bool there, int key, int position) __attribute__((always_inline))
 		{
-			const bool there = i + lane < here;
-			const int from = first + min(i + lane, here - 1);
-			const int key = p.key(from), position = p.keys != nullptr ? p.positions[from] : from;
 			const int digit = p.digit(key);
 			const uint64_t same = lanes_alike(digit, p.bits, there);
 			const int below = lanes_below(same);
@@ -267,7 +284,19 @@ namespace
 				p.keys_out[place] = key;
 				p.positions_out[place] = position;
 			}
+		};
+		if constexpr (KEPT)
+		{
+#pragma unroll
+			for (int u = 0; u < ROUNDS; u++)
+				place_tokens(64 * u + lane < here, keys[u], positions[u]);
 		}
+		else
+			for (int i = 0; i < here; i += 64)
+			{
+				const int from = first + min(i + lane, here - 1);
+				place_tokens(i + lane < here, p.key(from), p.keys != nullptr ? p.positions[from] : from);
+			}
 	}
 
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
@@ -314,7 +343,10 @@ namespace
 		}
 		return first;
 	}
-	/* v += the rows of every `step`th place from `first` on, AHEAD of them on their way at a time. row(i): where the i-th lies */
+	/*
+	 * v += the rows of every `step`th place from `first` on, AHEAD of them on their way at a time. row(i): where the i-th lies. Places behind the last one read it once more and count for nothing by a selection: the compiler
+	 * would move loads into a branch, where they wait for all others.
+	 */
 	template<typename T, int AHEAD, int VEC, typename Row>
 	__device__ __forceinline__ void add_rows(float (&v)[VEC], int first, int last, int step, Row &&row)
 	{
@@ -324,12 +356,12 @@ namespace
 #pragma unroll
 			for (int u = 0; u < AHEAD; u++)
 				x[u].load(row(min(i + u * step, last - 1)));
+			__builtin_amdgcn_sched_barrier(0); /* else they are asked for one by one, to spare registers */
 #pragma unroll
 			for (int u = 0; u < AHEAD; u++)
-				if (i + u * step < last)
 #pragma unroll
-					for (int e = 0; e < VEC; e++)
-						v[e] += x[u][e];
+				for (int e = 0; e < VEC; e++)
+					v[e] += i + u * step < last ? x[u][e] : 0.0f;
 		}
 	}
 	/* the sums of a workgroup's 256 / lanes groups of threads in the first of them, in order. Every thread calls it */
@@ -382,7 +414,7 @@ namespace
 		if (static_cast<int>(threadIdx.x) < p.lanes && column < p.columns)
 			store_nearest<VEC>(place.in(p.partial + static_cast<size_t>(blockIdx.x) * p.columns), v, place.skip);
 	}
-	constexpr int MOST_CLASSES_OF_GROUP = 32;
+	constexpr int MOST_CLASSES_OF_GROUP = 256;
 	/* a class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's */
 	constexpr int ROWS_OF_ALL = 16;
 	template<typename T, typename Out, int VEC>
@@ -400,8 +432,8 @@ namespace
 				ends[wave] = bound;
 		}
 		__syncthreads();
-		if (static_cast<int>(threadIdx.x) <= classes)
-			bounds[threadIdx.x] = lower_bound(p.keys, ends[0], ends[1] - ends[0], first_class + threadIdx.x);
+		for (int c = threadIdx.x; c <= classes; c += 256)
+			bounds[c] = lower_bound(p.keys, ends[0], ends[1] - ends[0], first_class + c);
 		__syncthreads();
 		const int column = (span * p.lanes + threadIdx.x % p.lanes) * VEC, groups = 256 / p.lanes, group = threadIdx.x / p.lanes;
 		const bool inside = column < p.columns;
@@ -465,25 +497,25 @@ namespace
 						key[u] = p.keys[min(i + u, last - 1)];
 						x[u].load(row_of_list(min(i + u, last - 1)));
 					}
+					__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 					for (int u = 0; u < AHEAD; u++)
-						if (i + u < last)
+					{
+						if (key[u] != current)
 						{
-							if (key[u] != current)
-							{
-								if (current >= 0)
-									write(current, v, old);
-								current = key[u];
-								if (p.beta != 0.0f)
-									old.load(row_of_table(current));
-#pragma unroll
-								for (int e = 0; e < VEC; e++)
-									v[e] = 0.0f;
-							}
+							if (current >= 0)
+								write(current, v, old);
+							current = key[u];
+							if (p.beta != 0.0f)
+								old.load(row_of_table(current));
 #pragma unroll
 							for (int e = 0; e < VEC; e++)
-								v[e] += x[u][e];
+								v[e] = 0.0f;
 						}
+#pragma unroll
+						for (int e = 0; e < VEC; e++)
+							v[e] += i + u < last ? x[u][e] : 0.0f; /* behind the last place: its class, nothing more */
+					}
 				}
 				if (current >= 0)
 					write(current, v, old);
@@ -638,8 +670,9 @@ namespace
 					pass * plan.digit_bits, plan.digit_bits, plan.per_group };
 			const int bytes = static_cast<int>(sizeof(int)) << plan.digit_bits;
 			hipLaunchKernelGGL(kernel_sort_count, dim3(plan.groups), dim3(SORT_THREADS), bytes, stream, p);
-			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel_sort_place), (SORT_WAVES + 2) * bytes);
-			hipLaunchKernelGGL(kernel_sort_place, dim3(plan.groups), dim3(SORT_THREADS), (SORT_WAVES + 2) * bytes, stream, p);
+			auto place = plan.per_group <= 2 * SORT_THREADS ? kernel_sort_place<true> : kernel_sort_place<false>;
+			ensure_dynamic_lds(reinterpret_cast<const void*>(place), (SORT_WAVES + 2) * bytes);
+			hipLaunchKernelGGL(place, dim3(plan.groups), dim3(SORT_THREADS), (SORT_WAVES + 2) * bytes, stream, p);
 			MLHIP_CHECK(hipGetLastError());
 		}
 		const int last = (plan.passes - 1) & 1;
@@ -651,7 +684,7 @@ namespace
 		const int lanes = lanes_of_row(s, VEC);
 		const int spans = ceil_div(s.columns, lanes * VEC);
 		const size_t units = static_cast<size_t>(s.classes) * spans;
-		const int most = static_cast<int>(std::min<size_t>(MOST_CLASSES_OF_GROUP, std::max<size_t>(1, units / 2048)));
+		const int most = static_cast<int>(std::min<size_t>(std::max(32, 256 / lanes), std::max<size_t>(1, units / 2048)));
 		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk_of(s, VEC), scale, beta };
 		if (s.rows >= p.chunk)
 		{
