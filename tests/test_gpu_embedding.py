@@ -100,3 +100,20 @@ def test_the_same_bits_every_time(ctx):
             ml.embeddingBackward(ctx, T, DY, 1.0, 0.0, dtable, space(ctx, T, dtable))
             results.append(dtable.copyToHost(ctx))
         assert all(np.array_equal(results[0], r) for r in results)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_tensors_that_begin_at_any_element(ctx, dtype):
+    rng = np.random.default_rng(6)
+    for rows, classes, features in ((50, 20, 24), (50, 20, 33), (700, 3, 2050)):
+        tokens, dy = tokens_of(rng, rows, classes), R.bits(rng.standard_normal((rows, features)), dtype)
+        table = R.bits(rng.standard_normal((classes, features)), dtype)
+        shifted = lambda a: ml.toDevice(ctx, np.concatenate([a.reshape(-1)[:1], a.reshape(-1)])).view(a.shape, 1)
+        T, y, dtable = shifted(tokens), shifted(dy), shifted(table)
+        ml.embeddingForward(ctx, T, shifted(table), 3.0, y)
+        want = V.embedding(tokens, R.numbers(table), 3.0)
+        assert R.worst(y.copyToHost(ctx), want, V.embedding_bound(want, dtype)) <= 1
+        ml.embeddingBackward(ctx, T, shifted(dy), 1.0, 0.0, dtable, space(ctx, T, dtable))
+        exact, weighted = V.embedding_gradient(tokens, R.numbers(dy), classes, 1.0)
+        assert R.worst(dtable.copyToHost(ctx), exact, V.embedding_gradient_bound(exact, weighted, 0 * exact, dtype)) <= 1
+        assert R.numbers(dtable._owner.copyToHost(ctx))[0] == R.numbers(table).reshape(-1)[0]

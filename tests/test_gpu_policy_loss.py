@@ -145,3 +145,17 @@ def test_gradient_against_differences(ctx):
                 nll[s, t] += step
                 values.append(exact(nll, *data[1:], "sequences")[0][0][0])
             assert abs((values[0] - values[1]) / 2e-5 - gradient[s, t]) < 1e-8
+
+
+def test_tensors_that_begin_at_any_element(ctx):
+    rng = np.random.default_rng(4)
+    for sequences, length in ((3, 61), (300, 77), (2, 9001)):
+        data = inputs(rng, sequences, length, True)
+        plain = Loss(ctx, *data)
+        shifted = [ml.toDevice(ctx, np.concatenate([a.reshape(-1)[:1], a.reshape(-1)])).view(a.shape, 1) for a in data]
+        loss, weights, dnll = ml.Tensor((5,), "float32").view((4,), 1), ml.Tensor((sequences + 1,), "float32").view((sequences,), 1), ml.Tensor((sequences * length + 1,), "float32").view((sequences, length), 1)
+        space = ml.Tensor((max(1, ml.policyLossGetWorkspaceSize(ctx, shifted[0])),), "uint8")
+        ml.policyLossForward(ctx, *shifted, CLASSES, CLIP, KL_WEIGHT, "tokens", loss, weights, space)
+        ml.policyLossBackward(ctx, *shifted, CLASSES, CLIP, KL_WEIGHT, weights, None, 0.0, dnll)
+        assert np.array_equal(loss.copyToHost(ctx), plain.loss.copyToHost(ctx)) and np.array_equal(weights.copyToHost(ctx), plain.weights.copyToHost(ctx))
+        assert np.array_equal(dnll.copyToHost(ctx), plain.gradient())

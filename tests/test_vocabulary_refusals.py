@@ -112,12 +112,17 @@ def test_policy_loss_refusals_of_the_library():
     forward(loss=NULL)
     forward(loss=fake((4,)).desc())
     forward(weights=NULL)
-    forward(space=None, why="workspace")
-    forward(space=0x7010, why="workspace")
-    forward(n=need - 1, why="workspace")
+    assert need == 0  # a few tokens need none
+    many = dict(zip(names, (t.desc() for t in policy_tensors(300, 40))))
+    of_many = dict(many, weights=fake((300,), "float32").desc())
+    need = B.fn("policy_loss_get_workspace_size")(B.make_shape((300, 40)))
+    forward(**of_many, space=None, why="workspace")
+    forward(**of_many, space=0x7010, n=need, why="workspace")
+    forward(**of_many, n=need - 1, why="workspace")
+    forward(**of_many, n=need, why="null context")
     forward(loss=weights, weights=weights, why="4")
     forward(weights=given["advantages"], why="overlap")
-    forward(loss=ml.Tensor((4,), "float32", _ptr=0x7000).desc(), why="overlap")
+    forward(**of_many, n=need, loss=ml.Tensor((4,), "float32", _ptr=0x7000).desc(), why="overlap")
     backward(dnll=fake((3, 8), "float32").desc())
     backward(dnll=NULL)
     backward(dnll=given["nll"], why="overlap")
@@ -152,5 +157,104 @@ def test_policy_loss_refusals_of_the_mirror():
             call()
         assert "null context" not in str(failure.value)
     for call in (forward, backward, lambda: forward(**{"2": None}), lambda: backward(**{"2": None}, dloss=fake((1,), "float32"))):
+        with pytest.raises(ValueError, match="null context"):
+            call()
+
+
+def test_distillation_refusals_of_the_library():
+    x, w, b, named, taught, f, p = (fake(s, d).desc() for s, d in (((4, 16), "float16"), ((90, 16), "float16"), ((90,), "float16"), ((4, 8), "int32"), ((4, 8), "float16"), ((4,), "float32"), ((4, 8), "float32")))
+    lse = fake((4,), "float32").desc()
+    size = lambda backward, count=8: B.fn("linear_distillation_get_workspace_size")(B.make_shape((4, 16)), B.make_shape((90, 16)), count, B.DTYPE_FLOAT16, backward)
+    assert size(True) >= size(False) > 0
+
+    def forward(x=x, w=w, b=b, named=named, taught=taught, t=2.0, loss=f, lse=lse, p=p, space=0x7000, n=1 << 30, why=None):
+        refused("linear_distillation_forward", x, w, b, named, taught, t, loss, lse, p, space, n, why=why)
+
+    dx, dw, db, g = fake((4, 16)).desc(), fake((90, 16)).desc(), fake((90,)).desc(), fake((4,), "float32").desc()
+
+    def backward(x=x, w=w, b=b, named=named, taught=taught, t=2.0, lse=lse, p=p, dloss=g, dx=dx, dw=dw, db=db, space=0x7000, n=1 << 30, why=None):
+        refused("linear_distillation_backward", x, w, b, named, taught, t, lse, p, dloss, 0.0, dx, 0.0, dw, db, space, n, why=why)
+
+    for call in (forward, backward):
+        call(x=fake((4, 15)).desc())
+        call(x=fake((4, 16), "int8").desc(), why="data type")
+        call(w=fake((2, 90, 16)).desc())
+        call(w=fake((0, 16)).desc())
+        call(w=fake((90, 16), "float32").desc())
+        call(b=fake((89,)).desc(), why="bias")
+        call(named=fake((4, 8), "float32").desc(), why="int32")
+        call(named=fake((3, 8), "int32").desc())
+        call(named=fake((4, 0), "int32").desc(), why="1 to 1024")
+        call(named=fake((4, 1025), "int32").desc(), taught=fake((4, 1025)).desc(), why="1 to 1024")
+        call(named=NULL)
+        call(taught=fake((4, 7)).desc(), why="logit")
+        call(taught=fake((4, 8), "int32").desc(), why="logit")
+        call(taught=NULL, why="logit")
+        for t in (0.0, -1.0, float("nan"), float("inf"), 1e-45):
+            call(t=t, why="temperature")
+        call(lse=fake((5,), "float32").desc())
+        call(lse=fake((4,)).desc())
+        call(p=fake((4, 8)).desc(), why="log probabilities")
+        call(p=fake((4, 9), "float32").desc(), why="log probabilities")
+        call(p=NULL, why="log probabilities")
+        call(x=ml.Tensor((4, 16), "float16", _ptr=0x7008).desc(), why="aligned")
+        call(w=ml.Tensor((90, 16), "float16", _ptr=0x7002).desc(), why="aligned")
+        call(space=None, why="workspace")
+        call(space=0x7080, why="workspace")
+        call(why="null context")
+        call(b=NULL, taught=fake((4, 8), "float32").desc(), why="null context")
+    # logits of half the type of an fp32 layer
+    wide = dict(x=fake((4, 16), "float32").desc(), w=fake((90, 16), "float32").desc(), b=NULL)
+    forward(**wide, why="logit")
+    forward(n=size(False) - 1, why="workspace")
+    forward(loss=fake((4, 2), "float32").desc())
+    forward(loss=lse, why="overlap")
+    forward(p=taught, why="log probabilities")
+    backward(n=size(True) - 1, why="workspace")
+    backward(dloss=fake((4,)).desc())
+    backward(dx=fake((4, 17)).desc())
+    backward(dx=fake((4, 16), "float32").desc())
+    backward(dw=fake((91, 16)).desc())
+    backward(dw=fake((90, 16), "int32").desc())
+    backward(db=fake((91,)).desc())
+    backward(dx=x, why="overlap")
+    backward(dw=w, why="overlap")
+    backward(dx=ml.Tensor((4, 16), "float16", _ptr=0x7000).desc(), why="overlap")
+    B.fn("linear_distillation_backward")(None, x, w, b, named, taught, 1.0, lse, p, g, 0.0, NULL, 0.0, NULL, NULL, None, 0)  # nothing asked for
+    for count in (0, -1, 1025):
+        with pytest.raises(ValueError, match="1 to 1024"):
+            size(True, count)
+
+
+def test_distillation_workspace_does_not_grow_with_rows_times_classes():
+    """What the cross entropy's backward pass holds, 16 bytes for every place and 2 for every row of every tile; for few rows also their logits in the forward pass."""
+    for dtype in (B.DTYPE_FLOAT16, B.DTYPE_FLOAT32):
+        for rows, features, classes, count in ((4096, 2048, 65536, 64), (5000, 64, 200000, 1024), (7, 2048, 65536, 16), (64, 64, 1000, 3)):
+            shapes = B.make_shape((rows, features)), B.make_shape((classes, features))
+            size = B.fn("linear_distillation_get_workspace_size")(*shapes, count, dtype, True)
+            other = B.fn("linear_cross_entropy_get_workspace_size")(*shapes, dtype, True)
+            assert size <= other + rows * (16 * count + 2 * (classes // 128 + 2) + 8) + (4 * rows * classes if rows <= 64 else 0) + 4096
+
+
+def test_distillation_refusals_of_the_mirror():
+    x, w, b, named, taught, f, p = fake((2, 3, 16)), fake((90, 16)), fake((90,)), fake((2, 3, 8), "int32"), fake((2, 3, 8)), fake((2, 3), "float32"), fake((2, 3, 8), "float32")
+    space = ml.Tensor((1 << 24,), "uint8", _ptr=1 << 50)
+
+    def forward(x=x, w=w, b=b, named=named, taught=taught, loss=f, lse=fake((2, 3), "float32"), p=p):
+        ml.linearDistillationForward(Ctx, x, w, b, named, taught, 2.0, loss, lse, p, space)
+
+    def backward(x=x, w=w, b=b, named=named, taught=taught, lse=f, p=p, g=fake((2, 3), "float32"), dx=fake((2, 3, 16)), dw=fake((90, 16), "float32"), db=fake((90,))):
+        ml.linearDistillationBackward(Ctx, x, w, b, named, taught, 2.0, lse, p, g, 0.0, dx, 0.0, dw, db, space)
+
+    bad = [lambda: forward(loss=fake((6,), "float32")), lambda: backward(g=fake((2, 3))), lambda: backward(dx=fake((6, 16))), lambda: backward(dw=fake((90, 15))), lambda: backward(db=fake((90,), "int32"))]
+    for call in (forward, backward):
+        bad += [lambda call=call, kw=kw: call(**kw) for kw in (dict(w=fake((90, 8))), dict(b=fake((91,))), dict(named=fake((6, 8), "int32")), dict(named=fake((2, 3, 8), "float32")), dict(taught=fake((2, 3, 7))),
+                                                             dict(taught=fake((2, 3, 8), "int8")), dict(p=fake((2, 3, 8))), dict(p=fake((2, 3, 1), "float32")), dict(lse=fake((3, 2), "float32")))]
+    for call in bad:
+        with pytest.raises(ValueError) as failure:
+            call()
+        assert "null context" not in str(failure.value)
+    one = dict(x=fake((16,)), named=fake((8,), "int32"), taught=fake((8,)), p=fake((8,), "float32"), lse=fake((1,), "float32"))
+    for call in (forward, backward, lambda: backward(dx=None, db=None, b=None), lambda: forward(**one, loss=fake((1,), "float32")), lambda: backward(**one, g=fake((1,), "float32"), dx=fake((16,)))):
         with pytest.raises(ValueError, match="null context"):
             call()
