@@ -68,16 +68,25 @@ namespace
 			{
 				return 0;
 			}
+			struct Nothing
+			{
+			};
+			template<int BM, int BN>
+			__device__ __forceinline__ Nothing begin_loss(const TilePlace<BM, BN>&, int) const
+			{
+				return Nothing { };
+			}
 			template<int BM, int BN, typename Acc, typename Columns>
-			__device__ __forceinline__ void take_tile(const Acc&, const Columns&, const TilePlace<BM, BN>&, uint8_t*, int) const
+			__device__ __forceinline__ void take_tile(const Acc&, const Columns&, const TilePlace<BM, BN>&, const Nothing&, uint8_t*) const
 			{
 			}
 			template<int BM, int BN>
-			__device__ __forceinline__ void begin_gradient(uint8_t*) const
+			__device__ __forceinline__ Nothing begin_gradient(const TilePlace<BM, BN>&, int, const float*, uint8_t*) const
 			{
+				return Nothing { };
 			}
 			template<int BM, int BN, int ROWS, typename TileStage>
-			__device__ __forceinline__ void correct(const TileStage&, uint8_t*, const TilePlace<BM, BN>&, int, int, int, int, const float*) const
+			__device__ __forceinline__ void correct(const TileStage&, uint8_t*, const TilePlace<BM, BN>&, const Nothing&, int, int) const
 			{
 			}
 			template<int BM, int BN>

@@ -168,11 +168,66 @@ namespace
 			int count, stride; /* stride: of begins */
 			float slope; /* 1 / t */
 
-			__device__ __forceinline__ void range_of(int tile_n, int m, int &first, int &last) const
+			/*
+			 * A thread's row of the tile and its classes there: first .. last - 1 of the row's, the first two of them with what is known of them. Asked for when the tile is complete, before anything is computed of it: the
+			 * tile's end would wait for one load after another (us, so / when they are used: @@)
+			 */
+			static constexpr int AHEAD = 2;
+			struct OfTile
 			{
-				const uint16_t *of_row = begins + static_cast<size_t>(m) * stride + tile_n;
-				first = of_row[0];
-				last = of_row[1];
+					int row, m, first, last, named[AHEAD];
+					float share[AHEAD], probability[AHEAD], factor;
+			};
+			template<bool BACKWARD, int BM, int BN>
+			__device__ __forceinline__ OfTile classes_of(const TilePlace<BM, BN> &at, int rows, const float *factors) const
+			{
+				OfTile t;
+				t.row = threadIdx.x;
+				t.m = at.tile_m * BM + t.row;
+				t.first = t.last = 0;
+				t.factor = 0.0f;
+				if (t.row < BM && t.m < rows)
+				{
+					const uint16_t *of_row = begins + static_cast<size_t>(t.m) * stride + at.tile_n;
+					t.first = of_row[0];
+					t.last = of_row[1];
+					if (BACKWARD)
+					{
+						t.factor = factors[t.m];
+						t.last = t.factor != 0.0f ? t.last : t.first;
+					}
+				}
+#pragma unroll
+				for (int u = 0; u < AHEAD; u++)
+				{
+					t.named[u] = 0;
+					t.share[u] = t.probability[u] = 0.0f;
+					if (t.first + u < t.last)
+					{
+						const size_t place = static_cast<size_t>(t.m) * count + t.first + u;
+						t.named[u] = classes[place];
+						if (BACKWARD)
+						{
+							t.share[u] = shares[place];
+							t.probability[u] = known[place];
+						}
+					}
+				}
+				return t;
+			}
+			/* f(place of the row, class, probabilities of teacher and student) for all of them */
+			template<bool BACKWARD, typename F>
+			__device__ __forceinline__ void for_classes(const OfTile &t, F &&f) const
+			{
+#pragma unroll
+				for (int u = 0; u < AHEAD; u++)
+					if (t.first + u < t.last)
+						f(static_cast<size_t>(t.m) * count + t.first + u, t.named[u], t.share[u], t.probability[u]);
+				for (int k = t.first + AHEAD; k < t.last; k++)
+				{
+					const size_t place = static_cast<size_t>(t.m) * count + k;
+					f(place, classes[place], BACKWARD ? shares[place] : 0.0f, BACKWARD ? known[place] : 0.0f);
+				}
 			}
 			template<int BLOCKS>
 			struct Rows
@@ -198,18 +253,19 @@ namespace
 			{
 				return Stage<float, BN>::bytes(rows_at_a_time(BM));
 			}
+			template<int BM, int BN>
+			__device__ __forceinline__ OfTile begin_loss(const TilePlace<BM, BN> &at, int rows) const
+			{
+				return classes_of<false>(at, rows, nullptr);
+			}
 			/* the logits of the rows' classes, through LDS in fp32, a part of the rows at a time */
 			template<int BM, int BN, typename Acc, typename Columns>
-			__device__ __forceinline__ void take_tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const Columns &columns, const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
+			__device__ __forceinline__ void take_tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const Columns &columns, const TilePlace<BM, BN> &at, const OfTile &of_tile, uint8_t *lds) const
 			{
 				constexpr int ROWS = rows_at_a_time(BM), BLOCKS = ROWS / 64;
 				typedef Stage<float, BN> TileStage;
 				const TileStage stage { reinterpret_cast<float*>(lds) };
-				const int row = threadIdx.x, m = at.tile_m * BM + row;
-				int first = 0, last = 0;
-				if (row < BM && m < rows)
-					range_of(at.tile_n, m, first, last);
-				if (__syncthreads_or(first < last) == 0)
+				if (__syncthreads_or(of_tile.first < of_tile.last) == 0)
 					return;
 				static_for<BM / ROWS>([&](auto part)
 				{
@@ -230,12 +286,11 @@ namespace
 								stage.put(at.row(i) - h * ROWS, at.column(j) + at.lane_column(q), z[0], z[1], z[2], z[3]);
 							}
 					__syncthreads();
-					if (row >= h * ROWS && row < (h + 1) * ROWS)
-						for (int k = first; k < last; k++)
+					if (of_tile.row >= h * ROWS && of_tile.row < (h + 1) * ROWS)
+						for_classes<false>(of_tile, [&](size_t place, int n, float, float) __attribute__((always_inline))
 						{
-							const size_t place = static_cast<size_t>(m) * count + k;
-							logits[place] = stage.place[(row - h * ROWS) * TileStage::STRIDE + classes[place] - at.tile_n * BN];
-						}
+							logits[place] = stage.place[(of_tile.row - h * ROWS) * TileStage::STRIDE + n - at.tile_n * BN];
+						});
 				});
 			}
 
@@ -259,34 +314,30 @@ namespace
 					}
 			};
 			template<int BM, int BN>
-			__device__ __forceinline__ void begin_gradient(uint8_t *lds) const
+			__device__ __forceinline__ OfTile begin_gradient(const TilePlace<BM, BN> &at, int rows, const float *factors, uint8_t *lds) const
 			{
 				for (int i = threadIdx.x; i < gradient_lds<BM, BN>() / 4; i += TilePlace<BM, BN>::THREADS)
 					reinterpret_cast<int*>(lds)[i] = 0;
+				return classes_of<true>(at, rows, factors);
 			}
 			/* the places of the rows' classes in a tile that lies in LDS, written again with p - q instead of p; a thread has a row's, so what rounding takes of them is added up in order */
 			template<int BM, int BN, int ROWS, typename TileStage>
-			__device__ __forceinline__ void correct(const TileStage &stage, uint8_t *lds, const TilePlace<BM, BN> &at, int first_row, int rows, int first_class, int, const float *factors) const
+			__device__ __forceinline__ void correct(const TileStage &stage, uint8_t *lds, const TilePlace<BM, BN> &at, const OfTile &of_tile, int first_row, int first_class) const
 			{
 				typedef typename std::remove_pointer<decltype(stage.place)>::type T;
 				const Extra<BM, BN> extra(lds);
-				const int row = threadIdx.x, m = at.tile_m * BM + first_row + row;
-				if (row < ROWS && m < rows)
+				const int row = of_tile.row - first_row;
+				if (row >= 0 && row < ROWS)
 				{
-					const float factor = factors[m];
-					int first = 0, last = 0;
-					if (factor != 0.0f)
-						range_of(at.tile_n, m, first, last);
 					float taken = 0.0f;
 					int before = -1;
-					for (int k = first; k < last; k++)
+					for_classes<true>(of_tile, [&](size_t, int n, float share, float probability) __attribute__((always_inline))
 					{
-						const size_t place = static_cast<size_t>(m) * count + k;
-						const int column = classes[place] - first_class - at.tile_n * BN;
+						const int column = n - first_class - at.tile_n * BN;
 						if (column == before) /* its share is at the class's first place */
-							continue;
+							return;
 						before = column;
-						const float pf = known[place] * factor, qf = shares[place] * factor, d = pf - qf;
+						const float pf = probability * of_tile.factor, qf = share * of_tile.factor, d = pf - qf;
 						T *stored = stage.place + row * TileStage::STRIDE + column;
 						const T rounded = static_cast<T>(d);
 						taken += (d - static_cast<float>(rounded)) - (pf - static_cast<float>(*stored));
@@ -295,8 +346,8 @@ namespace
 							atomicAdd(&extra.columns[column], static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(qf) * static_cast<double>(1ll << FIXED_BITS))));
 						else
 							extra.no_number[column] = 1;
-					}
-					extra.lost[first_row + row] = taken;
+					});
+					extra.lost[of_tile.row] = taken;
 				}
 				__syncthreads();
 			}

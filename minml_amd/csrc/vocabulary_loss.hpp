@@ -118,6 +118,7 @@ namespace mlhip
 				constexpr float NOTHING = -std::numeric_limits<float>::infinity();
 				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
+				const auto of_tile = goal.template begin_loss<BM, BN>(at, rows);
 				typename Goal::template Rows<BLOCKS> of_rows;
 #pragma unroll
 				for (int i = 0; i < BLOCKS; i++)
@@ -175,7 +176,7 @@ namespace mlhip
 						p = join(p, meeting[w * BM + row]);
 					partials[static_cast<size_t>(m) * tiles_n + at.tile_n] = p;
 				}
-				goal.template take_tile<BM, BN>(acc, columns, at, lds, rows);
+				goal.template take_tile<BM, BN>(acc, columns, at, of_tile, lds);
 			}
 	};
 	/* a row's pairs joined by THREADS threads, a wavefront or a workgroup, each with 8 on their way at a time; every thread gets it */
@@ -330,7 +331,7 @@ namespace mlhip
 					target[i] = Goal::ONE && factor[i] != 0.0f ? goal.targets[m] - first_class : -1; /* a class then */
 					taken[i] = 0.0f;
 				}
-				goal.template begin_gradient<BM, BN>(lds + stage_lds<BM, BN>());
+				const auto of_tile = goal.template begin_gradient<BM, BN>(at, rows, factors, lds + stage_lds<BM, BN>());
 				static_for<PASSES>([&](auto pass)
 				{
 					constexpr int PASS = decltype(pass)::value, FIRST = PASS * BLOCKS / PASSES;
@@ -374,7 +375,7 @@ namespace mlhip
 							}
 					}
 					__syncthreads();
-					goal.template correct<BM, BN, ROWS>(stage, lds + stage_lds<BM, BN>(), at, PASS * ROWS, rows, first_class, classes, factors);
+					goal.template correct<BM, BN, ROWS>(stage, lds + stage_lds<BM, BN>(), at, of_tile, PASS * ROWS, first_class);
 					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
 				});
 				const bool of_columns = sums != nullptr, of_rows = sizeof(T) == 2 && lost != nullptr;
