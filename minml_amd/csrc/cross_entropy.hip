@@ -162,7 +162,7 @@ namespace
 	template<typename T>
 	void loss_forward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const int *targets, float *loss, float *lse, uint8_t *workspace)
 	{
-		const LossSpace space = loss_space(s, false);
+		const LossSpace space = loss_space(s, false, few_rows(s));
 		Partial *partials = reinterpret_cast<Partial*>(workspace + space.partials);
 		float *target_logits = reinterpret_cast<float*>(workspace + space.target_logits);
 		int columns;
@@ -215,7 +215,8 @@ extern "C"
 	size_t hip_linear_cross_entropy_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, mlDataType_t dtype, bool backward)
 	try
 	{
-		return loss_space(loss_shape(input_shape, weights_shape, dtype, "linear_cross_entropy_get_workspace_size"), backward).total;
+		const LossShape s = loss_shape(input_shape, weights_shape, dtype, "linear_cross_entropy_get_workspace_size");
+		return loss_space(s, backward, few_rows(s)).total;
 	}
 	catch (...)
 	{
@@ -231,7 +232,7 @@ extern "C"
 		MLHIP_REQUIRE(per_row(loss, s, DTYPE_FLOAT32) && per_row(lse, s, DTYPE_FLOAT32), "linear_cross_entropy_forward: loss and lse must be fp32 with one element per row");
 		if (s.rows == 0)
 			return;
-		check_space(workspace, workspace_size, loss_space(s, false).total, name);
+		check_space(workspace, workspace_size, loss_space(s, false, few_rows(s)).total, name);
 		require_apart( { loss, lse, Extent(workspace, workspace_size) }, { x, w, b, targets }, name);
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
@@ -264,14 +265,14 @@ extern "C"
 		{
 			return OneClass { ptr<int>(targets), nullptr };
 		};
-		check_space(workspace, workspace_size, loss_space(s, true).total, name);
+		check_space(workspace, workspace_size, loss_space(s, true, few_rows(s)).total, name);
 		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, b, targets, lse, dloss }, name);
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db,
+			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, few_rows(s),
 					reinterpret_cast<uint8_t*>(workspace));
 		else
-			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db,
+			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db, few_rows(s),
 					reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)

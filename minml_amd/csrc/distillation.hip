@@ -170,7 +170,7 @@ namespace
 
 			/*
 			 * A thread's row of the tile and its classes there: first .. last - 1 of the row's, the first two of them with what is known of them. Asked for when the tile is complete, before anything is computed of it: the
-			 * tile's end would wait for one load after another (us, so / when they are used: @@)
+			 * tile's end would wait for one load after another (us, so / when they are used: 2048 x 1024 x 50001 267 / 271, gradients of 4096 x 2048 x 65536 4050 / 4078)
 			 */
 			static constexpr int AHEAD = 2;
 			struct OfTile
@@ -520,6 +520,14 @@ namespace
 	}
 
 	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
+	/*
+	 * The cross entropy's rule, but that 17 to 32 rows of large weights in fp16 go on tiles: they fill two blocks of 16 rows, and their logits are kept. us of a forward pass, so / on tiles: 24 rows fp16 of 2048 x 65536 67 / 56,
+	 * 1024 x 32000 29 / 28, 1023 x 32000 68 / 50, 256 x 100000 55 / 31, 1024 x 8000 12 / 26; fp32 1024 x 32000 47 / 54; 16 rows fp16 47 / 55, 20 / 27, 46 / 50, 27 / 31, 11 / 25
+	 */
+	bool few_logits(const LossShape &s)
+	{
+		return few_rows(s) && (s.rows <= 16 || s.element_size == 4 || static_cast<size_t>(s.classes) * s.features * s.element_size <= (size_t(1) << 24));
+	}
 	struct DistillationSpace
 	{
 			LossSpace loss;
@@ -528,7 +536,7 @@ namespace
 	DistillationSpace distillation_space(const LossShape &s, int count, bool backward)
 	{
 		DistillationSpace space { };
-		space.loss = loss_space(s, backward);
+		space.loss = loss_space(s, backward, few_logits(s));
 		size_t at = space.loss.total;
 		const auto take = [&](size_t bytes)
 		{
@@ -537,7 +545,7 @@ namespace
 			return begin;
 		};
 		const size_t rows = s.rows, places = rows * count;
-		if (s.rows > 0 && !backward && few_rows(s))
+		if (s.rows > 0 && !backward && few_logits(s))
 			space.logits = take(sizeof(float) * rows * s.classes);
 		else if (s.rows > 0)
 		{
@@ -583,7 +591,7 @@ namespace
 		const DistillationSpace space = distillation_space(s, count, false);
 		Partial *partials = at<Partial>(workspace, space.loss.partials);
 		float *kept = at<float>(workspace, space.logits);
-		if (few_rows(s))
+		if (few_logits(s))
 		{
 			const int columns = ceil_div(s.classes, FEW_CLASSES);
 			with_few_rows<T>(s.rows, s.features, [&](auto blocks, auto streamed)
@@ -635,7 +643,7 @@ namespace
 		{
 			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + first_tile, nullptr, count, tiles + 1, 1.0f / temperature };
 		};
-		loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, workspace);
+		loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), workspace);
 	}
 
 	/* the rows' shape with another last dimension */

@@ -635,7 +635,8 @@ namespace mlhip
 	{
 		return piece < s.classes || input_plan(s, piece).parts > 1;
 	}
-	inline LossSpace loss_space(const LossShape &s, bool backward)
+	/* few: whether the forward pass streams the weights past a few rows, which asks for no padded copies */
+	inline LossSpace loss_space(const LossShape &s, bool backward, bool few)
 	{
 		LossSpace space { };
 		size_t at = 0;
@@ -649,7 +650,6 @@ namespace mlhip
 		{
 			const int pieces = 16 / s.element_size;
 			const size_t padded = (s.features % pieces == 0) ? 0 : round_up(s.features, pieces) * s.element_size;
-			const bool few = few_rows(s);
 			/* the forward pass's pieces lie in the same places as far as both have them: one workspace serves both */
 			space.x = take(backward || !few ? padded * s.rows : 0);
 			space.w = take(backward || !few ? padded * s.classes : 0);
@@ -680,9 +680,9 @@ namespace mlhip
 	/* targets: of every row a class that takes what rounding took from the row, or none where the row has no gradient; goal(first): for the piece whose first column of tiles it is */
 	template<typename T, typename GoalOf>
 	void loss_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const int *targets, GoalOf &&goal_of, float slope, const float *lse, const float *dloss, float beta_dx,
-			T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, uint8_t *workspace)
+			T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, bool few, uint8_t *workspace)
 	{
-		const LossSpace space = loss_space(s, true);
+		const LossSpace space = loss_space(s, true, few);
 		const int padded = padded_columns<T>(s.features), most = classes_of_piece(s);
 		T *d = reinterpret_cast<T*>(workspace + space.d);
 		float *partial_dx = reinterpret_cast<float*>(workspace + space.dx), *parts = reinterpret_cast<float*>(workspace + space.parts);

@@ -70,7 +70,7 @@ def check(ctx, data, temperature, dtype):
 
 
 SIZES = [(1, 8, 1, 1), (1, 64, 300, 5), (3, 63, 20, 40), (16, 200, 37, 8), (17, 130, 16, 16), (33, 72, 1000, 64), (64, 333, 100, 3), (65, 40, 513, 100), (130, 65, 257, 256), (300, 200, 130, 17),
-         (129, 1096, 24, 2), (2, 2056, 70, 1), (3500, 24, 3700, 9), (513, 64, 8, 300), (1, 16, 40001, 1024), (2, 8, 300000, 33), (9000, 8, 20, 4), (257, 48, 3000, 65)]
+         (129, 1096, 24, 2), (2, 2056, 70, 1), (3500, 24, 3700, 9), (513, 64, 8, 300), (1, 16, 40001, 1024), (2, 8, 300000, 33), (9000, 8, 20, 4), (257, 48, 3000, 65), (24, 1021, 9000, 12), (17, 1024, 9000, 5)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "float32"])

@@ -258,3 +258,16 @@ def test_distillation_refusals_of_the_mirror():
     for call in (forward, backward, lambda: backward(dx=None, db=None, b=None), lambda: forward(**one, loss=fake((1,), "float32")), lambda: backward(**one, g=fake((1,), "float32"), dx=fake((16,)))):
         with pytest.raises(ValueError, match="null context"):
             call()
+
+
+def test_distillation_workspace_of_odd_widths_holds_the_padded_rows():
+    """Rows that are no multiple of 16 bytes are copied before tiles read them, in the forward pass of more than 16 rows (in fp32 32) of large weights and in every backward pass; also of rows whose cross entropy goes without."""
+    for dtype, element in ((B.DTYPE_FLOAT16, 2), (B.DTYPE_FLOAT32, 4)):
+        for rows, features, classes in ((17, 1021, 32000), (24, 2047, 65536), (32, 1021, 20000), (33, 1021, 32000), (100, 1021, 200000), (4096, 2047, 65536), (7, 2045, 65536), (40, 30, 500)):
+            piece = 16 // element
+            whole = -(-features // piece) * piece
+            for backward in (False, True):
+                size = B.fn("linear_distillation_get_workspace_size")(B.make_shape((rows, features)), B.make_shape((classes, features)), 16, dtype, backward)
+                tiles = rows > (16 if element == 2 else 32) and (rows > 64 or classes * features * element > 1 << 24)
+                least = (rows + classes) * whole * element if backward or tiles else rows * classes * 4
+                assert size >= least + rows * 16 * (16 if tiles else 0)
