@@ -27,9 +27,7 @@ def inputs(rng, rows, features, classes, count, dtype, logits_dtype=None, ignore
 
 
 def space(ctx, x, w, count, backward):
-    t = ml.Tensor((max(1, ml.linearDistillationGetWorkspaceSize(ctx, x, w, count, backward)),), "uint8")
-    t.setall(ctx, 0xff)
-    return t
+    return V.workspace(ctx, ml.linearDistillationGetWorkspaceSize(ctx, x, w, count, backward))
 
 
 class Distillation:
@@ -42,13 +40,16 @@ class Distillation:
         self.named, self.logits = ml.toDevice(ctx, named), guarded(ctx, logits, "float16" if logits.dtype == np.uint16 else "float32", np.nan)
         self.loss, self.lse = (guarded(ctx, np.full(self.rows, np.nan, np.float32), "float32", 9.0) for _ in range(2))
         self.log_p = guarded(ctx, np.full(named.shape, np.nan, np.float32), "float32", 9.0)
-        ml.linearDistillationForward(ctx, self.X, self.W, self.B, self.named, self.logits, temperature, self.loss, self.lse, self.log_p, space(ctx, self.X, self.W, self.count, False))
+        work = space(ctx, self.X, self.W, self.count, False)
+        ml.linearDistillationForward(ctx, self.X, self.W, self.B, self.named, self.logits, temperature, self.loss, self.lse, self.log_p, work)
+        V.check_workspace(ctx, work)
         for t in (self.loss, self.lse, self.log_p):
             check_guards(ctx, t, 9.0)
 
     def backward(self, dloss, dx, dw, db, beta=0.0, beta_weights=0.0):
-        ml.linearDistillationBackward(self.ctx, self.X, self.W, self.B, self.named, self.logits, self.temperature, self.lse, self.log_p, ml.toDevice(self.ctx, dloss), beta, dx, beta_weights, dw, db,
-                                      space(self.ctx, self.X, self.W, self.count, True))
+        work = space(self.ctx, self.X, self.W, self.count, True)
+        ml.linearDistillationBackward(self.ctx, self.X, self.W, self.B, self.named, self.logits, self.temperature, self.lse, self.log_p, ml.toDevice(self.ctx, dloss), beta, dx, beta_weights, dw, db, work)
+        V.check_workspace(self.ctx, work)
 
     def gradients(self, dloss):
         out = [guarded(self.ctx, R.bits(np.full(t.shape, np.nan), self.dtype), self.dtype, 9.0) for t in (self.X, self.W, self.B)]

@@ -23,9 +23,7 @@ def tokens_of(rng, rows, classes, ignored=0.1):
 
 
 def space(ctx, tokens, table):
-    t = ml.Tensor((max(1, ml.embeddingGetWorkspaceSize(ctx, tokens, table)),), "uint8")
-    t.setall(ctx, 0xff)
-    return t
+    return V.workspace(ctx, ml.embeddingGetWorkspaceSize(ctx, tokens, table))
 
 
 @pytest.mark.parametrize("dtype", ["float16", "float32"])
@@ -56,7 +54,9 @@ def test_gradient(ctx, rows, classes, features, dtype, out):
     old = R.bits(rng.standard_normal((classes, features)), out)
     for beta in (0.0, 1.0, -0.75):
         dtable = guarded(ctx, R.bits(np.full(old.shape, np.nan), out) if beta == 0 else old, out, 9.0)
-        ml.embeddingBackward(ctx, T, DY, 0.5, beta, dtable, space(ctx, T, dtable))
+        work = space(ctx, T, dtable)
+        ml.embeddingBackward(ctx, T, DY, 0.5, beta, dtable, work)
+        V.check_workspace(ctx, work)
         kept = beta * R.numbers(old)
         assert R.worst(dtable.copyToHost(ctx), exact + kept, V.embedding_gradient_bound(exact, weighted, kept, out)) <= 1
         check_guards(ctx, dtable, 9.0)

@@ -33,9 +33,9 @@ class Loss:
         self.inputs = [None if a is None else guarded(ctx, a, "float32", np.nan) for a in (nll, old, reference, advantages)] + [ml.toDevice(ctx, targets)]
         sequences = nll.shape[0] if nll.ndim == 2 else 1
         self.loss, self.weights = (guarded(ctx, np.full(n, np.nan, np.float32), "float32", 9.0) for n in (4, sequences))
-        space = ml.Tensor((max(1, ml.policyLossGetWorkspaceSize(ctx, self.inputs[0])),), "uint8")
-        space.setall(ctx, 0xff)
+        space = V.workspace(ctx, ml.policyLossGetWorkspaceSize(ctx, self.inputs[0]))
         ml.policyLossForward(ctx, *self.inputs, CLASSES, clip, kl_weight, average, self.loss, self.weights, space)
+        V.check_workspace(ctx, space)
 
     def gradient(self, dloss=None, beta=0.0, before=None):
         shape = self.inputs[0].shape

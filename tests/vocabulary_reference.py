@@ -1,7 +1,17 @@
 """What a model over a vocabulary learns from, in 64 bits and straight from the definitions, and bounds of what rounding may do to it."""
 import numpy as np
 
+from minml_amd import core as ml
 from training_reference import FP32, STEP, TINY, product_error, rounded
+
+
+def workspace(ctx, size):
+    """A workspace of `size` bytes that holds NaN in both types (nothing may be read before it was written), with as much behind it as tells whether a call kept to it."""
+    return ml.toDevice(ctx, np.full(size + 4096, 0xff, np.uint8)).view((max(1, size),))
+
+
+def check_workspace(ctx, space):
+    assert (space._owner.copyToHost(ctx)[-4095:] == 0xff).all()
 
 
 def embedding(tokens, table, scale):
