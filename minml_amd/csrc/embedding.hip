@@ -302,8 +302,9 @@ namespace
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
 	/*
 	 * A class's rows are added up by those who write its row of the table; but where one class has many (a few tokens are in every line), they would wait for it alone. The list is therefore cut into chunks of 64 places (32 where a row takes
-	 * all threads of a workgroup, so that nothing adds up rows side by side), and of a class of as many rows and more every chunk that it has from its first place on is added up beforehand, by a launch of its own, so that what is
-	 * left is less than a chunk's rows before its first whole chunk and one sum in fp32 for every further one. Neither asks more than the list to know who does what.
+	 * all threads of a workgroup, so that nothing adds up rows side by side), and a class of as many rows and more has every chunk that begins with it added up by a workgroup of its own, beside those
+	 * that write the other classes' rows; a second launch adds these sums in fp32 and the rows before the class's first whole chunk, less than a chunk's, and writes the class's row. None asks more than the list to know who does
+	 * what. (With the chunks in a launch of their own before all rows, which then joined them: us, so / that way, 16384 x 4096 of 65536 classes fp16 173 / 176, 20011 x 1001 of 5003 fp32 43.5 / 45.5.)
 	 */
 	constexpr int MOST_OF_CHUNK = 64;
 	template<typename T, typename Out>
@@ -313,7 +314,7 @@ namespace
 			const T *dy;
 			float *partial; /* [chunks][columns] */
 			Out *out;
-			int count, classes, columns, classes_of_group, lanes, spans, chunk; /* lanes: threads of a row, a power of two; spans: that a row takes of them */
+			int count, classes, columns, classes_of_group, lanes, spans, chunk, chunks; /* chunks: workgroups for them, or 0; lanes: threads of a row, a power of two; spans: that a row takes of them */
 			float scale, beta;
 	};
 	/* the first place of [first, first + length) whose key is not below `key` */
@@ -381,38 +382,105 @@ namespace
 				for (int e = 0; e < VEC; e++)
 					v[e] += meeting[t][e];
 	}
-	template<typename T, typename Out, int VEC>
-	__global__ __launch_bounds__(256) void kernel_chunk_sums(TableGradient<T, Out> p)
+	/* whether the chunk at `first` begins with a class of a chunk's rows and more: as many neighbouring places are the class's with `first` among them. Of a wavefront; the same in all of them */
+	template<typename T, typename Out>
+	__device__ __forceinline__ bool begins_with_many(const TableGradient<T, Out> &p, int first, int key)
 	{
-		__shared__ float meeting[256][VEC];
-		__shared__ int rows[MOST_OF_CHUNK];
-		const int first = blockIdx.x * p.chunk, lane = threadIdx.x & 63;
-		const int key = p.keys[first];
-		if (key >= p.classes)
-			return;
-		/* as many places as a chunk's of one class with the chunk's first one among them; and where the class ends in the chunk */
-		const int from = first - lane, to = from + p.chunk - 1;
+		const int lane = threadIdx.x & 63, from = first - lane, to = from + p.chunk - 1;
 		const bool all = lane < p.chunk && from >= 0 && to < p.count && p.keys[max(from, 0)] == key && p.keys[min(to, p.count - 1)] == key;
-		if (__ballot(all) == 0)
-			return;
-		const bool mine = lane < p.chunk && first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
-		const int here = __popcll(__ballot(mine));
-		if (static_cast<int>(threadIdx.x) < p.chunk)
-			rows[threadIdx.x] = p.positions[min(first + lane, p.count - 1)];
-		__syncthreads();
-		const int column = (blockIdx.y * p.lanes + threadIdx.x % p.lanes) * VEC;
-		const RowPlace place = place_in_row<VEC>(min(column, p.columns - 1), p.columns);
-		float v[VEC];
+		return key < p.classes && __ballot(all) != 0;
+	}
+	/* a thread's column of a row, and where it lies */
+	template<typename T, typename Out, int VEC>
+	struct Column
+	{
+			int group, groups;
+			bool inside;
+			RowPlace place;
+
+			__device__ __forceinline__ Column(const TableGradient<T, Out> &p, int span) :
+					group(threadIdx.x / p.lanes),
+					groups(256 / p.lanes)
+			{
+				const int column = (span * p.lanes + static_cast<int>(threadIdx.x) % p.lanes) * VEC;
+				inside = column < p.columns;
+				place = place_in_row<VEC>(min(column, p.columns - 1), p.columns);
+			}
+			__device__ __forceinline__ const T* of_list(const TableGradient<T, Out> &p, int i) const
+			{
+				return place.in(p.dy + static_cast<size_t>(p.positions[i]) * p.columns);
+			}
+			__device__ __forceinline__ Out* of_table(const TableGradient<T, Out> &p, int c) const
+			{
+				return place.in(p.out + static_cast<size_t>(c) * p.columns);
+			}
+			__device__ __forceinline__ float* of_chunk(const TableGradient<T, Out> &p, int i) const
+			{
+				return place.in(p.partial + static_cast<size_t>(i) * p.columns);
+			}
+			/* old: what is added to, if anything is */
+			__device__ __forceinline__ void write(const TableGradient<T, Out> &p, int c, float (&v)[VEC], const Elements<Out, VEC> &old) const
+			{
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] = p.beta != 0.0f ? fmaf(p.beta, old[e], p.scale * v[e]) : p.scale * v[e];
+				store_nearest<VEC>(of_table(p, c), v, place.skip);
+			}
+	};
+	constexpr int AHEAD = 8;
+	template<int VEC>
+	__device__ __forceinline__ void clear(float (&v)[VEC])
+	{
 #pragma unroll
 		for (int e = 0; e < VEC; e++)
 			v[e] = 0.0f;
-		add_rows<T, 16>(v, threadIdx.x / p.lanes, here, 256 / p.lanes, [&](int i) __attribute__((always_inline))
+	}
+	template<typename T, typename Out, int VEC>
+	__device__ __forceinline__ void sum_chunk(const TableGradient<T, Out> &p, int chunk, int span, float (*meeting)[VEC])
+	{
+		const int first = chunk * p.chunk, lane = threadIdx.x & 63, key = p.keys[first];
+		if (!begins_with_many(p, first, key))
+			return;
+		const bool mine = lane < p.chunk && first + lane < p.count && p.keys[min(first + lane, p.count - 1)] == key;
+		const int here = __popcll(__ballot(mine));
+		const Column<T, Out, VEC> column(p, span);
+		float v[VEC];
+		clear(v);
+		add_rows<T, AHEAD>(v, first + column.group, first + here, column.groups, [&](int i) __attribute__((always_inline))
 		{
-			return place.in(p.dy + static_cast<size_t>(rows[i]) * p.columns);
+			return column.of_list(p, i);
 		});
 		join_groups<VEC>(v, p.lanes, meeting);
-		if (static_cast<int>(threadIdx.x) < p.lanes && column < p.columns)
-			store_nearest<VEC>(place.in(p.partial + static_cast<size_t>(blockIdx.x) * p.columns), v, place.skip);
+		if (column.group == 0 && column.inside)
+			store_nearest<VEC>(column.of_chunk(p, chunk), v, column.place.skip);
+	}
+	/* of the class that has its first whole chunk here: that chunk's sum, the others', and the rows before */
+	template<typename T, typename Out, int VEC>
+	__global__ __launch_bounds__(256) void kernel_join_chunks(TableGradient<T, Out> p)
+	{
+		__shared__ float meeting[256][VEC];
+		const int chunk = blockIdx.x / p.spans, span = blockIdx.x % p.spans, first = chunk * p.chunk, lane = threadIdx.x & 63, key = p.keys[first];
+		if (!begins_with_many(p, first, key) || (chunk > 0 && p.keys[first - p.chunk] == key))
+			return;
+		const bool mine = lane < p.chunk && first - 1 - lane >= 0 && p.keys[max(first - 1 - lane, 0)] == key;
+		const int begin = first - __popcll(__ballot(mine)), end = first + lower_bound_by_wave(p.keys + first, p.count - first, key + 1);
+		const Column<T, Out, VEC> column(p, span);
+		Elements<Out, VEC> old;
+		if (p.beta != 0.0f && column.group == 0)
+			old.load(column.of_table(p, key));
+		float v[VEC];
+		clear(v);
+		add_rows<T, AHEAD>(v, begin + column.group, first, column.groups, [&](int i) __attribute__((always_inline))
+		{
+			return column.of_list(p, i);
+		});
+		add_rows<float, AHEAD>(v, chunk + column.group, (end + p.chunk - 1) / p.chunk, column.groups, [&](int i) __attribute__((always_inline))
+		{
+			return static_cast<const float*>(column.of_chunk(p, i));
+		});
+		join_groups<VEC>(v, p.lanes, meeting);
+		if (column.group == 0 && column.inside)
+			column.write(p, key, v, old);
 	}
 	constexpr int MOST_CLASSES_OF_GROUP = 1024;
 	/* a class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's */
@@ -420,10 +488,11 @@ namespace
 	template<typename T, typename Out, int VEC>
 	__global__ __launch_bounds__(256) void kernel_table_gradient(TableGradient<T, Out> p)
 	{
-		constexpr int AHEAD = 8;
 		__shared__ int bounds[MOST_CLASSES_OF_GROUP + 1], large[MOST_CLASSES_OF_GROUP], ends[2], large_ones;
 		__shared__ float meeting[256][VEC];
-		const int unit = blockIdx.x / p.spans, span = blockIdx.x % p.spans;
+		const int unit = static_cast<int>(blockIdx.x / p.spans) - p.chunks, span = blockIdx.x % p.spans;
+		if (unit < 0)
+			return sum_chunk<T, Out, VEC>(p, unit + p.chunks, span, meeting);
 		const int first_class = unit * p.classes_of_group, classes = min(p.classes_of_group, p.classes - first_class);
 		if (threadIdx.x < 128)
 		{
@@ -449,58 +518,44 @@ namespace
 			for (int c = threadIdx.x; c <= classes; c += 256)
 				bounds[c] = c == 0 ? list_first : c == classes ? list_last : lower_bound(p.keys, list_first, list_last - list_first, first_class + c);
 		__syncthreads();
-		const int column = (span * p.lanes + threadIdx.x % p.lanes) * VEC, groups = 256 / p.lanes, group = threadIdx.x / p.lanes;
-		const bool inside = column < p.columns;
-		const RowPlace place = place_in_row<VEC>(min(column, p.columns - 1), p.columns);
-		const auto of_all = [&](int c)
+		const Column<T, Out, VEC> column(p, span);
+		const int groups = column.groups, group = column.group;
+		/* one group's of threads; the workgroup's; that of the chunks and their joining */
+		const auto rows_of = [&](int c)
 		{
-			const int rows = bounds[c + 1] - bounds[c];
-			return (groups > 1 && rows >= ROWS_OF_ALL) || rows >= p.chunk;
+			return bounds[c + 1] - bounds[c];
 		};
-		const auto row_of_list = [&](int i) __attribute__((always_inline))
+		const auto of_group = [&](int c)
 		{
-			return place.in(p.dy + static_cast<size_t>(p.positions[i]) * p.columns);
-		};
-		const auto row_of_table = [&](int c) __attribute__((always_inline))
-		{
-			return place.in(p.out + static_cast<size_t>(c) * p.columns);
-		};
-		const auto write = [&](int c, float (&v)[VEC], const Elements<Out, VEC> &old) __attribute__((always_inline))
-		{
-#pragma unroll
-			for (int e = 0; e < VEC; e++)
-				v[e] = p.beta != 0.0f ? fmaf(p.beta, old[e], p.scale * v[e]) : p.scale * v[e];
-			store_nearest<VEC>(row_of_table(c), v, place.skip);
+			return rows_of(c) < (groups > 1 ? ROWS_OF_ALL : p.chunk);
 		};
 		for (int c = threadIdx.x; c < classes; c += 256)
-			if (of_all(c))
+			if (!of_group(c) && rows_of(c) < p.chunk)
 				large[atomicAdd(&large_ones, 1)] = c; /* in any order: each has a row of its own */
 		float v[VEC];
 		Elements<Out, VEC> old;
-		if (inside)
+		if (column.inside)
 		{
 			/* neighbouring classes of a group of threads: first those without rows, which wait for nothing; then the others' rows in one go, whichever class they are of */
 			const int each = (classes + groups - 1) / groups, begin = min(group * each, classes), end = min(begin + each, classes);
 			if (p.beta != 1.0f)
 				for (int c = begin; c < end; c++)
-					if (bounds[c] == bounds[c + 1])
+					if (rows_of(c) == 0)
 					{
-#pragma unroll
-						for (int e = 0; e < VEC; e++)
-							v[e] = 0.0f;
+						clear(v);
 						if (p.beta != 0.0f)
-							old.load(row_of_table(first_class + c));
-						write(first_class + c, v, old);
+							old.load(column.of_table(p, first_class + c));
+						column.write(p, first_class + c, v, old);
 					}
 			for (int c = begin; c < end;)
 			{
-				if (of_all(c))
+				if (!of_group(c))
 				{
 					c++;
 					continue;
 				}
 				const int first = bounds[c];
-				while (c < end && !of_all(c))
+				while (c < end && of_group(c))
 					c++;
 				const int last = bounds[c];
 				int current = -1;
@@ -512,7 +567,7 @@ namespace
 					for (int u = 0; u < AHEAD; u++)
 					{
 						key[u] = p.keys[min(i + u, last - 1)];
-						x[u].load(row_of_list(min(i + u, last - 1)));
+						x[u].load(column.of_list(p, min(i + u, last - 1)));
 					}
 					__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -521,13 +576,11 @@ namespace
 						if (key[u] != current)
 						{
 							if (current >= 0)
-								write(current, v, old);
+								column.write(p, current, v, old);
 							current = key[u];
 							if (p.beta != 0.0f)
-								old.load(row_of_table(current));
-#pragma unroll
-							for (int e = 0; e < VEC; e++)
-								v[e] = 0.0f;
+								old.load(column.of_table(p, current));
+							clear(v);
 						}
 #pragma unroll
 						for (int e = 0; e < VEC; e++)
@@ -535,28 +588,23 @@ namespace
 					}
 				}
 				if (current >= 0)
-					write(current, v, old);
+					column.write(p, current, v, old);
 			}
 		}
 		__syncthreads();
 		for (int i = 0; i < large_ones; i++)
 		{
-			const int c = large[i], begin = bounds[c], end = bounds[c + 1];
-			const int chunk = (begin + p.chunk - 1) / p.chunk, direct = end - begin < p.chunk ? end : min(end, chunk * p.chunk);
-#pragma unroll
-			for (int e = 0; e < VEC; e++)
-				v[e] = 0.0f;
+			const int c = large[i];
+			clear(v);
 			if (p.beta != 0.0f && group == 0)
-				old.load(row_of_table(first_class + c));
-			add_rows<T, AHEAD>(v, begin + group, direct, groups, row_of_list);
-			if (direct < end)
-				add_rows<float, AHEAD>(v, chunk + group, (end + p.chunk - 1) / p.chunk, groups, [&](int i) __attribute__((always_inline))
-				{
-					return place.in(static_cast<const float*>(p.partial) + static_cast<size_t>(i) * p.columns);
-				});
+				old.load(column.of_table(p, first_class + c));
+			add_rows<T, AHEAD>(v, bounds[c] + group, bounds[c + 1], groups, [&](int at) __attribute__((always_inline))
+			{
+				return column.of_list(p, at);
+			});
 			join_groups<VEC>(v, p.lanes, meeting);
-			if (group == 0 && inside)
-				write(first_class + c, v, old);
+			if (group == 0 && column.inside)
+				column.write(p, first_class + c, v, old);
 		}
 	}
 
@@ -704,13 +752,17 @@ namespace
 		const int spans = ceil_div(s.columns, lanes * VEC);
 		const size_t units = static_cast<size_t>(s.classes) * spans;
 		const int most = static_cast<int>(std::min<size_t>(std::max(32, 1024 / lanes), std::max<size_t>(1, units / 1024)));
-		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk_of(s, VEC), scale, beta };
-		if (s.rows >= p.chunk)
+		const int chunk = chunk_of(s, VEC), chunks = s.rows >= chunk ? ceil_div(s.rows, chunk) : 0;
+		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk, chunks, scale, beta };
+		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3((static_cast<unsigned int>(ceil_div(s.classes, most)) + chunks) * spans), dim3(256), 0, stream, p);
+		if (chunks > 0)
 		{
-			hipLaunchKernelGGL((kernel_chunk_sums<T, Out, VEC>), dim3(ceil_div(s.rows, p.chunk), spans), dim3(256), 0, stream, p);
-			MLHIP_CHECK(hipGetLastError());
+			/* several groups of threads to a row, however wide it is: a class's chunks wait for one another otherwise */
+			TableGradient<T, Out> joined = p;
+			joined.lanes = std::min(lanes, 64);
+			joined.spans = ceil_div(s.columns, joined.lanes * VEC);
+			hipLaunchKernelGGL((kernel_join_chunks<T, Out, VEC>), dim3(static_cast<unsigned int>(chunks) * joined.spans), dim3(256), 0, stream, joined);
 		}
-		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3(static_cast<unsigned int>(ceil_div(s.classes, most)) * spans), dim3(256), 0, stream, p);
 		MLHIP_CHECK(hipGetLastError());
 	}
 	template<typename T, typename Out>
