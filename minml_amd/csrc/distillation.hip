@@ -519,6 +519,206 @@ namespace
 		}
 	}
 
+	/* ---- backward of few rows ------------------------------------------------------------------------------------------------ */
+	/*
+	 * Up to 16 rows: tiles would be empty but for a few rows, and each of three products would read or write the weights' size for itself on them. Here d is kept in fp32, [classes][rows], 64 bytes of a class at most; making it
+	 * reads the weights once, past the rows, as the forward pass does; dx = d W reads them once more, every thread with its columns of all rows in registers; dW = d^T x writes as much, with its columns of x in registers. Rows of
+	 * any width and alignment are read as they lie. Memory bounds all three. us of loss and gradients, so / on tiles: 1 row fp16 of 2048 x 65536 226 / 270, 1024 x 32000 68 / 98, 1023 x 32000 106 / 144, 1024 x 4000 34 / 53,
+	 * 128 x 100000 80 / 149; 8 rows 262 / 278, 80 / 99, 136 / 152, 46 / 59, 106 / 150; fp32 1024 x 32000 1 row 106 / 202, 16 rows 127 / 205
+	 */
+	constexpr int FEW_GRADIENT_ROWS = 16;
+	template<typename T, bool STREAM>
+	__global__ __launch_bounds__(256) void kernel_few_gradient(const T *x, const T *w, const T *bias, TopClasses goal, const int *anchors, const float *lse, const float *dloss, int rows, int features, int classes, int stride, float *d,
+			void *db, bool db_half, float beta)
+	{
+		extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+		__shared__ float tile[FEW_CLASSES][FEW_GRADIENT_ROWS + 1];
+		float (*sums)[2][16][16] = reinterpret_cast<float (*)[2][16][16]>(lds);
+		const int n0 = blockIdx.x * FEW_CLASSES;
+		const T *first = w + static_cast<size_t>(n0) * features;
+		const bool second = n0 + 16 < classes; /* else the first block stands in for it */
+		const int last_first = min(15, classes - 1 - n0), last_second = second ? min(15, classes - 1 - n0 - 16) : last_first;
+		const T *next = second ? first + static_cast<size_t>(16) * features : first;
+		const int c = threadIdx.x & 15, row = threadIdx.x >> 4, m = min(row, rows - 1);
+		/* a row without gradient has none, whatever its logits are */
+		const float factor = row < rows && anchors[m] >= 0 ? dloss[m] * goal.slope : 0.0f, norm = lse[m];
+		int from = 0, to = 0;
+		if (factor != 0.0f)
+		{
+			const uint16_t *of_row = goal.begins + static_cast<size_t>(m) * goal.stride + blockIdx.x;
+			from = of_row[0];
+			to = of_row[1];
+		}
+		if constexpr (STREAM)
+			few_rows_stream<T, 1>(x, rows, first, next, last_first, last_second, features, lds);
+		else
+			few_rows_sums<T, 1>(x, rows, first, next, last_first, last_second, features, sums);
+#pragma unroll
+		for (int i = 0; i < 2; i++)
+		{
+			const int n = n0 + 16 * i + c;
+			const bool there = factor != 0.0f && n < classes;
+			const float z = sums[0][i][row][c] + ((bias != nullptr && there) ? static_cast<float>(bias[n]) : 0.0f);
+			tile[16 * i + c][row] = there ? factor * expf(goal.less(z, norm)) : 0.0f;
+		}
+		__syncthreads();
+		/* 16 threads share a row's classes; of those that stand there twice the first place has the share */
+		for (int k = from + c; k < to; k += 16)
+		{
+			const size_t place = static_cast<size_t>(m) * goal.count + k;
+			const int n = goal.classes[place];
+			if (k == from || goal.classes[place - 1] != n)
+				tile[n - n0][row] = factor * (goal.known[place] - goal.shares[place]);
+		}
+		__syncthreads();
+		for (int i = threadIdx.x; i < FEW_CLASSES * stride; i += 256)
+			if (n0 + i / stride < classes)
+				d[static_cast<size_t>(n0) * stride + i] = tile[i / stride][i % stride];
+		const int n = n0 + static_cast<int>(threadIdx.x);
+		if (db != nullptr && threadIdx.x < FEW_CLASSES && n < classes)
+		{
+			float sum = 0.0f;
+			for (int r = 0; r < rows; r++)
+				sum += tile[threadIdx.x][r];
+			if (db_half)
+			{
+				half_t *out = reinterpret_cast<half_t*>(db) + n;
+				*out = static_cast<half_t>(beta != 0.0f ? fmaf(beta, static_cast<float>(*out), sum) : sum);
+			}
+			else
+			{
+				float *out = reinterpret_cast<float*>(db) + n;
+				*out = beta != 0.0f ? fmaf(beta, *out, sum) : sum;
+			}
+		}
+	}
+	/* a thread's columns of a row, of which `lanes` threads (a power of two from 64 on) take one; the workgroup's other threads take other classes. Whole wavefronts have the same class, so its row of d comes by scalar loads */
+	template<int VEC>
+	struct FewColumns
+	{
+			int group, groups;
+			bool inside;
+			RowPlace place;
+
+			__device__ __forceinline__ FewColumns(int columns, int lanes) :
+					group(__builtin_amdgcn_readfirstlane(threadIdx.x / lanes)),
+					groups(256 / lanes)
+			{
+				const int column = (blockIdx.y * lanes + static_cast<int>(threadIdx.x) % lanes) * VEC;
+				inside = column < columns;
+				place = place_in_row<VEC>(min(column, columns - 1), columns);
+			}
+	};
+	template<int ROWS>
+	struct ClassRow
+	{
+			float d[ROWS];
+
+			__device__ __forceinline__ void load(const float *src, int n)
+			{
+#pragma unroll
+				for (int r = 0; r < ROWS; r++)
+					d[r] = src[static_cast<size_t>(n) * ROWS + r];
+			}
+	};
+	/* partial[part][row][column]: the part's classes */
+	template<typename T, int VEC, int ROWS>
+	__global__ __launch_bounds__(256) void kernel_few_input(const T *w, const float *d, int rows, int columns, int classes, int classes_of_part, int lanes, float *partial)
+	{
+		constexpr int AHEAD = 4;
+		__shared__ float meeting[256][VEC];
+		const FewColumns<VEC> column(columns, lanes);
+		const int first = blockIdx.x * classes_of_part, last = first + min(classes_of_part, classes - first);
+		float sums[ROWS][VEC];
+#pragma unroll
+		for (int r = 0; r < ROWS; r++)
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				sums[r][e] = 0.0f;
+		const auto add = [&](const Elements<T, VEC> &weights, int n) __attribute__((always_inline))
+		{
+			ClassRow<ROWS> of_class;
+			of_class.load(d, n);
+#pragma unroll
+			for (int r = 0; r < ROWS; r++)
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					sums[r][e] = fmaf(of_class.d[r], weights[e], sums[r][e]);
+		};
+		int n = first + column.group;
+		for (; n + (AHEAD - 1) * column.groups < last; n += AHEAD * column.groups)
+		{
+			Elements<T, VEC> weights[AHEAD];
+#pragma unroll
+			for (int u = 0; u < AHEAD; u++)
+				weights[u].load(column.place.in(w + static_cast<size_t>(n + u * column.groups) * columns));
+			__builtin_amdgcn_sched_barrier(0); /* all on their way before one is waited for */
+#pragma unroll
+			for (int u = 0; u < AHEAD; u++)
+				add(weights[u], n + u * column.groups);
+		}
+		for (; n < last; n += column.groups)
+		{
+			Elements<T, VEC> weights;
+			weights.load(column.place.in(w + static_cast<size_t>(n) * columns));
+			add(weights, n);
+		}
+#pragma unroll
+		for (int r = 0; r < ROWS; r++)
+		{
+			if (column.groups > 1)
+			{
+				__syncthreads();
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					meeting[threadIdx.x][e] = sums[r][e];
+				__syncthreads();
+				if (column.group == 0)
+					for (int t = threadIdx.x + lanes; t < 256; t += lanes)
+#pragma unroll
+						for (int e = 0; e < VEC; e++)
+							sums[r][e] += meeting[t][e];
+			}
+			if (r < rows && column.group == 0 && column.inside)
+				store_nearest<VEC>(column.place.in(partial + (static_cast<size_t>(blockIdx.x) * rows + r) * columns), sums[r], column.place.skip);
+		}
+	}
+	template<typename T, typename Out, int VEC, int ROWS>
+	__global__ __launch_bounds__(256) void kernel_few_weights(const T *x, const float *d, int rows, int columns, int classes, int classes_of_group, int lanes, Out *out, float beta)
+	{
+		const FewColumns<VEC> column(columns, lanes);
+		Elements<T, VEC> of_row[ROWS];
+#pragma unroll
+		for (int r = 0; r < ROWS; r++)
+			of_row[r].load(column.place.in(x + static_cast<size_t>(min(r, rows - 1)) * columns)); /* of rows that are not there d is zero */
+		if (!column.inside)
+			return;
+		const int first = blockIdx.x * classes_of_group, last = first + min(classes_of_group, classes - first);
+		for (int n = first + column.group; n < last; n += column.groups)
+		{
+			ClassRow<ROWS> of_class;
+			of_class.load(d, n);
+			Out *dst = column.place.in(out + static_cast<size_t>(n) * columns);
+			Elements<Out, VEC> old;
+			if (beta != 0.0f)
+				old.load(dst);
+			float v[VEC];
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				v[e] = 0.0f;
+#pragma unroll
+			for (int r = 0; r < ROWS; r++)
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] = fmaf(of_class.d[r], of_row[r][e], v[e]);
+			if (beta != 0.0f)
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					v[e] = fmaf(beta, old[e], v[e]);
+			store_nearest<VEC>(dst, v, column.place.skip);
+		}
+	}
+
 	/* ---- sizes ---------------------------------------------------------------------------------------------------------------- */
 	/*
 	 * The cross entropy's rule, but that 17 to 32 rows of large weights in fp16 go on tiles: they fill two blocks of 16 rows, and their logits are kept. us of a forward pass, so / on tiles: 24 rows fp16 of 2048 x 65536 67 / 56,
@@ -528,15 +728,47 @@ namespace
 	{
 		return few_rows(s) && (s.rows <= 16 || s.element_size == 4 || static_cast<size_t>(s.classes) * s.features * s.element_size <= (size_t(1) << 24));
 	}
+	/* beyond, 16 rows in fp16 (us of loss and gradients, so / on tiles: 2048 x 65536 332 / 281, 1024 x 32000 101 / 100), the vector units bound the products, which take an element of the weights times every row */
+	bool few_gradients(const LossShape &s)
+	{
+		return s.rows <= (s.element_size == 2 ? 8 : FEW_GRADIENT_ROWS);
+	}
+	struct FewGradientPlan
+	{
+			int stride, vector, lanes, spans; /* rows of d's layout, a power of two; elements of a thread; threads and workgroups of a row */
+			int parts, classes_of_part; /* of dx */
+			int classes_of_group; /* of dW */
+	};
+	FewGradientPlan few_gradient_plan(const LossShape &s)
+	{
+		FewGradientPlan plan { };
+		plan.stride = 1;
+		while (plan.stride < s.rows)
+			plan.stride *= 2;
+		plan.vector = s.features >= 16 / s.element_size ? 16 / s.element_size : 1;
+		plan.lanes = 64;
+		while (plan.lanes < 256 && plan.lanes * plan.vector < s.features)
+			plan.lanes *= 2;
+		plan.spans = ceil_div(s.features, plan.lanes * plan.vector);
+		/* a workgroup to every compute unit and a second one, whatever the width; no less than four classes to a group of threads */
+		plan.classes_of_part = std::max(4 * 256 / plan.lanes, ceil_div(s.classes, std::max(1, 512 / plan.spans)));
+		plan.parts = ceil_div(s.classes, plan.classes_of_part);
+		plan.classes_of_group = std::max(256 / plan.lanes, ceil_div(s.classes, std::max(1, 2048 / plan.spans)));
+		return plan;
+	}
 	struct DistillationSpace
 	{
 			LossSpace loss;
-			size_t classes, places, shares, known, begins, anchors, entropies, logits, total;
+			size_t classes, places, shares, known, begins, anchors, entropies, logits;
+			size_t d, partial; /* backward of few rows */
+			size_t total;
 	};
 	DistillationSpace distillation_space(const LossShape &s, int count, bool backward)
 	{
 		DistillationSpace space { };
-		space.loss = loss_space(s, backward, few_logits(s));
+		const bool few = backward && few_gradients(s);
+		if (!few)
+			space.loss = loss_space(s, backward, few_logits(s));
 		size_t at = space.loss.total;
 		const auto take = [&](size_t bytes)
 		{
@@ -553,7 +785,13 @@ namespace
 			space.places = take(sizeof(uint16_t) * places);
 			space.shares = take(sizeof(float) * places);
 			space.logits = space.known = take(sizeof(float) * places);
-			space.begins = take(sizeof(uint16_t) * rows * (ceil_div(s.classes, tile_width(s, backward ? classes_of_piece(s) : s.classes)) + 1));
+			space.begins = take(sizeof(uint16_t) * rows * (ceil_div(s.classes, few ? FEW_CLASSES : tile_width(s, backward ? classes_of_piece(s) : s.classes)) + 1));
+			if (few)
+			{
+				const FewGradientPlan plan = few_gradient_plan(s);
+				space.d = take(sizeof(float) * s.classes * plan.stride);
+				space.partial = take(sizeof(float) * plan.parts * rows * s.features);
+			}
 			space.anchors = take(sizeof(int) * rows);
 			space.entropies = take(sizeof(float) * rows);
 		}
@@ -631,19 +869,82 @@ namespace
 					log_probabilities);
 		MLHIP_CHECK(hipGetLastError());
 	}
+	/* f(rows of d's layout, a power of two) as a compile-time constant */
+	template<typename T, typename F>
+	void with_stride(int stride, F &&f)
+	{
+		switch (stride)
+		{
+			case 1:
+				return f(std::integral_constant<int, 1>());
+			case 2:
+				return f(std::integral_constant<int, 2>());
+			case 4:
+				return f(std::integral_constant<int, 4>());
+			case 8:
+				return f(std::integral_constant<int, 8>());
+			default:
+				if constexpr (sizeof(T) == 4)
+					return f(std::integral_constant<int, 16>());
+				else
+					fail_logic("HIP backend: d of 16 rows is for fp32");
+		}
+	}
+	template<typename T>
+	void few_gradients(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const TopClasses &goal, const Teaching &teaching, const float *lse, const float *dloss, float beta_dx, T *dx,
+			float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, float *d, float *partial)
+	{
+		const FewGradientPlan plan = few_gradient_plan(s);
+		const bool stream_rows = (s.features * sizeof(T)) % 16 == 0;
+		const int bytes = few_rows_lds<1>(stream_rows);
+		auto kernel = stream_rows ? kernel_few_gradient<T, true> : kernel_few_gradient<T, false>;
+		ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
+		hipLaunchKernelGGL(kernel, dim3(ceil_div(s.classes, FEW_CLASSES)), dim3(256), bytes, stream, x, w, bias, goal, teaching.anchors, lse, dloss, s.rows, s.features, s.classes, plan.stride, d, db.data,
+				db.dtype == DTYPE_FLOAT16, beta_weights);
+		MLHIP_CHECK(hipGetLastError());
+		const auto products = [&](auto vector, auto stride)
+		{
+			constexpr int VEC = decltype(vector)::value, ROWS = decltype(stride)::value;
+			if (dx != nullptr)
+			{
+				hipLaunchKernelGGL((kernel_few_input<T, VEC, ROWS>), dim3(plan.parts, plan.spans), dim3(256), 0, stream, w, d, s.rows, s.features, s.classes, plan.classes_of_part, plan.lanes, partial);
+				MLHIP_CHECK(hipGetLastError());
+				const int outputs = s.rows * s.features;
+				launch_sum_partials(stream, partial, plan.parts, outputs, dx, sizeof(T) == 2 ? DTYPE_FLOAT16 : DTYPE_FLOAT32, outputs, beta_dx);
+			}
+			const dim3 grid(ceil_div(s.classes, plan.classes_of_group), plan.spans);
+			if (dw.data != nullptr && dw.dtype == DTYPE_FLOAT32)
+				hipLaunchKernelGGL((kernel_few_weights<T, float, VEC, ROWS>), grid, dim3(256), 0, stream, x, d, s.rows, s.features, s.classes, plan.classes_of_group, plan.lanes, ptr<float>(dw), beta_weights);
+			else if constexpr (sizeof(T) == 2)
+				if (dw.data != nullptr)
+					hipLaunchKernelGGL((kernel_few_weights<T, T, VEC, ROWS>), grid, dim3(256), 0, stream, x, d, s.rows, s.features, s.classes, plan.classes_of_group, plan.lanes, ptr<T>(dw), beta_weights);
+			MLHIP_CHECK(hipGetLastError());
+		};
+		with_stride<T>(plan.stride, [&](auto stride)
+		{
+			if (plan.vector == 1)
+				products(std::integral_constant<int, 1>(), stride);
+			else
+				products(std::integral_constant<int, 16 / sizeof(T)>(), stride);
+		});
+	}
 	template<typename T>
 	void distillation_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const mlTensor_t &classes, const mlTensor_t &logits, int count, float temperature, const float *lse,
 			const float *log_probabilities, const float *dloss, float beta_dx, T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, uint8_t *workspace)
 	{
 		const DistillationSpace space = distillation_space(s, count, true);
 		const Teaching teaching = teaching_of(workspace, space);
-		const int width = tile_width(s, classes_of_piece(s)), tiles = ceil_div(s.classes, width);
+		const bool few = few_gradients(s);
+		const int width = few ? FEW_CLASSES : tile_width(s, classes_of_piece(s)), tiles = ceil_div(s.classes, width);
 		sort_teacher(stream, s, classes, logits, log_probabilities, count, temperature, width, teaching);
 		const auto goal = [&](int first_tile)
 		{
 			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + first_tile, nullptr, count, tiles + 1, 1.0f / temperature };
 		};
-		loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), workspace);
+		if (few)
+			few_gradients(stream, s, x, w, bias, goal(0), teaching, lse, dloss, beta_dx, dx, beta_weights, dw, db, at<float>(workspace, space.d), at<float>(workspace, space.partial));
+		else
+			loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), workspace);
 	}
 
 	/* the rows' shape with another last dimension */

@@ -227,13 +227,13 @@ def test_distillation_refusals_of_the_library():
 
 
 def test_distillation_workspace_does_not_grow_with_rows_times_classes():
-    """What the cross entropy's backward pass holds, 16 bytes for every place and 2 for every row of every tile; for few rows also their logits in the forward pass."""
+    """What the cross entropy's backward pass holds, 16 bytes for every place and 2 for every row of every tile; for few rows their logits or gradients of them, 2 bytes of every 32 classes, and up to 512 sums of dx."""
     for dtype in (B.DTYPE_FLOAT16, B.DTYPE_FLOAT32):
         for rows, features, classes, count in ((4096, 2048, 65536, 64), (5000, 64, 200000, 1024), (7, 2048, 65536, 16), (64, 64, 1000, 3)):
             shapes = B.make_shape((rows, features)), B.make_shape((classes, features))
             size = B.fn("linear_distillation_get_workspace_size")(*shapes, count, dtype, True)
             other = B.fn("linear_cross_entropy_get_workspace_size")(*shapes, dtype, True)
-            assert size <= other + rows * (16 * count + 2 * (classes // 128 + 2) + 8) + (4 * rows * classes if rows <= 64 else 0) + 4096
+            assert size <= other + rows * (16 * count + 2 * (classes // 128 + 2) + 8) + (5 * rows * classes if rows <= 64 else 0) + (512 * 4 * rows * features if rows <= 16 else 0) + 4096
 
 
 def test_distillation_refusals_of_the_mirror():
@@ -261,7 +261,8 @@ def test_distillation_refusals_of_the_mirror():
 
 
 def test_distillation_workspace_of_odd_widths_holds_the_padded_rows():
-    """Rows that are no multiple of 16 bytes are copied before tiles read them, in the forward pass of more than 16 rows (in fp32 32) of large weights and in every backward pass; also of rows whose cross entropy goes without."""
+    """Rows that are no multiple of 16 bytes are copied before tiles read them, in the forward pass of more than 16 rows (in fp32 32) of large weights, where the cross entropy goes without, and in the
+    backward pass of more than 8 (16)."""
     for dtype, element in ((B.DTYPE_FLOAT16, 2), (B.DTYPE_FLOAT32, 4)):
         for rows, features, classes in ((17, 1021, 32000), (24, 2047, 65536), (32, 1021, 20000), (33, 1021, 32000), (100, 1021, 200000), (4096, 2047, 65536), (7, 2045, 65536), (40, 30, 500)):
             piece = 16 // element
@@ -269,5 +270,5 @@ def test_distillation_workspace_of_odd_widths_holds_the_padded_rows():
             for backward in (False, True):
                 size = B.fn("linear_distillation_get_workspace_size")(B.make_shape((rows, features)), B.make_shape((classes, features)), 16, dtype, backward)
                 tiles = rows > (16 if element == 2 else 32) and (rows > 64 or classes * features * element > 1 << 24)
-                least = (rows + classes) * whole * element if backward or tiles else rows * classes * 4
+                least = (rows + classes) * whole * element if tiles or (backward and rows > (8 if element == 2 else 16)) else rows * classes * 4
                 assert size >= least + rows * 16 * (16 if tiles else 0)
