@@ -10,6 +10,8 @@
  * The passes are the cross entropy's (vocabulary_loss.hpp). What is new is that a row has many classes of its own, spread over the tiles of logits. A launch before sorts every row's classes and notes where each column of tiles
  * begins among them; then one thread of a tile has a row's few in that tile, and they meet the logits in LDS, through which the tile goes anyway in the backward pass, and in the forward pass where it has any.
  * In the backward pass the student's probability at these places is known from the forward pass's log p, so that d there is p - q in fp32, rounded once, however close p and q are.
+ * fp16, what it takes beside the cross entropy of the same size: 2048 rows of 1024 x 50001, 32 classes a row, 245 to 267 us, card to card (the products 257 / 246, sorting 9); 4096 of 2048 x 65536, 64 classes, loss and gradients
+ * 3.96 to 4.05 ms (products 1030 / 1003, making d 562 / 560 twice, sorting 13 twice). 3 rows of 1024 x 32000 18.5 us (14.2 at 4.6 TB/s, 5.2 to join). What bounds the rest is said there.
  */
 #include "vocabulary_loss.hpp"
 

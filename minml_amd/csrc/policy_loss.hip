@@ -6,7 +6,7 @@
  * The result is the mean over the tokens, or over the sequences' means; the gradient of n is the token's weight times ([not clipped] r A + kl_weight (exp(q) - 1)).
  * Whether a token is clipped is decided in 64 bits by o - n against the logarithm of the border (r > 1 + high where A > 0, r < 1 - low where A < 0), so no rounding of an exponential moves a token across it.
  * kl of close models is a small number from which 1 and q have been taken: below |q| = 1/2 it is q^2 (1/2 + q/6 + ..), where nothing cancels. Sums are in 64 bits: gains have both signs and cancel.
- * Memory bounds both passes: 12 to 20 bytes of a token.
+ * Memory bounds both passes, 12 to 20 bytes of a token: 1024 sequences of 8191 tokens, all five inputs, 28 us and 5 to join the sums (6.0 TB/s), the gradient 30 (6.8, partly from the last-level cache); 512 x 1024 6.2 and 2.9.
  */
 #include "training_utils.hpp"
 
@@ -241,25 +241,31 @@ namespace
 		}
 	}
 
-	/* few tokens: everything by one workgroup, a wavefront to a sequence */
-	constexpr int FEW_TOKENS = 8192, FEW_SEQUENCES = 256;
-	template<int VEC>
-	__global__ __launch_bounds__(1024) void kernel_policy_few(PolicyArgs p, bool average_sequences, float *loss, float *weights)
+	/* few tokens: everything by one workgroup, LANES threads to a sequence */
+	constexpr int FEW_THREADS = 1024, FEW_SEQUENCES = 512;
+	template<int LANES, int VEC>
+	__global__ __launch_bounds__(FEW_THREADS) void kernel_policy_few(PolicyArgs p, bool average_sequences, float *loss, float *weights)
 	{
-		constexpr int WAVES = 16;
+		constexpr int WAVES = FEW_THREADS / 64;
 		__shared__ Sums waves[WAVES];
 		__shared__ int counts[FEW_SEQUENCES];
-		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 		Sums total { 0.0, 0.0, 0.0, 0.0 };
-		for (int s = wave; s < p.sequences; s += WAVES)
+		for (int s0 = 0; s0 < p.sequences; s0 += FEW_THREADS / LANES)
 		{
-			Sums sums = lanes_sum<64>(sums_of_thread<64, VEC>(p, s, 0, p.length));
-			if (lane == 0)
+			const int s = s0 + static_cast<int>(threadIdx.x) / LANES;
+			Sums sums { 0.0, 0.0, 0.0, 0.0 };
+			if (s < p.sequences)
+				sums = sums_of_thread<LANES, VEC>(p, s, 0, p.length);
+			sums = lanes_sum<LANES>(sums);
+			if (s < p.sequences && threadIdx.x % LANES == 0)
+			{
 				counts[s] = static_cast<int>(sums.count);
-			total = total + (average_sequences ? mean_of_sequence(sums) : sums);
+				total = total + (average_sequences ? mean_of_sequence(sums) : sums);
+			}
 		}
-		if (lane == 0)
-			waves[wave] = total;
+		total = lanes_sum<64>(total);
+		if ((threadIdx.x & 63) == 0)
+			waves[threadIdx.x >> 6] = total;
 		__syncthreads();
 		total = waves[0];
 #pragma unroll
@@ -268,7 +274,7 @@ namespace
 		const double each = total.count > 0.0 ? 1.0 / total.count : 0.0;
 		if (threadIdx.x == 0)
 			write_loss(total, each, p.kl_weight, loss);
-		for (int s = threadIdx.x; s < p.sequences; s += 64 * WAVES)
+		for (int s = threadIdx.x; s < p.sequences; s += FEW_THREADS)
 			weights[s] = weight_of_sequence(counts[s], each, average_sequences);
 	}
 
@@ -312,7 +318,10 @@ namespace
 			int lanes, sequences_of_group, groups, chunks, chunk_length;
 	};
 	constexpr int MOST_GROUPS = 1024;
-	/* every group's sums are read by the join, so there are 1024 of them at most; sequences are cut where there are too few of them to give every compute unit work */
+	/*
+	 * Every group's sums are read by the join, so there are 1024 of them at most; sequences are cut where there are too few of them to give every compute unit work. us of a forward call, sequences of up to 1024 tokens by a
+	 * wavefront / by a workgroup: 4096 x 1024 19.0 / 22.9, 4096 x 300 12.6 / 19.4, 2048 x 1024 12.4 / 15.0, 2048 x 512 12.2 / 13.8; 512 x 1024 12.8 / 12.4, of which the sums are 7.9 / 6.2
+	 */
 	PolicyPlan policy_plan(int sequences, int length)
 	{
 		PolicyPlan plan { };
@@ -340,13 +349,24 @@ namespace
 		MLHIP_REQUIRE(sequences <= (1 << 28) && length <= (1 << 28), who + ": too many sequences or tokens");
 		return PolicyShape { sequences, length };
 	}
-	bool few_tokens(const PolicyShape &s)
+	/*
+	 * Threads of a sequence where one workgroup does everything, or 0 where two launches do. It takes about 2 us for every time that a thread goes to memory, and saves what a launch costs: us of a forward call and (on the device),
+	 * so / in two launches: 4 x 113 tokens, once, 9.6 (3.6) / 12 (5.4); 32 x 128, twice, 9.5 (7.7) / 12 (6.7); 32 x 512, four times, 10.1 (9.5) / 12 (6.7); 64 x 500, eight times, 17 (17) / 12 (6.6)
+	 */
+	int lanes_of_few(const PolicyShape &s)
 	{
-		return s.sequences <= FEW_SEQUENCES && static_cast<size_t>(s.sequences) * s.length <= FEW_TOKENS;
+		if (s.sequences > FEW_SEQUENCES)
+			return 0;
+		const auto times = [&](int lanes)
+		{
+			return static_cast<long long>(ceil_div(s.sequences, FEW_THREADS / lanes)) * ceil_div(s.length, 4 * lanes);
+		};
+		const int lanes = times(8) < times(64) ? 8 : 64;
+		return times(lanes) <= 4 ? lanes : 0;
 	}
 	size_t policy_space(const PolicyShape &s)
 	{
-		if (few_tokens(s))
+		if (lanes_of_few(s) > 0)
 			return 0;
 		const PolicyPlan plan = policy_plan(s.sequences, s.length);
 		return round_up(sizeof(Sums) * (plan.chunks > 0 ? static_cast<size_t>(s.sequences) * plan.chunks : plan.groups), 256) + sizeof(int) * s.sequences;
@@ -407,12 +427,18 @@ extern "C"
 		const OnDeviceOf on(context);
 		const PolicyPlan plan = policy_plan(p.sequences, p.length);
 		const bool average_sequences = average == AVERAGE_SEQUENCES;
-		if (few_tokens(s))
+		if (const int lanes = lanes_of_few(s))
 		{
+			const auto launch = [&](auto kernel)
+			{
+				hipLaunchKernelGGL(kernel, dim3(1), dim3(FEW_THREADS), 0, on.stream, p, average_sequences, ptr<float>(loss), ptr<float>(weights));
+			};
 			if (p.length < 4)
-				hipLaunchKernelGGL((kernel_policy_few<1>), dim3(1), dim3(1024), 0, on.stream, p, average_sequences, ptr<float>(loss), ptr<float>(weights));
+				launch(kernel_policy_few<8, 1>);
+			else if (lanes == 8)
+				launch(kernel_policy_few<8, 4>);
 			else
-				hipLaunchKernelGGL((kernel_policy_few<4>), dim3(1), dim3(1024), 0, on.stream, p, average_sequences, ptr<float>(loss), ptr<float>(weights));
+				launch(kernel_policy_few<64, 4>);
 			MLHIP_CHECK(hipGetLastError());
 			return;
 		}
