@@ -841,7 +841,7 @@ def _require_embedding(tokens, table):
 def embeddingForward(context, tokens, table, scale, output):
     """output = scale * table[tokens]: tokens int32 [..], table [classes, features], output [.., features]. A token that is no class of the table gives zeros."""
     _require_embedding(tokens, table)
-    _require(_same_dtype(table, output) and output.volume() == tokens.volume() * table.shape[1] and output.shape[-1] == table.shape[1], "output must be [.., features] of the table's type")
+    _require(_same_dtype(table, output) and output.volume() == tokens.volume() * table.shape[1] and tuple(output.shape[-1:]) == (table.shape[1],), "output must be [.., features] of the table's type")
     _launch("embedding_forward", context.handle, tokens.desc(), table.desc(), scale, output.desc())
 
 
@@ -854,7 +854,7 @@ def embeddingBackward(context, tokens, gradient, scale, beta_weights, gradient_t
     """gradient_table = beta_weights * gradient_table + scale * (the rows of `gradient` [.., features] of every class added up), of the gradient's type or fp32."""
     _require_embedding(tokens, gradient_table)
     _require(gradient.dtype in _FLOATS and gradient_table.dtype in (gradient.dtype, B.DTYPE_FLOAT32), "the table's gradient must be of the gradient's type or fp32")
-    _require(gradient.volume() == tokens.volume() * gradient_table.shape[1] and gradient.shape[-1] == gradient_table.shape[1], "the gradient must be [.., features]")
+    _require(gradient.volume() == tokens.volume() * gradient_table.shape[1] and tuple(gradient.shape[-1:]) == (gradient_table.shape[1],), "the gradient must be [.., features]")
     _launch("embedding_backward", context.handle, tokens.desc(), gradient.desc(), scale, beta_weights, gradient_table.desc(), *_space(workspace))
 
 

@@ -12,6 +12,7 @@
 #include "training_utils.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <tuple>
 #include <utility>
 
@@ -303,7 +304,7 @@ namespace
 	/* ---- backward ----------------------------------------------------------------------------------------------------------- */
 	/*
 	 * A class's rows are added up by those who write its row of the table; but where one class has many (a few tokens are in every line), they would wait for it alone. The list is therefore cut into chunks of 64 places (32 where a row takes
-	 * all threads of a workgroup, so that nothing adds up rows side by side), and a class of as many rows and more has every chunk that begins with it added up by a workgroup of its own, beside those
+	 * all threads of a workgroup, so that nothing adds up rows side by side: 20011 x 1001 of 5003 fp32 43.5 us, with 64 45), and a class of as many rows and more has every chunk that begins with it added up by a workgroup of its own, beside those
 	 * that write the other classes' rows; a second launch adds these sums in fp32 and the rows before the class's first whole chunk, less than a chunk's, and writes the class's row. None asks more than the list to know who does
 	 * what. (With the chunks in a launch of their own before all rows, which then joined them: us, so / that way, 16384 x 4096 of 65536 classes fp16 173 / 176, 20011 x 1001 of 5003 fp32 43.5 / 45.5.)
 	 */
@@ -484,7 +485,9 @@ namespace
 			column.write(p, key, v, old);
 	}
 	constexpr int MOST_CLASSES_OF_GROUP = 1024;
-	/* a class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's */
+	/*
+	 * A class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's. us with 8 / 16 / 32: 57600 x 256 of 400 classes 28.0 / 28.1 / 30.2, 65536 x 64 of 131072 59 / 54 / 50
+	 */
 	constexpr int ROWS_OF_ALL = 16;
 	template<typename T, typename Out, int VEC>
 	__global__ __launch_bounds__(256) void kernel_table_gradient(TableGradient<T, Out> p)
@@ -646,14 +649,12 @@ namespace
 	{
 		return s.rows <= (s.classes < 2048 ? 2048 : 8192);
 	}
-	/* threads that a row takes, a power of two; fewer where there are few classes, so that there are workgroups enough and groups of threads in each of them to share a class's chunks */
+	/* threads that a row takes, a power of two */
 	int lanes_of_row(const EmbeddingShape &s, int vector)
 	{
 		int lanes = 1;
 		while (lanes < 256 && lanes * vector < s.columns)
 			lanes *= 2;
-		while (lanes > 32 && static_cast<size_t>(s.classes) * ceil_div(s.columns, lanes * vector) < 2048)
-			lanes /= 2;
 		return lanes;
 	}
 	int chunk_of(const EmbeddingShape &s, int vector)
@@ -707,6 +708,7 @@ namespace
 			const size_t groups = std::min<size_t>((count + 256 * each - 1) / (256 * each), 1 << 20);
 			hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, tokens, table, y, s.rows, s.columns, s.classes, vectors, scale);
 		};
+		/* a vector to a thread / four of them, us on the device: 4096 x 256 fp16 2.7 / 3.3, 16384 x 256 4.6 / 4.6, 32768 x 256 6.5 / 6.1, 65536 x 256 9.9 / 9.1 */
 		if (count < (1 << 19))
 			launch(kernel_embedding_forward<T, VEC, 1>, 1);
 		else
@@ -752,6 +754,7 @@ namespace
 		const int lanes = lanes_of_row(s, VEC);
 		const int spans = ceil_div(s.columns, lanes * VEC);
 		const size_t units = static_cast<size_t>(s.classes) * spans;
+		/* classes of a workgroup: their search is its beginning, but four workgroups to a compute unit come first. us with 16 / 32 / 64 at most for wide rows: 16384 x 4096 of 65536 174 / 172 / 176 */
 		const int most = static_cast<int>(std::min<size_t>(std::max(32, 1024 / lanes), std::max<size_t>(1, units / 1024)));
 		const int chunk = chunk_of(s, VEC), chunks = s.rows >= chunk ? ceil_div(s.rows, chunk) : 0;
 		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk, chunks, scale, beta };
@@ -801,6 +804,7 @@ extern "C"
 		const char *name = "embedding_forward";
 		const EmbeddingShape s = embedding_shape(shape_of(tokens), shape_of(table), table.dtype, name);
 		check_tokens(tokens, s, name);
+		MLHIP_REQUIRE(std::isfinite(scale), "embedding_forward: the scale must be finite");
 		MLHIP_REQUIRE(y.dtype == table.dtype && rows_of(y, s), "embedding_forward: the result must hold a row of the table's type and width for every token");
 		if (s.rows == 0)
 			return;
@@ -842,6 +846,7 @@ extern "C"
 			return;
 		const EmbeddingShape s = embedding_shape(shape_of(tokens), shape_of(dtable), dy.dtype, name);
 		check_tokens(tokens, s, name);
+		MLHIP_REQUIRE(std::isfinite(scale), "embedding_backward: the scale must be finite"); /* classes without tokens get zeros, not zero times it */
 		MLHIP_REQUIRE(rows_of(dy, s), "embedding_backward: there must be a gradient of the table's width for every token");
 		MLHIP_REQUIRE(dtable.dtype == dy.dtype || dtable.dtype == DTYPE_FLOAT32, "embedding_backward: the table's gradient must be of the gradients' type or fp32");
 		const EmbeddingSpace space = embedding_space(s, dy.dtype);

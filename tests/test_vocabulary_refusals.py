@@ -12,7 +12,9 @@ class Ctx:
 
 def test_embedding_refusals_of_the_library():
     t, w, y = fake((4,), "int32").desc(), fake((90, 16)).desc(), fake((4, 16)).desc()
-    forward = lambda t=t, w=w, y=y, why=None: refused("embedding_forward", t, w, 2.0, y, why=why)
+    forward = lambda t=t, w=w, y=y, scale=2.0, why=None: refused("embedding_forward", t, w, scale, y, why=why)
+    for scale in (float("inf"), float("nan")):
+        forward(scale=scale, why="scale")
     forward(t=fake((4,), "float32").desc(), why="int32")
     forward(t=NULL)
     forward(t=ml.Tensor((4,), "int32", _ptr=0x7002).desc(), why="misaligned")
@@ -30,7 +32,9 @@ def test_embedding_refusals_of_the_library():
     size = B.fn("embedding_get_workspace_size")(fake((5000,), "int32").shape_desc(), fake((90, 16)).shape_desc(), B.DTYPE_FLOAT16)
     assert size >= 5000 * 8
     t, dy = fake((5000,), "int32").desc(), fake((5000, 16)).desc()
-    backward = lambda t=t, dy=dy, dw=w, space=0x7000, n=size, why=None: refused("embedding_backward", t, dy, 1.0, 0.0, dw, space, n, why=why)
+    backward = lambda t=t, dy=dy, dw=w, space=0x7000, n=size, scale=1.0, why=None: refused("embedding_backward", t, dy, scale, 0.0, dw, space, n, why=why)
+    for scale in (float("-inf"), float("nan")):
+        backward(scale=scale, why="scale")
     backward(t=fake((4999,), "int32").desc())
     backward(dy=fake((5000, 8)).desc())
     backward(dy=fake((5000, 16), "int8").desc())
@@ -58,11 +62,20 @@ def test_embedding_refuses_what_its_counters_do_not_reach():
             B.fn("embedding_get_workspace_size")(shape(8), shape(8, 8), dtype)
 
 
+def test_embedding_workspace_of_fp32_is_enough_for_fp16():
+    """A table's gradient in fp32 of rows in fp16: the size may be asked for with either type."""
+    for rows in (1, 31, 33, 5000, 70000):
+        for classes in (1, 300, 3000, 100000):
+            for features in (1, 5, 64, 520, 1000, 1032, 2048, 4100):
+                half, full = (B.fn("embedding_get_workspace_size")(B.make_shape((rows,)), B.make_shape((classes, features)), d) for d in (B.DTYPE_FLOAT16, B.DTYPE_FLOAT32))
+                assert full >= half > 0
+
+
 def test_embedding_refusals_of_the_mirror():
     t, w, y = fake((2, 3), "int32"), fake((90, 16)), fake((2, 3, 16))
     space = ml.Tensor((1 << 22,), "uint8", _ptr=1 << 50)
     for call in (lambda: ml.embeddingForward(Ctx, fake((2, 3)), w, 1.0, y), lambda: ml.embeddingForward(Ctx, t, w, 1.0, fake((2, 16))), lambda: ml.embeddingForward(Ctx, t, w, 1.0, fake((2, 3, 16), "float32")),
-                 lambda: ml.embeddingForward(Ctx, t, fake((16,)), 1.0, y), lambda: ml.embeddingBackward(Ctx, t, fake((2, 3, 8)), 1.0, 0.0, w, space),
+                 lambda: ml.embeddingForward(Ctx, t, fake((16,)), 1.0, y), lambda: ml.embeddingForward(Ctx, t, w, 1.0, fake(())), lambda: ml.embeddingForward(Ctx, fake((), "int32"), w, 1.0, y), lambda: ml.embeddingBackward(Ctx, t, fake((2, 3, 8)), 1.0, 0.0, w, space),
                  lambda: ml.embeddingBackward(Ctx, t, fake((2, 3, 16), "float32"), 1.0, 0.0, w, space), lambda: ml.embeddingBackward(Ctx, t, y, 1.0, 0.0, w, None)):
         with pytest.raises(ValueError):
             call()
