@@ -269,10 +269,10 @@ extern "C"
 		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, b, targets, lse, dloss }, name);
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), ptr<int>(targets), goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, few_rows(s),
+			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), GivenBack<half_t> { ptr<int>(targets), nullptr, nullptr, nullptr }, goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, few_rows(s),
 					reinterpret_cast<uint8_t*>(workspace));
 		else
-			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), ptr<int>(targets), goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db, few_rows(s),
+			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), GivenBack<float> { ptr<int>(targets), nullptr, nullptr, nullptr }, goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db, few_rows(s),
 					reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)

@@ -9,7 +9,8 @@
  * A place k whose class c is none of the layer's, or whose logit v is -inf, does not count; a row without any that does has loss 0 and no gradient. A class that a row names twice has the sum of both probabilities.
  * The passes are the cross entropy's (vocabulary_loss.hpp). What is new is that a row has many classes of its own, spread over the tiles of logits. A launch before sorts every row's classes and notes where each column of tiles
  * begins among them; then one thread of a tile has a row's few in that tile, and they meet the logits in LDS, through which the tile goes anyway in the backward pass, and in the forward pass where it has any.
- * In the backward pass the student's probability at these places is known from the forward pass's log p, so that d there is p - q in fp32, rounded once, however close p and q are.
+ * In the backward pass the student's probability at these places is known from the forward pass's log p, so that d there is p - q in fp32, rounded once, however close p and q are. In fp16, what rounding takes from d's rows is given back to the row of W with the teacher's largest share, as much as is its own, and
+ * the rest to the mean of rows that teachers name: dx is 2.3e-4 to 2.8e-4 off (norm), of which its own rounding is 2.1e-4; 2 to 4 us more than all of it to one class (3964 / 3974 of 4096 x 2048 x 65536, 78.5 / 82.5 of 40 x 512 x 20000).
  * fp16, what it takes beside the cross entropy of the same size: 2048 rows of 1024 x 50001, 32 classes a row, 245 to 267 us, card to card (the products 257 / 246, sorting 9); 4096 of 2048 x 65536, 64 classes, loss and gradients
  * 3.96 to 4.05 ms (products 1030 / 1003, making d 562 / 560 twice, sorting 13 twice). 3 rows of 1024 x 32000 18.5 us (14.2 at 4.6 TB/s, 5.2 to join). What bounds the rest is said there.
  */
@@ -34,6 +35,8 @@ namespace
 			uint16_t *begins; /* [rows][column tiles + 1]: how many of them lie before a column of tiles */
 			int *anchors; /* [rows]: the class with the largest share, -1 where none counts */
 			float *entropies; /* forward, [rows]: sum of q log q */
+			float *own, *there; /* backward in fp16, [rows] and one: zeros, and whether there is a common row */
+			half_t *common; /* [features in whole tiles]: what rows of the weights have in common */
 	};
 	template<typename V>
 	__device__ __forceinline__ V lanes_max(V v)
@@ -43,11 +46,58 @@ namespace
 			v = max(v, __shfl_xor(v, offset));
 		return v;
 	}
-	/* a wavefront per row. What a class's place is, is counted: as many classes are smaller, or equal and named before. L: type of the logits */
+	/*
+	 * The mean of up to 64 of the teacher's classes' rows of weights, taken evenly over what it names; one of four places that counts, for each. A class that the teacher names is one that the model is trained for, whose row of W
+	 * looks like those that d is large at. Columns behind the features: zeros. 64 columns to a workgroup, 16 rows to a wavefront
+	 */
+	constexpr int COMMON_ROWS = 64, COMMON_COLUMNS = 256; /* COMMON_COLUMNS: the widest tile's, which reads them without asking where they end */
 	template<typename L>
-	__global__ __launch_bounds__(256) void kernel_sort_teacher(const int *classes_in, const L *logits, const float *log_probabilities, int rows, int count, int classes, float temperature, int width, int tiles, Teaching out)
+	__device__ __forceinline__ void common_row(const int *classes_in, const L *logits, size_t places, int classes, const half_t *w, int features, int column0, half_t *common, float *there)
+	{
+		__shared__ int named[4][COMMON_ROWS];
+		__shared__ float sums[4][64];
+		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+		const size_t asked = min(places, static_cast<size_t>(4 * COMMON_ROWS));
+		named[wave][lane] = -1;
+		if (threadIdx.x < asked)
+		{
+			const size_t place = threadIdx.x * places / asked;
+			const int c = classes_in[place];
+			if (c >= 0 && c < classes && !(static_cast<float>(logits[place]) == -std::numeric_limits<float>::infinity()))
+				named[wave][lane] = c;
+		}
+		__syncthreads();
+		int mine = -1; /* of the lane's four places */
+#pragma unroll
+		for (int k = 3; k >= 0; k--)
+			mine = named[k][lane] >= 0 ? named[k][lane] : mine;
+		const int rows = __popcll(__ballot(mine >= 0)), column = column0 + lane;
+		float v[COMMON_ROWS / 4];
+#pragma unroll
+		for (int u = 0; u < COMMON_ROWS / 4; u++)
+		{
+			const int c = __shfl(mine, wave * (COMMON_ROWS / 4) + u);
+			v[u] = c >= 0 && column < features ? static_cast<float>(w[static_cast<size_t>(c) * features + column]) : 0.0f;
+		}
+		float sum = 0.0f;
+#pragma unroll
+		for (int u = 0; u < COMMON_ROWS / 4; u++)
+			sum += v[u];
+		sums[wave][lane] = sum;
+		__syncthreads();
+		if (wave == 0)
+			common[column] = static_cast<half_t>((sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]) / static_cast<float>(max(rows, 1)));
+		if (column0 == 0 && threadIdx.x == 0)
+			*there = rows > 0 ? 1.0f : 0.0f;
+	}
+	/* a wavefront per row; workgroups behind the rows': common_row. What a class's place is, is counted: as many classes are smaller, or equal and named before. L: type of the logits */
+	template<typename L>
+	__global__ __launch_bounds__(256) void kernel_sort_teacher(const int *classes_in, const L *logits, const float *log_probabilities, int rows, int count, int classes, float temperature, int width, int tiles, const half_t *w, int features, Teaching out)
 	{
 		extern __shared__ int memory[];
+		const int groups = (rows + 3) / 4;
+		if (static_cast<int>(blockIdx.x) >= groups)
+			return common_row(classes_in, logits, static_cast<size_t>(rows) * count, classes, w, features, (static_cast<int>(blockIdx.x) - groups) * 64, out.common, out.there);
 		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave;
 		if (row >= rows)
 			return;
@@ -132,6 +182,8 @@ namespace
 			out.anchors[row] = best_at >= 0 ? sorted[best_at] : -1;
 			if (log_probabilities == nullptr)
 				out.entropies[row] = entropy;
+			if (w != nullptr)
+				out.own[row] = 0.0f;
 		}
 		/* several columns of tiles at a time, by halves of the row's classes: no read of LDS waits for another column's */
 		constexpr int AT_A_TIME = 8;
@@ -169,6 +221,8 @@ namespace
 			float *logits; /* forward: [rows][count] */
 			int count, stride; /* stride: of begins */
 			float slope; /* 1 / t */
+			const int *anchors; /* backward: of every row the class whose part of what rounding took is kept for itself, in own; own null: of none */
+			float *own;
 
 			/*
 			 * A thread's row of the tile and its classes there: first .. last - 1 of the row's, the first two of them with what is known of them. Asked for when the tile is complete, before anything is computed of it: the
@@ -177,7 +231,7 @@ namespace
 			static constexpr int AHEAD = 2;
 			struct OfTile
 			{
-					int row, m, first, last, named[AHEAD];
+					int row, m, first, last, anchor, named[AHEAD];
 					float share[AHEAD], probability[AHEAD], factor;
 			};
 			template<bool BACKWARD, int BM, int BN>
@@ -187,6 +241,7 @@ namespace
 				t.row = threadIdx.x;
 				t.m = at.tile_m * BM + t.row;
 				t.first = t.last = 0;
+				t.anchor = -1;
 				t.factor = 0.0f;
 				if (t.row < BM && t.m < rows)
 				{
@@ -197,6 +252,8 @@ namespace
 					{
 						t.factor = factors[t.m];
 						t.last = t.factor != 0.0f ? t.last : t.first;
+						if (own != nullptr)
+							t.anchor = anchors[t.m];
 					}
 				}
 #pragma unroll
@@ -344,6 +401,8 @@ namespace
 						const T rounded = static_cast<T>(d);
 						taken += (d - static_cast<float>(rounded)) - (pf - static_cast<float>(*stored));
 						*stored = rounded;
+						if (n == of_tile.anchor)
+							own[of_tile.m] = d - static_cast<float>(rounded);
 						if (fabsf(qf) < std::numeric_limits<float>::infinity())
 							atomicAdd(&extra.columns[column], static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(qf) * static_cast<double>(1ll << FIXED_BITS))));
 						else
@@ -761,7 +820,7 @@ namespace
 	struct DistillationSpace
 	{
 			LossSpace loss;
-			size_t classes, places, shares, known, begins, anchors, entropies, logits;
+			size_t classes, places, shares, known, begins, anchors, entropies, logits, own, common, there;
 			size_t d, partial; /* backward of few rows */
 			size_t total;
 	};
@@ -796,6 +855,12 @@ namespace
 			}
 			space.anchors = take(sizeof(int) * rows);
 			space.entropies = take(sizeof(float) * rows);
+			if (backward && !few && s.element_size == 2)
+			{
+				space.own = take(sizeof(float) * rows);
+				space.there = take(sizeof(float));
+				space.common = take(sizeof(half_t) * round_up(s.features, COMMON_COLUMNS));
+			}
 		}
 		space.total = at;
 		return space;
@@ -808,15 +873,18 @@ namespace
 	Teaching teaching_of(uint8_t *workspace, const DistillationSpace &space)
 	{
 		return Teaching { at<int>(workspace, space.classes), at<uint16_t>(workspace, space.places), at<float>(workspace, space.shares), at<float>(workspace, space.known), at<uint16_t>(workspace, space.begins),
-				at<int>(workspace, space.anchors), at<float>(workspace, space.entropies) };
+				at<int>(workspace, space.anchors), at<float>(workspace, space.entropies), at<float>(workspace, space.own), at<float>(workspace, space.there), at<half_t>(workspace, space.common) };
 	}
-	void sort_teacher(hipStream_t stream, const LossShape &s, const mlTensor_t &classes, const mlTensor_t &logits, const float *log_probabilities, int count, float temperature, int width, const Teaching &out)
+	/* w: for the common row, else null */
+	void sort_teacher(hipStream_t stream, const LossShape &s, const mlTensor_t &classes, const mlTensor_t &logits, const float *log_probabilities, int count, float temperature, int width, const half_t *w,
+			const Teaching &out)
 	{
 		const int tiles = ceil_div(s.classes, width), bytes = 4 * 4 * static_cast<int>(sizeof(int)) * count;
+		const int groups = ceil_div(s.rows, 4) + (w != nullptr ? static_cast<int>(round_up(s.features, COMMON_COLUMNS)) / 64 : 0);
 		const auto launch = [&](auto kernel, auto values)
 		{
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
-			hipLaunchKernelGGL(kernel, dim3(ceil_div(s.rows, 4)), dim3(256), bytes, stream, ptr<int>(classes), values, log_probabilities, s.rows, count, s.classes, temperature, width, tiles, out);
+			hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), bytes, stream, ptr<int>(classes), values, log_probabilities, s.rows, count, s.classes, temperature, width, tiles, w, s.features, out);
 		};
 		if (logits.dtype == DTYPE_FLOAT16)
 			launch(kernel_sort_teacher<half_t>, static_cast<const half_t*>(ptr<half_t>(logits)));
@@ -855,8 +923,8 @@ namespace
 		}
 		const Teaching teaching = teaching_of(workspace, space);
 		const int width = tile_width(s, s.classes), columns = ceil_div(s.classes, width), padded = padded_columns<T>(s.features);
-		sort_teacher(stream, s, classes, logits, nullptr, count, temperature, width, teaching);
-		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, kept, count, columns + 1, 1.0f / temperature };
+		sort_teacher(stream, s, classes, logits, nullptr, count, temperature, width, nullptr, teaching);
+		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, kept, count, columns + 1, 1.0f / temperature, nullptr, nullptr };
 		x = pad_rows(stream, x, at<T>(workspace, space.loss.x), s.rows, s.features);
 		w = pad_rows(stream, w, at<T>(workspace, space.loss.w), s.classes, s.features);
 		const ProductPlan plan = logits_plan(s, s.classes);
@@ -938,15 +1006,24 @@ namespace
 		const Teaching teaching = teaching_of(workspace, space);
 		const bool few = few_gradients(s);
 		const int width = few ? FEW_CLASSES : tile_width(s, classes_of_piece(s)), tiles = ceil_div(s.classes, width);
-		sort_teacher(stream, s, classes, logits, log_probabilities, count, temperature, width, teaching);
+		GivenBack<T> to { teaching.anchors, nullptr, nullptr, nullptr };
+		const half_t *for_common = nullptr;
+		if constexpr (sizeof(T) == 2)
+			if (!few && dx != nullptr)
+			{
+				to = GivenBack<T> { teaching.anchors, teaching.own, teaching.common, teaching.there };
+				for_common = w;
+			}
+		sort_teacher(stream, s, classes, logits, log_probabilities, count, temperature, width, for_common, teaching);
 		const auto goal = [&](int first_tile)
 		{
-			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + first_tile, nullptr, count, tiles + 1, 1.0f / temperature };
+			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + first_tile, nullptr, count, tiles + 1, 1.0f / temperature, teaching.anchors,
+					for_common != nullptr ? teaching.own : nullptr };
 		};
 		if (few)
 			few_gradients(stream, s, x, w, bias, goal(0), teaching, lse, dloss, beta_dx, dx, beta_weights, dw, db, at<float>(workspace, space.d), at<float>(workspace, space.partial));
 		else
-			loss_backward(stream, s, x, w, bias, teaching.anchors, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), workspace);
+			loss_backward(stream, s, x, w, bias, to, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), workspace);
 	}
 
 	/* the rows' shape with another last dimension */

@@ -280,7 +280,7 @@ namespace mlhip
 	 * d, the sums of its columns for db, and what rounding to fp16 took from its rows. The elements of a row add up to zero by definition, so that what the rows of W have in common has no part in dx; their roundings
 	 * do not, and with W's common part ten times the rest dx would be 1.9e-3 off (2.8e-4 without one). What was taken from a row is therefore added up here, in fp32, and given back to the target's class when dx is made,
 	 * dx += lost W[target]: the row adds up to zero again, and the target's element, the largest of d by far until a model is sure of something else, counts unrounded. dx is 2.1e-4 off then, as much as its own rounding
-	 * costs, and 2.6e-4 where other classes have large probabilities; dW, where nothing cancels, 2.8e-4.
+	 * costs, and 2.6e-4 where other classes have large probabilities; dW, where nothing cancels, 2.8e-4. A goal that makes many elements large has more places to give it back to (GivenBack).
 	 */
 	template<typename T, typename Goal>
 	struct GradientEpilogue
@@ -427,10 +427,27 @@ namespace mlhip
 			}
 	};
 	/*
+	 * Where what rounding took from a row goes: to the target's row of W; or only the target's own part e_a, and the rest to c, a row that stands for what all rows of W have in common. Either way dx has no error of that common
+	 * part. It has sum e_j (W_j - W_a) or sum e_j (W_j - c), j other than a; where e_a is not most of it, the first is about twice the second's square: of distillations dx is 2.9e-4 to 3.3e-4 off, or 2.3e-4 to 2.8e-4.
+	 */
+	template<typename T>
+	struct GivenBack
+	{
+			const int *targets; /* of every row a class, or none where the row has no gradient */
+			const float *own; /* [rows], and the others: null where everything goes to the target */
+			const T *common; /* in whole tiles of columns, zeros behind the features */
+			const float *there; /* 0: no such row was found */
+
+			__device__ __forceinline__ bool splits() const
+			{
+				return own != nullptr && *there != 0.0f;
+			}
+	};
+	/*
 	 * dx = back (sum + lost W[target]) + beta dx in fp16, where one product gives all of dx: in the accumulators, so that nothing in fp32 goes to memory. us, so / over fp32 and the launch that joins parts / without
 	 * giving back: gradients of 65536 x 1024, 300 classes 383 / 521 / 363, 8192 x 4096, 1000 classes 387 / 442 / 376, 16384 x 2048, 4000 classes 1031 / 1075 / 986 (its rows of W, 67 MB, come from beyond the L2).
 	 */
-	template<typename T>
+	template<typename T, bool ONE>
 	struct InputEpilogue
 	{
 			T *out;
@@ -438,7 +455,7 @@ namespace mlhip
 			float beta;
 			const float *back, *lost;
 			int lost_tiles;
-			const int *targets;
+			GivenBack<T> to;
 			int classes;
 			const T *w;
 			int w_elements;
@@ -461,7 +478,7 @@ namespace mlhip
 				vec_t weights_of[TURNS]; /* all on their way at once: one workgroup has the unit to itself and would wait for each */
 #pragma unroll
 				for (int u = 0; u < TURNS; u++)
-					target[u] = targets[min(first + row0 + u * AT_A_TIME, rows - 1)];
+					target[u] = to.targets[min(first + row0 + u * AT_A_TIME, rows - 1)];
 #pragma unroll
 				for (int u = 0; u < TURNS; u++)
 				{
@@ -497,6 +514,19 @@ namespace mlhip
 				for (int u = 0; u < TURNS; u++)
 					*reinterpret_cast<vec_t*>(stage.place + (row0 + u * AT_A_TIME) * TileStage::STRIDE + column) = weights_of[u];
 				__syncthreads();
+				float rest[BLOCKS];
+				const bool splits = !ONE && to.splits();
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++)
+				{
+					rest[i] = 0.0f;
+					if (splits)
+					{
+						const float own = to.own[min(first + at.row(i), rows - 1)];
+						rest[i] = taken[i] - own;
+						taken[i] = own;
+					}
+				}
 				Acc whole[BLOCKS][2];
 #pragma unroll
 				for (int i = 0; i < BLOCKS; i++)
@@ -509,6 +539,13 @@ namespace mlhip
 #pragma unroll
 							for (int e = 0; e < 4; e++)
 								whole[i][j][4 * q + e] = fmaf(taken[i], static_cast<float>(weights[e]), acc[i][j][4 * q + e]);
+							if (splits)
+							{
+								const typename TileStage::vec4_t common = *reinterpret_cast<const typename TileStage::vec4_t*>(to.common + at.tile_n * BN + at.column(j) + at.lane_column(q));
+#pragma unroll
+								for (int e = 0; e < 4; e++)
+									whole[i][j][4 * q + e] = fmaf(rest[i], static_cast<float>(common[e]), whole[i][j][4 * q + e]);
+							}
 						}
 				StoreEpilogue<T> { out, columns, beta, back }.template tile<BM, BN>(whole, at, lds, rows);
 			}
@@ -519,11 +556,12 @@ namespace mlhip
 	 */
 	template<typename T>
 	__global__ __launch_bounds__(256) void kernel_join_input(const float *partial, int parts, int rows, int features, int spans, T *dx, float beta, const float *back, const float *lost, int lost_tiles,
-			const int *targets, int classes, const T *w, int w_elements)
+			GivenBack<T> to, int classes, const T *w, int w_elements)
 	{
 		const int lane = threadIdx.x & 63;
 		const size_t units = static_cast<size_t>(rows) * spans, count = static_cast<size_t>(rows) * features;
 		const float scale = *back;
+		const bool splits = to.splits();
 		for (size_t unit = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); unit < units; unit += static_cast<size_t>(gridDim.x) * 4)
 		{
 			int span;
@@ -532,7 +570,13 @@ namespace mlhip
 			for (int t = lane; t < lost_tiles; t += 64)
 				taken += lost[row * lost_tiles + t];
 			taken = lanes_sum<64>(taken);
-			const int target = targets[row];
+			float rest = 0.0f;
+			if (splits)
+			{
+				rest = taken - to.own[row];
+				taken = to.own[row];
+			}
+			const int target = to.targets[row];
 			const bool given = target >= 0 && target < classes; /* else nothing was lost, and there is no row of weights to look at */
 			const T *weights = w + static_cast<size_t>(given ? target : 0) * w_elements;
 			const int column = span * 256 + lane * 4;
@@ -552,14 +596,19 @@ namespace mlhip
 					for (int e = 0; e < 4; e++)
 						v[e] += x[e];
 				}
-				Elements<T, 4> of_target, old;
+				Elements<T, 4> of_target, common, old;
 				of_target.load(place.in(weights));
+				if (splits)
+					common.load(place.in(to.common));
 				if (beta != 0.0f)
 					old.load(place.in(dst));
 #pragma unroll
 				for (int e = 0; e < 4; e++)
 				{
-					v[e] = scale * (given ? fmaf(taken, of_target[e], v[e]) : v[e]);
+					v[e] = given ? fmaf(taken, of_target[e], v[e]) : v[e];
+					if (splits && given)
+						v[e] = fmaf(rest, common[e], v[e]);
+					v[e] *= scale;
 					if (beta != 0.0f)
 						v[e] = fmaf(beta, old[e], v[e]);
 				}
@@ -571,7 +620,10 @@ namespace mlhip
 					float v = 0.0f;
 					for (int p = 0; p < parts; p++)
 						v += src[p * count + c];
-					v = scale * (given ? fmaf(taken, static_cast<float>(weights[c]), v) : v);
+					v = given ? fmaf(taken, static_cast<float>(weights[c]), v) : v;
+					if (splits && given)
+						v = fmaf(rest, static_cast<float>(to.common[c]), v);
+					v *= scale;
 					dst[c] = static_cast<T>(beta != 0.0f ? fmaf(beta, static_cast<float>(dst[c]), v) : v);
 				}
 		}
@@ -677,9 +729,9 @@ namespace mlhip
 		return space;
 	}
 
-	/* targets: of every row a class that takes what rounding took from the row, or none where the row has no gradient; goal(first): for the piece whose first column of tiles it is */
+	/* goal(first): for the piece whose first column of tiles it is */
 	template<typename T, typename GoalOf>
-	void loss_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const int *targets, GoalOf &&goal_of, float slope, const float *lse, const float *dloss, float beta_dx,
+	void loss_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const GivenBack<T> &to, GoalOf &&goal_of, float slope, const float *lse, const float *dloss, float beta_dx,
 			T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, bool few, uint8_t *workspace)
 	{
 		const LossSpace space = loss_space(s, true, few);
@@ -690,11 +742,11 @@ namespace mlhip
 		float *largest = reinterpret_cast<float*>(workspace + space.scale), *back = largest + SCALE_GROUPS;
 		const int groups = std::min(ceil_div(s.rows, 256), SCALE_GROUPS);
 		if (s.rows <= ROWS_OF_ONE_GROUP)
-			hipLaunchKernelGGL(kernel_row_factors_of_few, dim3(1), dim3(1024), 0, stream, dloss, targets, s.rows, s.classes, slope, factors, back);
+			hipLaunchKernelGGL(kernel_row_factors_of_few, dim3(1), dim3(1024), 0, stream, dloss, to.targets, s.rows, s.classes, slope, factors, back);
 		else
 		{
-			hipLaunchKernelGGL(kernel_largest_gradient, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest);
-			hipLaunchKernelGGL(kernel_row_factors, dim3(groups), dim3(256), 0, stream, dloss, targets, s.rows, s.classes, largest, groups, slope, factors, back);
+			hipLaunchKernelGGL(kernel_largest_gradient, dim3(groups), dim3(256), 0, stream, dloss, to.targets, s.rows, s.classes, largest);
+			hipLaunchKernelGGL(kernel_row_factors, dim3(groups), dim3(256), 0, stream, dloss, to.targets, s.rows, s.classes, largest, groups, slope, factors, back);
 		}
 		MLHIP_CHECK(hipGetLastError());
 		x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
@@ -729,7 +781,7 @@ namespace mlhip
 				if (in_parts)
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
 				else if constexpr (sizeof(T) == 2)
-					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, InputEpilogue<T> { dx, s.features, beta_dx, back, lost, lost_tiles, targets, s.classes, w, padded });
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, InputEpilogue<T, decltype(goal_of(0))::ONE> { dx, s.features, beta_dx, back, lost, lost_tiles, to, s.classes, w, padded });
 				else
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, StoreEpilogue<T> { dx, s.features, beta_dx, back });
 			}
@@ -753,7 +805,7 @@ namespace mlhip
 				const int spans = ceil_div(s.features, 256);
 				const size_t groups = std::min<size_t>((static_cast<size_t>(s.rows) * spans + 3) / 4, 1 << 16);
 				hipLaunchKernelGGL((kernel_join_input<T>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, partial_dx, whole_input.parts, s.rows, s.features, spans, dx, beta_dx, back, lost,
-						lost_tiles, targets, s.classes, w, padded);
+						lost_tiles, to, s.classes, w, padded);
 				MLHIP_CHECK(hipGetLastError());
 			}
 			else

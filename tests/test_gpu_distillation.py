@@ -172,6 +172,21 @@ def test_one_class_of_the_teacher_is_the_cross_entropy(ctx):
             assert (np.abs(R.numbers(got) - R.numbers(same.copyToHost(ctx))) <= 2 * off).all()
 
 
+@pytest.mark.parametrize("common", [0, 10])
+@pytest.mark.parametrize("rows,features,classes,count,ignored", [(40, 512, 2000, 24, 0.1), (300, 200, 900, 64, 0.1), (1100, 96, 300, 1, 0.1), (1500, 1024, 256, 40, 0.1), (600, 333, 500, 16, 0.99)])
+def test_fp16_gradients_are_off_by_their_roundings_alone(ctx, rows, features, classes, count, ignored, common):
+    """Teachers and students that are sure of nothing, so that no class has most of d, also where the rows of W have much in common: dx is as far off as random roundings are. The sum over rows x features (20480 at least) and,
+    for d, rows x as many classes as are likely, is within a tenth of what is expected."""
+    rng = np.random.default_rng(rows + common)
+    x, w, b, named, logits, _ = inputs(rng, rows, features, classes, count, "float16", ignored=ignored)
+    w, logits = R.bits(R.numbers(w) + common * 2 / np.sqrt(features) * rng.standard_normal(features), "float16"), R.bits(np.where(np.isneginf(R.numbers(logits)), -np.inf, R.numbers(logits) / 3), "float16")
+    dloss = rng.uniform(0.5, 1, rows).astype(np.float32) * rng.choice([-1, 1], rows).astype(np.float32)
+    step = Distillation(ctx, x, w, b, named, logits, 2.0, "float16")
+    args = [R.numbers(a) for a in (x, w, b)] + [named, R.numbers(logits), 2.0, dloss.astype(np.float64)]
+    error = np.linalg.norm(R.numbers(step.gradients(dloss)[0]) - V.distillation_gradients(*args)[0])
+    assert error <= 1.1 * V.distillation_input_noise(*args)
+
+
 def test_rows_without_a_teacher_and_without_gradient(ctx):
     rng = np.random.default_rng(9)
     for rows in (9, 90):

@@ -127,9 +127,18 @@ def distillation_gradients(x, w, b, classes, logits, temperature, dloss):
     return d @ w, d.T @ x, d.sum(0)
 
 
+def common_row(w, classes, logits):
+    """The mean of up to 64 of the rows of W that the teacher names, by one of four places of 256 each."""
+    named, places = np.where(np.isneginf(logits), -1, classes).reshape(-1), min(classes.size, 256)
+    named = named[np.arange(places) * classes.size // places]
+    named = np.pad(np.where((named >= 0) & (named < len(w)), named, -1), (0, 256 - places), constant_values=-1).reshape(4, 64)
+    named = named[(named >= 0).argmax(0), np.arange(64)]
+    return w[named[named >= 0]].mean(0) if (named >= 0).any() else None
+
+
 def distillation_gradient_bounds(x, w, b, classes, logits, temperature, dloss, dtype):
-    """dx in fp16: with e_j what rounding takes from d_j, and -sum e_j given back to the class a with the teacher's largest share, it is off by sum e_j W_j - (sum e_j) W_a = sum over j other than a of
-    e_j (W_j - W_a), so by |e_j| (|W_j| + |W_a|) for each of them at most: the sums of d's errors with |W|, and their sum for the row times |W_a|."""
+    """dx in fp16: e_j is what rounding takes from d_j. For a, the class with the teacher's largest share, it is given back to W_a, for all others to c, the common row, or to W_a where no row is common. So dx is off by the
+    sum over j other than a of e_j (W_j - c), by |e_j| (|W_j| + |c|) for each of them at most: the sums of d's errors with |W|, and their sum for the row times |c|."""
     _, lse, _, z = distillation(x, w, b, classes, logits, temperature)
     dense, _, kept = teacher(classes, logits, len(w), temperature)
     weight = np.where(kept.any(1), np.abs(dloss), 0)[:, None] / temperature
@@ -140,7 +149,28 @@ def distillation_gradient_bounds(x, w, b, classes, logits, temperature, dloss, d
     d = np.abs(p - dense) * weight
     # d is kept in the tensors' type, times 2^15 over a power of two that is at most twice the largest |dloss|
     stored = off + STEP[dtype] * d + TINY[dtype] * 2.0 ** -14 * weight.max(initial=0)
-    given_back = stored.sum(1, keepdims=True) * np.abs(w[dense.argmax(1)]) if dtype == "float16" else 0
+    common = common_row(w, classes, logits)
+    given_back = stored.sum(1, keepdims=True) * np.abs(w[dense.argmax(1)] if common is None else common) if dtype == "float16" else 0
     dx, dw, db = distillation_gradients(x, w, b, classes, logits, temperature, dloss)
     return (rounded(dx, dtype) + product_error(d, w, dtype) + stored @ np.abs(w) + given_back, rounded(dw, dtype) + product_error(d.T, x, dtype) + stored.T @ np.abs(x),
             rounded(db, dtype) + off.sum(0) + (x.shape[0] + 80) * FP32 * (weight * (p + dense)).sum(0))
+
+
+def spacing(v):
+    """From an fp16 number's size to the next."""
+    return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(v), 2.0 ** -14))) - 10)
+
+
+def distillation_input_noise(x, w, b, classes, logits, temperature, dloss):
+    """The 2-norm that the error of dx in fp16 has where roundings are as good as random, evenly over a spacing, whose mean square is a twelfth: of every element of d but the largest share's, times W_j - c, and of dx."""
+    dense, _, kept = teacher(classes, logits, len(w), temperature)
+    _, lse, _, z = distillation(x, w, b, classes, logits, temperature)
+    scale = 2.0 ** 15
+    d = (np.exp(z - lse[:, None]) - dense) * np.where(kept.any(1), dloss, 0)[:, None] / temperature
+    squares = (spacing(d * scale) / scale) ** 2
+    squares[np.arange(len(d)), dense.argmax(1)] = 0
+    squares[~kept.any(1)] = 0
+    common = common_row(w, classes, logits)
+    to = w[dense.argmax(1)] if common is None else np.broadcast_to(common, x.shape)
+    away = (w ** 2).sum(1) - 2 * to @ w.T + (to ** 2).sum(1)[:, None]
+    return np.sqrt(((squares * away).sum() + (spacing(d @ w) ** 2).sum()) / 12)
