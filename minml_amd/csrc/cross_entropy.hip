@@ -81,9 +81,13 @@ namespace
 			{
 			}
 			template<int BM, int BN>
-			__device__ __forceinline__ Nothing begin_gradient(const TilePlace<BM, BN>&, int, const float*, uint8_t*) const
+			__device__ __forceinline__ Nothing begin_gradient(const TilePlace<BM, BN>&, int, const float*) const
 			{
 				return Nothing { };
+			}
+			template<int BM, int BN>
+			__device__ __forceinline__ void begin_sums(uint8_t*) const
+			{
 			}
 			template<int BM, int BN, int ROWS, typename TileStage>
 			__device__ __forceinline__ void correct(const TileStage&, uint8_t*, const TilePlace<BM, BN>&, const Nothing&, int, int) const

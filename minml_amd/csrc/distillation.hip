@@ -373,11 +373,16 @@ namespace
 					}
 			};
 			template<int BM, int BN>
-			__device__ __forceinline__ OfTile begin_gradient(const TilePlace<BM, BN> &at, int rows, const float *factors, uint8_t *lds) const
+			__device__ __forceinline__ OfTile begin_gradient(const TilePlace<BM, BN> &at, int rows, const float *factors) const
+			{
+				return classes_of<true>(at, rows, factors);
+			}
+			/* the place may be an operand's until every wavefront is through with the product */
+			template<int BM, int BN>
+			__device__ __forceinline__ void begin_sums(uint8_t *lds) const
 			{
 				for (int i = threadIdx.x; i < gradient_lds<BM, BN>() / 4; i += TilePlace<BM, BN>::THREADS)
 					reinterpret_cast<int*>(lds)[i] = 0;
-				return classes_of<true>(at, rows, factors);
 			}
 			/* the places of the rows' classes in a tile that lies in LDS, written again with p - q instead of p; a thread has a row's, so what rounding takes of them is added up in order */
 			template<int BM, int BN, int ROWS, typename TileStage>

@@ -331,11 +331,13 @@ namespace mlhip
 					target[i] = Goal::ONE && factor[i] != 0.0f ? goal.targets[m] - first_class : -1; /* a class then */
 					taken[i] = 0.0f;
 				}
-				const auto of_tile = goal.template begin_gradient<BM, BN>(at, rows, factors, lds + stage_lds<BM, BN>());
+				const auto of_tile = goal.template begin_gradient<BM, BN>(at, rows, factors);
 				static_for<PASSES>([&](auto pass)
 				{
 					constexpr int PASS = decltype(pass)::value, FIRST = PASS * BLOCKS / PASSES;
-					__syncthreads();
+					__syncthreads(); /* nobody reads the operands any more, or the rows before */
+					if (PASS == 0)
+						goal.template begin_sums<BM, BN>(lds + stage_lds<BM, BN>());
 #pragma unroll
 					for (int i = FIRST; i < FIRST + BLOCKS / PASSES; i++)
 					{

@@ -81,6 +81,14 @@ def test_loss_and_gradients(ctx, rows, features, classes, count, dtype):
     check(ctx, inputs(rng, rows, features, classes, count, dtype), (1.0, 2.0, 0.7)[(rows + count) % 3], dtype)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("rows,features,classes,count", [(6819, 48, 838, 66), (3001, 160, 2000, 40), (1200, 96, 3000, 20), (700, 256, 5000, 100)])
+def test_many_tiles_at_once(ctx, rows, features, classes, count, dtype):
+    """More tiles than the units take at a time, which keeps the wavefronts of a workgroup apart: what one lays down for a tile's end may not be where another still reads the product's operands, whose chunks are even in number."""
+    rng = np.random.default_rng(rows)
+    check(ctx, inputs(rng, rows, features, classes, count, dtype), 2.0, dtype)
+
+
 def test_logits_of_the_teacher_in_fp32(ctx):
     rng = np.random.default_rng(1)
     for rows, features, classes, count in ((5, 64, 700, 12), (200, 40, 400, 30)):
