@@ -556,14 +556,14 @@ namespace mlhip
 	 * The same where dx comes about in parts or over several pieces of the classes. A wavefront has 256 columns of a row at a time and adds up what the tiles of the row lost by itself; the last 4 columns of a row are moved back to end
 	 * with it, as in RowPlace.
 	 */
-	template<typename T>
+	template<typename T, bool ONE>
 	__global__ __launch_bounds__(256) void kernel_join_input(const float *partial, int parts, int rows, int features, int spans, T *dx, float beta, const float *back, const float *lost, int lost_tiles,
 			GivenBack<T> to, int classes, const T *w, int w_elements)
 	{
 		const int lane = threadIdx.x & 63;
 		const size_t units = static_cast<size_t>(rows) * spans, count = static_cast<size_t>(rows) * features;
 		const float scale = *back;
-		const bool splits = to.splits();
+		const bool splits = !ONE && to.splits();
 		for (size_t unit = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); unit < units; unit += static_cast<size_t>(gridDim.x) * 4)
 		{
 			int span;
@@ -806,7 +806,7 @@ namespace mlhip
 			{
 				const int spans = ceil_div(s.features, 256);
 				const size_t groups = std::min<size_t>((static_cast<size_t>(s.rows) * spans + 3) / 4, 1 << 16);
-				hipLaunchKernelGGL((kernel_join_input<T>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, partial_dx, whole_input.parts, s.rows, s.features, spans, dx, beta_dx, back, lost,
+				hipLaunchKernelGGL((kernel_join_input<T, decltype(goal_of(0))::ONE>), dim3(static_cast<unsigned int>(groups)), dim3(256), 0, stream, partial_dx, whole_input.parts, s.rows, s.features, spans, dx, beta_dx, back, lost,
 						lost_tiles, to, s.classes, w, padded);
 				MLHIP_CHECK(hipGetLastError());
 			}
