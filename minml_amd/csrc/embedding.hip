@@ -6,7 +6,7 @@
  *
  * Forward: memory bounds it (a row of the table read for every row written, from the caches where tokens repeat): 57600 x 256 fp16 from 400 classes 7.8 us (3.8 TB/s, the stores of 29 MB alone take 6).
  * Backward: tokens are sorted first, stably, so that a class's rows stand in a list in the order they have in dy, and one reader adds them up: no two threads meet at a row of the table, every element of dy is read once and
- * every row of the table written once, with zeros where there is no token. The same bits on every run. us: 16384 x 4096 fp16 into 65536 classes 172 (3.9 TB/s: 23 for the order, 141 with 4.6 TB/s for the rows, 12 to join the long
+ * every row of the table written once, with zeros where there is no token. The same bits on every run. us: 16384 x 4096 fp16 into 65536 classes 170 (3.9 TB/s: 22 for the order, 141 with 4.6 TB/s for the rows, 12 to join the long
  * classes), 57600 x 256 fp16 into 400 classes 28, 20011 x 1001 fp32 into 5003 classes 44 to 50: launches of 4 to 9 us, one after another, whose reads wait for each other.
  */
 #include "training_utils.hpp"
@@ -229,7 +229,7 @@ namespace
 			p.count_digits<64>(mine, first, first + here, lane);
 		for (int d = threadIdx.x; d < digits; d += SORT_THREADS)
 		{
-			constexpr int AHEAD = 32;
+			constexpr int AHEAD = 16; /* with 32 embedding gradients of 16384 x 4096 take 172.8 us, not 170.5, with 8 57600 x 256 29.0, not 28.4 */
 			int sum_before = 0, sum_behind = 0;
 			for (int g = 0; g < groups; g += AHEAD)
 			{
