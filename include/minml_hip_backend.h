@@ -277,7 +277,7 @@ extern "C"
 	/*
 	 * What a model over a vocabulary begins with: y[i] = scale * table[tokens[i]], tokens int32 [..], table [classes, features], y [.., features] of the table's type; a token that is none of 0 .. classes - 1 gives zeros.
 	 * Backward: dtable = beta_weights * dtable + scale * (the sum of the rows of dy [.., features] whose token is the class), of dy's type or fp32; rows of dy without a class count for nothing, whatever they hold.
-	 * Everything is aligned to one element. The scale has to be finite. The workspace holds the tokens in order, 16 bytes for each at most, and sums of every 32 or 64 rows in fp32.
+	 * Everything is aligned to one element. The scale has to be finite. The workspace holds the tokens in order, 16 bytes for each at most, sums of every 32 or 64 rows in fp32 and 8 bytes for every class.
 	 */
 	void hip_embedding_forward(mlContext_t context, const mlTensor_t tokens, const mlTensor_t table, float scale, mlTensor_t y);
 	size_t hip_embedding_get_workspace_size(mlShape_t tokens_shape, mlShape_t table_shape, mlDataType_t dtype); /* bytes, for the backward pass; dtype: dy's, or fp32 for either */

@@ -315,6 +315,7 @@ namespace
 			const int *keys, *positions; /* in order */
 			const T *dy;
 			float *partial; /* [chunks][columns] */
+			int *ranges; /* [classes][2], of those with chunks of their own: first place and the one behind the last */
 			Out *out;
 			int count, classes, columns, classes_of_group, lanes, spans, chunk, chunks; /* chunks: workgroups for them, or 0; lanes: threads of a row, a power of two; spans: that a row takes of them */
 			float scale, beta;
@@ -461,11 +462,10 @@ namespace
 	__global__ __launch_bounds__(256) void kernel_join_chunks(TableGradient<T, Out> p)
 	{
 		__shared__ float meeting[256][VEC];
-		const int chunk = blockIdx.x / p.spans, span = blockIdx.x % p.spans, first = chunk * p.chunk, lane = threadIdx.x & 63, key = p.keys[first];
+		const int chunk = blockIdx.x / p.spans, span = blockIdx.x % p.spans, first = chunk * p.chunk, key = p.keys[first];
 		if (!begins_with_many(p, first, key) || (chunk > 0 && p.keys[first - p.chunk] == key))
 			return;
-		const bool mine = lane < p.chunk && first - 1 - lane >= 0 && p.keys[max(first - 1 - lane, 0)] == key;
-		const int begin = first - __popcll(__ballot(mine)), end = first + lower_bound_by_wave(p.keys + first, p.count - first, key + 1);
+		const int begin = p.ranges[2 * key], end = p.ranges[2 * key + 1];
 		const Column<T, Out, VEC> column(p, span);
 		Elements<Out, VEC> old;
 		if (p.beta != 0.0f && column.group == 0)
@@ -536,6 +536,11 @@ namespace
 		for (int c = threadIdx.x; c < classes; c += 256)
 			if (!of_group(c) && rows_of(c) < p.chunk)
 				large[atomicAdd(&large_ones, 1)] = c; /* in any order: each has a row of its own */
+			else if (rows_of(c) >= p.chunk && span == 0)
+			{
+				p.ranges[2 * (first_class + c)] = bounds[c];
+				p.ranges[2 * (first_class + c) + 1] = bounds[c + 1];
+			}
 		float v[VEC];
 		Elements<Out, VEC> old;
 		if (column.inside)
@@ -669,7 +674,7 @@ namespace
 	}
 	struct EmbeddingSpace
 	{
-			size_t keys[2], positions[2], counts, partial, total;
+			size_t keys[2], positions[2], counts, partial, ranges, total;
 	};
 	EmbeddingSpace embedding_space(const EmbeddingShape &s, mlDataType_t dtype)
 	{
@@ -693,6 +698,7 @@ namespace
 			space.counts = take(small ? 0 : (sizeof(int) * plan.groups << plan.digit_bits));
 			const int chunk = chunk_of(s, vector_of(s, dtype));
 			space.partial = take(s.rows >= chunk ? sizeof(float) * ceil_div(s.rows, chunk) * s.columns : 0);
+			space.ranges = take(s.rows >= chunk ? 2 * sizeof(int) * s.classes : 0);
 		}
 		space.total = at;
 		return space;
@@ -749,7 +755,7 @@ namespace
 		return { keys(last), positions(last) };
 	}
 	template<typename T, typename Out, int VEC>
-	void table_gradient(hipStream_t stream, const EmbeddingShape &s, const int *keys, const int *positions, const T *dy, float *partial, float scale, float beta, Out *out)
+	void table_gradient(hipStream_t stream, const EmbeddingShape &s, const int *keys, const int *positions, const T *dy, float *partial, int *ranges, float scale, float beta, Out *out)
 	{
 		const int lanes = lanes_of_row(s, VEC);
 		const int spans = ceil_div(s.columns, lanes * VEC);
@@ -757,7 +763,7 @@ namespace
 		/* classes of a workgroup: their search is its beginning, but four workgroups to a compute unit come first. us with 16 / 32 / 64 at most for wide rows: 16384 x 4096 of 65536 174 / 172 / 176 */
 		const int most = static_cast<int>(std::min<size_t>(std::max(32, 1024 / lanes), std::max<size_t>(1, units / 1024)));
 		const int chunk = chunk_of(s, VEC), chunks = s.rows >= chunk ? ceil_div(s.rows, chunk) : 0;
-		const TableGradient<T, Out> p { keys, positions, dy, partial, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk, chunks, scale, beta };
+		const TableGradient<T, Out> p { keys, positions, dy, partial, ranges, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk, chunks, scale, beta };
 		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3((static_cast<unsigned int>(ceil_div(s.classes, most)) + chunks) * spans), dim3(256), 0, stream, p);
 		if (chunks > 0)
 		{
@@ -775,12 +781,13 @@ namespace
 		constexpr int VEC = 16 / sizeof(T);
 		const int *keys = nullptr, *positions = nullptr;
 		float *partial = reinterpret_cast<float*>(workspace + space.partial);
+		int *ranges = reinterpret_cast<int*>(workspace + space.ranges);
 		if (s.rows > 0)
 			std::tie(keys, positions) = sort_tokens(stream, s, space, tokens, workspace);
 		if (s.columns >= VEC)
-			table_gradient<T, Out, VEC>(stream, s, keys, positions, dy, partial, scale, beta, out);
+			table_gradient<T, Out, VEC>(stream, s, keys, positions, dy, partial, ranges, scale, beta, out);
 		else
-			table_gradient<T, Out, 1>(stream, s, keys, positions, dy, partial, scale, beta, out);
+			table_gradient<T, Out, 1>(stream, s, keys, positions, dy, partial, ranges, scale, beta, out);
 	}
 	void check_tokens(const mlTensor_t &tokens, const EmbeddingShape &s, const char *name)
 	{
