@@ -750,7 +750,7 @@ namespace
 		}
 	}
 	template<typename T, typename Out, int VEC, int ROWS>
-	__global__ __launch_bounds__(256) void kernel_few_weights(const T *x, const float *d, int rows, int columns, int classes, int classes_of_group, int lanes, Out *out, float beta)
+	__global__ __launch_bounds__(256) void kernel_few_weights(const T *x, const float *d, int rows, int columns, int classes, int classes_of_group, int lanes, Out *out, float beta, bool past)
 	{
 		const FewColumns<VEC> column(columns, lanes);
 		Elements<T, VEC> of_row[ROWS];
@@ -781,7 +781,10 @@ namespace
 #pragma unroll
 				for (int e = 0; e < VEC; e++)
 					v[e] = fmaf(beta, old[e], v[e]);
-			store_nearest<VEC>(dst, v, column.place.skip);
+			if (past)
+				store_past_caches<VEC>(dst, v, column.place.skip);
+			else
+				store_nearest<VEC>(dst, v, column.place.skip);
 		}
 	}
 
@@ -989,10 +992,12 @@ namespace
 			}
 			const dim3 grid(ceil_div(s.classes, plan.classes_of_group), plan.spans);
 			if (dw.data != nullptr && dw.dtype == DTYPE_FLOAT32)
-				hipLaunchKernelGGL((kernel_few_weights<T, float, VEC, ROWS>), grid, dim3(256), 0, stream, x, d, s.rows, s.features, s.classes, plan.classes_of_group, plan.lanes, ptr<float>(dw), beta_weights);
+				hipLaunchKernelGGL((kernel_few_weights<T, float, VEC, ROWS>), grid, dim3(256), 0, stream, x, d, s.rows, s.features, s.classes, plan.classes_of_group, plan.lanes, ptr<float>(dw), beta_weights,
+						past_caches(s.classes, s.features * sizeof(float)));
 			else if constexpr (sizeof(T) == 2)
 				if (dw.data != nullptr)
-					hipLaunchKernelGGL((kernel_few_weights<T, T, VEC, ROWS>), grid, dim3(256), 0, stream, x, d, s.rows, s.features, s.classes, plan.classes_of_group, plan.lanes, ptr<T>(dw), beta_weights);
+					hipLaunchKernelGGL((kernel_few_weights<T, T, VEC, ROWS>), grid, dim3(256), 0, stream, x, d, s.rows, s.features, s.classes, plan.classes_of_group, plan.lanes, ptr<T>(dw), beta_weights,
+							past_caches(s.classes, s.features * sizeof(T)));
 			MLHIP_CHECK(hipGetLastError());
 		};
 		with_stride<T>(plan.stride, [&](auto stride)

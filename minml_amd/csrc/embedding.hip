@@ -6,7 +6,7 @@
  *
  * Forward: memory bounds it (a row of the table read for every row written, from the caches where tokens repeat): 57600 x 256 fp16 from 400 classes 7.8 us (3.8 TB/s, the stores of 29 MB alone take 6).
  * Backward: tokens are sorted first, stably, so that a class's rows stand in a list in the order they have in dy, and one reader adds them up: no two threads meet at a row of the table, every element of dy is read once and
- * every row of the table written once, with zeros where there is no token. The same bits on every run. us: 16384 x 4096 fp16 into 65536 classes 170 (3.9 TB/s: 22 for the order, 141 with 4.6 TB/s for the rows, 12 to join the long
+ * every row of the table written once, with zeros where there is no token. The same bits on every run. us: 16384 x 4096 fp16 into 65536 classes 168 (4.0 TB/s: 22 for the order, 139 with 4.7 TB/s for the rows, 11 to join the long
  * classes), 57600 x 256 fp16 into 400 classes 28, 20011 x 1001 fp32 into 5003 classes 44 to 50: launches of 4 to 9 us, one after another, whose reads wait for each other.
  */
 #include "training_utils.hpp"
@@ -319,6 +319,7 @@ namespace
 			Out *out;
 			int count, classes, columns, classes_of_group, lanes, spans, chunk, chunks; /* chunks: workgroups for them, or 0; lanes: threads of a row, a power of two; spans: that a row takes of them */
 			float scale, beta;
+			bool past; /* the caches */
 	};
 	/* the first place of [first, first + length) whose key is not below `key` */
 	__device__ __forceinline__ int lower_bound(const int *keys, int first, int length, int key)
@@ -427,7 +428,10 @@ namespace
 #pragma unroll
 				for (int e = 0; e < VEC; e++)
 					v[e] = p.beta != 0.0f ? fmaf(p.beta, old[e], p.scale * v[e]) : p.scale * v[e];
-				store_nearest<VEC>(of_table(p, c), v, place.skip);
+				if (p.past)
+					store_past_caches<VEC>(of_table(p, c), v, place.skip);
+				else
+					store_nearest<VEC>(of_table(p, c), v, place.skip);
 			}
 	};
 	constexpr int AHEAD = 8;
@@ -763,7 +767,8 @@ namespace
 		/* classes of a workgroup: their search is its beginning, but four workgroups to a compute unit come first. us with 16 / 32 / 64 at most for wide rows: 16384 x 4096 of 65536 174 / 172 / 176 */
 		const int most = static_cast<int>(std::min<size_t>(std::max(32, 1024 / lanes), std::max<size_t>(1, units / 1024)));
 		const int chunk = chunk_of(s, VEC), chunks = s.rows >= chunk ? ceil_div(s.rows, chunk) : 0;
-		const TableGradient<T, Out> p { keys, positions, dy, partial, ranges, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk, chunks, scale, beta };
+		const TableGradient<T, Out> p { keys, positions, dy, partial, ranges, out, s.rows, s.classes, s.columns, most, lanes, spans, chunk, chunks, scale, beta,
+				past_caches(s.classes, s.columns * sizeof(Out)) };
 		hipLaunchKernelGGL((kernel_table_gradient<T, Out, VEC>), dim3((static_cast<unsigned int>(ceil_div(s.classes, most)) + chunks) * spans), dim3(256), 0, stream, p);
 		if (chunks > 0)
 		{

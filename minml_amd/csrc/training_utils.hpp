@@ -129,6 +129,31 @@ namespace mlhip
 		}
 	}
 	/*
+	 * The same past the caches, for rows of whole lines of a result that is larger than the L2s: nobody finds it there later, and what somebody would find is not pushed out. us with the inputs in the memory's own cache as
+	 * far as they fit there, so / through the caches (with inputs from memory, the same either way): embedding gradients of
+	 * 16384 x 4096 of 65536 classes 138 / 170, 8192 x 2048 of 65536 fp32 131 / 152, 4096 x 1024 of 131072 68.5 / 73.4, 30000 x 256 of 100000 48 / 49.7, 5 x 1072 of 66507 fp32 (nearly all zeros) 72 / 69.5; distillations of
+	 * 8 rows, 2048 x 65536 218 / 259, 1024 x 32000 79.3 / 80.5; rows that end inside a line (1 row, 1023 x 32000) 110 / 104.
+	 */
+	inline bool past_caches(size_t rows, size_t row_bytes)
+	{
+		return row_bytes % 64 == 0 && rows * row_bytes > (size_t(32) << 20);
+	}
+	template<int VEC, typename T>
+	__device__ __forceinline__ void store_past_caches(T *p, const float (&v)[VEC], int skip)
+	{
+		if constexpr (VEC > 1)
+			if (skip == 0)
+			{
+				typename Elements<T, VEC>::vec_t tmp;
+#pragma unroll
+				for (int e = 0; e < VEC; e++)
+					tmp[e] = static_cast<T>(v[e]);
+				__builtin_nontemporal_store(tmp, reinterpret_cast<typename Elements<T, VEC>::unaligned_t*>(p));
+				return;
+			}
+		store_nearest<VEC>(p, v, skip);
+	}
+	/*
 	 * Where the vector that begins at column j of a row of `columns` (>= VEC) elements lies. The vector that would pass the row's end is moved back to end with it; its first `skip`
 	 * elements belong to the vector before it and count for nothing here. So every load is a whole vector inside its row, for any length, and none stands under a test.
 	 */
