@@ -282,10 +282,25 @@ namespace
 				for (int u = 0; u < AHEAD; u++)
 					if (t.first + u < t.last)
 						f(static_cast<size_t>(t.m) * count + t.first + u, t.named[u], t.share[u], t.probability[u]);
-				for (int k = t.first + AHEAD; k < t.last; k++)
+				/* many in a tile: so many on their way at a time. us, one / 4 / 8: gradients of 532 x 421 of 421 classes, 105 a row 184 / 147 / 141, 2048 x 512 of 1000, 64 a row 126 / 112 / 111 */
+				constexpr int MORE = 8;
+				for (int k = t.first + AHEAD; k < t.last; k += MORE)
 				{
-					const size_t place = static_cast<size_t>(t.m) * count + k;
-					f(place, classes[place], BACKWARD ? shares[place] : 0.0f, BACKWARD ? known[place] : 0.0f);
+					int named[MORE];
+					float share[MORE], probability[MORE];
+#pragma unroll
+					for (int u = 0; u < MORE; u++)
+					{
+						const size_t place = static_cast<size_t>(t.m) * count + min(k + u, t.last - 1);
+						named[u] = classes[place];
+						share[u] = BACKWARD ? shares[place] : 0.0f;
+						probability[u] = BACKWARD ? known[place] : 0.0f;
+					}
+					__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+					for (int u = 0; u < MORE; u++)
+						if (k + u < t.last)
+							f(static_cast<size_t>(t.m) * count + k + u, named[u], share[u], probability[u]);
 				}
 			}
 			template<int BLOCKS>
