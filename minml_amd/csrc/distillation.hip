@@ -11,8 +11,8 @@
  * begins among them; then one thread of a tile has a row's few in that tile, and they meet the logits in LDS, through which the tile goes anyway in the backward pass, and in the forward pass where it has any.
  * In the backward pass the student's probability at these places is known from the forward pass's log p, so that d there is p - q in fp32, rounded once, however close p and q are. In fp16, what rounding takes from d's rows is given back to the row of W with the teacher's largest share, as much as is its own, and
  * the rest to the mean of rows that teachers name: dx is 2.3e-4 to 2.8e-4 off (norm), of which its own rounding is 2.1e-4; 2 to 4 us more than all of it to one class (3964 / 3974 of 4096 x 2048 x 65536, 78.5 / 82.5 of 40 x 512 x 20000).
- * fp16, what it takes beside the cross entropy of the same size: 2048 rows of 1024 x 50001, 32 classes a row, 245 to 267 us, card to card (the products 257 / 246, sorting 9); 4096 of 2048 x 65536, 64 classes, loss and gradients
- * 3.96 to 4.05 ms (products 1030 / 1003, making d 562 / 560 twice, sorting 13 twice). 3 rows of 1024 x 32000 18.5 us (14.2 at 4.6 TB/s, 5.2 to join). What bounds the rest is said there.
+ * fp16, what it takes beside the cross entropy of the same size: 2048 rows of 1024 x 50001, 32 classes a row, 245 to 267 us, card to card (the products 257 / 246, sorting 8); 4096 of 2048 x 65536, 64 classes, loss and gradients
+ * 3.96 to 4.05 ms (products 1030 / 1003, making d 562 / 560 twice, sorting 12 twice). 3 rows of 1024 x 32000 18.5 us (14.2 at 4.6 TB/s, 5.2 to join). What bounds the rest is said there.
  */
 #include "vocabulary_loss.hpp"
 
@@ -38,6 +38,11 @@ namespace
 			float *own, *there; /* backward in fp16, [rows] and one: zeros, and whether there is a common row */
 			half_t *common; /* [features in whole tiles]: what rows of the weights have in common */
 	};
+	/* whole vectors of four */
+	__host__ __device__ inline int places_in_lds(int count)
+	{
+		return (count + 3) / 4 * 4;
+	}
 	template<typename V>
 	__device__ __forceinline__ V lanes_max(V v)
 	{
@@ -94,32 +99,37 @@ namespace
 	template<typename L>
 	__global__ __launch_bounds__(256) void kernel_sort_teacher(const int *classes_in, const L *logits, const float *log_probabilities, int rows, int count, int classes, float temperature, int width, int tiles, const half_t *w, int features, Teaching out)
 	{
-		extern __shared__ int memory[];
+		extern __shared__ __attribute__((aligned(16))) int memory[];
 		const int groups = (rows + 3) / 4;
 		if (static_cast<int>(blockIdx.x) >= groups)
 			return common_row(classes_in, logits, static_cast<size_t>(rows) * count, classes, w, features, (static_cast<int>(blockIdx.x) - groups) * 64, out.common, out.there);
 		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave;
 		if (row >= rows)
 			return;
-		int *named = memory + wave * 4 * count, *sorted = named + count;
-		float *values = reinterpret_cast<float*>(sorted + count), *shares = values + count;
+		const int stride = places_in_lds(count);
+		int *named = memory + wave * 4 * stride, *sorted = named + stride;
+		float *values = reinterpret_cast<float*>(sorted + stride), *shares = values + stride;
 		const size_t base = static_cast<size_t>(row) * count;
 		float top = -std::numeric_limits<float>::infinity();
-		int there = 0;
-		for (int k = lane; k < count; k += 64)
+		int there = 0, missing = 0;
+		for (int k0 = 0; k0 < stride; k0 += 64)
 		{
-			const int c = classes_in[base + k];
-			const float v = static_cast<float>(logits[base + k]) / temperature;
+			const int k = k0 + lane;
+			const int c = k < count ? classes_in[base + k] : -1;
+			const float v = k < count ? static_cast<float>(logits[base + k]) / temperature : 0.0f;
 			const bool counts = c >= 0 && c < classes && !(v == -std::numeric_limits<float>::infinity());
-			named[k] = counts ? c : 0x7fffffff;
-			values[k] = v;
+			const uint64_t all = __ballot(counts), none = __ballot(k < count && !counts);
+			if (k < stride)
+			{
+				named[k] = counts ? c : 0x7fffffff;
+				/* of one that does not count: how many others before do not either */
+				values[k] = counts ? v : __int_as_float(missing + __popcll(none & ((1ull << lane) - 1)));
+			}
 			top = counts ? fmaxf(top, v) : top;
-			there += counts ? 1 : 0;
+			there += __popcll(all);
+			missing += __popcll(none);
 		}
 		top = lanes_max(top);
-#pragma unroll
-		for (int offset = 32; offset >= 1; offset >>= 1)
-			there += __shfl_xor(there, offset);
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 		float sum = 0.0f;
 		for (int k = lane; k < count; k += 64)
@@ -134,15 +144,17 @@ namespace
 		{
 			const int c = named[k];
 			int place = 0;
-#pragma unroll 8
-			for (int other = 0; other < count; other++)
-				place += named[other] < c + (other < k && c != 0x7fffffff ? 1 : 0) ? 1 : 0;
-			if (c == 0x7fffffff)
+#pragma unroll 4
+			for (int other = 0; other < stride; other += 4)
 			{
-				place = there;
-				for (int other = 0; other < k; other++)
-					place += named[other] == c ? 1 : 0;
+				typedef int int4_t __attribute__((ext_vector_type(4)));
+				const int4_t n = *reinterpret_cast<const int4_t*>(named + other);
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					place += static_cast<uint32_t>(n[e]) < static_cast<uint32_t>(c) + (other + e < k ? 1 : 0) ? 1 : 0;
 			}
+			if (c == 0x7fffffff)
+				place = there + __float_as_int(values[k]);
 			sorted[place] = c;
 			shares[place] = c == 0x7fffffff ? 0.0f : values[k] / sum;
 			out.places[base + place] = static_cast<uint16_t>(k);
@@ -902,7 +914,7 @@ namespace
 	void sort_teacher(hipStream_t stream, const LossShape &s, const mlTensor_t &classes, const mlTensor_t &logits, const float *log_probabilities, int count, float temperature, int width, const half_t *w,
 			const Teaching &out)
 	{
-		const int tiles = ceil_div(s.classes, width), bytes = 4 * 4 * static_cast<int>(sizeof(int)) * count;
+		const int tiles = ceil_div(s.classes, width), bytes = 4 * 4 * static_cast<int>(sizeof(int)) * places_in_lds(count);
 		const int groups = ceil_div(s.rows, 4) + (w != nullptr ? static_cast<int>(round_up(s.features, COMMON_COLUMNS)) / 64 : 0);
 		const auto launch = [&](auto kernel, auto values)
 		{
