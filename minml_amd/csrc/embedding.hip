@@ -369,19 +369,28 @@ namespace
 					v[e] += i + u * step < last ? x[u][e] : 0.0f;
 		}
 	}
-	/* the sums of a workgroup's 256 / lanes groups of threads in the first of them, in order. Every thread calls it */
+	/*
+	 * The sums of a workgroup's 256 / lanes groups of threads in the first of them, always in the same order: those of a wavefront by exchange, the wavefronts' in LDS. Every thread calls it. (All of them in LDS, by the first
+	 * group's threads one after another: us, embedding gradients so / that way, 31058 x 16 of 119601 classes 36 / 57, 57600 x 64 of 400 25 / 28, 65536 x 64 of 131072 49 / 54.)
+	 */
 	template<int VEC>
 	__device__ __forceinline__ void join_groups(float (&v)[VEC], int lanes, float (*meeting)[VEC])
 	{
 		if (lanes == 256)
 			return;
-		__syncthreads();
+		for (int offset = 32; offset >= lanes; offset >>= 1)
 #pragma unroll
-		for (int e = 0; e < VEC; e++)
-			meeting[threadIdx.x][e] = v[e];
+			for (int e = 0; e < VEC; e++)
+				v[e] += __shfl_xor(v[e], offset);
 		__syncthreads();
+		if (static_cast<int>(threadIdx.x & 63) < lanes)
+#pragma unroll
+			for (int e = 0; e < VEC; e++)
+				meeting[threadIdx.x][e] = v[e];
+		__syncthreads();
+		const int step = max(lanes, 64);
 		if (static_cast<int>(threadIdx.x) < lanes)
-			for (int t = threadIdx.x + lanes; t < 256; t += lanes)
+			for (int t = threadIdx.x + step; t < 256; t += step)
 #pragma unroll
 				for (int e = 0; e < VEC; e++)
 					v[e] += meeting[t][e];
