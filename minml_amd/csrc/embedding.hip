@@ -499,7 +499,7 @@ namespace
 	}
 	constexpr int MOST_CLASSES_OF_GROUP = 1024;
 	/*
-	 * A class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's. us with 8 / 16 / 32: 57600 x 256 of 400 classes 28.0 / 28.1 / 30.2, 65536 x 64 of 131072 59 / 54 / 50
+	 * A class of fewer rows is one group's of threads, which may be a small part of the workgroup; of more, the whole workgroup's. us with 8 / 16 / 32: 57600 x 256 of 400 classes 26.3 / 26.3 / 28.6, 65536 x 64 of 131072 50.7 / 49.1 / 46.9, 31058 x 16 of 119601 38.8 / 36.2 / 36.6
 	 */
 	constexpr int ROWS_OF_ALL = 16;
 	template<typename T, typename Out, int VEC>
