@@ -7,7 +7,7 @@
  * Forward: memory bounds it (a row of the table read for every row written, from the caches where tokens repeat): 57600 x 256 fp16 from 400 classes 7.8 us (3.8 TB/s, the stores of 29 MB alone take 6).
  * Backward: tokens are sorted first, stably, so that a class's rows stand in a list in the order they have in dy, and one reader adds them up: no two threads meet at a row of the table, every element of dy is read once and
  * every row of the table written once, with zeros where there is no token. The same bits on every run. us: 16384 x 4096 fp16 into 65536 classes 168 (4.0 TB/s: 22 for the order, 139 with 4.7 TB/s for the rows, 11 to join the long
- * classes), 57600 x 256 fp16 into 400 classes 28, 20011 x 1001 fp32 into 5003 classes 44 to 50: launches of 4 to 9 us, one after another, whose reads wait for each other.
+ * classes), 57600 x 256 fp16 into 400 classes 25, 20011 x 1001 fp32 into 5003 classes 43 to 49: launches of 4 to 9 us, one after another, whose reads wait for each other.
  */
 #include "training_utils.hpp"
 
@@ -670,10 +670,13 @@ namespace
 		plan.groups = ceil_div(s.rows, plan.per_group);
 		return plan;
 	}
-	/* by counting 1024, 4096 and 8192 tokens take 5.6, 10.6 and 15.4 us; by digits 8.2 us for each pass, for up to 65536 tokens about as long */
+	/*
+	 * Counting takes longer the more tokens there are, a digit about as long for all up to 65536, longer ones longer. us of gradients of rows of 64, counted / by digits: 400 classes, 3000, 4096 and 6000 tokens 19.7 / 20.3,
+	 * 20.9 / 20.0, 24.3 / 20.4; 1500 classes, 4096, 6000 and 8192 22.9 / 25.6, 26.2 / 26.4, 29.6 / 26.9; 8000 classes, 6000, 8192 and 12000 26.0 / 28.3, 29.2 / 29.4, 34.8 / 30.0; 100000 classes 30.5 / 33.4, 32.2 / 34.0, 38.0 / 34.2
+	 */
 	bool sorted_by_counting(const EmbeddingShape &s)
 	{
-		return s.rows <= (s.classes < 2048 ? 2048 : 8192);
+		return s.rows <= (s.classes < 512 ? 3500 : s.classes < 2048 ? 6000 : 8192);
 	}
 	/* threads that a row takes, a power of two */
 	int lanes_of_row(const EmbeddingShape &s, int vector)

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 # one token to more than one workgroup sorts at once and more than one of its digits; tables of one row, of one digit of the sort and of two; rows below, at and beyond a vector
 SIZES = [(1, 1, 1), (1, 7, 3), (3, 2, 8), (5, 300, 7), (63, 2, 5), (64, 1, 9), (65, 300, 16), (129, 40, 4096), (1000, 17, 40), (2047, 2048, 13), (4096, 50, 24), (4097, 3000, 33), (9000, 2, 260),
-         (20000, 70000, 8), (70001, 1023, 12), (3001, 5, 2056), (70, 3, 9000), (300000, 5, 4)]
+         (20000, 70000, 8), (70001, 1023, 12), (3001, 5, 2056), (70, 3, 9000), (300000, 5, 4), (4000, 1, 24), (3501, 400, 16), (6001, 1500, 24), (8193, 2049, 9), (12000, 130000, 16)]
 
 
 def tokens_of(rng, rows, classes, ignored=0.1):
