@@ -289,7 +289,7 @@ extern "C"
 	 * over the row's classes: loss = sum of q (log q - log p), fp32 [..], with lse fp32 [..] and log_probabilities (log p) fp32 [.., count] as the backward pass needs them. A place whose class is none of 0 .. classes - 1 or
 	 * whose logit is -inf does not count, whatever else it holds (log p is 0 there); a class that stands there twice has the sum of both probabilities; a row where nothing counts has loss 0 and no gradient (its lse is given
 	 * all the same; its x has to be finite). Loss and gradients are of the softened distributions: callers that want them multiplied by temperature^2 do so in dloss.
-	 * Backward: dloss fp32 [..] -> dx, dw, db as above, with the gradients of the logits kept as the cross entropy's are. The workspace holds what the cross entropy's does, 16 bytes for every place, and 2 for every row of
+	 * Backward: dloss fp32 [..] -> dx, dw, db as above, with the gradients of the logits kept as the cross entropy's are (of up to 64 rows mostly with what rounding leaves of them). The workspace holds what the cross entropy's does, 16 bytes for every place, and 2 for every row of
 	 * every tile; of a few rows their logits, and gradients of them in fp32 with up to 512 sums of dx, instead.
 	 */
 	size_t hip_linear_distillation_get_workspace_size(mlShape_t input_shape, mlShape_t weights_shape, int count, mlDataType_t dtype, bool backward); /* bytes; the backward pass's is enough for both */

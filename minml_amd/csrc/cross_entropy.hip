@@ -166,7 +166,7 @@ namespace
 	template<typename T>
 	void loss_forward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const int *targets, float *loss, float *lse, uint8_t *workspace)
 	{
-		const LossSpace space = loss_space(s, false, few_rows(s));
+		const LossSpace space = loss_space(s, false, few_rows(s), false);
 		Partial *partials = reinterpret_cast<Partial*>(workspace + space.partials);
 		float *target_logits = reinterpret_cast<float*>(workspace + space.target_logits);
 		int columns;
@@ -220,7 +220,7 @@ extern "C"
 	try
 	{
 		const LossShape s = loss_shape(input_shape, weights_shape, dtype, "linear_cross_entropy_get_workspace_size");
-		return loss_space(s, backward, few_rows(s)).total;
+		return loss_space(s, backward, few_rows(s), false).total;
 	}
 	catch (...)
 	{
@@ -236,7 +236,7 @@ extern "C"
 		MLHIP_REQUIRE(per_row(loss, s, DTYPE_FLOAT32) && per_row(lse, s, DTYPE_FLOAT32), "linear_cross_entropy_forward: loss and lse must be fp32 with one element per row");
 		if (s.rows == 0)
 			return;
-		check_space(workspace, workspace_size, loss_space(s, false, few_rows(s)).total, name);
+		check_space(workspace, workspace_size, loss_space(s, false, few_rows(s), false).total, name);
 		require_apart( { loss, lse, Extent(workspace, workspace_size) }, { x, w, b, targets }, name);
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
@@ -269,14 +269,14 @@ extern "C"
 		{
 			return OneClass { ptr<int>(targets), nullptr };
 		};
-		check_space(workspace, workspace_size, loss_space(s, true, few_rows(s)).total, name);
+		check_space(workspace, workspace_size, loss_space(s, true, few_rows(s), false).total, name);
 		require_apart( { dx, dw, db, Extent(workspace, workspace_size) }, { x, w, b, targets, lse, dloss }, name);
 		const OnDeviceOf on(context);
 		if (x.dtype == DTYPE_FLOAT16)
-			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), GivenBack<half_t> { ptr<int>(targets), nullptr, nullptr, nullptr }, goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, few_rows(s),
+			loss_backward(on.stream, s, ptr<half_t>(x), ptr<half_t>(w), ptr<half_t>(b), GivenBack<half_t> { ptr<int>(targets), nullptr, nullptr, nullptr }, goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<half_t>(dx), beta_weights, dw, db, few_rows(s), false,
 					reinterpret_cast<uint8_t*>(workspace));
 		else
-			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), GivenBack<float> { ptr<int>(targets), nullptr, nullptr, nullptr }, goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db, few_rows(s),
+			loss_backward(on.stream, s, ptr<float>(x), ptr<float>(w), ptr<float>(b), GivenBack<float> { ptr<int>(targets), nullptr, nullptr, nullptr }, goal, 1.0f, ptr<float>(lse), ptr<float>(dloss), beta_dx, ptr<float>(dx), beta_weights, dw, db, few_rows(s), false,
 					reinterpret_cast<uint8_t*>(workspace));
 	}
 	catch (...)

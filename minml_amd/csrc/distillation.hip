@@ -10,7 +10,8 @@
  * The passes are the cross entropy's (vocabulary_loss.hpp). What is new is that a row has many classes of its own, spread over the tiles of logits. A launch before sorts every row's classes and notes where each column of tiles
  * begins among them; then one thread of a tile has a row's few in that tile, and they meet the logits in LDS, through which the tile goes anyway in the backward pass, and in the forward pass where it has any.
  * In the backward pass the student's probability at these places is known from the forward pass's log p, so that d there is p - q in fp32, rounded once, however close p and q are. In fp16, what rounding takes from d's rows is given back to the row of W with the teacher's largest share, as much as is its own, and
- * the rest to the mean of rows that teachers name: dx is 2.3e-4 to 2.8e-4 off (norm), of which its own rounding is 2.1e-4; 2 to 4 us more than all of it to one class (3964 / 3974 of 4096 x 2048 x 65536, 78.5 / 82.5 of 40 x 512 x 20000).
+ * the rest to the mean of rows that teachers name: dx is 2.3e-4 to 2.8e-4 off (norm), of which its own rounding is 2.1e-4; 2 to 4 us more than all of it to one class (3964 / 3974 of 4096 x 2048 x 65536, 135.7 / 139.5 of 400 x 1024 x 10000).
+ * Up to 64 rows d's low parts are kept (see LOW_ROWS).
  * fp16, what it takes beside the cross entropy of the same size: 2048 rows of 1024 x 50001, 32 classes a row, 245 to 267 us, card to card (the products 257 / 246, sorting 8); 4096 of 2048 x 65536, 64 classes, loss and gradients
  * 3.96 to 4.05 ms (products 1030 / 1003, making d 562 / 560 twice, sorting 12 twice). 3 rows of 1024 x 32000 18.5 us (14.2 at 4.6 TB/s, 5.2 to join). What bounds the rest is said there.
  */
@@ -235,6 +236,7 @@ namespace
 			float slope; /* 1 / t */
 			const int *anchors; /* backward: of every row the class whose part of what rounding took is kept for itself, in own; own null: of none */
 			float *own;
+			bool low; /* backward, of up to LOW_ROWS rows: d's low parts behind them */
 
 			/*
 			 * A thread's row of the tile and its classes there: first .. last - 1 of the row's, the first two of them with what is known of them. Asked for when the tile is complete, before anything is computed of it: the
@@ -433,6 +435,8 @@ namespace
 						const T rounded = static_cast<T>(d);
 						taken += (d - static_cast<float>(rounded)) - (pf - static_cast<float>(*stored));
 						*stored = rounded;
+						if (sizeof(T) == 2 && BM == 2 * LOW_ROWS && low)
+							stored[LOW_ROWS * TileStage::STRIDE] = low_part(d, rounded);
 						if (n == of_tile.anchor)
 							own[of_tile.m] = d - static_cast<float>(rounded);
 						if (fabsf(qf) < std::numeric_limits<float>::infinity())
@@ -864,7 +868,7 @@ namespace
 		DistillationSpace space { };
 		const bool few = backward && few_gradients(s);
 		if (!few)
-			space.loss = loss_space(s, backward, few_logits(s));
+			space.loss = loss_space(s, backward, few_logits(s), backward && may_keep_low(s));
 		size_t at = space.loss.total;
 		const auto take = [&](size_t bytes)
 		{
@@ -890,7 +894,7 @@ namespace
 			}
 			space.anchors = take(sizeof(int) * rows);
 			space.entropies = take(sizeof(float) * rows);
-			if (backward && !few && s.element_size == 2)
+			if (backward && !few && s.element_size == 2 && !may_keep_low(s))
 			{
 				space.own = take(sizeof(float) * rows);
 				space.there = take(sizeof(float));
@@ -959,7 +963,7 @@ namespace
 		const Teaching teaching = teaching_of(workspace, space);
 		const int width = tile_width(s, s.classes), columns = ceil_div(s.classes, width), padded = padded_columns<T>(s.features);
 		sort_teacher(stream, s, classes, logits, nullptr, count, temperature, width, nullptr, teaching);
-		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, kept, count, columns + 1, 1.0f / temperature, nullptr, nullptr };
+		const TopClasses goal { nullptr, teaching.classes, teaching.shares, nullptr, teaching.begins, kept, count, columns + 1, 1.0f / temperature, nullptr, nullptr, false };
 		x = pad_rows(stream, x, at<T>(workspace, space.loss.x), s.rows, s.features);
 		w = pad_rows(stream, w, at<T>(workspace, space.loss.w), s.classes, s.features);
 		const ProductPlan plan = logits_plan(s, s.classes);
@@ -1041,12 +1045,12 @@ namespace
 	{
 		const DistillationSpace space = distillation_space(s, count, true);
 		const Teaching teaching = teaching_of(workspace, space);
-		const bool few = few_gradients(s);
+		const bool few = few_gradients(s), low = !few && may_keep_low(s);
 		const int width = few ? FEW_CLASSES : tile_width(s, classes_of_piece(s)), tiles = ceil_div(s.classes, width);
 		GivenBack<T> to { teaching.anchors, nullptr, nullptr, nullptr };
 		const half_t *for_common = nullptr;
 		if constexpr (sizeof(T) == 2)
-			if (!few && dx != nullptr)
+			if (!few && !low && dx != nullptr)
 			{
 				to = GivenBack<T> { teaching.anchors, teaching.own, teaching.common, teaching.there };
 				for_common = w;
@@ -1055,12 +1059,12 @@ namespace
 		const auto goal = [&](int first_tile)
 		{
 			return TopClasses { nullptr, teaching.classes, teaching.shares, teaching.known, teaching.begins + first_tile, nullptr, count, tiles + 1, 1.0f / temperature, teaching.anchors,
-					for_common != nullptr ? teaching.own : nullptr };
+					for_common != nullptr ? teaching.own : nullptr, low };
 		};
 		if (few)
 			few_gradients(stream, s, x, w, bias, goal(0), teaching, lse, dloss, beta_dx, dx, beta_weights, dw, db, at<float>(workspace, space.d), at<float>(workspace, space.partial));
 		else
-			loss_backward(stream, s, x, w, bias, to, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), workspace);
+			loss_backward(stream, s, x, w, bias, to, goal, 1.0f / temperature, lse, dloss, beta_dx, dx, beta_weights, dw, db, few_logits(s), low, workspace);
 	}
 
 	/* the rows' shape with another last dimension */

@@ -282,6 +282,32 @@ namespace mlhip
 	 * dx += lost W[target]: the row adds up to zero again, and the target's element, the largest of d by far until a model is sure of something else, counts unrounded. dx is 2.1e-4 off then, as much as its own rounding
 	 * costs, and 2.6e-4 where other classes have large probabilities; dW, where nothing cancels, 2.8e-4. A goal that makes many elements large has more places to give it back to (GivenBack).
 	 */
+	/*
+	 * Up to 64 rows leave half of a tile empty. A goal that asks for it has what rounding leaves of d there, 64 rows further, so that both products take d with it: dx as two results that are added up, dW with x standing twice.
+	 * Few rows have few elements that are large, so roundings add up to anything (dW up to 1.6 times its own rounding's error), and dx and dW are now off by their own rounding alone. us of distillations' losses and gradients in fp16, so /
+	 * giving back: 9 rows of 512 x 20000 73 / 70, 40 rows 82 / 79, 24 of 1023 x 8000 92 / 94, 64 of 1024 x 32000 117 / 112, 64 of 2048 x 65536 342 / 321.
+	 */
+	constexpr int LOW_ROWS = 64;
+	/* what rounding left of v; an infinite one has no low part */
+	template<typename T>
+	__device__ __forceinline__ T low_part(float v, T rounded)
+	{
+		return static_cast<T>(fabsf(static_cast<float>(rounded)) < std::numeric_limits<float>::infinity() ? v - static_cast<float>(rounded) : 0.0f);
+	}
+	/* x [rows][columns] twice, in rows of whole pieces: from row 0 and from row LOW_ROWS on, zeros between and behind */
+	template<typename T>
+	__global__ __launch_bounds__(256) void kernel_rows_twice(const T *src, T *dst, int rows, int columns, int pieces)
+	{
+		constexpr int N = 16 / sizeof(T);
+		const int i = blockIdx.x * 256 + threadIdx.x, row = i / pieces, column = i % pieces * N, from = row % LOW_ROWS;
+		if (row >= 2 * LOW_ROWS)
+			return;
+		float v[N];
+#pragma unroll
+		for (int e = 0; e < N; e++)
+			v[e] = from < rows && column + e < columns ? static_cast<float>(src[static_cast<size_t>(from) * columns + column + e]) : 0.0f;
+		store_nearest<N>(dst + static_cast<size_t>(row) * pieces * N + column, v);
+	}
 	template<typename T, typename Goal>
 	struct GradientEpilogue
 	{
@@ -309,6 +335,10 @@ namespace mlhip
 			__device__ __forceinline__ void tile(const Acc (&acc)[TilePlace<BM, BN>::BLOCKS][2], const TilePlace<BM, BN> &at, uint8_t *lds, int rows) const
 			{
 				constexpr int BLOCKS = TilePlace<BM, BN>::BLOCKS, ROWS = (sizeof(T) == 2) ? BM : rows_at_a_time(BM), PASSES = BM / ROWS, WAVES_N = BN / 64;
+				constexpr bool MAY_KEEP = !Goal::ONE && sizeof(T) == 2 && BM == 2 * LOW_ROWS; /* low parts */
+				bool low = false;
+				if constexpr (MAY_KEEP)
+					low = goal.low;
 				static_assert((2 * BN + WAVES_N * BM) * static_cast<int>(sizeof(float)) <= GradientEpilogue::template stage_lds<BM, BN>(), "the sums meet where the rows were");
 				TileColumns<T, BM, BN> columns;
 				columns.begin(at, bias, classes);
@@ -341,6 +371,8 @@ namespace mlhip
 #pragma unroll
 					for (int i = FIRST; i < FIRST + BLOCKS / PASSES; i++)
 					{
+						if (MAY_KEEP && i == 1 && low)
+							continue; /* there are no such rows, their place is that of the low parts */
 						float v[2][16];
 #pragma unroll
 						for (int j = 0; j < 2; j++)
@@ -372,13 +404,21 @@ namespace mlhip
 #pragma unroll
 								for (int e = 0; e < 4; e++)
 									total[j][4 * q + e] += v[j][4 * q + e];
+								if (MAY_KEEP && low)
+								{
+									typename Stage<T, BN>::vec4_t rest;
+#pragma unroll
+									for (int e = 0; e < 4; e++)
+										rest[e] = low_part(v[j][4 * q + e], stored[e]);
+									stage.put(LOW_ROWS + at.row(i), at.column(j) + at.lane_column(q), rest);
+								}
 								if constexpr (sizeof(T) == 2)
 									taken[i] = add_what_rounding_takes(taken[i], &v[j][4 * q], stored);
 							}
 					}
 					__syncthreads();
 					goal.template correct<BM, BN, ROWS>(stage, lds + stage_lds<BM, BN>(), at, of_tile, PASS * ROWS, first_class);
-					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, rows, at.tile_n * BN, row_elements);
+					stage.template copy<ROWS, TilePlace<BM, BN>::THREADS>(d, row_elements, at.tile_m * BM + PASS * ROWS, low ? 2 * LOW_ROWS : rows, at.tile_n * BN, row_elements);
 				});
 				const bool of_columns = sums != nullptr, of_rows = sizeof(T) == 2 && lost != nullptr;
 				if (!of_columns && !of_rows)
@@ -681,7 +721,7 @@ namespace mlhip
 	struct LossSpace
 	{
 			size_t x, w, partials, target_logits; /* forward */
-			size_t d, dx, parts, sums, lost, factors, scale; /* backward */
+			size_t d, dx, parts, sums, lost, factors, scale, twice; /* backward */
 			size_t total;
 	};
 	/* whether dx comes about in fp32 first */
@@ -689,8 +729,18 @@ namespace mlhip
 	{
 		return piece < s.classes || input_plan(s, piece).parts > 1;
 	}
-	/* few: whether the forward pass streams the weights past a few rows, which asks for no padded copies */
-	inline LossSpace loss_space(const LossShape &s, bool backward, bool few)
+	/* whether a goal that asks for it has d's low parts kept: they lie in the rows of a tile that would be empty */
+	inline bool may_keep_low(const LossShape &s)
+	{
+		return s.element_size == 2 && s.rows <= LOW_ROWS && logits_plan(s, classes_of_piece(s)).tile == 2 * LOW_ROWS;
+	}
+	inline LossShape with_low(LossShape s, bool low)
+	{
+		s.rows = low ? 2 * LOW_ROWS : s.rows;
+		return s;
+	}
+	/* few: whether the forward pass streams the weights past a few rows, which asks for no padded copies; low: whether d's low parts are kept */
+	inline LossSpace loss_space(const LossShape &s, bool backward, bool few, bool low)
 	{
 		LossSpace space { };
 		size_t at = 0;
@@ -716,9 +766,11 @@ namespace mlhip
 				const size_t forward_end = at;
 				at = begin;
 				const int classes = classes_of_piece(s);
-				const ProductPlan input = input_plan(s, classes), weights = weights_plan(s, classes);
-				space.d = take(round_up(classes, pieces) * s.element_size * s.rows);
-				space.dx = take(dx_in_parts(s, classes) ? sizeof(float) * input.parts * s.rows * s.features : 0);
+				const LossShape all = with_low(s, low);
+				const ProductPlan input = input_plan(all, classes), weights = weights_plan(all, classes);
+				space.d = take(round_up(classes, pieces) * s.element_size * all.rows);
+				space.dx = take(low || dx_in_parts(s, classes) ? sizeof(float) * input.parts * all.rows * s.features : 0);
+				space.twice = take(low ? round_up(s.features, pieces) * s.element_size * all.rows : 0);
 				space.parts = take(part_bytes(weights, classes, s.features));
 				space.sums = take(sizeof(float) * classes * logits_plan(s, classes).tiles_m);
 				space.lost = take(s.element_size == 2 ? sizeof(float) * s.rows * ceil_div(s.classes, tile_width(s, classes)) : 0);
@@ -734,9 +786,10 @@ namespace mlhip
 	/* goal(first): for the piece whose first column of tiles it is */
 	template<typename T, typename GoalOf>
 	void loss_backward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const GivenBack<T> &to, GoalOf &&goal_of, float slope, const float *lse, const float *dloss, float beta_dx,
-			T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, bool few, uint8_t *workspace)
+			T *dx, float beta_weights, const mlTensor_t &dw, const mlTensor_t &db, bool few, bool low, uint8_t *workspace)
 	{
-		const LossSpace space = loss_space(s, true, few);
+		const LossSpace space = loss_space(s, true, few, low);
+		const LossShape all = with_low(s, low); /* rows of d */
 		const int padded = padded_columns<T>(s.features), most = classes_of_piece(s);
 		T *d = reinterpret_cast<T*>(workspace + space.d);
 		float *partial_dx = reinterpret_cast<float*>(workspace + space.dx), *parts = reinterpret_cast<float*>(workspace + space.parts);
@@ -751,11 +804,20 @@ namespace mlhip
 			hipLaunchKernelGGL(kernel_row_factors, dim3(groups), dim3(256), 0, stream, dloss, to.targets, s.rows, s.classes, largest, groups, slope, factors, back);
 		}
 		MLHIP_CHECK(hipGetLastError());
-		x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
+		if (low)
+		{
+			T *twice = reinterpret_cast<T*>(workspace + space.twice);
+			const int pieces = padded * static_cast<int>(sizeof(T)) / 16;
+			hipLaunchKernelGGL((kernel_rows_twice<T>), dim3(ceil_div(all.rows * pieces, 256)), dim3(256), 0, stream, x, twice, s.rows, s.features, pieces);
+			MLHIP_CHECK(hipGetLastError());
+			x = twice;
+		}
+		else
+			x = pad_rows(stream, x, reinterpret_cast<T*>(workspace + space.x), s.rows, s.features);
 		w = pad_rows(stream, w, reinterpret_cast<T*>(workspace + space.w), s.classes, s.features);
-		const size_t row_bytes = padded * sizeof(T), outputs = static_cast<size_t>(s.rows) * s.features;
-		const ProductPlan whole_input = input_plan(s, most);
-		const bool in_parts = dx_in_parts(s, most);
+		const size_t row_bytes = padded * sizeof(T), outputs = static_cast<size_t>(all.rows) * s.features;
+		const ProductPlan whole_input = input_plan(all, most);
+		const bool in_parts = low || dx_in_parts(s, most);
 		const int width = tile_width(s, most), lost_tiles = ceil_div(s.classes, width);
 		float *lost = reinterpret_cast<float*>(workspace + space.lost);
 		/* the last piece, which may be smaller, is cut by the plans of the others: the workspace is sized by them */
@@ -769,7 +831,7 @@ namespace mlhip
 				const Operand a { reinterpret_cast<const uint8_t*>(x), row_bytes, s.rows, padded };
 				const Operand b { weights, row_bytes, classes, padded };
 				launch_product<T, Side::ROWS, Side::ROWS, false>(stream, plan, a, b, s.rows, GradientEpilogue<T, decltype(goal_of(0))> { bias != nullptr ? bias + first : nullptr, goal_of(first / width), lse, factors, d,
-						db.data != nullptr ? sums : nullptr, dx != nullptr ? lost + first / width : nullptr, lost_tiles, first, classes, row_elements });
+						db.data != nullptr ? sums : nullptr, dx != nullptr && !low ? lost + first / width : nullptr, lost_tiles, first, classes, row_elements });
 				if (db.data != nullptr)
 					launch_sum_partials(stream, sums, plan.tiles_m, static_cast<size_t>(classes), static_cast<uint8_t*>(db.data) + static_cast<size_t>(first) * size_of(db.dtype), db.dtype, classes,
 							beta_weights, back);
@@ -778,10 +840,10 @@ namespace mlhip
 			{
 				ProductPlan plan = whole_input; /* a part that has no chunk left adds nothing */
 				plan.chunks = ceil_div(classes, 128 / static_cast<int>(sizeof(T)));
-				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), s.rows, row_elements };
+				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), all.rows, row_elements };
 				const Operand b { weights, row_bytes, padded, classes };
 				if (in_parts)
-					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
+					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, all.rows, PartEpilogue { partial_dx, outputs, s.features, first > 0 });
 				else if constexpr (sizeof(T) == 2)
 					launch_product<T, Side::ROWS, Side::COLUMNS, false>(stream, plan, a, b, s.rows, InputEpilogue<T, decltype(goal_of(0))::ONE> { dx, s.features, beta_dx, back, lost, lost_tiles, to, s.classes, w, padded });
 				else
@@ -789,10 +851,10 @@ namespace mlhip
 			}
 			if (dw.data != nullptr)
 			{
-				ProductPlan plan = weights_plan(s, most);
+				ProductPlan plan = weights_plan(all, most);
 				plan.tiles_m = ceil_div(classes, plan.tile);
-				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), row_elements, s.rows };
-				const Operand b { reinterpret_cast<const uint8_t*>(x), row_bytes, padded, s.rows };
+				const Operand a { reinterpret_cast<const uint8_t*>(d), row_elements * sizeof(T), row_elements, all.rows };
+				const Operand b { reinterpret_cast<const uint8_t*>(x), row_bytes, padded, all.rows };
 				const size_t offset = static_cast<size_t>(first) * s.features;
 				if (dw.dtype == DTYPE_FLOAT32)
 					product_to<T, float, Side::COLUMNS, Side::COLUMNS>(stream, plan, a, b, classes, s.features, ptr<float>(dw) + offset, beta_weights, back, parts);
@@ -800,7 +862,9 @@ namespace mlhip
 					product_to<T, T, Side::COLUMNS, Side::COLUMNS>(stream, plan, a, b, classes, s.features, ptr<T>(dw) + offset, beta_weights, back, parts);
 			}
 		}
-		if (dx != nullptr && in_parts)
+		if (dx != nullptr && low) /* [part][d, its low part][LOW_ROWS][features] */
+			launch_sum_partials(stream, partial_dx, 2 * whole_input.parts, static_cast<size_t>(LOW_ROWS) * s.features, dx, sizeof(T) == 2 ? DTYPE_FLOAT16 : DTYPE_FLOAT32, s.rows * s.features, beta_dx, back);
+		else if (dx != nullptr && in_parts)
 		{
 			if constexpr (sizeof(T) == 2)
 			{

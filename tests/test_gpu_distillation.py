@@ -195,6 +195,20 @@ def test_fp16_gradients_are_off_by_their_roundings_alone(ctx, rows, features, cl
     assert error <= 1.1 * V.distillation_input_noise(*args)
 
 
+@pytest.mark.parametrize("common", [0, 10])
+@pytest.mark.parametrize("rows,features,classes,count", [(9, 512, 2000, 24), (33, 333, 500, 16), (64, 200, 3001, 40), (17, 1024, 300, 1)])
+def test_fp16_gradients_of_few_rows_are_off_by_their_own_roundings_alone(ctx, rows, features, classes, count, common):
+    """Up to 64 rows what rounding leaves of d takes part in both products: dx and dW are as far off as rounding them makes them, a twelfth of a spacing squared for each element, of 4608 elements or more (a tenth is four
+    standard deviations and more)."""
+    rng = np.random.default_rng(rows + common)
+    x, w, b, named, logits, dloss = inputs(rng, rows, features, classes, count, "float16")
+    w = R.bits(R.numbers(w) + common * 2 / np.sqrt(features) * rng.standard_normal(features), "float16")
+    step = Distillation(ctx, x, w, b, named, logits, 2.0, "float16")
+    args = [R.numbers(a) for a in (x, w, b)] + [named, R.numbers(logits), 2.0, dloss.astype(np.float64)]
+    for got, want in zip(step.gradients(dloss)[:2], V.distillation_gradients(*args)):
+        assert np.linalg.norm(R.numbers(got) - want) <= 1.1 * np.sqrt((V.spacing(want) ** 2).sum() / 12)
+
+
 def test_rows_without_a_teacher_and_without_gradient(ctx):
     rng = np.random.default_rng(9)
     for rows in (9, 90):
