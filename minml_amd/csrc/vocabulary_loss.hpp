@@ -277,12 +277,6 @@ namespace mlhip
 		return __builtin_amdgcn_fdot2(half2_t { stored[2], stored[3] }, minus_ones, sum + (v[2] + v[3]), false);
 	}
 	/*
-	 * d, the sums of its columns for db, and what rounding to fp16 took from its rows. The elements of a row add up to zero by definition, so that what the rows of W have in common has no part in dx; their roundings
-	 * do not, and with W's common part ten times the rest dx would be 1.9e-3 off (2.8e-4 without one). What was taken from a row is therefore added up here, in fp32, and given back to the target's class when dx is made,
-	 * dx += lost W[target]: the row adds up to zero again, and the target's element, the largest of d by far until a model is sure of something else, counts unrounded. dx is 2.1e-4 off then, as much as its own rounding
-	 * costs, and 2.6e-4 where other classes have large probabilities; dW, where nothing cancels, 2.8e-4. A goal that makes many elements large has more places to give it back to (GivenBack).
-	 */
-	/*
 	 * Up to 64 rows leave half of a tile empty. A goal that asks for it has what rounding leaves of d there, 64 rows further, so that both products take d with it: dx as two results that are added up, dW with x standing twice.
 	 * Few rows have few elements that are large, so roundings add up to anything (dW up to 1.6 times its own rounding's error), and dx and dW are now off by their own rounding alone. us of distillations' losses and gradients in fp16, so /
 	 * giving back: 9 rows of 512 x 20000 73 / 70, 40 rows 82 / 79, 24 of 1023 x 8000 92 / 94, 64 of 1024 x 32000 117 / 112, 64 of 2048 x 65536 342 / 321.
@@ -308,6 +302,12 @@ namespace mlhip
 			v[e] = from < rows && column + e < columns ? static_cast<float>(src[static_cast<size_t>(from) * columns + column + e]) : 0.0f;
 		store_nearest<N>(dst + static_cast<size_t>(row) * pieces * N + column, v);
 	}
+	/*
+	 * d, the sums of its columns for db, and what rounding to fp16 took from its rows. The elements of a row add up to zero by definition, so that what the rows of W have in common has no part in dx; their roundings
+	 * do not, and with W's common part ten times the rest dx would be 1.9e-3 off (2.8e-4 without one). What was taken from a row is therefore added up here, in fp32, and given back to the target's class when dx is made,
+	 * dx += lost W[target]: the row adds up to zero again, and the target's element, the largest of d by far until a model is sure of something else, counts unrounded. dx is 2.1e-4 off then, as much as its own rounding
+	 * costs, and 2.6e-4 where other classes have large probabilities; dW, where nothing cancels, 2.8e-4. A goal that makes many elements large has more places to give it back to (GivenBack).
+	 */
 	template<typename T, typename Goal>
 	struct GradientEpilogue
 	{
