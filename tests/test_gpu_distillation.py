@@ -108,6 +108,11 @@ def test_more_classes_than_one_piece_holds(ctx):
         assert R.worst(got.copyToHost(ctx), exact + beta * old.astype(np.float64), off + 2 * R.rounded(old, "float32")) <= 1
 
 
+def test_more_classes_than_one_piece_holds_of_few_rows(ctx):
+    """A piece has 524288 classes at most; the rows' low parts lie behind d's rows in both."""
+    check(ctx, inputs(np.random.default_rng(12), 20, 8, 530000, 9, "float16"), 2.0, "float16")
+
+
 @pytest.mark.parametrize("dtype", ["float16", "float32"])
 def test_gradients_are_added_and_may_be_left_out(ctx, dtype):
     rng = np.random.default_rng(3)
