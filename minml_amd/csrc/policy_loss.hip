@@ -5,6 +5,8 @@
  *   r = exp(o - n),   gain = min(r A, clip(r, 1 - low, 1 + high) A),   q = n - f,   kl = exp(q) - q - 1,   loss = -gain + kl_weight kl
  * The result is the mean over the tokens, or over the sequences' means; the gradient of n is the token's weight times ([not clipped] r A + kl_weight (exp(q) - 1)).
  * Whether a token is clipped is decided in 64 bits by o - n against the logarithm of the border (r > 1 + high where A > 0, r < 1 - low where A < 0), so no rounding of an exponential moves a token across it.
+ * r is a number of 64 bits that holds 32: beyond exp(88) it is none of fp32, but its product with an advantage or a weight may be one, and with an advantage of 0 is 0. A token without an advantage has no gain whatever its
+ * likelihoods are, as long as they are numbers or infinite.
  * kl of close models is a small number from which 1 and q have been taken: below |q| = 1/2 it is q^2 (1/2 + q/6 + ..), where nothing cancels. Sums are in 64 bits: gains have both signs and cancel.
  * Memory bounds both passes, 12 to 20 bytes of a token: 1024 sequences of 8191 tokens, all five inputs, 28 us and 5 to join the sums (6.0 TB/s), the gradient 30 (6.8, partly from the last-level cache); 512 x 1024 6.2 and 2.9.
  */
@@ -24,26 +26,34 @@ namespace
 			int sequences, length, classes;
 			bool per_token; /* advantages: of every token, else of every sequence */
 			double log_low, log_high;
-			float low, high, kl_weight;
+			double low, high;
+			float kl_weight;
 	};
 	struct TokenLoss
 	{
-			float gain, slope, kl, kl_slope;
+			double gain, slope, kl, kl_slope;
 			bool clipped;
 	};
+	/* exp(x) = 2^f 2^n with the 32 bits of the hardware's 2^f, f in [-1/2, 1/2], at any power of two that 64 bits reach. Infinities and NaN, and what is beyond, go by f: so does what is left of x by then */
+	__device__ __forceinline__ double exp_of(double x)
+	{
+		const double t = x * 1.4426950408889634 /* 1 / log 2 */, n = rint(fmin(fmax(t, -1100.0), 1100.0));
+		return ldexp(static_cast<double>(__builtin_amdgcn_exp2f(static_cast<float>(t - n))), static_cast<int>(n));
+	}
 	__device__ __forceinline__ TokenLoss token_loss(const PolicyArgs &p, float nll, float old, float reference, float advantage)
 	{
 		TokenLoss t;
 		const double d = static_cast<double>(old) - static_cast<double>(nll);
 		const bool up = advantage > 0.0f && d > p.log_high, down = advantage < 0.0f && d < p.log_low;
 		t.clipped = up || down;
-		const float free = expf(static_cast<float>(d)) * advantage;
-		t.gain = up ? p.high * advantage : down ? p.low * advantage : free;
-		t.slope = t.clipped ? 0.0f : free;
-		t.kl = t.kl_slope = 0.0f;
+		const double a = static_cast<double>(advantage), free = (a == 0.0 && d == d) ? 0.0 : exp_of(d) * a;
+		t.gain = up ? p.high * a : down ? p.low * a : free;
+		t.slope = t.clipped ? 0.0 : free;
+		t.kl = t.kl_slope = 0.0;
 		if (p.reference != nullptr)
 		{
-			const float q = static_cast<float>(static_cast<double>(nll) - static_cast<double>(reference));
+			const double wide = static_cast<double>(nll) - static_cast<double>(reference);
+			const float q = static_cast<float>(wide);
 			/* the terms left out are below 2^-28 of the sum */
 			float series = 1.0f / 362880.0f;
 			series = fmaf(series, q, 1.0f / 40320.0f);
@@ -53,10 +63,11 @@ namespace
 			series = fmaf(series, q, 1.0f / 24.0f);
 			series = fmaf(series, q, 1.0f / 6.0f);
 			series = fmaf(series, q, 0.5f);
-			const float close = series * q * q, beyond = expf(q) - 1.0f;
+			const float close = series * q * q;
+			const double beyond = exp_of(wide) - 1.0;
 			const bool is_close = fabsf(q) < 0.5f;
-			t.kl = is_close ? close : beyond - q;
-			t.kl_slope = is_close ? close + q : beyond;
+			t.kl = is_close ? static_cast<double>(close) : beyond < HUGE_VAL ? beyond - wide : beyond;
+			t.kl_slope = is_close ? static_cast<double>(close + q) : beyond;
 		}
 		return t;
 	}
@@ -163,8 +174,8 @@ namespace
 				if (tokens.there(p, e))
 				{
 					const TokenLoss t = tokens.loss(p, e);
-					sums.gain += static_cast<double>(t.gain);
-					sums.kl += static_cast<double>(t.kl);
+					sums.gain += t.gain;
+					sums.kl += t.kl;
 					clipped += t.clipped ? 1 : 0;
 					count++;
 				}
@@ -292,7 +303,7 @@ namespace
 			float *dst = place.in(dnll + static_cast<size_t>(sequence) * p.length);
 			Tokens<VEC> tokens;
 			tokens.load(p, sequence, vector * VEC);
-			const float weight = weights[sequence] * scale;
+			const double weight = static_cast<double>(weights[sequence]) * static_cast<double>(scale);
 			Elements<float, VEC> before;
 			if (beta != 0.0f)
 				before.load(dst);
@@ -304,7 +315,7 @@ namespace
 				if (tokens.there(p, e))
 				{
 					const TokenLoss t = tokens.loss(p, e);
-					v[e] = weight * fmaf(p.kl_weight, t.kl_slope, t.slope);
+					v[e] = static_cast<float>(weight * fma(static_cast<double>(p.kl_weight), t.kl_slope, t.slope));
 				}
 				if (beta != 0.0f)
 					v[e] = fmaf(beta, before[e], v[e]);
@@ -391,7 +402,7 @@ namespace
 		MLHIP_REQUIRE(std::isfinite(kl_weight), who + ": the divergence's weight must be finite");
 		const double low = 1.0 - clip_low, high = 1.0 + clip_high;
 		return PolicyArgs { ptr<float>(nll), ptr<float>(old), ptr<float>(reference), ptr<float>(advantages), ptr<int>(targets), s.sequences, s.length, classes, given == tokens,
-				low > 0.0 ? std::log(low) : -HUGE_VAL, std::log(high), static_cast<float>(std::max(low, 0.0)), static_cast<float>(high), reference.data != nullptr ? kl_weight : 0.0f };
+				low > 0.0 ? std::log(low) : -HUGE_VAL, std::log(high), std::max(low, 0.0), high, reference.data != nullptr ? kl_weight : 0.0f };
 	}
 }
 

@@ -159,3 +159,49 @@ def test_tensors_that_begin_at_any_element(ctx):
         ml.policyLossBackward(ctx, *shifted, CLASSES, CLIP, KL_WEIGHT, weights, None, 0.0, dnll)
         assert np.array_equal(loss.copyToHost(ctx), plain.loss.copyToHost(ctx)) and np.array_equal(weights.copyToHost(ctx), plain.weights.copyToHost(ctx))
         assert np.array_equal(dnll.copyToHost(ctx), plain.gradient())
+
+
+def test_ratios_beyond_fp32(ctx):
+    """exp(100) is no number of fp32: an advantage of 0 makes nothing of it, a positive one is held by the clip, a negative one counts with what the product is, if that is a number again; whole sequences, one after the other,
+    by 8 threads, by a wavefront and by a workgroup."""
+    advantages = np.array([0, 1, -2.0 ** -70, 0, 2, -2.0 ** -100], np.float32)
+    for length in (3, 50, 500, 2000):
+        for per_token in (False, True):
+            old, nll = np.repeat(np.array([[101, 101, 101, 1, 1, 131], [1, 1, 1, 121, 121, 1]], np.float32)[:, :, None], length, 2)
+            given = np.repeat(advantages[:, None], length, 1) if per_token else advantages
+            targets = np.zeros(old.shape, np.int32)
+            for average in ("tokens", "sequences"):
+                step = Loss(ctx, nll, old, None, given, targets, average=average)
+                loss, _, gradient = exact(nll, old, None, given, targets, average)[0]
+                assert np.isfinite(gradient).all() and (gradient[[0, 1, 3]] == 0).all() and abs(gradient[2]).min() > 0
+                # an exponent of up to 130, rounded, an exponential, a product and the means, all of one sign beside the few clipped ones; nothing where it is 0
+                assert R.worst(step.loss.copyToHost(ctx), loss, 146 * R.FP32 * abs(loss) + 1e-300) <= 1 and R.worst(step.gradient(), gradient, 146 * R.FP32 * abs(gradient) + 2.0 ** -140) <= 1
+
+
+def test_infinite_ratios_without_advantage(ctx):
+    """A token that was impossible when it was sampled (old_nll inf) or is now (nll inf): nothing without an advantage, but a likelihood that is no number is none."""
+    old, nll = np.array([[np.inf, 1, 1, 1]], np.float32), np.array([[1, np.inf, 1, 2]], np.float32)
+    advantages, targets = np.zeros((1, 4), np.float32), np.zeros((1, 4), np.int32)
+    step = Loss(ctx, nll, old, None, advantages, targets)
+    assert (step.loss.copyToHost(ctx) == 0).all() and (step.gradient() == 0).all()
+    nll[0, 2] = np.nan
+    step = Loss(ctx, nll, old, None, advantages, targets)
+    assert np.isnan(step.loss.copyToHost(ctx)[0]) and np.array_equal(np.isnan(step.gradient()), [[False, False, True, False]])
+
+
+def test_divergences_beyond_fp32(ctx):
+    """exp(q) - q - 1 of q = 100 is no number of fp32, but a small weight makes one of it; of an impossible token it is infinite, not undefined."""
+    rng = np.random.default_rng(5)
+    for length in (3, 50, 2000):
+        nll = rng.uniform(0.5, 2, (4, length)).astype(np.float32)
+        nll[1] += 100
+        old, reference, advantages, targets = nll.copy(), np.ones(nll.shape, np.float32), np.ones(4, np.float32), np.zeros(nll.shape, np.int32)
+        weight = float(np.float32(1e-20))
+        step = Loss(ctx, nll, old, reference, advantages, targets, kl_weight=weight)
+        (loss, _, gradient), (loss_off, _, gradient_off) = exact(nll, old, reference, advantages, targets, "tokens", kl_weight=weight)
+        assert loss[0] > 1e20 and R.worst(step.gradient(), gradient, gradient_off) <= 1
+        got = step.loss.copyToHost(ctx)
+        assert got[2] == np.inf and R.worst(got[[0, 1, 3]], loss[[0, 1, 3]], loss_off[[0, 1, 3]]) <= 1
+        nll[1, 0] = np.inf
+        step = Loss(ctx, nll, old, reference, advantages, targets)
+        assert np.array_equal(step.loss.copyToHost(ctx)[[0, 2]], [np.inf, np.inf])
