@@ -302,7 +302,8 @@ extern "C"
 	 * The clipped policy loss over sampled tokens, fp32 [sequences, tokens] (or [tokens] of one sequence): nll, the negative log likelihoods that hip_linear_cross_entropy_forward gives as its loss; old_nll, what they were when
 	 * the tokens were sampled; reference_nll, those of a model to stay close to, or empty; advantages of every sequence or of every token; targets int32 as for the cross entropy: a token whose target is none of
 	 * 0 .. classes - 1 (prompts, padding) has no part in anything, whatever the other tensors hold for it. With r = exp(old_nll - nll) and q = nll - reference_nll a token's loss is
-	 *     -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(q) - q - 1).
+	 *     -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(q) - q - 1),
+	 * without the second part where kl_weight is 0, whatever the reference says (its mean is given all the same), and without the first one where A is 0.
 	 * loss fp32 [4]: the mean loss, its two parts -min(..) and exp(q) - q - 1, and the share of tokens that the clip holds. AVERAGE_TOKENS: over all tokens; AVERAGE_SEQUENCES: over the means of the sequences that have tokens.
 	 * Without any token all four are 0. weights fp32 [sequences]: what a token of each sequence counts in the means, for the backward pass.
 	 * Backward: dnll = beta * dnll + the gradient of nll for the loss's gradient dloss (one fp32 number on the device, or empty for 1); it is hip_linear_cross_entropy_backward's dloss.

@@ -919,7 +919,7 @@ def policyLossGetWorkspaceSize(context, nll):
 def policyLossForward(context, nll, old_nll, reference_nll, advantages, targets, classes, clip, kl_weight, average, loss, weights, workspace):
     """loss fp32 [4] = the mean of -min(r A, clip(r, 1 - clip[0], 1 + clip[1]) A) + kl_weight (exp(q) - q - 1) with r = exp(old_nll - nll) and q = nll - reference_nll, its two parts, and the share
     of clipped tokens. nll (linearCrossEntropyForward's loss) and the others fp32 [sequences, tokens], advantages [sequences, tokens] or [sequences], reference_nll may be None. A token whose target is
-    none of 0 .. classes - 1 has no part in it. average: "tokens" or "sequences" (of the means of the sequences that have tokens). weights fp32 [sequences] are for policyLossBackward."""
+    none of 0 .. classes - 1 has no part in it; with a kl_weight of 0 the reference has none in loss[0] and the gradient. average: "tokens" or "sequences" (of the means of the sequences that have tokens). weights fp32 [sequences] are for policyLossBackward."""
     sequences = _require_policy(nll, old_nll, reference_nll, advantages, targets, clip)
     _require(average in AVERAGES or average in AVERAGES.values(), "unknown average")
     _require(loss.dtype == B.DTYPE_FLOAT32 and loss.volume() == 4, "the loss must be fp32 [4]")

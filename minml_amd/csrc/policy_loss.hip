@@ -2,7 +2,7 @@
  * policy_loss.hip — the clipped policy loss over the likelihoods of sampled tokens with a penalty for leaving a reference model, and its gradient.
  *
  * Of a token with negative log likelihood n now, o when it was sampled and f by the reference, and with advantage A:
- *   r = exp(o - n),   gain = min(r A, clip(r, 1 - low, 1 + high) A),   q = n - f,   kl = exp(q) - q - 1,   loss = -gain + kl_weight kl
+ *   r = exp(o - n),   gain = min(r A, clip(r, 1 - low, 1 + high) A),   q = n - f,   kl = exp(q) - q - 1,   loss = -gain + kl_weight kl (with a weight of 0 without kl, whatever it is)
  * The result is the mean over the tokens, or over the sequences' means; the gradient of n is the token's weight times ([not clipped] r A + kl_weight (exp(q) - 1)).
  * Whether a token is clipped is decided in 64 bits by o - n against the logarithm of the border (r > 1 + high where A > 0, r < 1 - low where A < 0), so no rounding of an exponential moves a token across it.
  * r is a number of 64 bits that holds 32: beyond exp(88) it is none of fp32, but its product with an advantage or a weight may be one, and with an advantage of 0 is 0. A token without an advantage has no gain whatever its
@@ -149,7 +149,7 @@ namespace
 	__device__ __forceinline__ void write_loss(const Sums &total, double each, float kl_weight, float *loss)
 	{
 		const double gain = total.gain * each, kl = total.kl * each;
-		loss[0] = static_cast<float>(kl_weight * kl - gain);
+		loss[0] = static_cast<float>((kl_weight != 0.0f ? kl_weight * kl : 0.0) - gain);
 		loss[1] = static_cast<float>(-gain);
 		loss[2] = static_cast<float>(kl);
 		loss[3] = static_cast<float>(total.clipped * each);
@@ -315,7 +315,7 @@ namespace
 				if (tokens.there(p, e))
 				{
 					const TokenLoss t = tokens.loss(p, e);
-					v[e] = static_cast<float>(weight * fma(static_cast<double>(p.kl_weight), t.kl_slope, t.slope));
+					v[e] = static_cast<float>(weight * (p.kl_weight != 0.0f ? fma(static_cast<double>(p.kl_weight), t.kl_slope, t.slope) : t.slope));
 				}
 				if (beta != 0.0f)
 					v[e] = fmaf(beta, before[e], v[e]);

@@ -205,3 +205,20 @@ def test_divergences_beyond_fp32(ctx):
         nll[1, 0] = np.inf
         step = Loss(ctx, nll, old, reference, advantages, targets)
         assert np.array_equal(step.loss.copyToHost(ctx)[[0, 2]], [np.inf, np.inf])
+
+
+@pytest.mark.parametrize("average", ["tokens", "sequences"])
+def test_divergences_without_weight(ctx, average):
+    """With a weight of 0 the reference has no part in the loss and its gradient, however far away it is: the bits are those of a call without one, and the mean divergence is given all the same."""
+    rng = np.random.default_rng(6)
+    for sequences, length in ((3, 3), (5, 60), (40, 700), (2, 9000)):
+        data = list(inputs(rng, sequences, length))
+        data[4][0, 0] = 1
+        nothing = Loss(ctx, data[0], data[1], None, *data[3:], kl_weight=0.0, average=average)
+        for far, mean in ((data[0] - 100, np.inf), (data[0] - 1000, np.inf), (np.full_like(data[0], -np.inf), np.inf), (np.full_like(data[0], np.nan), np.nan), (data[0] - 1, np.e - 2)):
+            data[2] = far.astype(np.float32)
+            step = Loss(ctx, *data, kl_weight=0.0, average=average)
+            loss, want = step.loss.copyToHost(ctx), nothing.loss.copyToHost(ctx)
+            assert np.array_equal(loss[[0, 1, 3]], want[[0, 1, 3]]) and np.isfinite(loss[0]) and np.array_equal(step.gradient(), nothing.gradient())
+            # nll - 1 is rounded to fp32, by 2^-24 of numbers up to 8 beside a slope of e - 1
+            assert (np.array_equal(loss[2], mean, equal_nan=True) if not np.isfinite(mean) else abs(loss[2] - mean) < 32 * R.FP32)
