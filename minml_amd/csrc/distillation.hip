@@ -6,6 +6,7 @@
  *   q[i, k] = softmax over k of v[i, k] / t,   loss[i] = sum_k q[i, k] (log q[i, k] - log p[i, k])
  *   d[i, j] = (exp(z[i, j] - lse[i]) - sum over k with c[i, k] = j of q[i, k]) dloss[i] / t,   dx = d W,   dW = d^T x,   db[j] = sum_i d[i, j]
  *
+ * q is of (v - largest v) / t: of v / t the rounding alone would be off by |v / t| 2^-24, and at a small t it is no number of fp32.
  * A place k whose class c is none of the layer's, or whose logit v is -inf, does not count; a row without any that does has loss 0 and no gradient. A class that a row names twice has the sum of both probabilities.
  * The passes are the cross entropy's (vocabulary_loss.hpp). What is new is that a row has many classes of its own, spread over the tiles of logits. A launch before sorts every row's classes and notes where each column of tiles
  * begins among them; then one thread of a tile has a row's few in that tile, and they meet the logits in LDS, through which the tile goes anyway in the backward pass, and in the forward pass where it has any.
@@ -117,7 +118,7 @@ namespace
 		{
 			const int k = k0 + lane;
 			const int c = k < count ? classes_in[base + k] : -1;
-			const float v = k < count ? static_cast<float>(logits[base + k]) / temperature : 0.0f;
+			const float v = k < count ? static_cast<float>(logits[base + k]) : 0.0f;
 			const bool counts = c >= 0 && c < classes && !(v == -std::numeric_limits<float>::infinity());
 			const uint64_t all = __ballot(counts), none = __ballot(k < count && !counts);
 			if (k < stride)
@@ -136,7 +137,7 @@ namespace
 		for (int k = lane; k < count; k += 64)
 			if (named[k] != 0x7fffffff)
 			{
-				values[k] = expf(values[k] - top);
+				values[k] = expf((values[k] - top) / temperature);
 				sum += values[k];
 			}
 		sum = lanes_sum<64>(sum);
@@ -515,7 +516,7 @@ namespace
 		for (int k = threadIdx.x; k < count; k += 256)
 		{
 			const int c = classes_in[base + k];
-			const float v = static_cast<float>(taught[base + k]) / temperature;
+			const float v = static_cast<float>(taught[base + k]);
 			const bool counts = c >= 0 && c < classes && !(v == -std::numeric_limits<float>::infinity());
 			named[k] = counts ? c : -1;
 			shares[k] = v;
@@ -546,7 +547,7 @@ namespace
 		for (int k = threadIdx.x; k < count; k += 256)
 			if (named[k] >= 0)
 			{
-				shares[k] = expf(shares[k] - top);
+				shares[k] = expf((shares[k] - top) / temperature);
 				sum += shares[k];
 			}
 		sum = of_all(sum, add); /* behind its barriers every share is there for all */

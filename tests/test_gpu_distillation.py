@@ -265,3 +265,42 @@ def test_the_same_bits_every_time(ctx):
     first = step.gradients(dloss)
     for _ in range(3):
         assert all(np.array_equal(a, b) for a, b in zip(first, step.gradients(dloss)))
+
+
+@pytest.mark.parametrize("dtype,logits_dtype", [("float16", "float16"), ("float16", "float32"), ("float32", "float32")])
+@pytest.mark.parametrize("rows", [3, 20, 130])
+def test_probabilities_of_the_teacher_at_a_small_temperature(ctx, rows, dtype, logits_dtype):
+    """Logits of about 20 at a temperature of 0.01: v / t is about 2000, whose rounding to fp32 would take 6e-5 of a probability, but only v - max v counts. The student's logits are zeros, and no class is named twice, so db
+    is what all rows have of it, 1 / 4000 each, less the one probability of the teacher."""
+    rng = np.random.default_rng(rows)
+    classes, count, temperature = 4000, 20, float(np.float32(0.01))
+    named = rng.permutation(classes)[:rows * count].reshape(rows, count).astype(np.int32)
+    logits = R.bits(20 + 0.05 * rng.random((rows, count)), logits_dtype)
+    x, w, b = (R.bits(a, dtype) for a in (rng.standard_normal((rows, 16)), np.zeros((classes, 16)), np.zeros(classes)))
+    step = Distillation(ctx, x, w, b, named, logits, temperature, dtype)
+    db = ml.Tensor((classes,), "float32")
+    step.backward(np.ones(rows, np.float32), None, None, db)
+    dense, q, _ = V.teacher(named, R.numbers(logits), classes, temperature)
+    # v - max v is exact (both are between 16 and 32); the quotient, up to 6, is rounded once; 24 roundings for the exponential, the sum's joins and the division; the sum's additions
+    relative = R.FP32 * (6 + 24 + count / 32)
+    p = rows / classes
+    # the student's: lse is 8.3, rounded, the hardware's exponential takes 8.3 log2(e) in fp32: below 2^-18
+    assert R.worst(db.copyToHost(ctx), (p - dense.sum(0)) / temperature, (dense.sum(0) * (relative + 4 * R.FP32) + p * 2.0 ** -18) / temperature) <= 1
+    log_q = np.log(q)
+    loss = (q * (log_q + np.log(classes))).sum(1)
+    assert R.worst(step.loss.copyToHost(ctx), loss, (relative + 24 * R.FP32) * (q * (np.abs(log_q) + np.log(classes) + 1)).sum(1)) <= 1
+
+
+@pytest.mark.parametrize("rows", [3, 20, 130])
+def test_a_temperature_that_makes_infinities(ctx, rows):
+    """At 1e-38 a logit of 5 over it is none of fp32, and one of -5 is no -inf that does not count: the teacher is sure of its best class, or of both."""
+    rng = np.random.default_rng(rows)
+    classes = 300
+    named, logits = np.array([[7, 8, 9], [10, -1, -1], [20, 30, 40]], np.int32), np.array([[4, 5, -5], [-5, 9, 9], [7, 7, 6]], np.float32)
+    named, logits = (np.tile(a, (rows // 3 + 1, 1))[:rows] for a in (named, logits))
+    x, w, b = rng.standard_normal((rows, 16)).astype(np.float32), np.zeros((classes, 16), np.float32), np.zeros(classes, np.float32)
+    step = Distillation(ctx, x, w, b, named, logits, 1e-38, "float32")
+    want = np.tile(np.log(classes) - np.array([0, 0, np.log(2)]), rows // 3 + 1)[:rows]
+    # logarithms below 8 and sums of them
+    assert R.worst(step.loss.copyToHost(ctx), want, np.full(rows, 32 * R.FP32)) <= 1
+    assert R.worst(step.log_p.copyToHost(ctx), np.where(named >= 0, -np.log(classes), 0), np.full(named.shape, 32 * R.FP32)) <= 1
