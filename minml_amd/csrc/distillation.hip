@@ -97,15 +97,15 @@ namespace
 		if (column0 == 0 && threadIdx.x == 0)
 			*there = rows > 0 ? 1.0f : 0.0f;
 	}
-	/* a wavefront per row; workgroups behind the rows': common_row. What a class's place is, is counted: as many classes are smaller, or equal and named before. L: type of the logits */
+	/* a wavefront per row from first_row on; workgroups behind the rows': common_row. What a class's place is, is counted: as many classes are smaller, or equal and named before. L: type of the logits */
 	template<typename L>
-	__global__ __launch_bounds__(256) void kernel_sort_teacher(const int *classes_in, const L *logits, const float *log_probabilities, int rows, int count, int classes, float temperature, int width, int tiles, const half_t *w, int features, Teaching out)
+	__global__ __launch_bounds__(256) void kernel_sort_teacher(const int *classes_in, const L *logits, const float *log_probabilities, int first_row, int groups, int rows, int count, int classes, float temperature, int width, int tiles, const half_t *w,
+			int features, Teaching out)
 	{
 		extern __shared__ __attribute__((aligned(16))) int memory[];
-		const int groups = (rows + 3) / 4;
 		if (static_cast<int>(blockIdx.x) >= groups)
 			return common_row(classes_in, logits, static_cast<size_t>(rows) * count, classes, w, features, (static_cast<int>(blockIdx.x) - groups) * 64, out.common, out.there);
-		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave;
+		const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = first_row + static_cast<int>(blockIdx.x) * 4 + wave;
 		if (row >= rows)
 			return;
 		const int stride = places_in_lds(count);
@@ -920,17 +920,24 @@ namespace
 			const Teaching &out)
 	{
 		const int tiles = ceil_div(s.classes, width), bytes = 4 * 4 * static_cast<int>(sizeof(int)) * places_in_lds(count);
-		const int groups = ceil_div(s.rows, 4) + (w != nullptr ? static_cast<int>(round_up(s.features, COMMON_COLUMNS)) / 64 : 0);
+		/* a launch has less than 2^32 threads, so 2^26 rows and more go out in several (a loop over the rows in the kernel would take 2 us of every call); the common row in the last one */
+		constexpr int MOST_ROWS = 1 << 25;
 		const auto launch = [&](auto kernel, auto values)
 		{
 			ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes);
-			hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), bytes, stream, ptr<int>(classes), values, log_probabilities, s.rows, count, s.classes, temperature, width, tiles, w, s.features, out);
+			for (int first = 0; first < s.rows; first += MOST_ROWS)
+			{
+				const int groups = ceil_div(std::min(MOST_ROWS, s.rows - first), 4);
+				const int others = w != nullptr && s.rows - first <= MOST_ROWS ? static_cast<int>(round_up(s.features, COMMON_COLUMNS)) / 64 : 0;
+				hipLaunchKernelGGL(kernel, dim3(groups + others), dim3(256), bytes, stream, ptr<int>(classes), values, log_probabilities, first, groups, s.rows, count, s.classes, temperature, width, tiles, w,
+						s.features, out);
+				MLHIP_CHECK(hipGetLastError());
+			}
 		};
 		if (logits.dtype == DTYPE_FLOAT16)
 			launch(kernel_sort_teacher<half_t>, static_cast<const half_t*>(ptr<half_t>(logits)));
 		else
 			launch(kernel_sort_teacher<float>, static_cast<const float*>(ptr<float>(logits)));
-		MLHIP_CHECK(hipGetLastError());
 	}
 	template<typename T>
 	void distillation_forward(hipStream_t stream, const LossShape &s, const T *x, const T *w, const T *bias, const mlTensor_t &classes, const mlTensor_t &logits, int count, float temperature, float *loss,

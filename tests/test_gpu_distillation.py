@@ -304,3 +304,41 @@ def test_a_temperature_that_makes_infinities(ctx, rows):
     # logarithms below 8 and sums of them
     assert R.worst(step.loss.copyToHost(ctx), want, np.full(rows, 32 * R.FP32)) <= 1
     assert R.worst(step.log_p.copyToHost(ctx), np.where(named >= 0, -np.log(classes), 0), np.full(named.shape, 32 * R.FP32)) <= 1
+
+
+def test_more_rows_than_a_launch_has_wavefronts_for(ctx):
+    """2^26 + 5 rows of zeros and three classes: the student's distribution is that of the bias alone, the teacher's is all of class 0, which it names twice; a few rows have a teacher of their own. dx is checked at them, and db,
+    which is a sum of equal numbers but for them, over all."""
+    rows, classes, features = 2 ** 26 + 5, 3, 8
+    picked = {0: (1, 2), 4: (2, -1), 2 ** 22 + 3: (0, 1), 2 ** 26 - 1: (1, 1), 2 ** 26: (2, 1), rows - 1: (-1, 1)}
+    x, named, logits = ml.Tensor((rows, features), "float16"), ml.Tensor((rows, 2), "int32"), ml.Tensor((rows, 2), "float16")
+    for t in (x, named, logits):
+        t.zeroall(ctx)
+    for row, c in picked.items():
+        named.view((2,), 2 * row).copyFromHost(ctx, np.array(c, np.int32))
+    w, bias = R.bits(np.arange(24).reshape(classes, features) / 16, "float16"), np.array([0.0, 1.0, -2.0])
+    W, B = ml.toDevice(ctx, w), ml.toDevice(ctx, R.bits(bias, "float16"))
+    loss, lse, log_p, dloss, dx, db = (ml.Tensor(s, d) for s, d in (((rows,), "float32"), ((rows,), "float32"), ((rows, 2), "float32"), ((rows,), "float32"), ((rows, features), "float16"), ((classes,), "float32")))
+    dloss.setall(ctx, 1.0)
+    work = ml.Tensor((ml.linearDistillationGetWorkspaceSize(ctx, x, W, 2, True),), "uint8")
+    ml.linearDistillationForward(ctx, x, W, B, named, logits, 1.0, loss, lse, log_p, work)
+    ml.linearDistillationBackward(ctx, x, W, B, named, logits, 1.0, lse, log_p, dloss, 0.0, dx, 0.0, None, db, work)
+    p = np.exp(bias) / np.exp(bias).sum()
+    losses, log_ps = loss.copyToHost(ctx), log_p.copyToHost(ctx)
+    total, others = rows * p, np.ones(rows, bool)
+    total[0] -= rows - len(picked)
+    for row, c in picked.items():
+        q = np.zeros(classes)
+        for v in c:
+            if v >= 0:
+                q[v] += 1 / (np.array(c) >= 0).sum()
+        total -= q
+        others[row] = False
+        want = sum(v * (np.log(v) - np.log(p[k])) for k, v in enumerate(q) if v > 0)
+        assert abs(losses[row] - want) <= 40 * R.FP32  # as for the cross entropy of as many rows
+        assert np.abs(log_ps[row] - np.array([np.log(p[v]) if v >= 0 else 0 for v in c])).max() <= 40 * R.FP32
+        # d of up to 1 in fp16, three of them times weights up to 1.5, and the result's rounding
+        assert np.abs(R.numbers(dx.view((features,), row * features).copyToHost(ctx)) - (p - q) @ R.numbers(w)).max() <= 4 * 3 * R.STEP["float16"]
+    assert np.abs(losses[others] + np.log(p[0])).max() <= 40 * R.FP32 and np.abs(log_ps[others] - np.log(p[0])).max() <= 40 * R.FP32
+    # a row's p is 2^-18 off at most (the hardware's exponential, lse), the sums of 128 and of 2^19 tiles, in eighths, go through below 2^17 additions of numbers that are equal but for few
+    assert np.abs(db.copyToHost(ctx) - total).max() <= rows * (2.0 ** -18 + 2 ** 17 * R.FP32)
