@@ -305,7 +305,7 @@ extern "C"
 	 *     -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(q) - q - 1),
 	 * without the second part where kl_weight is 0, whatever the reference says (its mean is given all the same), and without the first one where A is 0.
 	 * loss fp32 [4]: the mean loss, its two parts -min(..) and exp(q) - q - 1, and the share of tokens that the clip holds. AVERAGE_TOKENS: over all tokens; AVERAGE_SEQUENCES: over the means of the sequences that have tokens.
-	 * Without any token all four are 0. weights fp32 [sequences]: what a token of each sequence counts in the means, for the backward pass.
+	 * Without any token all four are 0. Everything is aligned to one element. weights fp32 [sequences]: what a token of each sequence counts in the means, for the backward pass.
 	 * Backward: dnll = beta * dnll + the gradient of nll for the loss's gradient dloss (one fp32 number on the device, or empty for 1); it is hip_linear_cross_entropy_backward's dloss.
 	 */
 	typedef enum

@@ -385,7 +385,7 @@ namespace
 	bool of_tokens(const mlTensor_t &t, const PolicyShape &s, mlDataType_t dtype)
 	{
 		const size_t tokens = static_cast<size_t>(s.sequences) * s.length;
-		return t.dtype == dtype && volume(t) == tokens && (tokens == 0 || (t.data != nullptr && reinterpret_cast<uintptr_t>(t.data) % 4 == 0));
+		return t.dtype == dtype && volume(t) == tokens && (tokens == 0 || t.data != nullptr) && on_elements(t);
 	}
 	PolicyArgs check_policy(const mlTensor_t &nll, const mlTensor_t &old, const mlTensor_t &reference, const mlTensor_t &advantages, const mlTensor_t &targets, int classes, double clip_low, double clip_high,
 			float kl_weight, const char *name)
@@ -396,7 +396,7 @@ namespace
 		MLHIP_REQUIRE(reference.data == nullptr || of_tokens(reference, s, DTYPE_FLOAT32), who + ": the reference's likelihoods must be fp32, one for every token");
 		MLHIP_REQUIRE(of_tokens(targets, s, DTYPE_INT32), who + ": there must be one int32 target for every token");
 		const size_t given = volume(advantages), tokens = static_cast<size_t>(s.sequences) * s.length;
-		MLHIP_REQUIRE(advantages.dtype == DTYPE_FLOAT32 && (given == tokens || given == static_cast<size_t>(s.sequences)) && (tokens == 0 || (advantages.data != nullptr && reinterpret_cast<uintptr_t>(advantages.data) % 4 == 0)),
+		MLHIP_REQUIRE(advantages.dtype == DTYPE_FLOAT32 && (given == tokens || given == static_cast<size_t>(s.sequences)) && (tokens == 0 || advantages.data != nullptr) && on_elements(advantages),
 				who + ": there must be one fp32 advantage for every token or every sequence");
 		MLHIP_REQUIRE(clip_low >= 0.0 && clip_high >= 0.0, who + ": the clip's range must not be negative");
 		MLHIP_REQUIRE(std::isfinite(kl_weight), who + ": the divergence's weight must be finite");
@@ -427,9 +427,9 @@ extern "C"
 		const char *name = "policy_loss_forward";
 		const PolicyArgs p = check_policy(nll, old_nll, reference_nll, advantages, targets, classes, clip_low, clip_high, kl_weight, name);
 		MLHIP_REQUIRE(average == AVERAGE_TOKENS || average == AVERAGE_SEQUENCES, "policy_loss_forward: unknown average");
-		MLHIP_REQUIRE(loss.dtype == DTYPE_FLOAT32 && volume(loss) == 4 && loss.data != nullptr, "policy_loss_forward: the loss must be fp32 [4]");
-		MLHIP_REQUIRE(weights.dtype == DTYPE_FLOAT32 && volume(weights) == static_cast<size_t>(p.sequences) && (p.sequences == 0 || weights.data != nullptr),
-				"policy_loss_forward: the weights must be fp32, one for every sequence");
+		MLHIP_REQUIRE(loss.dtype == DTYPE_FLOAT32 && volume(loss) == 4 && loss.data != nullptr && on_elements(loss), "policy_loss_forward: the loss must be fp32 [4], aligned to an element");
+		MLHIP_REQUIRE(weights.dtype == DTYPE_FLOAT32 && volume(weights) == static_cast<size_t>(p.sequences) && (p.sequences == 0 || weights.data != nullptr) && on_elements(weights),
+				"policy_loss_forward: the weights must be fp32, one for every sequence, aligned to an element");
 		const PolicyShape s { p.sequences, p.length };
 		const size_t needed = policy_space(s);
 		MLHIP_REQUIRE(needed == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_size >= needed),
@@ -488,9 +488,9 @@ extern "C"
 	{
 		const char *name = "policy_loss_backward";
 		const PolicyArgs p = check_policy(nll, old_nll, reference_nll, advantages, targets, classes, clip_low, clip_high, kl_weight, name);
-		MLHIP_REQUIRE(weights.dtype == DTYPE_FLOAT32 && volume(weights) == static_cast<size_t>(p.sequences) && (p.sequences == 0 || weights.data != nullptr),
-				"policy_loss_backward: the weights must be fp32, one for every sequence");
-		MLHIP_REQUIRE(dloss.data == nullptr || (dloss.dtype == DTYPE_FLOAT32 && volume(dloss) == 1), "policy_loss_backward: the loss's gradient must be a single fp32 number");
+		MLHIP_REQUIRE(weights.dtype == DTYPE_FLOAT32 && volume(weights) == static_cast<size_t>(p.sequences) && (p.sequences == 0 || weights.data != nullptr) && on_elements(weights),
+				"policy_loss_backward: the weights must be fp32, one for every sequence, aligned to an element");
+		MLHIP_REQUIRE(dloss.data == nullptr || (dloss.dtype == DTYPE_FLOAT32 && volume(dloss) == 1 && on_elements(dloss)), "policy_loss_backward: the loss's gradient must be a single fp32 number, aligned to an element");
 		const PolicyShape s { p.sequences, p.length };
 		MLHIP_REQUIRE(of_tokens(dnll, s, DTYPE_FLOAT32), "policy_loss_backward: the gradient must be fp32, one for every token");
 		if (volume(dnll) == 0)

@@ -72,6 +72,12 @@ namespace mlhip
 		}
 	}
 
+	/* one element is the least that a tensor is aligned to: a single number may be read by a scalar load, which takes an address in between for the multiple of 4 below */
+	inline bool on_elements(const mlTensor_t &t)
+	{
+		return t.data == nullptr || reinterpret_cast<uintptr_t>(t.data) % size_of(t.dtype) == 0;
+	}
+
 	/* VEC consecutive elements that need no more alignment than one of them: one memory instruction all the same (global memory takes any address) */
 	template<typename T, int VEC>
 	struct Elements

@@ -285,3 +285,31 @@ def test_distillation_workspace_of_odd_widths_holds_the_padded_rows():
                 tiles = rows > (16 if element == 2 else 32) and (rows > 64 or classes * features * element > 1 << 24)
                 least = (rows + classes) * whole * element if tiles or (backward and rows > (8 if element == 2 else 16)) else rows * classes * 4
                 assert size >= least + rows * 16 * (16 if tiles else 0)
+
+
+def between(shape, dtype="float32"):
+    """A tensor that begins between two elements, at an address of its own."""
+    t = fake(shape, dtype).desc()
+    t.data += 1 if dtype == "float16" else 2
+    return t
+
+
+def test_policy_loss_refuses_tensors_between_elements():
+    names = ("nll", "old", "reference", "advantages", "targets")
+    given = dict(zip(names, (t.desc() for t in policy_tensors())))
+    results = dict(loss=fake((4,), "float32").desc(), weights=fake((3,), "float32").desc())
+    of_gradient = dict(weights=results["weights"], dloss=fake((1,), "float32").desc(), dnll=fake((3, 7), "float32").desc())
+
+    def forward(why=None, **other):
+        tensors, out = dict(given, **{k: v for k, v in other.items() if k in given}), dict(results, **{k: v for k, v in other.items() if k in results})
+        refused("policy_loss_forward", *tensors.values(), 100, 0.2, 0.2, 0.1, 0, out["loss"], out["weights"], 0x7000, 1 << 20, why=why)
+
+    def backward(why=None, **other):
+        tensors, out = dict(given, **{k: v for k, v in other.items() if k in given}), dict(of_gradient, **{k: v for k, v in other.items() if k in of_gradient})
+        refused("policy_loss_backward", *tensors.values(), 100, 0.2, 0.2, 0.1, out["weights"], out["dloss"], 0.0, out["dnll"], why=why)
+
+    for call, mine in ((forward, results), (backward, of_gradient)):
+        call(why="null context")
+        for name, t in dict(given, **mine).items():
+            shape = tuple(t.dim[:t.rank])
+            call(**{name: between(shape, "int32" if name == "targets" else "float32")}, why="^(?!.*null context)")
