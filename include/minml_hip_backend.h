@@ -288,7 +288,7 @@ extern "C"
 	 * every row (1 to 1024), int32 [.., count], in any order, and their logits [.., count] of x's type or fp32. With z = (x w^T + b) / temperature, lse = log sum exp z, log p = z[class] - lse and q = softmax(logits / temperature)
 	 * over the row's classes: loss = sum of q (log q - log p), fp32 [..], with lse fp32 [..] and log_probabilities (log p) fp32 [.., count] as the backward pass needs them. A place whose class is none of 0 .. classes - 1 or
 	 * whose logit is -inf does not count, whatever else it holds (log p is 0 there); a class that stands there twice has the sum of both probabilities; a row where nothing counts has loss 0 and no gradient (its lse is given
-	 * all the same; its x has to be finite). Loss and gradients are of the softened distributions: callers that want them multiplied by temperature^2 do so in dloss.
+	 * all the same; its x has to be finite). Everything but x and w is aligned to one element at least. Loss and gradients are of the softened distributions: callers that want them multiplied by temperature^2 do so in dloss.
 	 * Backward: dloss fp32 [..] -> dx, dw, db as above, with the gradients of the logits kept as the cross entropy's are (of up to 64 rows mostly with what rounding leaves of them). The workspace holds what the cross entropy's does, 16 bytes for every place, and 2 for every row of
 	 * every tile; of a few rows their logits, and gradients of them in fp32 with up to 512 sums of dx, instead.
 	 */

@@ -1078,17 +1078,17 @@ namespace
 	/* the rows' shape with another last dimension */
 	bool places_of_rows(const mlTensor_t &t, const LossShape &s, int count)
 	{
-		return t.rank >= 1 && last_dim(t) == count && volume(t) == static_cast<size_t>(s.rows) * count && (s.rows == 0 || t.data != nullptr);
+		return t.rank >= 1 && last_dim(t) == count && volume(t) == static_cast<size_t>(s.rows) * count && (s.rows == 0 || t.data != nullptr) && on_elements(t);
 	}
 	LossShape check_distillation(const mlTensor_t &x, const mlTensor_t &w, const mlTensor_t &b, const mlTensor_t &classes, const mlTensor_t &logits, float temperature, int &count, const char *name)
 	{
 		const std::string who(name);
 		const LossShape s = loss_shape(shape_of(x), shape_of(w), x.dtype, name);
 		MLHIP_REQUIRE(w.dtype == x.dtype, who + ": weights must have the input's type");
-		MLHIP_REQUIRE(b.data == nullptr || (b.dtype == x.dtype && volume(b) == static_cast<size_t>(s.classes)), who + ": the bias must be [classes] of the input's type");
+		MLHIP_REQUIRE(b.data == nullptr || (b.dtype == x.dtype && volume(b) == static_cast<size_t>(s.classes) && on_elements(b)), who + ": the bias must be [classes] of the input's type");
 		count = last_dim(classes);
 		MLHIP_REQUIRE(count >= 1 && count <= MOST_CLASSES_OF_ROW, who + ": the teacher must name 1 to 1024 classes for every row");
-		MLHIP_REQUIRE(classes.dtype == DTYPE_INT32 && places_of_rows(classes, s, count) && reinterpret_cast<uintptr_t>(classes.data) % 4 == 0, who + ": the teacher's classes must be int32, as many for every row");
+		MLHIP_REQUIRE(classes.dtype == DTYPE_INT32 && places_of_rows(classes, s, count), who + ": the teacher's classes must be int32, as many for every row");
 		MLHIP_REQUIRE((logits.dtype == x.dtype || logits.dtype == DTYPE_FLOAT32) && places_of_rows(logits, s, count), who + ": there must be one logit of the input's type or fp32 for every class of the teacher");
 		MLHIP_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(1.0f / temperature), who + ": the temperature must be positive and finite");
 		MLHIP_REQUIRE(s.rows == 0 || (x.data != nullptr && w.data != nullptr), who + ": null pointer");
@@ -1151,6 +1151,7 @@ extern "C"
 		MLHIP_REQUIRE(per_row(lse, s, DTYPE_FLOAT32) && per_row(dloss, s, DTYPE_FLOAT32), "linear_distillation_backward: lse and dloss must be fp32 with one element per row");
 		MLHIP_REQUIRE(log_probabilities.dtype == DTYPE_FLOAT32 && places_of_rows(log_probabilities, s, count), "linear_distillation_backward: the log probabilities must be fp32, one for every class of the teacher");
 		check_gradients(x, w, s, dx, dw, db, name);
+		MLHIP_REQUIRE(on_elements(dx) && on_elements(dw) && on_elements(db), "linear_distillation_backward: the gradients must be aligned to an element");
 		if (dx.data == nullptr && dw.data == nullptr && db.data == nullptr)
 			return;
 		if (s.rows == 0)

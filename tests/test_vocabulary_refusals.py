@@ -313,3 +313,22 @@ def test_policy_loss_refuses_tensors_between_elements():
         for name, t in dict(given, **mine).items():
             shape = tuple(t.dim[:t.rank])
             call(**{name: between(shape, "int32" if name == "targets" else "float32")}, why="^(?!.*null context)")
+
+
+def test_distillation_refuses_tensors_between_elements():
+    shapes = dict(b=((90,), "float16"), named=((4, 8), "int32"), taught=((4, 8), "float16"), loss=((4,), "float32"), lse=((4,), "float32"), p=((4, 8), "float32"), dloss=((4,), "float32"), dx=((4, 16), "float16"), dw=((90, 16), "float32"),
+                  db=((90,), "float16"))
+    x, w, whole = fake((4, 16)).desc(), fake((90, 16)).desc(), {k: fake(*v).desc() for k, v in shapes.items()}
+
+    def forward(t, why):
+        refused("linear_distillation_forward", x, w, t["b"], t["named"], t["taught"], 2.0, t["loss"], t["lse"], t["p"], 0x7000, 1 << 30, why=why)
+
+    def backward(t, why):
+        refused("linear_distillation_backward", x, w, t["b"], t["named"], t["taught"], 2.0, t["lse"], t["p"], t["dloss"], 0.0, t["dx"], 0.0, t["dw"], t["db"], 0x7000, 1 << 30, why=why)
+
+    for call, names in ((forward, ("b", "named", "taught", "loss", "lse", "p")), (backward, ("b", "named", "taught", "lse", "p", "dloss", "dx", "dw", "db"))):
+        call(whole, "null context")
+        call(dict(whole, taught=fake((4, 8), "float32").desc()), "null context")
+        for name in names:
+            call(dict(whole, **{name: between(*shapes[name])}), "^(?!.*null context)")
+        call(dict(whole, taught=between((4, 8))), "logit")
