@@ -817,12 +817,12 @@ namespace
 	void check_tokens(const mlTensor_t &tokens, const EmbeddingShape &s, const char *name)
 	{
 		MLHIP_REQUIRE(tokens.dtype == DTYPE_INT32, std::string(name) + ": tokens must be int32");
-		MLHIP_REQUIRE(s.rows == 0 || (tokens.data != nullptr && reinterpret_cast<uintptr_t>(tokens.data) % 4 == 0), std::string(name) + ": null or misaligned tokens");
+		MLHIP_REQUIRE((s.rows == 0 || tokens.data != nullptr) && on_elements(tokens), std::string(name) + ": null or misaligned tokens");
 	}
-	/* one row of features for every token */
+	/* one row of features for every token, aligned to an element */
 	bool rows_of(const mlTensor_t &t, const EmbeddingShape &s)
 	{
-		return t.rank >= 1 && last_dim(t) == s.columns && volume(t) == static_cast<size_t>(s.rows) * s.columns && (s.rows == 0 || t.data != nullptr);
+		return t.rank >= 1 && last_dim(t) == s.columns && volume(t) == static_cast<size_t>(s.rows) * s.columns && (s.rows == 0 || t.data != nullptr) && on_elements(t);
 	}
 }
 
@@ -840,7 +840,7 @@ extern "C"
 		MLHIP_REQUIRE(y.dtype == table.dtype && rows_of(y, s), "embedding_forward: the result must hold a row of the table's type and width for every token");
 		if (s.rows == 0)
 			return;
-		MLHIP_REQUIRE(table.data != nullptr, "embedding_forward: null table");
+		MLHIP_REQUIRE(table.data != nullptr && on_elements(table), "embedding_forward: null or misaligned table");
 		require_apart( { y }, { tokens, table }, name);
 		const OnDeviceOf on(context);
 		if (table.dtype == DTYPE_FLOAT16)
@@ -881,6 +881,7 @@ extern "C"
 		MLHIP_REQUIRE(std::isfinite(scale), "embedding_backward: the scale must be finite"); /* classes without tokens get zeros, not zero times it */
 		MLHIP_REQUIRE(rows_of(dy, s), "embedding_backward: there must be a gradient of the table's width for every token");
 		MLHIP_REQUIRE(dtable.dtype == dy.dtype || dtable.dtype == DTYPE_FLOAT32, "embedding_backward: the table's gradient must be of the gradients' type or fp32");
+		MLHIP_REQUIRE(on_elements(dtable), "embedding_backward: the table's gradient must be aligned to an element");
 		const EmbeddingSpace space = embedding_space(s, dy.dtype);
 		MLHIP_REQUIRE(space.total == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_size >= space.total),
 				"embedding_backward: the workspace is too small or not aligned to 256 bytes");

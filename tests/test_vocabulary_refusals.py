@@ -332,3 +332,15 @@ def test_distillation_refuses_tensors_between_elements():
         for name in names:
             call(dict(whole, **{name: between(*shapes[name])}), "^(?!.*null context)")
         call(dict(whole, taught=between((4, 8))), "logit")
+
+
+def test_embedding_refuses_tensors_between_elements():
+    size = B.fn("embedding_get_workspace_size")(fake((40,), "int32").shape_desc(), fake((90, 16)).shape_desc(), B.DTYPE_FLOAT32)
+    for dtype in ("float16", "float32"):
+        tokens, table, rows = ((40,), "int32"), ((90, 16), dtype), ((40, 16), dtype)
+        forward = lambda why, t=fake(*tokens).desc(), w=fake(*table).desc(), y=fake(*rows).desc(): refused("embedding_forward", t, w, 1.0, y, why=why)
+        backward = lambda why, t=fake(*tokens).desc(), dw=fake(*table).desc(), y=fake(*rows).desc(): refused("embedding_backward", t, y, 1.0, 0.0, dw, 0x7000, size, why=why)
+        for call, gradient in ((forward, {}), (backward, dict(dw=between(*table)))):
+            call("null context")
+            for name, t in dict(dict(t=between(*tokens), y=between(*rows)), **(gradient or dict(w=between(*table)))).items():
+                call("^(?!.*null context)", **{name: t})
