@@ -117,3 +117,30 @@ def test_tensors_that_begin_at_any_element(ctx, dtype):
         exact, weighted = V.embedding_gradient(tokens, R.numbers(dy), classes, 1.0)
         assert R.worst(dtable.copyToHost(ctx), exact, V.embedding_gradient_bound(exact, weighted, 0 * exact, dtype)) <= 1
         assert R.numbers(dtable._owner.copyToHost(ctx))[0] == R.numbers(table).reshape(-1)[0]
+
+
+# classes of up to 100000 rows; more tokens than the sort keeps in registers, with one digit, two and, of 2^22 classes and more, three
+WHOLE = [(1, 7, 3), (65, 300, 16), (2047, 2048, 13), (9000, 2, 260), (3001, 5, 2056), (12000, 130000, 16), (70001, 1023, 12), (70001, 5000, 8), (66000, 2048, 1), (200000, 60000, 4), (300000, 5, 4), (9000, 4200000, 1), (90000, 5000000, 3)]
+
+
+@pytest.mark.parametrize("dtype,out", [("float16", "float16"), ("float16", "float32"), ("float32", "float32")])
+@pytest.mark.parametrize("rows,classes,features", WHOLE)
+def test_gradient_of_whole_numbers(ctx, rows, classes, features, dtype, out):
+    """Rows of whole numbers from 1 to 7, of either sign, times 2^-8, whose sums are exact in 32 bits in any order: a row that is left out, taken twice or added to another class changes every column of its class. In fp16 what
+    is left is one rounding to nearest."""
+    rng = np.random.default_rng(rows * 10037 + classes * 107 + features)
+    tokens = tokens_of(rng, rows, classes)
+    dy = rng.integers(1, 8, (rows, features)) * rng.choice([-1, 1], (rows, features), p=[0.3, 0.7])
+    kept = (tokens >= 0) & (tokens < classes)
+    total = np.zeros((classes, features), np.int64)
+    np.add.at(total, tokens[kept], dy[kept])
+    old = rng.integers(-8, 9, total.shape)
+    assert np.abs(total).max() + 8 < 2 ** 24
+    T, DY = ml.toDevice(ctx, tokens), guarded(ctx, R.bits(dy, dtype), dtype, np.nan)
+    for beta in (0.0, 1.0):
+        dtable = guarded(ctx, R.bits(np.full(old.shape, np.nan) if beta == 0 else old / 256, out), out, 9.0)
+        work = space(ctx, T, dtable)
+        ml.embeddingBackward(ctx, T, DY, 2.0 ** -8, beta, dtable, work)
+        V.check_workspace(ctx, work)
+        assert np.array_equal(R.numbers(dtable.copyToHost(ctx)), R.numbers(R.bits((total + int(beta) * old) / 256, out)))
+        check_guards(ctx, dtable, 9.0)
