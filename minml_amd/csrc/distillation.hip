@@ -55,7 +55,7 @@ namespace
 	}
 	/*
 	 * The mean of up to 64 of the teacher's classes' rows of weights, taken evenly over what it names; one of four places that counts, for each. A class that the teacher names is one that the model is trained for, whose row of W
-	 * looks like those that d is large at. Columns behind the features: zeros. 64 columns to a workgroup, 16 rows to a wavefront
+	 * looks like those that d is large at. It is kept in fp16, where a row of W is: whatever row it is, what is given back to it is taken from it as it stands, so its own rounding is no error of dx. Columns behind the features: zeros. 64 columns to a workgroup, 16 rows to a wavefront
 	 */
 	constexpr int COMMON_ROWS = 64, COMMON_COLUMNS = 256; /* COMMON_COLUMNS: the widest tile's, which reads them without asking where they end */
 	template<typename L>
@@ -622,7 +622,8 @@ namespace
 	 * Up to 16 rows: tiles would be empty but for a few rows, and each of three products would read or write the weights' size for itself on them. Here d is kept in fp32, [classes][rows], 64 bytes of a class at most; making it
 	 * reads the weights once, past the rows, as the forward pass does; dx = d W reads them once more, every thread with its columns of all rows in registers; dW = d^T x writes as much, with its columns of x in registers. Rows of
 	 * any width and alignment are read as they lie. Memory bounds all three. us of loss and gradients, so / on tiles: 1 row fp16 of 2048 x 65536 226 / 270, 1024 x 32000 68 / 98, 1023 x 32000 106 / 144, 1024 x 4000 34 / 53,
-	 * 128 x 100000 80 / 149; 8 rows 262 / 278, 80 / 99, 136 / 152, 46 / 59, 106 / 150; fp32 1024 x 32000 1 row 106 / 202, 16 rows 127 / 205
+	 * 128 x 100000 80 / 149; 8 rows 262 / 278, 80 / 99, 136 / 152, 46 / 59, 106 / 150; fp32 1024 x 32000 1 row 106 / 202, 16 rows 127 / 205. (dW past the caches since: 8 rows of 2048 x 65536 227.) The second read of the weights, 54 of those 227 us, is
+	 * there because a class's row has left the registers by the time its d is known; a run of classes that stays in LDS until then would spare it
 	 */
 	constexpr int FEW_GRADIENT_ROWS = 16;
 	template<typename T, bool STREAM>

@@ -2,12 +2,14 @@
  * embedding.hip — rows of a table by token, and the table's gradient.
  *
  *   y[i] = scale table[token[i]]                                           a token that is none of the table's: zeros
- *   dtable[v] = scale sum over i with token[i] = v of dy[i] + beta dtable[v]     in fp32, in the order of i
+ *   dtable[v] = scale sum over i with token[i] = v of dy[i] + beta dtable[v]     in fp32, always in the same order
  *
  * Forward: memory bounds it (a row of the table read for every row written, from the caches where tokens repeat): 57600 x 256 fp16 from 400 classes 7.8 us (3.8 TB/s, the stores of 29 MB alone take 6).
- * Backward: tokens are sorted first, stably, so that a class's rows stand in a list in the order they have in dy, and one reader adds them up: no two threads meet at a row of the table, every element of dy is read once and
- * every row of the table written once, with zeros where there is no token. The same bits on every run. us: 16384 x 4096 fp16 into 65536 classes 168 (4.0 TB/s: 22 for the order, 139 with 4.7 TB/s for the rows, 11 to join the long
- * classes), 57600 x 256 fp16 into 400 classes 25, 20011 x 1001 fp32 into 5003 classes 43 to 49: launches of 4 to 9 us, one after another, whose reads wait for each other.
+ * Backward: tokens are sorted first, stably, so that a class's rows stand in a list in the order they have in dy. Up to 15 rows of a class are added up in that order by one group of threads; of more, each of a workgroup's groups
+ * takes every so many-th, in chunks of 32 or 64 rows where there are as many, and their sums are added up, groups and chunks in order. So no two threads write to the same row of the table, every element of dy is read once and
+ * every row of the table written once, with zeros where there is no token, and the bits are the same on every run. us: 16384 x 4096 fp16 into 65536 classes 169 (4.0 TB/s: 22 for the order, 139 with 4.7 TB/s for the rows, 11 to
+ * join the long classes), 57600 x 256 fp16 into 400 classes 25, 20011 x 1001 fp32 into 5003 classes 43 to 51: launches of 4 to 9 us, one after another, whose reads wait for each other. Many tokens: 131072 x 1024 fp16 into
+ * 50000 classes 122, 28 of them for the order, 262144 x 256 99 and 37, 2^20 x 64 231.
  */
 #include "training_utils.hpp"
 
@@ -145,7 +147,8 @@ namespace
 	}
 	/*
 	 * More of them: a launch that counts the digits of every group's tokens and one that puts them in place, for every digit of up to 11 bits. At most 64 groups, so that each can add up the others' counts by itself (that it also
-	 * counts the others' tokens, without the first launch, takes 16 us where the two take 12, at 16384 tokens). `keys` null: the tokens themselves, which stand where they are
+	 * counts the others' tokens, without the first launch, takes 16 us where the two take 12, at 16384 tokens). So from 65536 tokens on the groups grow instead, a quarter of the compute units sort, and tokens are read twice: a digit of
+	 * 131072 takes 14 us, of 262144 19. `keys` null: the tokens themselves, which stand where they are
 	 */
 	constexpr int SORT_GROUPS = 64, SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES;
 	struct SortPass

@@ -221,7 +221,9 @@ namespace
 			partial[static_cast<size_t>(blockIdx.x) * gridDim.y + blockIdx.y] = total;
 	}
 	/*
-	 * The workgroups' sums joined (every group does it for itself, the first one gives the loss), then the weights of a token of every sequence. `chunks`: of a sequence, whose sums `partial` holds; else (0) of `items` workgroups
+	 * The workgroups' sums joined (every group does it for itself, the first one gives the loss), then the weights of a token of every sequence. `chunks`: of a sequence, whose sums `partial` holds; else (0) of `items` workgroups.
+	 * One thread walks a sequence's chunks, twice, which bounds few sequences that are very long: us of this launch and of the sums', 1 sequence of 2^20 tokens (256 chunks) 50 and 8, 4 of 2^20 56 and 17; a call of one of 2^22 213,
+	 * of 2^18 23
 	 */
 	__global__ __launch_bounds__(256) void kernel_policy_join(const Sums *partial, int items, int chunks, bool average_sequences, int sequences, float kl_weight, const int *counts, float *loss, float *weights)
 	{
@@ -361,8 +363,9 @@ namespace
 		return PolicyShape { sequences, length };
 	}
 	/*
-	 * Threads of a sequence where one workgroup does everything, or 0 where two launches do. It takes about 2 us for every time that a thread goes to memory, and saves what a launch costs: us of a forward call and (on the device),
-	 * so / in two launches: 4 x 113 tokens, once, 9.6 (3.6) / 12 (5.4); 32 x 128, twice, 9.5 (7.7) / 12 (6.7); 32 x 512, four times, 10.1 (9.5) / 12 (6.7); 64 x 500, eight times, 17 (17) / 12 (6.6)
+	 * Threads of a sequence where one workgroup does everything, or 0 where two launches do. It takes about 2 us for every time that a thread goes to memory, and saves what a launch costs: us of a forward call and (on the device,
+	 * profiled), so / in two launches: 4 x 113 tokens, once, 10.6 (6.1) / 14.1 (5.6); 32 x 128, twice, 10.9 (10.1) / 13.9 (6.6); 200 x 40, four times, 10.9 (10.1) / 14.0 (8.4); 32 x 512, four times, 13.0 (12.2) / 14.1 (6.7);
+	 * 64 x 500, eight times, 21 (21) / 14.2 (6.6)
 	 */
 	int lanes_of_few(const PolicyShape &s)
 	{

@@ -138,7 +138,8 @@ namespace mlhip
 	 * The same past the caches, for rows of whole lines of a result that is larger than the L2s: nobody finds it there later, and what somebody would find is not pushed out. us with the inputs in the memory's own cache as
 	 * far as they fit there, so / through the caches (with inputs from memory, the same either way): embedding gradients of
 	 * 16384 x 4096 of 65536 classes 138 / 170, 8192 x 2048 of 65536 fp32 131 / 152, 4096 x 1024 of 131072 68.5 / 73.4, 30000 x 256 of 100000 48 / 49.7, 5 x 1072 of 66507 fp32 (nearly all zeros) 72 / 69.5; distillations of
-	 * 8 rows, 2048 x 65536 218 / 259, 1024 x 32000 79.3 / 80.5; rows that end inside a line (1 row, 1023 x 32000) 110 / 104.
+	 * 8 rows, 2048 x 65536 218 / 259, 1024 x 32000 79.3 / 80.5; rows that end inside a line (1 row, 1023 x 32000) 110 / 104. The rule asks only for the size: how much of a table gets more than zeros, where the caches are the
+	 * better way by 3 to 4 %, is not known before the launch.
 	 */
 	inline bool past_caches(size_t rows, size_t row_bytes)
 	{
